@@ -297,7 +297,7 @@ def _prepare_own(st, table):
     tables.cursor.copy_(st["cursor"])
     H, G = case.get("kv_heads", 8), case.get("group", 1)
     plan = tables.make_plan(st["tokens"], kv_heads=H, query_heads=H * G,
-                            max_fresh=max(st["host"][1]))
+                            head_dim=case.get("dim", 128), max_fresh=max(st["host"][1]))
     st["tables"], st["plan"] = tables, plan
     if case["op"] == "plan":
         return
