@@ -84,6 +84,12 @@ _SIGS = {
                                         _P]),
     "grm_b200_mount_ref_rope": (_I, [_P, _P, _I64, _I64, _I64, _I64, _P, _P, _I64, _P, _P]),
     "grm_b200_arena_splice": (_I, [_P, _I64, _I64, _P, _I64, _I64, _I64, _I64, _P, _P, _P]),
+    "grm_b200_paged_scratch_bytes": (_I, [_P, _P]),
+    "grm_b200_paged_plan_step": (_I, [_P, _P, _P]),
+    "grm_b200_paged_release": (_I, [_P, _I64, _I64, _I64, _I64, _I, _P, _P, _P, _P, _P]),
+    "grm_b200_paged_append": (_I, [_P, _P, _P, _P, _I, _I64, _I64, _I64, _I64, _P]),
+    "grm_b200_paged_read": (_I, [_P, _P, _I64, _I, _P, _P, _P]),
+    "grm_b200_paged_attend": (_I, [_P, _P, _P, _I, _I64, _I64, ctypes.c_float, _I, _P, _P, _P]),
     "grm_b200_merge_topk": (_I, [_P, _P, _I, _I, _I, _I, _P, _P, _P]),
     "grm_b200_merge_topk_strided": (_I, [_P, ctypes.c_int64, _P, ctypes.c_int64, _I, _I, _I, _I,
                                          _P, _P, _P]),

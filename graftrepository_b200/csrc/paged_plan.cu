@@ -1,0 +1,554 @@
+// paged_plan.cu -- a step of the 8-bit paged arena planned on the GPU: block
+// table, slots, positions, and the work lists of append and attention, all
+// from the requests' lengths in one launch.
+//
+// With have = ceil(cached / P) and need = ceil((cached + fresh) / P), request
+// r takes need - have pages; page j in [have, need) is
+//   ring[(taken + sum of the requests before r + j - have) mod pages],
+// and token t of the step's packed rows, at position p of its request, has the
+// slot page(p / P) * P + p % P.  Everything is a prefix sum over the requests
+// followed by one independent write for each entry.
+//
+// One launch without a barrier between blocks: every block runs the prefix
+// sums over all requests itself (8 bytes a request, from L2), in chunks of
+// kPlanThreads, and writes its share of each chunk's entries, which it finds
+// by a binary search in the chunk's sums in shared memory.  A new page's number
+// comes from the ring, not from the table entry another block writes, so no
+// block waits for another.
+#include <algorithm>
+
+#include "paged.cuh"
+
+namespace grm_b200 {
+namespace paged {
+
+namespace {
+
+constexpr int kPlanThreads = 1024;
+constexpr int kPlanWarps = kPlanThreads / 32;
+// The sums over requests: pages taken, rows, pages touched, prompt tiles (all
+// of them below 2^31 in a step that can be planned) and the split kernel's units.
+constexpr int kSums = 5;
+constexpr int kTake = 0, kRows = 1, kTouched = 2, kTiles = 3, kUnits = 4;
+
+struct PlanParams {
+  int64_t requests, tokens, max_fresh, width, ring_size;
+  int page_shift, grow, kv_heads;
+  Shape s;
+  int min_units;
+  const int32_t* cached;
+  const int32_t* fresh;
+  const int32_t* ring;
+  const int64_t* cursor_in;
+  int32_t* table;
+  int32_t* lens;
+  int32_t* starts;
+  int32_t* positions;
+  int32_t* rows;
+  int64_t* slots;
+  int64_t* cursor;
+  int32_t* status;
+  Lists l;
+};
+
+struct Request {
+  int cached, fresh, after, have, need;
+};
+
+// What request r adds to each sum.
+__device__ __forceinline__ void weigh(const PlanParams& p, const Request& q, int64_t (&v)[kSums]) {
+  v[0] = q.need - q.have;
+  v[1] = q.fresh;
+  v[2] = p.grow && q.fresh > 0 ? q.need - (q.cached >> p.page_shift) : 0;
+  const int64_t pairs = (int64_t)q.fresh * p.s.group;
+  const bool prompt = pairs > p.s.split_rows;
+  v[3] = prompt ? ceil_div64(q.fresh, p.s.qtile_tokens) : 0;
+  v[4] = prompt ? 0
+                : p.kv_heads * ceil_div64(pairs, p.s.block_rows) *
+                      (ceil_div64(q.after, kTile) + 1);
+}
+
+__device__ __forceinline__ int64_t warp_sum(int64_t v) {
+#pragma unroll
+  for (int o = 16; o >= 1; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
+  return v;
+}
+
+// The last of the n + 1 ascending sums s[0..n] that is <= x (s[n] > x).
+template <typename T>
+__device__ __forceinline__ int find(const T* s, int n, T x) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (s[mid] <= x) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+// Inclusive prefix sum over a warp.
+template <typename T>
+__device__ __forceinline__ T warp_scan(T v, int lane) {
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const T up = __shfl_up_sync(kFull, v, o);
+    if (lane >= o) v += up;
+  }
+  return v;
+}
+
+__global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) {
+  __shared__ int sum[4][kPlanThreads + 1];  // before each request of the chunk, from the start
+  __shared__ int64_t sum_units[kPlanThreads + 1];
+  __shared__ int s_cached[kPlanThreads], s_have[kPlanThreads];
+  __shared__ int64_t part[kSums][kPlanWarps];
+  __shared__ int64_t total[kSums];
+  __shared__ int bad;
+
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int gid = blockIdx.x * kPlanThreads + tid;
+  const int gsize = gridDim.x * kPlanThreads;
+  const int page = 1 << p.page_shift;
+  const int64_t taken0 = p.cursor_in[0], returned = p.cursor_in[1];
+
+  auto request = [&](int64_t r, int* flags) {
+    Request q{0, 0, 0, 0, 0};
+    if (r >= p.requests) return q;
+    q.cached = p.cached[r];
+    q.fresh = p.fresh[r];
+    const int64_t after = (int64_t)q.cached + (p.grow ? q.fresh : 0);
+    if (q.cached < 0 || q.fresh < 0 || after > INT32_MAX - page) {
+      *flags |= GRM_B200_PLAN_BAD_LENGTH;
+      return Request{0, 0, 0, 0, 0};
+    }
+    if (q.fresh > p.max_fresh) *flags |= GRM_B200_PLAN_ROWS;
+    q.after = (int)after;
+    q.have = (q.cached + page - 1) >> p.page_shift;
+    q.need = (q.after + page - 1) >> p.page_shift;
+    if (q.need > p.width) *flags |= GRM_B200_PLAN_TABLE;
+    return q;
+  };
+
+  // ---- totals and errors
+  if (tid == 0) bad = 0;
+  int64_t v[kSums] = {};
+  int flags = 0;
+  for (int64_t r = tid; r < p.requests; r += kPlanThreads) {
+    int64_t a[kSums];
+    weigh(p, request(r, &flags), a);
+#pragma unroll
+    for (int i = 0; i < kSums; ++i) v[i] += a[i];
+  }
+#pragma unroll
+  for (int i = 0; i < kSums; ++i) {
+    const int64_t w = warp_sum(v[i]);
+    if (lane == 0) part[i][warp] = w;
+  }
+  __syncthreads();
+  if (flags) atomicOr(&bad, flags);
+  if (warp < kSums) {
+    const int64_t w = warp_sum(part[warp][lane]);
+    if (lane == 0) total[warp] = w;
+  }
+  __syncthreads();
+  int failed = bad;
+  if (total[kRows] > p.tokens) failed |= GRM_B200_PLAN_ROWS;
+  if (taken0 < 0 || returned - taken0 > p.ring_size || total[kTake] > returned - taken0)
+    failed |= GRM_B200_PLAN_PAGES;
+  const int64_t units = failed ? 0 : total[kUnits];
+  const int all_rows = failed ? 0 : (int)total[kRows];
+  // Few units: fewer workers, so that none gets less than min_units of them.
+  int64_t most = (units + p.min_units - 1) / p.min_units;
+  const int workers = most < p.s.workers ? (int)most : p.s.workers;
+
+  if (gid == 0) {
+    p.status[0] = failed;
+    p.cursor[0] = taken0 + (failed ? 0 : total[kTake]);
+    p.cursor[1] = returned;
+    p.starts[p.requests] = all_rows;
+    p.l.base[p.requests] = units;
+    *p.l.header = Header{units, workers, failed ? 0 : (int)total[kTouched],
+                         failed ? 0 : (int)total[kTiles], all_rows};
+  }
+  for (int i = gid; i < p.s.workers; i += gsize) p.l.count[i] = 0;
+  for (int64_t i = all_rows + gid; i < p.tokens; i += gsize) {
+    p.positions[i] = -1;
+    p.rows[i] = -1;
+    p.slots[i] = -1;
+  }
+  if (failed) {
+    for (int64_t r = gid; r < p.requests; r += gsize) {
+      p.lens[r] = p.cached[r];
+      p.starts[r] = 0;
+      p.l.base[r] = 0;
+    }
+    return;
+  }
+
+  // ---- chunk by chunk: prefix sums, then this block's share of the entries
+  const int ring0 = (int)(taken0 % p.ring_size);
+  auto ring_page = [&](int64_t x) {  // the x-th page this step takes
+    const int64_t at = ring0 + x;
+    return p.ring[at < p.ring_size ? at : at - p.ring_size];
+  };
+  int before[4] = {};
+  int64_t before_units = 0;
+  for (int64_t r0 = 0; r0 < p.requests; r0 += kPlanThreads) {
+    const int n = (int)(p.requests - r0 < kPlanThreads ? p.requests - r0 : kPlanThreads);
+    int unused = 0;
+    const Request q = request(r0 + tid, &unused);
+    int64_t a[kSums];
+    weigh(p, q, a);
+    int incl[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) incl[i] = warp_scan((int)a[i], lane);
+    const int64_t incl_units = warp_scan(a[kUnits], lane);
+    __syncthreads();  // every thread is done with the sums of the chunk before
+    if (lane == 31) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) part[i][warp] = incl[i];
+      part[kUnits][warp] = incl_units;
+    }
+    s_cached[tid] = q.cached;
+    s_have[tid] = q.have;
+    __syncthreads();
+    if (warp < kSums) {
+      const int64_t own = part[warp][lane];
+      const int64_t w = warp_scan(own, lane);
+      part[warp][lane] = w - own;
+      if (lane == 31) total[warp] = w;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      sum[i][tid] = before[i] + (int)part[i][warp] + incl[i] - (int)a[i];
+      before[i] += (int)total[i];
+    }
+    sum_units[tid] = before_units + part[kUnits][warp] + incl_units - a[kUnits];
+    before_units += total[kUnits];
+    __syncthreads();
+    if (tid == 0) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum[i][n] = before[i];
+      sum_units[n] = before_units;
+    }
+    __syncthreads();
+
+    if (blockIdx.x == r0 / kPlanThreads % gridDim.x && tid < n) {
+      p.lens[r0 + tid] = q.after;
+      p.starts[r0 + tid] = sum[kRows][tid];
+      p.l.base[r0 + tid] = sum_units[tid];
+    }
+    for (int64_t x = sum[kTake][0] + (int64_t)gid; x < sum[kTake][n]; x += gsize) {
+      const int i = find(sum[kTake], n, (int)x);
+      p.table[(r0 + i) * p.width + s_have[i] + ((int)x - sum[kTake][i])] = ring_page(x);
+    }
+    for (int64_t x = sum[kRows][0] + (int64_t)gid; x < sum[kRows][n]; x += gsize) {
+      const int i = find(sum[kRows], n, (int)x);
+      const int pos = s_cached[i] + ((int)x - sum[kRows][i]);
+      p.rows[x] = (int)(r0 + i);
+      p.positions[x] = pos;
+      int64_t slot = -1;
+      if (p.grow) {
+        // a page taken in this step is read from the ring, not from the entry
+        // that another block writes
+        const int j = pos >> p.page_shift;
+        const int64_t pg = j < s_have[i] ? p.table[(r0 + i) * p.width + j]
+                                         : ring_page((int64_t)sum[kTake][i] + j - s_have[i]);
+        slot = (pg << p.page_shift) + (pos & (page - 1));
+      }
+      p.slots[x] = slot;
+    }
+    for (int64_t x = sum[kTouched][0] + (int64_t)gid; x < sum[kTouched][n]; x += gsize) {
+      const int i = find(sum[kTouched], n, (int)x);
+      p.l.pages[x] = make_int2((int)(r0 + i), (s_cached[i] >> p.page_shift) +
+                                                  ((int)x - sum[kTouched][i]));
+    }
+    for (int64_t x = sum[kTiles][0] + (int64_t)gid; x < sum[kTiles][n]; x += gsize) {
+      const int i = find(sum[kTiles], n, (int)x);
+      p.l.qtiles[x] = make_int2((int)(r0 + i), ((int)x - sum[kTiles][i]) * p.s.qtile_tokens);
+    }
+    for (int w = gid; w < workers; w += gsize) {
+      const int64_t u = worker_first(w, units, workers);
+      if (u >= sum_units[0] && u < sum_units[n])
+        p.l.start[w] = (int)(r0 + find(sum_units, n, u));
+    }
+  }
+}
+
+constexpr int kReleaseThreads = 1024;
+
+// One block: the list in chunks, a prefix sum of the page counts in each.
+__global__ void __launch_bounds__(kReleaseThreads)
+    release_kernel(const int32_t* rows, int64_t count, int64_t requests, int64_t width,
+                   int64_t ring_size, int page_shift, const int32_t* table, int32_t* lens,
+                   int32_t* ring, int64_t* cursor) {
+  __shared__ int64_t sum[kReleaseThreads + 1];
+  __shared__ int64_t part[32];
+  __shared__ int row_of[kReleaseThreads];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  int64_t returned = cursor[1];
+  if (returned < 0) return;
+  for (int64_t c0 = 0; c0 < count; c0 += kReleaseThreads) {
+    int64_t n_pages = 0;
+    int row = -1;
+    if (c0 + tid < count) {
+      row = rows[c0 + tid];
+      // a row listed twice gives its pages to whichever of the two comes first
+      if (row >= 0 && row < requests) {
+        const int len = atomicExch(&lens[row], 0);
+        n_pages = ((int64_t)(len > 0 ? len : 0) + (1 << page_shift) - 1) >> page_shift;
+        n_pages = n_pages < width ? n_pages : width;
+      }
+    }
+    const int64_t incl = warp_scan(n_pages, lane);
+    __syncthreads();
+    if (lane == 31) part[warp] = incl;
+    row_of[tid] = row;
+    __syncthreads();
+    if (warp == 0) {
+      const int64_t own = part[lane];
+      const int64_t w = warp_scan(own, lane);
+      part[lane] = w - own;
+      if (lane == 31) sum[kReleaseThreads] = w;
+    }
+    __syncthreads();
+    sum[tid] = part[warp] + incl - n_pages;
+    __syncthreads();
+    for (int64_t x = tid; x < sum[kReleaseThreads]; x += kReleaseThreads) {
+      const int i = find(sum, kReleaseThreads, x);
+      ring[(returned + x) % ring_size] = table[row_of[i] * width + (x - sum[i])];
+    }
+    returned += sum[kReleaseThreads];
+  }
+  if (tid == 0) cursor[1] = returned;
+}
+
+int64_t align256(int64_t v) { return (v + 255) & ~(int64_t)255; }
+
+}  // namespace
+
+int make_shape(const grm_b200_paged_plan& p, int sms, Shape* s) {
+  s->group = p.query_heads / p.kv_heads;
+  const int64_t most = std::min(p.max_fresh, p.tokens) * s->group;
+  s->block_rows = most <= 8 || p.head_dim == 256 ? 8 : 16;
+  s->split_rows = INT32_MAX;
+  s->qtile_tokens = 1;
+  s->workers = sms * (p.head_dim == 256 ? 2 : 3);
+  const int64_t R = p.requests, T = p.tokens;
+  s->page_cap = p.grow ? std::min(T, T / p.page_tokens + 2 * std::min(R, T)) : 0;
+  s->qtile_cap = 0;
+  int64_t at = align256(sizeof(Header));
+  auto take = [&](int64_t bytes) {
+    const int64_t o = at;
+    at += align256(bytes);
+    return o;
+  };
+  s->off_base = take((R + 1) * 8);
+  s->off_start = take((int64_t)s->workers * 4);
+  s->off_count = take((int64_t)s->workers * 4);
+  s->off_pages = take(std::min(T, T / p.page_tokens + 2 * std::min(R, T)) * 8);
+  s->off_qtiles = take(s->qtile_cap * 8);
+  s->off_part = take((int64_t)s->workers * 2 * kWorkerSlot * 4);
+  s->bytes = at;
+  return 0;
+}
+
+int current_sms(int* sms) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) {
+    set_thread_error("no current device: %s", cudaGetErrorString(e));
+    return cuda_status(e);
+  }
+  DeviceInfo info;
+  const int rc = device_info(dev, &info);
+  if (rc != 0) {
+    set_thread_error("device %d has no properties", dev);
+    return rc;
+  }
+  *sms = info.sms;
+  return 0;
+}
+
+int launch_status(const char* what) {
+  const cudaError_t e = cudaGetLastError();
+  if (e == cudaSuccess) return 0;
+  set_thread_error("%s launch failed: %s", what, cudaGetErrorString(e));
+  return cuda_status(e);
+}
+
+namespace {
+
+bool page_ok(int v) { return v == 16 || v == 32 || v == 64 || v == 128; }
+bool dim_ok(int v) { return v == 64 || v == 128 || v == 256; }
+
+int check_sizes(const grm_b200_paged_plan* p) {
+  if (!p) {
+    set_thread_error("paged plan: null plan");
+    return GRM_B200_EINVAL;
+  }
+  if (p->requests < 1 || p->requests > (1 << 24) || p->tokens < 1 || p->tokens > INT32_MAX ||
+      p->max_fresh < 1 || p->table_width < 1 || p->table_width > (1 << 28) || p->pages < 1 ||
+      p->pages > INT32_MAX) {
+    set_thread_error("paged plan: sizes out of range (requests %lld, tokens %lld, max_fresh %lld, "
+                     "table_width %lld, pages %lld)",
+                     (long long)p->requests, (long long)p->tokens, (long long)p->max_fresh,
+                     (long long)p->table_width, (long long)p->pages);
+    return GRM_B200_EINVAL;
+  }
+  if (!page_ok(p->page_tokens) || !dim_ok(p->head_dim)) {
+    set_thread_error("paged plan: page_tokens %d must be 16, 32, 64 or 128 and head_dim %d must be "
+                     "64, 128 or 256", p->page_tokens, p->head_dim);
+    return GRM_B200_EINVAL;
+  }
+  if (p->kv_heads < 1 || p->kv_heads > 1024 || p->query_heads < p->kv_heads ||
+      p->query_heads % p->kv_heads || p->query_heads / p->kv_heads > 128) {
+    set_thread_error("paged plan: query_heads %d must be a multiple of kv_heads %d, at most 128 "
+                     "query heads for each", p->query_heads, p->kv_heads);
+    return GRM_B200_EINVAL;
+  }
+  return 0;
+}
+
+}  // namespace
+
+int check_plan(const grm_b200_paged_plan* p) {
+  int rc = check_sizes(p);
+  if (rc) return rc;
+  if (!p->cached || !p->ring || !p->cursor_in || !p->table || !p->lens || !p->starts ||
+      !p->positions || !p->rows || !p->slots || !p->cursor || !p->status || !p->scratch) {
+    set_thread_error("paged plan: a buffer is missing");
+    return GRM_B200_EINVAL;
+  }
+  if (p->cursor == p->cursor_in || p->lens == p->cached) {
+    set_thread_error("paged plan: cursor and lens must not be the buffers they are made from");
+    return GRM_B200_EINVAL;
+  }
+  if (reinterpret_cast<uintptr_t>(p->scratch) & 255) {
+    set_thread_error("paged plan: scratch must be 256-byte aligned");
+    return GRM_B200_EINVAL;
+  }
+  int64_t need = 0;
+  rc = grm_b200_paged_scratch_bytes(p, &need);
+  if (rc) return rc;
+  if (p->scratch_bytes < need) {
+    set_thread_error("paged plan: scratch of %lld bytes, %lld needed",
+                     (long long)p->scratch_bytes, (long long)need);
+    return GRM_B200_EINVAL;
+  }
+  return 0;
+}
+
+int check_arena(const grm_b200_paged_arena* a) {
+  if (!a || !a->k_codes || !a->v_codes || !a->k_scales || !a->v_scales) {
+    set_thread_error("paged arena: a buffer is missing");
+    return GRM_B200_EINVAL;
+  }
+  if (a->pages < 1 || a->pages > INT32_MAX || a->kv_heads < 1 || a->kv_heads > 1024 ||
+      !page_ok(a->page_tokens) || !dim_ok(a->head_dim)) {
+    set_thread_error("paged arena: pages %lld, kv_heads %d, page_tokens %d (16, 32, 64, 128), "
+                     "head_dim %d (64, 128, 256)",
+                     (long long)a->pages, a->kv_heads, a->page_tokens, a->head_dim);
+    return GRM_B200_EINVAL;
+  }
+  if ((reinterpret_cast<uintptr_t>(a->k_codes) | reinterpret_cast<uintptr_t>(a->v_codes)) & 15) {
+    set_thread_error("paged arena: codes must be 16-byte aligned");
+    return GRM_B200_EINVAL;
+  }
+  return 0;
+}
+
+int check_match(const grm_b200_paged_plan* p, const grm_b200_paged_arena* a) {
+  if (a->pages != p->pages || a->kv_heads != p->kv_heads || a->page_tokens != p->page_tokens ||
+      a->head_dim != p->head_dim) {
+    set_thread_error("paged plan and arena differ: pages %lld / %lld, kv_heads %d / %d, "
+                     "page_tokens %d / %d, head_dim %d / %d",
+                     (long long)p->pages, (long long)a->pages, p->kv_heads, a->kv_heads,
+                     p->page_tokens, a->page_tokens, p->head_dim, a->head_dim);
+    return GRM_B200_EINVAL;
+  }
+  return 0;
+}
+
+}  // namespace paged
+}  // namespace grm_b200
+
+using namespace grm_b200;
+using namespace grm_b200::paged;
+
+extern "C" {
+
+int grm_b200_paged_scratch_bytes(const grm_b200_paged_plan* plan, int64_t* out_bytes) {
+  int rc = check_sizes(plan);
+  if (rc) return rc;
+  if (!out_bytes) {
+    set_thread_error("paged plan: null out_bytes");
+    return GRM_B200_EINVAL;
+  }
+  int sms = 0;
+  rc = current_sms(&sms);
+  if (rc) return rc;
+  Shape s;
+  make_shape(*plan, sms, &s);
+  *out_bytes = s.bytes;
+  return 0;
+}
+
+int grm_b200_paged_plan_step(const grm_b200_paged_plan* plan, const int32_t* fresh_device,
+                             void* stream) {
+  int rc = check_plan(plan);
+  if (rc) return rc;
+  if (!fresh_device) {
+    set_thread_error("paged plan: null fresh");
+    return GRM_B200_EINVAL;
+  }
+  int sms = 0;
+  if ((rc = current_sms(&sms))) return rc;
+  PlanParams p;
+  p.requests = plan->requests;
+  p.tokens = plan->tokens;
+  p.max_fresh = plan->max_fresh;
+  p.width = plan->table_width;
+  p.ring_size = plan->pages;
+  p.page_shift = shift_of(plan->page_tokens);
+  p.grow = plan->grow ? 1 : 0;
+  p.kv_heads = plan->kv_heads;
+  make_shape(*plan, sms, &p.s);
+  p.min_units = 3;
+  p.cached = plan->cached;
+  p.fresh = fresh_device;
+  p.ring = plan->ring;
+  p.cursor_in = plan->cursor_in;
+  p.table = plan->table;
+  p.lens = plan->lens;
+  p.starts = plan->starts;
+  p.positions = plan->positions;
+  p.rows = plan->rows;
+  p.slots = plan->slots;
+  p.cursor = plan->cursor;
+  p.status = plan->status;
+  p.l = lists_of(p.s, plan->scratch);
+  // a block for every 2,048 rows, at most one an SM: each also repeats the sums
+  const int64_t blocks = std::min<int64_t>(sms, ceil_div64(plan->tokens, 2 * kPlanThreads));
+  plan_kernel<<<(unsigned)blocks, kPlanThreads, 0, static_cast<cudaStream_t>(stream)>>>(p);
+  return launch_status("paged plan");
+}
+
+int grm_b200_paged_release(const int32_t* rows_device, int64_t count, int64_t requests,
+                           int64_t table_width, int64_t pages, int page_tokens,
+                           const int32_t* table, int32_t* lens, int32_t* ring, int64_t* cursor,
+                           void* stream) {
+  if (!rows_device || !table || !lens || !ring || !cursor || count < 0 || requests < 1 ||
+      table_width < 1 || pages < 1 || !page_ok(page_tokens)) {
+    set_thread_error("invalid paged release arguments");
+    return GRM_B200_EINVAL;
+  }
+  if (count == 0) return 0;
+  release_kernel<<<1, kReleaseThreads, 0, static_cast<cudaStream_t>(stream)>>>(
+      rows_device, count, requests, table_width, pages, shift_of(page_tokens), table, lens, ring,
+      cursor);
+  return launch_status("paged release");
+}
+
+}  // extern "C"

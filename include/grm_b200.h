@@ -404,6 +404,143 @@ int grm_b200_upload_rows(const void* const* parts_host, const int64_t* part_row_
                          int n_parts, int64_t rows, void* dst_device, int64_t dst_row_bytes,
                          void* stream);
 
+/* ------------------------------------------------------------ 8-bit paged arena */
+
+/* A mounted arena for many requests, held at 8 bits: pages of page_tokens
+ * tokens, each page belonging to one request at a time, and for every (page,
+ * kv head) one fp32 scale for the keys and one for the values.  A stored value
+ * is code * scale; a scale is the largest absolute value of its page and head
+ * divided by 127, so codes lie in [-127, 127].  No reference counterpart: the
+ * reference's arena is one request's 16-bit cache, and its model adapters run
+ * attention in the external engine (core/graft_arena.py:1-26); the codes follow
+ * the symmetric law of core/graft_quant.py:93-133 with the group made one head
+ * of one page.
+ *
+ * One grm_b200_paged_arena names the device buffers of one layer:
+ * k_codes / v_codes int8 [pages, kv_heads, page_tokens, head_dim] (16-byte
+ * aligned), k_scales / v_scales fp32 [pages, kv_heads].  page_tokens is 16,
+ * 32, 64 or 128 and head_dim 64, 128 or 256. */
+typedef struct grm_b200_paged_arena {
+  int8_t* k_codes;
+  int8_t* v_codes;
+  float* k_scales;
+  float* v_scales;
+  int64_t pages;
+  int32_t kv_heads;
+  int32_t page_tokens;
+  int32_t head_dim;
+} grm_b200_paged_arena;
+
+/* One step of `requests` requests.  Sizes first: `tokens` is the capacity of
+ * the step's packed rows (request 0's new rows, request 1's, ...), max_fresh
+ * the most new rows one request may have, table_width the entries of a block
+ * table row, pages the size of the ring of free pages.
+ * In (device): cached[requests], the tokens each request holds; ring[pages],
+ * page numbers of which entries cursor_in[0] .. cursor_in[1]-1 (modulo pages)
+ * are free: cursor_in = {pages ever taken, pages ever returned}.
+ * In and out: table[requests, table_width], page numbers in token order.
+ * Out: lens[requests] (cached + fresh); starts[requests + 1], the first packed
+ * row of each request; positions[tokens], rows[tokens] (the request of a packed
+ * row) and slots[tokens] (page * page_tokens + offset), -1 past the last row;
+ * cursor[2]; status[1], GRM_B200_PLAN_* bits.  cursor and cursor_in must not
+ * be the same buffer, nor lens and cached: planning again plans the same step,
+ * and the caller takes a step up by making the new lengths the cached ones.
+ * scratch: scratch_bytes (grm_b200_paged_scratch_bytes) of device memory, the
+ * step's work lists and the partial results of attention; calls that share it
+ * must not overlap on the GPU. */
+typedef struct grm_b200_paged_plan {
+  int64_t requests;
+  int64_t tokens;
+  int64_t max_fresh;
+  int64_t table_width;
+  int64_t pages;
+  int32_t page_tokens;
+  int32_t kv_heads;
+  int32_t query_heads;
+  int32_t head_dim;
+  int32_t grow;
+  const int32_t* cached;
+  const int32_t* ring;
+  const int64_t* cursor_in;
+  int32_t* table;
+  int32_t* lens;
+  int32_t* starts;
+  int32_t* positions;
+  int32_t* rows;
+  int64_t* slots;
+  int64_t* cursor;
+  int32_t* status;
+  void* scratch;
+  int64_t scratch_bytes;
+} grm_b200_paged_plan;
+
+/* Status bits of a plan.  A step that cannot be planned takes no page and has
+ * no rows: lens = cached, starts = 0, rows/positions/slots = -1; append writes
+ * nothing and attend returns empty rows. */
+#define GRM_B200_PLAN_BAD_LENGTH 1  /* a negative length, or past 2^31 - 1 tokens */
+#define GRM_B200_PLAN_ROWS 2        /* more new rows than `tokens` or `max_fresh` */
+#define GRM_B200_PLAN_TABLE 4       /* a request needs more than table_width pages */
+#define GRM_B200_PLAN_PAGES 8       /* not enough free pages */
+
+/* Scratch bytes of a plan of these sizes (the pointers are not read). */
+int grm_b200_paged_scratch_bytes(const grm_b200_paged_plan* plan, int64_t* out_bytes);
+
+/* Plan a step from the requests' lengths, on the GPU and in one launch:
+ * request r holds cached[r] tokens and brings fresh_device[r] new rows.  With
+ * plan->grow != 0 the new rows are tokens that join the request: their pages
+ * are taken from the ring (in request order) and entered in the table.  With
+ * grow == 0 they only read what is cached: no page is taken, lens = cached,
+ * slots are -1, and attention over the plan is not causal. */
+int grm_b200_paged_plan_step(const grm_b200_paged_plan* plan, const int32_t* fresh_device,
+                             void* stream);
+
+/* Return the pages of the requests rows_device[count] to the ring (in the
+ * order of the list) and set their lengths to 0; a row that is out of range or
+ * listed twice is returned once or not at all.  Changes lens, ring, cursor in
+ * place. */
+int grm_b200_paged_release(const int32_t* rows_device, int64_t count, int64_t requests,
+                           int64_t table_width, int64_t pages, int page_tokens,
+                           const int32_t* table, int32_t* lens, int32_t* ring, int64_t* cursor,
+                           void* stream);
+
+/* Quantise a planned step's rows into the arena: k and v [tokens, kv_heads,
+ * head_dim] of element type `dtype` (GRM_B200_F16 or GRM_B200_BF16), given by
+ * their row and head strides in elements (multiples of 8, 16-byte aligned
+ * pointers; the head_dim values of a row are contiguous).  The scale of a page
+ * becomes max(scale of the older tokens it holds, max |x| / 127); when it
+ * grows, the older codes are rescaled, code' = rint(code * old / new).  New
+ * codes are rint(x / scale), ties to even, every step in fp32.  A page that
+ * takes a NaN or an infinity gets scale NaN, so what it holds reads as NaN
+ * until the page starts anew.  Writing the same step twice writes the same
+ * codes.  The plan must have been made with grow != 0. */
+int grm_b200_paged_append(const grm_b200_paged_plan* plan, const grm_b200_paged_arena* arena,
+                          const void* k_device, const void* v_device, int dtype,
+                          int64_t k_row_stride, int64_t k_head_stride, int64_t v_row_stride,
+                          int64_t v_head_stride, void* stream);
+
+/* Rows of the arena as values: out_k / out_v [count, kv_heads, head_dim] of
+ * type out_dtype (GRM_B200_F32, _F16 or _BF16) = code * scale at
+ * slots_device[count], rounded once; a negative slot gives a row of zeros.
+ * Slots must be below pages * page_tokens (others read as zeros too). */
+int grm_b200_paged_read(const grm_b200_paged_arena* arena, const int64_t* slots_device,
+                        int64_t count, int out_dtype, void* out_k_device, void* out_v_device,
+                        void* stream);
+
+/* Attention of a planned step's query rows q [tokens, query_heads, head_dim]
+ * (GRM_B200_F16 or GRM_B200_BF16; strides and alignment as append's) over the
+ * arena: query head j reads kv head j / (query_heads / kv_heads);
+ *   out[i, j] = sum_t w_t v_t,  w = softmax_t(softmax_scale * q_ij . k_t),
+ * over the request's lens[r] tokens, or with causal != 0 over the positions up
+ * to the row's own.  out [tokens, query_heads, head_dim] has q's type; lse
+ * [tokens, query_heads] fp32 (may be NULL) is the natural logarithm of the sum
+ * of exponentials.  A row that sees nothing is 0 with lse -inf, as are the
+ * rows past the step's last one.  Results do not depend on the order in which
+ * blocks run. */
+int grm_b200_paged_attend(const grm_b200_paged_plan* plan, const grm_b200_paged_arena* arena,
+                          const void* q_device, int dtype, int64_t q_row_stride,
+                          int64_t q_head_stride, float softmax_scale, int causal,
+                          void* out_device, float* lse_device, void* stream);
+
 /* ----------------------------------------------------- multi-GPU top-k merge */
 
 /* Merge `lists` candidate lists of `per_list` (score, id) entries each (device
