@@ -68,6 +68,83 @@ __host__ __device__ inline int64_t worker_of(int64_t u, int64_t units, int64_t w
   return ((u + 1) * workers - 1) / units;
 }
 
+// ---- attention
+
+constexpr float kLazy = 8.0f;  // how far a row's scores may pass its reference exponent
+
+struct AttendParams {
+  Lists l;
+  const int32_t* table;
+  const int32_t* lens;
+  const int32_t* starts;
+  int64_t width, tokens, pages;
+  int page_shift, kv_heads, group, causal, block_rows, qtile_tokens;
+  const int8_t* k;
+  const int8_t* v;
+  const float* ks;
+  const float* vs;
+  const uint16_t* q;
+  int64_t q_row, q_head;
+  float scale_log2;
+  uint16_t* out;
+  float* lse;
+  int32_t* status;
+};
+
+// Rows of requests with more than split_rows (row, head) pairs (paged_prompt.cu).
+int launch_prompt(int dtype, int dim, const AttendParams& p, int64_t blocks, cudaStream_t st);
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Two codes, chosen by `sel` from the four of w (already + 128), as halves.
+__device__ __forceinline__ uint32_t halves(uint32_t w, uint32_t sel) {
+  const uint32_t v = __byte_perm(w, 0x64646464u, sel);
+  const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&v),
+                            __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480)));
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+__device__ __forceinline__ uint32_t pack_half2(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack_out(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack_out<__half>(float a, float b) { return pack_half2(a, b); }
+template <>
+__device__ __forceinline__ uint32_t pack_out<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// The power of two that brings a bf16 row, whose largest magnitude has the bits
+// m, into [2^14, 2^15), and its inverse; rows of zeros or below 2^-100 keep out
+// of the way of overflow.
+__device__ __forceinline__ void row_scale(unsigned m, float* up, float* down) {
+  const int e = max((int)(m >> 7), 27);  // biased exponent
+  *up = m ? __uint_as_float((unsigned)(127 + 14 + 127 - e) << 23) : 1.0f;
+  *down = m ? __uint_as_float((unsigned)(e - 14) << 23) : 1.0f;
+}
+// Base-2 logarithm and inverse of a value scale.  A page of zeros (scale 0)
+// takes 2^-40, any scale being right for it: small enough to leave the other
+// pages' weights alone, large enough for its own to stay above 2^-126 when the
+// reference exponent is another page's.  Scales below 2^-100 count as 2^-100.
+__device__ __forceinline__ void value_scale(float u, float* log2_u, float* inv_u) {
+  const float w = u == 0.0f ? 0x1p-40f : fmaxf(u, 0x1p-100f);
+  *log2_u = u != u ? u : __log2f(w);
+  *inv_u = 1.0f / w;
+}
+// Two bf16 times `up` as halves.
+__device__ __forceinline__ uint32_t scale_pair(uint32_t v, float up) {
+  return pack_half2(__uint_as_float(v << 16) * up, __uint_as_float(v & 0xFFFF0000u) * up);
+}
+
 int check_plan(const grm_b200_paged_plan* p);
 int check_arena(const grm_b200_paged_arena* a);
 // The two describe the same pages and heads.

@@ -10,8 +10,7 @@
 // p_t u-weighted is what multiplies b_t, and the sum of weights is
 // sum_t p_t / u_t, so p_t never exceeds 2^8 whatever the scales are and fp16
 // holds it (m trails the largest y seen by at most 8: it moves only when a y
-// passes m + 8, so the accumulators are rarely rescaled).  Scales below 2^-100
-// count as 2^-100.  The log-sum-exp is m ln 2 + log of that sum.
+// passes m + 8, so the accumulators are rarely rescaled).   The log-sum-exp is m ln 2 + log of that sum.
 //
 // The split kernel serves few query rows a kv head (decoding, a few proposed
 // tokens): it is bound by the bytes of the codes, 2 * head_dim a token and kv
@@ -32,6 +31,7 @@
 // value into [2^14, 2^15), so only values 2^29 times smaller than the largest
 // round.
 #include <algorithm>
+#include <type_traits>
 
 #include "paged.cuh"
 
@@ -42,25 +42,6 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-constexpr float kLazy = 8.0f;
-
-struct AttendParams {
-  Lists l;
-  const int32_t* table;
-  const int32_t* lens;
-  const int32_t* starts;
-  int64_t width, tokens, pages;
-  int page_shift, kv_heads, group, causal, block_rows;
-  const int8_t* k;
-  const int8_t* v;
-  const float* ks;
-  const float* vs;
-  const uint16_t* q;
-  int64_t q_row, q_head;
-  float scale_log2;
-  uint16_t* out;
-  float* lse;
-};
 
 template <int D, int NT>
 struct Layout {
@@ -113,35 +94,6 @@ __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-// Two codes, chosen by `sel` from the four of w (already + 128), as halves.
-__device__ __forceinline__ uint32_t halves(uint32_t w, uint32_t sel) {
-  const uint32_t v = __byte_perm(w, 0x64646464u, sel);
-  const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&v),
-                            __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480)));
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-
-__device__ __forceinline__ uint32_t pack_half2(float a, float b) {
-  const __half2 h = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-
-template <typename T>
-__device__ __forceinline__ uint32_t pack_out(float a, float b);
-template <>
-__device__ __forceinline__ uint32_t pack_out<__half>(float a, float b) { return pack_half2(a, b); }
-template <>
-__device__ __forceinline__ uint32_t pack_out<__nv_bfloat16>(float a, float b) {
-  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-
 // Byte of chunk c (16 codes) of row r in a 16-row tile whose rows are D codes:
 // 16-byte chunks are permuted so that eight rows of one chunk lie in eight
 // different bank groups (ldmatrix reads them together).
@@ -305,7 +257,7 @@ __global__ void __launch_bounds__(kThreads, Layout<D, NT>::kBlocks)
           raw[c] = __ldg(reinterpret_cast<const uint2*>(qp + c * 16));
       }
       float unscale = 1.0f;
-      if constexpr (sizeof(T) == 2 && !std::is_same<T, __half>::value) {
+      if constexpr (!std::is_same<T, __half>::value) {
         unsigned m = 0;
 #pragma unroll
         for (int c = 0; c < kChunks; ++c)
@@ -313,15 +265,12 @@ __global__ void __launch_bounds__(kThreads, Layout<D, NT>::kBlocks)
         m = max(m & 0xFFFFu, m >> 16);
         m = max(m, __shfl_xor_sync(kFull, m, 1));
         m = max(m, __shfl_xor_sync(kFull, m, 2));
-        const int e = max((int)(m >> 7), 27);  // biased exponent of the largest value
-        const float up = m ? __uint_as_float((unsigned)(127 + 14 + 127 - e) << 23) : 1.0f;
-        unscale = m ? __uint_as_float((unsigned)(e - 14) << 23) : 1.0f;
+        float up;
+        row_scale(m, &up, &unscale);
 #pragma unroll
         for (int c = 0; c < kChunks; ++c) {
-          qf[c][nt][0] = pack_half2(__uint_as_float(raw[c].x << 16) * up,
-                                    __uint_as_float(raw[c].x & 0xFFFF0000u) * up);
-          qf[c][nt][1] = pack_half2(__uint_as_float(raw[c].y << 16) * up,
-                                    __uint_as_float(raw[c].y & 0xFFFF0000u) * up);
+          qf[c][nt][0] = scale_pair(raw[c].x, up);
+          qf[c][nt][1] = scale_pair(raw[c].y, up);
         }
       } else {
 #pragma unroll
@@ -361,8 +310,8 @@ __global__ void __launch_bounds__(kThreads, Layout<D, NT>::kBlocks)
       if (tok < s.len) {
         const uint32_t kb = ring + stage * LY::kStage, vb = kb + LY::kSide;
         const float ks = scales[(warp * LY::kStages + stage) * 2];
-        const float vs = fmaxf(scales[(warp * LY::kStages + stage) * 2 + 1], 0x1p-100f);
-        const float vs_raw = scales[(warp * LY::kStages + stage) * 2 + 1];
+        float lv, inv;
+        value_scale(scales[(warp * LY::kStages + stage) * 2 + 1], &lv, &inv);
         // scores of 16 tokens x 8 NT rows, in two independent chains
         float sc[NT][2][4];
 #pragma unroll
@@ -383,8 +332,6 @@ __global__ void __launch_bounds__(kThreads, Layout<D, NT>::kBlocks)
               mma(sc[nt][x], a0, a1, a2, a3, qf[c + x][nt][0], qf[c + x][nt][1]);
           }
         }
-        const float lv = vs_raw != vs_raw ? vs_raw : __log2f(vs);
-        const float inv = 1.0f / vs;
         uint32_t b[NT][2];
         float y[NT][4];
         bool moves = false;
@@ -704,10 +651,15 @@ int grm_b200_paged_attend(const grm_b200_paged_plan* plan, const grm_b200_paged_
   p.scale_log2 = softmax_scale * 1.44269504088896341f;
   p.out = static_cast<uint16_t*>(out_device);
   p.lse = lse_device;
+  p.qtile_tokens = s.qtile_tokens;
+  p.status = plan->status;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return dtype == GRM_B200_F16
-             ? launch_split_any<__half>(plan->head_dim, s.block_rows, p, s.workers, st)
-             : launch_split_any<__nv_bfloat16>(plan->head_dim, s.block_rows, p, s.workers, st);
+  rc = dtype == GRM_B200_F16
+           ? launch_split_any<__half>(plan->head_dim, s.block_rows, p, s.workers, st)
+           : launch_split_any<__nv_bfloat16>(plan->head_dim, s.block_rows, p, s.workers, st);
+  if (rc == 0 && s.qtile_cap > 0)
+    rc = launch_prompt(dtype, plan->head_dim, p, s.qtile_cap * plan->kv_heads, st);
+  return rc;
 }
 
 }  // extern "C"

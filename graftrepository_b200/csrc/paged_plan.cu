@@ -324,6 +324,9 @@ __global__ void __launch_bounds__(kReleaseThreads)
   if (tid == 0) cursor[1] = returned;
 }
 
+// Requests with more (row, head) pairs a kv head than this are prompts.
+constexpr int kPromptRows = 64;
+
 int64_t align256(int64_t v) { return (v + 255) & ~(int64_t)255; }
 
 }  // namespace
@@ -332,12 +335,13 @@ int make_shape(const grm_b200_paged_plan& p, int sms, Shape* s) {
   s->group = p.query_heads / p.kv_heads;
   const int64_t most = std::min(p.max_fresh, p.tokens) * s->group;
   s->block_rows = most <= 8 || p.head_dim == 256 ? 8 : 16;
-  s->split_rows = INT32_MAX;
-  s->qtile_tokens = 1;
+  const bool prompts = p.head_dim <= 128 && most > kPromptRows;
+  s->split_rows = prompts ? kPromptRows : INT32_MAX;
+  s->qtile_tokens = 2 * (128 / s->group);
   s->workers = sms * (p.head_dim == 256 ? 2 : 3);
   const int64_t R = p.requests, T = p.tokens;
   s->page_cap = p.grow ? std::min(T, T / p.page_tokens + 2 * std::min(R, T)) : 0;
-  s->qtile_cap = 0;
+  s->qtile_cap = prompts ? std::min(T, T / s->qtile_tokens + std::min(R, T)) : 0;
   int64_t at = align256(sizeof(Header));
   auto take = [&](int64_t bytes) {
     const int64_t o = at;

@@ -42,12 +42,13 @@ __all__ = ["PAGE_TOKENS", "HEAD_DIMS", "PageTables", "PagePlan", "PagedArena"]
 PAGE_TOKENS = (16, 32, 64, 128)
 HEAD_DIMS = (64, 128, 256)
 
-PLAN_BAD_LENGTH, PLAN_ROWS, PLAN_TABLE, PLAN_PAGES = 1, 2, 4, 8
+PLAN_BAD_LENGTH, PLAN_ROWS, PLAN_TABLE, PLAN_PAGES, PLAN_WAIT = 1, 2, 4, 8, 16
 _REASONS = {
     PLAN_BAD_LENGTH: "a negative length, or one past 2^31 - 1",
     PLAN_ROWS: "more new rows than the plan has room for (tokens, max_fresh)",
     PLAN_TABLE: "a request needs more pages than its block table row has entries",
     PLAN_PAGES: "not enough free pages",
+    PLAN_WAIT: "a wait inside attention gave up and rows are missing",
 }
 
 
@@ -180,12 +181,12 @@ class PagePlan:
         return bool(self.c.grow)
 
     def check(self) -> None:
-        """Wait for the plan and raise if the step could not be planned (it
-        then took no pages and has no rows)."""
+        """Wait for the plan (and calls that used it) and raise if the step
+        could not be planned: it then took no pages and has no rows."""
         bits = int(self.status.item())
         if bits:
             why = "; ".join(text for bit, text in _REASONS.items() if bits & bit)
-            raise _lib.GrmB200Error(bits, f"the step cannot be planned: {why}")
+            raise _lib.GrmB200Error(bits, f"the step failed: {why}")
 
 
 class PageTables:

@@ -481,6 +481,7 @@ typedef struct grm_b200_paged_plan {
 #define GRM_B200_PLAN_ROWS 2        /* more new rows than `tokens` or `max_fresh` */
 #define GRM_B200_PLAN_TABLE 4       /* a request needs more than table_width pages */
 #define GRM_B200_PLAN_PAGES 8       /* not enough free pages */
+#define GRM_B200_PLAN_WAIT 16       /* a bounded wait inside attend gave up: rows are missing */
 
 /* Scratch bytes of a plan of these sizes (the pointers are not read). */
 int grm_b200_paged_scratch_bytes(const grm_b200_paged_plan* plan, int64_t* out_bytes);
