@@ -16,11 +16,15 @@
 //                   tensor memory, p back as fp16 over them, and when a row's
 //                   reference exponent has to move (rarely: it trails by up
 //                   to 8), its result in tensor memory rescaled
-//   warps 8-11      codes from their pages to fp16 key and value tiles in
-//                   shared memory (two of each), read one tile ahead
-//   warp 12         tensor memory, and one lane that issues the products
-//                   S = Q K^T (both from shared memory) and O += P V (P from
-//                   tensor memory)
+//   warps 8-11      codes in shared memory to fp16 key and value tiles (two of
+//                   each)
+//   warps 12, 13    one lane each that issues a query tile's products, S = Q K^T
+//                   (both from shared memory) and O += P V (P from tensor
+//                   memory).  A thread that waits on a barrier first sees its
+//                   own commits out of the queue of products, so with one
+//                   thread for both tiles the tensor cores ran dry at every
+//                   wait, about 250 clocks each
+//   warp 14         codes from their pages to shared memory, one bulk copy a page
 // While one query tile's softmax runs, the tensor cores work for the other.
 // Keys and values have the same layout in shared memory, 128-byte rows of 64
 // dims with a 128-byte swizzle: K is read K-major, V with its dims contiguous.
@@ -37,10 +41,12 @@ namespace {
 
 constexpr int kM = 128;             // rows of a query tile
 constexpr int kN = 128;             // tokens of a key tile
+constexpr int kHalf = kN / 2;       // tokens of one softmax step
 constexpr int kSoftWarps = 8;
 constexpr int kConvWarps = 4;
 constexpr int kMmaWarp = kSoftWarps + kConvWarps;
-constexpr int kPromptThreads = (kMmaWarp + 1) * 32;
+constexpr int kLoadWarp = kMmaWarp + 2;
+constexpr int kPromptThreads = (kLoadWarp + 1) * 32;
 constexpr int kScaleRing = 4;       // key tiles whose scales are held
 constexpr uint32_t kTmemCols = 512;
 constexpr unsigned kProbes = 1u << 22;  // probes of a bounded wait
@@ -49,7 +55,8 @@ template <int D>
 struct PromptLayout {
   static constexpr int kAtom = kN * 128;            // 128 rows x 64 halves
   static constexpr int kTile = (D / 64) * kAtom;    // a query, key or value tile
-  static constexpr int kUsed = 1024 + 6 * kTile + kScaleRing * 8 * 16;
+  static constexpr int kRaw = kN * D;               // its codes
+  static constexpr int kUsed = 1024 + 6 * kTile + 2 * kRaw + kScaleRing * 8 * 16;
   // one block an SM: it owns all of tensor memory
   static constexpr int kSmem = kUsed > 120 * 1024 ? kUsed : 120 * 1024;
   static constexpr uint32_t kScore = 0;             // tensor memory columns
@@ -65,6 +72,31 @@ __host__ __device__ constexpr uint32_t idesc(int n, bool b_mn) {
 
 // Byte of 16-byte chunk c (8 halves of 64) of row r in a swizzled atom.
 __device__ __forceinline__ uint32_t atom_byte(int r, int c) { return r * 128 + ((c ^ (r & 7)) << 4); }
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ float max3(uint32_t a, uint32_t b, uint32_t c) {
+  return max3(__uint_as_float(a), __uint_as_float(b), __uint_as_float(c));
+}
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)),
+        "l"(reinterpret_cast<const uint64_t&>(c)));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)));
+  return d;
+}
 
 // Every lane of a warp waits; false, for all of them, when a wait gave up.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, unsigned parity, volatile int* fail) {
@@ -98,9 +130,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
   unsigned char* const sm_q = sm;                       // [2]
   unsigned char* const sm_k = sm + 2 * LY::kTile;       // [2]
   unsigned char* const sm_v = sm + 4 * LY::kTile;       // [2]
-  Scale* const sm_scale = reinterpret_cast<Scale*>(sm + 6 * LY::kTile);  // [kScaleRing][8]
-  __shared__ __align__(8) uint64_t q_full, drained, k_full[2], k_empty[2], v_full[2], v_empty[2],
-      scale_full[kScaleRing], s_full[2], p_full[2], o_done[2];
+  unsigned char* const sm_raw = sm + 6 * LY::kTile;     // codes: keys, values
+  Scale* const sm_scale = reinterpret_cast<Scale*>(sm_raw + 2 * LY::kRaw);  // [kScaleRing][8]
+  __shared__ __align__(8) uint64_t q_full[2], drained[2], k_full[2], k_empty[2], v_full[2], v_empty[2],
+      scale_full[kScaleRing], raw_full[2], raw_empty[2], s_full[2][2], p_full[2][2], o_full[2];
   __shared__ uint32_t sh_tmem;
   __shared__ int sh_fail;
 
@@ -123,6 +156,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
   const int heads = p.kv_heads * p.group;
   const int sees = p.causal ? min(len, cached + tok0 + toks[0] + toks[1]) : len;
   const int tiles = (sees + kN - 1) / kN;
+  const int halves_seen = (sees + kHalf - 1) / kHalf;
 
   if (tiles == 0) {  // nothing cached: empty rows
     for (int x = threadIdx.x; x < (toks[0] + toks[1]) * p.group * (D / 2); x += kPromptThreads) {
@@ -135,16 +169,20 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
   }
 
   if (threadIdx.x == 0) {
-    mbar_init(&q_full, two ? kSoftWarps : kSoftWarps / 2);
-    mbar_init(&drained, 1);
     for (int i = 0; i < 2; ++i) {
+      mbar_init(&q_full[i], kSoftWarps / 2);
+      mbar_init(&drained[i], 1);
       mbar_init(&k_full[i], kConvWarps);
-      mbar_init(&k_empty[i], 1);
+      mbar_init(&k_empty[i], two ? 2 : 1);
       mbar_init(&v_full[i], kConvWarps);
-      mbar_init(&v_empty[i], 1);
-      mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], kSoftWarps / 2);
-      mbar_init(&o_done[i], 1);
+      mbar_init(&v_empty[i], two ? 2 : 1);
+      mbar_init(&raw_full[i], 1);
+      mbar_init(&raw_empty[i], kConvWarps);
+      for (int x = 0; x < 2; ++x) {
+        mbar_init(&s_full[i][x], 1);
+        mbar_init(&p_full[i][x], kSoftWarps / 2);
+      }
+      mbar_init(&o_full[i], 1);
     }
     for (int i = 0; i < kScaleRing; ++i) mbar_init(&scale_full[i], 1);
     mbar_fence_init();
@@ -205,96 +243,113 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
       }
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&q_full);
+      if (lane == 0) mbar_arrive(&q_full[t]);
 
       const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
       const uint32_t s_col = tmem + lanes + LY::kScore + t * kN;
       const uint32_t o_col = tmem + lanes + LY::kResult + t * D;
       float m = -INFINITY, l = 0.0f;
       bool ok = true;
-      for (int j = 0; j < tiles && ok; ++j) {
-        ok = warp_wait(&scale_full[j % kScaleRing], (j / kScaleRing) & 1, fail) &&
-             warp_wait(&s_full[t], j & 1, fail);
-        if (!ok) break;
+#pragma unroll 1
+      for (int i = 0; i < halves_seen; ++i) {
+        const int j = i >> 1, hb = i & 1;
+        if ((hb == 0 && !warp_wait(&scale_full[j % kScaleRing], (j / kScaleRing) & 1, fail)) ||
+            !warp_wait(&s_full[t][hb], j & 1, fail)) {
+          ok = false;
+          break;
+        }
         tc_fence_after();
-        const Scale* sc = sm_scale + (j % kScaleRing) * 8;
-        const int t0 = j * kN;
-        const bool masked = __any_sync(kFull, t0 + kN > lim);
-        // the largest exponent of the row's 128 scores
+        const Scale* sc = sm_scale + (j % kScaleRing) * 8 + hb * 4;
+        const int t0 = i * kHalf;
+        // Factor and offset of the exponents of 16 tokens.  Hidden from the row
+        // altogether they have 1 and 0, so that a page without a number does not
+        // reach it; a factor too small for fp32 stays above 0.
+        auto factors = [&](int g, float* k, float* lu) {
+          const bool hidden = t0 + 16 * g >= lim;
+          *k = kq * sc[g].key;
+          if (*k == 0.0f) *k = 0x1p-126f;
+          if (hidden) *k = 1.0f;
+          *lu = hidden ? 0.0f : sc[g].log2_value;
+        };
+        // the row's 64 scores, in registers from here on
+        uint32_t v[2][32];
+        tmem_ld32_nowait(s_col + hb * kHalf, v[0]);
+        tmem_ld32_nowait(s_col + hb * kHalf + 32, v[1]);
+        tmem_wait_ld32(v[0]);
+        tmem_wait_ld32(v[1]);
+        // hidden tokens: scores of -inf (no factor is 0)
+        if (__any_sync(kFull, t0 + kHalf > lim)) {
+#pragma unroll
+          for (int x = 0; x < kHalf; ++x)
+            if (t0 + x >= lim) v[x / 32][x % 32] = 0xFF800000u;
+        }
         float top = -INFINITY;
-        uint32_t v[32];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          tmem_ld32_nowait(s_col + 32 * c, v);
-          tmem_wait_ld32(v);
-#pragma unroll
-          for (int g = 0; g < 2; ++g) {
-            const Scale x = sc[2 * c + g];
-            const float k = kq * x.key;
-            if (masked) {
-#pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                const float y = fmaf(__uint_as_float(v[16 * g + i]), k, x.log2_value);
-                top = fmaxf(top, t0 + 32 * c + 16 * g + i < lim ? y : -INFINITY);
-              }
-            } else {
-              float y = __uint_as_float(v[16 * g]);
-#pragma unroll
-              for (int i = 1; i < 16; ++i) y = fmaxf(y, __uint_as_float(v[16 * g + i]));
-              top = fmaxf(top, fmaf(y, k, x.log2_value));
-            }
-          }
+        for (int g = 0; g < 4; ++g) {
+          const uint32_t* x = v[g / 2] + 16 * (g % 2);
+          const float y = max3(max3(max3(x[0], x[1], x[2]), max3(x[3], x[4], x[5]),
+                                    max3(x[6], x[7], x[8])),
+                               max3(x[9], x[10], x[11]),
+                               max3(max3(x[12], x[13], x[14]), __uint_as_float(x[15]),
+                                    -INFINITY));
+          float k, lu;
+          factors(g, &k, &lu);
+          top = fmaxf(top, fmaf(y, k, lu));
         }
         if (__any_sync(kFull, top > m + kLazy)) {
           const float next = top > m + kLazy ? top : m;
           const float a = next == m ? 1.0f : ex2(m - next);
           m = next;
           l *= a;
-          if (j > 0) {  // the products up to tile j - 1 ended before these scores
+          if (i > 0) {  // once the products of the half before have ended
+            if (!warp_wait(&o_full[t], (i - 1) & 1, fail)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < D / 16; ++c) {
+              uint32_t o[16];
+              tmem_ld16(o_col + 16 * c, o);
 #pragma unroll
-            for (int c = 0; c < D / 32; ++c) {
-              tmem_ld32_nowait(o_col + 32 * c, v);
-              tmem_wait_ld32(v);
-#pragma unroll
-              for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * a);
-              tmem_st32(o_col + 32 * c, v);
+              for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * a);
+              tmem_st16(o_col + 16 * c, o);
             }
           }
         }
         const float ref = m == -INFINITY ? 0.0f : m;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          tmem_ld32_nowait(s_col + 32 * c, v);
-          tmem_wait_ld32(v);
+        for (int c = 0; c < 2; ++c) {
           uint32_t w[16];
 #pragma unroll
-          for (int g = 0; g < 2; ++g) {
-            const Scale x = sc[2 * c + g];
-            const float k = kq * x.key, off = x.log2_value - ref;
-            float pr[16];
+          for (int h2 = 0; h2 < 2; ++h2) {
+            float k1, lu;
+            factors(2 * c + h2, &k1, &lu);
+            const float2 k = make_float2(k1, k1), off = make_float2(lu - ref, lu - ref);
+            float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              float y = fmaf(__uint_as_float(v[16 * g + i]), k, off);
-              if (masked && t0 + 32 * c + 16 * g + i >= lim) y = -INFINITY;
-              pr[i] = ex2(y);
-            }
-            float sum = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 16; i += 2) {
-              sum += pr[i] + pr[i + 1];
-              w[8 * g + i / 2] = pack_half2(pr[i], pr[i + 1]);
+            for (int x = 0; x < 16; x += 2) {
+              const float2 y = fma2(make_float2(__uint_as_float(v[c][16 * h2 + x]),
+                                                __uint_as_float(v[c][16 * h2 + x + 1])),
+                                    k, off);
+              const float2 pr = make_float2(ex2(y.x), ex2(y.y));
+              sum = add2(sum, pr);
+              w[8 * h2 + x / 2] = pack_half2(pr.x, pr.y);
             }
             // a page without a number counts only where it is seen
-            l += sum == 0.0f ? 0.0f : sum * x.inv_value;
+            const float total = sum.x + sum.y;
+            l += total == 0.0f ? 0.0f : total * sc[2 * c + h2].inv_value;
           }
-          tmem_st16(s_col + 16 * c, w);
+          tmem_st16(s_col + hb * kHalf + 16 * c, w);
         }
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[t]);
+        if (lane == 0) mbar_arrive(&p_full[t][hb]);
       }
-      if (ok && warp_wait(&o_done[t], 0, fail)) {
+      // the last two products: a barrier is waited for phase by phase
+      if (ok && halves_seen > 1) ok = warp_wait(&o_full[t], (halves_seen - 2) & 1, fail);
+      if (ok && warp_wait(&o_full[t], (halves_seen - 1) & 1, fail)) {
         tc_fence_after();
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
@@ -323,140 +378,153 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
     // ---------------------------------------------- codes to fp16 tiles
     constexpr int kLanes = D / 16;          // lanes of a row, 16 codes each
     constexpr int kRows = 32 / kLanes;      // rows of one load of the warp
-    const int cw = warp - kSoftWarps;
     const int c = lane % kLanes;
-    const int last = (len - 1) >> p.page_shift;
-    const int mask = (1 << p.page_shift) - 1;
-    const int32_t* table = p.table + tile.x * p.width;
-    // pages of the two 16-token groups of this warp's 32 tokens of tile j
-    auto page_of = [&](int j, int half) {
-      const int i = min((j * kN + cw * 32 + half * 16) >> p.page_shift, last);
-      return (int64_t)min(max((int64_t)__ldg(table + i), (int64_t)0), p.pages - 1);
-    };
-    auto load = [&](uint4 (&r)[kLanes], const int8_t* codes, int j, const int64_t (&page)[2]) {
+    const int row0 = (warp - kSoftWarps) * 32 + lane / kLanes;
+    // lanes of the upper half of a row write their second chunk first, so that
+    // eight lanes of a store hit eight different bank groups
+    const int swap = (c >> 2) & 1;
+    auto convert = [&](int side, int j, unsigned char* dst, uint64_t* empty) {
+      const unsigned char* src = sm_raw + side * LY::kRaw + row0 * D + c * 16;
+      unsigned char* at = dst + (c / 4) * LY::kAtom;
+      if (!warp_wait(&raw_full[side], j & 1, fail)) return false;
+      uint4 r[kLanes];
+#pragma unroll
+      for (int i = 0; i < kLanes; ++i)
+        r[i] = *reinterpret_cast<const uint4*>(src + i * kRows * D);
+      if (j >= 2 && !warp_wait(empty, ((j >> 1) - 1) & 1, fail)) return false;
 #pragma unroll
       for (int i = 0; i < kLanes; ++i) {
-        const int in = i * kRows + lane / kLanes;  // row of the warp's 32
-        const int tok = j * kN + cw * 32 + in;
-        const int64_t pg = i * kRows < 16 ? page[0] : page[1];
-        r[i] = make_uint4(0, 0, 0, 0);
-        if (tok < len)
-          r[i] = __ldg(reinterpret_cast<const uint4*>(
-              codes + ((((pg * p.kv_heads + h) << p.page_shift) + (tok & mask)) * D) + c * 16));
-      }
-    };
-    auto convert = [&](unsigned char* dst, const uint4 (&r)[kLanes]) {
-      // lanes of the upper half of a row write their second chunk first, so that
-      // eight lanes of a store hit eight different bank groups
-      const int swap = (c >> 2) & 1;
-#pragma unroll
-      for (int i = 0; i < kLanes; ++i) {
-        const int row = cw * 32 + i * kRows + lane / kLanes;
-        unsigned char* at = dst + (c / 4) * LY::kAtom;
+        const int row = row0 + i * kRows;
         const uint32_t x[4] = {r[i].x ^ 0x80808080u, r[i].y ^ 0x80808080u, r[i].z ^ 0x80808080u,
                                r[i].w ^ 0x80808080u};
-        const uint4 a = make_uint4(halves(x[0], 0x4140), halves(x[0], 0x4342),
-                                   halves(x[1], 0x4140), halves(x[1], 0x4342));
-        const uint4 b = make_uint4(halves(x[2], 0x4140), halves(x[2], 0x4342),
-                                   halves(x[3], 0x4140), halves(x[3], 0x4342));
+        const uint4 lo = make_uint4(halves(x[0], 0x4140), halves(x[0], 0x4342),
+                                    halves(x[1], 0x4140), halves(x[1], 0x4342));
+        const uint4 hi = make_uint4(halves(x[2], 0x4140), halves(x[2], 0x4342),
+                                    halves(x[3], 0x4140), halves(x[3], 0x4342));
         const int ch = (c % 4) * 2;
-        *reinterpret_cast<uint4*>(at + atom_byte(row, ch + swap)) = swap ? b : a;
-        *reinterpret_cast<uint4*>(at + atom_byte(row, ch + 1 - swap)) = swap ? a : b;
+        *reinterpret_cast<uint4*>(at + atom_byte(row, ch + swap)) = swap ? hi : lo;
+        *reinterpret_cast<uint4*>(at + atom_byte(row, ch + 1 - swap)) = swap ? lo : hi;
       }
+      fence_proxy_async_smem();  // the tile for the tensor cores, the codes' place for the next copy
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&raw_empty[side]);
+      return true;
     };
-    // lane g < 8 of the first of these warps: scales of the tile's group g
-    float s_key = 0.0f, s_value = 0.0f;
-    auto load_scales = [&](int j) {
-      if (cw == 0 && lane < 8) {
-        const int i = min((j * kN + lane * 16) >> p.page_shift, last);
-        const int64_t pg = min(max((int64_t)__ldg(table + i), (int64_t)0), p.pages - 1);
-        s_key = __ldg(p.ks + pg * p.kv_heads + h);
-        s_value = __ldg(p.vs + pg * p.kv_heads + h);
-      }
-    };
-    uint4 rk[kLanes], rv[kLanes];
-    int64_t page[2] = {page_of(0, 0), page_of(0, 1)};
-    load(rk, p.k, 0, page);
-    load_scales(0);
-    load(rv, p.v, 0, page);
-    bool ok = true;
     for (int j = 0; j < tiles; ++j) {
       const int st = j & 1;
-      const int64_t next[2] = {page_of(j + 1, 0), page_of(j + 1, 1)};
-      if (j >= 2 && !(ok = warp_wait(&k_empty[st], ((j >> 1) - 1) & 1, fail))) break;
-      convert(sm_k + st * LY::kTile, rk);
-      if (cw == 0) {
-        if (lane < 8) {
-          Scale x{s_key, 0.0f, 0.0f, 0.0f};
-          value_scale(s_value, &x.log2_value, &x.inv_value);
-          sm_scale[(j % kScaleRing) * 8 + lane] = x;
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&scale_full[j % kScaleRing]);
-      }
-      fence_proxy_async_smem();
-      __syncwarp();
+      if (!convert(0, j, sm_k + st * LY::kTile, &k_empty[st])) break;
       if (lane == 0) mbar_arrive(&k_full[st]);
-      if (j + 1 < tiles) {
-        load(rk, p.k, j + 1, next);
-        load_scales(j + 1);
-      }
-      if (j >= 2 && !(ok = warp_wait(&v_empty[st], ((j >> 1) - 1) & 1, fail))) break;
-      convert(sm_v + st * LY::kTile, rv);
-      fence_proxy_async_smem();
-      __syncwarp();
+      if (!convert(1, j, sm_v + st * LY::kTile, &v_empty[st])) break;
       if (lane == 0) mbar_arrive(&v_full[st]);
-      if (j + 1 < tiles) load(rv, p.v, j + 1, next);
     }
-  } else if (lane == 0) {
-    // ------------------------------------------------------------ products
-    auto scores = [&](int t, int st) {
+  } else if (warp < kLoadWarp) {
+    const int t = warp - kMmaWarp;
+    if (lane == 0 && (t == 0 || two)) {
+      // ---------------------------------------------------------- products
+      // Descriptors of the first step; later steps and stages add to the address
+      // field (16-byte units), which no tile of shared memory overflows.
+      constexpr uint32_t kHi = (uint32_t)(((uint64_t)64 << 32 | (uint64_t)1 << 46 |
+                                           (uint64_t)2 << 61) >> 32);
+      constexpr uint32_t kTile16 = LY::kTile / 16, kHalf16 = kHalf * 128 / 16;
+      const uint32_t q_lo = (uint32_t)sw128_desc(sm_q + t * LY::kTile);
+      const uint32_t k_lo = (uint32_t)sw128_desc(sm_k);
+      const uint32_t v_lo = (uint32_t)sw128_mn_desc(sm_v, LY::kAtom);
+      const uint32_t s_at = tmem + LY::kScore + t * kN, o_at = tmem + LY::kResult + t * D;
+      auto scores = [&](int i) {  // half i of the tokens
+        const uint32_t kd = k_lo + ((i >> 1) & 1) * kTile16 + (i & 1) * kHalf16;
 #pragma unroll
-      for (int k = 0; k < D / 16; ++k)
-        umma_f16(tmem + LY::kScore + t * kN,
-                 sw128_desc(sm_q + t * LY::kTile + (k / 4) * LY::kAtom + (k % 4) * 32),
-                 sw128_desc(sm_k + st * LY::kTile + (k / 4) * LY::kAtom + (k % 4) * 32),
-                 idesc(kN, false), k != 0);
-    };
-    auto results = [&](int t, int st, bool first) {
+        for (int k = 0; k < D / 16; ++k) {
+          const uint32_t step = ((k / 4) * LY::kAtom + (k % 4) * 32) / 16;
+          umma_f16_lo(s_at + (i & 1) * kHalf, q_lo + step, kd + step, kHi, kHi,
+                      idesc(kHalf, false), k != 0);
+        }
+        umma_commit(&s_full[t][i & 1]);
+      };
+      auto results = [&](int i) {
+        const uint32_t vd = v_lo + ((i >> 1) & 1) * kTile16 + (i & 1) * kHalf16;
 #pragma unroll
-      for (int k = 0; k < kN / 16; ++k)
-        umma_f16_ts(tmem + LY::kResult + t * D, tmem + LY::kScore + t * kN + 8 * k,
-                    sw128_mn_desc(sm_v + st * LY::kTile + k * 16 * 128, LY::kAtom),
-                    idesc(D, true), !first || k != 0);
-    };
-    const int both = two ? 2 : 1;
-    bool ok = lane_wait(&q_full, 0, fail) && lane_wait(&k_full[0], 0, fail);
-    if (ok) {
-      tc_fence_after();
-      for (int t = 0; t < both; ++t) {
-        scores(t, 0);
-        umma_commit(&s_full[t]);
-      }
-      umma_commit(&k_empty[0]);
-    }
-    for (int j = 0; j < tiles && ok; ++j) {
-      const int st = j & 1;
-      ok = lane_wait(&v_full[st], (j >> 1) & 1, fail);
-      for (int t = 0; t < both && ok; ++t) {
-        if (!(ok = lane_wait(&p_full[t], j & 1, fail))) break;
+        for (int k = 0; k < kHalf / 16; ++k)
+          umma_f16_ts_lo(o_at, s_at + (i & 1) * kHalf + 8 * k, vd + k * (16 * 128 / 16), kHi,
+                         idesc(D, true), i != 0 || k != 0);
+        umma_commit(&o_full[t]);
+      };
+      bool ok = lane_wait(&q_full[t], 0, fail) && lane_wait(&k_full[0], 0, fail);
+      if (ok) {
         tc_fence_after();
-        results(t, st, j == 0);
-        if (t + 1 == both) umma_commit(&v_empty[st]);
-        if (j + 1 < tiles) {
-          if (t == 0 && !(ok = lane_wait(&k_full[st ^ 1], ((j + 1) >> 1) & 1, fail))) break;
-          tc_fence_after();
-          scores(t, st ^ 1);
-          umma_commit(&s_full[t]);
-          if (t + 1 == both) umma_commit(&k_empty[st ^ 1]);
-        } else {
-          umma_commit(&o_done[t]);
+        scores(0);
+        if (halves_seen > 1) scores(1);
+        umma_commit(&k_empty[0]);
+      }
+#pragma unroll 1
+      for (int i = 0; i < halves_seen && ok; ++i) {
+        const int j = i >> 1, hb = i & 1;
+        if (hb == 0) ok = lane_wait(&v_full[j & 1], (j >> 1) & 1, fail);
+        const bool more = i + 2 < halves_seen;  // scores of half i + 2 take this half's place
+        if (ok && more && hb == 0) ok = lane_wait(&k_full[(j + 1) & 1], ((j + 1) >> 1) & 1, fail);
+        ok = ok && lane_wait(&p_full[t][hb], j & 1, fail);
+        if (!ok) break;
+        tc_fence_after();
+        results(i);
+        if (more) scores(i + 2);
+        if (hb == 1) {
+          umma_commit(&v_empty[j & 1]);
+          umma_commit(&k_empty[(j + 1) & 1]);
+        }
+      }
+      // whatever happened, nothing is in flight when tensor memory is given back
+      umma_commit(&drained[t]);
+      mbar_wait(&drained[t], 0, kProbes);
+    }
+  } else {
+    // ------------------------------------- codes and scales from their pages
+    const int last = (len - 1) >> p.page_shift;
+    const int page_tokens = 1 << p.page_shift;
+    const unsigned piece = (unsigned)(min(page_tokens, kN) * D);  // codes of a page in a tile
+    auto page_of = [&](int j) {  // lane g < 8: page of the tile's tokens 16 g ..
+      const int i = min((j * kN + (lane & 7) * 16) >> p.page_shift, last);
+      return min(max(__ldg(p.table + tile.x * p.width + i), 0), (int)p.pages - 1);
+    };
+    int page = page_of(0);
+    int issued[2] = {0, 0};
+    bool ok = true;
+    for (int j = 0; j < tiles && ok; ++j) {
+      const int64_t at = (int64_t)page * p.kv_heads + h;
+      const int t0 = j * kN + (lane & 7) * 16;
+      // a lane at the start of a page's share of the tile copies it; a page is
+      // copied whole, past the request's last token too
+      const bool leads = lane < 8 && t0 <= len - 1 && ((lane * 16) & (page_tokens - 1)) == 0;
+      const unsigned bytes = __popc(__ballot_sync(kFull, leads)) * piece;
+      const int64_t off = ((at << p.page_shift) + (t0 & (page_tokens - 1))) * D;
+      float s_key = 0.0f, s_value = 0.0f;
+      if (lane < 8) {
+        s_key = __ldg(p.ks + at);
+        s_value = __ldg(p.vs + at);
+      }
+      page = page_of(j + 1);
+#pragma unroll
+      for (int side = 0; side < 2; ++side) {
+        if (j >= 1 && !(ok = warp_wait(&raw_empty[side], (j - 1) & 1, fail))) break;
+        issued[side] = j + 1;
+        if (lane == 0) mbar_arrive_expect_tx(&raw_full[side], bytes);
+        __syncwarp();
+        if (leads)
+          bulk_g2s(sm_raw + side * LY::kRaw + lane * 16 * D, (side ? p.v : p.k) + off, piece,
+                   &raw_full[side]);
+        if (side == 0) {
+          if (lane < 8) {
+            Scale x{s_key, 0.0f, 0.0f, 0.0f};
+            value_scale(s_value, &x.log2_value, &x.inv_value);
+            sm_scale[(j % kScaleRing) * 8 + lane] = x;
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&scale_full[j % kScaleRing]);
         }
       }
     }
-    // whatever happened, nothing is in flight when tensor memory is given back
-    umma_commit(&drained);
-    mbar_wait(&drained, 0, kProbes);
+    // no copy is in flight when the block ends, whatever happened
+#pragma unroll
+    for (int side = 0; side < 2; ++side)
+      if (issued[side]) mbar_wait(&raw_full[side], (issued[side] - 1) & 1, kProbes);
   }
 
   __syncwarp();
