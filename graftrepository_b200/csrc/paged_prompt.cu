@@ -46,10 +46,14 @@ constexpr int kSoftWarps = 8;
 constexpr int kConvWarps = 4;
 constexpr int kMmaWarp = kSoftWarps + kConvWarps;
 constexpr int kLoadWarp = kMmaWarp + 2;
-constexpr int kPromptThreads = (kLoadWarp + 1) * 32;
+// Four warpgroups with registers shared out by setmaxnreg: softmax 2 x 184 a
+// thread, codes 88, products and copies 56: the 4 x 128 that the block is
+// launched with.
+constexpr int kPromptThreads = 512;
+constexpr int kPromptRegs = 128;
 constexpr int kScaleRing = 4;       // key tiles whose scales are held
 constexpr uint32_t kTmemCols = 512;
-constexpr unsigned kProbes = 1u << 22;  // probes of a bounded wait
+constexpr unsigned kProbes = 1u << 18;  // probes of a bounded wait
 
 template <int D>
 struct PromptLayout {
@@ -133,7 +137,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
   unsigned char* const sm_raw = sm + 6 * LY::kTile;     // codes: keys, values
   Scale* const sm_scale = reinterpret_cast<Scale*>(sm_raw + 2 * LY::kRaw);  // [kScaleRing][8]
   __shared__ __align__(8) uint64_t q_full[2], drained[2], k_full[2], k_empty[2], v_full[2], v_empty[2],
-      scale_full[kScaleRing], raw_full[2], raw_empty[2], s_full[2][2], p_full[2][2], o_full[2];
+      scale_full[kScaleRing], raw_full[2], raw_empty[2], s_full[2][2], p_full[2][2], o_full[2], o_done[2];
   __shared__ uint32_t sh_tmem;
   __shared__ int sh_fail;
 
@@ -183,6 +187,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
         mbar_init(&p_full[i][x], kSoftWarps / 2);
       }
       mbar_init(&o_full[i], 1);
+      mbar_init(&o_done[i], 1);
     }
     for (int i = 0; i < kScaleRing; ++i) mbar_init(&scale_full[i], 1);
     mbar_fence_init();
@@ -199,6 +204,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
   volatile int* const fail = &sh_fail;
 
   if (warp < kSoftWarps) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
     // ------------------------------------------------------------- softmax
     const int t = warp >> 2;
     if (t == 0 || two) {
@@ -249,39 +255,43 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
       const uint32_t s_col = tmem + lanes + LY::kScore + t * kN;
       const uint32_t o_col = tmem + lanes + LY::kResult + t * D;
       float m = -INFINITY, l = 0.0f;
-      bool ok = true;
-#pragma unroll 1
-      for (int i = 0; i < halves_seen; ++i) {
-        const int j = i >> 1, hb = i & 1;
-        if ((hb == 0 && !warp_wait(&scale_full[j % kScaleRing], (j / kScaleRing) & 1, fail)) ||
-            !warp_wait(&s_full[t][hb], j & 1, fail)) {
-          ok = false;
-          break;
+      // Factors and offsets of the exponents of the 4 x 16 tokens of half i.
+      // Hidden from the row altogether they have 1 and 0, so that a page without
+      // a number does not reach it; a factor too small for fp32 stays above 0.
+      struct Factors {
+        float k[4], lu[4];
+      };
+      auto factors = [&](int i, Factors& f) {
+        const Scale* sc = sm_scale + ((i >> 1) % kScaleRing) * 8 + (i & 1) * 4;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const bool hidden = i * kHalf + 16 * g >= lim;
+          const float k = kq * sc[g].key;
+          f.k[g] = hidden ? 1.0f : k == 0.0f ? 0x1p-126f : k;
+          f.lu[g] = hidden ? 0.0f : sc[g].log2_value;
         }
+      };
+      // The scores of half i are there: start loading them.
+      auto fetch = [&](int i, uint32_t (&v)[2][32], Factors& f) {
+        const int j = i >> 1, hb = i & 1;
+        if (hb == 0 && !warp_wait(&scale_full[j % kScaleRing], (j / kScaleRing) & 1, fail))
+          return false;
+        factors(i, f);
+        if (!warp_wait(&s_full[t][hb], j & 1, fail)) return false;
         tc_fence_after();
-        const Scale* sc = sm_scale + (j % kScaleRing) * 8 + hb * 4;
-        const int t0 = i * kHalf;
-        // Factor and offset of the exponents of 16 tokens.  Hidden from the row
-        // altogether they have 1 and 0, so that a page without a number does not
-        // reach it; a factor too small for fp32 stays above 0.
-        auto factors = [&](int g, float* k, float* lu) {
-          const bool hidden = t0 + 16 * g >= lim;
-          *k = kq * sc[g].key;
-          if (*k == 0.0f) *k = 0x1p-126f;
-          if (hidden) *k = 1.0f;
-          *lu = hidden ? 0.0f : sc[g].log2_value;
-        };
-        // the row's 64 scores, in registers from here on
-        uint32_t v[2][32];
         tmem_ld32_nowait(s_col + hb * kHalf, v[0]);
         tmem_ld32_nowait(s_col + hb * kHalf + 32, v[1]);
         tmem_wait_ld32(v[0]);
         tmem_wait_ld32(v[1]);
-        // hidden tokens: scores of -inf (no factor is 0)
-        if (__any_sync(kFull, t0 + kHalf > lim)) {
+        return true;
+      };
+      // The largest exponent of half i; hidden tokens get scores of -inf (no
+      // factor is 0).
+      auto largest = [&](int i, uint32_t (&v)[2][32], const Factors& f) {
+        if (__any_sync(kFull, (i + 1) * kHalf > lim)) {
 #pragma unroll
           for (int x = 0; x < kHalf; ++x)
-            if (t0 + x >= lim) v[x / 32][x % 32] = 0xFF800000u;
+            if (i * kHalf + x >= lim) v[x / 32][x % 32] = 0xFF800000u;
         }
         float top = -INFINITY;
 #pragma unroll
@@ -292,20 +302,48 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
                                max3(x[9], x[10], x[11]),
                                max3(max3(x[12], x[13], x[14]), __uint_as_float(x[15]),
                                     -INFINITY));
-          float k, lu;
-          factors(g, &k, &lu);
-          top = fmaxf(top, fmaf(y, k, lu));
+          top = fmaxf(top, fmaf(y, f.k[g], f.lu[g]));
         }
+        return top;
+      };
+      // 32 tokens' p, packed, to tensor memory; their share of the sum
+      auto weigh = [&](int i, int c, const uint32_t (&v)[2][32], const Factors& f, float ref) {
+        const Scale* sc = sm_scale + ((i >> 1) % kScaleRing) * 8 + (i & 1) * 4;
+        uint32_t w[16];
+#pragma unroll
+        for (int h2 = 0; h2 < 2; ++h2) {
+          const int g = 2 * c + h2;
+          const float2 k = make_float2(f.k[g], f.k[g]);
+          const float2 off = make_float2(f.lu[g] - ref, f.lu[g] - ref);
+          float2 sum = make_float2(0.0f, 0.0f);
+#pragma unroll
+          for (int x = 0; x < 16; x += 2) {
+            const float2 y = fma2(make_float2(__uint_as_float(v[c][16 * h2 + x]),
+                                              __uint_as_float(v[c][16 * h2 + x + 1])),
+                                  k, off);
+            const float2 pr = make_float2(ex2(y.x), ex2(y.y));
+            sum = add2(sum, pr);
+            w[8 * h2 + x / 2] = pack_half2(pr.x, pr.y);
+          }
+          // a page without a number counts only where it is seen
+          const float total = sum.x + sum.y;
+          l += total == 0.0f ? 0.0f : total * sc[g].inv_value;
+        }
+        tmem_st16(s_col + (i & 1) * kHalf + 16 * c, w);
+      };
+      // Half i, loaded in v with its largest exponent `top`: weights out, and the
+      // next half's scores in, with their largest exponent found under this
+      // half's exponentials.
+      float top = -INFINITY;
+      auto step = [&](int i, uint32_t (&v)[2][32], Factors& f, uint32_t (&nv)[2][32],
+                      Factors& nf) {
         if (__any_sync(kFull, top > m + kLazy)) {
           const float next = top > m + kLazy ? top : m;
           const float a = next == m ? 1.0f : ex2(m - next);
           m = next;
           l *= a;
           if (i > 0) {  // once the products of the half before have ended
-            if (!warp_wait(&o_full[t], (i - 1) & 1, fail)) {
-              ok = false;
-              break;
-            }
+            if (!warp_wait(&o_full[t], (i - 1) & 1, fail)) return false;
             tc_fence_after();
 #pragma unroll 1
             for (int c = 0; c < D / 16; ++c) {
@@ -318,38 +356,27 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
           }
         }
         const float ref = m == -INFINITY ? 0.0f : m;
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t w[16];
-#pragma unroll
-          for (int h2 = 0; h2 < 2; ++h2) {
-            float k1, lu;
-            factors(2 * c + h2, &k1, &lu);
-            const float2 k = make_float2(k1, k1), off = make_float2(lu - ref, lu - ref);
-            float2 sum = make_float2(0.0f, 0.0f);
-#pragma unroll
-            for (int x = 0; x < 16; x += 2) {
-              const float2 y = fma2(make_float2(__uint_as_float(v[c][16 * h2 + x]),
-                                                __uint_as_float(v[c][16 * h2 + x + 1])),
-                                    k, off);
-              const float2 pr = make_float2(ex2(y.x), ex2(y.y));
-              sum = add2(sum, pr);
-              w[8 * h2 + x / 2] = pack_half2(pr.x, pr.y);
-            }
-            // a page without a number counts only where it is seen
-            const float total = sum.x + sum.y;
-            l += total == 0.0f ? 0.0f : total * sc[2 * c + h2].inv_value;
-          }
-          tmem_st16(s_col + hb * kHalf + 16 * c, w);
-        }
+        const bool more = i + 1 < halves_seen;
+        if (more && !fetch(i + 1, nv, nf)) return false;
+        weigh(i, 0, v, f, ref);
+        if (more) top = largest(i + 1, nv, nf);
+        weigh(i, 1, v, f, ref);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[t][hb]);
+        if (lane == 0) mbar_arrive(&p_full[t][i & 1]);
+        return true;
+      };
+      uint32_t va[2][32], vb[2][32];
+      Factors fa, fb;
+      bool ok = fetch(0, va, fa);
+      if (ok) top = largest(0, va, fa);
+#pragma unroll 1
+      for (int i = 0; i < halves_seen && ok; i += 2) {
+        ok = step(i, va, fa, vb, fb);
+        if (ok && i + 1 < halves_seen) ok = step(i + 1, vb, fb, va, fa);
       }
-      // the last two products: a barrier is waited for phase by phase
-      if (ok && halves_seen > 1) ok = warp_wait(&o_full[t], (halves_seen - 2) & 1, fail);
-      if (ok && warp_wait(&o_full[t], (halves_seen - 1) & 1, fail)) {
+      if (ok && warp_wait(&o_done[t], 0, fail)) {
         tc_fence_after();
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
@@ -375,6 +402,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
       }
     }
   } else if (warp < kMmaWarp) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     // ---------------------------------------------- codes to fp16 tiles
     constexpr int kLanes = D / 16;          // lanes of a row, 16 codes each
     constexpr int kRows = 32 / kLanes;      // rows of one load of the warp
@@ -417,114 +445,118 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
       if (!convert(1, j, sm_v + st * LY::kTile, &v_empty[st])) break;
       if (lane == 0) mbar_arrive(&v_full[st]);
     }
-  } else if (warp < kLoadWarp) {
-    const int t = warp - kMmaWarp;
-    if (lane == 0 && (t == 0 || two)) {
-      // ---------------------------------------------------------- products
-      // Descriptors of the first step; later steps and stages add to the address
-      // field (16-byte units), which no tile of shared memory overflows.
-      constexpr uint32_t kHi = (uint32_t)(((uint64_t)64 << 32 | (uint64_t)1 << 46 |
-                                           (uint64_t)2 << 61) >> 32);
-      constexpr uint32_t kTile16 = LY::kTile / 16, kHalf16 = kHalf * 128 / 16;
-      const uint32_t q_lo = (uint32_t)sw128_desc(sm_q + t * LY::kTile);
-      const uint32_t k_lo = (uint32_t)sw128_desc(sm_k);
-      const uint32_t v_lo = (uint32_t)sw128_mn_desc(sm_v, LY::kAtom);
-      const uint32_t s_at = tmem + LY::kScore + t * kN, o_at = tmem + LY::kResult + t * D;
-      auto scores = [&](int i) {  // half i of the tokens
-        const uint32_t kd = k_lo + ((i >> 1) & 1) * kTile16 + (i & 1) * kHalf16;
-#pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          const uint32_t step = ((k / 4) * LY::kAtom + (k % 4) * 32) / 16;
-          umma_f16_lo(s_at + (i & 1) * kHalf, q_lo + step, kd + step, kHi, kHi,
-                      idesc(kHalf, false), k != 0);
-        }
-        umma_commit(&s_full[t][i & 1]);
-      };
-      auto results = [&](int i) {
-        const uint32_t vd = v_lo + ((i >> 1) & 1) * kTile16 + (i & 1) * kHalf16;
-#pragma unroll
-        for (int k = 0; k < kHalf / 16; ++k)
-          umma_f16_ts_lo(o_at, s_at + (i & 1) * kHalf + 8 * k, vd + k * (16 * 128 / 16), kHi,
-                         idesc(D, true), i != 0 || k != 0);
-        umma_commit(&o_full[t]);
-      };
-      bool ok = lane_wait(&q_full[t], 0, fail) && lane_wait(&k_full[0], 0, fail);
-      if (ok) {
-        tc_fence_after();
-        scores(0);
-        if (halves_seen > 1) scores(1);
-        umma_commit(&k_empty[0]);
-      }
-#pragma unroll 1
-      for (int i = 0; i < halves_seen && ok; ++i) {
-        const int j = i >> 1, hb = i & 1;
-        if (hb == 0) ok = lane_wait(&v_full[j & 1], (j >> 1) & 1, fail);
-        const bool more = i + 2 < halves_seen;  // scores of half i + 2 take this half's place
-        if (ok && more && hb == 0) ok = lane_wait(&k_full[(j + 1) & 1], ((j + 1) >> 1) & 1, fail);
-        ok = ok && lane_wait(&p_full[t][hb], j & 1, fail);
-        if (!ok) break;
-        tc_fence_after();
-        results(i);
-        if (more) scores(i + 2);
-        if (hb == 1) {
-          umma_commit(&v_empty[j & 1]);
-          umma_commit(&k_empty[(j + 1) & 1]);
-        }
-      }
-      // whatever happened, nothing is in flight when tensor memory is given back
-      umma_commit(&drained[t]);
-      mbar_wait(&drained[t], 0, kProbes);
-    }
   } else {
-    // ------------------------------------- codes and scales from their pages
-    const int last = (len - 1) >> p.page_shift;
-    const int page_tokens = 1 << p.page_shift;
-    const unsigned piece = (unsigned)(min(page_tokens, kN) * D);  // codes of a page in a tile
-    auto page_of = [&](int j) {  // lane g < 8: page of the tile's tokens 16 g ..
-      const int i = min((j * kN + (lane & 7) * 16) >> p.page_shift, last);
-      return min(max(__ldg(p.table + tile.x * p.width + i), 0), (int)p.pages - 1);
-    };
-    int page = page_of(0);
-    int issued[2] = {0, 0};
-    bool ok = true;
-    for (int j = 0; j < tiles && ok; ++j) {
-      const int64_t at = (int64_t)page * p.kv_heads + h;
-      const int t0 = j * kN + (lane & 7) * 16;
-      // a lane at the start of a page's share of the tile copies it; a page is
-      // copied whole, past the request's last token too
-      const bool leads = lane < 8 && t0 <= len - 1 && ((lane * 16) & (page_tokens - 1)) == 0;
-      const unsigned bytes = __popc(__ballot_sync(kFull, leads)) * piece;
-      const int64_t off = ((at << p.page_shift) + (t0 & (page_tokens - 1))) * D;
-      float s_key = 0.0f, s_value = 0.0f;
-      if (lane < 8) {
-        s_key = __ldg(p.ks + at);
-        s_value = __ldg(p.vs + at);
-      }
-      page = page_of(j + 1);
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp < kLoadWarp) {
+      const int t = warp - kMmaWarp;
+      if (lane == 0 && (t == 0 || two)) {
+        // ---------------------------------------------------------- products
+        // Descriptors of the first step; later steps and stages add to the address
+        // field (16-byte units), which no tile of shared memory overflows.
+        constexpr uint32_t kHi = (uint32_t)(((uint64_t)64 << 32 | (uint64_t)1 << 46 |
+                                             (uint64_t)2 << 61) >> 32);
+        constexpr uint32_t kTile16 = LY::kTile / 16, kHalf16 = kHalf * 128 / 16;
+        const uint32_t q_lo = (uint32_t)sw128_desc(sm_q + t * LY::kTile);
+        const uint32_t k_lo = (uint32_t)sw128_desc(sm_k);
+        const uint32_t v_lo = (uint32_t)sw128_mn_desc(sm_v, LY::kAtom);
+        const uint32_t s_at = tmem + LY::kScore + t * kN, o_at = tmem + LY::kResult + t * D;
+        auto scores = [&](int i) {  // half i of the tokens
+          const uint32_t kd = k_lo + ((i >> 1) & 1) * kTile16 + (i & 1) * kHalf16;
 #pragma unroll
-      for (int side = 0; side < 2; ++side) {
-        if (j >= 1 && !(ok = warp_wait(&raw_empty[side], (j - 1) & 1, fail))) break;
-        issued[side] = j + 1;
-        if (lane == 0) mbar_arrive_expect_tx(&raw_full[side], bytes);
-        __syncwarp();
-        if (leads)
-          bulk_g2s(sm_raw + side * LY::kRaw + lane * 16 * D, (side ? p.v : p.k) + off, piece,
-                   &raw_full[side]);
-        if (side == 0) {
-          if (lane < 8) {
-            Scale x{s_key, 0.0f, 0.0f, 0.0f};
-            value_scale(s_value, &x.log2_value, &x.inv_value);
-            sm_scale[(j % kScaleRing) * 8 + lane] = x;
+          for (int k = 0; k < D / 16; ++k) {
+            const uint32_t step = ((k / 4) * LY::kAtom + (k % 4) * 32) / 16;
+            umma_f16_lo(s_at + (i & 1) * kHalf, q_lo + step, kd + step, kHi, kHi,
+                        idesc(kHalf, false), k != 0);
           }
+          umma_commit(&s_full[t][i & 1]);
+        };
+        auto results = [&](int i) {
+          const uint32_t vd = v_lo + ((i >> 1) & 1) * kTile16 + (i & 1) * kHalf16;
+#pragma unroll
+          for (int k = 0; k < kHalf / 16; ++k)
+            umma_f16_ts_lo(o_at, s_at + (i & 1) * kHalf + 8 * k, vd + k * (16 * 128 / 16), kHi,
+                           idesc(D, true), i != 0 || k != 0);
+          umma_commit(&o_full[t]);
+        };
+        bool ok = lane_wait(&q_full[t], 0, fail) && lane_wait(&k_full[0], 0, fail);
+        if (ok) {
+          tc_fence_after();
+          scores(0);
+          if (halves_seen > 1) scores(1);
+          umma_commit(&k_empty[0]);
+        }
+#pragma unroll 1
+        for (int i = 0; i < halves_seen && ok; ++i) {
+          const int j = i >> 1, hb = i & 1;
+          if (hb == 0) ok = lane_wait(&v_full[j & 1], (j >> 1) & 1, fail);
+          const bool more = i + 2 < halves_seen;  // scores of half i + 2 take this half's place
+          if (ok && more && hb == 0) ok = lane_wait(&k_full[(j + 1) & 1], ((j + 1) >> 1) & 1, fail);
+          ok = ok && lane_wait(&p_full[t][hb], j & 1, fail);
+          if (!ok) break;
+          tc_fence_after();
+          results(i);
+          if (more) scores(i + 2);
+          if (i + 1 == halves_seen) umma_commit(&o_done[t]);
+          if (hb == 1) {
+            umma_commit(&v_empty[j & 1]);
+            umma_commit(&k_empty[(j + 1) & 1]);
+          }
+        }
+        // whatever happened, nothing is in flight when tensor memory is given back
+        umma_commit(&drained[t]);
+        mbar_wait(&drained[t], 0, kProbes);
+      }
+    } else if (warp == kLoadWarp) {
+      // ------------------------------------- codes and scales from their pages
+      const int last = (len - 1) >> p.page_shift;
+      const int page_tokens = 1 << p.page_shift;
+      const unsigned piece = (unsigned)(min(page_tokens, kN) * D);  // codes of a page in a tile
+      auto page_of = [&](int j) {  // lane g < 8: page of the tile's tokens 16 g ..
+        const int i = min((j * kN + (lane & 7) * 16) >> p.page_shift, last);
+        return min(max(__ldg(p.table + tile.x * p.width + i), 0), (int)p.pages - 1);
+      };
+      int page = page_of(0);
+      int issued[2] = {0, 0};
+      bool ok = true;
+      for (int j = 0; j < tiles && ok; ++j) {
+        const int64_t at = (int64_t)page * p.kv_heads + h;
+        const int t0 = j * kN + (lane & 7) * 16;
+        // a lane at the start of a page's share of the tile copies it; a page is
+        // copied whole, past the request's last token too
+        const bool leads = lane < 8 && t0 <= len - 1 && ((lane * 16) & (page_tokens - 1)) == 0;
+        const unsigned bytes = __popc(__ballot_sync(kFull, leads)) * piece;
+        const int64_t off = ((at << p.page_shift) + (t0 & (page_tokens - 1))) * D;
+        float s_key = 0.0f, s_value = 0.0f;
+        if (lane < 8) {
+          s_key = __ldg(p.ks + at);
+          s_value = __ldg(p.vs + at);
+        }
+        page = page_of(j + 1);
+#pragma unroll
+        for (int side = 0; side < 2; ++side) {
+          if (j >= 1 && !(ok = warp_wait(&raw_empty[side], (j - 1) & 1, fail))) break;
+          issued[side] = j + 1;
+          if (lane == 0) mbar_arrive_expect_tx(&raw_full[side], bytes);
           __syncwarp();
-          if (lane == 0) mbar_arrive(&scale_full[j % kScaleRing]);
+          if (leads)
+            bulk_g2s(sm_raw + side * LY::kRaw + lane * 16 * D, (side ? p.v : p.k) + off, piece,
+                     &raw_full[side]);
+          if (side == 0) {
+            if (lane < 8) {
+              Scale x{s_key, 0.0f, 0.0f, 0.0f};
+              value_scale(s_value, &x.log2_value, &x.inv_value);
+              sm_scale[(j % kScaleRing) * 8 + lane] = x;
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&scale_full[j % kScaleRing]);
+          }
         }
       }
-    }
-    // no copy is in flight when the block ends, whatever happened
+      // no copy is in flight when the block ends, whatever happened
 #pragma unroll
-    for (int side = 0; side < 2; ++side)
-      if (issued[side]) mbar_wait(&raw_full[side], (issued[side] - 1) & 1, kProbes);
+      for (int side = 0; side < 2; ++side)
+        if (issued[side]) mbar_wait(&raw_full[side], (issued[side] - 1) & 1, kProbes);
+    }
   }
 
   __syncwarp();
@@ -538,8 +570,16 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
 template <typename T, int D>
 int launch(const AttendParams& p, int64_t blocks, cudaStream_t st) {
   auto kernel = prompt_kernel<T, D>;
-  const cudaError_t e = cudaFuncSetAttribute(
-      kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PromptLayout<D>::kSmem);
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       PromptLayout<D>::kSmem);
+  cudaFuncAttributes attr{};
+  if (e == cudaSuccess) e = cudaFuncGetAttributes(&attr, kernel);
+  if (e == cudaSuccess && attr.numRegs != kPromptRegs) {
+    // the shares of setmaxnreg would not add up, and a group would wait for good
+    set_thread_error("paged attend: built with %d registers a thread, not %d", attr.numRegs,
+                     kPromptRegs);
+    return GRM_B200_EINVAL;
+  }
   if (e != cudaSuccess) {
     set_thread_error("paged attend: %s", cudaGetErrorString(e));
     return cuda_status(e);
