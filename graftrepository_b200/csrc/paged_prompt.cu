@@ -46,11 +46,7 @@ constexpr int kSoftWarps = 8;
 constexpr int kConvWarps = 4;
 constexpr int kMmaWarp = kSoftWarps + kConvWarps;
 constexpr int kLoadWarp = kMmaWarp + 2;
-// Four warpgroups with registers shared out by setmaxnreg: softmax 2 x 184 a
-// thread, codes 88, products and copies 56: the 4 x 128 that the block is
-// launched with.
-constexpr int kPromptThreads = 512;
-constexpr int kPromptRegs = 128;
+constexpr int kPromptThreads = (kLoadWarp + 1) * 32;
 constexpr int kScaleRing = 4;       // key tiles whose scales are held
 constexpr uint32_t kTmemCols = 512;
 constexpr unsigned kProbes = 1u << 18;  // probes of a bounded wait
@@ -103,7 +99,9 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
 }
 
 // Every lane of a warp waits; false, for all of them, when a wait gave up.
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, unsigned parity, volatile int* fail) {
+// The loops of this kernel share an instruction cache that they barely fit, so
+// what is not the common path stays out of line.
+__device__ __noinline__ bool wait_long(uint64_t* bar, unsigned parity, volatile int* fail) {
   bool ok = false;
   for (unsigned i = 0; i < kProbes; ++i) {
     if ((ok = mbar_try_wait(bar, parity))) break;
@@ -113,13 +111,9 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, unsigned parity, volati
   if (!ok) *fail = 1;
   return ok;
 }
-__device__ __forceinline__ bool lane_wait(uint64_t* bar, unsigned parity, volatile int* fail) {
-  for (unsigned i = 0; i < kProbes; ++i) {
-    if (mbar_try_wait(bar, parity)) return true;
-    if (*fail) return false;
-  }
-  *fail = 1;
-  return false;
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, unsigned parity, volatile int* fail) {
+  if (__all_sync(kFull, mbar_try_wait(bar, parity))) return true;
+  return wait_long(bar, parity, fail);
 }
 
 struct Scale {
@@ -204,7 +198,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
   volatile int* const fail = &sh_fail;
 
   if (warp < kSoftWarps) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
     // ------------------------------------------------------------- softmax
     const int t = warp >> 2;
     if (t == 0 || two) {
@@ -255,39 +248,33 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
       const uint32_t s_col = tmem + lanes + LY::kScore + t * kN;
       const uint32_t o_col = tmem + lanes + LY::kResult + t * D;
       float m = -INFINITY, l = 0.0f;
-      // Factors and offsets of the exponents of the 4 x 16 tokens of half i.
-      // Hidden from the row altogether they have 1 and 0, so that a page without
-      // a number does not reach it; a factor too small for fp32 stays above 0.
-      struct Factors {
-        float k[4], lu[4];
-      };
-      auto factors = [&](int i, Factors& f) {
-        const Scale* sc = sm_scale + ((i >> 1) % kScaleRing) * 8 + (i & 1) * 4;
+      bool ok = true;
+#pragma unroll 1
+      for (int i = 0; i < halves_seen; ++i) {
+        const int j = i >> 1, hb = i & 1;
+        if (hb == 0 && !(ok = warp_wait(&scale_full[j % kScaleRing], (j / kScaleRing) & 1, fail)))
+          break;
+        // Factors and offsets of the exponents of 4 x 16 tokens.  Hidden from the
+        // row altogether they have 1 and 0, so that a page without a number does
+        // not reach it; a factor too small for fp32 stays above 0.
+        const Scale* sc = sm_scale + (j % kScaleRing) * 8 + hb * 4;
+        float fk[4], fo[4];
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           const bool hidden = i * kHalf + 16 * g >= lim;
           const float k = kq * sc[g].key;
-          f.k[g] = hidden ? 1.0f : k == 0.0f ? 0x1p-126f : k;
-          f.lu[g] = hidden ? 0.0f : sc[g].log2_value;
+          fk[g] = hidden ? 1.0f : k == 0.0f ? 0x1p-126f : k;
+          fo[g] = hidden ? 0.0f : sc[g].log2_value;
         }
-      };
-      // The scores of half i are there: start loading them.
-      auto fetch = [&](int i, uint32_t (&v)[2][32], Factors& f) {
-        const int j = i >> 1, hb = i & 1;
-        if (hb == 0 && !warp_wait(&scale_full[j % kScaleRing], (j / kScaleRing) & 1, fail))
-          return false;
-        factors(i, f);
-        if (!warp_wait(&s_full[t][hb], j & 1, fail)) return false;
+        if (!(ok = warp_wait(&s_full[t][hb], j & 1, fail))) break;
         tc_fence_after();
+        // the row's 64 scores, in registers from here on
+        uint32_t v[2][32];
         tmem_ld32_nowait(s_col + hb * kHalf, v[0]);
         tmem_ld32_nowait(s_col + hb * kHalf + 32, v[1]);
         tmem_wait_ld32(v[0]);
         tmem_wait_ld32(v[1]);
-        return true;
-      };
-      // The largest exponent of half i; hidden tokens get scores of -inf (no
-      // factor is 0).
-      auto largest = [&](int i, uint32_t (&v)[2][32], const Factors& f) {
+        // hidden tokens: scores of -inf (no factor is 0)
         if (__any_sync(kFull, (i + 1) * kHalf > lim)) {
 #pragma unroll
           for (int x = 0; x < kHalf; ++x)
@@ -302,48 +289,15 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
                                max3(x[9], x[10], x[11]),
                                max3(max3(x[12], x[13], x[14]), __uint_as_float(x[15]),
                                     -INFINITY));
-          top = fmaxf(top, fmaf(y, f.k[g], f.lu[g]));
+          top = fmaxf(top, fmaf(y, fk[g], fo[g]));
         }
-        return top;
-      };
-      // 32 tokens' p, packed, to tensor memory; their share of the sum
-      auto weigh = [&](int i, int c, const uint32_t (&v)[2][32], const Factors& f, float ref) {
-        const Scale* sc = sm_scale + ((i >> 1) % kScaleRing) * 8 + (i & 1) * 4;
-        uint32_t w[16];
-#pragma unroll
-        for (int h2 = 0; h2 < 2; ++h2) {
-          const int g = 2 * c + h2;
-          const float2 k = make_float2(f.k[g], f.k[g]);
-          const float2 off = make_float2(f.lu[g] - ref, f.lu[g] - ref);
-          float2 sum = make_float2(0.0f, 0.0f);
-#pragma unroll
-          for (int x = 0; x < 16; x += 2) {
-            const float2 y = fma2(make_float2(__uint_as_float(v[c][16 * h2 + x]),
-                                              __uint_as_float(v[c][16 * h2 + x + 1])),
-                                  k, off);
-            const float2 pr = make_float2(ex2(y.x), ex2(y.y));
-            sum = add2(sum, pr);
-            w[8 * h2 + x / 2] = pack_half2(pr.x, pr.y);
-          }
-          // a page without a number counts only where it is seen
-          const float total = sum.x + sum.y;
-          l += total == 0.0f ? 0.0f : total * sc[g].inv_value;
-        }
-        tmem_st16(s_col + (i & 1) * kHalf + 16 * c, w);
-      };
-      // Half i, loaded in v with its largest exponent `top`: weights out, and the
-      // next half's scores in, with their largest exponent found under this
-      // half's exponentials.
-      float top = -INFINITY;
-      auto step = [&](int i, uint32_t (&v)[2][32], Factors& f, uint32_t (&nv)[2][32],
-                      Factors& nf) {
         if (__any_sync(kFull, top > m + kLazy)) {
           const float next = top > m + kLazy ? top : m;
           const float a = next == m ? 1.0f : ex2(m - next);
           m = next;
           l *= a;
           if (i > 0) {  // once the products of the half before have ended
-            if (!warp_wait(&o_full[t], (i - 1) & 1, fail)) return false;
+            if (!(ok = warp_wait(&o_full[t], (i - 1) & 1, fail))) break;
             tc_fence_after();
 #pragma unroll 1
             for (int c = 0; c < D / 16; ++c) {
@@ -356,25 +310,34 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
           }
         }
         const float ref = m == -INFINITY ? 0.0f : m;
-        const bool more = i + 1 < halves_seen;
-        if (more && !fetch(i + 1, nv, nf)) return false;
-        weigh(i, 0, v, f, ref);
-        if (more) top = largest(i + 1, nv, nf);
-        weigh(i, 1, v, f, ref);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t w[16];
+#pragma unroll
+          for (int h2 = 0; h2 < 2; ++h2) {
+            const int g = 2 * c + h2;
+            const float2 k = make_float2(fk[g], fk[g]);
+            const float2 off = make_float2(fo[g] - ref, fo[g] - ref);
+            float2 sum = make_float2(0.0f, 0.0f);
+#pragma unroll
+            for (int x = 0; x < 16; x += 2) {
+              const float2 y = fma2(make_float2(__uint_as_float(v[c][16 * h2 + x]),
+                                                __uint_as_float(v[c][16 * h2 + x + 1])),
+                                    k, off);
+              const float2 pr = make_float2(ex2(y.x), ex2(y.y));
+              sum = add2(sum, pr);
+              w[8 * h2 + x / 2] = pack_half2(pr.x, pr.y);
+            }
+            // a page without a number counts only where it is seen
+            const float total = sum.x + sum.y;
+            l += total == 0.0f ? 0.0f : total * sc[g].inv_value;
+          }
+          tmem_st16(s_col + hb * kHalf + 16 * c, w);
+        }
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[t][i & 1]);
-        return true;
-      };
-      uint32_t va[2][32], vb[2][32];
-      Factors fa, fb;
-      bool ok = fetch(0, va, fa);
-      if (ok) top = largest(0, va, fa);
-#pragma unroll 1
-      for (int i = 0; i < halves_seen && ok; i += 2) {
-        ok = step(i, va, fa, vb, fb);
-        if (ok && i + 1 < halves_seen) ok = step(i + 1, vb, fb, va, fa);
+        if (lane == 0) mbar_arrive(&p_full[t][hb]);
       }
       if (ok && warp_wait(&o_done[t], 0, fail)) {
         tc_fence_after();
@@ -402,7 +365,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
       }
     }
   } else if (warp < kMmaWarp) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     // ---------------------------------------------- codes to fp16 tiles
     constexpr int kLanes = D / 16;          // lanes of a row, 16 codes each
     constexpr int kRows = 32 / kLanes;      // rows of one load of the warp
@@ -411,99 +373,108 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
     // lanes of the upper half of a row write their second chunk first, so that
     // eight lanes of a store hit eight different bank groups
     const int swap = (c >> 2) & 1;
-    auto convert = [&](int side, int j, unsigned char* dst, uint64_t* empty) {
+    bool ok = true;
+#pragma unroll 1
+    for (int x = 0; x < 2 * tiles; ++x) {  // keys, values, keys, ...
+      const int j = x >> 1, side = x & 1, st = j & 1;
       const unsigned char* src = sm_raw + side * LY::kRaw + row0 * D + c * 16;
-      unsigned char* at = dst + (c / 4) * LY::kAtom;
-      if (!warp_wait(&raw_full[side], j & 1, fail)) return false;
-      uint4 r[kLanes];
+      unsigned char* at = (side ? sm_v : sm_k) + st * LY::kTile + (c / 4) * LY::kAtom;
+      if (!(ok = warp_wait(&raw_full[side], j & 1, fail))) break;
+      if (j >= 2 &&
+          !(ok = warp_wait(side ? &v_empty[st] : &k_empty[st], ((j >> 1) - 1) & 1, fail)))
+        break;
+#pragma unroll 1
+      for (int i0 = 0; i0 < kLanes; i0 += 4) {
+        uint4 r[4];
 #pragma unroll
-      for (int i = 0; i < kLanes; ++i)
-        r[i] = *reinterpret_cast<const uint4*>(src + i * kRows * D);
-      if (j >= 2 && !warp_wait(empty, ((j >> 1) - 1) & 1, fail)) return false;
+        for (int i = 0; i < 4; ++i)
+          r[i] = *reinterpret_cast<const uint4*>(src + (i0 + i) * kRows * D);
 #pragma unroll
-      for (int i = 0; i < kLanes; ++i) {
-        const int row = row0 + i * kRows;
-        const uint32_t x[4] = {r[i].x ^ 0x80808080u, r[i].y ^ 0x80808080u, r[i].z ^ 0x80808080u,
-                               r[i].w ^ 0x80808080u};
-        const uint4 lo = make_uint4(halves(x[0], 0x4140), halves(x[0], 0x4342),
-                                    halves(x[1], 0x4140), halves(x[1], 0x4342));
-        const uint4 hi = make_uint4(halves(x[2], 0x4140), halves(x[2], 0x4342),
-                                    halves(x[3], 0x4140), halves(x[3], 0x4342));
-        const int ch = (c % 4) * 2;
-        *reinterpret_cast<uint4*>(at + atom_byte(row, ch + swap)) = swap ? hi : lo;
-        *reinterpret_cast<uint4*>(at + atom_byte(row, ch + 1 - swap)) = swap ? lo : hi;
+        for (int i = 0; i < 4; ++i) {
+          const int row = row0 + (i0 + i) * kRows;
+          const uint32_t x[4] = {r[i].x ^ 0x80808080u, r[i].y ^ 0x80808080u,
+                                 r[i].z ^ 0x80808080u, r[i].w ^ 0x80808080u};
+          const uint4 lo = make_uint4(halves(x[0], 0x4140), halves(x[0], 0x4342),
+                                      halves(x[1], 0x4140), halves(x[1], 0x4342));
+          const uint4 hi = make_uint4(halves(x[2], 0x4140), halves(x[2], 0x4342),
+                                      halves(x[3], 0x4140), halves(x[3], 0x4342));
+          const int ch = (c % 4) * 2;
+          *reinterpret_cast<uint4*>(at + atom_byte(row, ch + swap)) = swap ? hi : lo;
+          *reinterpret_cast<uint4*>(at + atom_byte(row, ch + 1 - swap)) = swap ? lo : hi;
+        }
       }
       fence_proxy_async_smem();  // the tile for the tensor cores, the codes' place for the next copy
       __syncwarp();
-      if (lane == 0) mbar_arrive(&raw_empty[side]);
-      return true;
-    };
-    for (int j = 0; j < tiles; ++j) {
-      const int st = j & 1;
-      if (!convert(0, j, sm_k + st * LY::kTile, &k_empty[st])) break;
-      if (lane == 0) mbar_arrive(&k_full[st]);
-      if (!convert(1, j, sm_v + st * LY::kTile, &v_empty[st])) break;
-      if (lane == 0) mbar_arrive(&v_full[st]);
+      if (lane == 0) {
+        mbar_arrive(&raw_empty[side]);
+        mbar_arrive(side ? &v_full[st] : &k_full[st]);
+      }
     }
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp < kLoadWarp) {
-      const int t = warp - kMmaWarp;
-      if (lane == 0 && (t == 0 || two)) {
-        // ---------------------------------------------------------- products
+      // ---------------------------------------------------------- products
+      // The whole warp runs this, one lane issues; what the instructions read is
+      // the same in every lane and known to be (broadcast), so that it stays in
+      // uniform registers.
+      const int t = __shfl_sync(kFull, warp, 0) - kMmaWarp;
+      const int steps = __shfl_sync(kFull, halves_seen, 0);
+      const uint32_t base = __shfl_sync(kFull, tmem, 0);
+      const uint32_t issue = lane == 0;
+      if (t == 0 || two) {
         // Descriptors of the first step; later steps and stages add to the address
         // field (16-byte units), which no tile of shared memory overflows.
         constexpr uint32_t kHi = (uint32_t)(((uint64_t)64 << 32 | (uint64_t)1 << 46 |
                                              (uint64_t)2 << 61) >> 32);
         constexpr uint32_t kTile16 = LY::kTile / 16, kHalf16 = kHalf * 128 / 16;
-        const uint32_t q_lo = (uint32_t)sw128_desc(sm_q + t * LY::kTile);
+        const uint32_t q_lo = (uint32_t)sw128_desc(sm_q) + t * kTile16;
         const uint32_t k_lo = (uint32_t)sw128_desc(sm_k);
         const uint32_t v_lo = (uint32_t)sw128_mn_desc(sm_v, LY::kAtom);
-        const uint32_t s_at = tmem + LY::kScore + t * kN, o_at = tmem + LY::kResult + t * D;
+        const uint32_t s_at = base + LY::kScore + t * kN, o_at = base + LY::kResult + t * D;
         auto scores = [&](int i) {  // half i of the tokens
           const uint32_t kd = k_lo + ((i >> 1) & 1) * kTile16 + (i & 1) * kHalf16;
+          const uint32_t to = s_at + (i & 1) * kHalf;
 #pragma unroll
           for (int k = 0; k < D / 16; ++k) {
             const uint32_t step = ((k / 4) * LY::kAtom + (k % 4) * 32) / 16;
-            umma_f16_lo(s_at + (i & 1) * kHalf, q_lo + step, kd + step, kHi, kHi,
-                        idesc(kHalf, false), k != 0);
+            umma_f16_if(issue, to, q_lo + step, kd + step, kHi, kHi, idesc(kHalf, false), k != 0);
           }
-          umma_commit(&s_full[t][i & 1]);
+          umma_commit_if(issue, &s_full[t][i & 1]);
         };
         auto results = [&](int i) {
           const uint32_t vd = v_lo + ((i >> 1) & 1) * kTile16 + (i & 1) * kHalf16;
+          const uint32_t from = s_at + (i & 1) * kHalf;
 #pragma unroll
           for (int k = 0; k < kHalf / 16; ++k)
-            umma_f16_ts_lo(o_at, s_at + (i & 1) * kHalf + 8 * k, vd + k * (16 * 128 / 16), kHi,
+            umma_f16_ts_if(issue, o_at, from + 8 * k, vd + k * (16 * 128 / 16), kHi,
                            idesc(D, true), i != 0 || k != 0);
-          umma_commit(&o_full[t]);
+          umma_commit_if(issue, &o_full[t]);
         };
-        bool ok = lane_wait(&q_full[t], 0, fail) && lane_wait(&k_full[0], 0, fail);
+        bool ok = warp_wait(&q_full[t], 0, fail) && warp_wait(&k_full[0], 0, fail);
         if (ok) {
           tc_fence_after();
           scores(0);
-          if (halves_seen > 1) scores(1);
-          umma_commit(&k_empty[0]);
+          if (steps > 1) scores(1);
+          umma_commit_if(issue, &k_empty[0]);
         }
 #pragma unroll 1
-        for (int i = 0; i < halves_seen && ok; ++i) {
+        for (int i = 0; i < steps && ok; ++i) {
           const int j = i >> 1, hb = i & 1;
-          if (hb == 0) ok = lane_wait(&v_full[j & 1], (j >> 1) & 1, fail);
-          const bool more = i + 2 < halves_seen;  // scores of half i + 2 take this half's place
-          if (ok && more && hb == 0) ok = lane_wait(&k_full[(j + 1) & 1], ((j + 1) >> 1) & 1, fail);
-          ok = ok && lane_wait(&p_full[t][hb], j & 1, fail);
+          if (hb == 0) ok = warp_wait(&v_full[j & 1], (j >> 1) & 1, fail);
+          const bool more = i + 2 < steps;  // scores of half i + 2 take this half's place
+          if (ok && more && hb == 0) ok = warp_wait(&k_full[(j + 1) & 1], ((j + 1) >> 1) & 1, fail);
+          ok = ok && warp_wait(&p_full[t][hb], j & 1, fail);
           if (!ok) break;
           tc_fence_after();
           results(i);
           if (more) scores(i + 2);
-          if (i + 1 == halves_seen) umma_commit(&o_done[t]);
+          if (i + 1 == steps) umma_commit_if(issue, &o_done[t]);
           if (hb == 1) {
-            umma_commit(&v_empty[j & 1]);
-            umma_commit(&k_empty[(j + 1) & 1]);
+            umma_commit_if(issue, &v_empty[j & 1]);
+            umma_commit_if(issue, &k_empty[(j + 1) & 1]);
           }
         }
         // whatever happened, nothing is in flight when tensor memory is given back
-        umma_commit(&drained[t]);
+        umma_commit_if(issue, &drained[t]);
         mbar_wait(&drained[t], 0, kProbes);
       }
     } else if (warp == kLoadWarp) {
@@ -570,16 +541,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
 template <typename T, int D>
 int launch(const AttendParams& p, int64_t blocks, cudaStream_t st) {
   auto kernel = prompt_kernel<T, D>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       PromptLayout<D>::kSmem);
-  cudaFuncAttributes attr{};
-  if (e == cudaSuccess) e = cudaFuncGetAttributes(&attr, kernel);
-  if (e == cudaSuccess && attr.numRegs != kPromptRegs) {
-    // the shares of setmaxnreg would not add up, and a group would wait for good
-    set_thread_error("paged attend: built with %d registers a thread, not %d", attr.numRegs,
-                     kPromptRegs);
-    return GRM_B200_EINVAL;
-  }
+  const cudaError_t e = cudaFuncSetAttribute(
+      kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PromptLayout<D>::kSmem);
   if (e != cudaSuccess) {
     set_thread_error("paged attend: %s", cudaGetErrorString(e));
     return cuda_status(e);
