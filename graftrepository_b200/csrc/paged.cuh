@@ -134,7 +134,8 @@ __device__ __forceinline__ void row_scale(unsigned m, float* up, float* down) {
 // Base-2 logarithm and inverse of a value scale.  A page of zeros (scale 0)
 // takes 2^-40, any scale being right for it: small enough to leave the other
 // pages' weights alone, large enough for its own to stay above 2^-126 when the
-// reference exponent is another page's.  Scales below 2^-100 count as 2^-100.
+// reference exponent is another page's.  Scales below 2^-100 count as 2^-100, so
+// the inverse is a number even where the scale is none.
 __device__ __forceinline__ void value_scale(float u, float* log2_u, float* inv_u) {
   const float w = u == 0.0f ? 0x1p-40f : fmaxf(u, 0x1p-100f);
   *log2_u = u != u ? u : __log2f(w);

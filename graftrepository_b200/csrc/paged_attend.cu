@@ -378,9 +378,7 @@ __global__ void __launch_bounds__(kThreads, Layout<D, NT>::kBlocks)
           }
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
-            const float sum = pr[x] + pr[x + 2];
-            // a page without a number counts only where it is seen
-            l[nt][x] += sum == 0.0f ? 0.0f : sum * inv;
+            l[nt][x] = fmaf(pr[x] + pr[x + 2], inv, l[nt][x]);
           }
           b[nt][0] = transpose8(pack_half2(pr[0], pr[1]));
           b[nt][1] = transpose8(pack_half2(pr[2], pr[3]));

@@ -81,23 +81,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 __device__ __forceinline__ float max3(uint32_t a, uint32_t b, uint32_t c) {
   return max3(__uint_as_float(a), __uint_as_float(b), __uint_as_float(c));
 }
-// Two fp32 operations in one instruction.
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  float2 d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;"
-      : "=l"(reinterpret_cast<uint64_t&>(d))
-      : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)),
-        "l"(reinterpret_cast<const uint64_t&>(c)));
-  return d;
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-  float2 d;
-  asm("add.rn.f32x2 %0, %1, %2;"
-      : "=l"(reinterpret_cast<uint64_t&>(d))
-      : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)));
-  return d;
-}
-
 // Every lane of a warp waits; false, for all of them, when a wait gave up.
 // The loops of this kernel share an instruction cache that they barely fit, so
 // what is not the common path stays out of line.
@@ -254,17 +237,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
         const int j = i >> 1, hb = i & 1;
         if (hb == 0 && !(ok = warp_wait(&scale_full[j % kScaleRing], (j / kScaleRing) & 1, fail)))
           break;
-        // Factors and offsets of the exponents of 4 x 16 tokens.  Hidden from the
-        // row altogether they have 1 and 0, so that a page without a number does
-        // not reach it; a factor too small for fp32 stays above 0.
+        // factors and offsets of the exponents of 4 x 16 tokens
         const Scale* sc = sm_scale + (j % kScaleRing) * 8 + hb * 4;
         float fk[4], fo[4];
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-          const bool hidden = i * kHalf + 16 * g >= lim;
-          const float k = kq * sc[g].key;
-          fk[g] = hidden ? 1.0f : k == 0.0f ? 0x1p-126f : k;
-          fo[g] = hidden ? 0.0f : sc[g].log2_value;
+          fk[g] = kq * sc[g].key;
+          fo[g] = sc[g].log2_value;
         }
         if (!(ok = warp_wait(&s_full[t][hb], j & 1, fail))) break;
         tc_fence_after();
@@ -274,11 +253,19 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
         tmem_ld32_nowait(s_col + hb * kHalf + 32, v[1]);
         tmem_wait_ld32(v[0]);
         tmem_wait_ld32(v[1]);
-        // hidden tokens: scores of -inf (no factor is 0)
+        // Hidden tokens: scores of -inf, with factors kept above 0.  16 tokens that
+        // are all hidden from the row take factor 1 and offset 0, so that a page
+        // without a number does not reach it.
         if (__any_sync(kFull, (i + 1) * kHalf > lim)) {
 #pragma unroll
           for (int x = 0; x < kHalf; ++x)
             if (i * kHalf + x >= lim) v[x / 32][x % 32] = 0xFF800000u;
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const bool hidden = i * kHalf + 16 * g >= lim;
+            fk[g] = hidden ? 1.0f : fk[g] == 0.0f ? 0x1p-126f : fk[g];
+            fo[g] = hidden ? 0.0f : fo[g];
+          }
         }
         float top = -INFINITY;
 #pragma unroll
@@ -316,21 +303,17 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
 #pragma unroll
           for (int h2 = 0; h2 < 2; ++h2) {
             const int g = 2 * c + h2;
-            const float2 k = make_float2(fk[g], fk[g]);
-            const float2 off = make_float2(fo[g] - ref, fo[g] - ref);
-            float2 sum = make_float2(0.0f, 0.0f);
+            const float k = fk[g], off = fo[g] - ref;
+            float sum0 = 0.0f, sum1 = 0.0f;
 #pragma unroll
             for (int x = 0; x < 16; x += 2) {
-              const float2 y = fma2(make_float2(__uint_as_float(v[c][16 * h2 + x]),
-                                                __uint_as_float(v[c][16 * h2 + x + 1])),
-                                    k, off);
-              const float2 pr = make_float2(ex2(y.x), ex2(y.y));
-              sum = add2(sum, pr);
-              w[8 * h2 + x / 2] = pack_half2(pr.x, pr.y);
+              const float p0 = ex2(fmaf(__uint_as_float(v[c][16 * h2 + x]), k, off));
+              const float p1 = ex2(fmaf(__uint_as_float(v[c][16 * h2 + x + 1]), k, off));
+              sum0 += p0;
+              sum1 += p1;
+              w[8 * h2 + x / 2] = pack_half2(p0, p1);
             }
-            // a page without a number counts only where it is seen
-            const float total = sum.x + sum.y;
-            l += total == 0.0f ? 0.0f : total * sc[g].inv_value;
+            l = fmaf(sum0 + sum1, sc[g].inv_value, l);
           }
           tmem_st16(s_col + hb * kHalf + 16 * c, w);
         }
@@ -368,11 +351,20 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
     // ---------------------------------------------- codes to fp16 tiles
     constexpr int kLanes = D / 16;          // lanes of a row, 16 codes each
     constexpr int kRows = 32 / kLanes;      // rows of one load of the warp
-    const int c = lane % kLanes;
-    const int row0 = (warp - kSoftWarps) * 32 + lane / kLanes;
-    // lanes of the upper half of a row write their second chunk first, so that
-    // eight lanes of a store hit eight different bank groups
-    const int swap = (c >> 2) & 1;
+    // Eight lanes together take the first half of one row's codes and the second
+    // half of the next row's: reads in 8 different bank groups, and writes too,
+    // the swizzle putting what an even row's lanes write, 32 bytes apart, into
+    // even places of 16 bytes and what an odd row's write into odd ones.
+    const int odd = kLanes == 8 ? (lane >> 2) & 1 : 0;
+    const int c = kLanes == 8 ? (lane & 3) + (odd ^ ((lane >> 3) & 1)) * 4 : lane & 3;
+    const int row0 = (warp - kSoftWarps) * 32 + (kLanes == 8 ? odd + (lane >> 4) * 2 : lane >> 2);
+    // places of a lane's two chunks in rows row0 and row0 + 4 (of 8), less the row
+    uint32_t put[2][2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+        put[i][x] = atom_byte(row0 + 4 * i, (c % 4) * 2 + x) - 4 * i * 128;
     bool ok = true;
 #pragma unroll 1
     for (int x = 0; x < 2 * tiles; ++x) {  // keys, values, keys, ...
@@ -388,20 +380,21 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
         uint4 r[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          r[i] = *reinterpret_cast<const uint4*>(src + (i0 + i) * kRows * D);
+          r[i] = *reinterpret_cast<const uint4*>(src + i * kRows * D);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int row = row0 + (i0 + i) * kRows;
           const uint32_t x[4] = {r[i].x ^ 0x80808080u, r[i].y ^ 0x80808080u,
                                  r[i].z ^ 0x80808080u, r[i].w ^ 0x80808080u};
           const uint4 lo = make_uint4(halves(x[0], 0x4140), halves(x[0], 0x4342),
                                       halves(x[1], 0x4140), halves(x[1], 0x4342));
           const uint4 hi = make_uint4(halves(x[2], 0x4140), halves(x[2], 0x4342),
                                       halves(x[3], 0x4140), halves(x[3], 0x4342));
-          const int ch = (c % 4) * 2;
-          *reinterpret_cast<uint4*>(at + atom_byte(row, ch + swap)) = swap ? hi : lo;
-          *reinterpret_cast<uint4*>(at + atom_byte(row, ch + 1 - swap)) = swap ? lo : hi;
+          // rows kRows apart: the swizzle repeats every 8
+          *reinterpret_cast<uint4*>(at + i * kRows * 128 + put[i * kRows / 4 % 2][0]) = lo;
+          *reinterpret_cast<uint4*>(at + i * kRows * 128 + put[i * kRows / 4 % 2][1]) = hi;
         }
+        src += 4 * kRows * D;
+        at += 4 * kRows * 128;
       }
       fence_proxy_async_smem();  // the tile for the tensor cores, the codes' place for the next copy
       __syncwarp();
