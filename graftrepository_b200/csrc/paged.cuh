@@ -7,16 +7,18 @@
 namespace grm_b200 {
 namespace paged {
 
-// Attention walks a request's tokens in tiles of kTile.  The split kernel gives
+// The split kernel of attention walks a request's tokens in tiles and gives
 // every worker (a resident block) the same number of units: a request, kv head
 // and block of query rows ("segment") costs its tiles and one unit more for
 // its start and end.
-constexpr int kTile = 64;
+__host__ __device__ constexpr int split_tile(int dim) { return dim == 256 ? 64 : 128; }
+__host__ __device__ constexpr int split_blocks(int dim) { return dim == 64 ? 3 : 2; }  // an SM
 constexpr int kWorkerSlot = 2048 + 64;  // fp32 of one partial result: rows x dim, then (M, L)
 
 struct Header {           // written by the plan kernel
-  int64_t units;          // units of the split kernel's work, all requests
+  int32_t units;          // units of the split kernel's work, all requests
   int32_t workers;        // workers that share them (<= Shape::workers)
+  int32_t share, more;    // units of a worker, and how many workers have one more
   int32_t pages;          // entries of the append list
   int32_t qtiles;         // entries of the prompt kernel's list
   int32_t rows;           // packed rows of the step
@@ -29,6 +31,7 @@ struct Shape {
   int split_rows;       // requests with more (row, head) pairs a kv head than this are prompts
   int block_rows;       // rows of a segment: 8 or 16
   int qtile_tokens;     // tokens of a prompt tile
+  int tile;             // tokens of a tile of the split kernel
   int workers;          // resident blocks of the split kernel
   int64_t page_cap;     // most pages a step can touch
   int64_t qtile_cap;    // most prompt tiles (0: no request can be a prompt)
@@ -40,7 +43,7 @@ int make_shape(const grm_b200_paged_plan& p, int sms, Shape* s);
 
 struct Lists {
   Header* header;
-  int64_t* base;      // [requests + 1] first unit of each request
+  int32_t* base;      // [requests + 1] first unit of each request
   int32_t* start;     // [workers] request of a worker's first unit
   unsigned* count;    // [workers] arrivals at the segment that a worker starts; 0 between calls
   int2* pages;        // [page_cap] (request, page of the request)
@@ -51,7 +54,7 @@ struct Lists {
 inline Lists lists_of(const Shape& s, void* scratch) {
   char* b = static_cast<char*>(scratch);
   return {reinterpret_cast<Header*>(b),
-          reinterpret_cast<int64_t*>(b + s.off_base),
+          reinterpret_cast<int32_t*>(b + s.off_base),
           reinterpret_cast<int32_t*>(b + s.off_start),
           reinterpret_cast<unsigned*>(b + s.off_count),
           reinterpret_cast<int2*>(b + s.off_pages),
@@ -59,13 +62,13 @@ inline Lists lists_of(const Shape& s, void* scratch) {
           reinterpret_cast<float*>(b + s.off_part)};
 }
 
-// First unit of worker w of `workers`, and the worker that holds unit u: the
-// largest w with first(w) <= u.
-__host__ __device__ inline int64_t worker_first(int64_t w, int64_t units, int64_t workers) {
-  return w * units / workers;
+// First unit of worker w, and the worker that holds unit u.
+__host__ __device__ inline int worker_first(int w, const Header& h) {
+  return w * h.share + (w < h.more ? w : h.more);
 }
-__host__ __device__ inline int64_t worker_of(int64_t u, int64_t units, int64_t workers) {
-  return ((u + 1) * workers - 1) / units;
+__host__ __device__ inline int worker_of(int u, const Header& h) {
+  const int big = h.more * (h.share + 1);  // units of the workers that have one more
+  return u < big ? u / (h.share + 1) : h.more + (u - big) / h.share;
 }
 
 // ---- attention

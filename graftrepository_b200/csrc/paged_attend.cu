@@ -20,16 +20,18 @@
 // finishes it last, in the order of the workers, so results do not depend on
 // timing.
 //
-// A warp owns 16 of a tile's 64 tokens, in a private ring of shared-memory
-// stages that it fills with 16-byte asynchronous copies and drains without a
-// barrier of the block.  Products run on mma.m16n8k16 with fp16 operands and
-// fp32 accumulators, tokens (or value dims) on the M side and the query rows on
-// the 8-wide N side: four query heads of a group waste half of the columns
-// instead of three quarters.  Codes become fp16 exactly: byte b of code + 128
-// under the exponent of 1024 is the half 1024 + b, less 1152.  Queries are
-// fp16: a bf16 row is first scaled by the power of two that brings its largest
-// value into [2^14, 2^15), so only values 2^29 times smaller than the largest
-// round.
+// A warp owns a quarter of a tile's tokens (32 of 128; 16 of 64 at head_dim
+// 256), in a private ring of shared-memory stages that tensor-map copies fill
+// and that it drains without a barrier of the block.  Products run on
+// mma.m16n8k16 with fp16 operands and fp32 accumulators, tokens (or value dims)
+// on the M side and the query rows on the 8-wide N side: four query heads of a
+// group waste half of the columns instead of three quarters.  Codes become fp16
+// exactly: byte b of code + 128 under the exponent of 1024 is the half 1024 + b,
+// less 1152.  Queries are fp16: a bf16 row is first scaled by the power of two
+// that brings its largest value into [2^14, 2^15), so only values 2^29 times
+// smaller than the largest round.
+#include <cuda.h>
+
 #include <algorithm>
 #include <type_traits>
 
@@ -42,32 +44,27 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
+constexpr unsigned kProbes = 1u << 18;  // probes of a bounded wait
+
+struct SplitParams {
+  CUtensorMap k_map, v_map;  // codes as [pages * kv_heads][page_tokens][head_dim] bytes
+  AttendParams a;
+};
 
 template <int D, int NT>
 struct Layout {
-  static constexpr int kStages = D == 256 ? 3 : D == 128 ? 3 : 5;
-  static constexpr int kSide = 16 * D;            // codes of 16 tokens
+  static constexpr int kTokens = split_tile(D) / kWarps;  // of a warp's stage
+  static constexpr int kBlocks16 = kTokens / 16;
+  static constexpr int kStages = D == 64 ? 4 : D == 128 ? 3 : 2;
+  static constexpr int kSide = kTokens * D;       // codes
   static constexpr int kStage = 2 * kSide;
   static constexpr int kRow = D + 4;              // floats of a row in the merge buffer
   static constexpr int kRing = kWarps * kStages * kStage;
-  static constexpr int kMerge = 2 * NT * 8 * kRow * 4;
-  static constexpr int kScales = kWarps * kStages * 2 * 4;
+  static constexpr int kMerge = 2 * 8 * kRow * 4;
+  static constexpr int kScales = kWarps * kStages * 2 * 16;
   static constexpr int kML = 2 * kWarps * NT * 8 * 4;
-  static constexpr int kSmem = kRing + kMerge + kScales + kML + 16;
-  static constexpr int kBlocks = D == 256 ? 2 : 3;
+  static constexpr int kSmem = 1024 + kRing + kMerge + kScales + kML;
 };
-
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -94,74 +91,94 @@ __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// Byte of chunk c (16 codes) of row r in a 16-row tile whose rows are D codes:
-// 16-byte chunks are permuted so that eight rows of one chunk lie in eight
-// different bank groups (ldmatrix reads them together).
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y,
+                                            int z, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+      "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+      : "memory");
+}
+
+// Byte of 16-code chunk c of row r in a warp's stage of `rows` rows.  The
+// copies' swizzle (128 bytes; 64 at head_dim 64) puts eight rows of one chunk
+// into eight different bank groups, which ldmatrix reads together; head_dim 256
+// is two blocks of 128 codes.
 template <int D>
-__device__ __forceinline__ uint32_t tile_byte(int r, int c) {
+__device__ __forceinline__ uint32_t tile_byte(int rows, int r, int c) {
   if (D == 64) return (r >> 1) * 128 + ((((r & 1) << 2) | (c ^ ((r >> 1) & 3))) << 4);
-  return r * D + ((c ^ (r & 7)) << 4);
+  return (c >> 3) * rows * 128 + r * 128 + (((c & 7) ^ (r & 7)) << 4);
 }
 
 // A segment: up to block_rows query rows of a kv head of a request.
 struct Segment {
-  int64_t first;  // its first unit
+  int first;  // its first unit
   int request, tiles, len, start, pairs, head, row0, cached;
 };
 
 // The share of one worker, walked segment by segment.
+template <int TILE>
 struct Walk {
   const AttendParams& p;
-  int64_t begin, end;  // units
-  int64_t u;           // first unit of the next segment to look at
+  int begin, end;  // units
+  int u;           // first unit of the next segment to look at
   int r;
   Segment s;
-  int t, t1;           // tiles of s that are the worker's, from t on
+  int t, t1;       // tiles of s that are the worker's, from t on
 
-  __device__ __forceinline__ Walk(const AttendParams& pp, int64_t b, int64_t e, int request)
-      : p(pp), begin(b), end(e), u(b), r(request) {}
+  __device__ __forceinline__ Walk(const AttendParams& pp, int b, int e, int request)
+      : p(pp), begin(b), end(e), u(b), r(request), t(0), t1(0) {}
 
   // Step to the next segment that reaches into the share; false at its end.
   __device__ __forceinline__ bool next() {
     if (u >= end) return false;
-    while (__ldg(p.l.base + r + 1) <= u) ++r;
-    const int64_t base = __ldg(p.l.base + r);
+    int base = __ldg(p.l.base + r), after = __ldg(p.l.base + r + 1);
+    while (after <= u) {
+      ++r;
+      base = after;
+      after = __ldg(p.l.base + r + 1);
+    }
     s.request = r;
     s.start = __ldg(p.starts + r);
     const int n = __ldg(p.starts + r + 1) - s.start;
     s.len = __ldg(p.lens + r);
     s.cached = s.len - n;
     s.pairs = n * p.group;
-    s.tiles = (s.len + kTile - 1) / kTile;
+    s.tiles = (s.len + TILE - 1) / TILE;
     const int blocks = (s.pairs + p.block_rows - 1) / p.block_rows;
-    const int64_t i = (u - base) / (s.tiles + 1);
+    const int i = (u - base) / (s.tiles + 1);
     s.first = base + i * (s.tiles + 1);
-    s.head = (int)(i / blocks);
-    s.row0 = (int)(i - (int64_t)s.head * blocks) * p.block_rows;
+    s.head = i / blocks;
+    s.row0 = (i - s.head * blocks) * p.block_rows;
     u = s.first + s.tiles + 1;
-    const int64_t a = begin - s.first - 1, b = end - s.first - 1;
-    t = a > 0 ? (int)a : 0;
-    t1 = b < s.tiles ? (int)b : s.tiles;
+    t = max(begin - s.first - 1, 0);
+    t1 = min(end - s.first - 1, s.tiles);
     return true;
   }
 };
 
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kThreads, Layout<D, NT>::kBlocks)
-    split_kernel(const AttendParams p) {
+__global__ void __launch_bounds__(kThreads, split_blocks(D))
+    split_kernel(const __grid_constant__ SplitParams sp) {
   using LY = Layout<D, NT>;
   constexpr int kChunks = D / 16;
-  extern __shared__ __align__(128) unsigned char smem[];
+  constexpr int kTokens = LY::kTokens, kB = LY::kBlocks16;
+  const AttendParams& p = sp.a;
+  extern __shared__ unsigned char raw_smem[];
+  unsigned char* const smem = raw_smem + ((1024u - (smem_u32(raw_smem) & 1023u)) & 1023u);
   float* const merge = reinterpret_cast<float*>(smem + LY::kRing);
-  float* const scales = reinterpret_cast<float*>(smem + LY::kRing + LY::kMerge);
+  float4* const scales = reinterpret_cast<float4*>(smem + LY::kRing + LY::kMerge);
   float* const sm_m = reinterpret_cast<float*>(smem + LY::kRing + LY::kMerge + LY::kScales);
   float* const sm_l = sm_m + kWarps * NT * 8;
-  int* const sm_last = reinterpret_cast<int*>(sm_l + kWarps * NT * 8);
+  __shared__ __align__(8) uint64_t bars[kWarps][LY::kStages];
+  __shared__ int sm_last, sm_fail;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t4 = lane & 3;
   const int heads = p.kv_heads * p.group;
   const Header hd = *p.l.header;
+  const int w = blockIdx.x;
+  const int request0 = p.l.start[w];
 
   // rows past the step's last one
   for (int64_t i = hd.rows + (int64_t)blockIdx.x; i < p.tokens; i += gridDim.x) {
@@ -170,60 +187,93 @@ __global__ void __launch_bounds__(kThreads, Layout<D, NT>::kBlocks)
     if (p.lse)
       for (int x = threadIdx.x; x < heads; x += kThreads) p.lse[i * heads + x] = -INFINITY;
   }
-  const int w = blockIdx.x;
   if (w >= hd.workers) return;
-  const int64_t begin = worker_first(w, hd.units, hd.workers);
-  const int64_t end = worker_first(w + 1, hd.units, hd.workers);
-  const int request0 = p.l.start[w];
+  if (lane == 0) {
+    for (int i = 0; i < LY::kStages; ++i) mbar_init(&bars[warp][i], 1);
+    mbar_fence_init();
+  }
+  if (threadIdx.x == 0) sm_fail = 0;
+  __syncthreads();
+  const int begin = worker_first(w, hd), end = worker_first(w + 1, hd);
 
-  // ---- the loader: 16 tokens of a tile for this warp, one stage at a time
+  // ---- the loader: this warp's tokens of a tile, one stage at a time
   const uint32_t ring = smem_u32(smem) + warp * LY::kStages * LY::kStage;
-  const uint32_t ring_scales = smem_u32(scales) + warp * LY::kStages * 8;
-  Walk load(p, begin, end, request0);
-  bool loading = true;
-  load.t = load.t1 = 0;
-  int ids = 0, ids_base = 0, ids_request = -1;  // lane i: page ids_base + i of the request
-  auto issue = [&](int stage) {
-    while (loading && load.t >= load.t1) loading = load.next();
-    if (loading) {
-      const Segment& s = load.s;
-      const int tok = load.t * kTile + warp * 16;
-      if (tok < s.len) {
-        const int j = tok >> p.page_shift;
-        if (s.request != ids_request || j >= ids_base + 32 || j < ids_base) {
-          const int last = (s.len - 1) >> p.page_shift;
-          ids = __ldg(p.table + s.request * p.width + min(j + lane, last));
-          ids_base = j;
-          ids_request = s.request;
-        }
-        int64_t page = __shfl_sync(kFull, ids, j - ids_base);
-        page = min(max(page, (int64_t)0), p.pages - 1);
-        const int64_t at = page * p.kv_heads + s.head;
-        const int64_t off = ((at << p.page_shift) + (tok & ((1 << p.page_shift) - 1))) * D;
-        const int8_t* kp = p.k + off;
-        const int8_t* vp = p.v + off;
-        const uint32_t dst = ring + stage * LY::kStage;
-#pragma unroll
-        for (int i = 0; i < kChunks / 2; ++i) {
-          const int c = lane + 32 * i;
-          const uint32_t to = dst + tile_byte<D>(c / kChunks, c % kChunks);
-          cp_async16(to, kp + c * 16);
-          cp_async16(to + LY::kSide, vp + c * 16);
-        }
-        if (lane < 2) cp_async4(ring_scales + stage * 8 + lane * 4, (lane ? p.vs : p.ks) + at);
-      }
-      ++load.t;
+  float4* const ring_scales = scales + warp * LY::kStages * 2;
+  Walk<LY::kTokens * kWarps> load(p, begin, end, request0);
+  int issued = 0, used = 0;        // stages
+  // Lane i: page ids_base + i of request and head, its key scale, log2 and inverse
+  // of its value scale; and the page 32 further on.
+  int ids = 0, ids_ahead = 0, ids_base = 0, ids_first = -1;
+  float l_key = 0.0f, l_log = 0.0f, l_inv = 0.0f;
+  auto issue = [&]() {
+    int tok = 0;
+    for (;;) {  // the next tile of the share with tokens for this warp
+      while (load.t >= load.t1)
+        if (!load.next()) return;
+      tok = load.t++ * kTokens * kWarps + warp * kTokens;
+      if (tok < load.s.len) break;
     }
-    cp_commit();
-  };
+    const Segment& s = load.s;
+    const int j = tok >> p.page_shift;
+    if (s.first != ids_first || j >= ids_base + 32) {
+      const int last = (s.len - 1) >> p.page_shift;
+      const int32_t* row = p.table + s.request * p.width;
+      const bool follows = s.first == ids_first && j == ids_base + 32;
+      ids = follows ? ids_ahead : __ldg(row + min(j + lane, last));
+      ids = min(max(ids, 0), (int)p.pages - 1);
+      ids_ahead = __ldg(row + min(j + 32 + lane, last));
+      ids_base = j;
+      ids_first = s.first;
+      const int64_t at = (int64_t)ids * p.kv_heads + s.head;
+      l_key = __ldg(p.ks + at);
+      value_scale(__ldg(p.vs + at), &l_log, &l_inv);
+    }
+    const int stage = issued % LY::kStages;
+    ++issued;
+    const int per = 1 << p.page_shift;
+    const int rows = min(per, kTokens);  // of one copy
+    uint64_t* bar = &bars[warp][stage];
 #pragma unroll
-  for (int i = 0; i < LY::kStages - 1; ++i) issue(i);
-  int stage = 0;
+    for (int b = 0; b < kB; ++b) {  // scales of 16 tokens
+      const int from = ((tok + 16 * b) >> p.page_shift) - ids_base;
+      const float key = __shfl_sync(kFull, l_key, from), lg = __shfl_sync(kFull, l_log, from);
+      const float inv = __shfl_sync(kFull, l_inv, from);
+      if (lane == 0) ring_scales[stage * 2 + b] = make_float4(key, lg, inv, 0.0f);
+    }
+    const int page0 = __shfl_sync(kFull, ids, j - ids_base);
+    const int page1 = __shfl_sync(kFull, ids, min(j + 1 - ids_base, 31));
+    if (lane == 0) {
+      // a second copy where pages are smaller than the stage, unless it would
+      // begin past the request's tokens (what then lies there is not read)
+      const bool both = rows < kTokens && tok + rows < s.len;
+      mbar_arrive_expect_tx(bar, (both ? 2 : 1) * 2 * rows * D);
+      const uint32_t to = ring + stage * LY::kStage;
+      const int y = tok & (per - 1);
+#pragma unroll
+      for (int x = 0; x < D; x += 128) {
+        const uint32_t at = to + (x / 128) * kTokens * 128;
+        tma_load_3d(at, &sp.k_map, x, y, page0 * p.kv_heads + s.head, bar);
+        tma_load_3d(at + LY::kSide, &sp.v_map, x, y, page0 * p.kv_heads + s.head, bar);
+        if (both) {
+          const uint32_t at1 = at + rows * (D < 128 ? D : 128);
+          tma_load_3d(at1, &sp.k_map, x, 0, page1 * p.kv_heads + s.head, bar);
+          tma_load_3d(at1 + LY::kSide, &sp.v_map, x, 0, page1 * p.kv_heads + s.head, bar);
+        }
+      }
+    }
+  };
+#pragma unroll 1
+  for (int i = 0; i < LY::kStages; ++i) issue();
 
   // ldmatrix source of this lane: rows 0-7 / 8-15 of an even chunk, then of an odd one
-  const int lm_row = lane & 15, lm_chunk = lane >> 4;
+  uint32_t lm[kChunks / 2];
+#pragma unroll
+  for (int c = 0; c < kChunks; c += 2)
+    lm[c / 2] = tile_byte<D>(kTokens, lane & 15, c + (lane >> 4));
+  constexpr uint32_t kNext16 = 16 * (D < 128 ? D : 128);  // bytes from 16 rows to the next
 
-  Walk walk(p, begin, end, request0);
+  bool failed = false;
+  Walk<LY::kTokens * kWarps> walk(p, begin, end, request0);
   while (walk.next()) {
     const Segment s = walk.s;
     const int rows = min(s.pairs - s.row0, NT * 8);
@@ -302,26 +352,31 @@ __global__ void __launch_bounds__(kThreads, Layout<D, NT>::kBlocks)
     }
 
     // ---- this worker's tiles
+#pragma unroll 1
     for (int t = walk.t; t < walk.t1; ++t) {
-      cp_wait<LY::kStages - 2>();
+      const int tok = t * kTokens * kWarps + warp * kTokens;
+      if (tok >= s.len) break;  // the last tile, and none of it is this warp's
+      const int stage = used % LY::kStages;
+      if (!failed)
+        failed = !__all_sync(
+            kFull, mbar_wait(&bars[warp][stage], (used / LY::kStages) & 1, kProbes));
+      ++used;
       __syncwarp();
-      issue(stage == 0 ? LY::kStages - 1 : stage - 1);
-      const int tok = t * kTile + warp * 16;
-      if (tok < s.len) {
-        const uint32_t kb = ring + stage * LY::kStage, vb = kb + LY::kSide;
-        const float ks = scales[(warp * LY::kStages + stage) * 2];
-        float lv, inv;
-        value_scale(scales[(warp * LY::kStages + stage) * 2 + 1], &lv, &inv);
-        // scores of 16 tokens x 8 NT rows, in two independent chains
-        float sc[NT][2][4];
+      const uint32_t kb = ring + stage * LY::kStage;
+      // scores of kB x 16 tokens x 8 NT rows
+      float sc[kB][NT][4];
+#pragma unroll
+      for (int b = 0; b < kB; ++b)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int x = 0; x < 4; ++x) sc[nt][0][x] = sc[nt][1][x] = 0.0f;
+          for (int x = 0; x < 4; ++x) sc[b][nt][x] = 0.0f;
 #pragma unroll
-        for (int c = 0; c < kChunks; c += 2) {
+      for (int c = 0; c < kChunks; c += 2)
+#pragma unroll
+        for (int b = 0; b < kB; ++b) {
           uint32_t r[4];
-          ldsm4(r, kb + tile_byte<D>(lm_row, c + lm_chunk));
+          ldsm4(r, kb + lm[c / 2] + b * kNext16);
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
             const uint32_t lo = r[2 * x] ^ 0x80808080u, hi = r[2 * x + 1] ^ 0x80808080u;
@@ -329,76 +384,98 @@ __global__ void __launch_bounds__(kThreads, Layout<D, NT>::kBlocks)
             const uint32_t a1 = halves(hi, 0x4140), a3 = halves(hi, 0x4342);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
-              mma(sc[nt][x], a0, a1, a2, a3, qf[c + x][nt][0], qf[c + x][nt][1]);
+              mma(sc[b][nt], a0, a1, a2, a3, qf[c + x][nt][0], qf[c + x][nt][1]);
           }
         }
-        uint32_t b[NT][2];
-        float y[NT][4];
-        bool moves = false;
+      bool moves = false;
+      float inv[kB];
+#pragma unroll
+      for (int b = 0; b < kB; ++b) {
+        const float4 f = ring_scales[stage * 2 + b];
+        inv[b] = f.z;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-          for (int x = 0; x < 4; ++x)
-            y[nt][x] = fmaf(sc[nt][0][x] + sc[nt][1][x], kq[nt][x & 1] * ks, lv);
-          if (tok + 16 > all_see) {
-#pragma unroll
-            for (int x = 0; x < 4; ++x)
-              if (tok + g + (x >> 1) * 8 >= min(lim[nt][x & 1], s.len)) y[nt][x] = -INFINITY;
+          for (int x = 0; x < 4; ++x) {
+            sc[b][nt][x] = fmaf(sc[b][nt][x], kq[nt][x & 1] * f.x, f.y);
           }
-#pragma unroll
-          for (int x = 0; x < 4; ++x) moves |= y[nt][x] > m[nt][x & 1] + kLazy;
         }
-        if (__any_sync(kFull, moves)) {
+      }
+      if (tok + kTokens > all_see) {
+#pragma unroll
+        for (int b = 0; b < kB; ++b)
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-              float top = fmaxf(y[nt][x], y[nt][x + 2]);
+            for (int x = 0; x < 4; ++x)
+              if (tok + 16 * b + g + (x >> 1) * 8 >= min(lim[nt][x & 1], s.len))
+                sc[b][nt][x] = -INFINITY;
+      }
 #pragma unroll
-              for (int i = 4; i <= 16; i <<= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, i));
-              // each row by its own scores, so that no row's rounding hangs on another's
-              if (!(top > m[nt][x] + kLazy)) top = m[nt][x];
-              const float a = top == m[nt][x] ? 1.0f : ex2(m[nt][x] - top);
-              m[nt][x] = top;
-              l[nt][x] *= a;
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-              for (int c = 0; c < kChunks; ++c) {
-                o[c][nt][x] *= a;
-                o[c][nt][x + 2] *= a;
-              }
-            }
+        for (int x = 0; x < 2; ++x) {
+          float top = fmaxf(sc[0][nt][x], sc[0][nt][x + 2]);
+          if (kB == 2) top = fmaxf(top, fmaxf(sc[kB - 1][nt][x], sc[kB - 1][nt][x + 2]));
+          moves |= top > m[nt][x] + kLazy;
         }
+      if (__any_sync(kFull, moves)) {
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          float pr[4];
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const float ref = m[nt][x & 1] == -INFINITY ? 0.0f : m[nt][x & 1];
-            pr[x] = ex2(y[nt][x] - ref);
-          }
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
-            l[nt][x] = fmaf(pr[x] + pr[x + 2], inv, l[nt][x]);
-          }
-          b[nt][0] = transpose8(pack_half2(pr[0], pr[1]));
-          b[nt][1] = transpose8(pack_half2(pr[2], pr[3]));
-        }
-        // result dims 16c + 2g (rows g) and 16c + 2g + 1 (rows g + 8)
+            float top = fmaxf(sc[0][nt][x], sc[0][nt][x + 2]);
+            if (kB == 2) top = fmaxf(top, fmaxf(sc[kB - 1][nt][x], sc[kB - 1][nt][x + 2]));
 #pragma unroll
-        for (int c = 0; c < kChunks; c += 2) {
+            for (int i = 4; i <= 16; i <<= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, i));
+            // each row by its own scores, so that no row's rounding hangs on another's
+            if (!(top > m[nt][x] + kLazy)) top = m[nt][x];
+            const float a = top == m[nt][x] ? 1.0f : ex2(m[nt][x] - top);
+            m[nt][x] = top;
+            l[nt][x] *= a;
+#pragma unroll
+            for (int c = 0; c < kChunks; ++c) {
+              o[c][nt][x] *= a;
+              o[c][nt][x + 2] *= a;
+            }
+          }
+      }
+      uint32_t bp[kB][NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float ref[2];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) ref[x] = m[nt][x] == -INFINITY ? 0.0f : m[nt][x];
+#pragma unroll
+        for (int b = 0; b < kB; ++b) {
+          float pr[4];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) pr[x] = ex2(sc[b][nt][x] - ref[x & 1]);
+#pragma unroll
+          for (int x = 0; x < 2; ++x) l[nt][x] = fmaf(pr[x] + pr[x + 2], inv[b], l[nt][x]);
+          bp[b][nt][0] = transpose8(pack_half2(pr[0], pr[1]));
+          bp[b][nt][1] = transpose8(pack_half2(pr[2], pr[3]));
+        }
+      }
+      // result dims 16c + 2g (rows g) and 16c + 2g + 1 (rows g + 8)
+#pragma unroll
+      for (int c = 0; c < kChunks; c += 2)
+#pragma unroll
+        for (int b = 0; b < kB; ++b) {
           uint32_t r[4];
-          ldsm4t(r, vb + tile_byte<D>(lm_row, c + lm_chunk));
+          ldsm4t(r, kb + lm[c / 2] + (LY::kSide + b * kNext16));
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
             const uint32_t lo = r[2 * x] ^ 0x80808080u, hi = r[2 * x + 1] ^ 0x80808080u;
             const uint32_t a0 = halves(lo, 0x4240), a1 = halves(lo, 0x4341);
             const uint32_t a2 = halves(hi, 0x4240), a3 = halves(hi, 0x4341);
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma(o[c + x][nt], a0, a1, a2, a3, b[nt][0], b[nt][1]);
+            for (int nt = 0; nt < NT; ++nt)
+              mma(o[c + x][nt], a0, a1, a2, a3, bp[b][nt][0], bp[b][nt][1]);
           }
         }
-      }
-      stage = stage + 1 == LY::kStages ? 0 : stage + 1;
+      __syncwarp();  // the stage is read: its place is free
+      if (!failed) issue();
     }
 
     // ---- join the four warps
@@ -438,41 +515,40 @@ __global__ void __launch_bounds__(kThreads, Layout<D, NT>::kBlocks)
           o[c][nt][x + 2] *= a;
         }
       }
-    auto at = [&](int buf, int c, int nt, int x) {
-      return reinterpret_cast<float2*>(merge + (buf * NT * 8 + nt * 8 + 2 * t4 + x) * LY::kRow +
-                                       16 * c + 2 * g);
-    };
-    auto put = [&](int buf) {
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+    for (int nt = 0; nt < NT; ++nt) {  // 8 rows at a time: 2, 3 to 0, 1, then 1 to 0
+      auto at = [&](int buf, int c, int x) {
+        return reinterpret_cast<float2*>(merge + (buf * 8 + 2 * t4 + x) * LY::kRow + 16 * c +
+                                         2 * g);
+      };
+      auto put = [&](int buf) {
 #pragma unroll
         for (int c = 0; c < kChunks; ++c)
 #pragma unroll
-          for (int x = 0; x < 2; ++x) *at(buf, c, nt, x) = make_float2(o[c][nt][x], o[c][nt][x + 2]);
-    };
-    auto add = [&](int buf) {
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+          for (int x = 0; x < 2; ++x) *at(buf, c, x) = make_float2(o[c][nt][x], o[c][nt][x + 2]);
+      };
+      auto add = [&](int buf) {
 #pragma unroll
         for (int c = 0; c < kChunks; ++c)
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
-            const float2 v = *at(buf, c, nt, x);
+            const float2 v = *at(buf, c, x);
             o[c][nt][x] += v.x;
             o[c][nt][x + 2] += v.y;
           }
-    };
-    if (warp >= 2) put(warp - 2);
-    __syncthreads();
-    if (warp < 2) add(warp);
-    __syncthreads();
-    if (warp == 1) put(0);
-    __syncthreads();
-    if (warp == 0) add(0);
+      };
+      if (warp >= 2) put(warp - 2);
+      __syncthreads();
+      if (warp < 2) add(warp);
+      __syncthreads();
+      if (warp == 1) put(0);
+      __syncthreads();
+      if (warp == 0) add(0);
+      if (nt + 1 < NT) __syncthreads();
+    }
 
     // ---- alone on the segment: done
-    const int64_t wa = worker_of(s.first + 1, hd.units, hd.workers);
-    const int64_t wb = worker_of(s.first + s.tiles, hd.units, hd.workers);
+    const int wa = worker_of(s.first + 1, hd), wb = worker_of(s.first + s.tiles, hd);
     if (wa == wb) {
       if (warp == 0) {
 #pragma unroll
@@ -519,12 +595,12 @@ __global__ void __launch_bounds__(kThreads, Layout<D, NT>::kBlocks)
         const unsigned arrived = atomicAdd(p.l.count + wa, 1u);
         const int last = arrived + 1 == (unsigned)(wb - wa + 1);
         if (last) p.l.count[wa] = 0;  // for the next call
-        *sm_last = last;
+        sm_last = last;
         __threadfence();
       }
     }
     __syncthreads();
-    if (*sm_last) {
+    if (sm_last) {
       const int n = (int)(wb - wa + 1);
       auto part = [&](int i) {
         return p.l.part + (2 * (wa + i) + (i == 0 ? 1 : 0)) * (int64_t)kWorkerSlot;
@@ -561,13 +637,20 @@ __global__ void __launch_bounds__(kThreads, Layout<D, NT>::kBlocks)
       }
     }
   }
-  cp_wait<0>();
+  if (failed) {  // copies still in flight end before the block does
+    if (lane == 0) sm_fail = 1;
+    for (; used < issued; ++used)
+      mbar_wait(&bars[warp][used % LY::kStages], (used / LY::kStages) & 1, kProbes);
+  }
+  __syncthreads();
+  if (threadIdx.x == 0 && sm_fail) atomicOr(p.status, GRM_B200_PLAN_WAIT);
 }
 
 template <typename T, int D, int NT>
-int launch_split(const AttendParams& p, int workers, cudaStream_t st) {
+int launch_split(const SplitParams& p, int workers, cudaStream_t st) {
   using LY = Layout<D, NT>;
   static_assert(NT * 8 * D <= 2048, "a partial result fits its slot");
+  static_assert((LY::kSmem + 2048) * split_blocks(D) <= 228 * 1024, "blocks of an SM");
   auto kernel = split_kernel<T, D, NT>;
   const cudaError_t e =
       cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, LY::kSmem);
@@ -580,7 +663,7 @@ int launch_split(const AttendParams& p, int workers, cudaStream_t st) {
 }
 
 template <typename T>
-int launch_split_any(int dim, int block_rows, const AttendParams& p, int workers,
+int launch_split_any(int dim, int block_rows, const SplitParams& p, int workers,
                      cudaStream_t st) {
   if (dim == 64)
     return block_rows == 8 ? launch_split<T, 64, 1>(p, workers, st)
@@ -589,6 +672,49 @@ int launch_split_any(int dim, int block_rows, const AttendParams& p, int workers
     return block_rows == 8 ? launch_split<T, 128, 1>(p, workers, st)
                            : launch_split<T, 128, 2>(p, workers, st);
   return launch_split<T, 256, 1>(p, workers, st);
+}
+
+// cuTensorMapEncodeTiled from the driver, looked up once (no libcuda link).
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
+                                 const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                 const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiled encode_tiled() {
+  static const EncodeTiled fn = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault,
+                                         &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      f = nullptr;
+    return reinterpret_cast<EncodeTiled>(f);
+  }();
+  return fn;
+}
+
+// The codes of one side as rows of bytes: a box is the rows that one copy brings
+// (a page, at most a warp's stage) by 128 bytes.
+int make_map(CUtensorMap* map, const int8_t* codes, const grm_b200_paged_arena& a) {
+  const EncodeTiled encode = encode_tiled();
+  const int stage = split_tile(a.head_dim) / kWarps;
+  const cuuint64_t dims[3] = {(cuuint64_t)a.head_dim, (cuuint64_t)a.page_tokens,
+                              (cuuint64_t)a.pages * a.kv_heads};
+  const cuuint64_t strides[2] = {(cuuint64_t)a.head_dim,
+                                 (cuuint64_t)a.head_dim * a.page_tokens};
+  const cuuint32_t box[3] = {(cuuint32_t)std::min(a.head_dim, 128),
+                             (cuuint32_t)std::min(a.page_tokens, stage), 1};
+  const cuuint32_t step[3] = {1, 1, 1};
+  if (!encode ||
+      encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<int8_t*>(codes), dims, strides, box,
+             step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             a.head_dim == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS) {
+    set_thread_error("paged attend: no tensor map of the arena (pages %lld, kv_heads %d)",
+                     (long long)a.pages, a.kv_heads);
+    return GRM_B200_EINVAL;
+  }
+  return 0;
 }
 
 }  // namespace
@@ -626,7 +752,11 @@ int grm_b200_paged_attend(const grm_b200_paged_plan* plan, const grm_b200_paged_
   if ((rc = current_sms(&sms))) return rc;
   Shape s;
   make_shape(*plan, sms, &s);
-  AttendParams p;
+  SplitParams sp;
+  if ((rc = make_map(&sp.k_map, arena->k_codes, *arena)) ||
+      (rc = make_map(&sp.v_map, arena->v_codes, *arena)))
+    return rc;
+  AttendParams& p = sp.a;
   p.l = lists_of(s, plan->scratch);
   p.table = plan->table;
   p.lens = plan->lens;
@@ -653,8 +783,8 @@ int grm_b200_paged_attend(const grm_b200_paged_plan* plan, const grm_b200_paged_
   p.status = plan->status;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   rc = dtype == GRM_B200_F16
-           ? launch_split_any<__half>(plan->head_dim, s.block_rows, p, s.workers, st)
-           : launch_split_any<__nv_bfloat16>(plan->head_dim, s.block_rows, p, s.workers, st);
+           ? launch_split_any<__half>(plan->head_dim, s.block_rows, sp, s.workers, st)
+           : launch_split_any<__nv_bfloat16>(plan->head_dim, s.block_rows, sp, s.workers, st);
   if (rc == 0 && s.qtile_cap > 0)
     rc = launch_prompt(dtype, plan->head_dim, p, s.qtile_cap * plan->kv_heads, st);
   return rc;

@@ -65,7 +65,7 @@ __device__ __forceinline__ void weigh(const PlanParams& p, const Request& q, int
   v[3] = prompt ? ceil_div64(q.fresh, p.s.qtile_tokens) : 0;
   v[4] = prompt ? 0
                 : p.kv_heads * ceil_div64(pairs, p.s.block_rows) *
-                      (ceil_div64(q.after, kTile) + 1);
+                      (ceil_div64(q.after, p.s.tile) + 1);
 }
 
 __device__ __forceinline__ int64_t warp_sum(int64_t v) {
@@ -155,11 +155,12 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
   if (total[kRows] > p.tokens) failed |= GRM_B200_PLAN_ROWS;
   if (taken0 < 0 || returned - taken0 > p.ring_size || total[kTake] > returned - taken0)
     failed |= GRM_B200_PLAN_PAGES;
-  const int64_t units = failed ? 0 : total[kUnits];
+  if (total[kUnits] > INT32_MAX - (1 << 20)) failed |= GRM_B200_PLAN_ROWS;
+  const int units = failed ? 0 : (int)total[kUnits];
   const int all_rows = failed ? 0 : (int)total[kRows];
   // Few units: fewer workers, so that none gets less than min_units of them.
-  int64_t most = (units + p.min_units - 1) / p.min_units;
-  const int workers = most < p.s.workers ? (int)most : p.s.workers;
+  const int most = (units + p.min_units - 1) / p.min_units;
+  const int workers = most < p.s.workers ? most : p.s.workers;
 
   if (gid == 0) {
     p.status[0] = failed;
@@ -167,8 +168,13 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
     p.cursor[1] = returned;
     p.starts[p.requests] = all_rows;
     p.l.base[p.requests] = units;
-    *p.l.header = Header{units, workers, failed ? 0 : (int)total[kTouched],
-                         failed ? 0 : (int)total[kTiles], all_rows};
+    *p.l.header = Header{units,
+                         workers,
+                         workers ? units / workers : 0,
+                         workers ? units % workers : 0,
+                         failed ? 0 : (int)total[kTouched],
+                         failed ? 0 : (int)total[kTiles],
+                         all_rows};
   }
   for (int i = gid; i < p.s.workers; i += gsize) p.l.count[i] = 0;
   for (int64_t i = all_rows + gid; i < p.tokens; i += gsize) {
@@ -237,7 +243,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
     if (blockIdx.x == r0 / kPlanThreads % gridDim.x && tid < n) {
       p.lens[r0 + tid] = q.after;
       p.starts[r0 + tid] = sum[kRows][tid];
-      p.l.base[r0 + tid] = sum_units[tid];
+      p.l.base[r0 + tid] = (int)sum_units[tid];
     }
     for (int64_t x = sum[kTake][0] + (int64_t)gid; x < sum[kTake][n]; x += gsize) {
       const int i = find(sum[kTake], n, (int)x);
@@ -269,7 +275,8 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
       p.l.qtiles[x] = make_int2((int)(r0 + i), ((int)x - sum[kTiles][i]) * p.s.qtile_tokens);
     }
     for (int w = gid; w < workers; w += gsize) {
-      const int64_t u = worker_first(w, units, workers);
+      const int share = units / workers, more = units % workers;
+      const int64_t u = w * share + (w < more ? w : more);
       if (u >= sum_units[0] && u < sum_units[n])
         p.l.start[w] = (int)(r0 + find(sum_units, n, u));
     }
@@ -338,7 +345,8 @@ int make_shape(const grm_b200_paged_plan& p, int sms, Shape* s) {
   const bool prompts = p.head_dim <= 128 && most > kPromptRows;
   s->split_rows = prompts ? kPromptRows : INT32_MAX;
   s->qtile_tokens = 2 * (128 / s->group);
-  s->workers = sms * (p.head_dim == 256 ? 2 : 3);
+  s->tile = split_tile(p.head_dim);
+  s->workers = sms * split_blocks(p.head_dim);
   const int64_t R = p.requests, T = p.tokens;
   s->page_cap = p.grow ? std::min(T, T / p.page_tokens + 2 * std::min(R, T)) : 0;
   s->qtile_cap = prompts ? std::min(T, T / s->qtile_tokens + std::min(R, T)) : 0;
@@ -348,7 +356,7 @@ int make_shape(const grm_b200_paged_plan& p, int sms, Shape* s) {
     at += align256(bytes);
     return o;
   };
-  s->off_base = take((R + 1) * 8);
+  s->off_base = take((R + 1) * 4);
   s->off_start = take((int64_t)s->workers * 4);
   s->off_count = take((int64_t)s->workers * 4);
   s->off_pages = take(std::min(T, T / p.page_tokens + 2 * std::min(R, T)) * 8);
@@ -449,7 +457,7 @@ int check_arena(const grm_b200_paged_arena* a) {
     set_thread_error("paged arena: a buffer is missing");
     return GRM_B200_EINVAL;
   }
-  if (a->pages < 1 || a->pages > INT32_MAX || a->kv_heads < 1 || a->kv_heads > 1024 ||
+  if (a->pages < 1 || a->kv_heads < 1 || a->pages > INT32_MAX / a->kv_heads || a->kv_heads > 1024 ||
       !page_ok(a->page_tokens) || !dim_ok(a->head_dim)) {
     set_thread_error("paged arena: pages %lld, kv_heads %d, page_tokens %d (16, 32, 64, 128), "
                      "head_dim %d (64, 128, 256)",
@@ -519,7 +527,7 @@ int grm_b200_paged_plan_step(const grm_b200_paged_plan* plan, const int32_t* fre
   p.grow = plan->grow ? 1 : 0;
   p.kv_heads = plan->kv_heads;
   make_shape(*plan, sms, &p.s);
-  p.min_units = 3;
+  p.min_units = 2;
   p.cached = plan->cached;
   p.fresh = fresh_device;
   p.ring = plan->ring;
