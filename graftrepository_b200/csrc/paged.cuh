@@ -12,7 +12,10 @@ namespace paged {
 // and block of query rows ("segment") costs its tiles and one unit more for
 // its start and end.
 __host__ __device__ constexpr int split_tile(int dim) { return dim == 256 ? 64 : 128; }
-__host__ __device__ constexpr int split_blocks(int dim) { return dim == 64 ? 3 : 2; }  // an SM
+// Its blocks on an SM, for segments of `rows` query rows.
+__host__ __device__ constexpr int split_blocks(int dim, int rows) {
+  return dim == 64 || (dim == 128 && rows == 8) ? 3 : 2;
+}
 constexpr int kWorkerSlot = 2048 + 64;  // fp32 of one partial result: rows x dim, then (M, L)
 
 struct Header {           // written by the plan kernel

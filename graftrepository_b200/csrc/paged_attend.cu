@@ -55,7 +55,8 @@ template <int D, int NT>
 struct Layout {
   static constexpr int kTokens = split_tile(D) / kWarps;  // of a warp's stage
   static constexpr int kBlocks16 = kTokens / 16;
-  static constexpr int kStages = D == 64 ? 4 : D == 128 ? 3 : 2;
+  static constexpr int kBlocks = split_blocks(D, NT * 8);
+  static constexpr int kStages = D == 64 ? 4 : kBlocks == 3 || D == 256 ? 2 : 3;
   static constexpr int kSide = kTokens * D;       // codes
   static constexpr int kStage = 2 * kSide;
   static constexpr int kRow = D + 4;              // floats of a row in the merge buffer
@@ -158,7 +159,7 @@ struct Walk {
 };
 
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kThreads, split_blocks(D))
+__global__ void __launch_bounds__(kThreads, (Layout<D, NT>::kBlocks))
     split_kernel(const __grid_constant__ SplitParams sp) {
   using LY = Layout<D, NT>;
   constexpr int kChunks = D / 16;
@@ -371,12 +372,22 @@ __global__ void __launch_bounds__(kThreads, split_blocks(D))
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int x = 0; x < 4; ++x) sc[b][nt][x] = 0.0f;
+      // (fragments one step ahead of their use)
+      uint32_t fr[2][kB][4];
 #pragma unroll
-      for (int c = 0; c < kChunks; c += 2)
+      for (int b = 0; b < kB; ++b) ldsm4(fr[0][b], kb + lm[0] + b * kNext16);
+#pragma unroll
+      for (int c = 0; c < kChunks; c += 2) {
 #pragma unroll
         for (int b = 0; b < kB; ++b) {
-          uint32_t r[4];
-          ldsm4(r, kb + lm[c / 2] + b * kNext16);
+          if (c + 2 < kChunks)
+            ldsm4(fr[(c / 2 + 1) % 2][b], kb + lm[(c + 2) / 2 % (kChunks / 2)] + b * kNext16);
+          else  // the first value fragments
+            ldsm4t(fr[(c / 2 + 1) % 2][b], kb + lm[0] + (LY::kSide + b * kNext16));
+        }
+#pragma unroll
+        for (int b = 0; b < kB; ++b) {
+          const uint32_t* r = fr[(c / 2) % 2][b];
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
             const uint32_t lo = r[2 * x] ^ 0x80808080u, hi = r[2 * x + 1] ^ 0x80808080u;
@@ -387,6 +398,7 @@ __global__ void __launch_bounds__(kThreads, split_blocks(D))
               mma(sc[b][nt], a0, a1, a2, a3, qf[c + x][nt][0], qf[c + x][nt][1]);
           }
         }
+      }
       bool moves = false;
       float inv[kB];
 #pragma unroll
@@ -459,11 +471,17 @@ __global__ void __launch_bounds__(kThreads, split_blocks(D))
       }
       // result dims 16c + 2g (rows g) and 16c + 2g + 1 (rows g + 8)
 #pragma unroll
-      for (int c = 0; c < kChunks; c += 2)
+      for (int c = 0; c < kChunks; c += 2) {
+        constexpr int kFirst = kChunks / 2;  // the buffer that the loop above left them in
+        if (c + 2 < kChunks) {
+#pragma unroll
+          for (int b = 0; b < kB; ++b)
+            ldsm4t(fr[(c / 2 + kFirst + 1) % 2][b],
+                   kb + lm[(c + 2) / 2 % (kChunks / 2)] + (LY::kSide + b * kNext16));
+        }
 #pragma unroll
         for (int b = 0; b < kB; ++b) {
-          uint32_t r[4];
-          ldsm4t(r, kb + lm[c / 2] + (LY::kSide + b * kNext16));
+          const uint32_t* r = fr[(c / 2 + kFirst) % 2][b];
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
             const uint32_t lo = r[2 * x] ^ 0x80808080u, hi = r[2 * x + 1] ^ 0x80808080u;
@@ -474,6 +492,7 @@ __global__ void __launch_bounds__(kThreads, split_blocks(D))
               mma(o[c + x][nt], a0, a1, a2, a3, bp[b][nt][0], bp[b][nt][1]);
           }
         }
+      }
       __syncwarp();  // the stage is read: its place is free
       if (!failed) issue();
     }
@@ -650,7 +669,7 @@ template <typename T, int D, int NT>
 int launch_split(const SplitParams& p, int workers, cudaStream_t st) {
   using LY = Layout<D, NT>;
   static_assert(NT * 8 * D <= 2048, "a partial result fits its slot");
-  static_assert((LY::kSmem + 2048) * split_blocks(D) <= 228 * 1024, "blocks of an SM");
+  static_assert((LY::kSmem + 2048) * LY::kBlocks <= 228 * 1024, "blocks of an SM");
   auto kernel = split_kernel<T, D, NT>;
   const cudaError_t e =
       cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, LY::kSmem);

@@ -346,7 +346,7 @@ int make_shape(const grm_b200_paged_plan& p, int sms, Shape* s) {
   s->split_rows = prompts ? kPromptRows : INT32_MAX;
   s->qtile_tokens = 2 * (128 / s->group);
   s->tile = split_tile(p.head_dim);
-  s->workers = sms * split_blocks(p.head_dim);
+  s->workers = sms * split_blocks(p.head_dim, s->block_rows);
   const int64_t R = p.requests, T = p.tokens;
   s->page_cap = p.grow ? std::min(T, T / p.page_tokens + 2 * std::min(R, T)) : 0;
   s->qtile_cap = prompts ? std::min(T, T / s->qtile_tokens + std::min(R, T)) : 0;
