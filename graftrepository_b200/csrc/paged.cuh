@@ -2,6 +2,8 @@
 // plan's scratch (work lists and partial results) and the checks of arguments.
 #pragma once
 
+#include <atomic>
+
 #include "common.cuh"
 
 namespace grm_b200 {
@@ -159,6 +161,9 @@ int check_match(const grm_b200_paged_plan* p, const grm_b200_paged_arena* a);
 int check_rows(const char* what, const void* ptr, int dtype, int64_t row_stride,
                int64_t head_stride);
 int current_sms(int* sms);
+// Lets a kernel use `bytes` of dynamic shared memory; `done` (one a kernel)
+// remembers the devices where that is set.
+int allow_shared(const void* kernel, int bytes, std::atomic<uint64_t>* done);
 inline int shift_of(int page_tokens) {  // log2 of 16, 32, 64 or 128
   return page_tokens == 16 ? 4 : page_tokens == 32 ? 5 : page_tokens == 64 ? 6 : 7;
 }

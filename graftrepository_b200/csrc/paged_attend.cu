@@ -671,12 +671,9 @@ int launch_split(const SplitParams& p, int workers, cudaStream_t st) {
   static_assert(NT * 8 * D <= 2048, "a partial result fits its slot");
   static_assert((LY::kSmem + 2048) * LY::kBlocks <= 228 * 1024, "blocks of an SM");
   auto kernel = split_kernel<T, D, NT>;
-  const cudaError_t e =
-      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, LY::kSmem);
-  if (e != cudaSuccess) {
-    set_thread_error("paged attend: %s", cudaGetErrorString(e));
-    return cuda_status(e);
-  }
+  static std::atomic<uint64_t> done{0};
+  const int rc = allow_shared(reinterpret_cast<const void*>(kernel), LY::kSmem, &done);
+  if (rc) return rc;
   kernel<<<workers, kThreads, LY::kSmem, st>>>(p);
   return launch_status("paged attend");
 }

@@ -383,6 +383,21 @@ int current_sms(int* sms) {
   return 0;
 }
 
+int allow_shared(const void* kernel, int bytes, std::atomic<uint64_t>* done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  const uint64_t bit = (uint64_t)1 << (dev & 63);
+  if (e == cudaSuccess && (done->load(std::memory_order_relaxed) & bit)) return 0;
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) {
+    set_thread_error("paged attend: %s", cudaGetErrorString(e));
+    return cuda_status(e);
+  }
+  done->fetch_or(bit, std::memory_order_relaxed);
+  return 0;
+}
+
 int launch_status(const char* what) {
   const cudaError_t e = cudaGetLastError();
   if (e == cudaSuccess) return 0;

@@ -534,12 +534,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
 template <typename T, int D>
 int launch(const AttendParams& p, int64_t blocks, cudaStream_t st) {
   auto kernel = prompt_kernel<T, D>;
-  const cudaError_t e = cudaFuncSetAttribute(
-      kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PromptLayout<D>::kSmem);
-  if (e != cudaSuccess) {
-    set_thread_error("paged attend: %s", cudaGetErrorString(e));
-    return cuda_status(e);
-  }
+  static std::atomic<uint64_t> done{0};
+  const int rc =
+      allow_shared(reinterpret_cast<const void*>(kernel), PromptLayout<D>::kSmem, &done);
+  if (rc) return rc;
   kernel<<<(unsigned)blocks, kPromptThreads, PromptLayout<D>::kSmem, st>>>(p);
   return launch_status("paged attend");
 }

@@ -35,6 +35,8 @@ from __future__ import annotations
 import ctypes
 import math
 
+import torch
+
 from . import _lib
 
 __all__ = ["PAGE_TOKENS", "HEAD_DIMS", "PageTables", "PagePlan", "PagedArena"]
@@ -74,50 +76,53 @@ class _PlanC(ctypes.Structure):
                 ("scratch_bytes", ctypes.c_int64)]
 
 
-def _stream(stream, device, *tensors):
-    """(torch stream, handle) of a call; the caching allocator is told of
-    `tensors` where the stream is not the current one."""
-    import torch
+_TYPES = {torch.float16: _lib.GRM_B200_F16, torch.bfloat16: _lib.GRM_B200_BF16}
+_READ_TYPES = {torch.float32: _lib.GRM_B200_F32, **_TYPES}
 
-    current = torch.cuda.current_stream(device)
-    if stream is None:
-        return current, current.cuda_stream
+# A decoding step makes these calls for every layer, so their host side is kept
+# short: shapes and entry points are looked up once, and the current stream's
+# handle comes straight from torch's binding where it has one.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _torch_stream(stream, index, *tensors):
+    """`stream` (a torch stream or a raw handle) as a torch stream; the caching
+    allocator is told that `tensors` are used on it."""
     if not hasattr(stream, "cuda_stream"):
-        stream = torch.cuda.ExternalStream(int(stream), device=device)
-    if stream.cuda_stream != current.cuda_stream:
-        for t in tensors:
-            t.record_stream(stream)
-    return stream, stream.cuda_stream
+        stream = torch.cuda.ExternalStream(int(stream), device=torch.device("cuda", index))
+    for t in tensors:
+        t.record_stream(stream)
+    return stream
 
 
-def _empty(shape, dtype, device, stream):
-    """A result that belongs to the stream that writes it."""
-    import torch
+def _handle(stream, index, *tensors) -> int:
+    if stream is None:
+        return _raw_stream(index)
+    return _torch_stream(stream, index, *tensors).cuda_stream
 
-    if stream == torch.cuda.current_stream(device):
-        return torch.empty(shape, dtype=dtype, device=device)
-    with torch.cuda.stream(stream):
-        return torch.empty(shape, dtype=dtype, device=device)
+
+def _empty(like, shape, dtype, stream):
+    """A result on the device of `like` that belongs to the stream that writes it."""
+    if stream is None:
+        return like.new_empty(shape, dtype=dtype)
+    with torch.cuda.stream(_torch_stream(stream, like.get_device())):
+        return like.new_empty(shape, dtype=dtype)
 
 
 def _device(device):
-    import torch
-
     d = torch.device(device)
     if d.type != "cuda":
         raise ValueError(f"the paged arena lives on a CUDA device, not {device!r}")
     return d if d.index is not None else torch.device("cuda", torch.cuda.current_device())
 
 
-def _call(name: str, device, *args) -> None:
-    """One library call with `device` current."""
-    import torch
-
-    fn = getattr(_lib.load(), name)
-    if torch.cuda.current_device() == device.index:
+def _call(fn, index, *args) -> None:
+    """One library call with device `index` current."""
+    if torch.cuda.current_device() == index:
         rc = fn(*args)
     else:
-        with torch.cuda.device(device):
+        with torch.cuda.device(index):
             rc = fn(*args)
     if rc:
         _lib.check(rc, _lib.thread_error)
@@ -137,8 +142,6 @@ class PagePlan:
 
     def __init__(self, tables: "PageTables", tokens: int, kv_heads: int, query_heads: int,
                  head_dim: int, max_fresh: int | None):
-        import torch
-
         if head_dim not in HEAD_DIMS:
             raise ValueError(f"head_dim must be one of {HEAD_DIMS}, got {head_dim}")
         if kv_heads < 1 or query_heads < 1 or query_heads % kv_heads:
@@ -150,7 +153,9 @@ class PagePlan:
         self.max_fresh = self.tokens if max_fresh is None else int(max_fresh)
         if self.max_fresh < 1:
             raise ValueError(f"max_fresh must be at least 1, got {max_fresh}")
-        self.device = tables.device
+        self.device, self._index = tables.device, tables._index
+        self.query_shape = torch.Size((self.tokens, query_heads, head_dim))
+        self.kv_shape = torch.Size((self.tokens, kv_heads, head_dim))
 
         def ints(n, dtype=torch.int32):
             return torch.zeros(n, dtype=dtype, device=self.device)
@@ -162,7 +167,7 @@ class PagePlan:
         self.c = _PlanC(tables.requests, self.tokens, self.max_fresh, tables.width, tables.pages,
                         tables.page_tokens, kv_heads, query_heads, head_dim, 1)
         need = ctypes.c_int64(0)
-        _call("grm_b200_paged_scratch_bytes", self.device, ctypes.byref(self.c),
+        _call(_lib.load().grm_b200_paged_scratch_bytes, self._index, ctypes.byref(self.c),
               ctypes.byref(need))
         self.scratch = torch.zeros(need.value, dtype=torch.uint8, device=self.device)
         c = self.c
@@ -173,12 +178,8 @@ class PagePlan:
         c.slots, c.cursor = self.slots.data_ptr(), self.cursor.data_ptr()
         c.status = self.status.data_ptr()
         c.scratch, c.scratch_bytes = self.scratch.data_ptr(), need.value
-        self.planned = False
+        self.planned, self.grow = False, True
         self._ref = ctypes.byref(c)
-
-    @property
-    def grow(self) -> bool:
-        return bool(self.c.grow)
 
     def check(self) -> None:
         """Wait for the plan (and calls that used it) and raise if the step
@@ -196,14 +197,14 @@ class PageTables:
 
     def __init__(self, requests: int, pages: int, width: int, *, page_tokens: int = 64,
                  device="cuda"):
-        import torch
-
         if requests < 1 or pages < 1 or width < 1:
             raise ValueError(f"requests, pages and width must be positive, got "
                              f"{requests}, {pages}, {width}")
         self.requests, self.pages, self.width = int(requests), int(pages), int(width)
         self.page_tokens = _check_page(page_tokens)
         self.device = _device(device)
+        self._index, self._shape = self.device.index, torch.Size((self.requests,))
+        self._plan_step = _lib.load().grm_b200_paged_plan_step
         self.table = torch.full((requests, width), -1, dtype=torch.int32, device=self.device)
         self.lens = torch.zeros(requests, dtype=torch.int32, device=self.device)
         self.ring = torch.arange(pages, dtype=torch.int32, device=self.device)
@@ -221,48 +222,45 @@ class PageTables:
         """Lay out a step: request r brings ``fresh[r]`` new rows (int32 on the
         device).  `grow`: the rows are tokens that join the requests; without
         it they are query rows that only read what is cached."""
-        import torch
-
         if plan.tables is not self:
             raise ValueError("the plan was made for other tables")
-        if (not isinstance(fresh, torch.Tensor) or fresh.dtype != torch.int32 or
-                fresh.device != self.device or fresh.shape != (self.requests,) or
+        if (not isinstance(fresh, torch.Tensor) or fresh.dtype is not torch.int32 or
+                fresh.get_device() != self._index or fresh.shape != self._shape or
                 not fresh.is_contiguous()):
             raise ValueError(f"fresh must be int32 [{self.requests}] on {self.device}")
-        plan.c.grow = 1 if grow else 0
-        _, handle = _stream(stream, self.device, fresh)
-        _call("grm_b200_paged_plan_step", self.device, plan._ref, fresh.data_ptr(), handle)
+        if grow is not plan.grow:
+            plan.grow = bool(grow)
+            plan.c.grow = 1 if grow else 0
+        _call(self._plan_step, self._index, plan._ref, fresh.data_ptr(),
+              _handle(stream, self._index, fresh))
         plan.planned = True
         return plan
 
     def commit(self, plan: PagePlan, *, stream=None) -> None:
         """Take up the lengths of a planned step: requests hold `plan.lens`
         tokens from here on.  The plan stays good for append and attend."""
-        import torch
-
         if plan.tables is not self or not plan.planned:
             raise ValueError("commit takes a plan of these tables that has been planned")
         if not plan.grow:
             return
-        stream, _ = _stream(stream, self.device)
-        with torch.cuda.stream(stream):
-            self.lens.copy_(plan.lens)
-            self.cursor.copy_(plan.cursor)
+        if stream is not None:
+            with torch.cuda.stream(_torch_stream(stream, self._index)):
+                return self.commit(plan)
+        self.lens.copy_(plan.lens)
+        self.cursor.copy_(plan.cursor)
 
     def release(self, rows, *, stream=None) -> None:
         """Return the pages of the requests ``rows`` (int32 on the device) to
         the ring and empty them."""
-        import torch
-
         if (not isinstance(rows, torch.Tensor) or rows.dtype != torch.int32 or rows.dim() != 1 or
                 rows.device != self.device or not rows.is_contiguous()):
             raise ValueError(f"rows must be int32 [n] on {self.device}")
         if rows.numel() == 0:
             return
-        _, handle = _stream(stream, self.device, rows)
-        _call("grm_b200_paged_release", self.device, rows.data_ptr(), rows.numel(), self.requests,
+        _call(_lib.load().grm_b200_paged_release, self._index, rows.data_ptr(), rows.numel(), self.requests,
               self.width, self.pages, self.page_tokens, self.table.data_ptr(),
-              self.lens.data_ptr(), self.ring.data_ptr(), self.cursor.data_ptr(), handle)
+              self.lens.data_ptr(), self.ring.data_ptr(), self.cursor.data_ptr(),
+              _handle(stream, self._index, rows))
 
 
 class PagedArena:
@@ -271,8 +269,6 @@ class PagedArena:
 
     def __init__(self, layers: int, pages: int, kv_heads: int, head_dim: int, *,
                  page_tokens: int = 64, device="cuda"):
-        import torch
-
         if layers < 1 or pages < 1 or kv_heads < 1:
             raise ValueError(f"layers, pages and kv_heads must be positive, got "
                              f"{layers}, {pages}, {kv_heads}")
@@ -292,43 +288,56 @@ class PagedArena:
                            self.k_scales[i].data_ptr(), self.v_scales[i].data_ptr(), pages,
                            kv_heads, page_tokens, head_dim) for i in range(layers)]
         self._refs = [ctypes.byref(c) for c in self._c]
-        self._types = {torch.float16: _lib.GRM_B200_F16, torch.bfloat16: _lib.GRM_B200_BF16}
+        lib = _lib.load()
+        self._index = self.device.index
+        self._append, self._attend = lib.grm_b200_paged_append, lib.grm_b200_paged_attend
+        self._read = lib.grm_b200_paged_read
+        self._scale = 1.0 / math.sqrt(head_dim)
 
-    def _rows(self, plan, name, x, heads):
-        """Checks rows [tokens, heads, head_dim]; returns (type, row and head strides)."""
-        kind = self._types.get(x.dtype)
+    def _rows(self, name, x, shape):
+        """Checks rows of `shape`; returns (type, pointer, row and head strides)."""
+        kind = _TYPES.get(x.dtype)
         if kind is None:
             raise ValueError(f"{name} must be float16 or bfloat16, got {x.dtype}")
-        if x.shape != (plan.tokens, heads, self.head_dim):
-            raise ValueError(f"{name} must be [{plan.tokens}, {heads}, {self.head_dim}], got "
-                             f"{tuple(x.shape)}")
-        if x.device != self.device:
+        if x.shape != shape:
+            raise ValueError(f"{name} must be {list(shape)}, got {list(x.shape)}")
+        if x.get_device() != self._index:
             raise ValueError(f"{name} is on {x.device}, the arena on {self.device}")
         row, head, inner = x.stride()
-        if inner != 1 or row % 8 or head % 8 or x.data_ptr() % 16:
+        ptr = x.data_ptr()
+        if inner != 1 or (row | head) & 7 or ptr & 15:
             raise ValueError(f"{name}: a head's values must be contiguous, rows and heads at "
                              f"multiples of 8 elements and 16-byte aligned (strides {x.stride()})")
-        return kind, row, head
+        return kind, ptr, row, head
 
-    def _plan(self, plan, layer):
-        if not 0 <= layer < self.layers:
-            raise ValueError(f"layer {layer} of {self.layers}")
+    def _ready(self, plan, layer):
+        """The layer's buffers, for a plan that is good for a call."""
         if not plan.planned:
             raise ValueError("the plan has not been planned yet (PageTables.plan)")
+        if not 0 <= layer < self.layers:
+            raise ValueError(f"layer {layer} of {self.layers}")
+        return self._refs[layer]
+
+    def _result(self, name, t, like, shape, dtype, stream):
+        if t is None:
+            return _empty(like, shape, dtype, stream)
+        if (t.shape != shape or t.dtype is not dtype or t.get_device() != self._index or
+                not t.is_contiguous()):
+            raise ValueError(f"{name} must be contiguous {dtype} {list(shape)} on {self.device}")
+        return t
 
     def append(self, plan: PagePlan, k, v, *, layer: int = 0, stream=None) -> None:
         """Quantise the step's rows ``k`` and ``v`` [tokens, kv_heads, head_dim]
         into the pages of `layer`."""
-        self._plan(plan, layer)
-        kind, k_row, k_head = self._rows(plan, "k", k, self.kv_heads)
-        v_kind, v_row, v_head = self._rows(plan, "v", v, self.kv_heads)
+        ref = self._ready(plan, layer)
+        kind, k_ptr, k_row, k_head = self._rows("k", k, plan.kv_shape)
+        v_kind, v_ptr, v_row, v_head = self._rows("v", v, plan.kv_shape)
         if kind != v_kind:
             raise ValueError(f"k and v differ in type: {k.dtype}, {v.dtype}")
-        if not plan.c.grow:
+        if not plan.grow:
             raise ValueError("the plan's rows do not join the arena (planned with grow=False)")
-        _, handle = _stream(stream, self.device, k, v)
-        _call("grm_b200_paged_append", self.device, plan._ref, self._refs[layer], k.data_ptr(),
-              v.data_ptr(), kind, k_row, k_head, v_row, v_head, handle)
+        _call(self._append, self._index, plan._ref, ref, k_ptr, v_ptr, kind, k_row, k_head, v_row,
+              v_head, _handle(stream, self._index, k, v))
 
     def attend(self, plan: PagePlan, q, *, layer: int = 0, causal: bool = True,
                scale: float | None = None, out=None, lse=None, stream=None):
@@ -337,50 +346,38 @@ class PagedArena:
         the positions up to the row's own.  `scale` defaults to
         head_dim ** -0.5.  Returns (out like q, lse fp32 [tokens, query_heads]);
         rows that see nothing are 0 with lse -inf."""
-        import torch
-
-        self._plan(plan, layer)
-        kind, row, head = self._rows(plan, "q", q, plan.query_heads)
-        if causal and not plan.c.grow:
+        ref = self._ready(plan, layer)
+        shape = plan.query_shape
+        kind, ptr, row, head = self._rows("q", q, shape)
+        if causal and not plan.grow:
             raise ValueError("rows that do not join the arena (planned with grow=False) have no "
                              "position in it; attend with causal=False")
-        stream, handle = _stream(stream, self.device, q)
-        shape = (plan.tokens, plan.query_heads, self.head_dim)
-        if out is None:
-            out = _empty(shape, q.dtype, self.device, stream)
-        elif (out.shape != shape or out.dtype != q.dtype or out.device != self.device or
-              not out.is_contiguous()):
-            raise ValueError(f"out must be contiguous {q.dtype} {list(shape)} on {self.device}")
-        if lse is None:
-            lse = _empty(shape[:2], torch.float32, self.device, stream)
-        elif (lse.shape != shape[:2] or lse.dtype != torch.float32 or
-              lse.device != self.device or not lse.is_contiguous()):
-            raise ValueError(f"lse must be contiguous float32 {list(shape[:2])} on {self.device}")
-        _call("grm_b200_paged_attend", self.device, plan._ref, self._refs[layer], q.data_ptr(),
-              kind, row, head, 1.0 / math.sqrt(self.head_dim) if scale is None else float(scale),
-              1 if causal else 0, out.data_ptr(), lse.data_ptr(), handle)
+        out = self._result("out", out, q, shape, q.dtype, stream)
+        lse = self._result("lse", lse, q, shape[:2], torch.float32, stream)
+        _call(self._attend, self._index, plan._ref, ref, ptr, kind, row, head,
+              self._scale if scale is None else float(scale), 1 if causal else 0, out.data_ptr(),
+              lse.data_ptr(), _handle(stream, self._index, q))
         return out, lse
 
     def read(self, slots, *, layer: int = 0, dtype=None, stream=None):
         """Rows of values (k, v) [n, kv_heads, head_dim] of type `dtype`
         (default bfloat16; float16 and float32 too) at ``slots`` int64 [n]; a
         negative slot gives zeros."""
-        import torch
-
         if not 0 <= layer < self.layers:
             raise ValueError(f"layer {layer} of {self.layers}")
-        if (not isinstance(slots, torch.Tensor) or slots.dtype != torch.int64 or
-                slots.dim() != 1 or slots.device != self.device or not slots.is_contiguous()):
+        if (not isinstance(slots, torch.Tensor) or slots.dtype is not torch.int64 or
+                slots.dim() != 1 or slots.get_device() != self._index or
+                not slots.is_contiguous()):
             raise ValueError(f"slots must be int64 [n] on {self.device}")
         dtype = torch.bfloat16 if dtype is None else dtype
-        kind = _lib.GRM_B200_F32 if dtype == torch.float32 else self._types.get(dtype)
+        kind = _READ_TYPES.get(dtype)
         if kind is None:
             raise ValueError(f"read gives float32, float16 or bfloat16, not {dtype}")
-        shape = (slots.numel(), self.kv_heads, self.head_dim)
-        stream, handle = _stream(stream, self.device, slots)
-        k = _empty(shape, dtype, self.device, stream)
-        v = _empty(shape, dtype, self.device, stream)
-        if slots.numel():
-            _call("grm_b200_paged_read", self.device, self._refs[layer], slots.data_ptr(),
-                  slots.numel(), kind, k.data_ptr(), v.data_ptr(), handle)
+        n = slots.numel()
+        shape = (n, self.kv_heads, self.head_dim)
+        k = _empty(slots, shape, dtype, stream)
+        v = _empty(slots, shape, dtype, stream)
+        if n:
+            _call(self._read, self._index, self._refs[layer], slots.data_ptr(), n, kind,
+                  k.data_ptr(), v.data_ptr(), _handle(stream, self._index, slots))
         return k, v
