@@ -18,7 +18,8 @@ __host__ __device__ constexpr int split_tile(int dim) { return dim == 256 ? 64 :
 __host__ __device__ constexpr int split_blocks(int dim, int rows) {
   return dim == 64 || (dim == 128 && rows == 8) ? 3 : 2;
 }
-constexpr int kWorkerSlot = 2048 + 64;  // fp32 of one partial result: rows x dim, then (M, L)
+// fp32 of one partial result: rows x dim, then (reference exponent, sum) a row.
+__host__ __device__ constexpr int split_slot(int dim, int rows) { return rows * dim + 2 * rows; }
 
 struct Header {           // written by the plan kernel
   int32_t units;          // units of the split kernel's work, all requests
@@ -53,7 +54,7 @@ struct Lists {
   unsigned* count;    // [workers] arrivals at the segment that a worker starts; 0 between calls
   int2* pages;        // [page_cap] (request, page of the request)
   int2* qtiles;       // [qtile_cap] (request, first row of the tile within the request)
-  float* part;        // [workers * 2][kWorkerSlot]
+  float* part;        // [workers * 2][split_slot]
 };
 
 inline Lists lists_of(const Shape& s, void* scratch) {
@@ -87,6 +88,7 @@ struct AttendParams {
   const int32_t* starts;
   int64_t width, tokens, pages;
   int page_shift, kv_heads, group, causal, block_rows, qtile_tokens;
+  unsigned group_inv;  // above 2^32 / group: x / group for small x, where group > 1
   const int8_t* k;
   const int8_t* v;
   const float* ks;
@@ -147,7 +149,7 @@ __device__ __forceinline__ void row_scale(unsigned m, float* up, float* down) {
 __device__ __forceinline__ void value_scale(float u, float* log2_u, float* inv_u) {
   const float w = u == 0.0f ? 0x1p-40f : fmaxf(u, 0x1p-100f);
   *log2_u = u != u ? u : __log2f(w);
-  *inv_u = 1.0f / w;
+  *inv_u = __fdividef(1.0f, w);
 }
 // Two bf16 times `up` as halves.
 __device__ __forceinline__ uint32_t scale_pair(uint32_t v, float up) {

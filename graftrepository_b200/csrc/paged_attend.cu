@@ -62,7 +62,7 @@ struct Layout {
   static constexpr int kRow = D + 4;              // floats of a row in the merge buffer
   static constexpr int kRing = kWarps * kStages * kStage;
   static constexpr int kMerge = 2 * 8 * kRow * 4;
-  static constexpr int kScales = kWarps * kStages * 2 * 16;
+  static constexpr int kScales = kWarps * kStages * 2 * 8;
   static constexpr int kML = 2 * kWarps * NT * 8 * 4;
   static constexpr int kSmem = 1024 + kRing + kMerge + kScales + kML;
 };
@@ -101,6 +101,15 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
       : "memory");
 }
 
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+// One of the barrier's arrivals, once this thread's copies above have landed.
+__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar))
+               : "memory");
+}
+
 // Byte of 16-code chunk c of row r in a warp's stage of `rows` rows.  The
 // copies' swizzle (128 bytes; 64 at head_dim 64) puts eight rows of one chunk
 // into eight different bank groups, which ldmatrix reads together; head_dim 256
@@ -114,7 +123,8 @@ __device__ __forceinline__ uint32_t tile_byte(int rows, int r, int c) {
 // A segment: up to block_rows query rows of a kv head of a request.
 struct Segment {
   int first;  // its first unit
-  int request, tiles, len, start, pairs, head, row0, cached;
+  int request, tiles, len, start, pairs, head, cached;
+  int row0, row0_token, row0_head;  // its first row: token, and head of the group
 };
 
 // The share of one worker, walked segment by segment.
@@ -151,6 +161,8 @@ struct Walk {
     s.first = base + i * (s.tiles + 1);
     s.head = i / blocks;
     s.row0 = (i - s.head * blocks) * p.block_rows;
+    s.row0_token = s.row0 / p.group;
+    s.row0_head = s.row0 - s.row0_token * p.group;
     u = s.first + s.tiles + 1;
     t = max(begin - s.first - 1, 0);
     t1 = min(end - s.first - 1, s.tiles);
@@ -158,17 +170,75 @@ struct Walk {
   }
 };
 
+// Row `row` of a segment whose n partial results workers wa, wa + 1, ... left:
+// summed in that order by a warp, and written as packed row `out_row`.  A call
+// of its own, so that its registers are not the tile loop's.
+template <typename T, int D, int ROWS>
+__device__ __noinline__ void join_row(const AttendParams& p, int wa, int n, int row,
+                                      int64_t out_row) {
+  constexpr int kDims = D / 32, kAhead = 8, kSlot = split_slot(D, ROWS);
+  const int lane = threadIdx.x & 31;
+  auto part = [&](int i) {  // the first left the segment unfinished, the others took it up
+    return p.l.part + (2 * (wa + i) + (i == 0 ? 1 : 0)) * (int64_t)kSlot;
+  };
+  auto sums = [&](int i) {  // (reference exponent, sum)
+    return i < n ? __ldcg(reinterpret_cast<const float2*>(part(i) + ROWS * D + 2 * row))
+                 : make_float2(-INFINITY, 0.0f);
+  };
+  float top = -INFINITY;
+  for (int i = lane; i < n; i += 32) top = fmaxf(top, sums(i).x);
+#pragma unroll
+  for (int i = 16; i >= 1; i >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, i));
+  float sum = 0.0f, acc[kDims] = {};
+  for (int i0 = 0; i0 < n; i0 += 32) {
+    const float2 ml = sums(i0 + lane);
+    const float a = ml.x == top ? 1.0f : ex2(ml.x - top);
+    float l = ml.y == 0.0f ? 0.0f : ml.y * a;
+#pragma unroll
+    for (int i = 16; i >= 1; i >>= 1) l += __shfl_xor_sync(kFull, l, i);
+    sum += l;
+    for (int i1 = 0; i1 < 32 && i0 + i1 < n; i1 += kAhead) {
+      float2 v[kAhead][kDims / 2];  // lane: D / 32 neighbouring dims
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const float* src = part(min(i0 + i1 + i, n - 1)) + row * D + kDims * lane;
+#pragma unroll
+        for (int d = 0; d < kDims / 2; ++d) v[i][d] = __ldcg(reinterpret_cast<const float2*>(src) + d);
+      }
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const float w = __shfl_sync(kFull, a, i1 + i);
+        if (i0 + i1 + i < n) {
+#pragma unroll
+          for (int d = 0; d < kDims / 2; ++d) {
+            acc[2 * d] = fmaf(v[i][d].x, w, acc[2 * d]);
+            acc[2 * d + 1] = fmaf(v[i][d].y, w, acc[2 * d + 1]);
+          }
+        }
+      }
+    }
+  }
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+  for (int d = 0; d < kDims / 2; ++d)
+    reinterpret_cast<uint32_t*>(p.out + out_row * D + kDims * lane)[d] =
+        pack_out<T>(acc[2 * d] * inv, acc[2 * d + 1] * inv);
+  if (p.lse && lane == 0)
+    p.lse[out_row] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.693147180559945309f;
+}
+
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kThreads, (Layout<D, NT>::kBlocks))
     split_kernel(const __grid_constant__ SplitParams sp) {
   using LY = Layout<D, NT>;
   constexpr int kChunks = D / 16;
   constexpr int kTokens = LY::kTokens, kB = LY::kBlocks16;
+  constexpr int kSums = NT * 8 * D, kSlot = split_slot(D, NT * 8);  // of a partial result
   const AttendParams& p = sp.a;
   extern __shared__ unsigned char raw_smem[];
   unsigned char* const smem = raw_smem + ((1024u - (smem_u32(raw_smem) & 1023u)) & 1023u);
   float* const merge = reinterpret_cast<float*>(smem + LY::kRing);
-  float4* const scales = reinterpret_cast<float4*>(smem + LY::kRing + LY::kMerge);
+  float2* const scales = reinterpret_cast<float2*>(smem + LY::kRing + LY::kMerge);
   float* const sm_m = reinterpret_cast<float*>(smem + LY::kRing + LY::kMerge + LY::kScales);
   float* const sm_l = sm_m + kWarps * NT * 8;
   __shared__ __align__(8) uint64_t bars[kWarps][LY::kStages];
@@ -189,23 +259,54 @@ __global__ void __launch_bounds__(kThreads, (Layout<D, NT>::kBlocks))
       for (int x = threadIdx.x; x < heads; x += kThreads) p.lse[i * heads + x] = -INFINITY;
   }
   if (w >= hd.workers) return;
+  const int begin = worker_first(w, hd), end = worker_first(w + 1, hd);
+  Walk<LY::kTokens * kWarps> walk(p, begin, end, request0);
+  bool more;
+
+  // ---- queries of a segment: column g of the B operand, dims 16c + 4 t4 .. + 3
+  uint2 raw[NT][kChunks];
+  // packed row and head of row `x` of a segment (a block's rows are few, so the
+  // division by the group is a multiplication)
+  auto pair_of = [&](const Segment& s, int x, int* token, int* head) {
+    const int j = s.row0_head + x;
+    const int q = p.group == 1 ? j : (int)__umulhi(j, p.group_inv);
+    *token = s.row0_token + q;
+    *head = s.head * p.group + j - q * p.group;
+  };
+  auto fetch_queries = [&](const Segment& s) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const bool there = s.row0 + nt * 8 + g < s.pairs;
+      int token, head;
+      pair_of(s, nt * 8 + g, &token, &head);
+      const uint16_t* qp = p.q + (int64_t)(s.start + token) * p.q_row + (int64_t)head * p.q_head +
+                           t4 * 4;
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c)
+        raw[nt][c] = there ? __ldg(reinterpret_cast<const uint2*>(qp + c * 16))
+                           : make_uint2(0, 0);
+    }
+  };
+  auto next_segment = [&]() {
+    more = walk.next();
+    if (more) fetch_queries(walk.s);
+  };
+  next_segment();
+
   if (lane == 0) {
-    for (int i = 0; i < LY::kStages; ++i) mbar_init(&bars[warp][i], 1);
+    for (int i = 0; i < LY::kStages; ++i) mbar_init(&bars[warp][i], 2);
     mbar_fence_init();
   }
   if (threadIdx.x == 0) sm_fail = 0;
   __syncthreads();
-  const int begin = worker_first(w, hd), end = worker_first(w + 1, hd);
 
   // ---- the loader: this warp's tokens of a tile, one stage at a time
   const uint32_t ring = smem_u32(smem) + warp * LY::kStages * LY::kStage;
-  float4* const ring_scales = scales + warp * LY::kStages * 2;
-  Walk<LY::kTokens * kWarps> load(p, begin, end, request0);
+  const float2* const ring_scales = scales + warp * LY::kStages * 2;
+  Walk<LY::kTokens * kWarps> load = walk;
   int issued = 0, used = 0;        // stages
-  // Lane i: page ids_base + i of request and head, its key scale, log2 and inverse
-  // of its value scale; and the page 32 further on.
-  int ids = 0, ids_ahead = 0, ids_base = 0, ids_first = -1;
-  float l_key = 0.0f, l_log = 0.0f, l_inv = 0.0f;
+  // lane i: page ids_base + i of the request, and the page 32 further on
+  int ids = 0, ids_ahead = 0, ids_base = 0, ids_request = -1;
   auto issue = [&]() {
     int tok = 0;
     for (;;) {  // the next tile of the share with tokens for this warp
@@ -216,31 +317,21 @@ __global__ void __launch_bounds__(kThreads, (Layout<D, NT>::kBlocks))
     }
     const Segment& s = load.s;
     const int j = tok >> p.page_shift;
-    if (s.first != ids_first || j >= ids_base + 32) {
+    if (s.request != ids_request || j >= ids_base + 32 || j < ids_base) {
       const int last = (s.len - 1) >> p.page_shift;
       const int32_t* row = p.table + s.request * p.width;
-      const bool follows = s.first == ids_first && j == ids_base + 32;
+      const bool follows = s.request == ids_request && j == ids_base + 32;
       ids = follows ? ids_ahead : __ldg(row + min(j + lane, last));
       ids = min(max(ids, 0), (int)p.pages - 1);
       ids_ahead = __ldg(row + min(j + 32 + lane, last));
       ids_base = j;
-      ids_first = s.first;
-      const int64_t at = (int64_t)ids * p.kv_heads + s.head;
-      l_key = __ldg(p.ks + at);
-      value_scale(__ldg(p.vs + at), &l_log, &l_inv);
+      ids_request = s.request;
     }
     const int stage = issued % LY::kStages;
     ++issued;
     const int per = 1 << p.page_shift;
     const int rows = min(per, kTokens);  // of one copy
     uint64_t* bar = &bars[warp][stage];
-#pragma unroll
-    for (int b = 0; b < kB; ++b) {  // scales of 16 tokens
-      const int from = ((tok + 16 * b) >> p.page_shift) - ids_base;
-      const float key = __shfl_sync(kFull, l_key, from), lg = __shfl_sync(kFull, l_log, from);
-      const float inv = __shfl_sync(kFull, l_inv, from);
-      if (lane == 0) ring_scales[stage * 2 + b] = make_float4(key, lg, inv, 0.0f);
-    }
     const int page0 = __shfl_sync(kFull, ids, j - ids_base);
     const int page1 = __shfl_sync(kFull, ids, min(j + 1 - ids_base, 31));
     if (lane == 0) {
@@ -250,17 +341,26 @@ __global__ void __launch_bounds__(kThreads, (Layout<D, NT>::kBlocks))
       mbar_arrive_expect_tx(bar, (both ? 2 : 1) * 2 * rows * D);
       const uint32_t to = ring + stage * LY::kStage;
       const int y = tok & (per - 1);
+      const int z0 = page0 * p.kv_heads + s.head;
+      const int z1 = both ? page1 * p.kv_heads + s.head : z0;
 #pragma unroll
       for (int x = 0; x < D; x += 128) {
         const uint32_t at = to + (x / 128) * kTokens * 128;
-        tma_load_3d(at, &sp.k_map, x, y, page0 * p.kv_heads + s.head, bar);
-        tma_load_3d(at + LY::kSide, &sp.v_map, x, y, page0 * p.kv_heads + s.head, bar);
+        tma_load_3d(at, &sp.k_map, x, y, z0, bar);
+        tma_load_3d(at + LY::kSide, &sp.v_map, x, y, z0, bar);
         if (both) {
           const uint32_t at1 = at + rows * (D < 128 ? D : 128);
-          tma_load_3d(at1, &sp.k_map, x, 0, page1 * p.kv_heads + s.head, bar);
-          tma_load_3d(at1 + LY::kSide, &sp.v_map, x, 0, page1 * p.kv_heads + s.head, bar);
+          tma_load_3d(at1, &sp.k_map, x, 0, z1, bar);
+          tma_load_3d(at1 + LY::kSide, &sp.v_map, x, 0, z1, bar);
         }
       }
+#pragma unroll
+      for (int b = 0; b < kB; ++b) {  // scales of 16 tokens
+        const uint32_t f = smem_u32(ring_scales + stage * 2 + b);
+        cp_async4(f, p.ks + (b ? z1 : z0));
+        cp_async4(f + 4, p.vs + (b ? z1 : z0));
+      }
+      cp_async_arrive(bar);
     }
   };
 #pragma unroll 1
@@ -274,15 +374,17 @@ __global__ void __launch_bounds__(kThreads, (Layout<D, NT>::kBlocks))
   constexpr uint32_t kNext16 = 16 * (D < 128 ? D : 128);  // bytes from 16 rows to the next
 
   bool failed = false;
-  Walk<LY::kTokens * kWarps> walk(p, begin, end, request0);
-  while (walk.next()) {
+  for (; more; next_segment()) {
     const Segment s = walk.s;
     const int rows = min(s.pairs - s.row0, NT * 8);
+    auto out_row = [&](int x) {  // of row x of the segment
+      int token, head;
+      pair_of(s, x, &token, &head);
+      return (int64_t)(s.start + token) * heads + head;
+    };
     if (s.tiles == 0) {  // nothing cached: empty rows (the segment is its one unit)
       for (int x = threadIdx.x; x < rows * (D / 2); x += kThreads) {
-        const int j = s.row0 + x / (D / 2);
-        const int64_t row = (int64_t)(s.start + j / p.group) * heads + s.head * p.group +
-                            j % p.group;
+        const int64_t row = out_row(x / (D / 2));
         reinterpret_cast<uint32_t*>(p.out + row * D)[x % (D / 2)] = 0;
         if (p.lse && x % (D / 2) == 0) p.lse[row] = -INFINITY;
       }
@@ -290,55 +392,41 @@ __global__ void __launch_bounds__(kThreads, (Layout<D, NT>::kBlocks))
     }
     if (walk.t >= walk.t1) continue;  // only its start is this worker's
 
-    // ---- queries: column g of the B operand, dims 16c + 4 t4 .. + 3
     uint32_t qf[kChunks][NT][2];
     float kq[NT][2];
     int lim[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int j = s.row0 + nt * 8 + g;
-      uint2 raw[kChunks];
-#pragma unroll
-      for (int c = 0; c < kChunks; ++c) raw[c] = make_uint2(0, 0);
-      if (j < s.pairs) {
-        const uint16_t* qp = p.q + (int64_t)(s.start + j / p.group) * p.q_row +
-                             (int64_t)(s.head * p.group + j % p.group) * p.q_head + t4 * 4;
-#pragma unroll
-        for (int c = 0; c < kChunks; ++c)
-          raw[c] = __ldg(reinterpret_cast<const uint2*>(qp + c * 16));
-      }
-      float unscale = 1.0f;
+      float up = 1.0f, unscale = 1.0f;
       if constexpr (!std::is_same<T, __half>::value) {
         unsigned m = 0;
 #pragma unroll
         for (int c = 0; c < kChunks; ++c)
-          m = __vmaxu2(m, __vmaxu2(raw[c].x & 0x7FFF7FFFu, raw[c].y & 0x7FFF7FFFu));
+          m = __vmaxu2(m, __vmaxu2(raw[nt][c].x & 0x7FFF7FFFu, raw[nt][c].y & 0x7FFF7FFFu));
         m = max(m & 0xFFFFu, m >> 16);
         m = max(m, __shfl_xor_sync(kFull, m, 1));
         m = max(m, __shfl_xor_sync(kFull, m, 2));
-        float up;
         row_scale(m, &up, &unscale);
+      }
 #pragma unroll
-        for (int c = 0; c < kChunks; ++c) {
-          qf[c][nt][0] = scale_pair(raw[c].x, up);
-          qf[c][nt][1] = scale_pair(raw[c].y, up);
-        }
-      } else {
-#pragma unroll
-        for (int c = 0; c < kChunks; ++c) {
-          qf[c][nt][0] = raw[c].x;
-          qf[c][nt][1] = raw[c].y;
-        }
+      for (int c = 0; c < kChunks; ++c) {
+        uint2 f = raw[nt][c];
+        if constexpr (!std::is_same<T, __half>::value)
+          f = make_uint2(scale_pair(f.x, up), scale_pair(f.y, up));
+        qf[c][nt][0] = f.x;
+        qf[c][nt][1] = f.y;
       }
       // columns 2 t4 and 2 t4 + 1 of the scores
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         kq[nt][x] = p.scale_log2 * __shfl_sync(kFull, unscale, (2 * t4 + x) * 4);
-        const int jc = s.row0 + nt * 8 + 2 * t4 + x;
-        lim[nt][x] = p.causal && jc < s.pairs ? s.cached + jc / p.group + 1 : s.len;
+        int token, head;
+        pair_of(s, nt * 8 + 2 * t4 + x, &token, &head);
+        lim[nt][x] = p.causal && s.row0 + nt * 8 + 2 * t4 + x < s.pairs ? s.cached + token + 1
+                                                                       : s.len;
       }
     }
-    const int all_see = p.causal ? s.cached + s.row0 / p.group + 1 : s.len;
+    const int all_see = p.causal ? s.cached + s.row0_token + 1 : s.len;
 
     float o[kChunks][NT][4];
     float m[NT][2], l[NT][2];
@@ -403,13 +491,14 @@ __global__ void __launch_bounds__(kThreads, (Layout<D, NT>::kBlocks))
       float inv[kB];
 #pragma unroll
       for (int b = 0; b < kB; ++b) {
-        const float4 f = ring_scales[stage * 2 + b];
-        inv[b] = f.z;
+        const float2 f = ring_scales[stage * 2 + b];
+        float log2_u;
+        value_scale(f.y, &log2_u, &inv[b]);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
-            sc[b][nt][x] = fmaf(sc[b][nt][x], kq[nt][x & 1] * f.x, f.y);
+            sc[b][nt][x] = fmaf(sc[b][nt][x], kq[nt][x & 1] * f.x, log2_u);
           }
         }
       }
@@ -574,10 +663,8 @@ __global__ void __launch_bounds__(kThreads, (Layout<D, NT>::kBlocks))
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
-            const int j = s.row0 + nt * 8 + 2 * t4 + x;
-            if (j < s.pairs) {
-              const int64_t row = (int64_t)(s.start + j / p.group) * heads + s.head * p.group +
-                                  j % p.group;
+            if (s.row0 + nt * 8 + 2 * t4 + x < s.pairs) {
+              const int64_t row = out_row(nt * 8 + 2 * t4 + x);
               const float sum = lt[nt][x];
               const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
@@ -595,7 +682,7 @@ __global__ void __launch_bounds__(kThreads, (Layout<D, NT>::kBlocks))
 
     // ---- shared: leave the partial result; the last worker joins them
     if (warp == 0) {
-      float* slot = p.l.part + (2 * w + (w == wa ? 1 : 0)) * (int64_t)kWorkerSlot;
+      float* slot = p.l.part + (2 * w + (w == wa ? 1 : 0)) * (int64_t)kSlot;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -606,54 +693,25 @@ __global__ void __launch_bounds__(kThreads, (Layout<D, NT>::kBlocks))
             *reinterpret_cast<float2*>(slot + row * D + 16 * c + 2 * g) =
                 make_float2(o[c][nt][x], o[c][nt][x + 2]);
           if (g == 0)
-            *reinterpret_cast<float2*>(slot + 2048 + 2 * row) = make_float2(m[nt][x], lt[nt][x]);
+            *reinterpret_cast<float2*>(slot + kSums + 2 * row) = make_float2(m[nt][x], lt[nt][x]);
         }
-      __threadfence();
       __syncwarp();
-      if (lane == 0) {
-        const unsigned arrived = atomicAdd(p.l.count + wa, 1u);
+      if (lane == 0) {  // releases the warp's stores, acquires the other workers'
+        unsigned arrived;
+        asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;"
+                     : "=r"(arrived)
+                     : "l"(p.l.count + wa)
+                     : "memory");
         const int last = arrived + 1 == (unsigned)(wb - wa + 1);
         if (last) p.l.count[wa] = 0;  // for the next call
         sm_last = last;
-        __threadfence();
       }
     }
     __syncthreads();
     if (sm_last) {
-      const int n = (int)(wb - wa + 1);
-      auto part = [&](int i) {
-        return p.l.part + (2 * (wa + i) + (i == 0 ? 1 : 0)) * (int64_t)kWorkerSlot;
-      };
-      for (int row = warp; row < rows; row += kWarps) {  // a warp takes a row
-        float top = -INFINITY;
-        for (int i = lane; i < n; i += 32) top = fmaxf(top, __ldcg(part(i) + 2048 + 2 * row));
-#pragma unroll
-        for (int i = 16; i >= 1; i >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, i));
-        float sum = 0.0f, acc[D / 32] = {};
-#pragma unroll 4
-        for (int i = 0; i < n; ++i) {
-          const float* src = part(i);
-          const float2 ml = __ldcg(reinterpret_cast<const float2*>(src + 2048 + 2 * row));
-          const float a = ml.x == top ? 1.0f : ex2(ml.x - top);
-          sum += ml.y == 0.0f ? 0.0f : ml.y * a;
-#pragma unroll
-          for (int d = 0; d < D / 64; ++d) {
-            const float2 v = __ldcg(reinterpret_cast<const float2*>(src + row * D + 64 * d + 2 * lane));
-            acc[2 * d] = fmaf(v.x, a, acc[2 * d]);
-            acc[2 * d + 1] = fmaf(v.y, a, acc[2 * d + 1]);
-          }
-        }
-        const int j = s.row0 + row;
-        const int64_t orow = (int64_t)(s.start + j / p.group) * heads + s.head * p.group +
-                             j % p.group;
-        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-#pragma unroll
-        for (int d = 0; d < D / 64; ++d)
-          *reinterpret_cast<uint32_t*>(p.out + orow * D + 64 * d + 2 * lane) =
-              pack_out<T>(acc[2 * d] * inv, acc[2 * d + 1] * inv);
-        if (p.lse && lane == 0)
-          p.lse[orow] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.693147180559945309f;
-      }
+#pragma unroll 1
+      for (int row = warp; row < rows; row += kWarps)  // a warp takes a row
+        join_row<T, D, NT * 8>(p, wa, wb - wa + 1, row, out_row(row));
     }
   }
   if (failed) {  // copies still in flight end before the block does
@@ -668,7 +726,6 @@ __global__ void __launch_bounds__(kThreads, (Layout<D, NT>::kBlocks))
 template <typename T, int D, int NT>
 int launch_split(const SplitParams& p, int workers, cudaStream_t st) {
   using LY = Layout<D, NT>;
-  static_assert(NT * 8 * D <= 2048, "a partial result fits its slot");
   static_assert((LY::kSmem + 2048) * LY::kBlocks <= 228 * 1024, "blocks of an SM");
   auto kernel = split_kernel<T, D, NT>;
   static std::atomic<uint64_t> done{0};
@@ -783,6 +840,7 @@ int grm_b200_paged_attend(const grm_b200_paged_plan* plan, const grm_b200_paged_
   p.page_shift = shift_of(plan->page_tokens);
   p.kv_heads = plan->kv_heads;
   p.group = s.group;
+  p.group_inv = (unsigned)(((uint64_t)1 << 32) / s.group) + 1;
   p.causal = causal ? 1 : 0;
   p.block_rows = s.block_rows;
   p.k = arena->k_codes;

@@ -26,16 +26,17 @@ namespace {
 
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanWarps = kPlanThreads / 32;
+constexpr int kJoinUnits = 5;
 // The sums over requests: pages taken, rows, pages touched, prompt tiles (all
 // of them below 2^31 in a step that can be planned) and the split kernel's units.
-constexpr int kSums = 5;
+constexpr int kSums = 6;
 constexpr int kTake = 0, kRows = 1, kTouched = 2, kTiles = 3, kUnits = 4;
+constexpr int kSegments = 5;  // of the split kernel; only their number is needed
 
 struct PlanParams {
   int64_t requests, tokens, max_fresh, width, ring_size;
   int page_shift, grow, kv_heads;
   Shape s;
-  int min_units;
   const int32_t* cached;
   const int32_t* fresh;
   const int32_t* ring;
@@ -57,15 +58,14 @@ struct Request {
 
 // What request r adds to each sum.
 __device__ __forceinline__ void weigh(const PlanParams& p, const Request& q, int64_t (&v)[kSums]) {
-  v[0] = q.need - q.have;
-  v[1] = q.fresh;
-  v[2] = p.grow && q.fresh > 0 ? q.need - (q.cached >> p.page_shift) : 0;
+  v[kTake] = q.need - q.have;
+  v[kRows] = q.fresh;
+  v[kTouched] = p.grow && q.fresh > 0 ? q.need - (q.cached >> p.page_shift) : 0;
   const int64_t pairs = (int64_t)q.fresh * p.s.group;
   const bool prompt = pairs > p.s.split_rows;
-  v[3] = prompt ? ceil_div64(q.fresh, p.s.qtile_tokens) : 0;
-  v[4] = prompt ? 0
-                : p.kv_heads * ceil_div64(pairs, p.s.block_rows) *
-                      (ceil_div64(q.after, p.s.tile) + 1);
+  v[kTiles] = prompt ? ceil_div64(q.fresh, p.s.qtile_tokens) : 0;
+  v[kSegments] = prompt ? 0 : p.kv_heads * ceil_div64(pairs, p.s.block_rows);
+  v[kUnits] = v[kSegments] * (ceil_div64(q.after, p.s.tile) + 1);
 }
 
 __device__ __forceinline__ int64_t warp_sum(int64_t v) {
@@ -158,8 +158,13 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
   if (total[kUnits] > INT32_MAX - (1 << 20)) failed |= GRM_B200_PLAN_ROWS;
   const int units = failed ? 0 : (int)total[kUnits];
   const int all_rows = failed ? 0 : (int)total[kRows];
-  // Few units: fewer workers, so that none gets less than min_units of them.
-  const int most = (units + p.min_units - 1) / p.min_units;
+  // Few units: fewer workers.  Joining a segment costs about what kJoinUnits
+  // tiles cost, so a step whose segments are no longer than that leaves them
+  // whole; longer ones are split down to two units a worker.
+  const int mean = failed || units == 0 ? 1 : (int)((units + total[kSegments] - 1) /
+                                                    total[kSegments]);
+  const int least = mean <= kJoinUnits ? (mean > 2 ? mean : 2) : 2;
+  const int most = (units + least - 1) / least;
   const int workers = most < p.s.workers ? most : p.s.workers;
 
   if (gid == 0) {
@@ -361,7 +366,7 @@ int make_shape(const grm_b200_paged_plan& p, int sms, Shape* s) {
   s->off_count = take((int64_t)s->workers * 4);
   s->off_pages = take(std::min(T, T / p.page_tokens + 2 * std::min(R, T)) * 8);
   s->off_qtiles = take(s->qtile_cap * 8);
-  s->off_part = take((int64_t)s->workers * 2 * kWorkerSlot * 4);
+  s->off_part = take((int64_t)s->workers * 2 * split_slot(p.head_dim, s->block_rows) * 4);
   s->bytes = at;
   return 0;
 }
@@ -542,7 +547,6 @@ int grm_b200_paged_plan_step(const grm_b200_paged_plan* plan, const int32_t* fre
   p.grow = plan->grow ? 1 : 0;
   p.kv_heads = plan->kv_heads;
   make_shape(*plan, sms, &p.s);
-  p.min_units = 2;
   p.cached = plan->cached;
   p.fresh = fresh_device;
   p.ring = plan->ring;
