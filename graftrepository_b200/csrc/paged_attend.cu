@@ -452,14 +452,17 @@ __global__ void __launch_bounds__(kThreads, (Layout<D, NT>::kBlocks))
       ++used;
       __syncwarp();
       const uint32_t kb = ring + stage * LY::kStage;
-      // scores of kB x 16 tokens x 8 NT rows
-      float sc[kB][NT][4];
+      // scores of kB x 16 tokens x 8 NT rows, two chains of products at least
+      constexpr int kChains = kB == 1 ? 2 : 1;
+      float sum[kChains][kB][NT][4];
 #pragma unroll
-      for (int b = 0; b < kB; ++b)
+      for (int i = 0; i < kChains; ++i)
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int b = 0; b < kB; ++b)
 #pragma unroll
-          for (int x = 0; x < 4; ++x) sc[b][nt][x] = 0.0f;
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) sum[i][b][nt][x] = 0.0f;
       // (fragments one step ahead of their use)
       uint32_t fr[2][kB][4];
 #pragma unroll
@@ -483,12 +486,12 @@ __global__ void __launch_bounds__(kThreads, (Layout<D, NT>::kBlocks))
             const uint32_t a1 = halves(hi, 0x4140), a3 = halves(hi, 0x4342);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
-              mma(sc[b][nt], a0, a1, a2, a3, qf[c + x][nt][0], qf[c + x][nt][1]);
+              mma(sum[x % kChains][b][nt], a0, a1, a2, a3, qf[c + x][nt][0], qf[c + x][nt][1]);
           }
         }
       }
       bool moves = false;
-      float inv[kB];
+      float sc[kB][NT][4], inv[kB];
 #pragma unroll
       for (int b = 0; b < kB; ++b) {
         const float2 f = ring_scales[stage * 2 + b];
@@ -498,7 +501,8 @@ __global__ void __launch_bounds__(kThreads, (Layout<D, NT>::kBlocks))
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
-            sc[b][nt][x] = fmaf(sc[b][nt][x], kq[nt][x & 1] * f.x, log2_u);
+            const float z = sum[0][b][nt][x] + (kChains == 2 ? sum[kChains - 1][b][nt][x] : 0.0f);
+            sc[b][nt][x] = fmaf(z, kq[nt][x & 1] * f.x, log2_u);
           }
         }
       }
