@@ -52,7 +52,7 @@ struct Lists {
   int32_t* base;      // [requests + 1] first unit of each request
   int32_t* start;     // [workers] request of a worker's first unit
   unsigned* count;    // [workers] arrivals at the segment that a worker starts; 0 between calls
-  int2* pages;        // [page_cap] (request, page of the request)
+  int4* pages;        // [page_cap] (first packed row, page, older tokens in it, new rows)
   int2* qtiles;       // [qtile_cap] (request, first row of the tile within the request)
   float* part;        // [workers * 2][split_slot]
 };
@@ -63,7 +63,7 @@ inline Lists lists_of(const Shape& s, void* scratch) {
           reinterpret_cast<int32_t*>(b + s.off_base),
           reinterpret_cast<int32_t*>(b + s.off_start),
           reinterpret_cast<unsigned*>(b + s.off_count),
-          reinterpret_cast<int2*>(b + s.off_pages),
+          reinterpret_cast<int4*>(b + s.off_pages),
           reinterpret_cast<int2*>(b + s.off_qtiles),
           reinterpret_cast<float*>(b + s.off_part)};
 }

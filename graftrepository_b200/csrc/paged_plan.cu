@@ -272,8 +272,14 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
     }
     for (int64_t x = sum[kTouched][0] + (int64_t)gid; x < sum[kTouched][n]; x += gsize) {
       const int i = find(sum[kTouched], n, (int)x);
-      p.l.pages[x] = make_int2((int)(r0 + i), (s_cached[i] >> p.page_shift) +
-                                                  ((int)x - sum[kTouched][i]));
+      const int j = (s_cached[i] >> p.page_shift) + ((int)x - sum[kTouched][i]);
+      const int first = j << p.page_shift, off = max(s_cached[i] - first, 0);
+      const int after = s_cached[i] + sum[kRows][i + 1] - sum[kRows][i];
+      p.l.pages[x] = make_int4(
+          sum[kRows][i] + first + off - s_cached[i],
+          j < s_have[i] ? p.table[(r0 + i) * p.width + j]
+                        : ring_page((int64_t)sum[kTake][i] + j - s_have[i]),
+          off, min(after - first, page) - off);
     }
     for (int64_t x = sum[kTiles][0] + (int64_t)gid; x < sum[kTiles][n]; x += gsize) {
       const int i = find(sum[kTiles], n, (int)x);
@@ -364,7 +370,7 @@ int make_shape(const grm_b200_paged_plan& p, int sms, Shape* s) {
   s->off_base = take((R + 1) * 4);
   s->off_start = take((int64_t)s->workers * 4);
   s->off_count = take((int64_t)s->workers * 4);
-  s->off_pages = take(std::min(T, T / p.page_tokens + 2 * std::min(R, T)) * 8);
+  s->off_pages = take(std::min(T, T / p.page_tokens + 2 * std::min(R, T)) * 16);
   s->off_qtiles = take(s->qtile_cap * 8);
   s->off_part = take((int64_t)s->workers * 2 * split_slot(p.head_dim, s->block_rows) * 4);
   s->bytes = at;
