@@ -371,9 +371,9 @@ int make_shape(const grm_b200_paged_plan& p, int sms, Shape* s) {
   s->group = p.query_heads / p.kv_heads;
   const int64_t most = std::min(p.max_fresh, p.tokens) * s->group;
   s->block_rows = most <= 8 || p.head_dim == 256 ? 8 : 16;
-  const bool prompts = p.head_dim <= 128 && most > kPromptRows;
+  const bool prompts = most > kPromptRows;
   s->split_rows = prompts ? kPromptRows : INT32_MAX;
-  s->qtile_tokens = 2 * (128 / s->group);
+  s->qtile_tokens = (p.head_dim == 256 ? 1 : 2) * (128 / s->group);
   s->tile = split_tile(p.head_dim);
   s->workers = sms * split_blocks(p.head_dim, s->block_rows);
   const int64_t R = p.requests, T = p.tokens;

@@ -40,28 +40,34 @@ namespace paged {
 namespace {
 
 constexpr int kM = 128;             // rows of a query tile
-constexpr int kN = 128;             // tokens of a key tile
-constexpr int kHalf = kN / 2;       // tokens of one softmax step
-constexpr int kSoftWarps = 8;
-constexpr int kConvWarps = 4;
-constexpr int kMmaWarp = kSoftWarps + kConvWarps;
-constexpr int kLoadWarp = kMmaWarp + 2;
-constexpr int kPromptThreads = (kLoadWarp + 1) * 32;
-constexpr int kScaleRing = 4;       // key tiles whose scales are held
+constexpr int kHalf = 64;           // tokens of one softmax step
+constexpr int kQueryAtom = kM * 128;  // 128 rows x 64 halves
+constexpr int kPromptThreads = 15 * 32;
+constexpr int kMmaWarp = 12, kLoadWarp = 14;
 constexpr uint32_t kTmemCols = 512;
 constexpr unsigned kProbes = 1u << 18;  // probes of a bounded wait
 
+// Two query tiles and key tiles of 128 tokens, in two steps of the softmax; at
+// head_dim 256, whose results alone take half of tensor memory, one query tile
+// and key tiles of one step, and the other tile's softmax warps convert codes.
 template <int D>
 struct PromptLayout {
-  static constexpr int kAtom = kN * 128;            // 128 rows x 64 halves
-  static constexpr int kTile = (D / 64) * kAtom;    // a query, key or value tile
-  static constexpr int kRaw = kN * D;               // its codes
-  static constexpr int kUsed = 1024 + 6 * kTile + 2 * kRaw + kScaleRing * 8 * 16;
+  static constexpr int kQueries = D == 256 ? 1 : 2;     // query tiles
+  static constexpr int kN = D == 256 ? 64 : 128;        // tokens of a key tile
+  static constexpr int kHalves = kN / kHalf;
+  static constexpr int kSoftWarps = 4 * kQueries;
+  static constexpr int kConvWarps = kMmaWarp - kSoftWarps;
+  static constexpr int kRing = 8 / kHalves;             // key tiles whose scales are held
+  static constexpr int kQuery = (D / 64) * kQueryAtom;  // a query tile
+  static constexpr int kAtom = kN * 128;                // kN rows x 64 halves
+  static constexpr int kTile = (D / 64) * kAtom;        // a key or value tile
+  static constexpr int kRaw = kN * D;                   // its codes
+  static constexpr int kUsed = 1024 + kQueries * kQuery + 4 * kTile + 2 * kRaw + 32 * 16;
   // one block an SM: it owns all of tensor memory
   static constexpr int kSmem = kUsed > 120 * 1024 ? kUsed : 120 * 1024;
-  static constexpr uint32_t kScore = 0;             // tensor memory columns
-  static constexpr uint32_t kResult = 2 * kN;
-  static_assert(2 * kN + 2 * D <= kTmemCols, "two score and two result tiles");
+  static constexpr uint32_t kScore = 0;                 // tensor memory columns
+  static constexpr uint32_t kResult = kQueries * 2 * kHalf;
+  static_assert(kResult + kQueries * D <= kTmemCols, "score and result tiles");
 };
 
 // fp32 accumulators, fp16 operands, 128 rows, N columns; B K-major or (bit 16) not.
@@ -106,15 +112,16 @@ struct Scale {
 template <typename T, int D>
 __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendParams p) {
   using LY = PromptLayout<D>;
+  constexpr int kN = LY::kN, kHalves = LY::kHalves, kRing = LY::kRing;
   extern __shared__ unsigned char raw[];
   unsigned char* const sm = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
-  unsigned char* const sm_q = sm;                       // [2]
-  unsigned char* const sm_k = sm + 2 * LY::kTile;       // [2]
-  unsigned char* const sm_v = sm + 4 * LY::kTile;       // [2]
-  unsigned char* const sm_raw = sm + 6 * LY::kTile;     // codes: keys, values
-  Scale* const sm_scale = reinterpret_cast<Scale*>(sm_raw + 2 * LY::kRaw);  // [kScaleRing][8]
+  unsigned char* const sm_q = sm;                                     // [kQueries]
+  unsigned char* const sm_k = sm + LY::kQueries * LY::kQuery;         // [2]
+  unsigned char* const sm_v = sm_k + 2 * LY::kTile;                   // [2]
+  unsigned char* const sm_raw = sm_v + 2 * LY::kTile;                 // codes: keys, values
+  Scale* const sm_scale = reinterpret_cast<Scale*>(sm_raw + 2 * LY::kRaw);  // [kRing][kN / 16]
   __shared__ __align__(8) uint64_t q_full[2], drained[2], k_full[2], k_empty[2], v_full[2], v_empty[2],
-      scale_full[kScaleRing], raw_full[2], raw_empty[2], s_full[2][2], p_full[2][2], o_full[2], o_done[2];
+      scale_full[kRing], raw_full[2], raw_empty[2], s_full[2][2], p_full[2][2], o_full[2], o_done[2];
   __shared__ uint32_t sh_tmem;
   __shared__ int sh_fail;
 
@@ -130,9 +137,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
   const int n = p.starts[tile.x + 1] - start;
   const int len = p.lens[tile.x];
   const int cached = len - n;
-  const int per = p.qtile_tokens >> 1;  // tokens of one query tile
+  const int per = p.qtile_tokens / LY::kQueries;  // tokens of one query tile
   const int tok0 = tile.y;
-  const int toks[2] = {min(per, n - tok0), max(0, min(per, n - tok0 - per))};
+  const int toks[2] = {min(per, n - tok0),
+                       LY::kQueries == 2 ? max(0, min(per, n - tok0 - per)) : 0};
   const bool two = toks[1] > 0;
   const int heads = p.kv_heads * p.group;
   const int sees = p.causal ? min(len, cached + tok0 + toks[0] + toks[1]) : len;
@@ -151,22 +159,22 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&q_full[i], kSoftWarps / 2);
+      mbar_init(&q_full[i], 4);
       mbar_init(&drained[i], 1);
-      mbar_init(&k_full[i], kConvWarps);
+      mbar_init(&k_full[i], LY::kConvWarps);
       mbar_init(&k_empty[i], two ? 2 : 1);
-      mbar_init(&v_full[i], kConvWarps);
+      mbar_init(&v_full[i], LY::kConvWarps);
       mbar_init(&v_empty[i], two ? 2 : 1);
       mbar_init(&raw_full[i], 1);
-      mbar_init(&raw_empty[i], kConvWarps);
+      mbar_init(&raw_empty[i], LY::kConvWarps);
       for (int x = 0; x < 2; ++x) {
         mbar_init(&s_full[i][x], 1);
-        mbar_init(&p_full[i][x], kSoftWarps / 2);
+        mbar_init(&p_full[i][x], 4);
       }
       mbar_init(&o_full[i], 1);
       mbar_init(&o_done[i], 1);
     }
-    for (int i = 0; i < kScaleRing; ++i) mbar_init(&scale_full[i], 1);
+    for (int i = 0; i < kRing; ++i) mbar_init(&scale_full[i], 1);
     mbar_fence_init();
     sh_fail = 0;
   }
@@ -180,7 +188,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
   const uint32_t tmem = sh_tmem;
   volatile int* const fail = &sh_fail;
 
-  if (warp < kSoftWarps) {
+  if (warp < LY::kSoftWarps) {
     // ------------------------------------------------------------- softmax
     const int t = warp >> 2;
     if (t == 0 || two) {
@@ -191,66 +199,59 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
       const int lim = active && p.causal ? cached + token + 1 : len;  // tokens that the row sees
 
       // the row as fp16 (a bf16 row scaled by a power of two), to shared memory
-      float kq = p.scale_log2;
-      {
-        uint4 x[D / 8];
-#pragma unroll
-        for (int c = 0; c < D / 8; ++c) x[c] = make_uint4(0, 0, 0, 0);
-        if (active) {
-          const uint16_t* qp = p.q + (int64_t)(start + token) * p.q_row +
-                               (int64_t)(h * p.group + row % p.group) * p.q_head;
-#pragma unroll
-          for (int c = 0; c < D / 8; ++c) x[c] = __ldg(reinterpret_cast<const uint4*>(qp) + c);
-        }
-        if constexpr (!std::is_same<T, __half>::value) {
-          unsigned m = 0;
-#pragma unroll
+      float kq = p.scale_log2, up = 1.0f;
+      const uint4* qp = reinterpret_cast<const uint4*>(
+          p.q + (int64_t)(start + token) * p.q_row +
+          (int64_t)(h * p.group + row % p.group) * p.q_head);
+      if constexpr (!std::is_same<T, __half>::value) {
+        unsigned m = 0;
+        if (active)
+#pragma unroll 8
           for (int c = 0; c < D / 8; ++c) {
-            m = __vmaxu2(m, __vmaxu2(x[c].x & 0x7FFF7FFFu, x[c].y & 0x7FFF7FFFu));
-            m = __vmaxu2(m, __vmaxu2(x[c].z & 0x7FFF7FFFu, x[c].w & 0x7FFF7FFFu));
+            const uint4 x = __ldg(qp + c);
+            m = __vmaxu2(m, __vmaxu2(x.x & 0x7FFF7FFFu, x.y & 0x7FFF7FFFu));
+            m = __vmaxu2(m, __vmaxu2(x.z & 0x7FFF7FFFu, x.w & 0x7FFF7FFFu));
           }
-          m = max(m & 0xFFFFu, m >> 16);
-          float up;
-          row_scale(m, &up, &kq);
-          kq *= p.scale_log2;
-#pragma unroll
-          for (int c = 0; c < D / 8; ++c)
-            x[c] = make_uint4(scale_pair(x[c].x, up), scale_pair(x[c].y, up),
-                              scale_pair(x[c].z, up), scale_pair(x[c].w, up));
-        }
-#pragma unroll
-        for (int c = 0; c < D / 8; ++c)
-          *reinterpret_cast<uint4*>(sm_q + t * LY::kTile + (c / 8) * LY::kAtom +
-                                    atom_byte(row, c % 8)) = x[c];
+        row_scale(max(m & 0xFFFFu, m >> 16), &up, &kq);
+        kq *= p.scale_log2;
+      }
+#pragma unroll 4
+      for (int c = 0; c < D / 8; ++c) {
+        uint4 x = active ? __ldg(qp + c) : make_uint4(0, 0, 0, 0);
+        if constexpr (!std::is_same<T, __half>::value)
+          x = make_uint4(scale_pair(x.x, up), scale_pair(x.y, up), scale_pair(x.z, up),
+                         scale_pair(x.w, up));
+        *reinterpret_cast<uint4*>(sm_q + t * LY::kQuery + (c / 8) * kQueryAtom +
+                                  atom_byte(row, c % 8)) = x;
       }
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&q_full[t]);
 
       const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-      const uint32_t s_col = tmem + lanes + LY::kScore + t * kN;
+      const uint32_t s_col = tmem + lanes + LY::kScore + t * 2 * kHalf;
       const uint32_t o_col = tmem + lanes + LY::kResult + t * D;
       float m = -INFINITY, l = 0.0f;
       bool ok = true;
 #pragma unroll 1
       for (int i = 0; i < halves_seen; ++i) {
-        const int j = i >> 1, hb = i & 1;
-        if (hb == 0 && !(ok = warp_wait(&scale_full[j % kScaleRing], (j / kScaleRing) & 1, fail)))
+        const int j = i / kHalves, buf = i & 1;
+        if (i % kHalves == 0 && !(ok = warp_wait(&scale_full[j % kRing], (j / kRing) & 1, fail)))
           break;
         // factors and offsets of the exponents of 4 x 16 tokens
-        const Scale* sc = sm_scale + (j % kScaleRing) * 8 + hb * 4;
+        const Scale* sc = sm_scale + i % 8 * 4;  // the ring holds eight halves
         float fk[4], fo[4];
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           fk[g] = kq * sc[g].key;
           fo[g] = sc[g].log2_value;
         }
-        if (!(ok = warp_wait(&s_full[t][hb], j & 1, fail))) break;
+        if (!(ok = warp_wait(&s_full[t][buf], (i >> 1) & 1, fail))) break;
         tc_fence_after();
         // the row's 64 scores, in registers from here on
         uint32_t v[2][32];
-        tmem_ld32_nowait(s_col + hb * kHalf, v[0]);
-        tmem_ld32_nowait(s_col + hb * kHalf + 32, v[1]);
+        tmem_ld32_nowait(s_col + buf * kHalf, v[0]);
+        tmem_ld32_nowait(s_col + buf * kHalf + 32, v[1]);
         tmem_wait_ld32(v[0]);
         tmem_wait_ld32(v[1]);
         // Hidden tokens: scores of -inf, with factors kept above 0.  16 tokens that
@@ -315,12 +316,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
             }
             l = fmaf(sum0 + sum1, sc[g].inv_value, l);
           }
-          tmem_st16(s_col + hb * kHalf + 16 * c, w);
+          tmem_st16(s_col + buf * kHalf + 16 * c, w);
         }
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[t][hb]);
+        if (lane == 0) mbar_arrive(&p_full[t][buf]);
       }
       if (ok && warp_wait(&o_done[t], 0, fail)) {
         tc_fence_after();
@@ -355,16 +356,19 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
     // half of the next row's: reads in 8 different bank groups, and writes too,
     // the swizzle putting what an even row's lanes write, 32 bytes apart, into
     // even places of 16 bytes and what an odd row's write into odd ones.
-    const int odd = kLanes == 8 ? (lane >> 2) & 1 : 0;
-    const int c = kLanes == 8 ? (lane & 3) + (odd ^ ((lane >> 3) & 1)) * 4 : lane & 3;
-    const int row0 = (warp - kSoftWarps) * 32 + (kLanes == 8 ? odd + (lane >> 4) * 2 : lane >> 2);
-    // places of a lane's two chunks in rows row0 and row0 + 4 (of 8), less the row
-    uint32_t put[2][2];
+    const int odd = kLanes == 4 ? 0 : (lane >> 2) & 1;
+    const int c = kLanes == 4 ? lane & 3
+                              : (lane & 3) + (((lane >> 3) ^ odd) & (kLanes / 4 - 1)) * 4;
+    const int row0 = (warp - LY::kSoftWarps) * (kN / LY::kConvWarps) +
+                     (kLanes == 4 ? lane >> 2 : kLanes == 8 ? odd + (lane >> 4) * 2 : odd);
+    // places of a lane's two chunks, less the row's: the swizzle repeats every 8 rows
+    constexpr int kPlaces = 8 / kRows;
+    uint32_t put[kPlaces][2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < kPlaces; ++i)
 #pragma unroll
       for (int x = 0; x < 2; ++x)
-        put[i][x] = atom_byte(row0 + 4 * i, (c % 4) * 2 + x) - 4 * i * 128;
+        put[i][x] = atom_byte(row0 + kRows * i, (c % 4) * 2 + x) - kRows * i * 128;
     bool ok = true;
 #pragma unroll 1
     for (int x = 0; x < 2 * tiles; ++x) {  // keys, values, keys, ...
@@ -376,7 +380,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
           !(ok = warp_wait(side ? &v_empty[st] : &k_empty[st], ((j >> 1) - 1) & 1, fail)))
         break;
 #pragma unroll 1
-      for (int i0 = 0; i0 < kLanes; i0 += 4) {
+      for (int i0 = 0; i0 < kN / LY::kConvWarps / kRows; i0 += 4) {
         uint4 r[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -389,9 +393,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
                                       halves(x[1], 0x4140), halves(x[1], 0x4342));
           const uint4 hi = make_uint4(halves(x[2], 0x4140), halves(x[2], 0x4342),
                                       halves(x[3], 0x4140), halves(x[3], 0x4342));
-          // rows kRows apart: the swizzle repeats every 8
-          *reinterpret_cast<uint4*>(at + i * kRows * 128 + put[i * kRows / 4 % 2][0]) = lo;
-          *reinterpret_cast<uint4*>(at + i * kRows * 128 + put[i * kRows / 4 % 2][1]) = hi;
+          *reinterpret_cast<uint4*>(at + i * kRows * 128 + put[i % kPlaces][0]) = lo;
+          *reinterpret_cast<uint4*>(at + i * kRows * 128 + put[i % kPlaces][1]) = hi;
         }
         src += 4 * kRows * D;
         at += 4 * kRows * 128;
@@ -419,22 +422,24 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
         constexpr uint32_t kHi = (uint32_t)(((uint64_t)64 << 32 | (uint64_t)1 << 46 |
                                              (uint64_t)2 << 61) >> 32);
         constexpr uint32_t kTile16 = LY::kTile / 16, kHalf16 = kHalf * 128 / 16;
-        const uint32_t q_lo = (uint32_t)sw128_desc(sm_q) + t * kTile16;
+        const uint32_t q_lo = (uint32_t)sw128_desc(sm_q) + t * (LY::kQuery / 16);
         const uint32_t k_lo = (uint32_t)sw128_desc(sm_k);
         const uint32_t v_lo = (uint32_t)sw128_mn_desc(sm_v, LY::kAtom);
-        const uint32_t s_at = base + LY::kScore + t * kN, o_at = base + LY::kResult + t * D;
+        const uint32_t s_at = base + LY::kScore + t * 2 * kHalf, o_at = base + LY::kResult + t * D;
         auto scores = [&](int i) {  // half i of the tokens
-          const uint32_t kd = k_lo + ((i >> 1) & 1) * kTile16 + (i & 1) * kHalf16;
+          const uint32_t kd = k_lo + ((i / kHalves) & 1) * kTile16 + (i % kHalves) * kHalf16;
           const uint32_t to = s_at + (i & 1) * kHalf;
 #pragma unroll
           for (int k = 0; k < D / 16; ++k) {
-            const uint32_t step = ((k / 4) * LY::kAtom + (k % 4) * 32) / 16;
-            umma_f16_if(issue, to, q_lo + step, kd + step, kHi, kHi, idesc(kHalf, false), k != 0);
+            const uint32_t q_step = ((k / 4) * kQueryAtom + (k % 4) * 32) / 16;
+            const uint32_t k_step = ((k / 4) * LY::kAtom + (k % 4) * 32) / 16;
+            umma_f16_if(issue, to, q_lo + q_step, kd + k_step, kHi, kHi, idesc(kHalf, false),
+                        k != 0);
           }
           umma_commit_if(issue, &s_full[t][i & 1]);
         };
         auto results = [&](int i) {
-          const uint32_t vd = v_lo + ((i >> 1) & 1) * kTile16 + (i & 1) * kHalf16;
+          const uint32_t vd = v_lo + ((i / kHalves) & 1) * kTile16 + (i % kHalves) * kHalf16;
           const uint32_t from = s_at + (i & 1) * kHalf;
 #pragma unroll
           for (int k = 0; k < kHalf / 16; ++k)
@@ -442,29 +447,30 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
                            idesc(D, true), i != 0 || k != 0);
           umma_commit_if(issue, &o_full[t]);
         };
-        bool ok = warp_wait(&q_full[t], 0, fail) && warp_wait(&k_full[0], 0, fail);
-        if (ok) {
-          tc_fence_after();
-          scores(0);
-          if (steps > 1) scores(1);
-          umma_commit_if(issue, &k_empty[0]);
-        }
+        // scores of half i: the first half of a key tile waits for it, the last gives it back
+        auto next_scores = [&](int i) {
+          const int j = i / kHalves;
+          if (i % kHalves == 0) {
+            if (!warp_wait(&k_full[j & 1], (j >> 1) & 1, fail)) return false;
+            tc_fence_after();
+          }
+          scores(i);
+          if ((i + 1) % kHalves == 0) umma_commit_if(issue, &k_empty[j & 1]);
+          return true;
+        };
+        bool ok = warp_wait(&q_full[t], 0, fail) && next_scores(0);
+        if (ok && steps > 1) ok = next_scores(1);
 #pragma unroll 1
         for (int i = 0; i < steps && ok; ++i) {
-          const int j = i >> 1, hb = i & 1;
-          if (hb == 0) ok = warp_wait(&v_full[j & 1], (j >> 1) & 1, fail);
-          const bool more = i + 2 < steps;  // scores of half i + 2 take this half's place
-          if (ok && more && hb == 0) ok = warp_wait(&k_full[(j + 1) & 1], ((j + 1) >> 1) & 1, fail);
-          ok = ok && warp_wait(&p_full[t][hb], j & 1, fail);
+          const int j = i / kHalves;
+          if (i % kHalves == 0) ok = warp_wait(&v_full[j & 1], (j >> 1) & 1, fail);
+          ok = ok && warp_wait(&p_full[t][i & 1], (i >> 1) & 1, fail);
           if (!ok) break;
           tc_fence_after();
           results(i);
-          if (more) scores(i + 2);
+          if ((i + 1) % kHalves == 0) umma_commit_if(issue, &v_empty[j & 1]);
           if (i + 1 == steps) umma_commit_if(issue, &o_done[t]);
-          if (hb == 1) {
-            umma_commit_if(issue, &v_empty[j & 1]);
-            umma_commit_if(issue, &k_empty[(j + 1) & 1]);
-          }
+          if (i + 2 < steps) ok = next_scores(i + 2);  // in this half's place
         }
         // whatever happened, nothing is in flight when tensor memory is given back
         umma_commit_if(issue, &drained[t]);
@@ -487,7 +493,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
         const int t0 = j * kN + (lane & 7) * 16;
         // a lane at the start of a page's share of the tile copies it; a page is
         // copied whole, past the request's last token too
-        const bool leads = lane < 8 && t0 <= len - 1 && ((lane * 16) & (page_tokens - 1)) == 0;
+        const bool leads = lane < kN / 16 && t0 <= len - 1 && ((lane * 16) & (page_tokens - 1)) == 0;
         const unsigned bytes = __popc(__ballot_sync(kFull, leads)) * piece;
         const int64_t off = ((at << p.page_shift) + (t0 & (page_tokens - 1))) * D;
         float s_key = 0.0f, s_value = 0.0f;
@@ -509,10 +515,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
             if (lane < 8) {
               Scale x{s_key, 0.0f, 0.0f, 0.0f};
               value_scale(s_value, &x.log2_value, &x.inv_value);
-              sm_scale[(j % kScaleRing) * 8 + lane] = x;
+              sm_scale[(j % kRing) * (kN / 16) + lane] = x;
             }
             __syncwarp();
-            if (lane == 0) mbar_arrive(&scale_full[j % kScaleRing]);
+            if (lane == 0) mbar_arrive(&scale_full[j % kRing]);
           }
         }
       }
@@ -546,9 +552,12 @@ int launch(const AttendParams& p, int64_t blocks, cudaStream_t st) {
 
 int launch_prompt(int dtype, int dim, const AttendParams& p, int64_t blocks, cudaStream_t st) {
   if (dtype == GRM_B200_F16)
-    return dim == 64 ? launch<__half, 64>(p, blocks, st) : launch<__half, 128>(p, blocks, st);
-  return dim == 64 ? launch<__nv_bfloat16, 64>(p, blocks, st)
-                   : launch<__nv_bfloat16, 128>(p, blocks, st);
+    return dim == 64    ? launch<__half, 64>(p, blocks, st)
+           : dim == 128 ? launch<__half, 128>(p, blocks, st)
+                        : launch<__half, 256>(p, blocks, st);
+  return dim == 64    ? launch<__nv_bfloat16, 64>(p, blocks, st)
+         : dim == 128 ? launch<__nv_bfloat16, 128>(p, blocks, st)
+                      : launch<__nv_bfloat16, 256>(p, blocks, st);
 }
 
 }  // namespace paged
