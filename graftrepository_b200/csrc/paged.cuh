@@ -34,7 +34,7 @@ struct Header {           // written by the plan kernel
 // the kernels that read its lists agree without the host seeing a length.
 struct Shape {
   int group;            // query heads of a kv head
-  int split_rows;       // requests with more (row, head) pairs a kv head than this are prompts
+  int prompt_rows;      // requests with more (row, head) pairs a kv head can be prompts
   int block_rows;       // rows of a segment: 8 or 16
   int qtile_tokens;     // tokens of a prompt tile
   int tile;             // tokens of a tile of the split kernel
@@ -101,7 +101,7 @@ struct AttendParams {
   int32_t* status;
 };
 
-// Rows of requests with more than split_rows (row, head) pairs (paged_prompt.cu).
+// Rows of the requests that the plan made prompts (paged_prompt.cu).
 int launch_prompt(int dtype, int dim, const AttendParams& p, int64_t blocks, cudaStream_t st);
 
 __device__ __forceinline__ float ex2(float x) {

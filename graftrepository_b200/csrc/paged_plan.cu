@@ -30,6 +30,7 @@ namespace {
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanWarps = kPlanThreads / 32;
 constexpr int kJoinUnits = 5;
+constexpr int kBuckets = 256;  // of prompt tiles by what they see
 // The sums over requests: pages taken, rows, pages touched, prompt tiles (all
 // of them below 2^31 in a step that can be planned) and the split kernel's units.
 constexpr int kSums = 6;
@@ -38,7 +39,7 @@ constexpr int kSegments = 5;  // of the split kernel; only their number is neede
 
 struct PlanParams {
   int64_t requests, tokens, max_fresh, width, ring_size;
-  int page_shift, grow, kv_heads;
+  int page_shift, grow, kv_heads, sms;
   int block_shift, tile_shift;  // log2 of a segment's rows and a tile's tokens
   int chunks, row_blocks, page_blocks;  // blocks for a chunk's rows, and for its pages
   Shape s;
@@ -62,12 +63,13 @@ struct Request {
 };
 
 // What request r adds to each sum.
-__device__ __forceinline__ void weigh(const PlanParams& p, const Request& q, int64_t (&v)[kSums]) {
+__device__ __forceinline__ void weigh(const PlanParams& p, const Request& q, int64_t prompt_rows,
+                                      int64_t (&v)[kSums]) {
   v[kTake] = q.need - q.have;
   v[kRows] = q.fresh;
   v[kTouched] = p.grow && q.fresh > 0 ? q.need - (q.cached >> p.page_shift) : 0;
   const int64_t pairs = (int64_t)q.fresh * p.s.group;
-  const bool prompt = pairs > p.s.split_rows;
+  const bool prompt = pairs > prompt_rows;
   v[kTiles] = prompt ? ((unsigned)q.fresh + p.s.qtile_tokens - 1) / (unsigned)p.s.qtile_tokens : 0;
   v[kSegments] = prompt ? 0 : p.kv_heads * ((pairs + p.s.block_rows - 1) >> p.block_shift);
   v[kUnits] = v[kSegments] * (((q.after + p.s.tile - 1) >> p.tile_shift) + 1);
@@ -113,6 +115,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
   __shared__ int64_t part[2 * kSums][kPlanWarps];
   __shared__ int64_t total[2 * kSums];  // of all requests; of those before the chunk
   __shared__ int chunk_part[kScans][kPlanWarps];
+  __shared__ int bucket[kBuckets], most_seen;
   __shared__ int bad;
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -148,15 +151,38 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
     return q;
   };
 
-  // ---- totals, the chunk's own requests, and errors
+  // ---- which requests are prompts.  From prompt_rows pairs on, the prompt kernel
+  // takes less time than the split kernel, which reads and converts a request's
+  // codes once for every 8 or 16 of them -- where there are enough prompt tiles to
+  // fill the GPU: a tile is one block, however many tokens it sees.  With fewer,
+  // the limit grows in proportion (tables of both kernels' times for 1 to 64
+  // requests of 2,048 to 16,000 tokens and 16 to 512 pairs).
+  int64_t prompt_rows = INT32_MAX;
   if (tid == 0) bad = 0;
+  if (p.s.qtile_cap > 0) {
+    int64_t tiles = 0;
+    for (int64_t r = tid; r < p.requests; r += kPlanThreads) {
+      const int fresh = p.fresh[r];
+      if (fresh > 0 && (int64_t)fresh * p.s.group > p.s.prompt_rows)
+        tiles += ((unsigned)fresh + p.s.qtile_tokens - 1) / (unsigned)p.s.qtile_tokens;
+    }
+    tiles = warp_sum(tiles);
+    if (lane == 0) part[0][warp] = tiles;
+    __syncthreads();
+    tiles = warp_sum(part[0][lane]) * p.kv_heads;
+    prompt_rows = tiles >= p.sms || tiles == 0 ? p.s.prompt_rows
+                                               : p.s.prompt_rows * p.sms / tiles;
+    __syncthreads();
+  }
+
+  // ---- totals, the chunk's own requests, and errors
   int64_t v[kSums] = {}, before[kSums] = {}, own[kSums] = {};
   Request q{0, 0, 0, 0, 0};
   int flags = 0;
   for (int c = 0; c < p.chunks; ++c) {
     int64_t a[kSums];
     const Request x = request((int64_t)c * kPlanThreads + tid, &flags);
-    weigh(p, x, a);
+    weigh(p, x, prompt_rows, a);
     if (c == chunk) {
       q = x;
 #pragma unroll
@@ -299,9 +325,44 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
     }
   } else {
     if (tid < n) p.l.base[r0 + tid] = sum[kUnits][tid];
-    for (int x = sum[kTiles][0] + tid; x < sum[kTiles][n]; x += kPlanThreads) {
-      const int i = find(sum[kTiles], n, x);
-      p.l.qtiles[x] = make_int2((int)(r0 + i), (x - sum[kTiles][i]) * p.s.qtile_tokens);
+    const int tile0 = sum[kTiles][0], tiles = sum[kTiles][n] - tile0;
+    if (tiles > 0) {
+      // Prompt tiles in the order of what they see, longest first (the blocks of
+      // the prompt kernel start in this order, and the last ones to start decide
+      // when it ends): counted into kBuckets, then placed.  The order within a
+      // bucket does not matter.
+      auto sees = [&](int i, int tok) {  // a causal step's; otherwise about as good
+        return s_cached[i] + tok + p.s.qtile_tokens;
+      };
+      if (tid < kBuckets) bucket[tid] = 0;
+      if (tid == 0) most_seen = 0;
+      __syncthreads();
+      const int top = __reduce_max_sync(kFull, tid < n && own[kTiles] > 0 ? q.cached + q.fresh : 0);
+      if (lane == 0) atomicMax(&most_seen, top);
+      __syncthreads();
+      const int unit = (most_seen + p.s.qtile_tokens) / kBuckets + 1;
+      auto bucket_of = [&](int x, int* i, int* tok) {
+        *i = find(sum[kTiles], n, x);
+        *tok = (x - sum[kTiles][*i]) * p.s.qtile_tokens;
+        return kBuckets - 1 - min(sees(*i, *tok) / unit, kBuckets - 1);
+      };
+      int i, tok;
+      for (int x = tile0 + tid; x < tile0 + tiles; x += kPlanThreads)
+        atomicAdd(&bucket[bucket_of(x, &i, &tok)], 1);
+      __syncthreads();
+      if (warp == 0) {
+        int before = 0;
+        for (int b = 0; b < kBuckets; b += 32) {
+          const int x = bucket[b + lane], w = warp_scan(x, lane);
+          bucket[b + lane] = before + w - x;
+          before += __shfl_sync(kFull, w, 31);
+        }
+      }
+      __syncthreads();
+      for (int x = tile0 + tid; x < tile0 + tiles; x += kPlanThreads) {
+        const int b = bucket_of(x, &i, &tok);
+        p.l.qtiles[tile0 + atomicAdd(&bucket[b], 1)] = make_int2((int)(r0 + i), tok);
+      }
     }
     const int share = workers ? units / workers : 0, more = workers ? units % workers : 0;
     for (int w = tid; w < workers; w += kPlanThreads) {
@@ -360,9 +421,6 @@ __global__ void __launch_bounds__(kReleaseThreads)
   if (tid == 0) cursor[1] = returned;
 }
 
-// Requests with more (row, head) pairs a kv head than this are prompts.
-constexpr int kPromptRows = 64;
-
 int64_t align256(int64_t v) { return (v + 255) & ~(int64_t)255; }
 
 }  // namespace
@@ -371,14 +429,15 @@ int make_shape(const grm_b200_paged_plan& p, int sms, Shape* s) {
   s->group = p.query_heads / p.kv_heads;
   const int64_t most = std::min(p.max_fresh, p.tokens) * s->group;
   s->block_rows = most <= 8 || p.head_dim == 256 ? 8 : 16;
-  const bool prompts = most > kPromptRows;
-  s->split_rows = prompts ? kPromptRows : INT32_MAX;
+  s->prompt_rows = p.head_dim == 256 ? 16 : 32;
+  const bool prompts = most > s->prompt_rows;
   s->qtile_tokens = (p.head_dim == 256 ? 1 : 2) * (128 / s->group);
   s->tile = split_tile(p.head_dim);
   s->workers = sms * split_blocks(p.head_dim, s->block_rows);
   const int64_t R = p.requests, T = p.tokens;
   s->page_cap = p.grow ? std::min(T, T / p.page_tokens + 2 * std::min(R, T)) : 0;
-  s->qtile_cap = prompts ? std::min(T, T / s->qtile_tokens + std::min(R, T)) : 0;
+  // a tile for every qtile_tokens rows and one more for every prompt
+  s->qtile_cap = prompts ? T / s->qtile_tokens + std::min(R, T * s->group / s->prompt_rows) : 0;
   int64_t at = align256(sizeof(Header));
   auto take = [&](int64_t bytes) {
     const int64_t o = at;
@@ -570,6 +629,7 @@ int grm_b200_paged_plan_step(const grm_b200_paged_plan* plan, const int32_t* fre
   p.page_shift = shift_of(plan->page_tokens);
   p.grow = plan->grow ? 1 : 0;
   p.kv_heads = plan->kv_heads;
+  p.sms = sms;
   make_shape(*plan, sms, &p.s);
   p.block_shift = p.s.block_rows == 8 ? 3 : 4;
   p.tile_shift = shift_of(p.s.tile);

@@ -126,10 +126,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
   __shared__ int sh_fail;
 
   const Header hd = *p.l.header;
-  // later tiles first: in a causal step they see the most tokens
   const int h = blockIdx.x % p.kv_heads;
-  const int ti = hd.qtiles - 1 - (int)(blockIdx.x / p.kv_heads);
-  if (ti < 0) return;
+  const int ti = (int)(blockIdx.x / p.kv_heads);  // the longest come first in the list
+  if (ti >= hd.qtiles) return;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int2 tile = p.l.qtiles[ti];

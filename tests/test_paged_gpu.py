@@ -433,6 +433,16 @@ def test_prompts(dim, group, page, causal):
 
 
 @pytest.mark.parametrize("kind", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim,group,page", [(64, 1, 16), (64, 5, 128), (128, 1, 32), (128, 3, 64),
+                                            (256, 1, 64), (256, 4, 16), (128, 40, 16)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_prompts_on_many_heads(dim, group, page, kind, causal):
+    """Enough tiles to fill the GPU, so that short prompts are prompts too."""
+    run_attention([190, 45, 500, 64, 1, 130], [190, 40, 130, 64, 1, 33], heads=40, group=group,
+                  dim=dim, page=page, causal=causal, seed=dim + group, kind=kind)
+
+
+@pytest.mark.parametrize("kind", [torch.bfloat16, torch.float16])
 def test_prompts_and_single_tokens_in_one_step(kind):
     run_attention([2000, 700, 350, 1, 900, 1500], [1, 600, 0, 1, 1, 130], heads=2, group=4, dim=128,
                   page=64, kind=kind, seed=3)
