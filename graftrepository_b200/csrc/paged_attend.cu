@@ -64,7 +64,11 @@ struct Layout {
   static constexpr int kMerge = 2 * 8 * kRow * 4;
   static constexpr int kScales = kWarps * kStages * 2 * 8;
   static constexpr int kML = 2 * kWarps * NT * 8 * 4;
-  static constexpr int kSmem = 1024 + kRing + kMerge + kScales + kML;
+  // Sixteen rows: their fragments in shared memory, the same for every warp (in
+  // registers beside the results of 16 rows they would spill).
+  static constexpr bool kQShared = NT == 2;
+  static constexpr int kQ = kQShared ? (D / 16) * NT * 32 * 8 + NT * 8 * 4 : 0;
+  static constexpr int kSmem = 1024 + kRing + kMerge + kScales + kML + kQ;
 };
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
@@ -241,6 +245,8 @@ __global__ void __launch_bounds__(kThreads, (Layout<D, NT>::kBlocks))
   float2* const scales = reinterpret_cast<float2*>(smem + LY::kRing + LY::kMerge);
   float* const sm_m = reinterpret_cast<float*>(smem + LY::kRing + LY::kMerge + LY::kScales);
   float* const sm_l = sm_m + kWarps * NT * 8;
+  uint2* const sm_q = reinterpret_cast<uint2*>(sm_l + kWarps * NT * 8);
+  float* const sm_unscale = reinterpret_cast<float*>(sm_q + kChunks * NT * 32);
   __shared__ __align__(8) uint64_t bars[kWarps][LY::kStages];
   __shared__ int sm_last, sm_fail;
 
@@ -264,7 +270,7 @@ __global__ void __launch_bounds__(kThreads, (Layout<D, NT>::kBlocks))
   bool more;
 
   // ---- queries of a segment: column g of the B operand, dims 16c + 4 t4 .. + 3
-  uint2 raw[NT][kChunks];
+  uint2 raw[LY::kQShared ? 1 : NT][kChunks];
   // packed row and head of row `x` of a segment (a block's rows are few, so the
   // division by the group is a multiplication)
   auto pair_of = [&](const Segment& s, int x, int* token, int* head) {
@@ -287,9 +293,46 @@ __global__ void __launch_bounds__(kThreads, (Layout<D, NT>::kBlocks))
                            : make_uint2(0, 0);
     }
   };
+  // The same to shared memory, a warp the four rows 4 warp .. and eight lanes a row.
+  auto share_queries = [&](const Segment& s) {
+    const int x = warp * 4 + (lane >> 3), d0 = (lane & 7) * (D / 8);
+    const bool there = s.row0 + x < s.pairs;
+    int token, head;
+    pair_of(s, x, &token, &head);
+    const uint4* qp = reinterpret_cast<const uint4*>(
+        p.q + (int64_t)(s.start + token) * p.q_row + (int64_t)head * p.q_head + d0);
+    uint4 v[D / 64];
+    unsigned m = 0;
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) {
+      v[i] = there ? __ldg(qp + i) : make_uint4(0, 0, 0, 0);
+      m = __vmaxu2(m, __vmaxu2(v[i].x & 0x7FFF7FFFu, v[i].y & 0x7FFF7FFFu));
+      m = __vmaxu2(m, __vmaxu2(v[i].z & 0x7FFF7FFFu, v[i].w & 0x7FFF7FFFu));
+    }
+    float up = 1.0f, unscale = 1.0f;
+    if constexpr (!std::is_same<T, __half>::value) {
+      m = max(m & 0xFFFFu, m >> 16);
+#pragma unroll
+      for (int i = 1; i <= 4; i <<= 1) m = max(m, __shfl_xor_sync(kFull, m, i));
+      row_scale(m, &up, &unscale);
+#pragma unroll
+      for (int i = 0; i < D / 64; ++i)
+        v[i] = make_uint4(scale_pair(v[i].x, up), scale_pair(v[i].y, up), scale_pair(v[i].z, up),
+                          scale_pair(v[i].w, up));
+    }
+    if ((lane & 7) == 0) sm_unscale[x] = unscale;
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) {
+      const int d = d0 + 8 * i;
+      uint2* to = sm_q + (d / 16 * NT + x / 8) * 32 + (x % 8) * 4 + d % 16 / 4;
+      to[0] = make_uint2(v[i].x, v[i].y);
+      to[1] = make_uint2(v[i].z, v[i].w);
+    }
+    __syncthreads();
+  };
   auto next_segment = [&]() {
     more = walk.next();
-    if (more) fetch_queries(walk.s);
+    if (!LY::kQShared && more) fetch_queries(walk.s);
   };
   next_segment();
 
@@ -392,13 +435,14 @@ __global__ void __launch_bounds__(kThreads, (Layout<D, NT>::kBlocks))
     }
     if (walk.t >= walk.t1) continue;  // only its start is this worker's
 
-    uint32_t qf[kChunks][NT][2];
+    uint32_t qf[LY::kQShared ? 1 : kChunks][NT][2];
     float kq[NT][2];
     int lim[NT][2];
+    if constexpr (LY::kQShared) share_queries(s);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       float up = 1.0f, unscale = 1.0f;
-      if constexpr (!std::is_same<T, __half>::value) {
+      if constexpr (!LY::kQShared && !std::is_same<T, __half>::value) {
         unsigned m = 0;
 #pragma unroll
         for (int c = 0; c < kChunks; ++c)
@@ -409,7 +453,7 @@ __global__ void __launch_bounds__(kThreads, (Layout<D, NT>::kBlocks))
         row_scale(m, &up, &unscale);
       }
 #pragma unroll
-      for (int c = 0; c < kChunks; ++c) {
+      for (int c = 0; c < (LY::kQShared ? 0 : kChunks); ++c) {
         uint2 f = raw[nt][c];
         if constexpr (!std::is_same<T, __half>::value)
           f = make_uint2(scale_pair(f.x, up), scale_pair(f.y, up));
@@ -419,7 +463,8 @@ __global__ void __launch_bounds__(kThreads, (Layout<D, NT>::kBlocks))
       // columns 2 t4 and 2 t4 + 1 of the scores
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        kq[nt][x] = p.scale_log2 * __shfl_sync(kFull, unscale, (2 * t4 + x) * 4);
+        kq[nt][x] = p.scale_log2 * (LY::kQShared ? sm_unscale[nt * 8 + 2 * t4 + x]
+                                                 : __shfl_sync(kFull, unscale, (2 * t4 + x) * 4));
         int token, head;
         pair_of(s, nt * 8 + 2 * t4 + x, &token, &head);
         lim[nt][x] = p.causal && s.row0 + nt * 8 + 2 * t4 + x < s.pairs ? s.cached + token + 1
@@ -453,7 +498,7 @@ __global__ void __launch_bounds__(kThreads, (Layout<D, NT>::kBlocks))
       __syncwarp();
       const uint32_t kb = ring + stage * LY::kStage;
       // scores of kB x 16 tokens x 8 NT rows, two chains of products at least
-      constexpr int kChains = kB == 1 ? 2 : 1;
+      constexpr int kChains = kB * NT == 1 ? 2 : 1;
       float sum[kChains][kB][NT][4];
 #pragma unroll
       for (int i = 0; i < kChains; ++i)
@@ -476,6 +521,14 @@ __global__ void __launch_bounds__(kThreads, (Layout<D, NT>::kBlocks))
           else  // the first value fragments
             ldsm4t(fr[(c / 2 + 1) % 2][b], kb + lm[0] + (LY::kSide + b * kNext16));
         }
+        uint2 qs[2][NT];
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            if constexpr (LY::kQShared) qs[x][nt] = sm_q[((c + x) * NT + nt) * 32 + lane];
+            else qs[x][nt] = make_uint2(qf[c + x][nt][0], qf[c + x][nt][1]);
+          }
 #pragma unroll
         for (int b = 0; b < kB; ++b) {
           const uint32_t* r = fr[(c / 2) % 2][b];
@@ -486,7 +539,7 @@ __global__ void __launch_bounds__(kThreads, (Layout<D, NT>::kBlocks))
             const uint32_t a1 = halves(hi, 0x4140), a3 = halves(hi, 0x4342);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
-              mma(sum[x % kChains][b][nt], a0, a1, a2, a3, qf[c + x][nt][0], qf[c + x][nt][1]);
+              mma(sum[x % kChains][b][nt], a0, a1, a2, a3, qs[x][nt].x, qs[x][nt].y);
           }
         }
       }
@@ -748,7 +801,8 @@ int launch_split_any(int dim, int block_rows, const SplitParams& p, int workers,
   if (dim == 128)
     return block_rows == 8 ? launch_split<T, 128, 1>(p, workers, st)
                            : launch_split<T, 128, 2>(p, workers, st);
-  return launch_split<T, 256, 1>(p, workers, st);
+  return block_rows == 8 ? launch_split<T, 256, 1>(p, workers, st)
+                         : launch_split<T, 256, 2>(p, workers, st);
 }
 
 // cuTensorMapEncodeTiled from the driver, looked up once (no libcuda link).

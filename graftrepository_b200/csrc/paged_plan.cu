@@ -428,7 +428,7 @@ int64_t align256(int64_t v) { return (v + 255) & ~(int64_t)255; }
 int make_shape(const grm_b200_paged_plan& p, int sms, Shape* s) {
   s->group = p.query_heads / p.kv_heads;
   const int64_t most = std::min(p.max_fresh, p.tokens) * s->group;
-  s->block_rows = most <= 8 || p.head_dim == 256 ? 8 : 16;
+  s->block_rows = most <= 8 ? 8 : 16;
   s->prompt_rows = p.head_dim == 256 ? 16 : 32;
   const bool prompts = most > s->prompt_rows;
   s->qtile_tokens = (p.head_dim == 256 ? 1 : 2) * (128 / s->group);
