@@ -21,12 +21,16 @@ __host__ __device__ constexpr int split_blocks(int dim, int rows) {
 // fp32 of one partial result: rows x dim, then (reference exponent, sum) a row.
 __host__ __device__ constexpr int split_slot(int dim, int rows) { return rows * dim + 2 * rows; }
 
+// Query rows of a prompt tile, and fp32 of one part's result.
+__host__ __device__ constexpr int prompt_rows_of(int dim) { return dim == 256 ? 128 : 256; }
+__host__ __device__ constexpr int prompt_slot(int dim) { return prompt_rows_of(dim) * (dim + 2); }
+
 struct Header {           // written by the plan kernel
   int32_t units;          // units of the split kernel's work, all requests
   int32_t workers;        // workers that share them (<= Shape::workers)
   int32_t share, more;    // units of a worker, and how many workers have one more
   int32_t pages;          // entries of the append list
-  int32_t qtiles;         // entries of the prompt kernel's list
+  int32_t qtiles;         // entries of the prompt kernel's list: parts of prompt tiles
   int32_t rows;           // packed rows of the step
 };
 
@@ -40,9 +44,10 @@ struct Shape {
   int tile;             // tokens of a tile of the split kernel
   int workers;          // resident blocks of the split kernel
   int64_t page_cap;     // most pages a step can touch
-  int64_t qtile_cap;    // most prompt tiles (0: no request can be a prompt)
+  int64_t qtile_cap;    // most entries of the prompt kernel's list (0: no request can be a prompt)
   // byte offsets in the scratch
-  int64_t off_base, off_start, off_count, off_pages, off_qtiles, off_part, bytes;
+  int64_t off_base, off_start, off_count, off_pages, off_qtiles, off_part;
+  int64_t off_qcount, off_qpart, bytes;
 };
 
 int make_shape(const grm_b200_paged_plan& p, int sms, Shape* s);
@@ -53,8 +58,12 @@ struct Lists {
   int32_t* start;     // [workers] request of a worker's first unit
   unsigned* count;    // [workers] arrivals at the segment that a worker starts; 0 between calls
   int4* pages;        // [page_cap] (first packed row, page, older tokens in it, new rows)
-  int2* qtiles;       // [qtile_cap] (request, first row of the tile within the request)
+  // [qtile_cap] (request, first row of the tile within the request, part + 256 *
+  // parts, first entry of the tile)
+  int4* qtiles;
   float* part;        // [workers * 2][split_slot]
+  unsigned* qcount;   // [sms] arrivals at a prompt tile and head in parts; 0 between calls
+  float* qpart;       // [sms][prompt_slot]
 };
 
 inline Lists lists_of(const Shape& s, void* scratch) {
@@ -64,8 +73,10 @@ inline Lists lists_of(const Shape& s, void* scratch) {
           reinterpret_cast<int32_t*>(b + s.off_start),
           reinterpret_cast<unsigned*>(b + s.off_count),
           reinterpret_cast<int4*>(b + s.off_pages),
-          reinterpret_cast<int2*>(b + s.off_qtiles),
-          reinterpret_cast<float*>(b + s.off_part)};
+          reinterpret_cast<int4*>(b + s.off_qtiles),
+          reinterpret_cast<float*>(b + s.off_part),
+          reinterpret_cast<unsigned*>(b + s.off_qcount),
+          reinterpret_cast<float*>(b + s.off_qpart)};
 }
 
 // First unit of worker w, and the worker that holds unit u.

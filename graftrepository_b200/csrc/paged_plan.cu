@@ -31,6 +31,7 @@ constexpr int kPlanThreads = 1024;
 constexpr int kPlanWarps = kPlanThreads / 32;
 constexpr int kJoinUnits = 5;
 constexpr int kBuckets = 256;  // of prompt tiles by what they see
+constexpr int kPartTokens = 512;  // a part of a prompt tile has no fewer
 // The sums over requests: pages taken, rows, pages touched, prompt tiles (all
 // of them below 2^31 in a step that can be planned) and the split kernel's units.
 constexpr int kSums = 6;
@@ -63,14 +64,21 @@ struct Request {
 };
 
 // What request r adds to each sum.
-__device__ __forceinline__ void weigh(const PlanParams& p, const Request& q, int64_t prompt_rows,
+// Parts of a prompt request's tiles, for `part_tokens` in each (0: whole).
+__device__ __forceinline__ int parts_of(int after, int part_tokens) {
+  return part_tokens == 0 ? 1 : max(1, (after + part_tokens - 1) / part_tokens);
+}
+
+__device__ __forceinline__ void weigh(const PlanParams& p, const Request& q, int part_tokens,
                                       int64_t (&v)[kSums]) {
   v[kTake] = q.need - q.have;
   v[kRows] = q.fresh;
   v[kTouched] = p.grow && q.fresh > 0 ? q.need - (q.cached >> p.page_shift) : 0;
   const int64_t pairs = (int64_t)q.fresh * p.s.group;
-  const bool prompt = pairs > prompt_rows;
-  v[kTiles] = prompt ? ((unsigned)q.fresh + p.s.qtile_tokens - 1) / (unsigned)p.s.qtile_tokens : 0;
+  const bool prompt = pairs > p.s.prompt_rows && p.s.qtile_cap > 0;
+  v[kTiles] = prompt ? (int64_t)(((unsigned)q.fresh + p.s.qtile_tokens - 1) /
+                                 (unsigned)p.s.qtile_tokens) * parts_of(q.after, part_tokens)
+                     : 0;
   v[kSegments] = prompt ? 0 : p.kv_heads * ((pairs + p.s.block_rows - 1) >> p.block_shift);
   v[kUnits] = v[kSegments] * (((q.after + p.s.tile - 1) >> p.tile_shift) + 1);
 }
@@ -151,27 +159,35 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
     return q;
   };
 
-  // ---- which requests are prompts.  From prompt_rows pairs on, the prompt kernel
-  // takes less time than the split kernel, which reads and converts a request's
-  // codes once for every 8 or 16 of them -- where there are enough prompt tiles to
-  // fill the GPU: a tile is one block, however many tokens it sees.  With fewer,
-  // the limit grows in proportion (tables of both kernels' times for 1 to 64
-  // requests of 2,048 to 16,000 tokens and 16 to 512 pairs).
-  int64_t prompt_rows = INT32_MAX;
+  // ---- prompts.  A prompt tile and head is one block; where they are fewer than
+  // half of the SMs, tiles are cut along their tokens into parts, as many as there
+  // are SMs beyond the tiles: Sum ceil(len / part) <= Sum len / part + tiles, so all
+  // parts run at once.
+  int part_tokens = 0;
   if (tid == 0) bad = 0;
   if (p.s.qtile_cap > 0) {
-    int64_t tiles = 0;
+    int64_t tiles = 0, tokens = 0;
     for (int64_t r = tid; r < p.requests; r += kPlanThreads) {
-      const int fresh = p.fresh[r];
-      if (fresh > 0 && (int64_t)fresh * p.s.group > p.s.prompt_rows)
-        tiles += ((unsigned)fresh + p.s.qtile_tokens - 1) / (unsigned)p.s.qtile_tokens;
+      const int cached = max(p.cached[r], 0), fresh = p.fresh[r];
+      if (fresh > 0 && (int64_t)fresh * p.s.group > p.s.prompt_rows) {
+        const int x = ((unsigned)fresh + p.s.qtile_tokens - 1) / (unsigned)p.s.qtile_tokens;
+        tiles += x;
+        tokens += (int64_t)x * (cached + (p.grow ? (int64_t)fresh : 0));
+      }
     }
     tiles = warp_sum(tiles);
-    if (lane == 0) part[0][warp] = tiles;
+    tokens = warp_sum(tokens);
+    if (lane == 0) {
+      part[0][warp] = tiles;
+      part[1][warp] = tokens;
+    }
     __syncthreads();
     tiles = warp_sum(part[0][lane]) * p.kv_heads;
-    prompt_rows = tiles >= p.sms || tiles == 0 ? p.s.prompt_rows
-                                               : p.s.prompt_rows * p.sms / tiles;
+    tokens = warp_sum(part[1][lane]) * p.kv_heads;
+    if (tiles > 0 && tiles <= p.sms / 2) {
+      const int64_t each = ceil_div64(tokens, p.sms - tiles);
+      part_tokens = (int)(each < kPartTokens ? kPartTokens : each < (1 << 30) ? each : 1 << 30);
+    }
     __syncthreads();
   }
 
@@ -182,7 +198,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
   for (int c = 0; c < p.chunks; ++c) {
     int64_t a[kSums];
     const Request x = request((int64_t)c * kPlanThreads + tid, &flags);
-    weigh(p, x, prompt_rows, a);
+    weigh(p, x, part_tokens, a);
     if (c == chunk) {
       q = x;
 #pragma unroll
@@ -243,6 +259,8 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
                            all_rows};
     }
     for (int i = tid; i < p.s.workers; i += kPlanThreads) p.l.count[i] = 0;
+    if (p.s.qtile_cap > 0)
+      for (int i = tid; i < p.sms; i += kPlanThreads) p.l.qcount[i] = 0;
   }
   if (kind == kWriteRows)
     for (int64_t i = all_rows + (int64_t)chunk * gsize + gid; i < p.tokens;
@@ -327,7 +345,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
     if (tid < n) p.l.base[r0 + tid] = sum[kUnits][tid];
     const int tile0 = sum[kTiles][0], tiles = sum[kTiles][n] - tile0;
     if (tiles > 0) {
-      // Prompt tiles in the order of what they see, longest first (the blocks of
+      // Parts of prompt tiles in the order of what they see, longest first (the blocks of
       // the prompt kernel start in this order, and the last ones to start decide
       // when it ends): counted into kBuckets, then placed.  The order within a
       // bucket does not matter.
@@ -341,14 +359,19 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
       if (lane == 0) atomicMax(&most_seen, top);
       __syncthreads();
       const int unit = (most_seen + p.s.qtile_tokens) / kBuckets + 1;
-      auto bucket_of = [&](int x, int* i, int* tok) {
-        *i = find(sum[kTiles], n, x);
-        *tok = (x - sum[kTiles][*i]) * p.s.qtile_tokens;
-        return kBuckets - 1 - min(sees(*i, *tok) / unit, kBuckets - 1);
+      auto entry = [&](int x, int* b) {
+        const int i = find(sum[kTiles], n, x);
+        const int after = s_cached[i] + (p.grow ? sum[kRows][i + 1] - sum[kRows][i] : 0);
+        const int parts = parts_of(after, part_tokens), y = x - sum[kTiles][i];
+        const int tok = y / parts * p.s.qtile_tokens, part = y % parts;
+        *b = kBuckets - 1 - min(sees(i, tok) / unit, kBuckets - 1);
+        return make_int4((int)(r0 + i), tok, part + 256 * parts, x - part);
       };
-      int i, tok;
-      for (int x = tile0 + tid; x < tile0 + tiles; x += kPlanThreads)
-        atomicAdd(&bucket[bucket_of(x, &i, &tok)], 1);
+      int b;
+      for (int x = tile0 + tid; x < tile0 + tiles; x += kPlanThreads) {
+        entry(x, &b);
+        atomicAdd(&bucket[b], 1);
+      }
       __syncthreads();
       if (warp == 0) {
         int before = 0;
@@ -360,8 +383,8 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
       }
       __syncthreads();
       for (int x = tile0 + tid; x < tile0 + tiles; x += kPlanThreads) {
-        const int b = bucket_of(x, &i, &tok);
-        p.l.qtiles[tile0 + atomicAdd(&bucket[b], 1)] = make_int2((int)(r0 + i), tok);
+        const int4 e = entry(x, &b);
+        p.l.qtiles[tile0 + atomicAdd(&bucket[b], 1)] = e;
       }
     }
     const int share = workers ? units / workers : 0, more = workers ? units % workers : 0;
@@ -436,8 +459,11 @@ int make_shape(const grm_b200_paged_plan& p, int sms, Shape* s) {
   s->workers = sms * split_blocks(p.head_dim, s->block_rows);
   const int64_t R = p.requests, T = p.tokens;
   s->page_cap = p.grow ? std::min(T, T / p.page_tokens + 2 * std::min(R, T)) : 0;
-  // a tile for every qtile_tokens rows and one more for every prompt
-  s->qtile_cap = prompts ? T / s->qtile_tokens + std::min(R, T * s->group / s->prompt_rows) : 0;
+  // a tile for every qtile_tokens rows, one more for every prompt, and what the
+  // parts add
+  s->qtile_cap = prompts ? T / s->qtile_tokens + std::min(R, T * s->group / s->prompt_rows) +
+                               ceil_div64(sms, p.kv_heads)
+                         : 0;
   int64_t at = align256(sizeof(Header));
   auto take = [&](int64_t bytes) {
     const int64_t o = at;
@@ -448,8 +474,10 @@ int make_shape(const grm_b200_paged_plan& p, int sms, Shape* s) {
   s->off_start = take((int64_t)s->workers * 4);
   s->off_count = take((int64_t)s->workers * 4);
   s->off_pages = take(std::min(T, T / p.page_tokens + 2 * std::min(R, T)) * 16);
-  s->off_qtiles = take(s->qtile_cap * 8);
+  s->off_qtiles = take(s->qtile_cap * 16);
   s->off_part = take((int64_t)s->workers * 2 * split_slot(p.head_dim, s->block_rows) * 4);
+  s->off_qcount = take(prompts ? (int64_t)sms * 4 : 0);
+  s->off_qpart = take(prompts ? (int64_t)sms * prompt_slot(p.head_dim) * 4 : 0);
   s->bytes = at;
   return 0;
 }

@@ -123,7 +123,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
   __shared__ __align__(8) uint64_t q_full[2], drained[2], k_full[2], k_empty[2], v_full[2], v_empty[2],
       scale_full[kRing], raw_full[2], raw_empty[2], s_full[2][2], p_full[2][2], o_full[2], o_done[2];
   __shared__ uint32_t sh_tmem;
-  __shared__ int sh_fail;
+  __shared__ int sh_fail, sh_last;
 
   const Header hd = *p.l.header;
   const int h = blockIdx.x % p.kv_heads;
@@ -131,7 +131,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
   if (ti >= hd.qtiles) return;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int2 tile = p.l.qtiles[ti];
+  const int4 tile = p.l.qtiles[ti];
   const int start = p.starts[tile.x];
   const int n = p.starts[tile.x + 1] - start;
   const int len = p.lens[tile.x];
@@ -143,10 +143,16 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
   const bool two = toks[1] > 0;
   const int heads = p.kv_heads * p.group;
   const int sees = p.causal ? min(len, cached + tok0 + toks[0] + toks[1]) : len;
-  const int tiles = (sees + kN - 1) / kN;
-  const int halves_seen = (sees + kHalf - 1) / kHalf;
+  const int all_tiles = (sees + kN - 1) / kN;
+  // the part of them that is this block's, and what it begins with
+  const int parts = max(1, min(tile.z >> 8, all_tiles)), part = tile.z & 255;
+  const int tile0 = (int)((int64_t)all_tiles * part / parts);
+  const int tiles = (int)((int64_t)all_tiles * (part + 1) / parts) - tile0;
+  const int tok_base = tile0 * kN;
+  const int halves_seen = (min(sees - tok_base, tiles * kN) + kHalf - 1) / kHalf;
+  if (part >= parts) return;
 
-  if (tiles == 0) {  // nothing cached: empty rows
+  if (all_tiles == 0) {  // nothing cached: empty rows
     for (int x = threadIdx.x; x < (toks[0] + toks[1]) * p.group * (D / 2); x += kPromptThreads) {
       const int j = x / (D / 2);
       const int64_t row = (int64_t)(start + tok0 + j / p.group) * heads + h * p.group + j % p.group;
@@ -195,7 +201,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
       const bool active = row < (t == 0 ? toks[0] : toks[1]) * p.group;
       const int token = tok0 + t * per + row / p.group;
       const int64_t orow = (int64_t)(start + token) * heads + h * p.group + row % p.group;
-      const int lim = active && p.causal ? cached + token + 1 : len;  // tokens that the row sees
+      // tokens that the row sees, from the part's first on
+      const int lim = (active && p.causal ? cached + token + 1 : len) - tok_base;
 
       // the row as fp16 (a bf16 row scaled by a power of two), to shared memory
       float kq = p.scale_log2, up = 1.0f;
@@ -324,27 +331,45 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
       }
       if (ok && warp_wait(&o_done[t], 0, fail)) {
         tc_fence_after();
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        if (parts > 1) {  // the part's result, to be joined
+          float* slot = p.l.qpart +
+                        ((int64_t)(tile.w + part) * p.kv_heads + h) * prompt_slot(D);
+          float* to = slot + (t * kM + row) * D;
+#pragma unroll 1
+          for (int c = 0; c < D / 16; ++c) {
+            uint32_t v[16];
+            tmem_ld16(o_col + 16 * c, v);
+            if (active)
 #pragma unroll
-        for (int c = 0; c < D / 32; ++c) {
-          uint32_t v[32];
-          tmem_ld32_nowait(o_col + 32 * c, v);
-          tmem_wait_ld32(v);
-          if (active) {
-            uint4* out = reinterpret_cast<uint4*>(p.out + orow * D + 32 * c);
+              for (int i = 0; i < 4; ++i)
+                reinterpret_cast<uint4*>(to + 16 * c)[i] =
+                    make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+          }
+          if (active)
+            *reinterpret_cast<float2*>(slot + prompt_rows_of(D) * D + 2 * (t * kM + row)) =
+                make_float2(m, l);
+        } else {
+          const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll 1
+          for (int c = 0; c < D / 16; ++c) {
+            uint32_t v[16];
+            tmem_ld16(o_col + 16 * c, v);
+            if (active) {
+              uint4* out = reinterpret_cast<uint4*>(p.out + orow * D + 16 * c);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              uint32_t w[4];
+              for (int i = 0; i < 2; ++i) {
+                uint32_t w[4];
 #pragma unroll
-              for (int x = 0; x < 4; ++x)
-                w[x] = pack_out<T>(__uint_as_float(v[8 * i + 2 * x]) * inv,
-                                   __uint_as_float(v[8 * i + 2 * x + 1]) * inv);
-              out[i] = make_uint4(w[0], w[1], w[2], w[3]);
+                for (int x = 0; x < 4; ++x)
+                  w[x] = pack_out<T>(__uint_as_float(v[8 * i + 2 * x]) * inv,
+                                     __uint_as_float(v[8 * i + 2 * x + 1]) * inv);
+                out[i] = make_uint4(w[0], w[1], w[2], w[3]);
+              }
             }
           }
+          if (active && p.lse)
+            p.lse[orow] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.693147180559945309f;
         }
-        if (active && p.lse)
-          p.lse[orow] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.693147180559945309f;
       }
     }
   } else if (warp < kMmaWarp) {
@@ -481,7 +506,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
       const int page_tokens = 1 << p.page_shift;
       const unsigned piece = (unsigned)(min(page_tokens, kN) * D);  // codes of a page in a tile
       auto page_of = [&](int j) {  // lane g < 8: page of the tile's tokens 16 g ..
-        const int i = min((j * kN + (lane & 7) * 16) >> p.page_shift, last);
+        const int i = min((tok_base + j * kN + (lane & 7) * 16) >> p.page_shift, last);
         return min(max(__ldg(p.table + tile.x * p.width + i), 0), (int)p.pages - 1);
       };
       int page = page_of(0);
@@ -489,7 +514,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
       bool ok = true;
       for (int j = 0; j < tiles && ok; ++j) {
         const int64_t at = (int64_t)page * p.kv_heads + h;
-        const int t0 = j * kN + (lane & 7) * 16;
+        const int t0 = tok_base + j * kN + (lane & 7) * 16;
         // a lane at the start of a page's share of the tile copies it; a page is
         // copied whole, past the request's last token too
         const bool leads = lane < kN / 16 && t0 <= len - 1 && ((lane * 16) & (page_tokens - 1)) == 0;
@@ -534,6 +559,59 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
   tc_fence_after();
   if (warp == kMmaWarp) tmem_dealloc(tmem, kTmemCols);
   if (threadIdx.x == 0 && sh_fail) atomicOr(p.status, GRM_B200_PLAN_WAIT);
+  if (parts == 1) return;
+
+  // ---- the last of a tile's parts to end joins them all, in their order: eight
+  // lanes a row
+  if (threadIdx.x == 0) {
+    unsigned arrived;
+    unsigned* count = p.l.qcount + tile.w * p.kv_heads + h;
+    asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;"
+                 : "=r"(arrived)
+                 : "l"(count)
+                 : "memory");
+    sh_last = arrived + 1 == (unsigned)parts;
+    if (sh_last) *count = 0;  // for the next call
+  }
+  __syncthreads();
+  if (!sh_last) return;
+  constexpr int kDims = D / 8;
+  const float* slot0 = p.l.qpart + ((int64_t)tile.w * p.kv_heads + h) * prompt_slot(D);
+  const int64_t step = (int64_t)p.kv_heads * prompt_slot(D);
+#pragma unroll 1
+  for (int r = threadIdx.x / 8; r < LY::kQueries * kM; r += kPromptThreads / 8) {
+    const int t = r / kM, x = r % kM;
+    if (x >= (t == 0 ? toks[0] : toks[1]) * p.group) continue;
+    const float* sums = slot0 + prompt_rows_of(D) * D + 2 * r;
+    float top = -INFINITY, sum = 0.0f, acc[kDims] = {};
+    for (int q = 0; q < parts; ++q) top = fmaxf(top, __ldcg(sums + q * step));
+#pragma unroll 2
+    for (int q = 0; q < parts; ++q) {
+      const float2 ml = __ldcg(reinterpret_cast<const float2*>(sums + q * step));
+      const float a = ml.x == top ? 1.0f : ex2(ml.x - top);
+      sum += ml.y == 0.0f ? 0.0f : ml.y * a;
+      const float4* src = reinterpret_cast<const float4*>(slot0 + q * step + r * D) +
+                          (threadIdx.x & 7) * (kDims / 4);
+#pragma unroll
+      for (int i = 0; i < kDims / 4; ++i) {
+        const float4 v = __ldcg(src + i);
+        acc[4 * i] = fmaf(v.x, a, acc[4 * i]);
+        acc[4 * i + 1] = fmaf(v.y, a, acc[4 * i + 1]);
+        acc[4 * i + 2] = fmaf(v.z, a, acc[4 * i + 2]);
+        acc[4 * i + 3] = fmaf(v.w, a, acc[4 * i + 3]);
+      }
+    }
+    const int64_t orow = (int64_t)(start + tok0 + t * per + x / p.group) * heads + h * p.group +
+                         x % p.group;
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    uint2* out = reinterpret_cast<uint2*>(p.out + orow * D + (threadIdx.x & 7) * kDims);
+#pragma unroll
+    for (int i = 0; i < kDims / 4; ++i)
+      out[i] = make_uint2(pack_out<T>(acc[4 * i] * inv, acc[4 * i + 1] * inv),
+                          pack_out<T>(acc[4 * i + 2] * inv, acc[4 * i + 3] * inv));
+    if (p.lse && (threadIdx.x & 7) == 0)
+      p.lse[orow] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.693147180559945309f;
+  }
 }
 
 template <typename T, int D>
