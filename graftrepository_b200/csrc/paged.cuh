@@ -21,8 +21,10 @@ __host__ __device__ constexpr int split_blocks(int dim, int rows) {
 // fp32 of one partial result: rows x dim, then (reference exponent, sum) a row.
 __host__ __device__ constexpr int split_slot(int dim, int rows) { return rows * dim + 2 * rows; }
 
-// Query rows of a prompt tile, and fp32 of one part's result.
+// Query rows and tokens of a step of a prompt tile, and fp32 of one part's result:
+// [dim / 4][rows][4], then (reference exponent, sum) a row.
 __host__ __device__ constexpr int prompt_rows_of(int dim) { return dim == 256 ? 128 : 256; }
+__host__ __device__ constexpr int prompt_step_of(int dim) { return dim == 256 ? 64 : 128; }
 __host__ __device__ constexpr int prompt_slot(int dim) { return prompt_rows_of(dim) * (dim + 2); }
 
 struct Header {           // written by the plan kernel
@@ -31,6 +33,7 @@ struct Header {           // written by the plan kernel
   int32_t share, more;    // units of a worker, and how many workers have one more
   int32_t pages;          // entries of the append list
   int32_t qtiles;         // entries of the prompt kernel's list: parts of prompt tiles
+  int32_t joins;          // qtiles, where tiles are in more than one part; 0 where none is
   int32_t rows;           // packed rows of the step
 };
 
@@ -47,7 +50,7 @@ struct Shape {
   int64_t qtile_cap;    // most entries of the prompt kernel's list (0: no request can be a prompt)
   // byte offsets in the scratch
   int64_t off_base, off_start, off_count, off_pages, off_qtiles, off_part;
-  int64_t off_qcount, off_qpart, bytes;
+  int64_t off_qpart, bytes;
 };
 
 int make_shape(const grm_b200_paged_plan& p, int sms, Shape* s);
@@ -62,7 +65,6 @@ struct Lists {
   // parts, first entry of the tile)
   int4* qtiles;
   float* part;        // [workers * 2][split_slot]
-  unsigned* qcount;   // [sms] arrivals at a prompt tile and head in parts; 0 between calls
   float* qpart;       // [sms][prompt_slot]
 };
 
@@ -75,7 +77,6 @@ inline Lists lists_of(const Shape& s, void* scratch) {
           reinterpret_cast<int4*>(b + s.off_pages),
           reinterpret_cast<int4*>(b + s.off_qtiles),
           reinterpret_cast<float*>(b + s.off_part),
-          reinterpret_cast<unsigned*>(b + s.off_qcount),
           reinterpret_cast<float*>(b + s.off_qpart)};
 }
 
@@ -114,6 +115,30 @@ struct AttendParams {
 
 // Rows of the requests that the plan made prompts (paged_prompt.cu).
 int launch_prompt(int dtype, int dim, const AttendParams& p, int64_t blocks, cudaStream_t st);
+
+// A prompt tile from its entry in the list: 128-row query tiles of `per` tokens,
+// the second one empty where the rows fit one.
+struct PromptTile {
+  int start, cached, len, tok0, per, toks[2];
+  int steps;  // of the tokens that its rows see
+  int parts;  // blocks that share them
+};
+template <int D>
+__device__ __forceinline__ PromptTile prompt_tile(const AttendParams& p, int4 e) {
+  PromptTile t;
+  t.start = p.starts[e.x];
+  const int n = p.starts[e.x + 1] - t.start;
+  t.len = p.lens[e.x];
+  t.cached = t.len - n;
+  t.per = p.qtile_tokens / (prompt_rows_of(D) / 128);
+  t.tok0 = e.y;
+  t.toks[0] = min(t.per, n - t.tok0);
+  t.toks[1] = prompt_rows_of(D) == 256 ? max(0, min(t.per, n - t.tok0 - t.per)) : 0;
+  const int sees = p.causal ? min(t.len, t.cached + t.tok0 + t.toks[0] + t.toks[1]) : t.len;
+  t.steps = (sees + prompt_step_of(D) - 1) / prompt_step_of(D);
+  t.parts = max(1, min(e.z >> 8, t.steps));
+  return t;
+}
 
 __device__ __forceinline__ float ex2(float x) {
   float y;

@@ -231,6 +231,74 @@ __device__ __noinline__ void join_row(const AttendParams& p, int wa, int n, int 
     p.lse[out_row] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.693147180559945309f;
 }
 
+// Prompt tiles that the prompt kernel left in parts: a warp takes eight rows and 16
+// dims, four a lane, and adds the parts up in their order, eight loads in flight.
+// As the last part's own work, by one block, it took 42 us for 256 rows of head_dim
+// 128 in 8 parts; over all blocks it takes 3.
+template <typename T, int D>
+__device__ __noinline__ void join_prompts(const AttendParams& p, int entries) {
+  constexpr int kRows = prompt_rows_of(D), kItems = kRows / 8 * (D / 16), kAhead = 8;
+  const int lane = threadIdx.x & 31, warps = gridDim.x * kWarps;
+  const int heads = p.kv_heads * p.group, items = p.kv_heads * kItems;
+  const int64_t step = (int64_t)p.kv_heads * prompt_slot(D);
+  int next = blockIdx.x * kWarps + (threadIdx.x >> 5);
+  for (int e0 = 0; e0 < entries; e0 += 32) {
+    const int4 mine = p.l.qtiles[min(e0 + lane, entries - 1)];
+    const int my_parts = prompt_tile<D>(p, mine).parts;
+    unsigned todo = __ballot_sync(kFull, e0 + lane < entries && (mine.z & 255) == 0 && my_parts > 1);
+    for (; todo; todo &= todo - 1) {
+      const int4 e = p.l.qtiles[e0 + __ffs(todo) - 1];
+      const PromptTile t = prompt_tile<D>(p, e);
+      for (; next < items; next += warps) {
+        const int h = next / kItems, x = next % kItems;
+        const int r = x / (D / 16) * 8 + (lane & 7), c = x % (D / 16) * 4 + (lane >> 3);
+        const int q = r / 128, in = r % 128;
+        if (in >= (q == 0 ? t.toks[0] : t.toks[1]) * p.group) continue;
+        const float* part = p.l.qpart + ((int64_t)e.w * p.kv_heads + h) * prompt_slot(D);
+        const float4* src = reinterpret_cast<const float4*>(part) + c * kRows + r;
+        const float2* sums = reinterpret_cast<const float2*>(part + kRows * D) + r;
+        float top = -INFINITY, sum = 0.0f;
+        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int i0 = 0; i0 < t.parts; i0 += kAhead) {
+          float2 ml[kAhead];
+          float4 v[kAhead];
+#pragma unroll
+          for (int i = 0; i < kAhead; ++i) {
+            const int64_t at = min(i0 + i, t.parts - 1) * step;
+            ml[i] = __ldcg(sums + at / 2);
+            v[i] = __ldcg(src + at / 4);
+          }
+          float high = top;
+#pragma unroll
+          for (int i = 0; i < kAhead; ++i) high = fmaxf(high, ml[i].x);
+          const float a = top == high ? 1.0f : ex2(top - high);
+          top = high;
+          sum *= a;
+          acc = make_float4(acc.x * a, acc.y * a, acc.z * a, acc.w * a);
+#pragma unroll
+          for (int i = 0; i < kAhead; ++i) {
+            if (i0 + i >= t.parts) break;
+            const float w = ml[i].x == top ? 1.0f : ex2(ml[i].x - top);
+            sum += ml[i].y == 0.0f ? 0.0f : ml[i].y * w;
+            acc.x = fmaf(v[i].x, w, acc.x);
+            acc.y = fmaf(v[i].y, w, acc.y);
+            acc.z = fmaf(v[i].z, w, acc.z);
+            acc.w = fmaf(v[i].w, w, acc.w);
+          }
+        }
+        const int64_t row = (int64_t)(t.start + t.tok0 + q * t.per + in / p.group) * heads +
+                            h * p.group + in % p.group;
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        reinterpret_cast<uint2*>(p.out + row * D)[c] =
+            make_uint2(pack_out<T>(acc.x * inv, acc.y * inv), pack_out<T>(acc.z * inv, acc.w * inv));
+        if (p.lse && c == 0)
+          p.lse[row] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.693147180559945309f;
+      }
+      next -= items;
+    }
+  }
+}
+
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kThreads, (Layout<D, NT>::kBlocks))
     split_kernel(const __grid_constant__ SplitParams sp) {
@@ -264,6 +332,7 @@ __global__ void __launch_bounds__(kThreads, (Layout<D, NT>::kBlocks))
     if (p.lse)
       for (int x = threadIdx.x; x < heads; x += kThreads) p.lse[i * heads + x] = -INFINITY;
   }
+  if (hd.joins > 0) join_prompts<T, D>(p, hd.joins);
   if (w >= hd.workers) return;
   const int begin = worker_first(w, hd), end = worker_first(w + 1, hd);
   Walk<LY::kTokens * kWarps> walk(p, begin, end, request0);
@@ -914,12 +983,12 @@ int grm_b200_paged_attend(const grm_b200_paged_plan* plan, const grm_b200_paged_
   p.qtile_tokens = s.qtile_tokens;
   p.status = plan->status;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  rc = dtype == GRM_B200_F16
-           ? launch_split_any<__half>(plan->head_dim, s.block_rows, sp, s.workers, st)
-           : launch_split_any<__nv_bfloat16>(plan->head_dim, s.block_rows, sp, s.workers, st);
-  if (rc == 0 && s.qtile_cap > 0)
-    rc = launch_prompt(dtype, plan->head_dim, p, s.qtile_cap * plan->kv_heads, st);
-  return rc;
+  if (s.qtile_cap > 0 &&
+      (rc = launch_prompt(dtype, plan->head_dim, p, s.qtile_cap * plan->kv_heads, st)))
+    return rc;
+  return dtype == GRM_B200_F16
+             ? launch_split_any<__half>(plan->head_dim, s.block_rows, sp, s.workers, st)
+             : launch_split_any<__nv_bfloat16>(plan->head_dim, s.block_rows, sp, s.workers, st);
 }
 
 }  // extern "C"

@@ -256,11 +256,10 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
                            workers ? units % workers : 0,
                            failed ? 0 : (int)total[kTouched],
                            failed ? 0 : (int)total[kTiles],
+                           failed || part_tokens == 0 ? 0 : (int)total[kTiles],
                            all_rows};
     }
     for (int i = tid; i < p.s.workers; i += kPlanThreads) p.l.count[i] = 0;
-    if (p.s.qtile_cap > 0)
-      for (int i = tid; i < p.sms; i += kPlanThreads) p.l.qcount[i] = 0;
   }
   if (kind == kWriteRows)
     for (int64_t i = all_rows + (int64_t)chunk * gsize + gid; i < p.tokens;
@@ -476,7 +475,6 @@ int make_shape(const grm_b200_paged_plan& p, int sms, Shape* s) {
   s->off_pages = take(std::min(T, T / p.page_tokens + 2 * std::min(R, T)) * 16);
   s->off_qtiles = take(s->qtile_cap * 16);
   s->off_part = take((int64_t)s->workers * 2 * split_slot(p.head_dim, s->block_rows) * 4);
-  s->off_qcount = take(prompts ? (int64_t)sms * 4 : 0);
   s->off_qpart = take(prompts ? (int64_t)sms * prompt_slot(p.head_dim) * 4 : 0);
   s->bytes = at;
   return 0;

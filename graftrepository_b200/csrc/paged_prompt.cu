@@ -52,8 +52,8 @@ constexpr unsigned kProbes = 1u << 18;  // probes of a bounded wait
 // and key tiles of one step, and the other tile's softmax warps convert codes.
 template <int D>
 struct PromptLayout {
-  static constexpr int kQueries = D == 256 ? 1 : 2;     // query tiles
-  static constexpr int kN = D == 256 ? 64 : 128;        // tokens of a key tile
+  static constexpr int kQueries = prompt_rows_of(D) / kM;  // query tiles
+  static constexpr int kN = prompt_step_of(D);          // tokens of a key tile
   static constexpr int kHalves = kN / kHalf;
   static constexpr int kSoftWarps = 4 * kQueries;
   static constexpr int kConvWarps = kMmaWarp - kSoftWarps;
@@ -123,7 +123,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
   __shared__ __align__(8) uint64_t q_full[2], drained[2], k_full[2], k_empty[2], v_full[2], v_empty[2],
       scale_full[kRing], raw_full[2], raw_empty[2], s_full[2][2], p_full[2][2], o_full[2], o_done[2];
   __shared__ uint32_t sh_tmem;
-  __shared__ int sh_fail, sh_last;
+  __shared__ int sh_fail;
 
   const Header hd = *p.l.header;
   const int h = blockIdx.x % p.kv_heads;
@@ -132,28 +132,21 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int4 tile = p.l.qtiles[ti];
-  const int start = p.starts[tile.x];
-  const int n = p.starts[tile.x + 1] - start;
-  const int len = p.lens[tile.x];
-  const int cached = len - n;
-  const int per = p.qtile_tokens / LY::kQueries;  // tokens of one query tile
-  const int tok0 = tile.y;
-  const int toks[2] = {min(per, n - tok0),
-                       LY::kQueries == 2 ? max(0, min(per, n - tok0 - per)) : 0};
-  const bool two = toks[1] > 0;
+  const PromptTile pt = prompt_tile<D>(p, tile);
+  const int start = pt.start, len = pt.len, cached = pt.cached, tok0 = pt.tok0, per = pt.per;
+  const int all_tiles = pt.steps, parts = pt.parts, part = tile.z & 255;
+  const bool two = pt.toks[1] > 0;
   const int heads = p.kv_heads * p.group;
-  const int sees = p.causal ? min(len, cached + tok0 + toks[0] + toks[1]) : len;
-  const int all_tiles = (sees + kN - 1) / kN;
-  // the part of them that is this block's, and what it begins with
-  const int parts = max(1, min(tile.z >> 8, all_tiles)), part = tile.z & 255;
+  if (part >= parts) return;
+  // the block's share of the key tiles, and the tokens that its rows see in it
   const int tile0 = (int)((int64_t)all_tiles * part / parts);
   const int tiles = (int)((int64_t)all_tiles * (part + 1) / parts) - tile0;
   const int tok_base = tile0 * kN;
+  const int sees = p.causal ? min(len, cached + tok0 + pt.toks[0] + pt.toks[1]) : len;
   const int halves_seen = (min(sees - tok_base, tiles * kN) + kHalf - 1) / kHalf;
-  if (part >= parts) return;
 
   if (all_tiles == 0) {  // nothing cached: empty rows
-    for (int x = threadIdx.x; x < (toks[0] + toks[1]) * p.group * (D / 2); x += kPromptThreads) {
+    for (int x = threadIdx.x; x < (pt.toks[0] + pt.toks[1]) * p.group * (D / 2); x += kPromptThreads) {
       const int j = x / (D / 2);
       const int64_t row = (int64_t)(start + tok0 + j / p.group) * heads + h * p.group + j % p.group;
       reinterpret_cast<uint32_t*>(p.out + row * D)[x % (D / 2)] = 0;
@@ -198,7 +191,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
     const int t = warp >> 2;
     if (t == 0 || two) {
       const int row = (warp & 3) * 32 + lane;
-      const bool active = row < (t == 0 ? toks[0] : toks[1]) * p.group;
+      const bool active = row < (t == 0 ? pt.toks[0] : pt.toks[1]) * p.group;
       const int token = tok0 + t * per + row / p.group;
       const int64_t orow = (int64_t)(start + token) * heads + h * p.group + row % p.group;
       // tokens that the row sees, from the part's first on
@@ -331,10 +324,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
       }
       if (ok && warp_wait(&o_done[t], 0, fail)) {
         tc_fence_after();
-        if (parts > 1) {  // the part's result, to be joined
+        if (parts > 1) {  // the part's result, for the split kernel to join
           float* slot = p.l.qpart +
                         ((int64_t)(tile.w + part) * p.kv_heads + h) * prompt_slot(D);
-          float* to = slot + (t * kM + row) * D;
+          float4* to = reinterpret_cast<float4*>(slot) + t * kM + row;
 #pragma unroll 1
           for (int c = 0; c < D / 16; ++c) {
             uint32_t v[16];
@@ -342,8 +335,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
             if (active)
 #pragma unroll
               for (int i = 0; i < 4; ++i)
-                reinterpret_cast<uint4*>(to + 16 * c)[i] =
-                    make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+                to[(4 * c + i) * prompt_rows_of(D)] =
+                    make_float4(__uint_as_float(v[4 * i]), __uint_as_float(v[4 * i + 1]),
+                                __uint_as_float(v[4 * i + 2]), __uint_as_float(v[4 * i + 3]));
           }
           if (active)
             *reinterpret_cast<float2*>(slot + prompt_rows_of(D) * D + 2 * (t * kM + row)) =
@@ -559,59 +553,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
   tc_fence_after();
   if (warp == kMmaWarp) tmem_dealloc(tmem, kTmemCols);
   if (threadIdx.x == 0 && sh_fail) atomicOr(p.status, GRM_B200_PLAN_WAIT);
-  if (parts == 1) return;
-
-  // ---- the last of a tile's parts to end joins them all, in their order: eight
-  // lanes a row
-  if (threadIdx.x == 0) {
-    unsigned arrived;
-    unsigned* count = p.l.qcount + tile.w * p.kv_heads + h;
-    asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;"
-                 : "=r"(arrived)
-                 : "l"(count)
-                 : "memory");
-    sh_last = arrived + 1 == (unsigned)parts;
-    if (sh_last) *count = 0;  // for the next call
-  }
-  __syncthreads();
-  if (!sh_last) return;
-  constexpr int kDims = D / 8;
-  const float* slot0 = p.l.qpart + ((int64_t)tile.w * p.kv_heads + h) * prompt_slot(D);
-  const int64_t step = (int64_t)p.kv_heads * prompt_slot(D);
-#pragma unroll 1
-  for (int r = threadIdx.x / 8; r < LY::kQueries * kM; r += kPromptThreads / 8) {
-    const int t = r / kM, x = r % kM;
-    if (x >= (t == 0 ? toks[0] : toks[1]) * p.group) continue;
-    const float* sums = slot0 + prompt_rows_of(D) * D + 2 * r;
-    float top = -INFINITY, sum = 0.0f, acc[kDims] = {};
-    for (int q = 0; q < parts; ++q) top = fmaxf(top, __ldcg(sums + q * step));
-#pragma unroll 2
-    for (int q = 0; q < parts; ++q) {
-      const float2 ml = __ldcg(reinterpret_cast<const float2*>(sums + q * step));
-      const float a = ml.x == top ? 1.0f : ex2(ml.x - top);
-      sum += ml.y == 0.0f ? 0.0f : ml.y * a;
-      const float4* src = reinterpret_cast<const float4*>(slot0 + q * step + r * D) +
-                          (threadIdx.x & 7) * (kDims / 4);
-#pragma unroll
-      for (int i = 0; i < kDims / 4; ++i) {
-        const float4 v = __ldcg(src + i);
-        acc[4 * i] = fmaf(v.x, a, acc[4 * i]);
-        acc[4 * i + 1] = fmaf(v.y, a, acc[4 * i + 1]);
-        acc[4 * i + 2] = fmaf(v.z, a, acc[4 * i + 2]);
-        acc[4 * i + 3] = fmaf(v.w, a, acc[4 * i + 3]);
-      }
-    }
-    const int64_t orow = (int64_t)(start + tok0 + t * per + x / p.group) * heads + h * p.group +
-                         x % p.group;
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    uint2* out = reinterpret_cast<uint2*>(p.out + orow * D + (threadIdx.x & 7) * kDims);
-#pragma unroll
-    for (int i = 0; i < kDims / 4; ++i)
-      out[i] = make_uint2(pack_out<T>(acc[4 * i] * inv, acc[4 * i + 1] * inv),
-                          pack_out<T>(acc[4 * i + 2] * inv, acc[4 * i + 3] * inv));
-    if (p.lse && (threadIdx.x & 7) == 0)
-      p.lse[orow] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.693147180559945309f;
-  }
 }
 
 template <typename T, int D>
