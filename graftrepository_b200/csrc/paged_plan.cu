@@ -31,7 +31,7 @@ constexpr int kPlanThreads = 1024;
 constexpr int kPlanWarps = kPlanThreads / 32;
 constexpr int kJoinUnits = 5;
 constexpr int kBuckets = 256;  // of prompt tiles by what they see
-constexpr int kPartTokens = 512;  // a part of a prompt tile has no fewer
+constexpr int kPartTokens = 256;  // a part of a prompt tile has no fewer
 // The sums over requests: pages taken, rows, pages touched, prompt tiles (all
 // of them below 2^31 in a step that can be planned) and the split kernel's units.
 constexpr int kSums = 6;
