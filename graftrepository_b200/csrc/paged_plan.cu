@@ -529,7 +529,7 @@ int check_sizes(const grm_b200_paged_plan* p) {
     set_thread_error("paged plan: null plan");
     return GRM_B200_EINVAL;
   }
-  if (p->requests < 1 || p->requests > (1 << 24) || p->tokens < 1 || p->tokens > INT32_MAX ||
+  if (p->requests < 1 || p->requests > (1 << 20) || p->tokens < 1 || p->tokens > INT32_MAX ||
       p->max_fresh < 1 || p->table_width < 1 || p->table_width > (1 << 28) || p->pages < 1 ||
       p->pages > INT32_MAX) {
     set_thread_error("paged plan: sizes out of range (requests %lld, tokens %lld, max_fresh %lld, "

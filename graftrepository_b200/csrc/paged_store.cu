@@ -388,7 +388,7 @@ int grm_b200_paged_read(const grm_b200_paged_arena* arena, const int64_t* slots_
   if (!slots_device || count < 0 || !out_k_device || !out_v_device ||
       ((reinterpret_cast<uintptr_t>(out_k_device) | reinterpret_cast<uintptr_t>(out_v_device)) &
        15) ||
-      count * arena->kv_heads * (arena->head_dim / 16) > (int64_t)INT32_MAX * 256) {
+      count > (int64_t)INT32_MAX * 256 / (arena->kv_heads * (arena->head_dim / 16))) {
     set_thread_error("invalid paged read arguments (count %lld; outputs must be 16-byte aligned)",
                      (long long)count);
     return GRM_B200_EINVAL;

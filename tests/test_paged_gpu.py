@@ -443,6 +443,22 @@ def test_prompts_on_many_heads(dim, group, page, kind, causal):
 
 
 @pytest.mark.parametrize("kind", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("lens,fresh", [([5000], [40]), ([9001, 130, 700], [33, 129, 70]),
+                                        ([3000, 90, 2000], [300, 64, 1])])
+@pytest.mark.parametrize("causal", [True, False])
+def test_prompts_in_parts(lens, fresh, dim, kind, causal):
+    """Few prompt tiles over long contexts, which several blocks share."""
+    run_attention(lens, fresh, heads=2, group=4, dim=dim, page=64, kind=kind, causal=causal, seed=41)
+
+
+def test_prompts_in_parts_on_one_head():
+    """All of the GPU on one tile, some parts past what a causal row sees."""
+    run_attention([40000], [20], heads=1, group=8, dim=128, page=128, seed=42)
+    run_attention([300], [260], heads=1, group=1, dim=128, page=16, seed=43)
+
+
+@pytest.mark.parametrize("kind", [torch.bfloat16, torch.float16])
 def test_prompts_and_single_tokens_in_one_step(kind):
     run_attention([2000, 700, 350, 1, 900, 1500], [1, 600, 0, 1, 1, 130], heads=2, group=4, dim=128,
                   page=64, kind=kind, seed=3)
