@@ -372,9 +372,14 @@ inline Ranges policy_ranges(const Policy& P, const char* blob, int* m_out) {
 }
 
 // pass 0: hits[node] += 1 over every posting; pass 1: take the counts into
-// the hit list (and leave hits zero).
+// the hit list, from its start (and leave hits zero).  The list has room for
+// every node once, so its counter starts at 0 in each query.
 inline int policy_pass(Policy& P, const Ranges& ranges, int pass, int sms, cudaStream_t s,
                        ErrorSlot& err) {
+  if (pass == 1) {
+    const cudaError_t e = cudaMemsetAsync(P.d_counter, 0, sizeof(uint32_t), s);
+    if (e != cudaSuccess) return err.set(cuda_status(e), "lexical counter reset failed");
+  }
   for (size_t c0 = 0; c0 < ranges.size(); c0 += kItemsPerLaunch) {
     ItemRanges r;
     std::memset(&r, 0, sizeof(r));
@@ -410,8 +415,6 @@ inline int policy_collect(Policy& P, const char* blob, int sms, cudaStream_t s, 
     for (const auto& r : ranges) *postings += r.second;
   }
   if (*m_out == 0) return 0;
-  cudaError_t e = cudaMemsetAsync(P.d_counter, 0, sizeof(uint32_t), s);
-  if (e != cudaSuccess) return err.set(cuda_status(e), "lexical counter reset failed");
   int rc = policy_pass(P, ranges, 0, sms, s, err);
   if (!rc) rc = policy_pass(P, ranges, 1, sms, s, err);
   return rc;
