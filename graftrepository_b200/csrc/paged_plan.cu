@@ -32,11 +32,13 @@ constexpr int kPlanWarps = kPlanThreads / 32;
 constexpr int kJoinUnits = 5;
 constexpr int kBuckets = 256;  // of prompt tiles by what they see
 constexpr int kPartTokens = 256;  // a part of a prompt tile has no fewer
-// The sums over requests: pages taken, rows, pages touched, prompt tiles (all
-// of them below 2^31 in a step that can be planned) and the split kernel's units.
-constexpr int kSums = 6;
+// The sums over requests: pages taken, rows, pages touched, prompt tiles or their
+// parts (all of them below 2^31 in a step that can be planned) and the split
+// kernel's units; and two that only totals are needed of, the split kernel's
+// segments and the tokens of the requests of all prompt tiles.
+constexpr int kSums = 7;
 constexpr int kTake = 0, kRows = 1, kTouched = 2, kTiles = 3, kUnits = 4;
-constexpr int kSegments = 5;  // of the split kernel; only their number is needed
+constexpr int kSegments = 5, kTokens = 6;
 
 struct PlanParams {
   int64_t requests, tokens, max_fresh, width, ring_size;
@@ -63,22 +65,22 @@ struct Request {
   int cached, fresh, after, have, need;
 };
 
-// What request r adds to each sum.
 // Parts of a prompt request's tiles, for `part_tokens` in each (0: whole).
 __device__ __forceinline__ int parts_of(int after, int part_tokens) {
   return part_tokens == 0 ? 1 : max(1, (after + part_tokens - 1) / part_tokens);
 }
 
-__device__ __forceinline__ void weigh(const PlanParams& p, const Request& q, int part_tokens,
-                                      int64_t (&v)[kSums]) {
+// What request r adds to each sum, its prompt tiles whole.
+__device__ __forceinline__ void weigh(const PlanParams& p, const Request& q, int64_t (&v)[kSums]) {
   v[kTake] = q.need - q.have;
   v[kRows] = q.fresh;
   v[kTouched] = p.grow && q.fresh > 0 ? q.need - (q.cached >> p.page_shift) : 0;
   const int64_t pairs = (int64_t)q.fresh * p.s.group;
   const bool prompt = pairs > p.s.prompt_rows && p.s.qtile_cap > 0;
   v[kTiles] = prompt ? (int64_t)(((unsigned)q.fresh + p.s.qtile_tokens - 1) /
-                                 (unsigned)p.s.qtile_tokens) * parts_of(q.after, part_tokens)
+                                 (unsigned)p.s.qtile_tokens)
                      : 0;
+  v[kTokens] = v[kTiles] * q.after;
   v[kSegments] = prompt ? 0 : p.kv_heads * ((pairs + p.s.block_rows - 1) >> p.block_shift);
   v[kUnits] = v[kSegments] * (((q.after + p.s.tile - 1) >> p.tile_shift) + 1);
 }
@@ -159,37 +161,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
     return q;
   };
 
-  // ---- prompts.  A prompt tile and head is one block; where they are fewer than
-  // half of the SMs, tiles are cut along their tokens into parts, as many as there
-  // are SMs beyond the tiles: Sum ceil(len / part) <= Sum len / part + tiles, so all
-  // parts run at once.
-  int part_tokens = 0;
   if (tid == 0) bad = 0;
-  if (p.s.qtile_cap > 0) {
-    int64_t tiles = 0, tokens = 0;
-    for (int64_t r = tid; r < p.requests; r += kPlanThreads) {
-      const int cached = max(p.cached[r], 0), fresh = p.fresh[r];
-      if (fresh > 0 && (int64_t)fresh * p.s.group > p.s.prompt_rows) {
-        const int x = ((unsigned)fresh + p.s.qtile_tokens - 1) / (unsigned)p.s.qtile_tokens;
-        tiles += x;
-        tokens += (int64_t)x * (cached + (p.grow ? (int64_t)fresh : 0));
-      }
-    }
-    tiles = warp_sum(tiles);
-    tokens = warp_sum(tokens);
-    if (lane == 0) {
-      part[0][warp] = tiles;
-      part[1][warp] = tokens;
-    }
-    __syncthreads();
-    tiles = warp_sum(part[0][lane]) * p.kv_heads;
-    tokens = warp_sum(part[1][lane]) * p.kv_heads;
-    if (tiles > 0 && tiles <= p.sms / 2) {
-      const int64_t each = ceil_div64(tokens, p.sms - tiles);
-      part_tokens = (int)(each < kPartTokens ? kPartTokens : each < (1 << 30) ? each : 1 << 30);
-    }
-    __syncthreads();
-  }
 
   // ---- totals, the chunk's own requests, and errors
   int64_t v[kSums] = {}, before[kSums] = {}, own[kSums] = {};
@@ -198,7 +170,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
   for (int c = 0; c < p.chunks; ++c) {
     int64_t a[kSums];
     const Request x = request((int64_t)c * kPlanThreads + tid, &flags);
-    weigh(p, x, part_tokens, a);
+    weigh(p, x, a);
     if (c == chunk) {
       q = x;
 #pragma unroll
@@ -227,6 +199,41 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
   }
   __syncthreads();
   int failed = bad;
+
+  // A prompt tile and head is one block; where they are fewer than half of the SMs,
+  // tiles are cut along their tokens into parts, as many as there are SMs beyond the
+  // tiles: Sum ceil(len / part) <= Sum len / part + tiles, so all parts run at once.
+  int part_tokens = 0;
+  const int64_t whole = total[kTiles] * p.kv_heads;
+  if (whole > 0 && whole <= p.sms / 2) {
+    const int64_t each = ceil_div64(total[kTokens] * p.kv_heads, p.sms - whole);
+    part_tokens = (int)(each < kPartTokens ? kPartTokens : each < (1 << 30) ? each : 1 << 30);
+    int64_t sum_parts = 0, sum_before = 0;
+    for (int c = 0; c < p.chunks; ++c) {
+      const Request x = c == chunk ? q : request((int64_t)c * kPlanThreads + tid, &flags);
+      int64_t a[kSums];
+      weigh(p, x, a);
+      a[kTiles] *= parts_of(x.after, part_tokens);
+      if (c == chunk) {
+        sum_before = sum_parts;
+        own[kTiles] = a[kTiles];
+      }
+      sum_parts += a[kTiles];
+    }
+    sum_parts = warp_sum(sum_parts);
+    sum_before = warp_sum(sum_before);
+    if (lane == 0) {
+      part[0][warp] = sum_parts;
+      part[1][warp] = sum_before;
+    }
+    __syncthreads();  // the tiles' totals have been read too
+    if (warp < 2) {
+      const int64_t w = warp_sum(part[warp][lane]);
+      if (lane == 0) total[warp == 0 ? kTiles : kSums + kTiles] = w;
+    }
+    __syncthreads();
+  }
+
   if (total[kRows] > p.tokens || total[kUnits] > INT32_MAX - (1 << 20))
     failed |= GRM_B200_PLAN_ROWS;
   if (taken0 < 0 || returned - taken0 > p.ring_size || total[kTake] > returned - taken0)

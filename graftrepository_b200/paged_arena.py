@@ -110,6 +110,15 @@ def _empty(like, shape, dtype, stream):
         return like.new_empty(shape, dtype=dtype)
 
 
+def _result(pattern, stream):
+    """The same of `pattern`'s shape and type, contiguous (1.4 us, where new_empty
+    takes 2.0 to 2.7)."""
+    if stream is None:
+        return torch.empty_like(pattern, memory_format=torch.contiguous_format)
+    with torch.cuda.stream(_torch_stream(stream, pattern.get_device())):
+        return torch.empty_like(pattern, memory_format=torch.contiguous_format)
+
+
 def _device(device):
     d = torch.device(device)
     if d.type != "cuda":
@@ -156,6 +165,11 @@ class PagePlan:
         self.device, self._index = tables.device, tables._index
         self.query_shape = torch.Size((self.tokens, query_heads, head_dim))
         self.kv_shape = torch.Size((self.tokens, kv_heads, head_dim))
+
+        # shapes and types of attention's results, one element each
+        self._out_like = {kind: torch.empty(1, dtype=kind, device=self.device).expand(
+            self.query_shape) for kind in _TYPES}
+        self._lse_like = torch.empty(1, device=self.device).expand(self.query_shape[:2])
 
         def ints(n, dtype=torch.int32):
             return torch.zeros(n, dtype=dtype, device=self.device)
@@ -318,12 +332,13 @@ class PagedArena:
             raise ValueError(f"layer {layer} of {self.layers}")
         return self._refs[layer]
 
-    def _result(self, name, t, like, shape, dtype, stream):
+    def _result(self, name, t, pattern, stream):
         if t is None:
-            return _empty(like, shape, dtype, stream)
-        if (t.shape != shape or t.dtype is not dtype or t.get_device() != self._index or
-                not t.is_contiguous()):
-            raise ValueError(f"{name} must be contiguous {dtype} {list(shape)} on {self.device}")
+            return _result(pattern, stream)
+        if (t.shape != pattern.shape or t.dtype is not pattern.dtype or
+                t.get_device() != self._index or not t.is_contiguous()):
+            raise ValueError(f"{name} must be contiguous {pattern.dtype} {list(pattern.shape)} on "
+                             f"{self.device}")
         return t
 
     def append(self, plan: PagePlan, k, v, *, layer: int = 0, stream=None) -> None:
@@ -347,13 +362,12 @@ class PagedArena:
         head_dim ** -0.5.  Returns (out like q, lse fp32 [tokens, query_heads]);
         rows that see nothing are 0 with lse -inf."""
         ref = self._ready(plan, layer)
-        shape = plan.query_shape
-        kind, ptr, row, head = self._rows("q", q, shape)
+        kind, ptr, row, head = self._rows("q", q, plan.query_shape)
         if causal and not plan.grow:
             raise ValueError("rows that do not join the arena (planned with grow=False) have no "
                              "position in it; attend with causal=False")
-        out = self._result("out", out, q, shape, q.dtype, stream)
-        lse = self._result("lse", lse, q, shape[:2], torch.float32, stream)
+        out = self._result("out", out, plan._out_like[q.dtype], stream)
+        lse = self._result("lse", lse, plan._lse_like, stream)
         _call(self._attend, self._index, plan._ref, ref, ptr, kind, row, head,
               self._scale if scale is None else float(scale), 1 if causal else 0, out.data_ptr(),
               lse.data_ptr(), _handle(stream, self._index, q))
@@ -374,9 +388,8 @@ class PagedArena:
         if kind is None:
             raise ValueError(f"read gives float32, float16 or bfloat16, not {dtype}")
         n = slots.numel()
-        shape = (n, self.kv_heads, self.head_dim)
-        k = _empty(slots, shape, dtype, stream)
-        v = _empty(slots, shape, dtype, stream)
+        k = _empty(slots, (n, self.kv_heads, self.head_dim), dtype, stream)
+        v = _result(k, stream)
         if n:
             _call(self._read, self._index, self._refs[layer], slots.data_ptr(), n, kind,
                   k.data_ptr(), v.data_ptr(), _handle(stream, self._index, slots))
