@@ -58,7 +58,10 @@ struct PromptLayout {
   static constexpr int kSoftWarps = 4 * kQueries;
   static constexpr int kConvWarps = kMmaWarp - kSoftWarps;
   static constexpr int kRing = 8 / kHalves;             // key tiles whose scales are held
-  static constexpr int kQuery = (D / 64) * kQueryAtom;  // a query tile
+  // Queries in tensor memory, where the results leave room for them: the products
+  // then read keys and values alone from shared memory.
+  static constexpr bool kQTmem = kQueries * (2 * kHalf + D + D / 2) <= (int)kTmemCols;
+  static constexpr int kQuery = kQTmem ? 0 : (D / 64) * kQueryAtom;  // a query tile
   static constexpr int kAtom = kN * 128;                // kN rows x 64 halves
   static constexpr int kTile = (D / 64) * kAtom;        // a key or value tile
   static constexpr int kRaw = kN * D;                   // its codes
@@ -67,7 +70,8 @@ struct PromptLayout {
   static constexpr int kSmem = kUsed > 120 * 1024 ? kUsed : 120 * 1024;
   static constexpr uint32_t kScore = 0;                 // tensor memory columns
   static constexpr uint32_t kResult = kQueries * 2 * kHalf;
-  static_assert(kResult + kQueries * D <= kTmemCols, "score and result tiles");
+  static constexpr uint32_t kQueryCol = kResult + kQueries * D;
+  static_assert(kQueryCol + (kQTmem ? kQueries * D / 2 : 0) <= kTmemCols, "tiles");
 };
 
 // fp32 accumulators, fp16 operands, 128 rows, N columns; B K-major or (bit 16) not.
@@ -214,20 +218,40 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
         row_scale(max(m & 0xFFFFu, m >> 16), &up, &kq);
         kq *= p.scale_log2;
       }
-#pragma unroll 4
-      for (int c = 0; c < D / 8; ++c) {
+      const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+      auto chunk = [&](int c) {  // eight values
         uint4 x = active ? __ldg(qp + c) : make_uint4(0, 0, 0, 0);
         if constexpr (!std::is_same<T, __half>::value)
           x = make_uint4(scale_pair(x.x, up), scale_pair(x.y, up), scale_pair(x.z, up),
                          scale_pair(x.w, up));
-        *reinterpret_cast<uint4*>(sm_q + t * LY::kQuery + (c / 8) * kQueryAtom +
-                                  atom_byte(row, c % 8)) = x;
+        return x;
+      };
+      if constexpr (LY::kQTmem) {
+#pragma unroll 1
+        for (int c = 0; c < D / 8; c += 4) {
+          uint32_t w[16];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint4 x = chunk(c + i);
+            w[4 * i] = x.x;
+            w[4 * i + 1] = x.y;
+            w[4 * i + 2] = x.z;
+            w[4 * i + 3] = x.w;
+          }
+          tmem_st16(tmem + lanes + LY::kQueryCol + t * (D / 2) + 4 * c, w);
+        }
+        tmem_wait_st();
+        tc_fence_before();
+      } else {
+#pragma unroll 4
+        for (int c = 0; c < D / 8; ++c)
+          *reinterpret_cast<uint4*>(sm_q + t * LY::kQuery + (c / 8) * kQueryAtom +
+                                    atom_byte(row, c % 8)) = chunk(c);
+        fence_proxy_async_smem();
       }
-      fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&q_full[t]);
 
-      const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
       const uint32_t s_col = tmem + lanes + LY::kScore + t * 2 * kHalf;
       const uint32_t o_col = tmem + lanes + LY::kResult + t * D;
       float m = -INFINITY, l = 0.0f;
@@ -444,6 +468,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
         const uint32_t k_lo = (uint32_t)sw128_desc(sm_k);
         const uint32_t v_lo = (uint32_t)sw128_mn_desc(sm_v, LY::kAtom);
         const uint32_t s_at = base + LY::kScore + t * 2 * kHalf, o_at = base + LY::kResult + t * D;
+        const uint32_t q_at = base + LY::kQueryCol + t * (D / 2);
         auto scores = [&](int i) {  // half i of the tokens
           const uint32_t kd = k_lo + ((i / kHalves) & 1) * kTile16 + (i % kHalves) * kHalf16;
           const uint32_t to = s_at + (i & 1) * kHalf;
@@ -451,8 +476,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
           for (int k = 0; k < D / 16; ++k) {
             const uint32_t q_step = ((k / 4) * kQueryAtom + (k % 4) * 32) / 16;
             const uint32_t k_step = ((k / 4) * LY::kAtom + (k % 4) * 32) / 16;
-            umma_f16_if(issue, to, q_lo + q_step, kd + k_step, kHi, kHi, idesc(kHalf, false),
-                        k != 0);
+            if constexpr (LY::kQTmem)
+              umma_f16_ts_if(issue, to, q_at + 8 * k, kd + k_step, kHi, idesc(kHalf, false),
+                             k != 0);
+            else
+              umma_f16_if(issue, to, q_lo + q_step, kd + k_step, kHi, kHi, idesc(kHalf, false),
+                          k != 0);
           }
           umma_commit_if(issue, &s_full[t][i & 1]);
         };
@@ -476,7 +505,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
           if ((i + 1) % kHalves == 0) umma_commit_if(issue, &k_empty[j & 1]);
           return true;
         };
-        bool ok = warp_wait(&q_full[t], 0, fail) && next_scores(0);
+        bool ok = warp_wait(&q_full[t], 0, fail);
+        tc_fence_after();
+        ok = ok && next_scores(0);
         if (ok && steps > 1) ok = next_scores(1);
 #pragma unroll 1
         for (int i = 0; i < steps && ok; ++i) {
