@@ -125,7 +125,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
   unsigned char* const sm_raw = sm_v + 2 * LY::kTile;                 // codes: keys, values
   Scale* const sm_scale = reinterpret_cast<Scale*>(sm_raw + 2 * LY::kRaw);  // [kRing][kN / 16]
   __shared__ __align__(8) uint64_t q_full[2], drained[2], k_full[2], k_empty[2], v_full[2], v_empty[2],
-      scale_full[kRing], raw_full[2], raw_empty[2], s_full[2][2], p_full[2][2], o_full[2], o_done[2];
+      scale_full[kRing], raw_full[2], raw_empty[2], s_full[2][2], p_full[2][2], o_full[2], o_done[2], turn[2][4];
   __shared__ uint32_t sh_tmem;
   __shared__ int sh_fail;
 
@@ -175,6 +175,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
       }
       mbar_init(&o_full[i], 1);
       mbar_init(&o_done[i], 1);
+      for (int x = 0; x < 4; ++x) mbar_init(&turn[i][x], 1);
     }
     for (int i = 0; i < kRing; ++i) mbar_init(&scale_full[i], 1);
     mbar_fence_init();
@@ -197,7 +198,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
       const int row = (warp & 3) * 32 + lane;
       const bool active = row < (t == 0 ? pt.toks[0] : pt.toks[1]) * p.group;
       const int token = tok0 + t * per + row / p.group;
-      const int64_t orow = (int64_t)(start + token) * heads + h * p.group + row % p.group;
       // tokens that the row sees, from the part's first on
       const int lim = (active && p.causal ? cached + token + 1 : len) - tok_base;
 
@@ -320,6 +320,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
             }
           }
         }
+        // The two warps of a scheduler take turns at the exponentials, so that one's
+        // other work lies under them.
+        if (two && t + i > 0 &&
+            !(ok = warp_wait(&turn[t][warp & 3], (i - 1 + t) & 1, fail)))
+          break;
         const float ref = m == -INFINITY ? 0.0f : m;
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
@@ -340,6 +345,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
             l = fmaf(sum0 + sum1, sc[g].inv_value, l);
           }
           tmem_st16(s_col + buf * kHalf + 16 * c, w);
+          if (c == 0 && two && lane == 0) mbar_arrive(&turn[1 - t][warp & 3]);
         }
         tmem_wait_st();
         tc_fence_before();
@@ -348,9 +354,18 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
       }
       if (ok && warp_wait(&o_done[t], 0, fail)) {
         tc_fence_after();
-        if (parts > 1) {  // the part's result, for the split kernel to join
+        // looked up again rather than kept in registers through the loop
+        int tid;
+        asm volatile("mov.u32 %0, %%tid.x;" : "=r"(tid));
+        const int4 e = p.l.qtiles[ti];
+        const PromptTile pt = prompt_tile<D>(p, e);
+        const int t = tid >> 7, row = tid & 127;
+        const bool active = row < (t == 0 ? pt.toks[0] : pt.toks[1]) * p.group;
+        const int64_t orow = (int64_t)(pt.start + pt.tok0 + t * pt.per + row / p.group) * heads +
+                             h * p.group + row % p.group;
+        if (pt.parts > 1) {  // the part's result, for the split kernel to join
           float* slot = p.l.qpart +
-                        ((int64_t)(tile.w + part) * p.kv_heads + h) * prompt_slot(D);
+                        ((int64_t)(e.w + (e.z & 255)) * p.kv_heads + h) * prompt_slot(D);
           float4* to = reinterpret_cast<float4*>(slot) + t * kM + row;
 #pragma unroll 1
           for (int c = 0; c < D / 16; ++c) {
