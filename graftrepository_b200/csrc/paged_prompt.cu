@@ -472,7 +472,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
       const int t = __shfl_sync(kFull, warp, 0) - kMmaWarp;
       const int steps = __shfl_sync(kFull, halves_seen, 0);
       const uint32_t base = __shfl_sync(kFull, tmem, 0);
-      const uint32_t issue = lane == 0;
       if (t == 0 || two) {
         // Descriptors of the first step; later steps and stages add to the address
         // field (16-byte units), which no tile of shared memory overflows.
@@ -484,30 +483,38 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
         const uint32_t v_lo = (uint32_t)sw128_mn_desc(sm_v, LY::kAtom);
         const uint32_t s_at = base + LY::kScore + t * 2 * kHalf, o_at = base + LY::kResult + t * D;
         const uint32_t q_at = base + LY::kQueryCol + t * (D / 2);
+        auto desc = [&](uint32_t lo) { return (uint64_t)kHi << 32 | lo; };
         auto scores = [&](int i) {  // half i of the tokens
           const uint32_t kd = k_lo + ((i / kHalves) & 1) * kTile16 + (i % kHalves) * kHalf16;
           const uint32_t to = s_at + (i & 1) * kHalf;
+          if (elect_one()) {
 #pragma unroll
-          for (int k = 0; k < D / 16; ++k) {
-            const uint32_t q_step = ((k / 4) * kQueryAtom + (k % 4) * 32) / 16;
-            const uint32_t k_step = ((k / 4) * LY::kAtom + (k % 4) * 32) / 16;
-            if constexpr (LY::kQTmem)
-              umma_f16_ts_if(issue, to, q_at + 8 * k, kd + k_step, kHi, idesc(kHalf, false),
-                             k != 0);
-            else
-              umma_f16_if(issue, to, q_lo + q_step, kd + k_step, kHi, kHi, idesc(kHalf, false),
-                          k != 0);
+            for (int k = 0; k < D / 16; ++k) {
+              const uint32_t q_step = ((k / 4) * kQueryAtom + (k % 4) * 32) / 16;
+              const uint32_t k_step = ((k / 4) * LY::kAtom + (k % 4) * 32) / 16;
+              if constexpr (LY::kQTmem)
+                umma_f16_ts(to, q_at + 8 * k, desc(kd + k_step), idesc(kHalf, false), k != 0);
+              else
+                umma_f16(to, desc(q_lo + q_step), desc(kd + k_step), idesc(kHalf, false), k != 0);
+            }
+            umma_commit(&s_full[t][i & 1]);
+            if ((i + 1) % kHalves == 0) umma_commit(&k_empty[(i / kHalves) & 1]);
           }
-          umma_commit_if(issue, &s_full[t][i & 1]);
+          __syncwarp();
         };
         auto results = [&](int i) {
           const uint32_t vd = v_lo + ((i / kHalves) & 1) * kTile16 + (i % kHalves) * kHalf16;
           const uint32_t from = s_at + (i & 1) * kHalf;
+          if (elect_one()) {
 #pragma unroll
-          for (int k = 0; k < kHalf / 16; ++k)
-            umma_f16_ts_if(issue, o_at, from + 8 * k, vd + k * (16 * 128 / 16), kHi,
-                           idesc(D, true), i != 0 || k != 0);
-          umma_commit_if(issue, &o_full[t]);
+            for (int k = 0; k < kHalf / 16; ++k)
+              umma_f16_ts(o_at, from + 8 * k, desc(vd + k * (16 * 128 / 16)), idesc(D, true),
+                          i != 0 || k != 0);
+            umma_commit(&o_full[t]);
+            if ((i + 1) % kHalves == 0) umma_commit(&v_empty[(i / kHalves) & 1]);
+            if (i + 1 == steps) umma_commit(&o_done[t]);
+          }
+          __syncwarp();
         };
         // scores of half i: the first half of a key tile waits for it, the last gives it back
         auto next_scores = [&](int i) {
@@ -517,7 +524,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
             tc_fence_after();
           }
           scores(i);
-          if ((i + 1) % kHalves == 0) umma_commit_if(issue, &k_empty[j & 1]);
           return true;
         };
         bool ok = warp_wait(&q_full[t], 0, fail);
@@ -532,12 +538,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
           if (!ok) break;
           tc_fence_after();
           results(i);
-          if ((i + 1) % kHalves == 0) umma_commit_if(issue, &v_empty[j & 1]);
-          if (i + 1 == steps) umma_commit_if(issue, &o_done[t]);
           if (i + 2 < steps) ok = next_scores(i + 2);  // in this half's place
         }
         // whatever happened, nothing is in flight when tensor memory is given back
-        umma_commit_if(issue, &drained[t]);
+        if (elect_one()) umma_commit(&drained[t]);
+        __syncwarp();
         mbar_wait(&drained[t], 0, kProbes);
       }
     } else if (warp == kLoadWarp) {

@@ -51,38 +51,14 @@ __device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, ui
       : "memory");
 }
 
-// The same two, issued by the lane whose `issue` is set while the whole warp
-// runs the code: the operands stay in uniform registers, which the instruction
-// reads (in a branch of one lane each would be moved there one by one).
-// Descriptors come in halves: the upper words are constants of the layout, so a
-// step along a tile is one 32-bit addition.
-__device__ __forceinline__ void umma_f16_if(uint32_t issue, uint32_t d_tmem, uint32_t alo,
-                                            uint32_t blo, uint32_t ahi, uint32_t bhi,
-                                            uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n .reg .pred p, q;\n .reg .b64 a, b;\n setp.ne.b32 p, %6, 0;\n setp.ne.b32 q, %7, 0;\n"
-      " mov.b64 a, {%1, %3};\n mov.b64 b, {%2, %4};\n"
-      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %5, p;\n}\n" ::"r"(d_tmem),
-      "r"(alo), "r"(blo), "r"(ahi), "r"(bhi), "r"(idesc), "r"(accumulate), "r"(issue)
-      : "memory");
-}
-__device__ __forceinline__ void umma_f16_ts_if(uint32_t issue, uint32_t d_tmem, uint32_t a_tmem,
-                                               uint32_t blo, uint32_t bhi, uint32_t idesc,
-                                               uint32_t accumulate) {
-  asm volatile(
-      "{\n .reg .pred p, q;\n .reg .b64 b;\n setp.ne.b32 p, %5, 0;\n setp.ne.b32 q, %6, 0;\n"
-      " mov.b64 b, {%2, %3};\n"
-      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n}\n" ::"r"(d_tmem),
-      "r"(a_tmem), "r"(blo), "r"(bhi), "r"(idesc), "r"(accumulate), "r"(issue)
-      : "memory");
-}
-__device__ __forceinline__ void umma_commit_if(uint32_t issue, uint64_t* bar) {
-  asm volatile(
-      "{\n .reg .pred q;\n setp.ne.b32 q, %1, 0;\n"
-      " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(
-          smem_u32(bar)),
-      "r"(issue)
-      : "memory");
+// True in one lane of a converged warp, the same one every time.  A branch on it is
+// known to be one lane's, so products in it cost a few clocks to issue; in a branch
+// on the lane's number, or each with a predicate of its own, they took 80.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n"
+               : "=r"(r));
+  return r != 0;
 }
 
 // Arrive on `bar` once every MMA issued so far by this thread has completed.
