@@ -57,7 +57,7 @@ struct PromptLayout {
   static constexpr int kHalves = kN / kHalf;
   static constexpr int kSoftWarps = 4 * kQueries;
   static constexpr int kConvWarps = kMmaWarp - kSoftWarps;
-  static constexpr int kRing = 8 / kHalves;             // key tiles whose scales are held
+  static constexpr int kRing = 16 / kHalves;            // key tiles whose scales are held
   // Queries in tensor memory, where the results leave room for them: the products
   // then read keys and values alone from shared memory.
   static constexpr bool kQTmem = kQueries * (2 * kHalf + D + D / 2) <= (int)kTmemCols;
@@ -65,7 +65,11 @@ struct PromptLayout {
   static constexpr int kAtom = kN * 128;                // kN rows x 64 halves
   static constexpr int kTile = (D / 64) * kAtom;        // a key or value tile
   static constexpr int kRaw = kN * D;                   // its codes
-  static constexpr int kUsed = 1024 + kQueries * kQuery + 4 * kTile + 2 * kRaw + 32 * 16;
+  // places for a side's codes: two where shared memory has room, so that a copy's
+  // latency hides behind a conversion
+  static constexpr int kRaws = kQTmem ? 2 : 1;
+  static constexpr int kUsed =
+      1024 + kQueries * kQuery + 4 * kTile + 2 * kRaws * kRaw + 16 * (kHalf / 16) * 16;
   // one block an SM: it owns all of tensor memory
   static constexpr int kSmem = kUsed > 120 * 1024 ? kUsed : 120 * 1024;
   static constexpr uint32_t kScore = 0;                 // tensor memory columns
@@ -116,16 +120,17 @@ struct Scale {
 template <typename T, int D>
 __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendParams p) {
   using LY = PromptLayout<D>;
-  constexpr int kN = LY::kN, kHalves = LY::kHalves, kRing = LY::kRing;
+  constexpr int kN = LY::kN, kHalves = LY::kHalves, kRing = LY::kRing, kRaws = LY::kRaws;
   extern __shared__ unsigned char raw[];
   unsigned char* const sm = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
   unsigned char* const sm_q = sm;                                     // [kQueries]
   unsigned char* const sm_k = sm + LY::kQueries * LY::kQuery;         // [2]
   unsigned char* const sm_v = sm_k + 2 * LY::kTile;                   // [2]
-  unsigned char* const sm_raw = sm_v + 2 * LY::kTile;                 // codes: keys, values
-  Scale* const sm_scale = reinterpret_cast<Scale*>(sm_raw + 2 * LY::kRaw);  // [kRing][kN / 16]
+  unsigned char* const sm_raw = sm_v + 2 * LY::kTile;                 // codes: [kRaws][2 sides]
+  Scale* const sm_scale =
+      reinterpret_cast<Scale*>(sm_raw + 2 * kRaws * LY::kRaw);        // [kRing][kN / 16]
   __shared__ __align__(8) uint64_t q_full[2], drained[2], k_full[2], k_empty[2], v_full[2], v_empty[2],
-      scale_full[kRing], raw_full[2], raw_empty[2], s_full[2][2], p_full[2][2], o_full[2], o_done[2], turn[2][4];
+      scale_full[kRing], raw_full[2][kRaws], raw_empty[2][kRaws], s_full[2][2], p_full[2][2], o_full[2], o_done[2], turn[2][4];
   __shared__ uint32_t sh_tmem;
   __shared__ int sh_fail;
 
@@ -167,8 +172,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
       mbar_init(&k_empty[i], two ? 2 : 1);
       mbar_init(&v_full[i], LY::kConvWarps);
       mbar_init(&v_empty[i], two ? 2 : 1);
-      mbar_init(&raw_full[i], 1);
-      mbar_init(&raw_empty[i], LY::kConvWarps);
+      for (int x = 0; x < kRaws; ++x) {
+        mbar_init(&raw_full[i][x], 1);
+        mbar_init(&raw_empty[i][x], LY::kConvWarps);
+      }
       for (int x = 0; x < 2; ++x) {
         mbar_init(&s_full[i][x], 1);
         mbar_init(&p_full[i][x], 4);
@@ -262,7 +269,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
         if (i % kHalves == 0 && !(ok = warp_wait(&scale_full[j % kRing], (j / kRing) & 1, fail)))
           break;
         // factors and offsets of the exponents of 4 x 16 tokens
-        const Scale* sc = sm_scale + i % 8 * 4;  // the ring holds eight halves
+        const Scale* sc = sm_scale + i % 16 * 4;  // the ring holds sixteen halves
         float fk[4], fo[4];
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
@@ -429,10 +436,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
     bool ok = true;
 #pragma unroll 1
     for (int x = 0; x < 2 * tiles; ++x) {  // keys, values, keys, ...
-      const int j = x >> 1, side = x & 1, st = j & 1;
-      const unsigned char* src = sm_raw + side * LY::kRaw + row0 * D + c * 16;
+      const int j = x >> 1, side = x & 1, st = j & 1, place = j % kRaws;
+      const unsigned char* src = sm_raw + (place * 2 + side) * LY::kRaw + row0 * D + c * 16;
       unsigned char* at = (side ? sm_v : sm_k) + st * LY::kTile + (c / 4) * LY::kAtom;
-      if (!(ok = warp_wait(&raw_full[side], j & 1, fail))) break;
+      if (!(ok = warp_wait(&raw_full[side][place], (j / kRaws) & 1, fail))) break;
       if (j >= 2 &&
           !(ok = warp_wait(side ? &v_empty[st] : &k_empty[st], ((j >> 1) - 1) & 1, fail)))
         break;
@@ -459,7 +466,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
       fence_proxy_async_smem();  // the tile for the tensor cores, the codes' place for the next copy
       __syncwarp();
       if (lane == 0) {
-        mbar_arrive(&raw_empty[side]);
+        mbar_arrive(&raw_empty[side][place]);
         mbar_arrive(side ? &v_full[st] : &k_full[st]);
       }
     }
@@ -573,13 +580,15 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
         page = page_of(j + 1);
 #pragma unroll
         for (int side = 0; side < 2; ++side) {
-          if (j >= 1 && !(ok = warp_wait(&raw_empty[side], (j - 1) & 1, fail))) break;
+          const int place = j % kRaws;
+          if (j >= kRaws && !(ok = warp_wait(&raw_empty[side][place], (j / kRaws - 1) & 1, fail)))
+            break;
           issued[side] = j + 1;
-          if (lane == 0) mbar_arrive_expect_tx(&raw_full[side], bytes);
+          if (lane == 0) mbar_arrive_expect_tx(&raw_full[side][place], bytes);
           __syncwarp();
           if (leads)
-            bulk_g2s(sm_raw + side * LY::kRaw + lane * 16 * D, (side ? p.v : p.k) + off, piece,
-                     &raw_full[side]);
+            bulk_g2s(sm_raw + (place * 2 + side) * LY::kRaw + lane * 16 * D,
+                     (side ? p.v : p.k) + off, piece, &raw_full[side][place]);
           if (side == 0) {
             if (lane < 8) {
               Scale x{s_key, 0.0f, 0.0f, 0.0f};
@@ -594,7 +603,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
       // no copy is in flight when the block ends, whatever happened
 #pragma unroll
       for (int side = 0; side < 2; ++side)
-        if (issued[side]) mbar_wait(&raw_full[side], (issued[side] - 1) & 1, kProbes);
+        for (int j = max(issued[side] - kRaws, 0); j < issued[side]; ++j)
+          mbar_wait(&raw_full[side][j % kRaws], (j / kRaws) & 1, kProbes);
     }
   }
 
