@@ -268,6 +268,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
         const int j = i / kHalves, buf = i & 1;
         if (i % kHalves == 0 && !(ok = warp_wait(&scale_full[j % kRing], (j / kRing) & 1, fail)))
           break;
+        if (!(ok = warp_wait(&s_full[t][buf], (i >> 1) & 1, fail))) break;
+        tc_fence_after();
+        // the row's 64 scores, in registers from here on
+        uint32_t v[2][32];
+        tmem_ld32_nowait(s_col + buf * kHalf, v[0]);
+        tmem_ld32_nowait(s_col + buf * kHalf + 32, v[1]);
         // factors and offsets of the exponents of 4 x 16 tokens
         const Scale* sc = sm_scale + i % 16 * 4;  // the ring holds sixteen halves
         float fk[4], fo[4];
@@ -276,12 +282,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
           fk[g] = kq * sc[g].key;
           fo[g] = sc[g].log2_value;
         }
-        if (!(ok = warp_wait(&s_full[t][buf], (i >> 1) & 1, fail))) break;
-        tc_fence_after();
-        // the row's 64 scores, in registers from here on
-        uint32_t v[2][32];
-        tmem_ld32_nowait(s_col + buf * kHalf, v[0]);
-        tmem_ld32_nowait(s_col + buf * kHalf + 32, v[1]);
         tmem_wait_ld32(v[0]);
         tmem_wait_ld32(v[1]);
         // Hidden tokens: scores of -inf, with factors kept above 0.  16 tokens that
