@@ -440,15 +440,20 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
       const unsigned char* src = sm_raw + (place * 2 + side) * LY::kRaw + row0 * D + c * 16;
       unsigned char* at = (side ? sm_v : sm_k) + st * LY::kTile + (c / 4) * LY::kAtom;
       if (!(ok = warp_wait(&raw_full[side][place], (j / kRaws) & 1, fail))) break;
+      uint4 r[4];
+      auto load = [&] {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          r[i] = *reinterpret_cast<const uint4*>(src + i * kRows * D);
+        src += 4 * kRows * D;
+      };
+      load();
       if (j >= 2 &&
           !(ok = warp_wait(side ? &v_empty[st] : &k_empty[st], ((j >> 1) - 1) & 1, fail)))
         break;
 #pragma unroll 1
       for (int i0 = 0; i0 < kN / LY::kConvWarps / kRows; i0 += 4) {
-        uint4 r[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          r[i] = *reinterpret_cast<const uint4*>(src + i * kRows * D);
+        if (i0 > 0) load();
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const uint32_t x[4] = {r[i].x ^ 0x80808080u, r[i].y ^ 0x80808080u,
@@ -460,7 +465,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
           *reinterpret_cast<uint4*>(at + i * kRows * 128 + put[i % kPlaces][0]) = lo;
           *reinterpret_cast<uint4*>(at + i * kRows * 128 + put[i % kPlaces][1]) = hi;
         }
-        src += 4 * kRows * D;
         at += 4 * kRows * 128;
       }
       fence_proxy_async_smem();  // the tile for the tensor cores, the codes' place for the next copy
