@@ -5,6 +5,8 @@ for the device mount of routed grafts (core/graft_arena.py swap/unpack_node):
 
 * ``cuda_router``  -- CudaMLARouteSidecar/Bank, CudaGQARouteSidecar/Bank
 * ``graft_mount``  -- fused dequantise + scatter into the bf16 arena
+* ``paged_arena``  -- keys and values of many requests at 8 bits in pages: step plans,
+  append, attention, read-back
 * ``sharded``      -- node-range sharded route over 1-8 GPUs (NCCL all-gather)
 * ``synth``        -- seeded synthetic banks with the benchmark configs' shapes
 

@@ -10,7 +10,8 @@
 // p_t u-weighted is what multiplies b_t, and the sum of weights is
 // sum_t p_t / u_t, so p_t never exceeds 2^8 whatever the scales are and fp16
 // holds it (m trails the largest y seen by at most 8: it moves only when a y
-// passes m + 8, so the accumulators are rarely rescaled).   The log-sum-exp is m ln 2 + log of that sum.
+// passes m + 8, so the accumulators are rarely rescaled).  The log-sum-exp is
+// m ln 2 + log of that sum.
 //
 // The split kernel serves few query rows a kv head (decoding, a few proposed
 // tokens): it is bound by the bytes of the codes, 2 * head_dim a token and kv
@@ -30,6 +31,16 @@
 // less 1152.  Queries are fp16: a bf16 row is first scaled by the power of two
 // that brings its largest value into [2^14, 2^15), so only values 2^29 times
 // smaller than the largest round.
+//
+// 64 requests of 200 to 16,384 tokens, one row x 4 each on 8 kv heads of head_dim
+// 128 (515 MB of codes), take 97 us, 5.3 TB/s; one request of 250,007 tokens 98
+// us.  In its stride the kernel reads 7.5 TB/s (1.94 us a tile and block); the
+// rest is the start (first data after 4.3 us of dependent loads) and the spread
+// of the blocks, which end between 61 and 90 us for equal shares.  Measured and
+// dropped: a last sixth of the tiles handed out in small shares as blocks finish
+// (98 -> 105 us: starts and joins cost more than the spread); score products in
+// int8, the codes as stored and the query in three digits (17 % fewer
+// instructions, the same time).
 #include <cuda.h>
 
 #include <algorithm>

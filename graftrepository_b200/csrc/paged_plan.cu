@@ -17,7 +17,8 @@
 // from the ring, not from the table entry another block writes, so no block
 // waits for another.  The kinds run side by side because each is a chain of
 // dependent reads, and a step's plan is bound by those: one block for all of
-// them, chunk after chunk, took 31 us for 4,096 requests and 262,694 rows.
+// them, chunk after chunk, took 31 us for 4,096 requests and 262,694 rows, where
+// this takes 13; 64 requests of one row take 6.5 us, about three such chains.
 #include <algorithm>
 
 #include "paged.cuh"
@@ -31,7 +32,9 @@ constexpr int kPlanThreads = 1024;
 constexpr int kPlanWarps = kPlanThreads / 32;
 constexpr int kJoinUnits = 5;
 constexpr int kBuckets = 256;  // of prompt tiles by what they see
-constexpr int kPartTokens = 256;  // a part of a prompt tile has no fewer
+// A part of a prompt tile has no fewer tokens.  One request of 4,096 tokens, 32
+// pairs, head_dim 256: 24 us in parts of 256, 28 of 512, 42 whole.
+constexpr int kPartTokens = 256;
 // The sums over requests: pages taken, rows, pages touched, prompt tiles or their
 // parts (all of them below 2^31 in a step that can be planned) and the split
 // kernel's units; and two that only totals are needed of, the split kernel's
@@ -458,6 +461,12 @@ int make_shape(const grm_b200_paged_plan& p, int sms, Shape* s) {
   s->group = p.query_heads / p.kv_heads;
   const int64_t most = std::min(p.max_fresh, p.tokens) * s->group;
   s->block_rows = most <= 8 ? 8 : 16;
+  // (row, head) pairs a kv head up to which the split kernel serves a request, in
+  // segments of 16 rows that read the codes again; a prompt tile costs the same for
+  // 1 row and 128.  Split / prompt, us, 16 requests of 4,096 tokens on 8 kv heads:
+  // head_dim 64, 32 pairs 50 / 60, 64 pairs 81 / 61; head_dim 128, 32 pairs 72 / 69 (64
+  // requests of 2,048 tokens: 132 / 141), 64 pairs 121 / 69; head_dim 256, 16 pairs
+  // 81 / 87, 24 pairs 126 / 87.
   s->prompt_rows = p.head_dim == 256 ? 16 : 32;
   const bool prompts = most > s->prompt_rows;
   s->qtile_tokens = (p.head_dim == 256 ? 1 : 2) * (128 / s->group);

@@ -11,24 +11,39 @@
 //
 // A block takes 2 x 128 query rows of one kv head (rows of the group's heads
 // side by side, so a key tile serves all of them) and walks the visible tokens
-// 128 at a time:
+// 128 at a time, 64 in a step of the softmax:
 //   warps 0-3, 4-7  softmax of query tile 0 / 1, one row a thread: scores from
 //                   tensor memory, p back as fp16 over them, and when a row's
 //                   reference exponent has to move (rarely: it trails by up
 //                   to 8), its result in tensor memory rescaled
 //   warps 8-11      codes in shared memory to fp16 key and value tiles (two of
 //                   each)
-//   warps 12, 13    one lane each that issues a query tile's products, S = Q K^T
-//                   (both from shared memory) and O += P V (P from tensor
-//                   memory).  A thread that waits on a barrier first sees its
-//                   own commits out of the queue of products, so with one
-//                   thread for both tiles the tensor cores ran dry at every
-//                   wait, about 250 clocks each
+//   warps 12, 13    a query tile's products, S = Q K^T and O += P V (P from
+//                   tensor memory), issued by one elected lane.  A thread that
+//                   waits on a barrier first sees its own commits out of the
+//                   queue of products, so with one thread for both tiles the
+//                   tensor cores ran dry at every wait, about 250 clocks each
 //   warp 14         codes from their pages to shared memory, one bulk copy a page
-// While one query tile's softmax runs, the tensor cores work for the other.
+// While one query tile's softmax runs, the tensor cores work for the other, and
+// the two softmax warps of a scheduler take turns at the exponentials.  At
+// head_dim 256 a result tile takes half of tensor memory: one query tile, key
+// tiles of 64 tokens, and warps 4-11 convert.  At head_dim 64 and 256 there is
+// room for the queries in tensor memory, too, so that the products read keys and
+// values alone from shared memory, and for two places of codes.
 // Keys and values have the same layout in shared memory, 128-byte rows of 64
 // dims with a 128-byte swizzle: K is read K-major, V with its dims contiguous.
 // A block whose rows fit one tile leaves the other tile's work out.
+//
+// Few tiles over long contexts are cut along their tokens into parts, a block
+// each; the split kernel, which runs after this one, joins them.
+//
+// 8,449 rows of 3 requests (1.4 TFLOP at 8 kv heads, 32 query heads, head_dim 128)
+// take 1.33 ms, 1.07 PFLOP/s.  What bounds it now is the softmax warps' chain of
+// dependent steps: per 64 tokens 2,000 clocks, where the exponentials alone need
+// 1,024 (both warps of a scheduler), the tensor cores as many, and shared memory
+// 1,536; tensor cores are active 45 %, the exponential unit 46 % and issue slots
+// 54 % of the time.  Measured on the way: both warps of a scheduler in the same
+// phase 1.51 ms; products with a predicate each, 80 clocks of issue apiece, 1.43.
 #include <type_traits>
 
 #include "paged.cuh"
@@ -477,8 +492,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
   } else {
     if (warp < kLoadWarp) {
       // ---------------------------------------------------------- products
-      // The whole warp runs this, one lane issues; what the instructions read is
-      // the same in every lane and known to be (broadcast), so that it stays in
+      // The whole warp runs this, an elected lane issues; what the instructions read
+      // is the same in every lane and known to be (broadcast), so that it stays in
       // uniform registers.
       const int t = __shfl_sync(kFull, warp, 0) - kMmaWarp;
       const int steps = __shfl_sync(kFull, halves_seen, 0);
