@@ -110,6 +110,23 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 __device__ __forceinline__ float max3(uint32_t a, uint32_t b, uint32_t c) {
   return max3(__uint_as_float(a), __uint_as_float(b), __uint_as_float(c));
 }
+// Two numbers at a time.
+__device__ __forceinline__ float2 fma2(float a, float b, float k, float o) {
+  float2 r;
+  asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %4};\n"
+      " mov.b64 z, {%5, %5};\n fma.rn.f32x2 x, x, y, z;\n mov.b64 {%0, %1}, x;\n}\n"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a), "f"(b), "f"(k), "f"(o));
+  return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n .reg .b64 x, y;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n"
+      " add.rn.f32x2 x, x, y;\n mov.b64 {%0, %1}, x;\n}\n"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
 // Every lane of a warp waits; false, for all of them, when a wait gave up.
 // The loops of this kernel share an instruction cache that they barely fit, so
 // what is not the common path stays out of line.
@@ -355,19 +372,20 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
           for (int h2 = 0; h2 < 2; ++h2) {
             const int g = 2 * c + h2;
             const float k = fk[g], off = fo[g] - ref;
-            float sum0 = 0.0f, sum1 = 0.0f;
+            float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll
             for (int x = 0; x < 16; x += 2) {
-              const float p0 = ex2(fmaf(__uint_as_float(v[c][16 * h2 + x]), k, off));
-              const float p1 = ex2(fmaf(__uint_as_float(v[c][16 * h2 + x + 1]), k, off));
-              sum0 += p0;
-              sum1 += p1;
-              w[8 * h2 + x / 2] = pack_half2(p0, p1);
+              const float2 y = fma2(__uint_as_float(v[c][16 * h2 + x]),
+                                    __uint_as_float(v[c][16 * h2 + x + 1]), k, off);
+              const float2 e = make_float2(ex2(y.x), ex2(y.y));
+              sum = add2(sum, e);
+              w[8 * h2 + x / 2] = pack_half2(e.x, e.y);
             }
-            l = fmaf(sum0 + sum1, sc[g].inv_value, l);
+            l = fmaf(sum.x + sum.y, sc[g].inv_value, l);
+            // three quarters done: the other's first ones fill the gaps of the last
+            if (g == 2 && two && lane == 0) mbar_arrive(&turn[1 - t][warp & 3]);
           }
           tmem_st16(s_col + buf * kHalf + 16 * c, w);
-          if (c == 0 && two && lane == 0) mbar_arrive(&turn[1 - t][warp & 3]);
         }
         tmem_wait_st();
         tc_fence_before();
