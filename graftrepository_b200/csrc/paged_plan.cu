@@ -35,6 +35,7 @@ constexpr int kBuckets = 256;  // of prompt tiles by what they see
 // A part of a prompt tile has no fewer tokens.  One request of 4,096 tokens, 32
 // pairs, head_dim 256: 24 us in parts of 256, 28 of 512, 42 whole.
 constexpr int kPartTokens = 256;
+constexpr int kSizes = 4;
 // The sums over requests: pages taken, rows, pages touched, prompt tiles or their
 // parts (all of them below 2^31 in a step that can be planned) and the split
 // kernel's units; and two that only totals are needed of, the split kernel's
@@ -128,6 +129,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
   __shared__ int64_t part[2 * kSums][kPlanWarps];
   __shared__ int64_t total[2 * kSums];  // of all requests; of those before the chunk
   __shared__ int chunk_part[kScans][kPlanWarps];
+  __shared__ int cut[2];  // parts of all tiles, and of those before the chunk
   __shared__ int bucket[kBuckets], most_seen;
   __shared__ int bad;
 
@@ -204,35 +206,45 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
   int failed = bad;
 
   // A prompt tile and head is one block; where they are fewer than half of the SMs,
-  // tiles are cut along their tokens into parts, as many as there are SMs beyond the
-  // tiles: Sum ceil(len / part) <= Sum len / part + tiles, so all parts run at once.
+  // tiles are cut along their tokens into parts that all run at once.  The fewest
+  // tokens that a part can have are between Sum len / SMs and Sum len / (SMs - tiles),
+  // which is always enough (Sum ceil(len / part) <= Sum len / part + tiles): of four
+  // sizes in between, the smallest whose parts the SMs can hold (16 requests of 100 to
+  // 8,192 tokens with 5 rows of head_dim 256: 44 us with the last one always).
   int part_tokens = 0;
   const int64_t whole = total[kTiles] * p.kv_heads;
   if (whole > 0 && whole <= p.sms / 2) {
-    const int64_t each = ceil_div64(total[kTokens] * p.kv_heads, p.sms - whole);
-    part_tokens = (int)(each < kPartTokens ? kPartTokens : each < (1 << 30) ? each : 1 << 30);
-    int64_t sum_parts = 0, sum_before = 0;
-    for (int c = 0; c < p.chunks; ++c) {
-      const Request x = c == chunk ? q : request((int64_t)c * kPlanThreads + tid, &flags);
-      int64_t a[kSums];
-      weigh(p, x, a);
-      a[kTiles] *= parts_of(x.after, part_tokens);
-      if (c == chunk) {
-        sum_before = sum_parts;
-        own[kTiles] = a[kTiles];
+#pragma unroll 1
+    for (int k = 1; k <= kSizes; ++k) {
+      const int64_t each = ceil_div64(total[kTokens] * p.kv_heads, p.sms - whole * k / kSizes);
+      part_tokens = (int)(each < kPartTokens ? kPartTokens : each < (1 << 30) ? each : 1 << 30);
+      int all = 0, all_before = 0;
+#pragma unroll 1
+      for (int c = 0; c < p.chunks; ++c) {
+        const Request x = c == chunk ? q : request((int64_t)c * kPlanThreads + tid, &flags);
+        int64_t a[kSums];
+        weigh(p, x, a);
+        if (c == chunk) all_before = all;
+        all += (int)a[kTiles] * parts_of(x.after, part_tokens);
       }
-      sum_parts += a[kTiles];
+      all = __reduce_add_sync(kFull, all);
+      all_before = __reduce_add_sync(kFull, all_before);
+      if (lane == 0) {
+        part[0][warp] = all;
+        part[1][warp] = all_before;
+      }
+      __syncthreads();
+      if (warp < 2) {
+        const int64_t w = warp_sum(part[warp][lane]);
+        if (lane == 0) cut[warp] = (int)w;
+      }
+      __syncthreads();
+      if ((int64_t)cut[0] * p.kv_heads <= p.sms) break;
     }
-    sum_parts = warp_sum(sum_parts);
-    sum_before = warp_sum(sum_before);
-    if (lane == 0) {
-      part[0][warp] = sum_parts;
-      part[1][warp] = sum_before;
-    }
-    __syncthreads();  // the tiles' totals have been read too
-    if (warp < 2) {
-      const int64_t w = warp_sum(part[warp][lane]);
-      if (lane == 0) total[warp == 0 ? kTiles : kSums + kTiles] = w;
+    own[kTiles] *= parts_of(q.after, part_tokens);
+    if (tid == 0) {
+      total[kTiles] = cut[0];
+      total[kSums + kTiles] = cut[1];
     }
     __syncthreads();
   }
