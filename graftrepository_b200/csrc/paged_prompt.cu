@@ -38,12 +38,12 @@
 // each; the split kernel, which runs after this one, joins them.
 //
 // 8,449 rows of 3 requests (1.4 TFLOP at 8 kv heads, 32 query heads, head_dim 128)
-// take 1.33 ms, 1.07 PFLOP/s.  What bounds it now is the softmax warps' chain of
-// dependent steps: per 64 tokens 2,000 clocks, where the exponentials alone need
-// 1,024 (both warps of a scheduler), the tensor cores as many, and shared memory
-// 1,536; tensor cores are active 45 %, the exponential unit 46 % and issue slots
-// 54 % of the time.  Measured on the way: both warps of a scheduler in the same
-// phase 1.51 ms; products with a predicate each, 80 clocks of issue apiece, 1.43.
+// take 1.27 ms, 1.12 PFLOP/s.  What bounds it now is the softmax warps' chain of
+// dependent steps: per 64 tokens about 1,900 clocks, where the exponentials alone
+// need 1,024 (both warps of a scheduler), the tensor cores as many, and shared
+// memory 1,536.  On the way: both warps of a scheduler in the same phase 1.51 ms,
+// in turns 1.43; then, where each product had had a predicate of its own (80
+// clocks of issue apiece), an elected branch 1.33; arithmetic two at a time 1.27.
 #include <type_traits>
 
 #include "paged.cuh"

@@ -171,19 +171,18 @@ class PagePlan:
             self.query_shape) for kind in _TYPES}
         self._lse_like = torch.empty(1, device=self.device).expand(self.query_shape[:2])
 
-        def ints(n, dtype=torch.int32):
-            return torch.zeros(n, dtype=dtype, device=self.device)
-
-        self.lens, self.starts = ints(tables.requests), ints(tables.requests + 1)
-        self.positions, self.rows = ints(self.tokens), ints(self.tokens)
-        self.slots, self.cursor = ints(self.tokens, torch.int64), ints(2, torch.int64)
-        self.status = ints(1)
+        # the step's outputs, in two allocations
+        n, t = tables.requests, self.tokens
+        self.lens, self.starts, self.positions, self.rows, self.status = torch.zeros(
+            2 * n + 2 * t + 2, dtype=torch.int32, device=self.device).split([n, n + 1, t, t, 1])
+        self.slots, self.cursor = torch.zeros(
+            t + 2, dtype=torch.int64, device=self.device).split([t, 2])
         self.c = _PlanC(tables.requests, self.tokens, self.max_fresh, tables.width, tables.pages,
                         tables.page_tokens, kv_heads, query_heads, head_dim, 1)
         need = ctypes.c_int64(0)
         _call(_lib.load().grm_b200_paged_scratch_bytes, self._index, ctypes.byref(self.c),
               ctypes.byref(need))
-        self.scratch = torch.zeros(need.value, dtype=torch.uint8, device=self.device)
+        self.scratch = torch.empty(need.value, dtype=torch.uint8, device=self.device)
         c = self.c
         c.cached, c.cursor_in = tables.lens.data_ptr(), tables.cursor.data_ptr()
         c.ring, c.table = tables.ring.data_ptr(), tables.table.data_ptr()

@@ -692,3 +692,17 @@ def test_refusals():
         arena.append(plan, kv, kv)
     with pytest.raises(ValueError):
         PA.PageTables(2, 8, 4, page_tokens=16, device=DEV).plan(plan, i32([0, 0]))
+
+
+@pytest.mark.parametrize("lens,fresh", [([400, 33, 5000], [1, 1, 1]), ([700, 5000], [300, 40])])
+def test_scratch_may_hold_anything(lens, fresh):
+    """A plan's scratch need not be cleared: what a step reads there, its plan wrote."""
+    tables, arena, plan = make_arena(lens, fresh, heads=2, group=4, dim=128, page=64, seed=51)
+    gen = torch.Generator(device=DEV).manual_seed(52)
+    q = torch.randn((plan.tokens, 8, 128), device=DEV, generator=gen).to(torch.bfloat16)
+    want = arena.attend(plan, q)
+    for byte in (0, 255, 17):
+        plan.scratch.fill_(byte)
+        tables.plan(plan, i32(fresh))
+        got = arena.attend(plan, q)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
