@@ -706,3 +706,25 @@ def test_scratch_may_hold_anything(lens, fresh):
         tables.plan(plan, i32(fresh))
         got = arena.attend(plan, q)
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("lens,fresh", [([700, 5000, 90], [300, 40, 1]), ([3000] * 40, [70, 1] * 20)])
+def test_a_mixed_step_in_a_cuda_graph(lens, fresh):
+    """Prompts and single tokens of one step, two kernels after one another, replayed on
+    other queries and in a row."""
+    tables, arena, plan = make_arena(lens, fresh, heads=2, group=4, dim=128, page=64, seed=61)
+    gen = torch.Generator(device=DEV).manual_seed(62)
+    q = torch.randn((plan.tokens, 8, 128), device=DEV, generator=gen).to(torch.bfloat16)
+    want = arena.attend(plan, q)
+    check_attention(*want, reference(tables, arena, plan, q, True), float(arena.v_scales.max()))
+    held = torch.zeros_like(q)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        first = arena.attend(plan, held)
+        second = arena.attend(plan, first[0])
+    held.copy_(q)
+    for _ in range(3):
+        graph.replay()
+    assert torch.equal(first[0], want[0]) and torch.equal(first[1], want[1])
+    again = arena.attend(plan, want[0])
+    assert torch.equal(second[0], again[0]) and torch.equal(second[1], again[1])
