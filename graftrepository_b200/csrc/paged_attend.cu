@@ -218,7 +218,8 @@ __device__ __noinline__ void join_row(const AttendParams& p, int wa, int n, int 
       for (int i = 0; i < kAhead; ++i) {
         const float* src = part(min(i0 + i1 + i, n - 1)) + row * D + kDims * lane;
 #pragma unroll
-        for (int d = 0; d < kDims / 2; ++d) v[i][d] = __ldcg(reinterpret_cast<const float2*>(src) + d);
+        for (int d = 0; d < kDims / 2; ++d)
+          v[i][d] = __ldcg(reinterpret_cast<const float2*>(src) + d);
       }
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
@@ -256,7 +257,8 @@ __device__ __noinline__ void join_prompts(const AttendParams& p, int entries) {
   for (int e0 = 0; e0 < entries; e0 += 32) {
     const int4 mine = p.l.qtiles[min(e0 + lane, entries - 1)];
     const int my_parts = prompt_tile<D>(p, mine).parts;
-    unsigned todo = __ballot_sync(kFull, e0 + lane < entries && (mine.z & 255) == 0 && my_parts > 1);
+    unsigned todo =
+        __ballot_sync(kFull, e0 + lane < entries && (mine.z & 255) == 0 && my_parts > 1);
     for (; todo; todo &= todo - 1) {
       const int4 e = p.l.qtiles[e0 + __ffs(todo) - 1];
       const PromptTile t = prompt_tile<D>(p, e);
@@ -301,7 +303,8 @@ __device__ __noinline__ void join_prompts(const AttendParams& p, int entries) {
                             h * p.group + in % p.group;
         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
         reinterpret_cast<uint2*>(p.out + row * D)[c] =
-            make_uint2(pack_out<T>(acc.x * inv, acc.y * inv), pack_out<T>(acc.z * inv, acc.w * inv));
+            make_uint2(pack_out<T>(acc.x * inv, acc.y * inv),
+                       pack_out<T>(acc.z * inv, acc.w * inv));
         if (p.lse && c == 0)
           p.lse[row] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.693147180559945309f;
       }

@@ -100,7 +100,9 @@ __host__ __device__ constexpr uint32_t idesc(int n, bool b_mn) {
 }
 
 // Byte of 16-byte chunk c (8 halves of 64) of row r in a swizzled atom.
-__device__ __forceinline__ uint32_t atom_byte(int r, int c) { return r * 128 + ((c ^ (r & 7)) << 4); }
+__device__ __forceinline__ uint32_t atom_byte(int r, int c) {
+  return r * 128 + ((c ^ (r & 7)) << 4);
+}
 
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
@@ -161,8 +163,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
   unsigned char* const sm_raw = sm_v + 2 * LY::kTile;                 // codes: [kRaws][2 sides]
   Scale* const sm_scale =
       reinterpret_cast<Scale*>(sm_raw + 2 * kRaws * LY::kRaw);        // [kRing][kN / 16]
-  __shared__ __align__(8) uint64_t q_full[2], drained[2], k_full[2], k_empty[2], v_full[2], v_empty[2],
-      scale_full[kRing], raw_full[2][kRaws], raw_empty[2][kRaws], s_full[2][2], p_full[2][2], o_full[2], o_done[2], turn[2][4];
+  __shared__ __align__(8) uint64_t q_full[2], drained[2], k_full[2], k_empty[2], v_full[2],
+      v_empty[2], scale_full[kRing], raw_full[2][kRaws], raw_empty[2][kRaws], s_full[2][2],
+      p_full[2][2], o_full[2], o_done[2], turn[2][4];
   __shared__ uint32_t sh_tmem;
   __shared__ int sh_fail;
 
@@ -187,7 +190,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
   const int halves_seen = (min(sees - tok_base, tiles * kN) + kHalf - 1) / kHalf;
 
   if (all_tiles == 0) {  // nothing cached: empty rows
-    for (int x = threadIdx.x; x < (pt.toks[0] + pt.toks[1]) * p.group * (D / 2); x += kPromptThreads) {
+    const int values = (pt.toks[0] + pt.toks[1]) * p.group * (D / 2);
+    for (int x = threadIdx.x; x < values; x += kPromptThreads) {
       const int j = x / (D / 2);
       const int64_t row = (int64_t)(start + tok0 + j / p.group) * heads + h * p.group + j % p.group;
       reinterpret_cast<uint32_t*>(p.out + row * D)[x % (D / 2)] = 0;
@@ -500,7 +504,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
         }
         at += 4 * kRows * 128;
       }
-      fence_proxy_async_smem();  // the tile for the tensor cores, the codes' place for the next copy
+      // the tile for the tensor cores, the codes' place for the next copy
+      fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) {
         mbar_arrive(&raw_empty[side][place]);
@@ -606,7 +611,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
         const int t0 = tok_base + j * kN + (lane & 7) * 16;
         // a lane at the start of a page's share of the tile copies it; a page is
         // copied whole, past the request's last token too
-        const bool leads = lane < kN / 16 && t0 <= len - 1 && ((lane * 16) & (page_tokens - 1)) == 0;
+        const bool leads =
+            lane < kN / 16 && t0 <= len - 1 && ((lane * 16) & (page_tokens - 1)) == 0;
         const unsigned bytes = __popc(__ballot_sync(kFull, leads)) * piece;
         const int64_t off = ((at << p.page_shift) + (t0 & (page_tokens - 1))) * D;
         float s_key = 0.0f, s_value = 0.0f;

@@ -270,8 +270,8 @@ class PageTables:
             raise ValueError(f"rows must be int32 [n] on {self.device}")
         if rows.numel() == 0:
             return
-        _call(_lib.load().grm_b200_paged_release, self._index, rows.data_ptr(), rows.numel(), self.requests,
-              self.width, self.pages, self.page_tokens, self.table.data_ptr(),
+        _call(_lib.load().grm_b200_paged_release, self._index, rows.data_ptr(), rows.numel(),
+              self.requests, self.width, self.pages, self.page_tokens, self.table.data_ptr(),
               self.lens.data_ptr(), self.ring.data_ptr(), self.cursor.data_ptr(),
               _handle(stream, self._index, rows))
 
