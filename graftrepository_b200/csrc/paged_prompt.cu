@@ -83,8 +83,10 @@ struct PromptLayout {
   // places for a side's codes: two where shared memory has room, so that a copy's
   // latency hides behind a conversion
   static constexpr int kRaws = kQTmem ? 2 : 1;
+  static constexpr int kGroups = kN / 16;               // pages' scales of a key tile
+  static constexpr int kScaleBytes = kRing * kGroups * 16;
   static constexpr int kUsed =
-      1024 + kQueries * kQuery + 4 * kTile + 2 * kRaws * kRaw + 16 * (kHalf / 16) * 16;
+      1024 + kQueries * kQuery + 4 * kTile + 2 * kRaws * kRaw + kScaleBytes;
   // one block an SM: it owns all of tensor memory
   static constexpr int kSmem = kUsed > 120 * 1024 ? kUsed : 120 * 1024;
   static constexpr uint32_t kScore = 0;                 // tensor memory columns
@@ -150,6 +152,7 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, unsigned parity, volati
 struct Scale {
   float key, log2_value, inv_value, unused;
 };
+static_assert(sizeof(Scale) == 16, "PromptLayout::kScaleBytes");
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendParams p) {
@@ -162,7 +165,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
   unsigned char* const sm_v = sm_k + 2 * LY::kTile;                   // [2]
   unsigned char* const sm_raw = sm_v + 2 * LY::kTile;                 // codes: [kRaws][2 sides]
   Scale* const sm_scale =
-      reinterpret_cast<Scale*>(sm_raw + 2 * kRaws * LY::kRaw);        // [kRing][kN / 16]
+      reinterpret_cast<Scale*>(sm_raw + 2 * kRaws * LY::kRaw);        // [kRing][kGroups]
   __shared__ __align__(8) uint64_t q_full[2], drained[2], k_full[2], k_empty[2], v_full[2],
       v_empty[2], scale_full[kRing], raw_full[2][kRaws], raw_empty[2][kRaws], s_full[2][2],
       p_full[2][2], o_full[2], o_done[2], turn[2][4];
@@ -599,8 +602,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
       const int last = (len - 1) >> p.page_shift;
       const int page_tokens = 1 << p.page_shift;
       const unsigned piece = (unsigned)(min(page_tokens, kN) * D);  // codes of a page in a tile
-      auto page_of = [&](int j) {  // lane g < 8: page of the tile's tokens 16 g ..
-        const int i = min((tok_base + j * kN + (lane & 7) * 16) >> p.page_shift, last);
+      constexpr int kGroups = LY::kGroups;  // 8 of a key tile, 4 at head_dim 256
+      const int group16 = lane & (kGroups - 1);
+      auto page_of = [&](int j) {  // lane g < kGroups: page of the tile's tokens 16 g ..
+        const int i = min((tok_base + j * kN + group16 * 16) >> p.page_shift, last);
         return min(max(__ldg(p.table + tile.x * p.width + i), 0), (int)p.pages - 1);
       };
       int page = page_of(0);
@@ -608,15 +613,15 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
       bool ok = true;
       for (int j = 0; j < tiles && ok; ++j) {
         const int64_t at = (int64_t)page * p.kv_heads + h;
-        const int t0 = tok_base + j * kN + (lane & 7) * 16;
+        const int t0 = tok_base + j * kN + group16 * 16;
         // a lane at the start of a page's share of the tile copies it; a page is
         // copied whole, past the request's last token too
         const bool leads =
-            lane < kN / 16 && t0 <= len - 1 && ((lane * 16) & (page_tokens - 1)) == 0;
+            lane < kGroups && t0 <= len - 1 && ((lane * 16) & (page_tokens - 1)) == 0;
         const unsigned bytes = __popc(__ballot_sync(kFull, leads)) * piece;
         const int64_t off = ((at << p.page_shift) + (t0 & (page_tokens - 1))) * D;
         float s_key = 0.0f, s_value = 0.0f;
-        if (lane < 8) {
+        if (lane < kGroups) {
           s_key = __ldg(p.ks + at);
           s_value = __ldg(p.vs + at);
         }
@@ -633,10 +638,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
             bulk_g2s(sm_raw + (place * 2 + side) * LY::kRaw + lane * 16 * D,
                      (side ? p.v : p.k) + off, piece, &raw_full[side][place]);
           if (side == 0) {
-            if (lane < 8) {
+            if (lane < kGroups) {
               Scale x{s_key, 0.0f, 0.0f, 0.0f};
               value_scale(s_value, &x.log2_value, &x.inv_value);
-              sm_scale[(j % kRing) * (kN / 16) + lane] = x;
+              sm_scale[(j % kRing) * kGroups + lane] = x;
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(&scale_full[j % kRing]);
