@@ -92,6 +92,13 @@ __host__ __device__ inline int worker_of(int u, const Header& h) {
 // ---- attention
 
 constexpr float kLazy = 8.0f;  // how far a row's scores may pass its reference exponent
+// Weights are held as fp16 times 2^7: at most 2^15, and what is lost at the small end
+// (fp16 ends at 2^-24) lies below 2^-32 of the row's largest.  Held as they are it
+// would be 2^-25, which the many small weights beside one that takes nearly all of
+// the sum reach (16,384 equal tokens e^-16 below one token: their part 6 % off).
+// Sums are of the weights themselves, results of the lifted ones.
+constexpr float kLift = 7.0f;
+constexpr float kUnlift = 0x1p-7f;
 
 struct AttendParams {
   Lists l;
@@ -177,7 +184,8 @@ __device__ __forceinline__ void row_scale(unsigned m, float* up, float* down) {
   *up = m ? __uint_as_float((unsigned)(127 + 14 + 127 - e) << 23) : 1.0f;
   *down = m ? __uint_as_float((unsigned)(e - 14) << 23) : 1.0f;
 }
-// Base-2 logarithm and inverse of a value scale.  A page of zeros (scale 0)
+// Base-2 logarithm of a value scale and what takes a lifted weight out of it,
+// 2^-7 / u.  A page of zeros (scale 0)
 // takes 2^-40, any scale being right for it: small enough to leave the other
 // pages' weights alone, large enough for its own to stay above 2^-126 when the
 // reference exponent is another page's.  Scales below 2^-100 count as 2^-100, so
@@ -185,7 +193,7 @@ __device__ __forceinline__ void row_scale(unsigned m, float* up, float* down) {
 __device__ __forceinline__ void value_scale(float u, float* log2_u, float* inv_u) {
   const float w = u == 0.0f ? 0x1p-40f : fmaxf(u, 0x1p-100f);
   *log2_u = u != u ? u : __log2f(w);
-  *inv_u = __fdividef(1.0f, w);
+  *inv_u = __fdividef(1.0f, w) * kUnlift;
 }
 // Two bf16 times `up` as halves.
 __device__ __forceinline__ uint32_t scale_pair(uint32_t v, float up) {

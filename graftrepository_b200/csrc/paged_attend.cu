@@ -8,9 +8,9 @@
 // unscaled result.  The value scale is folded into the exponent: with
 //   y_t = z_t * log2(e) + log2(u_t),  p_t = 2^(y_t - m),
 // p_t u-weighted is what multiplies b_t, and the sum of weights is
-// sum_t p_t / u_t, so p_t never exceeds 2^8 whatever the scales are and fp16
-// holds it (m trails the largest y seen by at most 8: it moves only when a y
-// passes m + 8, so the accumulators are rarely rescaled).  The log-sum-exp is
+// sum_t p_t / u_t, so p_t never exceeds 2^8 whatever the scales are (m trails the
+// largest y seen by at most 8: it moves only when a y passes m + 8, so the
+// accumulators are rarely rescaled), and fp16 holds 2^7 p_t.  The log-sum-exp is
 // m ln 2 + log of that sum.
 //
 // The split kernel serves few query rows a kv head (decoding, a few proposed
@@ -234,7 +234,7 @@ __device__ __noinline__ void join_row(const AttendParams& p, int wa, int n, int 
       }
     }
   }
-  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+  const float inv = sum == 0.0f ? 0.0f : kUnlift / sum;
 #pragma unroll
   for (int d = 0; d < kDims / 2; ++d)
     reinterpret_cast<uint32_t*>(p.out + out_row * D + kDims * lane)[d] =
@@ -301,7 +301,7 @@ __device__ __noinline__ void join_prompts(const AttendParams& p, int entries) {
         }
         const int64_t row = (int64_t)(t.start + t.tok0 + q * t.per + in / p.group) * heads +
                             h * p.group + in % p.group;
-        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        const float inv = sum == 0.0f ? 0.0f : kUnlift / sum;
         reinterpret_cast<uint2*>(p.out + row * D)[c] =
             make_uint2(pack_out<T>(acc.x * inv, acc.y * inv),
                        pack_out<T>(acc.z * inv, acc.w * inv));
@@ -686,7 +686,7 @@ __global__ void __launch_bounds__(kThreads, (Layout<D, NT>::kBlocks))
       for (int nt = 0; nt < NT; ++nt) {
         float ref[2];
 #pragma unroll
-        for (int x = 0; x < 2; ++x) ref[x] = m[nt][x] == -INFINITY ? 0.0f : m[nt][x];
+        for (int x = 0; x < 2; ++x) ref[x] = m[nt][x] == -INFINITY ? 0.0f : m[nt][x] - kLift;
 #pragma unroll
         for (int b = 0; b < kB; ++b) {
           float pr[4];
@@ -806,7 +806,7 @@ __global__ void __launch_bounds__(kThreads, (Layout<D, NT>::kBlocks))
             if (s.row0 + nt * 8 + 2 * t4 + x < s.pairs) {
               const int64_t row = out_row(nt * 8 + 2 * t4 + x);
               const float sum = lt[nt][x];
-              const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+              const float inv = sum == 0.0f ? 0.0f : kUnlift / sum;
 #pragma unroll
               for (int c = 0; c < kChunks; ++c)
                 *reinterpret_cast<uint32_t*>(p.out + row * D + 16 * c + 2 * g) =

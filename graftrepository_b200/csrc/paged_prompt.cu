@@ -3,7 +3,7 @@
 // The same sums as the split kernel's (paged_attend.cu): with key codes a_t and
 // value codes b_t, key scale s_t and value scale u_t,
 //   y_t = scale * log2(e) * s_t (q . a_t) + log2(u_t),  p_t = 2^(y_t - m),
-//   out = sum_t p_t b_t / sum_t (p_t / u_t),
+//   out = sum_t p_t b_t / sum_t (p_t / u_t), the fp16 operand being 2^7 p_t,
 // here bound by arithmetic: 4 head_dim operations a (row, visible token) on the
 // tensor cores and one exponential, 16 a clock and SM against 4,096 fp16
 // multiply-adds, so at head_dim 128 a 128 x 128 tile costs the two units about
@@ -371,7 +371,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
         if (two && t + i > 0 &&
             !(ok = warp_wait(&turn[t][warp & 3], (i - 1 + t) & 1, fail)))
           break;
-        const float ref = m == -INFINITY ? 0.0f : m;
+        const float ref = m == -INFINITY ? 0.0f : m - kLift;
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           uint32_t w[16];
@@ -429,7 +429,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
             *reinterpret_cast<float2*>(slot + prompt_rows_of(D) * D + 2 * (t * kM + row)) =
                 make_float2(m, l);
         } else {
-          const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+          const float inv = l == 0.0f ? 0.0f : kUnlift / l;
 #pragma unroll 1
           for (int c = 0; c < D / 16; ++c) {
             uint32_t v[16];

@@ -5,11 +5,14 @@ overtaken, waits that give up.
 The 64-bit reference, the makers of arenas and the tolerances of attention are
 those of test_paged_gpu.py, where they are derived."""
 
+import math
+
 import pytest
 
 torch = pytest.importorskip("torch")
 
-from test_paged_gpu import run_attention  # noqa: E402
+from graftrepository_b200 import paged_arena as PA  # noqa: E402
+from test_paged_gpu import DEV, ceil, i32, run_attention  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -22,3 +25,77 @@ def test_wide_heads_past_the_end_of_the_ring_of_scales(tokens, page):
     """At head_dim 256 a block holds the scales of 16 key tiles of 64 tokens: the
     last place, the first one again, and twice around."""
     run_attention([tokens] * 19, [40] * 19, heads=4, group=4, dim=256, page=page, seed=tokens)
+
+
+# ------------------------------------------------- weights far below the largest
+
+def two_kinds(requests, tokens, rows, far, gap, kind, *, heads, group, dim, page):
+    """Requests whose tokens in `far` score `gap` above the others and have value 0,
+    the others 1: (kernel's result, its lse, the formula's result, its lse)."""
+    tables = PA.PageTables(requests, requests * ceil(tokens, page), ceil(tokens, page),
+                           page_tokens=page, device=DEV)
+    plan = tables.make_plan(requests * rows, kv_heads=heads, query_heads=heads * group,
+                            head_dim=dim, max_fresh=rows)
+    if tokens > rows:
+        fill = tables.make_plan(requests * (tokens - rows), kv_heads=heads, query_heads=heads,
+                                head_dim=dim)
+        tables.plan(fill, i32([tokens - rows] * requests))
+        tables.commit(fill)
+    tables.plan(plan, i32([rows] * requests))
+    plan.check()
+    arena = PA.PagedArena(1, tables.pages, heads, dim, page_tokens=page, device=DEV)
+    arena.k_scales.fill_(abs(gap) / (127 * dim ** 0.5))
+    arena.v_scales.fill_(1 / 127)
+    arena.v_codes.fill_(127)
+    at = torch.tensor(far, device=DEV)
+    pages, places = tables.table.long()[:, at // page].reshape(-1), (at % page).repeat(requests)
+    arena.k_codes[0, pages, :, places] = 127 if gap > 0 else -127
+    arena.v_codes[0, pages, :, places] = 0
+    q = torch.ones((plan.tokens, heads * group, dim), dtype=kind, device=DEV)
+    got, lse = arena.attend(plan, q)
+    plan.check()
+    g = 127 * dim ** 0.5 * float(arena.k_scales[0, 0, 0]) * math.copysign(1, gap)
+    v = 127 * float(arena.v_scales[0, 0, 0])
+    n = tokens - rows + 1 + torch.arange(rows, device=DEV, dtype=torch.float64)  # a row sees
+    k = (at[None] < n[:, None]).sum(1).double()
+    total = k * math.exp(g) + n - k
+    want, want_lse = (n - k) * v / total, total.log()
+    return (got.double().view(requests, rows, -1), lse.double().view(requests, rows, -1),
+            want[:, None], want_lse[:, None], abs(g), n[:, None])
+
+
+def check_two_kinds(got, lse, want, want_lse, size, n):
+    """As in test_paged_gpu.py, but for weights that fp16 holds as subnormals: one of
+    the largest weight's 2^-32, since the largest is held as 2^7 at least."""
+    e = 2.0 ** -17 * size + 2.0 ** -20
+    tol = 2.0 ** -11 * want + (2.0 ** -11 + 2 * e) * want * (1 + 2.0 ** -11) + n * 2.0 ** -32 + \
+        2.0 ** -25
+    err = (got - want).abs()
+    assert bool((err <= tol).all()), f"worst {float((err / tol).max()):.2f} of the tolerance"
+    tol = e + n * 2.0 ** -24 + 2.0 ** -22 * want_lse.abs()
+    assert bool(((lse - want_lse).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 64), (256, 128)])
+@pytest.mark.parametrize("requests,rows", [(56, 1), (28, 4), (1, 300), (20, 65)])
+@pytest.mark.parametrize("gap", [12.0, 16.0, 17.6, 19.0])
+def test_a_token_that_takes_nearly_all_of_the_weight(gap, requests, rows, dim, page):
+    """Its value is 0, so the result is what the many others add up to."""
+    check_two_kinds(*two_kinds(requests, 16384, rows, [0], gap, torch.float16, heads=8, group=2,
+                               dim=dim, page=page))
+
+
+@pytest.mark.parametrize("rows", [1, 300])
+def test_the_same_over_a_long_context(rows):
+    for far in ([0], [5, 130000, 249000]):
+        check_two_kinds(*two_kinds(1, 250007, rows, far, 17.6, torch.float16, heads=1, group=2,
+                                   dim=64, page=128))
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("rows", [1, 4, 300])
+def test_scores_that_stay_just_below_a_new_reference(rows, dim):
+    """Every later weight is almost 2^8 of the first ones': the largest that fp16 has
+    to hold.  The first 512 tokens are all that any warp's first tile reads."""
+    check_two_kinds(*two_kinds(4, 9000, rows, list(range(512)), -5.5, torch.float16, heads=2,
+                               group=2, dim=dim, page=64))
