@@ -26,8 +26,14 @@ A step::
 
 Nothing here synchronises but ``PagePlan.check``; every call runs on ``stream``
 (a torch stream or a raw handle; default: the tensors' device's current torch
-stream) and can be captured in a CUDA graph.  Results do not depend on the
-order in which blocks run.
+stream) and can be captured in a CUDA graph.  Plans, tables and arenas follow
+the streams that they are used on: the first call on a stream waits for the one
+they were made on, and their memory is kept until those calls have ended, so a
+plan may be dropped as soon as its step is queued.  That the rows of a call are
+there when its stream comes to it, and that calls on several streams come in
+order, is the caller's affair, as with torch's own.  (A stream under capture
+waits for nothing outside its graph; what a graph uses has to outlive it.)
+Results do not depend on the order in which blocks run.
 """
 
 from __future__ import annotations
@@ -86,20 +92,59 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
-def _torch_stream(stream, index, *tensors):
-    """`stream` (a torch stream or a raw handle) as a torch stream; the caching
-    allocator is told that `tensors` are used on it."""
+def _torch_stream(stream, index):
+    """`stream` (a torch stream or a raw handle) as a torch stream."""
     if not hasattr(stream, "cuda_stream"):
         stream = torch.cuda.ExternalStream(int(stream), device=torch.device("cuda", index))
-    for t in tensors:
-        t.record_stream(stream)
     return stream
 
 
-def _handle(stream, index, *tensors) -> int:
+class _Buffers:
+    """Device buffers of an object, made on the torch stream that was current.  The
+    first call on any other stream waits for what that stream had queued by then
+    (their first contents, and whatever still ran on memory that they took over),
+    and the caching allocator learns of the stream, so that it gives none of them
+    away while that still runs."""
+
+    def _made(self, *tensors) -> None:
+        self._tensors = tensors
+        stream = torch.cuda.current_stream(self.device)
+        self._streams = {stream.cuda_stream}  # handles
+        self._event = None
+        if not _capturing(stream):
+            self._event = torch.cuda.Event()
+            self._event.record(stream)
+
+    def _join(self, stream) -> None:
+        # a stream that is being captured cannot wait for work outside the graph
+        if not _capturing(stream):
+            if self._event is not None:
+                stream.wait_event(self._event)
+            self._streams.add(stream.cuda_stream)
+        for t in self._tensors:
+            t.record_stream(stream)
+
+
+def _capturing(stream) -> bool:
+    with torch.cuda.stream(stream):
+        return torch.cuda.is_current_stream_capturing()
+
+
+def _handle(stream, index, owners, *tensors) -> int:
+    """The raw handle of `stream`, joined by the buffers of `owners`.  Of a stream
+    that is given, the allocator learns that `tensors` are used on it; those of the
+    current stream are the caller's affair, as with torch's own calls."""
     if stream is None:
-        return _raw_stream(index)
-    return _torch_stream(stream, index, *tensors).cuda_stream
+        handle = _raw_stream(index)
+    else:
+        stream = _torch_stream(stream, index)
+        handle = stream.cuda_stream
+        for t in tensors:
+            t.record_stream(stream)
+    for x in owners:
+        if handle not in x._streams:
+            x._join(torch.cuda.current_stream(index) if stream is None else stream)
+    return handle
 
 
 def _empty(like, shape, dtype, stream):
@@ -143,7 +188,7 @@ def _check_page(page_tokens: int) -> int:
     return int(page_tokens)
 
 
-class PagePlan:
+class PagePlan(_Buffers):
     """The buffers of one step (``PageTables.make_plan``), filled by
     ``PageTables.plan``: ``lens`` int32 [requests], ``starts`` int32
     [requests + 1], ``positions`` and ``rows`` int32 [tokens], ``slots`` int64
@@ -173,16 +218,18 @@ class PagePlan:
 
         # the step's outputs, in two allocations
         n, t = tables.requests, self.tokens
-        self.lens, self.starts, self.positions, self.rows, self.status = torch.zeros(
-            2 * n + 2 * t + 2, dtype=torch.int32, device=self.device).split([n, n + 1, t, t, 1])
-        self.slots, self.cursor = torch.zeros(
-            t + 2, dtype=torch.int64, device=self.device).split([t, 2])
+        words = torch.zeros(2 * n + 2 * t + 2, dtype=torch.int32, device=self.device)
+        self.lens, self.starts, self.positions, self.rows, self.status = words.split(
+            [n, n + 1, t, t, 1])
+        longs = torch.zeros(t + 2, dtype=torch.int64, device=self.device)
+        self.slots, self.cursor = longs.split([t, 2])
         self.c = _PlanC(tables.requests, self.tokens, self.max_fresh, tables.width, tables.pages,
                         tables.page_tokens, kv_heads, query_heads, head_dim, 1)
         need = ctypes.c_int64(0)
         _call(_lib.load().grm_b200_paged_scratch_bytes, self._index, ctypes.byref(self.c),
               ctypes.byref(need))
         self.scratch = torch.empty(need.value, dtype=torch.uint8, device=self.device)
+        self._made(words, longs, self.scratch)
         c = self.c
         c.cached, c.cursor_in = tables.lens.data_ptr(), tables.cursor.data_ptr()
         c.ring, c.table = tables.ring.data_ptr(), tables.table.data_ptr()
@@ -203,7 +250,7 @@ class PagePlan:
             raise _lib.GrmB200Error(bits, f"the step failed: {why}")
 
 
-class PageTables:
+class PageTables(_Buffers):
     """Block table ``table`` int32 [requests, width], lengths ``lens`` int32
     [requests], free pages ``ring`` int32 [pages] and ``cursor`` int64 [2]
     (pages ever taken, pages ever returned).  All pages are free at first."""
@@ -222,6 +269,7 @@ class PageTables:
         self.lens = torch.zeros(requests, dtype=torch.int32, device=self.device)
         self.ring = torch.arange(pages, dtype=torch.int32, device=self.device)
         self.cursor = torch.tensor([0, pages], dtype=torch.int64, device=self.device)
+        self._made(self.table, self.lens, self.ring, self.cursor)
 
     def make_plan(self, tokens: int, *, kv_heads: int, query_heads: int, head_dim: int,
                   max_fresh: int | None = None) -> PagePlan:
@@ -245,7 +293,7 @@ class PageTables:
             plan.grow = bool(grow)
             plan.c.grow = 1 if grow else 0
         _call(self._plan_step, self._index, plan._ref, fresh.data_ptr(),
-              _handle(stream, self._index, fresh))
+              _handle(stream, self._index, (plan, self), fresh))
         plan.planned = True
         return plan
 
@@ -259,6 +307,7 @@ class PageTables:
         if stream is not None:
             with torch.cuda.stream(_torch_stream(stream, self._index)):
                 return self.commit(plan)
+        _handle(None, self._index, (plan, self))
         self.lens.copy_(plan.lens)
         self.cursor.copy_(plan.cursor)
 
@@ -273,10 +322,10 @@ class PageTables:
         _call(_lib.load().grm_b200_paged_release, self._index, rows.data_ptr(), rows.numel(),
               self.requests, self.width, self.pages, self.page_tokens, self.table.data_ptr(),
               self.lens.data_ptr(), self.ring.data_ptr(), self.cursor.data_ptr(),
-              _handle(stream, self._index, rows))
+              _handle(stream, self._index, (self,), rows))
 
 
-class PagedArena:
+class PagedArena(_Buffers):
     """Codes int8 [layers, pages, kv_heads, page_tokens, head_dim] and scales
     fp32 [layers, pages, kv_heads] of the keys and of the values."""
 
@@ -297,6 +346,7 @@ class PagedArena:
         self.v_codes = torch.zeros(codes, dtype=torch.int8, device=self.device)
         self.k_scales = torch.zeros(shape, dtype=torch.float32, device=self.device)
         self.v_scales = torch.zeros(shape, dtype=torch.float32, device=self.device)
+        self._made(self.k_codes, self.v_codes, self.k_scales, self.v_scales)
         self._c = [_ArenaC(self.k_codes[i].data_ptr(), self.v_codes[i].data_ptr(),
                            self.k_scales[i].data_ptr(), self.v_scales[i].data_ptr(), pages,
                            kv_heads, page_tokens, head_dim) for i in range(layers)]
@@ -351,7 +401,7 @@ class PagedArena:
         if not plan.grow:
             raise ValueError("the plan's rows do not join the arena (planned with grow=False)")
         _call(self._append, self._index, plan._ref, ref, k_ptr, v_ptr, kind, k_row, k_head, v_row,
-              v_head, _handle(stream, self._index, k, v))
+              v_head, _handle(stream, self._index, (self, plan, plan.tables), k, v))
 
     def attend(self, plan: PagePlan, q, *, layer: int = 0, causal: bool = True,
                scale: float | None = None, out=None, lse=None, stream=None):
@@ -369,7 +419,7 @@ class PagedArena:
         lse = self._result("lse", lse, plan._lse_like, stream)
         _call(self._attend, self._index, plan._ref, ref, ptr, kind, row, head,
               self._scale if scale is None else float(scale), 1 if causal else 0, out.data_ptr(),
-              lse.data_ptr(), _handle(stream, self._index, q))
+              lse.data_ptr(), _handle(stream, self._index, (self, plan, plan.tables), q, out, lse))
         return out, lse
 
     def read(self, slots, *, layer: int = 0, dtype=None, stream=None):
@@ -391,5 +441,5 @@ class PagedArena:
         v = _result(k, stream)
         if n:
             _call(self._read, self._index, self._refs[layer], slots.data_ptr(), n, kind,
-                  k.data_ptr(), v.data_ptr(), _handle(stream, self._index, slots))
+                  k.data_ptr(), v.data_ptr(), _handle(stream, self._index, (self,), slots))
         return k, v

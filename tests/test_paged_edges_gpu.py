@@ -99,3 +99,106 @@ def test_scores_that_stay_just_below_a_new_reference(rows, dim):
     to hold.  The first 512 tokens are all that any warp's first tile reads."""
     check_two_kinds(*two_kinds(4, 9000, rows, list(range(512)), -5.5, torch.float16, heads=2,
                                group=2, dim=dim, page=64))
+
+
+# ---------------------------------------------------------------------- streams
+
+SLEEP = 40_000_000  # clocks, some 20 ms
+
+
+def small_step(stream, before=None):
+    """Tables, an arena and a plan made and used at once; (slots, out, lse, k, v)."""
+    if before:
+        before()
+    tables = PA.PageTables(3, 40, 20, page_tokens=16, device=DEV)
+    arena = PA.PagedArena(1, 40, 2, 64, page_tokens=16, device=DEV)
+    plan = tables.make_plan(120, kv_heads=2, query_heads=4, head_dim=64)
+    tables.plan(plan, FRESH, stream=stream)
+    arena.append(plan, KV[:, 0], KV[:, 1], stream=stream)
+    out, lse = arena.attend(plan, Q, stream=stream)
+    tables.commit(plan, stream=stream)
+    k, v = arena.read(plan.slots, stream=stream)
+    return (plan.slots, out, lse, k, v, tables.lens, tables.cursor), (tables, arena, plan)
+
+
+@pytest.fixture
+def inputs():
+    global FRESH, KV, Q
+    gen = torch.Generator(device=DEV).manual_seed(71)
+    FRESH = i32([70, 1, 40])
+    KV = torch.randn((120, 2, 2, 64), device=DEV, generator=gen).to(torch.float16)
+    Q = torch.randn((120, 4, 64), device=DEV, generator=gen).to(torch.float16)
+    torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("explicit", [True, False])
+def test_a_stream_waits_for_the_one_that_buffers_were_made_on(inputs, explicit):
+    want, _ = small_step(None)
+    want = [t.clone() for t in want]
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    if explicit:  # the buffers are made behind a long kernel and used at once elsewhere
+        got, _ = small_step(side, before=lambda: torch.cuda._sleep(SLEEP))
+    else:
+        torch.cuda._sleep(SLEEP)
+        tables = PA.PageTables(3, 40, 20, page_tokens=16, device=DEV)
+        plan = tables.make_plan(120, kv_heads=2, query_heads=4, head_dim=64)
+        with torch.cuda.stream(side):
+            tables.plan(plan, FRESH)
+        got, want = (plan.slots,), want[:1]
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("explicit", [True, False])
+def test_a_dropped_plan_keeps_its_memory_until_its_step_has_run(inputs, explicit):
+    (_, want, want_lse, *_), held = small_step(None)
+    tables, arena, _ = held
+    tables.release(i32([0, 1, 2]))
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    plan = tables.make_plan(120, kv_heads=2, query_heads=4, head_dim=64)
+    out, lse = torch.empty_like(Q), torch.empty((120, 4), device=DEV)
+    places = {t.data_ptr(): t.numel() * t.element_size() for t in (plan.scratch, plan.slots)}
+    if explicit:
+        places |= {t.data_ptr(): t.numel() * t.element_size() for t in (out, lse)}
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(SLEEP)
+    if explicit:
+        tables.plan(plan, FRESH, stream=side)
+        arena.append(plan, KV[:, 0], KV[:, 1], stream=side)
+        arena.attend(plan, Q, out=out, lse=lse, stream=side)
+        with torch.cuda.stream(side):
+            result = [out.clone(), lse.clone()]
+        del out, lse
+    else:
+        with torch.cuda.stream(side):
+            tables.plan(plan, FRESH)
+            arena.append(plan, KV[:, 0], KV[:, 1])
+            result = arena.attend(plan, Q, out=out, lse=lse)
+    del plan
+    # memory of the same sizes on the current stream, filled while the step waits
+    new = [torch.full((n,), 255, dtype=torch.uint8, device=DEV) for n in places.values()
+           for _ in range(3)]
+    assert not {t.data_ptr() for t in new} & set(places)
+    torch.cuda.synchronize()
+    assert torch.equal(result[0], want) and torch.equal(result[1], want_lse)
+
+
+def test_a_graph_of_a_step_whose_plan_no_stream_has_used(inputs):
+    """Captured at once, without a step before on the capturing stream."""
+    want, _ = small_step(None)
+    want = [t.clone() for t in want[:3]]
+    tables = PA.PageTables(3, 40, 20, page_tokens=16, device=DEV)
+    arena = PA.PagedArena(1, 40, 2, 64, page_tokens=16, device=DEV)
+    plan = tables.make_plan(120, kv_heads=2, query_heads=4, head_dim=64)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        tables.plan(plan, FRESH)
+        arena.append(plan, KV[:, 0], KV[:, 1])
+        out, lse = arena.attend(plan, Q)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip((plan.slots, out, lse), want))
