@@ -86,6 +86,7 @@ _SIGS = {
     "grm_b200_arena_splice": (_I, [_P, _I64, _I64, _P, _I64, _I64, _I64, _I64, _P, _P, _P]),
     "grm_b200_paged_scratch_bytes": (_I, [_P, _P]),
     "grm_b200_paged_plan_step": (_I, [_P, _P, _P]),
+    "grm_b200_paged_commit": (_I, [_P, _P, _P, _P]),
     "grm_b200_paged_release": (_I, [_P, _I64, _I64, _I64, _I64, _I, _P, _P, _P, _P, _P]),
     "grm_b200_paged_append": (_I, [_P, _P, _P, _P, _I, _I64, _I64, _I64, _I64, _P]),
     "grm_b200_paged_read": (_I, [_P, _P, _I64, _I, _P, _P, _P]),

@@ -35,6 +35,8 @@ struct Header {           // written by the plan kernel
   int32_t qtiles;         // entries of the prompt kernel's list: parts of prompt tiles
   int32_t joins;          // qtiles, where tiles are in more than one part; 0 where none is
   int32_t rows;           // packed rows of the step
+  int32_t take;           // pages that it takes
+  int32_t committed;      // whether a commit has taken it up
 };
 
 // Sizes that follow from the plan's sizes alone, so that the plan kernel and

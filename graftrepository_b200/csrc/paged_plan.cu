@@ -279,7 +279,9 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
                            failed ? 0 : (int)total[kTouched],
                            failed ? 0 : (int)total[kTiles],
                            failed || part_tokens == 0 ? 0 : (int)total[kTiles],
-                           all_rows};
+                           all_rows,
+                           failed ? 0 : (int)total[kTake],
+                           0};
     }
     for (int i = tid; i < p.s.workers; i += kPlanThreads) p.l.count[i] = 0;
   }
@@ -414,6 +416,42 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
       if (u >= sum[kUnits][0] && u < sum[kUnits][n])
         p.l.start[w] = (int)(r0 + find(sum[kUnits], n, u));
     }
+  }
+}
+
+constexpr int kCommitThreads = 1024;
+
+// One block, as nothing is written before every row has been looked at: a step is
+// taken up if its requests still hold what they held when it was planned and no
+// page has been taken since.  Pages returned meanwhile and requests without rows in
+// the step are left as they are.  (64 requests 1.7 us, 4,096 3.1, 65,536 34 beside a
+// plan's 98.)
+__global__ void __launch_bounds__(kCommitThreads)
+    commit_kernel(int64_t requests, const int32_t* after, const int32_t* starts, Header* header,
+                  const int64_t* cursor_after, int32_t* lens, int64_t* cursor, int32_t* status) {
+  const int take = header->take;
+  const bool again = header->committed != 0;
+  bool ready = !again && (take == 0 || cursor[0] == cursor_after[0] - take), done = again;
+#pragma unroll 4
+  for (int64_t r = threadIdx.x; r < requests; r += blockDim.x) {
+    const int n = starts[r + 1] - starts[r], held = lens[r], then = after[r];
+    ready &= n <= 0 || held == then - n;
+    done &= n <= 0 || held == then;
+  }
+  ready = __syncthreads_and(ready);
+  done = __syncthreads_and(done);
+  if (!ready) {
+    if (!done && threadIdx.x == 0) atomicOr(status, GRM_B200_PLAN_STALE);
+    return;
+  }
+#pragma unroll 4
+  for (int64_t r = threadIdx.x; r < requests; r += blockDim.x) {
+    const int n = starts[r + 1] - starts[r], then = after[r];
+    if (n > 0) lens[r] = then;
+  }
+  if (threadIdx.x == 0) {
+    if (take > 0) cursor[0] = cursor_after[0];
+    header->committed = 1;
   }
 }
 
@@ -713,6 +751,26 @@ int grm_b200_paged_plan_step(const grm_b200_paged_plan* plan, const int32_t* fre
   plan_kernel<<<p.chunks * (p.row_blocks + 2 * p.page_blocks + 1), kPlanThreads, 0,
                 static_cast<cudaStream_t>(stream)>>>(p);
   return launch_status("paged plan");
+}
+
+int grm_b200_paged_commit(const grm_b200_paged_plan* plan, int32_t* lens, int64_t* cursor,
+                          void* stream) {
+  int rc = check_sizes(plan);
+  if (rc) return rc;
+  if (!plan->grow || lens != plan->cached || cursor != plan->cursor_in) {
+    set_thread_error("paged commit: a step that joins (grow != 0), and the plan's own cached and "
+                     "cursor_in");
+    return GRM_B200_EINVAL;
+  }
+  int sms = 0;
+  if ((rc = check_plan(plan)) || (rc = current_sms(&sms))) return rc;
+  Shape s;
+  make_shape(*plan, sms, &s);
+  const int threads = (int)std::min<int64_t>(ceil_div64(plan->requests, 32) * 32, kCommitThreads);
+  commit_kernel<<<1, threads, 0, static_cast<cudaStream_t>(stream)>>>(
+      plan->requests, plan->lens, plan->starts, lists_of(s, plan->scratch).header, plan->cursor,
+      lens, cursor, plan->status);
+  return launch_status("paged commit");
 }
 
 int grm_b200_paged_release(const int32_t* rows_device, int64_t count, int64_t requests,

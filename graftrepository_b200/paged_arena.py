@@ -24,6 +24,11 @@ A step::
     tables.commit(plan)                       # the new lengths hold from here on
     tables.release(rows)                      # requests that are done give their pages back
 
+Steps whose rows join the arena go one at a time, from ``plan`` to ``commit``,
+whatever plans and streams they use: two that are planned side by side take the
+same pages.  Planning another step leaves one that is not committed behind; what
+is called with it then is refused.
+
 Nothing here synchronises but ``PagePlan.check``; every call runs on ``stream``
 (a torch stream or a raw handle; default: the tensors' device's current torch
 stream) and can be captured in a CUDA graph.  Plans, tables and arenas follow
@@ -50,13 +55,15 @@ __all__ = ["PAGE_TOKENS", "HEAD_DIMS", "PageTables", "PagePlan", "PagedArena"]
 PAGE_TOKENS = (16, 32, 64, 128)
 HEAD_DIMS = (64, 128, 256)
 
-PLAN_BAD_LENGTH, PLAN_ROWS, PLAN_TABLE, PLAN_PAGES, PLAN_WAIT = 1, 2, 4, 8, 16
+PLAN_BAD_LENGTH, PLAN_ROWS, PLAN_TABLE, PLAN_PAGES, PLAN_WAIT, PLAN_STALE = 1, 2, 4, 8, 16, 32
 _REASONS = {
     PLAN_BAD_LENGTH: "a negative length, or one past 2^31 - 1",
     PLAN_ROWS: "more new rows than the plan has room for (tokens, max_fresh)",
     PLAN_TABLE: "a request needs more pages than its block table row has entries",
     PLAN_PAGES: "not enough free pages",
     PLAN_WAIT: "a wait inside attention gave up and rows are missing",
+    PLAN_STALE: "its requests or free pages have changed since it was planned, and it was not "
+                "committed",
 }
 
 
@@ -239,11 +246,18 @@ class PagePlan(_Buffers):
         c.status = self.status.data_ptr()
         c.scratch, c.scratch_bytes = self.scratch.data_ptr(), need.value
         self.planned, self.grow = False, True
+        self._turn = None  # of the tables' joining steps, until it is committed
         self._ref = ctypes.byref(c)
+
+    def _in_turn(self) -> None:
+        if self._turn is not None and self._turn != self.tables._turn:
+            raise ValueError("another step of these tables has been planned since and takes the "
+                             "same pages; plan this one again")
 
     def check(self) -> None:
         """Wait for the plan (and calls that used it) and raise if the step
-        could not be planned: it then took no pages and has no rows."""
+        could not be planned (it then took no pages and has no rows) or its
+        commit came too late."""
         bits = int(self.status.item())
         if bits:
             why = "; ".join(text for bit, text in _REASONS.items() if bits & bit)
@@ -265,6 +279,7 @@ class PageTables(_Buffers):
         self.device = _device(device)
         self._index, self._shape = self.device.index, torch.Size((self.requests,))
         self._plan_step = _lib.load().grm_b200_paged_plan_step
+        self._turn = 0  # joining steps planned so far, those under capture left out
         self.table = torch.full((requests, width), -1, dtype=torch.int32, device=self.device)
         self.lens = torch.zeros(requests, dtype=torch.int32, device=self.device)
         self.ring = torch.arange(pages, dtype=torch.int32, device=self.device)
@@ -276,13 +291,14 @@ class PageTables(_Buffers):
         """Buffers for steps of up to `tokens` new rows, at most `max_fresh` of
         one request (default: `tokens`; a step that keeps it small, such as
         max_fresh = 1 for decoding, is served by the kernel made for that).  A
-        plan's steps may not overlap on the GPU; make one plan for each stream."""
+        plan's steps may not overlap on the GPU."""
         return PagePlan(self, tokens, kv_heads, query_heads, head_dim, max_fresh)
 
     def plan(self, plan: PagePlan, fresh, *, grow: bool = True, stream=None) -> PagePlan:
         """Lay out a step: request r brings ``fresh[r]`` new rows (int32 on the
         device).  `grow`: the rows are tokens that join the requests; without
-        it they are query rows that only read what is cached."""
+        it they are query rows that only read what is cached.  A joining step
+        leaves behind one that was planned and not committed."""
         if plan.tables is not self:
             raise ValueError("the plan was made for other tables")
         if (not isinstance(fresh, torch.Tensor) or fresh.dtype is not torch.int32 or
@@ -294,26 +310,34 @@ class PageTables(_Buffers):
             plan.c.grow = 1 if grow else 0
         _call(self._plan_step, self._index, plan._ref, fresh.data_ptr(),
               _handle(stream, self._index, (plan, self), fresh))
-        plan.planned = True
+        plan.planned, plan._turn = True, None
+        # a step that a graph plans again has no turn: the host does not see it
+        if grow and not (torch.cuda.is_current_stream_capturing() if stream is None else
+                         _capturing(_torch_stream(stream, self._index))):
+            plan._turn = self._turn = self._turn + 1
         return plan
 
     def commit(self, plan: PagePlan, *, stream=None) -> None:
-        """Take up the lengths of a planned step: requests hold `plan.lens`
-        tokens from here on.  The plan stays good for append and attend."""
+        """Take up the lengths of a planned step: requests with rows in it hold
+        `plan.lens` tokens from here on.  The plan stays good for append and
+        attend, and a second commit of it does nothing.  Other requests may be
+        released between plan and commit; where the step's own requests or the
+        pages it takes have changed since, nothing is taken up and
+        ``plan.check`` says so."""
         if plan.tables is not self or not plan.planned:
             raise ValueError("commit takes a plan of these tables that has been planned")
         if not plan.grow:
             return
-        if stream is not None:
-            with torch.cuda.stream(_torch_stream(stream, self._index)):
-                return self.commit(plan)
-        _handle(None, self._index, (plan, self))
-        self.lens.copy_(plan.lens)
-        self.cursor.copy_(plan.cursor)
+        plan._in_turn()
+        _call(_lib.load().grm_b200_paged_commit, self._index, plan._ref, self.lens.data_ptr(),
+              self.cursor.data_ptr(), _handle(stream, self._index, (plan, self)))
+        plan._turn = None
 
     def release(self, rows, *, stream=None) -> None:
-        """Return the pages of the requests ``rows`` (int32 on the device) to
-        the ring and empty them."""
+        """Return the pages that the requests ``rows`` (int32 on the device) hold
+        to the ring and empty them.  A step that is planned and not committed
+        does not hold its pages yet; if it has rows of these requests, its
+        commit comes too late."""
         if (not isinstance(rows, torch.Tensor) or rows.dtype != torch.int32 or rows.dim() != 1 or
                 rows.device != self.device or not rows.is_contiguous()):
             raise ValueError(f"rows must be int32 [n] on {self.device}")
@@ -377,6 +401,8 @@ class PagedArena(_Buffers):
         """The layer's buffers, for a plan that is good for a call."""
         if not plan.planned:
             raise ValueError("the plan has not been planned yet (PageTables.plan)")
+        if plan._turn is not None:
+            plan._in_turn()
         if not 0 <= layer < self.layers:
             raise ValueError(f"layer {layer} of {self.layers}")
         return self._refs[layer]

@@ -444,7 +444,9 @@ typedef struct grm_b200_paged_arena {
  * row) and slots[tokens] (page * page_tokens + offset), -1 past the last row;
  * cursor[2]; status[1], GRM_B200_PLAN_* bits.  cursor and cursor_in must not
  * be the same buffer, nor lens and cached: planning again plans the same step,
- * and the caller takes a step up by making the new lengths the cached ones.
+ * until grm_b200_paged_commit has made the new lengths the cached ones.  Steps
+ * with grow != 0 of the same tables go one at a time, from plan to commit: two
+ * that are planned side by side take the same pages.
  * scratch: scratch_bytes (grm_b200_paged_scratch_bytes) of device memory, the
  * step's work lists and the partial results of attention; calls that share it
  * must not overlap on the GPU. */
@@ -482,6 +484,7 @@ typedef struct grm_b200_paged_plan {
 #define GRM_B200_PLAN_TABLE 4       /* a request needs more than table_width pages */
 #define GRM_B200_PLAN_PAGES 8       /* not enough free pages */
 #define GRM_B200_PLAN_WAIT 16       /* a bounded wait inside attend gave up: rows are missing */
+#define GRM_B200_PLAN_STALE 32      /* the tables have changed since: the commit took nothing up */
 
 /* Scratch bytes of a plan of these sizes (the pointers are not read). */
 int grm_b200_paged_scratch_bytes(const grm_b200_paged_plan* plan, int64_t* out_bytes);
@@ -494,6 +497,16 @@ int grm_b200_paged_scratch_bytes(const grm_b200_paged_plan* plan, int64_t* out_b
  * slots are -1, and attention over the plan is not causal. */
 int grm_b200_paged_plan_step(const grm_b200_paged_plan* plan, const int32_t* fresh_device,
                              void* stream);
+
+/* Take a planned step up: the requests that have rows in it hold lens[r] tokens
+ * from here on, and its pages are theirs.  lens and cursor are the plan's cached
+ * and cursor_in.  Pages returned since the step was planned and requests without
+ * rows in it keep what they have.  A step whose requests have changed since, by
+ * a release or another commit, or whose pages another step has taken, is not
+ * taken up: nothing changes but the plan's status, which gets
+ * GRM_B200_PLAN_STALE.  A commit that is given twice is one. */
+int grm_b200_paged_commit(const grm_b200_paged_plan* plan, int32_t* lens, int64_t* cursor,
+                          void* stream);
 
 /* Return the pages of the requests rows_device[count] to the ring (in the
  * order of the list) and set their lengths to 0; a row that is out of range or

@@ -11,6 +11,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
+from graftrepository_b200 import _lib  # noqa: E402
 from graftrepository_b200 import paged_arena as PA  # noqa: E402
 from test_paged_gpu import DEV, ceil, i32, run_attention  # noqa: E402
 
@@ -202,3 +203,139 @@ def test_a_graph_of_a_step_whose_plan_no_stream_has_used(inputs):
     graph.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip((plan.slots, out, lse), want))
+
+
+# ----------------------------------------------------- steps that are overtaken
+
+def two_requests():
+    """Requests 0 and 1 of three hold 20 and 40 tokens in pages of 16."""
+    tables = PA.PageTables(3, 12, 6, page_tokens=16, device=DEV)
+    plans = [tables.make_plan(60, kv_heads=1, query_heads=1, head_dim=64) for _ in range(2)]
+    tables.plan(plans[0], i32([20, 40, 0]))
+    tables.commit(plans[0])
+    plans[0].check()
+    assert tables.lens.tolist() == [20, 40, 0] and tables.cursor.tolist() == [5, 12]
+    return tables, *plans
+
+
+def free_pages(tables):
+    a, b = tables.cursor.tolist()
+    ring = tables.ring.tolist()
+    return [ring[i % tables.pages] for i in range(a, b)]
+
+
+def held_pages(tables):
+    return [p for row, n in zip(tables.table.tolist(), tables.lens.tolist())
+            for p in row[: ceil(n, tables.page_tokens)]]
+
+
+def test_a_release_between_plan_and_commit():
+    tables, plan, _ = two_requests()
+    tables.plan(plan, i32([30, 0, 5]))  # 50 tokens and 5: three pages more
+    tables.release(i32([1]))            # has no row in the step
+    tables.commit(plan)
+    plan.check()
+    assert tables.lens.tolist() == [50, 0, 5]
+    assert sorted(free_pages(tables) + held_pages(tables)) == list(range(12))
+
+
+@pytest.mark.parametrize("fresh", [[30, 0, 5], [2, 0, 0]])
+def test_a_release_of_a_request_with_rows_in_the_step(fresh):
+    tables, plan, _ = two_requests()
+    tables.plan(plan, i32(fresh))
+    tables.release(i32([0]))
+    tables.commit(plan)
+    with pytest.raises(_lib.GrmB200Error, match="not committed"):
+        plan.check()
+    assert tables.lens.tolist() == [0, 40, 0]
+    assert sorted(free_pages(tables) + held_pages(tables)) == list(range(12))
+    tables.plan(plan, i32(fresh))  # planned again it is a step like any other
+    tables.commit(plan)
+    plan.check()
+    assert tables.lens.tolist() == [fresh[0], 40, fresh[2]]
+    assert sorted(free_pages(tables) + held_pages(tables)) == list(range(12))
+
+
+def test_a_commit_given_twice_and_one_that_is_late():
+    tables, plan, other = two_requests()
+    tables.plan(plan, i32([1, 0, 17]))
+    tables.commit(plan)
+    tables.commit(plan)
+    plan.check()
+    state = tables.lens.tolist(), tables.cursor.tolist()
+    assert state == ([21, 40, 17], [7, 12])
+    tables.plan(other, i32([0, 20, 0]))
+    tables.commit(other)
+    tables.commit(plan)  # its requests hold what it gave them: still nothing to do
+    plan.check()
+    assert tables.lens.tolist() == [21, 60, 17] and tables.cursor.tolist() == [8, 12]
+    tables.release(i32([2]))
+    tables.commit(plan)  # and now they do not
+    with pytest.raises(_lib.GrmB200Error, match="not committed"):
+        plan.check()
+    assert tables.lens.tolist() == [21, 60, 0] and tables.cursor.tolist() == [8, 14]
+    assert sorted(free_pages(tables) + held_pages(tables)) == list(range(12))
+
+
+def test_two_steps_side_by_side():
+    tables, plan, other = two_requests()
+    arena = PA.PagedArena(1, 12, 1, 64, page_tokens=16, device=DEV)
+    rows = torch.ones((60, 1, 64), dtype=torch.float16, device=DEV)
+    tables.plan(plan, i32([30, 0, 0]))
+    tables.plan(other, i32([0, 0, 33]))  # takes the pages that `plan` would
+    for call in (lambda: arena.append(plan, rows, rows), lambda: arena.attend(plan, rows),
+                 lambda: tables.commit(plan)):
+        with pytest.raises(ValueError, match="planned since"):
+            call()
+    arena.append(other, rows, rows)
+    arena.attend(other, rows)
+    tables.commit(other)
+    tables.plan(plan, i32([30, 0, 0]))
+    arena.append(plan, rows, rows)
+    tables.commit(plan)
+    arena.attend(other, rows)  # committed steps stay good
+    plan.check()
+    other.check()
+    assert tables.lens.tolist() == [50, 40, 33]
+    assert sorted(free_pages(tables) + held_pages(tables)) == list(range(12))
+    # rows that only read are no such step, and a step that is left behind harms none
+    reader = tables.make_plan(4, kv_heads=1, query_heads=1, head_dim=64)
+    tables.plan(plan, i32([1, 0, 0]))
+    tables.plan(reader, i32([2, 1, 1]), grow=False)
+    arena.attend(reader, rows[:4], causal=False)
+    arena.append(plan, rows, rows)
+    tables.commit(plan)
+    assert tables.lens.tolist() == [51, 40, 33]
+
+
+def test_a_graph_that_plans_is_committed_outside():
+    """The host does not see a replay's plan, and refuses nothing for it."""
+    tables, plan, other = two_requests()
+    fresh = i32([1, 1, 0])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        tables.plan(plan, fresh)
+    for step in range(3):
+        tables.plan(other, i32([0, 0, 7]))
+        tables.commit(other)
+        graph.replay()
+        tables.commit(plan)
+        plan.check()
+        assert tables.lens.tolist() == [21 + step, 41 + step, 7 + 7 * step]
+    assert sorted(free_pages(tables) + held_pages(tables)) == list(range(12))
+
+
+@pytest.mark.parametrize("requests", [1, 33, 1024, 5000])
+def test_commit_of_many_requests(requests):
+    gen = torch.Generator().manual_seed(requests)
+    tables = PA.PageTables(requests, 3 * requests, 3, page_tokens=16, device=DEV)
+    plan = tables.make_plan(20 * requests, kv_heads=1, query_heads=1, head_dim=64, max_fresh=20)
+    lens = torch.zeros(requests, dtype=torch.int32)
+    for _ in range(2):
+        fresh = torch.randint(0, 21, (requests,), generator=gen, dtype=torch.int32)
+        tables.plan(plan, fresh.to(DEV))
+        tables.commit(plan, stream=torch.cuda.current_stream())
+        plan.check()
+        lens += fresh
+        assert torch.equal(tables.lens.cpu(), lens)
+        assert tables.cursor.tolist() == [int(((lens + 15) // 16).sum()), 3 * requests]
