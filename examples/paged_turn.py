@@ -89,13 +89,13 @@ class PagedTurn:
         plan.check()
 
     def step(self, x, fresh):
-        """Hidden rows `x` [tokens, width], the requests' `fresh` rows one after
-        another; returns the hidden rows after all layers."""
-        plan = self.one if x.shape[0] == self.one.tokens else self.many
+        """Hidden rows `x` [tokens, width], the requests' `fresh` rows (a list of
+        counts) one after another; returns the hidden rows after all layers."""
+        plan = self.one if max(fresh) <= 1 else self.many
         rows = x.shape[0]
         if rows < plan.tokens:
             x = torch.cat([x, x.new_zeros((plan.tokens - rows, self.width))])
-        self.tables.plan(plan, fresh)
+        self.tables.plan(plan, self.counts(fresh))
         for layer in range(self.layers):
             y = torch.nn.functional.rms_norm(x, (self.width,))
             q = self.rotate((y @ self.wq[layer]).view(plan.query_shape), plan.positions)
@@ -105,6 +105,7 @@ class PagedTurn:
             out = self.attend(plan, q, layer)
             x = x + out.view(plan.tokens, self.width) @ self.wo[layer]
         self.tables.commit(plan)
+        plan.check()  # waits; the next plan call would clear what this step has to say
         return x[:rows]
 
     def attend(self, plan, q, layer):
@@ -137,20 +138,17 @@ def random_grafts(turn, n, tokens, seed):
 
 
 def run(turn, question=(5, 40, 1, 17), answer=16, grafts=2, graft_tokens=128):
-    """Admit every request, take the question, answer token by token; returns the
-    last hidden row of each request."""
+    """Admit every request, take the question (its rows for each of them), answer
+    those that asked token by token; returns the last hidden row of each of these."""
     for r in range(turn.requests):
         turn.admit(r, random_grafts(turn, grafts, graft_tokens, seed=r))
     gen = torch.Generator(device=turn.device).manual_seed(1)
     x = torch.randn((sum(question), turn.width), device=turn.device, generator=gen)
-    x = turn.step(x.to(torch.bfloat16), turn.counts(question))
-    last = torch.tensor(question).cumsum(0) - 1
-    x = x[last.to(turn.device)]
-    ones = turn.counts([1] * turn.requests)
+    x = turn.step(x.to(torch.bfloat16), question)
+    asked = torch.tensor(question) > 0
+    x = x[(torch.tensor(question).cumsum(0) - 1)[asked].to(turn.device)]
     for _ in range(answer):  # the stand-in feeds its own result back
-        x = turn.step(x, ones)
-    turn.one.check()
-    turn.many.check()
+        x = turn.step(x, asked.int().tolist())
     return x
 
 
