@@ -218,6 +218,7 @@ constexpr unsigned kWaitLimit = 1u << 24;
 // another value.  Tests set it to 0 so that every wait gives up at once and
 // the error path (drain the copies in flight, report status 3001) runs
 // without any wait actually hanging.  The drain itself always uses kWaitLimit.
+// Paged attention takes it where it is below its own limit.
 unsigned scan_wait_limit();
 
 __host__ __device__ inline int64_t ceil_div64(int64_t a, int64_t b) { return (a + b - 1) / b; }

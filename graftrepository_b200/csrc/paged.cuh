@@ -102,8 +102,14 @@ constexpr float kLazy = 8.0f;  // how far a row's scores may pass its reference 
 constexpr float kLift = 7.0f;
 constexpr float kUnlift = 0x1p-7f;
 
+// Probes of a bounded wait.  A wait that gives up leaves NaN in its rows and
+// GRM_B200_PLAN_WAIT in the plan's status; copies and products in flight are waited
+// for (with this limit, whatever AttendParams::probes is) before the block ends.
+constexpr unsigned kProbes = 1u << 18;
+
 struct AttendParams {
   Lists l;
+  unsigned probes;  // kProbes, or less by GRM_B200_WAIT_LIMIT
   const int32_t* table;
   const int32_t* lens;
   const int32_t* starts;

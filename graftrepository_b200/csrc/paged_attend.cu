@@ -55,7 +55,6 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-constexpr unsigned kProbes = 1u << 18;  // probes of a bounded wait
 
 struct SplitParams {
   CUtensorMap k_map, v_map;  // codes as [pages * kv_heads][page_tokens][head_dim] bytes
@@ -576,7 +575,8 @@ __global__ void __launch_bounds__(kThreads, (Layout<D, NT>::kBlocks))
       const int stage = used % LY::kStages;
       if (!failed)
         failed = !__all_sync(
-            kFull, mbar_wait(&bars[warp][stage], (used / LY::kStages) & 1, kProbes));
+            kFull, mbar_wait(&bars[warp][stage], (used / LY::kStages) & 1, p.probes));
+      if (failed) break;  // `used` stays at the first stage that was not seen to land
       ++used;
       __syncwarp();
       const uint32_t kb = ring + stage * LY::kStage;
@@ -723,7 +723,11 @@ __global__ void __launch_bounds__(kThreads, (Layout<D, NT>::kBlocks))
         }
       }
       __syncwarp();  // the stage is read: its place is free
-      if (!failed) issue();
+      issue();
+    }
+    if (failed) {  // tokens are missing: no number for these rows
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) l[nt][0] = l[nt][1] = __int_as_float(0x7FC00000);
     }
 
     // ---- join the four warps
@@ -995,6 +999,7 @@ int grm_b200_paged_attend(const grm_b200_paged_plan* plan, const grm_b200_paged_
   p.out = static_cast<uint16_t*>(out_device);
   p.lse = lse_device;
   p.qtile_tokens = s.qtile_tokens;
+  p.probes = std::min(scan_wait_limit(), kProbes);
   p.status = plan->status;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (s.qtile_cap > 0 &&

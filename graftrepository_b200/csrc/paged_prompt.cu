@@ -60,7 +60,6 @@ constexpr int kQueryAtom = kM * 128;  // 128 rows x 64 halves
 constexpr int kPromptThreads = 15 * 32;
 constexpr int kMmaWarp = 12, kLoadWarp = 14;
 constexpr uint32_t kTmemCols = 512;
-constexpr unsigned kProbes = 1u << 18;  // probes of a bounded wait
 
 // Two query tiles and key tiles of 128 tokens, in two steps of the softmax; at
 // head_dim 256, whose results alone take half of tensor memory, one query tile
@@ -134,9 +133,10 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
 // Every lane of a warp waits; false, for all of them, when a wait gave up.
 // The loops of this kernel share an instruction cache that they barely fit, so
 // what is not the common path stays out of line.
-__device__ __noinline__ bool wait_long(uint64_t* bar, unsigned parity, volatile int* fail) {
+__device__ __noinline__ bool wait_long(uint64_t* bar, unsigned parity, volatile int* fail,
+                                       unsigned probes) {
   bool ok = false;
-  for (unsigned i = 0; i < kProbes; ++i) {
+  for (unsigned i = 0; i < probes; ++i) {
     if ((ok = mbar_try_wait(bar, parity))) break;
     if (*fail) break;
   }
@@ -144,9 +144,10 @@ __device__ __noinline__ bool wait_long(uint64_t* bar, unsigned parity, volatile 
   if (!ok) *fail = 1;
   return ok;
 }
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, unsigned parity, volatile int* fail) {
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, unsigned parity, volatile int* fail,
+                                          unsigned probes) {
   if (__all_sync(kFull, mbar_try_wait(bar, parity))) return true;
-  return wait_long(bar, parity, fail);
+  return wait_long(bar, parity, fail, probes);
 }
 
 struct Scale {
@@ -154,8 +155,29 @@ struct Scale {
 };
 static_assert(sizeof(Scale) == 16, "PromptLayout::kScaleBytes");
 
+// Row `row` of query tile t of a block in which a wait gave up: no numbers.
+template <int D>
+__device__ __noinline__ void lose_row(const AttendParams& p, int4 e, int h, int t, int row) {
+  const PromptTile pt = prompt_tile<D>(p, e);
+  if (row >= (t == 0 ? pt.toks[0] : pt.toks[1]) * p.group) return;
+  const float nan = __int_as_float(0x7FC00000);
+  if (pt.parts > 1) {  // the sum of its part
+    float* slot = p.l.qpart + ((int64_t)(e.w + (e.z & 255)) * p.kv_heads + h) * prompt_slot(D);
+    *reinterpret_cast<float2*>(slot + prompt_rows_of(D) * D + 2 * (t * kM + row)) =
+        make_float2(-INFINITY, nan);
+    return;
+  }
+  const int64_t orow = (int64_t)(pt.start + pt.tok0 + t * pt.per + row / p.group) * p.kv_heads *
+                           p.group + h * p.group + row % p.group;
+  for (int c = 0; c < D / 8; ++c)
+    reinterpret_cast<uint4*>(p.out + orow * D)[c] =
+        make_uint4(0x7FFF7FFFu, 0x7FFF7FFFu, 0x7FFF7FFFu, 0x7FFF7FFFu);
+  if (p.lse) p.lse[orow] = nan;
+}
+
 template <typename T, int D>
-__global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendParams p) {
+__global__ void __launch_bounds__(kPromptThreads, 1)
+    prompt_kernel(const __grid_constant__ AttendParams p) {
   using LY = PromptLayout<D>;
   constexpr int kN = LY::kN, kHalves = LY::kHalves, kRing = LY::kRing, kRaws = LY::kRaws;
   extern __shared__ unsigned char raw[];
@@ -235,7 +257,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sh_tmem;
-  volatile int* const fail = &sh_fail;
+  auto wait = [&](uint64_t* bar, unsigned parity) {
+    return warp_wait(bar, parity, &sh_fail, p.probes);
+  };
 
   if (warp < LY::kSoftWarps) {
     // ------------------------------------------------------------- softmax
@@ -305,9 +329,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
 #pragma unroll 1
       for (int i = 0; i < halves_seen; ++i) {
         const int j = i / kHalves, buf = i & 1;
-        if (i % kHalves == 0 && !(ok = warp_wait(&scale_full[j % kRing], (j / kRing) & 1, fail)))
+        if (i % kHalves == 0 && !(ok = wait(&scale_full[j % kRing], (j / kRing) & 1)))
           break;
-        if (!(ok = warp_wait(&s_full[t][buf], (i >> 1) & 1, fail))) break;
+        if (!(ok = wait(&s_full[t][buf], (i >> 1) & 1))) break;
         tc_fence_after();
         // the row's 64 scores, in registers from here on
         uint32_t v[2][32];
@@ -354,7 +378,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
           m = next;
           l *= a;
           if (i > 0) {  // once the products of the half before have ended
-            if (!(ok = warp_wait(&o_full[t], (i - 1) & 1, fail))) break;
+            if (!(ok = wait(&o_full[t], (i - 1) & 1))) break;
             tc_fence_after();
 #pragma unroll 1
             for (int c = 0; c < D / 16; ++c) {
@@ -369,7 +393,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
         // The two warps of a scheduler take turns at the exponentials, so that one's
         // other work lies under them.
         if (two && t + i > 0 &&
-            !(ok = warp_wait(&turn[t][warp & 3], (i - 1 + t) & 1, fail)))
+            !(ok = wait(&turn[t][warp & 3], (i - 1 + t) & 1)))
           break;
         const float ref = m == -INFINITY ? 0.0f : m - kLift;
 #pragma unroll
@@ -399,7 +423,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[t][buf]);
       }
-      if (ok && warp_wait(&o_done[t], 0, fail)) {
+      if (ok && wait(&o_done[t], 0)) {
         tc_fence_after();
         // looked up again rather than kept in registers through the loop
         int tid;
@@ -479,7 +503,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
       const int j = x >> 1, side = x & 1, st = j & 1, place = j % kRaws;
       const unsigned char* src = sm_raw + (place * 2 + side) * LY::kRaw + row0 * D + c * 16;
       unsigned char* at = (side ? sm_v : sm_k) + st * LY::kTile + (c / 4) * LY::kAtom;
-      if (!(ok = warp_wait(&raw_full[side][place], (j / kRaws) & 1, fail))) break;
+      // (with no probes at all the block gives up here: a look at the limit in every
+      // wait costs 2 % of the kernel's time)
+      if (!(ok = p.probes > 0 && wait(&raw_full[side][place], (j / kRaws) & 1))) break;
       uint4 r[4];
       auto load = [&] {
 #pragma unroll
@@ -489,7 +515,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
       };
       load();
       if (j >= 2 &&
-          !(ok = warp_wait(side ? &v_empty[st] : &k_empty[st], ((j >> 1) - 1) & 1, fail)))
+          !(ok = wait(side ? &v_empty[st] : &k_empty[st], ((j >> 1) - 1) & 1)))
         break;
 #pragma unroll 1
       for (int i0 = 0; i0 < kN / LY::kConvWarps / kRows; i0 += 4) {
@@ -572,21 +598,21 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
         auto next_scores = [&](int i) {
           const int j = i / kHalves;
           if (i % kHalves == 0) {
-            if (!warp_wait(&k_full[j & 1], (j >> 1) & 1, fail)) return false;
+            if (!wait(&k_full[j & 1], (j >> 1) & 1)) return false;
             tc_fence_after();
           }
           scores(i);
           return true;
         };
-        bool ok = warp_wait(&q_full[t], 0, fail);
+        bool ok = wait(&q_full[t], 0);
         tc_fence_after();
         ok = ok && next_scores(0);
         if (ok && steps > 1) ok = next_scores(1);
 #pragma unroll 1
         for (int i = 0; i < steps && ok; ++i) {
           const int j = i / kHalves;
-          if (i % kHalves == 0) ok = warp_wait(&v_full[j & 1], (j >> 1) & 1, fail);
-          ok = ok && warp_wait(&p_full[t][i & 1], (i >> 1) & 1, fail);
+          if (i % kHalves == 0) ok = wait(&v_full[j & 1], (j >> 1) & 1);
+          ok = ok && wait(&p_full[t][i & 1], (i >> 1) & 1);
           if (!ok) break;
           tc_fence_after();
           results(i);
@@ -629,7 +655,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
 #pragma unroll
         for (int side = 0; side < 2; ++side) {
           const int place = j % kRaws;
-          if (j >= kRaws && !(ok = warp_wait(&raw_empty[side][place], (j / kRaws - 1) & 1, fail)))
+          if (j >= kRaws && !(ok = wait(&raw_empty[side][place], (j / kRaws - 1) & 1)))
             break;
           issued[side] = j + 1;
           if (lane == 0) mbar_arrive_expect_tx(&raw_full[side][place], bytes);
@@ -661,7 +687,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const AttendP
   __syncthreads();
   tc_fence_after();
   if (warp == kMmaWarp) tmem_dealloc(tmem, kTmemCols);
-  if (threadIdx.x == 0 && sh_fail) atomicOr(p.status, GRM_B200_PLAN_WAIT);
+  if (sh_fail) {
+    if (warp < LY::kSoftWarps)
+      lose_row<D>(p, p.l.qtiles[blockIdx.x / p.kv_heads], blockIdx.x % p.kv_heads,
+                  threadIdx.x >> 7, threadIdx.x & 127);
+    if (threadIdx.x == 0) atomicOr(p.status, GRM_B200_PLAN_WAIT);
+  }
 }
 
 template <typename T, int D>

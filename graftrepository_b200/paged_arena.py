@@ -61,7 +61,7 @@ _REASONS = {
     PLAN_ROWS: "more new rows than the plan has room for (tokens, max_fresh)",
     PLAN_TABLE: "a request needs more pages than its block table row has entries",
     PLAN_PAGES: "not enough free pages",
-    PLAN_WAIT: "a wait inside attention gave up and rows are missing",
+    PLAN_WAIT: "a wait inside attention gave up and left rows of NaN",
     PLAN_STALE: "its requests or free pages have changed since it was planned, and it was not "
                 "committed",
 }
@@ -256,8 +256,9 @@ class PagePlan(_Buffers):
 
     def check(self) -> None:
         """Wait for the plan (and calls that used it) and raise if the step
-        could not be planned (it then took no pages and has no rows) or its
-        commit came too late."""
+        could not be planned (it then took no pages and has no rows), its
+        commit came too late or attention gave up on rows.  Speaks of the
+        last step planned."""
         bits = int(self.status.item())
         if bits:
             why = "; ".join(text for bit, text in _REASONS.items() if bits & bit)

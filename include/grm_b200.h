@@ -476,14 +476,14 @@ typedef struct grm_b200_paged_plan {
   int64_t scratch_bytes;
 } grm_b200_paged_plan;
 
-/* Status bits of a plan.  A step that cannot be planned takes no page and has
+/* Status bits of a plan's last step (planning clears them).  A step that cannot be planned takes no page and has
  * no rows: lens = cached, starts = 0, rows/positions/slots = -1; append writes
  * nothing and attend returns empty rows. */
 #define GRM_B200_PLAN_BAD_LENGTH 1  /* a negative length, or past 2^31 - 1 tokens */
 #define GRM_B200_PLAN_ROWS 2        /* more new rows than `tokens` or `max_fresh` */
 #define GRM_B200_PLAN_TABLE 4       /* a request needs more than table_width pages */
 #define GRM_B200_PLAN_PAGES 8       /* not enough free pages */
-#define GRM_B200_PLAN_WAIT 16       /* a bounded wait inside attend gave up: rows are missing */
+#define GRM_B200_PLAN_WAIT 16       /* a bounded wait inside attend gave up: its rows are NaN */
 #define GRM_B200_PLAN_STALE 32      /* the tables have changed since: the commit took nothing up */
 
 /* Scratch bytes of a plan of these sizes (the pointers are not read). */
