@@ -402,6 +402,8 @@ class PagedArena(_Buffers):
         """The layer's buffers, for a plan that is good for a call."""
         if not plan.planned:
             raise ValueError("the plan has not been planned yet (PageTables.plan)")
+        if plan._index != self._index:
+            raise ValueError(f"the plan is on {plan.device}, the arena on {self.device}")
         if plan._turn is not None:
             plan._in_turn()
         if not 0 <= layer < self.layers:
