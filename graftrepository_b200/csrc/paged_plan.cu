@@ -35,6 +35,9 @@ constexpr int kBuckets = 256;  // of prompt tiles by what they see
 // A part of a prompt tile has no fewer tokens.  One request of 4,096 tokens, 32
 // pairs, head_dim 256: 24 us in parts of 256, 28 of 512, 42 whole.
 constexpr int kPartTokens = 256;
+// Most tokens of a request, its new rows included: what rounds up to tiles or looks
+// one tile ahead stays below 2^31.
+constexpr int64_t kMaxTokens = ((int64_t)1 << 31) - 1024;
 constexpr int kSizes = 4;
 // The sums over requests: pages taken, rows, pages touched, prompt tiles or their
 // parts (all of them below 2^31 in a step that can be planned) and the split
@@ -153,13 +156,12 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
     if (r >= p.requests) return q;
     q.cached = p.cached[r];
     q.fresh = p.fresh[r];
-    const int64_t after = (int64_t)q.cached + (p.grow ? q.fresh : 0);
-    if (q.cached < 0 || q.fresh < 0 || after > INT32_MAX - page) {
+    if (q.cached < 0 || q.fresh < 0 || (int64_t)q.cached + q.fresh > kMaxTokens) {
       *flags |= GRM_B200_PLAN_BAD_LENGTH;
       return Request{0, 0, 0, 0, 0};
     }
     if (q.fresh > p.max_fresh) *flags |= GRM_B200_PLAN_ROWS;
-    q.after = (int)after;
+    q.after = q.cached + (p.grow ? q.fresh : 0);
     q.have = (q.cached + page - 1) >> p.page_shift;
     q.need = (q.after + page - 1) >> p.page_shift;
     if (q.need > p.width) *flags |= GRM_B200_PLAN_TABLE;

@@ -57,7 +57,7 @@ HEAD_DIMS = (64, 128, 256)
 
 PLAN_BAD_LENGTH, PLAN_ROWS, PLAN_TABLE, PLAN_PAGES, PLAN_WAIT, PLAN_STALE = 1, 2, 4, 8, 16, 32
 _REASONS = {
-    PLAN_BAD_LENGTH: "a negative length, or one past 2^31 - 1",
+    PLAN_BAD_LENGTH: "a negative length, or one past 2^31 - 1024",
     PLAN_ROWS: "more new rows than the plan has room for (tokens, max_fresh)",
     PLAN_TABLE: "a request needs more pages than its block table row has entries",
     PLAN_PAGES: "not enough free pages",

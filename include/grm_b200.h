@@ -480,7 +480,7 @@ typedef struct grm_b200_paged_plan {
  * cannot be planned takes no page and has no rows: lens = cached, starts = 0,
  * rows/positions/slots = -1; append writes nothing and attend returns empty
  * rows. */
-#define GRM_B200_PLAN_BAD_LENGTH 1  /* a negative length, or past 2^31 - 1 tokens */
+#define GRM_B200_PLAN_BAD_LENGTH 1  /* a negative length, or cached + fresh past 2^31 - 1024 */
 #define GRM_B200_PLAN_ROWS 2        /* more new rows than `tokens` or `max_fresh` */
 #define GRM_B200_PLAN_TABLE 4       /* a request needs more than table_width pages */
 #define GRM_B200_PLAN_PAGES 8       /* not enough free pages */

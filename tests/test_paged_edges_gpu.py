@@ -339,3 +339,53 @@ def test_commit_of_many_requests(requests):
         lens += fresh
         assert torch.equal(tables.lens.cpu(), lens)
         assert tables.cursor.tolist() == [int(((lens + 15) // 16).sum()), 3 * requests]
+
+
+# ------------------------------------------------------------- the longest requests
+
+MOST = 2 ** 31 - 1024
+
+
+@pytest.mark.parametrize("grow", [True, False])
+@pytest.mark.parametrize("fresh", [1, 40, 1000])
+def test_lengths_up_to_the_last_that_is_planned(fresh, grow):
+    """Lengths that tiles and pages round up past 31 bits, for single tokens and for
+    prompts; the tokens themselves all lie in one page here."""
+    width = ceil(MOST, 128)
+    tables = PA.PageTables(2, 8, width, page_tokens=128, device=DEV)
+    tables.table.zero_()
+    plan = tables.make_plan(fresh + 5, kv_heads=1, query_heads=4, head_dim=64)
+    for over, bits in ((0, 0), (1, PA.PLAN_BAD_LENGTH), (1023, PA.PLAN_BAD_LENGTH)):
+        tables.lens.copy_(i32([MOST - fresh + over, 3]))
+        tables.plan(plan, i32([fresh, 2]), grow=grow)
+        assert plan.status.item() == bits
+        if not bits:
+            assert plan.lens.tolist() == ([MOST, 5] if grow else [MOST - fresh, 3])
+            assert plan.positions[[0, fresh - 1]].tolist() == [MOST - fresh, MOST - 1]
+            taken = ceil(MOST, 128) - ceil(MOST - fresh, 128)  # pages 0, 1, ... of the ring
+            last = 128 * max(taken - 1, 0) + 127
+            assert plan.slots[fresh - 1].item() == (last if grow else -1)
+    tables.lens.copy_(i32([2 ** 31 - 1, 3]))
+    tables.plan(plan, i32([0, 2]), grow=grow)
+    assert plan.status.item() == PA.PLAN_BAD_LENGTH
+
+
+def test_a_row_over_the_longest_request():
+    """2^31 - 1024 tokens of one page: equal weights, values 1."""
+    tables = PA.PageTables(1, 8, ceil(MOST, 128), page_tokens=128, device=DEV)
+    arena = PA.PagedArena(1, 8, 1, 64, page_tokens=128, device=DEV)
+    arena.k_scales.fill_(1.0)
+    arena.v_scales.fill_(1.0)
+    arena.v_codes.fill_(1)
+    tables.table.zero_()
+    tables.lens.fill_(MOST - 1)
+    plan = tables.make_plan(1, kv_heads=1, query_heads=4, head_dim=64)
+    q = torch.ones((1, 4, 64), dtype=torch.float16, device=DEV)
+    for grow in (True, False):
+        tables.plan(plan, i32([1]), grow=grow)
+        out, lse = arena.attend(plan, q, causal=grow)
+        plan.check()
+        assert bool((out == 1).all())
+        # sums of equal powers of two: one rounding of 2^-24 for each of the joins of a
+        # share's warps, of the shares, and of the logarithm
+        assert bool(((lse.double() - math.log(MOST - 1 + grow)).abs() < 2.0 ** -12).all())
