@@ -393,6 +393,8 @@ class PagedArena(_Buffers):
             raise ValueError(f"{name} is on {x.device}, the arena on {self.device}")
         row, head, inner = x.stride()
         ptr = x.data_ptr()
+        if (row | head) & 7:  # the stride of a dimension of one entry says nothing
+            row, head = row if shape[0] > 1 else 0, head if shape[1] > 1 else 0
         if inner != 1 or (row | head) & 7 or ptr & 15:
             raise ValueError(f"{name}: a head's values must be contiguous, rows and heads at "
                              f"multiples of 8 elements and 16-byte aligned (strides {x.stride()})")

@@ -389,3 +389,30 @@ def test_a_row_over_the_longest_request():
         # sums of equal powers of two: one rounding of 2^-24 for each of the joins of a
         # share's warps, of the shares, and of the logarithm
         assert bool(((lse.double() - math.log(MOST - 1 + grow)).abs() < 2.0 ** -12).all())
+
+
+# ----------------------------------------------------------------------- strides
+
+def test_a_dimension_of_one_entry_may_have_any_stride():
+    """One row cut out of a wide projection, and one head."""
+    tables = PA.PageTables(1, 4, 4, page_tokens=16, device=DEV)
+    for tokens, heads in ((1, 3), (5, 1), (1, 1)):
+        arena = PA.PagedArena(1, 4, heads, 64, page_tokens=16, device=DEV)
+        plan = tables.make_plan(tokens, kv_heads=heads, query_heads=heads, head_dim=64)
+        tables.plan(plan, i32([tokens]))
+        x = torch.randn(4096, device=DEV).to(torch.float16)
+        rows, head = 77 if tokens == 1 else 72, 13 if heads == 1 else 64
+        view = torch.as_strided(x, (tokens, heads, 64), (rows, head, 1))
+        arena.append(plan, view.contiguous(), view.contiguous())
+        want, want_lse = arena.attend(plan, view.contiguous())
+        codes, scales = arena.k_codes.clone(), arena.k_scales.clone()
+        arena.k_codes.zero_()
+        arena.k_scales.zero_()
+        arena.append(plan, view, view)
+        out, lse = arena.attend(plan, view)
+        assert torch.equal(arena.k_codes, codes) and torch.equal(arena.k_scales, scales)
+        assert torch.equal(out, want) and torch.equal(lse, want_lse)
+    with pytest.raises(ValueError, match="multiples of 8"):
+        plan = tables.make_plan(2, kv_heads=1, query_heads=1, head_dim=64)
+        tables.plan(plan, i32([2]))
+        arena.attend(plan, torch.as_strided(x, (2, 1, 64), (77, 13, 1)))
