@@ -416,3 +416,48 @@ def test_a_dimension_of_one_entry_may_have_any_stride():
         plan = tables.make_plan(2, kv_heads=1, query_heads=1, head_dim=64)
         tables.plan(plan, i32([2]))
         arena.attend(plan, torch.as_strided(x, (2, 1, 64), (77, 13, 1)))
+
+
+# ------------------------------------------------------------------ many requests
+
+@pytest.mark.parametrize("requests", [20_000, 70_001, 2 ** 20])
+def test_as_many_requests_as_a_plan_takes(requests):
+    """Two steps of 0 to 3 rows each; a first row sees itself alone."""
+    gen = torch.Generator(device=DEV).manual_seed(requests)
+    tables = PA.PageTables(requests, requests + 5, 1, page_tokens=16, device=DEV)
+    arena = PA.PagedArena(1, requests + 5, 1, 64, page_tokens=16, device=DEV)
+    tables.ring.copy_(torch.randperm(requests + 5, device=DEV, generator=gen).int())
+    plan = tables.make_plan(3 * requests, kv_heads=1, query_heads=2, head_dim=64, max_fresh=3)
+    cached = torch.zeros(requests, dtype=torch.int32, device=DEV)
+    for step in range(2):
+        fresh = torch.randint(0, 4, (requests,), device=DEV, generator=gen, dtype=torch.int32)
+        tables.plan(plan, fresh)
+        plan.check()
+        total = int(fresh.sum())
+        rows = torch.repeat_interleave(torch.arange(requests, device=DEV), fresh.long())
+        starts = torch.zeros(requests + 1, dtype=torch.int64, device=DEV)
+        starts[1:] = fresh.cumsum(0)
+        pos = cached[rows] + torch.arange(total, device=DEV) - starts[rows]
+        assert torch.equal(plan.starts.long(), starts)
+        assert torch.equal(plan.rows[:total].long(), rows)
+        assert torch.equal(plan.positions[:total].long(), pos)
+        assert torch.equal(plan.slots[:total], tables.table[rows, 0].long() * 16 + pos)
+        assert bool((plan.slots[total:] == -1).all())
+        kv = torch.randn((3 * requests, 4, 64), device=DEV, generator=gen).to(torch.float16)
+        arena.append(plan, kv[:, :1], kv[:, 1:2])
+        out, lse = arena.attend(plan, kv[:, 2:])
+        v = arena.read(plan.slots[:total], dtype=torch.float32)[1]
+        alone = pos == 0
+        assert bool(alone.any())
+        # weight 1 exactly, codes exact, one rounding of the scale's factors and one to fp16
+        err = (out[:total][alone] - v[alone]).abs()
+        assert bool((err <= 2.0 ** -10 * v[alone].abs() + 2.0 ** -24).all())
+        assert bool(torch.isfinite(out).all()) and bool(torch.isfinite(lse[:total]).all())
+        tables.commit(plan)
+        cached += fresh
+        assert torch.equal(tables.lens, cached)
+        held = tables.table[cached > 0, 0].long()
+        assert held.unique().numel() == held.numel()
+        assert tables.cursor.tolist() == [held.numel(), requests + 5]
+    tables.release(torch.arange(requests, dtype=torch.int32, device=DEV))
+    assert not tables.lens.any() and tables.ring.unique().numel() == requests + 5
