@@ -98,7 +98,9 @@ constexpr float kLazy = 8.0f;  // how far a row's scores may pass its reference 
 // (fp16 ends at 2^-24) lies below 2^-32 of the row's largest.  Held as they are it
 // would be 2^-25, which the many small weights beside one that takes nearly all of
 // the sum reach (16,384 equal tokens e^-16 below one token: their part 6 % off).
-// Sums are of the weights themselves, results of the lifted ones.
+// Sums are of the weights themselves, results of the lifted ones.  References are
+// whole numbers: less 7 they stay exact, where the rounding of any other one is a
+// factor on a row's whole sum (1e-6 in its logarithm).
 constexpr float kLift = 7.0f;
 constexpr float kUnlift = 0x1p-7f;
 

@@ -461,3 +461,17 @@ def test_as_many_requests_as_a_plan_takes(requests):
         assert tables.cursor.tolist() == [held.numel(), requests + 5]
     tables.release(torch.arange(requests, dtype=torch.int32, device=DEV))
     assert not tables.lens.any() and tables.ring.unique().numel() == requests + 5
+
+
+# ------------------------------------------------------- sums of few, small scores
+
+@pytest.mark.parametrize("dim,heads,group,kind,rows,seed", [
+    (64, 3, 8, torch.float16, 1, 2617), (64, 16, 16, torch.float16, 1, 1),
+    (128, 16, 16, torch.bfloat16, 1, 2), (256, 8, 32, torch.bfloat16, 1, 3),
+    (64, 4, 16, torch.bfloat16, 40, 4), (128, 4, 4, torch.float16, 40, 5),
+    (256, 4, 16, torch.float16, 40, 6)])
+def test_the_sum_where_scores_are_small_and_scales_far_apart(dim, heads, group, kind, rows, seed):
+    """There the log-sum-exp has little but its own roundings to be off by."""
+    n = 1 if seed == 2617 else 200 // rows
+    run_attention([rows] * n, [rows] * n, heads=heads, group=group, dim=dim, page=16, kind=kind,
+                  causal=False, grow=False, seed=seed, spread=2.0, max_fresh=501)
