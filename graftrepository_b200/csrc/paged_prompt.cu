@@ -503,9 +503,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       const int j = x >> 1, side = x & 1, st = j & 1, place = j % kRaws;
       const unsigned char* src = sm_raw + (place * 2 + side) * LY::kRaw + row0 * D + c * 16;
       unsigned char* at = (side ? sm_v : sm_k) + st * LY::kTile + (c / 4) * LY::kAtom;
-      // (with no probes at all the block gives up here: a look at the limit in every
-      // wait costs 2 % of the kernel's time)
-      if (!(ok = p.probes > 0 && wait(&raw_full[side][place], (j / kRaws) & 1))) break;
+      if (!(ok = wait(&raw_full[side][place], (j / kRaws) & 1))) break;
       uint4 r[4];
       auto load = [&] {
 #pragma unroll
@@ -636,7 +634,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       };
       int page = page_of(0);
       int issued[2] = {0, 0};
-      bool ok = true;
+      // With no probes at all the block gives up here: nothing comes, and everybody's
+      // waits run out.  (A look at the limit in every wait costs 2 % of the kernel.)
+      bool ok = p.probes > 0;
       for (int j = 0; j < tiles && ok; ++j) {
         const int64_t at = (int64_t)page * p.kv_heads + h;
         const int t0 = tok_base + j * kN + group16 * 16;

@@ -1,8 +1,8 @@
 """The path of attention over the 8-bit paged arena on which a bounded wait gives up.
 
-A child process with GRM_B200_WAIT_LIMIT=0 has every wait give up before its first
-probe, so no wait hangs and every copy that was issued ends as ever (the drain at the
-end of a block has a limit of its own).  The step's status says so, its rows are NaN
+A child process with GRM_B200_WAIT_LIMIT=0 has waits give up before their first probe,
+or after one where another warp has given up, so no wait hangs and every copy that was
+issued ends as ever (the drain at the end of a block has a limit of its own).  The step's status says so, its rows are NaN
 rather than what the memory held, parts of a prompt tile that others join included,
 rows that wait for nothing are what they always are, and the context stays usable."""
 
