@@ -116,9 +116,9 @@ class _Buffers:
     def _made(self, *tensors) -> None:
         self._tensors = tensors
         stream = torch.cuda.current_stream(self.device)
-        self._streams = {stream.cuda_stream}  # handles
-        self._event = None
+        self._streams, self._event = set(), None  # handles
         if not _capturing(stream):
+            self._streams.add(stream.cuda_stream)
             self._event = torch.cuda.Event()
             self._event.record(stream)
 
@@ -237,6 +237,7 @@ class PagePlan(_Buffers):
               ctypes.byref(need))
         self.scratch = torch.empty(need.value, dtype=torch.uint8, device=self.device)
         self._made(words, longs, self.scratch)
+        _handle(None, self._index, (tables,))
         c = self.c
         c.cached, c.cursor_in = tables.lens.data_ptr(), tables.cursor.data_ptr()
         c.ring, c.table = tables.ring.data_ptr(), tables.table.data_ptr()
@@ -248,6 +249,11 @@ class PagePlan(_Buffers):
         self.planned, self.grow = False, True
         self._turn = None  # of the tables' joining steps, until it is committed
         self._ref = ctypes.byref(c)
+
+    def _join(self, stream) -> None:  # and the tables, for every call that takes a plan
+        super()._join(stream)
+        if stream.cuda_stream not in self.tables._streams:
+            self.tables._join(stream)
 
     def _in_turn(self) -> None:
         if self._turn is not None and self._turn != self.tables._turn:
@@ -310,7 +316,7 @@ class PageTables(_Buffers):
             plan.grow = bool(grow)
             plan.c.grow = 1 if grow else 0
         _call(self._plan_step, self._index, plan._ref, fresh.data_ptr(),
-              _handle(stream, self._index, (plan, self), fresh))
+              _handle(stream, self._index, (plan,), fresh))
         plan.planned, plan._turn = True, None
         # a step that a graph plans again has no turn: the host does not see it
         if grow and not (torch.cuda.is_current_stream_capturing() if stream is None else
@@ -331,7 +337,7 @@ class PageTables(_Buffers):
             return
         plan._in_turn()
         _call(_lib.load().grm_b200_paged_commit, self._index, plan._ref, self.lens.data_ptr(),
-              self.cursor.data_ptr(), _handle(stream, self._index, (plan, self)))
+              self.cursor.data_ptr(), _handle(stream, self._index, (plan,)))
         plan._turn = None
 
     def release(self, rows, *, stream=None) -> None:
@@ -432,7 +438,7 @@ class PagedArena(_Buffers):
         if not plan.grow:
             raise ValueError("the plan's rows do not join the arena (planned with grow=False)")
         _call(self._append, self._index, plan._ref, ref, k_ptr, v_ptr, kind, k_row, k_head, v_row,
-              v_head, _handle(stream, self._index, (self, plan, plan.tables), k, v))
+              v_head, _handle(stream, self._index, (self, plan), k, v))
 
     def attend(self, plan: PagePlan, q, *, layer: int = 0, causal: bool = True,
                scale: float | None = None, out=None, lse=None, stream=None):
@@ -450,7 +456,7 @@ class PagedArena(_Buffers):
         lse = self._result("lse", lse, plan._lse_like, stream)
         _call(self._attend, self._index, plan._ref, ref, ptr, kind, row, head,
               self._scale if scale is None else float(scale), 1 if causal else 0, out.data_ptr(),
-              lse.data_ptr(), _handle(stream, self._index, (self, plan, plan.tables), q, out, lse))
+              lse.data_ptr(), _handle(stream, self._index, (self, plan), q, out, lse))
         return out, lse
 
     def read(self, slots, *, layer: int = 0, dtype=None, stream=None):

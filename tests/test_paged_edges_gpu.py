@@ -152,6 +152,32 @@ def test_a_stream_waits_for_the_one_that_buffers_were_made_on(inputs, explicit):
         assert torch.equal(a, b)
 
 
+def test_a_plan_made_on_another_stream_than_its_tables(inputs):
+    want, _ = small_step(None)
+    want = [t.clone() for t in want[:3]]
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    torch.cuda._sleep(SLEEP)
+    tables = PA.PageTables(3, 40, 20, page_tokens=16, device=DEV)
+    arena = PA.PagedArena(1, 40, 2, 64, page_tokens=16, device=DEV)
+    with torch.cuda.stream(side):
+        plan = tables.make_plan(120, kv_heads=2, query_heads=4, head_dim=64)
+        tables.plan(plan, FRESH)
+        arena.append(plan, KV[:, 0], KV[:, 1])
+        out, lse = arena.attend(plan, Q)
+        got = [t.clone() for t in (plan.slots, out, lse)]
+    places = {tables.table.data_ptr(), arena.k_codes.data_ptr()}
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(SLEEP)
+        arena.attend(plan, Q, out=out, lse=lse)
+    del tables, arena, plan
+    new = [torch.empty(n, dtype=torch.uint8, device=DEV) for n in (240, 240, 81920, 81920)]
+    assert not places & {t.data_ptr() for t in new}
+    torch.cuda.synchronize()
+    for a, b in zip(got + [out, lse], want + want[1:]):
+        assert torch.equal(a, b)
+
+
 @pytest.mark.parametrize("explicit", [True, False])
 def test_a_dropped_plan_keeps_its_memory_until_its_step_has_run(inputs, explicit):
     (_, want, want_lse, *_), held = small_step(None)
