@@ -98,11 +98,17 @@ constexpr float kLazy = 8.0f;  // how far a row's scores may pass its reference 
 // (fp16 ends at 2^-24) lies below 2^-32 of the row's largest.  Held as they are it
 // would be 2^-25, which the many small weights beside one that takes nearly all of
 // the sum reach (16,384 equal tokens e^-16 below one token: their part 6 % off).
-// Sums are of the weights themselves, results of the lifted ones.  References are
-// whole numbers: less 7 they stay exact, where the rounding of any other one is a
-// factor on a row's whole sum (1e-6 in its logarithm).
+// Sums are of the weights themselves, results of the lifted ones.
 constexpr float kLift = 7.0f;
 constexpr float kUnlift = 0x1p-7f;
+// The reference exponent for a largest score `top`: a multiple of 2^-14 (below 256).
+// Less 7 it stays exact, where the rounding of any other one would be a factor on the
+// row's whole sum (1e-6 in its logarithm), and the largest weight is a power of two
+// but for 2^-15, so that fp16 does not round the one that counts most (a whole number
+// is as exact, but one row over 250,007 tokens is then off by 2.7e-4 in fp16, not 2.3).
+__device__ __forceinline__ float reference_of(float top) {
+  return __fadd_rn(__fadd_rn(top, 768.0f), -768.0f);
+}
 
 // Probes of a bounded wait.  A wait that gives up leaves NaN in its rows and
 // GRM_B200_PLAN_WAIT in the plan's status; copies and products in flight are waited

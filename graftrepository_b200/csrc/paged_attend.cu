@@ -9,9 +9,8 @@
 //   y_t = z_t * log2(e) + log2(u_t),  p_t = 2^(y_t - m),
 // p_t u-weighted is what multiplies b_t, and the sum of weights is
 // sum_t p_t / u_t, so p_t never exceeds 2^8 whatever the scales are (m trails the
-// largest y seen by at most 8: it moves only when a y passes m + 8, to the whole
-// number below it, so the accumulators are rarely rescaled and y - m has no rounding
-// that all of a row shares), and fp16 holds 2^7 p_t.  The log-sum-exp is
+// largest y seen by at most 8: it moves only when a y passes m + 8, so the
+// accumulators are rarely rescaled), and fp16 holds 2^7 p_t.  The log-sum-exp is
 // m ln 2 + log of that sum.
 //
 // The split kernel serves few query rows a kv head (decoding, a few proposed
@@ -671,7 +670,7 @@ __global__ void __launch_bounds__(kThreads, (Layout<D, NT>::kBlocks))
 #pragma unroll
             for (int i = 4; i <= 16; i <<= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, i));
             // each row by its own scores, so that no row's rounding hangs on another's
-            top = top > m[nt][x] + kLazy ? floorf(top) : m[nt][x];
+            top = top > m[nt][x] + kLazy ? reference_of(top) : m[nt][x];
             const float a = top == m[nt][x] ? 1.0f : ex2(m[nt][x] - top);
             m[nt][x] = top;
             l[nt][x] *= a;

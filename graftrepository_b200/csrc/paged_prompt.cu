@@ -373,7 +373,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           top = fmaxf(top, fmaf(y, fk[g], fo[g]));
         }
         if (__any_sync(kFull, top > m + kLazy)) {
-          const float next = top > m + kLazy ? floorf(top) : m;
+          const float next = top > m + kLazy ? reference_of(top) : m;
           const float a = next == m ? 1.0f : ex2(m - next);
           m = next;
           l *= a;

@@ -501,3 +501,30 @@ def test_the_sum_where_scores_are_small_and_scales_far_apart(dim, heads, group, 
     n = 1 if seed == 2617 else 200 // rows
     run_attention([rows] * n, [rows] * n, heads=heads, group=group, dim=dim, page=16, kind=kind,
                   causal=False, grow=False, seed=seed, spread=2.0, max_fresh=501)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("requests,heads,group", [(6000, 16, 1), (1500, 16, 48)])
+def test_one_token_has_a_sum_of_one_and_its_weight_is_not_rounded(requests, heads, group, dim):
+    """Whatever the scale of its values: a query of zeros over one token, for which the
+    kernels take the logarithm of that scale, powers of it and a logarithm again.  Two
+    powers are off by 2^-22 each, the last logarithm by a unit in the last place of a
+    number below 16.  The result is rounded to fp16, 2^-11; its weight lies within 2^-15
+    of a power of two (in the exponent), and fp16 makes it that; the scale's logarithm,
+    two units off, and the power are 2^-19 each."""
+    gen = torch.Generator(device=DEV).manual_seed(dim + group)
+    tables = PA.PageTables(requests, requests, 1, page_tokens=16, device=DEV)
+    arena = PA.PagedArena(1, requests, heads, dim, page_tokens=16, device=DEV)
+    arena.v_scales.copy_(torch.exp2(22 * torch.rand(arena.v_scales.shape, device=DEV,
+                                                    generator=gen) - 14.9))
+    arena.v_codes.fill_(127)
+    plan = tables.make_plan(requests, kv_heads=heads, query_heads=heads * group, head_dim=dim,
+                            max_fresh=1)
+    tables.plan(plan, i32([1] * requests))
+    plan.check()
+    q = torch.zeros((requests, heads * group, dim), dtype=torch.float16, device=DEV)
+    out, lse = arena.attend(plan, q)
+    assert float(lse.abs().max()) <= 2 * 2.0 ** -22 + math.log(2) * 2.0 ** -20
+    want = 127 * arena.v_scales[0][tables.table[:, 0].long()].repeat_interleave(group, 1).double()
+    err = (out.double() / want[:, :, None] - 1).abs().amax()
+    assert float(err) <= 2.0 ** -11 + math.log(2) * 2.0 ** -15 + 2 * 2.0 ** -19
