@@ -33,8 +33,8 @@
 // smaller than the largest round.
 //
 // 64 requests of 200 to 16,384 tokens, one row x 4 each on 8 kv heads of head_dim
-// 128 (515 MB of codes), take 97 us, 5.3 TB/s; one request of 250,007 tokens 98
-// us.  In its stride the kernel reads 7.5 TB/s (1.94 us a tile and block); the
+// 128 (515 MB of codes), take 97 us, 5.3 TB/s (head_dim 64 67 us, 256 190); one
+// request of 250,007 tokens 100 us.  In its stride the kernel reads 7.5 TB/s (1.94 us a tile and block); the
 // rest is the start (first data after 4.3 us of dependent loads) and the spread
 // of the blocks, which end between 61 and 90 us for equal shares.  Measured and
 // dropped: a last sixth of the tiles handed out in small shares as blocks finish

@@ -33,15 +33,22 @@ namespace {
 
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanWarps = kPlanThreads / 32;
+// Segments of no more units are left whole.  us with 3, 5 and 8: one request of 333
+// tokens 12.1, 10.0, 10.1; 8 of 300 tokens 13.6, 11.1, 11.2; 24 of 200 to 2,000 at
+// head_dim 128 21.7, 21.8, 25.6; 24 of up to 3,000 at head_dim 64 18.5, 18.4, 19.9; 16
+// of 100 to 1,000 at head_dim 256 16.2, 16.0, 24.1.
 constexpr int kJoinUnits = 5;
 constexpr int kBuckets = 256;  // of prompt tiles by what they see
-// A part of a prompt tile has no fewer tokens.  One request of 4,096 tokens, 32
-// pairs, head_dim 256: 24 us in parts of 256, 28 of 512, 42 whole.
+// A part of a prompt tile has no fewer tokens.  us with 128, 256, 512 and 1,024: one
+// request of 4,096 tokens, 32 pairs, head_dim 256 25.7, 24.3, 26.0, 32.4; of 1,024
+// tokens, 160 pairs, head_dim 128 23.8, 23.6, 25.7, 31.7; 4 of 700 tokens at head_dim
+// 64 17.6, 17.7, 19.5, 21.7; 2 of 2,000 tokens, 400 pairs 40.0, 40.0, 40.0, 45.1; one of
+// 16,000 on 4 kv heads 39.9, 40.0, 38.1, 41.7.
 constexpr int kPartTokens = 256;
 // Most tokens of a request, its new rows included: what rounds up to tiles or looks
 // one tile ahead stays below 2^31.
 constexpr int64_t kMaxTokens = ((int64_t)1 << 31) - 1024;
-constexpr int kSizes = 4;
+constexpr int kSizes = 4;  // candidate part sizes, see plan_kernel
 // The sums over requests: pages taken, rows, pages touched, prompt tiles or their
 // parts (all of them below 2^31 in a step that can be planned) and the split
 // kernel's units; and two that only totals are needed of, the split kernel's
@@ -215,7 +222,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
   // tokens that a part can have are between Sum len / SMs and Sum len / (SMs - tiles),
   // which is always enough (Sum ceil(len / part) <= Sum len / part + tiles): of four
   // sizes in between, the smallest whose parts the SMs can hold (16 requests of 100 to
-  // 8,192 tokens with 5 rows of head_dim 256: 44 us with the last one always).
+  // 8,192 tokens with 5 rows of head_dim 256: 40 us, 44 with the last one always).
   int part_tokens = 0;
   const int64_t whole = total[kTiles] * p.kv_heads;
   if (whole > 0 && whole <= p.sms / 2) {
@@ -520,10 +527,20 @@ int make_shape(const grm_b200_paged_plan& p, int sms, Shape* s) {
   s->block_rows = most <= 8 ? 8 : 16;
   // (row, head) pairs a kv head up to which the split kernel serves a request, in
   // segments of 16 rows that read the codes again; a prompt tile costs the same for
-  // 1 row and 128.  Split / prompt, us, 16 requests of 4,096 tokens on 8 kv heads:
-  // head_dim 64, 32 pairs 50 / 60, 64 pairs 81 / 61; head_dim 128, 32 pairs 72 / 69 (64
-  // requests of 2,048 tokens: 132 / 141), 64 pairs 121 / 69; head_dim 256, 16 pairs
-  // 81 / 87, 24 pairs 126 / 87.
+  // 1 row and 128.  Split / prompt, us, at 16, 32 and 64 pairs, pages of 64:
+  //   head_dim  kv heads  requests x tokens   16 pairs   32 pairs   64 pairs
+  //      64        8          16 x 4,096       34 / 58    48 / 59    79 / 59
+  //      64        8          64 x 2,048       54 / 121   89 / 121  152 / 121
+  //     128        8          16 x 4,096       49 / 66    72 / 66   121 / 67
+  //     128        8          64 x 2,048       80 / 136  133 / 138  234 / 140
+  //     256        8          16 x 4,096       81 / 82   128 / 83   227 / 85
+  //     256        8          64 x 2,048      135 / 172  239 / 177  442 / 180
+  //     128        2          16 x 4,096       30 / 32    35 / 32    45 / 34
+  //     256        2          16 x 4,096       46 / 36    53 / 39    76 / 44
+  //     256        8          16 x 1,024       41 / 30    55 / 31    83 / 32
+  // So the rule holds where there is work for all SMs.  Where there is not, the prompt
+  // kernel is ahead from fewer pairs on, at head_dim 256 by a third at 16; the rule
+  // does not look at that.
   s->prompt_rows = p.head_dim == 256 ? 16 : 32;
   const bool prompts = most > s->prompt_rows;
   s->qtile_tokens = (p.head_dim == 256 ? 1 : 2) * (128 / s->group);

@@ -38,12 +38,15 @@
 // each; the split kernel, which runs after this one, joins them.
 //
 // 8,449 rows of 3 requests (1.4 TFLOP at 8 kv heads, 32 query heads, head_dim 128)
-// take 1.27 ms, 1.12 PFLOP/s.  What bounds it now is the softmax warps' chain of
-// dependent steps: per 64 tokens about 1,900 clocks, where the exponentials alone
-// need 1,024 (both warps of a scheduler), the tensor cores as many, and shared
-// memory 1,536.  On the way: both warps of a scheduler in the same phase 1.51 ms,
-// in turns 1.43; then, where each product had had a predicate of its own (80
-// clocks of issue apiece), an elected branch 1.33; arithmetic two at a time 1.27.
+// take 1.27 ms alone, 1.12 PFLOP/s, and 1.39 to 1.44 in a row of calls, where the
+// power cap lowers the clocks; at head_dim 64 1.13 ms (exponentials 0.60, products
+// 0.42 at the units' rates), at head_dim 256 2.6 to 2.9 ms (products 1.66).  What
+// bounds it now is the softmax warps' chain of dependent steps: per 64 tokens about
+// 1,900 clocks, where the exponentials alone need 1,024 (both warps of a scheduler),
+// the tensor cores as many, and shared memory 1,536.  On the way: both warps of a
+// scheduler in the same phase 1.51 ms, in turns 1.43; then, where each product had
+// had a predicate of its own (80 clocks of issue apiece), an elected branch 1.33;
+// arithmetic two at a time 1.27.
 #include <type_traits>
 
 #include "paged.cuh"

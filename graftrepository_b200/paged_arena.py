@@ -429,7 +429,7 @@ class PagedArena(_Buffers):
 
     def append(self, plan: PagePlan, k, v, *, layer: int = 0, stream=None) -> None:
         """Quantise the step's rows ``k`` and ``v`` [tokens, kv_heads, head_dim]
-        into the pages of `layer`."""
+        into the pages of `layer`, before those of any later step."""
         ref = self._ready(plan, layer)
         kind, k_ptr, k_row, k_head = self._rows("k", k, plan.kv_shape)
         v_kind, v_ptr, v_row, v_head = self._rows("v", v, plan.kv_shape)
@@ -444,9 +444,9 @@ class PagedArena(_Buffers):
                scale: float | None = None, out=None, lse=None, stream=None):
         """Attention of the step's query rows ``q`` [tokens, query_heads,
         head_dim]: over everything the row's request holds, or with `causal` over
-        the positions up to the row's own.  `scale` defaults to
-        head_dim ** -0.5.  Returns (out like q, lse fp32 [tokens, query_heads]);
-        rows that see nothing are 0 with lse -inf."""
+        the positions up to the row's own.  `scale` (positive; default
+        head_dim ** -0.5) multiplies the scores.  Returns (out like q, lse fp32
+        [tokens, query_heads]); rows that see nothing are 0 with lse -inf."""
         ref = self._ready(plan, layer)
         kind, ptr, row, head = self._rows("q", q, plan.query_shape)
         if causal and not plan.grow:

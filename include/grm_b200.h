@@ -432,10 +432,10 @@ typedef struct grm_b200_paged_arena {
 } grm_b200_paged_arena;
 
 /* One step of `requests` requests (at most 2^20; the plan's work grows with their
- * square, 18 us for 16,384 of one row and 18 ms for 2^20).  Sizes first: `tokens` is the capacity of
- * the step's packed rows (request 0's new rows, request 1's, ...), max_fresh
- * the most new rows one request may have, table_width the entries of a block
- * table row, pages the size of the ring of free pages.
+ * square, 18 us for 16,384 of one row and 18 ms for 2^20).  Sizes first: `tokens`
+ * is the capacity of the step's packed rows (request 0's new rows, request 1's,
+ * ...), max_fresh the most new rows one request may have, table_width the
+ * entries of a block table row, pages the size of the ring of free pages.
  * In (device): cached[requests], the tokens each request holds; ring[pages],
  * page numbers of which entries cursor_in[0] .. cursor_in[1]-1 (modulo pages)
  * are free: cursor_in = {pages ever taken, pages ever returned}.
@@ -525,10 +525,11 @@ int grm_b200_paged_release(const int32_t* rows_device, int64_t count, int64_t re
  * pointers; the head_dim values of a row are contiguous).  The scale of a page
  * becomes max(scale of the older tokens it holds, max |x| / 127); when it
  * grows, the older codes are rescaled, code' = rint(code * old / new).  New
- * codes are rint(x / scale), ties to even, every step in fp32.  A page that
+ * codes are rint(x / scale), ties to even, every step in fp32 with IEEE division.  A page that
  * takes a NaN or an infinity gets scale NaN, so what it holds reads as NaN
  * until the page starts anew.  Writing the same step twice writes the same
- * codes.  The plan must have been made with grow != 0. */
+ * codes.  A layer's steps are appended in the order in which they were planned.
+ * The plan must have been made with grow != 0. */
 int grm_b200_paged_append(const grm_b200_paged_plan* plan, const grm_b200_paged_arena* arena,
                           const void* k_device, const void* v_device, int dtype,
                           int64_t k_row_stride, int64_t k_head_stride, int64_t v_row_stride,
@@ -546,6 +547,7 @@ int grm_b200_paged_read(const grm_b200_paged_arena* arena, const int64_t* slots_
  * (GRM_B200_F16 or GRM_B200_BF16; strides and alignment as append's) over the
  * arena: query head j reads kv head j / (query_heads / kv_heads);
  *   out[i, j] = sum_t w_t v_t,  w = softmax_t(softmax_scale * q_ij . k_t),
+ * (softmax_scale positive and finite)
  * over the request's lens[r] tokens, or with causal != 0 over the positions up
  * to the row's own.  out [tokens, query_heads, head_dim] has q's type; lse
  * [tokens, query_heads] fp32 (may be NULL) is the natural logarithm of the sum
