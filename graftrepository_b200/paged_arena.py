@@ -117,6 +117,7 @@ class _Buffers:
         self._tensors = tensors
         stream = torch.cuda.current_stream(self.device)
         self._streams, self._event = set(), None  # handles
+        self._last = stream.cuda_stream  # of the call before
         if not _capturing(stream):
             self._streams.add(stream.cuda_stream)
             self._event = torch.cuda.Event()
@@ -151,6 +152,7 @@ def _handle(stream, index, owners, *tensors) -> int:
     for x in owners:
         if handle not in x._streams:
             x._join(torch.cuda.current_stream(index) if stream is None else stream)
+        x._last = handle
     return handle
 
 
@@ -261,10 +263,12 @@ class PagePlan(_Buffers):
                              "same pages; plan this one again")
 
     def check(self) -> None:
-        """Wait for the plan (and calls that used it) and raise if the step
-        could not be planned (it then took no pages and has no rows), its
-        commit came too late or attention gave up on rows.  Speaks of the
-        last step planned."""
+        """Wait for the plan (and calls that used it, on the stream of the last
+        one and on the current one) and raise if the step could not be planned
+        (it then took no pages and has no rows), its commit came too late or
+        attention gave up on rows.  Speaks of the last step planned."""
+        if self._last != _raw_stream(self._index):
+            _torch_stream(self._last, self._index).synchronize()
         bits = int(self.status.item())
         if bits:
             why = "; ".join(text for bit, text in _REASONS.items() if bits & bit)

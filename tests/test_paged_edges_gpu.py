@@ -213,6 +213,40 @@ def test_a_dropped_plan_keeps_its_memory_until_its_step_has_run(inputs, explicit
     assert torch.equal(result[0], want) and torch.equal(result[1], want_lse)
 
 
+@pytest.mark.parametrize("explicit", [True, False])
+def test_check_waits_for_the_stream_of_the_step(inputs, explicit):
+    tables = PA.PageTables(3, 4, 20, page_tokens=16, device=DEV)
+    plan = tables.make_plan(120, kv_heads=2, query_heads=4, head_dim=64)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(SLEEP)
+        if not explicit:
+            tables.plan(plan, FRESH)  # 8 pages of 4
+    if explicit:
+        tables.plan(plan, FRESH, stream=side.cuda_stream)
+    with pytest.raises(_lib.GrmB200Error, match="not enough free pages"):
+        plan.check()
+    tables.plan(plan, i32([1, 0, 0]))
+    plan.check()
+    torch.cuda._sleep(SLEEP)
+    tables.plan(plan, FRESH)  # and the other way round
+    with torch.cuda.stream(side), pytest.raises(_lib.GrmB200Error, match="free pages"):
+        plan.check()
+
+
+def test_check_after_the_replay_of_a_graph(inputs):
+    tables = PA.PageTables(3, 4, 20, page_tokens=16, device=DEV)
+    plan = tables.make_plan(120, kv_heads=2, query_heads=4, head_dim=64)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        tables.plan(plan, FRESH)
+    torch.cuda._sleep(SLEEP)
+    graph.replay()
+    with pytest.raises(_lib.GrmB200Error, match="not enough free pages"):
+        plan.check()
+
+
 def test_a_graph_of_a_step_whose_plan_no_stream_has_used(inputs):
     """Captured at once, without a step before on the capturing stream."""
     want, _ = small_step(None)
