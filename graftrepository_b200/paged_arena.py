@@ -101,9 +101,11 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
 
 def _torch_stream(stream, index):
     """`stream` (a torch stream or a raw handle) as a torch stream."""
-    if not hasattr(stream, "cuda_stream"):
-        stream = torch.cuda.ExternalStream(int(stream), device=torch.device("cuda", index))
-    return stream
+    if hasattr(stream, "cuda_stream"):
+        return stream
+    if int(stream) == 0:  # torch takes an external stream 0 for a new one
+        return torch.cuda.default_stream(index)
+    return torch.cuda.ExternalStream(int(stream), device=torch.device("cuda", index))
 
 
 class _Buffers:

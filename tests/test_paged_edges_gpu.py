@@ -235,6 +235,36 @@ def test_check_waits_for_the_stream_of_the_step(inputs, explicit):
         plan.check()
 
 
+@pytest.mark.parametrize("handle", [0, None])
+def test_a_raw_handle_is_that_stream(inputs, handle):
+    """0 is the default stream: what was queued there before comes first."""
+    side = torch.cuda.Stream()
+    stream = torch.cuda.default_stream() if handle == 0 else side
+    tables = PA.PageTables(3, 40, 20, page_tokens=16, device=DEV)
+    arena = PA.PagedArena(1, 40, 2, 64, page_tokens=16, device=DEV)
+    plan = tables.make_plan(120, kv_heads=2, query_heads=4, head_dim=64)
+    fresh = i32([1, 2, 3])
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        torch.cuda._sleep(SLEEP)
+        fresh.copy_(FRESH)
+    with torch.cuda.stream(side if handle == 0 else torch.cuda.default_stream()):
+        raw = stream.cuda_stream
+        assert (raw == 0) == (handle == 0)
+        tables.plan(plan, fresh, stream=raw)
+        arena.append(plan, KV[:, 0], KV[:, 1], stream=raw)
+        out, lse = arena.attend(plan, Q, stream=raw)
+        k, v = arena.read(plan.slots, stream=raw)
+        tables.commit(plan, stream=raw)
+        tables.release(FRESH[1:2], stream=raw)  # request 1
+        plan.check()
+    torch.cuda.synchronize()
+    (_, want, want_lse, want_k, want_v, *_), _ = small_step(None)
+    for a, b in zip((out, lse, k, v), (want, want_lse, want_k, want_v)):
+        assert torch.equal(a, b)
+    assert tables.lens.tolist() == [70, 0, 40]
+
+
 def test_check_after_the_replay_of_a_graph(inputs):
     tables = PA.PageTables(3, 4, 20, page_tokens=16, device=DEV)
     plan = tables.make_plan(120, kv_heads=2, query_heads=4, head_dim=64)
