@@ -91,6 +91,16 @@ _SIGS = {
     "grm_b200_paged_append": (_I, [_P, _P, _P, _P, _I, _I64, _I64, _I64, _I64, _P]),
     "grm_b200_paged_read": (_I, [_P, _P, _I64, _I, _P, _P, _P]),
     "grm_b200_paged_attend": (_I, [_P, _P, _P, _I, _I64, _I64, ctypes.c_float, _I, _P, _P, _P]),
+    "grm_b200_rotate": (_I, [_P, _P, _I, _I64, _I64, _I64, _I64, _I64, _P, _I, _P, _I64, _I64,
+                             _P]),
+    "grm_b200_paged_append_rotary": (_I, [_P, _P, _P, _P, _P, _I, _I64, _I64, _I64, _I64, _P]),
+    "grm_b200_latent_work_bytes": (_I, [_P, _P]),
+    "grm_b200_latent_plan_step": (_I, [_P, _P, _P]),
+    "grm_b200_latent_append": (_I, [_P, _P, _P, _P, _I64, _P, _I64, _P]),
+    "grm_b200_latent_attend": (_I, [_P, _P, _P, _I64, _I64, _P, _I64, _I64, ctypes.c_float, _I,
+                                    _P, _P, _P]),
+    "grm_b200_latent_attend_expanded": (_I, [_P, _P, _P, _I64, _I64, _P, _I64, _I64,
+                                             ctypes.c_float, _I, _P, _P, _P]),
     "grm_b200_merge_topk": (_I, [_P, _P, _I, _I, _I, _I, _P, _P, _P]),
     "grm_b200_merge_topk_strided": (_I, [_P, ctypes.c_int64, _P, ctypes.c_int64, _I, _I, _I, _I,
                                          _P, _P, _P]),

@@ -1,0 +1,415 @@
+// latent.cu -- pages of latent rows: step plans, append, and the entry points of
+// attention (latent_attend.cu).
+#include <algorithm>
+
+#include "latent.cuh"
+#include "rotary.cuh"
+
+namespace grm_b200 {
+namespace latent {
+
+namespace {
+
+using paged::check_plan;
+using paged::launch_status;
+
+constexpr int kScheduleThreads = 1024;
+
+struct ScheduleParams {
+  Work w;
+  const int32_t* lens;
+  const int32_t* starts;
+  int32_t* status;
+  int64_t requests, expand_tokens;
+};
+
+// One block: the requests in chunks, prefix sums of what they add.
+__global__ void __launch_bounds__(kScheduleThreads) schedule_kernel(const ScheduleParams p) {
+  __shared__ int64_t part[32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  int64_t expand = 0;  // before the chunk
+  for (int64_t r0 = 0; r0 < p.requests; r0 += kScheduleThreads) {
+    const int64_t r = r0 + tid;
+    int64_t n = 0;
+    if (r < p.requests && p.starts[r + 1] > p.starts[r])
+      n = ((int64_t)p.lens[r] + kExpandAlign - 1) / kExpandAlign * kExpandAlign;
+    int64_t incl = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t up = __shfl_up_sync(kFull, incl, o);
+      if (lane >= o) incl += up;
+    }
+    __syncthreads();
+    if (lane == 31) part[warp] = incl;
+    __syncthreads();
+    int64_t before = expand;
+    for (int w = 0; w < warp; ++w) before += part[w];
+    for (int w = 0; w < 32; ++w) expand += part[w];
+    if (r < p.requests)
+      p.w.base[r] = (int)min(before + incl - n, (int64_t)INT32_MAX);
+  }
+  if (tid == 0) {
+    const bool over = p.expand_tokens > 0 && expand > p.expand_tokens;
+    p.w.base[p.requests] = (int)min(expand, (int64_t)INT32_MAX);
+    *p.w.header = Header{p.starts[p.requests], over};
+    if (over) atomicOr(p.status, GRM_B200_PLAN_EXPAND);
+  }
+}
+
+struct AppendParams {
+  RotaryParams r;
+  const int64_t* slots;
+  const int32_t* positions;
+  int64_t tokens, limit;  // limit: pages * page_tokens
+  const uint16_t* latent_rows;
+  const uint16_t* rope_rows;
+  int64_t latent_stride, rope_stride;
+  uint16_t* cache;
+  int latent, rope, rotary;
+};
+
+// A thread for 8 values of a row, or for 8 pairs of its positional part.  Bound by
+// HBM where rows are many, else a launch and three dependent loads.
+template <typename T, bool IN, bool OUT>
+__global__ void __launch_bounds__(256) append_kernel(const AppendParams p) {
+  const int copies = p.latent / 8, entries = copies + (p.rotary ? p.rope / 16 : p.rope / 8);
+  const int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t t = x / entries;
+  if (t >= p.tokens) return;
+  const int e = (int)(x - t * entries);
+  const int64_t slot = p.slots[t];
+  if (slot < 0 || slot >= p.limit) return;
+  uint16_t* to = p.cache + slot * (p.latent + p.rope);
+  if (e < copies) {
+    reinterpret_cast<uint4*>(to)[e] = ld_nc16(p.latent_rows + t * p.latent_stride + e * 8);
+    return;
+  }
+  const uint16_t* from = p.rope_rows + t * p.rope_stride;
+  to += p.latent;
+  const int c = (e - copies) * 8;
+  if (!p.rotary) {
+    *reinterpret_cast<uint4*>(to + c) = ld_nc16(from + c);
+    return;
+  }
+  const int position = p.positions[t];
+  float2 angle[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const Turn a = turn_of(position, p.r.turns[c + i]);
+    angle[i] = make_float2(a.cos * p.r.amplitude, a.sin * p.r.amplitude);
+  }
+  turn_pairs<T, 8, IN, OUT>(p.rope / 2, angle, c, reinterpret_cast<const T*>(from),
+                            reinterpret_cast<T*>(to));
+}
+
+template <typename T>
+int launch_append(const AppendParams& p, cudaStream_t st) {
+  const int entries = p.latent / 8 + (p.rotary ? p.rope / 16 : p.rope / 8);
+  const unsigned blocks = (unsigned)ceil_div64(p.tokens * entries, 256);
+  if (!p.rotary || p.r.layout == GRM_B200_ROTARY_HALF)
+    append_kernel<T, false, false><<<blocks, 256, 0, st>>>(p);
+  else if (p.r.layout == GRM_B200_ROTARY_INTERLEAVED)
+    append_kernel<T, true, true><<<blocks, 256, 0, st>>>(p);
+  else
+    append_kernel<T, true, false><<<blocks, 256, 0, st>>>(p);
+  return launch_status("latent append");
+}
+
+int64_t align256(int64_t v) { return (v + 255) & ~(int64_t)255; }
+
+bool latent_ok(int v) { return v == 128 || v == 256 || v == 512; }
+bool rope_ok(int v) { return v == 32 || v == 64; }
+
+int check_sizes(const grm_b200_latent_plan* p) {
+  if (!p) {
+    set_thread_error("latent plan: null plan");
+    return GRM_B200_EINVAL;
+  }
+  if (!latent_ok(p->latent) || !rope_ok(p->rope)) {
+    set_thread_error("latent plan: latent %d must be 128, 256 or 512 and rope %d 32 or 64",
+                     p->latent, p->rope);
+    return GRM_B200_EINVAL;
+  }
+  if (p->heads < 1 || p->heads > 1024) {
+    set_thread_error("latent plan: heads %d must be 1 to 1024", p->heads);
+    return GRM_B200_EINVAL;
+  }
+  const bool none = p->nope == 0 && p->value == 0 && p->expand_tokens == 0;
+  const bool some = (p->nope == 64 || p->nope == 128) && p->value == p->nope &&
+                    p->expand_tokens >= 1 && p->expand_tokens <= (1 << 28);
+  if (!none && !some) {
+    set_thread_error("latent plan: nope %d and value %d must both be 64 or both 128, with "
+                     "expand_tokens %lld from 1 to 2^28 (or all 0)", p->nope, p->value,
+                     (long long)p->expand_tokens);
+    return GRM_B200_EINVAL;
+  }
+  return 0;
+}
+
+// What does not need a device first, so that a call that cannot be right is refused
+// without one.
+int check_latent_plan(const grm_b200_latent_plan* p) {
+  int rc = check_sizes(p);
+  if (rc) return rc;
+  if (!p->work || (reinterpret_cast<uintptr_t>(p->work) & 255)) {
+    set_thread_error("latent plan: work must be 256-byte aligned device memory");
+    return GRM_B200_EINVAL;
+  }
+  if ((rc = check_plan(&p->step))) return rc;
+  int64_t need = 0;
+  rc = grm_b200_latent_work_bytes(p, &need);
+  if (rc) return rc;
+  if (p->work_bytes < need) {
+    set_thread_error("latent plan: work of %lld bytes, %lld needed", (long long)p->work_bytes,
+                     (long long)need);
+    return GRM_B200_EINVAL;
+  }
+  return 0;
+}
+
+int check_latent_arena(const grm_b200_latent_arena* a) {
+  if (!a || !a->rows || (reinterpret_cast<uintptr_t>(a->rows) & 15)) {
+    set_thread_error("latent arena: rows must be 16-byte aligned device memory");
+    return GRM_B200_EINVAL;
+  }
+  if (a->pages < 1 || a->pages > INT32_MAX / 128 ||
+      (a->page_tokens != 16 && a->page_tokens != 32 && a->page_tokens != 64 &&
+       a->page_tokens != 128) ||
+      !latent_ok(a->latent) || !rope_ok(a->rope) ||
+      (a->dtype != GRM_B200_F16 && a->dtype != GRM_B200_BF16)) {
+    set_thread_error("latent arena: pages %lld (at most 2^24 - 1), page_tokens %d (16, 32, 64, "
+                     "128), latent %d (128, 256, 512), rope %d (32, 64), fp16 or bf16 rows",
+                     (long long)a->pages, a->page_tokens, a->latent, a->rope);
+    return GRM_B200_EINVAL;
+  }
+  return 0;
+}
+
+int check_match(const grm_b200_latent_plan* p, const grm_b200_latent_arena* a) {
+  if (a->pages != p->step.pages || a->page_tokens != p->step.page_tokens ||
+      a->latent != p->latent || a->rope != p->rope) {
+    set_thread_error("latent plan and arena differ: pages %lld / %lld, page_tokens %d / %d, "
+                     "latent %d / %d, rope %d / %d", (long long)p->step.pages, (long long)a->pages,
+                     p->step.page_tokens, a->page_tokens, p->latent, a->latent, p->rope, a->rope);
+    return GRM_B200_EINVAL;
+  }
+  return 0;
+}
+
+int check_attend(const grm_b200_latent_plan* plan, const grm_b200_latent_arena* arena,
+                 float softmax_scale, int causal, const void* out) {
+  int rc;
+  if ((rc = check_sizes(plan)) || (rc = check_latent_arena(arena)) ||
+      (rc = check_match(plan, arena)))
+    return rc;
+  if (!out || (reinterpret_cast<uintptr_t>(out) & 15)) {
+    set_thread_error("latent attend: out must be 16-byte aligned device memory");
+    return GRM_B200_EINVAL;
+  }
+  if (causal && !plan->step.grow) {
+    set_thread_error("latent attend: rows that do not join the arena (grow = 0) have no position "
+                     "in it; attend with causal = 0");
+    return GRM_B200_EINVAL;
+  }
+  if (!(softmax_scale > 0.0f) || !(softmax_scale < INFINITY)) {
+    set_thread_error("latent attend: softmax_scale %g must be positive and finite",
+                     (double)softmax_scale);
+    return GRM_B200_EINVAL;
+  }
+  return 0;
+}
+
+int fill(const grm_b200_latent_plan* plan, const grm_b200_latent_arena* arena,
+         float softmax_scale, int causal, void* out, float* lse, Params* p) {
+  int sms = 0;
+  int rc = paged::current_sms(&sms);
+  if (rc) return rc;
+  Shape s;
+  make_shape(*plan, sms, &s);
+  *p = Params{};
+  p->w = work_of(s, plan->work);
+  p->table = plan->step.table;
+  p->lens = plan->step.lens;
+  p->starts = plan->step.starts;
+  p->requests = plan->step.requests;
+  p->width = plan->step.table_width;
+  p->tokens = plan->step.tokens;
+  p->pages = plan->step.pages;
+  p->expand_tokens = plan->expand_tokens;
+  p->page_shift = paged::shift_of(plan->step.page_tokens);
+  p->heads = plan->heads;
+  p->latent = plan->latent;
+  p->rope = plan->rope;
+  p->nope = plan->nope;
+  p->value = plan->value;
+  p->causal = causal ? 1 : 0;
+  p->cache = static_cast<const uint16_t*>(arena->rows);
+  p->scale_log2 = softmax_scale * 1.44269504088896341f;
+  p->out = static_cast<uint16_t*>(out);
+  p->lse = lse;
+  p->status = plan->step.status;
+  return 0;
+}
+
+}  // namespace
+
+int make_shape(const grm_b200_latent_plan& p, int sms, Shape* s) {
+  int64_t at = align256(sizeof(Header));
+  auto take = [&](int64_t bytes) {
+    const int64_t o = at;
+    at += align256(bytes);
+    return o;
+  };
+  s->off_base = take((p.step.requests + 1) * 4);
+  s->off_keys = take(p.expand_tokens * p.heads * p.nope * 2);
+  s->off_values = take(p.expand_tokens * p.heads * p.value * 2);
+  s->bytes = at;
+  return 0;
+}
+
+}  // namespace latent
+}  // namespace grm_b200
+
+using namespace grm_b200;
+using namespace grm_b200::latent;
+
+extern "C" {
+
+int grm_b200_latent_work_bytes(const grm_b200_latent_plan* plan, int64_t* out_bytes) {
+  int rc = check_sizes(plan);
+  if (rc) return rc;
+  if (!out_bytes) {
+    set_thread_error("latent plan: null out_bytes");
+    return GRM_B200_EINVAL;
+  }
+  int64_t step = 0;
+  int sms = 0;
+  if ((rc = grm_b200_paged_scratch_bytes(&plan->step, &step)) || (rc = paged::current_sms(&sms)))
+    return rc;
+  Shape s;
+  make_shape(*plan, sms, &s);
+  *out_bytes = s.bytes;
+  return 0;
+}
+
+int grm_b200_latent_plan_step(const grm_b200_latent_plan* plan, const int32_t* fresh_device,
+                              void* stream) {
+  int rc = check_latent_plan(plan);
+  if (rc) return rc;
+  int sms = 0;
+  if ((rc = paged::current_sms(&sms)) ||
+      (rc = grm_b200_paged_plan_step(&plan->step, fresh_device, stream)))
+    return rc;
+  Shape s;
+  make_shape(*plan, sms, &s);
+  ScheduleParams p;
+  p.w = work_of(s, plan->work);
+  p.lens = plan->step.lens;
+  p.starts = plan->step.starts;
+  p.status = plan->step.status;
+  p.requests = plan->step.requests;
+  p.expand_tokens = plan->expand_tokens;
+  schedule_kernel<<<1, kScheduleThreads, 0, static_cast<cudaStream_t>(stream)>>>(p);
+  return launch_status("latent plan");
+}
+
+int grm_b200_latent_append(const grm_b200_latent_plan* plan, const grm_b200_latent_arena* arena,
+                           const grm_b200_rotary* rotary, const void* latent_device,
+                           int64_t latent_row_stride, const void* rope_device,
+                           int64_t rope_row_stride, void* stream) {
+  int rc;
+  if ((rc = check_sizes(plan)) || (rc = check_latent_arena(arena)) ||
+      (rc = check_match(plan, arena)) ||
+      (rc = paged::check_rows("latent append", latent_device, arena->dtype, latent_row_stride,
+                              0)) ||
+      (rc = paged::check_rows("latent append", rope_device, arena->dtype, rope_row_stride, 0)) ||
+      (rotary && (rc = check_rotary("latent append", rotary))))
+    return rc;
+  if (rotary && (rotary->dim != arena->rope || rotary->offset != 0)) {
+    set_thread_error("latent append: the rotary's dim %d and offset %d must be %d and 0",
+                     rotary->dim, rotary->offset, arena->rope);
+    return GRM_B200_EINVAL;
+  }
+  if (!plan->step.grow) {
+    set_thread_error("latent append: the plan's rows do not join the arena (grow = 0)");
+    return GRM_B200_EINVAL;
+  }
+  if ((rc = check_latent_plan(plan))) return rc;
+  AppendParams p;
+  p.r = rotary ? rotary_params(*rotary) : RotaryParams{};
+  p.slots = plan->step.slots;
+  p.positions = plan->step.positions;
+  p.tokens = plan->step.tokens;
+  p.limit = arena->pages * arena->page_tokens;
+  p.latent_rows = static_cast<const uint16_t*>(latent_device);
+  p.rope_rows = static_cast<const uint16_t*>(rope_device);
+  p.latent_stride = latent_row_stride;
+  p.rope_stride = rope_row_stride;
+  p.cache = static_cast<uint16_t*>(arena->rows);
+  p.latent = arena->latent;
+  p.rope = arena->rope;
+  p.rotary = rotary != nullptr;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return arena->dtype == GRM_B200_F16 ? launch_append<__half>(p, st)
+                                      : launch_append<__nv_bfloat16>(p, st);
+}
+
+int grm_b200_latent_attend(const grm_b200_latent_plan* plan, const grm_b200_latent_arena* arena,
+                           const void* q_latent_device, int64_t q_latent_row_stride,
+                           int64_t q_latent_head_stride, const void* q_rope_device,
+                           int64_t q_rope_row_stride, int64_t q_rope_head_stride,
+                           float softmax_scale, int causal, void* out_device, float* lse_device,
+                           void* stream) {
+  int rc;
+  Params p;
+  if ((rc = check_attend(plan, arena, softmax_scale, causal, out_device)) ||
+      (rc = paged::check_rows("latent attend", q_latent_device, arena->dtype, q_latent_row_stride,
+                              q_latent_head_stride)) ||
+      (rc = paged::check_rows("latent attend", q_rope_device, arena->dtype, q_rope_row_stride,
+                              q_rope_head_stride)) ||
+      (rc = check_latent_plan(plan)) ||
+      (rc = fill(plan, arena, softmax_scale, causal, out_device, lse_device, &p)))
+    return rc;
+  p.q = static_cast<const uint16_t*>(q_latent_device);
+  p.q_row = q_latent_row_stride;
+  p.q_head = q_latent_head_stride;
+  p.qr = static_cast<const uint16_t*>(q_rope_device);
+  p.qr_row = q_rope_row_stride;
+  p.qr_head = q_rope_head_stride;
+  return launch_absorbed(arena->dtype, p, static_cast<cudaStream_t>(stream));
+}
+
+int grm_b200_latent_attend_expanded(const grm_b200_latent_plan* plan,
+                                    const grm_b200_latent_arena* arena, const void* q_device,
+                                    int64_t q_row_stride, int64_t q_head_stride,
+                                    const void* weights_device, int64_t weights_head_stride,
+                                    int64_t weights_row_stride, float softmax_scale, int causal,
+                                    void* out_device, float* lse_device, void* stream) {
+  int rc;
+  Params p;
+  if ((rc = check_attend(plan, arena, softmax_scale, causal, out_device)) ||
+      (rc = paged::check_rows("latent attend", q_device, arena->dtype, q_row_stride,
+                              q_head_stride)) ||
+      (rc = paged::check_rows("latent attend", weights_device, arena->dtype, weights_row_stride,
+                              weights_head_stride)))
+    return rc;
+  if (plan->nope == 0) {
+    set_thread_error("latent attend: the plan has no room for the expanded form (expand_tokens)");
+    return GRM_B200_EINVAL;
+  }
+  if ((rc = check_latent_plan(plan)) ||
+      (rc = fill(plan, arena, softmax_scale, causal, out_device, lse_device, &p)))
+    return rc;
+  p.q = static_cast<const uint16_t*>(q_device);
+  p.q_row = q_row_stride;
+  p.q_head = q_head_stride;
+  p.qr = p.q + plan->nope;
+  p.qr_row = q_row_stride;
+  p.qr_head = q_head_stride;
+  p.weights = static_cast<const uint16_t*>(weights_device);
+  p.w_head = weights_head_stride;
+  p.w_row = weights_row_stride;
+  return launch_expanded(arena->dtype, p, static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

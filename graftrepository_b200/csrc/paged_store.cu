@@ -19,6 +19,7 @@
 #include <algorithm>
 
 #include "paged.cuh"
+#include "rotary.cuh"
 
 namespace grm_b200 {
 namespace paged {
@@ -202,6 +203,198 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendParams p) {
   if (t == 0) *scale = s;
 }
 
+// ---- append with the keys rotated on the way
+//
+// As append_kernel, with the values held as fp32 and two in three registers: 32 of
+// them a thread.  A thread's 16 values of a row are eight pairs whole: 8 values of
+// the first half of the rotated part and the 8 that turn with them, or 16 in a row
+// where pairs are side by side.  Angles are worked out where they are used, by every
+// kv head anew: about 25 instructions a pair, against a table's 8 bytes from L2.
+
+struct TurnedParams {
+  AppendParams a;
+  RotaryParams r;
+  const int32_t* positions;
+};
+
+// Codes of 16 values in fp32, as quantise.
+__device__ __forceinline__ void quantise_turned(const float (&x)[16], float s, float inv,
+                                                unsigned (&out)[4]) {
+  constexpr float kBase = 12582912.0f;
+  float far = inv < INFINITY ? 0.0f : 1.0f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    unsigned t[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float y = fmaf(x[4 * i + k], inv, kBase);
+      far = fmaxf(far, fabsf(fmaf(x[4 * i + k], inv, kBase - y)));
+      t[k] = __float_as_uint(y);
+    }
+    out[i] = pack4(t[0], t[1], t[2], t[3]);
+  }
+  if (far > 0.5f - 0x1p-15f) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      int t[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) t[k] = __float2int_rn(__fdiv_rn(x[4 * i + k], s));
+      out[i] = pack4(t[0], t[1], t[2], t[3]);
+    }
+  }
+}
+
+template <typename T, int D, int GROUP, int CACHE>
+__global__ void __launch_bounds__(256) append_turned_kernel(const TurnedParams tp) {
+  const AppendParams& p = tp.a;
+  constexpr int kLanes = D / 16;  // threads of a row
+  constexpr int kRowsPass = GROUP / kLanes;
+  __shared__ unsigned warp_max[8];
+  const int t = threadIdx.x % GROUP;
+  const int64_t job = (int64_t)blockIdx.x * (256 / GROUP) + threadIdx.x / GROUP;
+  const int heads2 = p.kv_heads * 2;
+  const int64_t unit = job / heads2;
+  if (unit >= p.header->pages) return;
+  const int side = (int)(job % heads2) & 1, h = (int)(job % heads2) >> 1;
+  const int4 entry = p.pages[unit];
+  const int off = entry.z, rows = entry.w;
+  const int64_t page = min(max((int64_t)entry.y, (int64_t)0), p.ring_size - 1);
+  const int64_t row_stride = side ? p.row_stride[1] : p.row_stride[0];
+  const uint16_t* x = (side ? p.x[1] : p.x[0]) + (int64_t)entry.x * row_stride +
+                      (int64_t)h * (side ? p.head_stride[1] : p.head_stride[0]);
+  int8_t* codes = (side ? p.codes[1] : p.codes[0]) + (((page * p.kv_heads + h) << p.page_shift) * D);
+  float* scale = (side ? p.scales[1] : p.scales[0]) + page * p.kv_heads + h;
+  const int position0 = tp.positions[entry.x];
+
+  // where the thread's two runs of 8 values lie, and its first pair (-1: none)
+  const int lane16 = (t % kLanes) * 16, within = lane16 - tp.r.offset;
+  const bool halves = tp.r.layout == GRM_B200_ROTARY_HALF;
+  const bool turns = side == 0 && within >= 0 && within < tp.r.dim;
+  const int pair0 = turns ? within / 2 : -1;
+  const int at0 = turns && halves ? tp.r.offset + pair0 : lane16;
+  const int at1 = turns && halves ? at0 + tp.r.dim / 2 : lane16 + 8;
+  uint64_t freq[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) freq[i] = turns ? tp.r.turns[pair0 + i] : 0;
+
+  auto load = [&](int r, float (&v)[16]) {
+    const uint16_t* row = x + r * row_stride;
+    const Chunk c{ld_nc16(row + at0), ld_nc16(row + at1)};
+    const unsigned w[8] = {c.a.x, c.a.y, c.a.z, c.a.w, c.b.x, c.b.y, c.b.z, c.b.w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float2 u = widen<T>(w[i]);
+      v[2 * i] = u.x;
+      v[2 * i + 1] = u.y;
+    }
+    if (turns) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const Turn a = turn_of(position0 + r, freq[i]);
+        const float c1 = a.cos * tp.r.amplitude, s1 = a.sin * tp.r.amplitude;
+        const float x1 = halves ? v[i] : v[2 * i], x2 = halves ? v[8 + i] : v[2 * i + 1];
+        const float y1 = x1 * c1 - x2 * s1, y2 = x2 * c1 + x1 * s1;
+        if (halves) {
+          v[i] = y1;
+          v[8 + i] = y2;
+        } else {
+          v[2 * i] = y1;
+          v[2 * i + 1] = y2;
+        }
+      }
+    }
+  };
+  // largest magnitude as bits, which order as numbers do, NaN above infinity
+  auto widest = [](const float (&v)[16]) {
+    unsigned m = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) m = max(m, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+    return m;
+  };
+
+  const int r0 = t / kLanes;
+  float c[CACHE][16];
+  unsigned m = 0;
+#pragma unroll
+  for (int i = 0; i < CACHE; ++i) {
+    const int r = r0 + i * kRowsPass;
+    if (r < rows) {
+      load(r, c[i]);
+      m = max(m, widest(c[i]));
+    }
+  }
+  const float old = off > 0 ? *scale : 0.0f;
+#pragma unroll 1
+  for (int r = r0 + CACHE * kRowsPass; r < rows; r += kRowsPass) {
+    float v[16];
+    load(r, v);
+    m = max(m, widest(v));
+  }
+  m = __reduce_max_sync(kFull, m);
+  if (GROUP > 32) {  // the group's warps exchange their maxima
+    const int first = threadIdx.x / GROUP * (GROUP / 32);
+    if (t % 32 == 0) warp_max[threadIdx.x / 32] = m;
+    asm volatile("bar.sync %0, %1;" ::"r"(1 + (int)threadIdx.x / GROUP), "n"(GROUP) : "memory");
+#pragma unroll
+    for (int w = 0; w < GROUP / 32; ++w) m = max(m, warp_max[first + w]);
+  }
+  float s = __fdiv_rn(__uint_as_float(m), 127.0f);
+  s = old > s || isnan(old) ? old : s;
+  if (!(s < INFINITY)) s = __int_as_float(0x7FC00000);
+  const bool zero = !(s > 0.0f);  // nothing but zeros, or no number: codes 0
+  const float inv = __fdiv_rn(1.0f, s);
+
+  auto store = [&](int r, const float (&v)[16]) {
+    unsigned w[4] = {0, 0, 0, 0};
+    if (!zero) quantise_turned(v, s, inv, w);
+    int8_t* to = codes + (off + r) * D;
+    *reinterpret_cast<uint2*>(to + at0) = make_uint2(w[0], w[1]);
+    *reinterpret_cast<uint2*>(to + at1) = make_uint2(w[2], w[3]);
+  };
+#pragma unroll
+  for (int i = 0; i < CACHE; ++i) {
+    const int r = r0 + i * kRowsPass;
+    if (r < rows) store(r, c[i]);
+  }
+#pragma unroll 1
+  for (int r = r0 + CACHE * kRowsPass; r < rows; r += kRowsPass) {
+    float v[16];
+    load(r, v);
+    store(r, v);
+  }
+  if (off > 0 && !(s == old)) {
+#pragma unroll 1
+    for (int r = r0; r < off; r += kRowsPass) {
+      uint4* q = reinterpret_cast<uint4*>(codes + r * D + lane16);
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (!zero) {
+        v = *q;
+        v = make_uint4(rescale4(v.x, old, s), rescale4(v.y, old, s), rescale4(v.z, old, s),
+                       rescale4(v.w, old, s));
+      }
+      *q = v;
+    }
+  }
+  if (GROUP == 32) __syncwarp();  // every lane has read the old scale (else: the barrier above)
+  if (t == 0) *scale = s;
+}
+
+template <typename T, int D, int GROUP, int CACHE>
+int launch_append_group(const TurnedParams& p, int64_t cap, cudaStream_t st) {
+  const int64_t blocks = ceil_div64(cap * p.a.kv_heads * 2, 256 / GROUP);
+  append_turned_kernel<T, D, GROUP, CACHE><<<(unsigned)blocks, 256, 0, st>>>(p);
+  return launch_status("paged append");
+}
+
+template <typename T, int D>
+int launch_append(const TurnedParams& p, int64_t cap, int64_t max_fresh, cudaStream_t st) {
+  const int64_t values = std::min<int64_t>(max_fresh, (int64_t)1 << p.a.page_shift) * D;
+  if (values <= 32 * 32) return launch_append_group<T, D, 32, 2>(p, cap, st);
+  if (values <= 64 * 32) return launch_append_group<T, D, 64, 2>(p, cap, st);
+  if (values <= 128 * 32) return launch_append_group<T, D, 128, 2>(p, cap, st);
+  return launch_append_group<T, D, 256, 2>(p, cap, st);
+}
+
 template <typename T, int D, int GROUP, int CACHE>
 int launch_append_group(const AppendParams& p, int64_t cap, cudaStream_t st) {
   const int64_t blocks = ceil_div64(cap * p.kv_heads * 2, 256 / GROUP);
@@ -223,9 +416,8 @@ int launch_append(const AppendParams& p, int64_t cap, int64_t max_fresh, cudaStr
   return launch_append_group<T, D, 256, 4>(p, cap, st);
 }
 
-template <typename T>
-int launch_append_dim(int dim, const AppendParams& p, int64_t cap, int64_t max_fresh,
-                      cudaStream_t st) {
+template <typename T, typename P>
+int launch_append_dim(int dim, const P& p, int64_t cap, int64_t max_fresh, cudaStream_t st) {
   if (dim == 64) return launch_append<T, 64>(p, cap, max_fresh, st);
   if (dim == 128) return launch_append<T, 128>(p, cap, max_fresh, st);
   return launch_append<T, 256>(p, cap, max_fresh, st);
@@ -335,12 +527,12 @@ int check_rows(const char* what, const void* ptr, int dtype, int64_t row_stride,
 using namespace grm_b200;
 using namespace grm_b200::paged;
 
-extern "C" {
+namespace {
 
-int grm_b200_paged_append(const grm_b200_paged_plan* plan, const grm_b200_paged_arena* arena,
-                          const void* k_device, const void* v_device, int dtype,
-                          int64_t k_row_stride, int64_t k_head_stride, int64_t v_row_stride,
-                          int64_t v_head_stride, void* stream) {
+int append(const grm_b200_paged_plan* plan, const grm_b200_paged_arena* arena,
+           const grm_b200_rotary* rotary, const void* k_device, const void* v_device, int dtype,
+           int64_t k_row_stride, int64_t k_head_stride, int64_t v_row_stride,
+           int64_t v_head_stride, void* stream) {
   int rc;
   if ((rc = check_plan(plan)) || (rc = check_arena(arena)) || (rc = check_match(plan, arena)) ||
       (rc = check_rows("paged append", k_device, dtype, k_row_stride, k_head_stride)) ||
@@ -378,9 +570,45 @@ int grm_b200_paged_append(const grm_b200_paged_plan* plan, const grm_b200_paged_
   p.scales[1] = arena->v_scales;
   const int64_t fresh = std::min(plan->max_fresh, plan->tokens);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (rotary) {
+    const TurnedParams tp{p, rotary_params(*rotary), plan->positions};
+    return dtype == GRM_B200_F16
+               ? launch_append_dim<__half>(plan->head_dim, tp, s.page_cap, fresh, st)
+               : launch_append_dim<__nv_bfloat16>(plan->head_dim, tp, s.page_cap, fresh, st);
+  }
   return dtype == GRM_B200_F16
              ? launch_append_dim<__half>(plan->head_dim, p, s.page_cap, fresh, st)
              : launch_append_dim<__nv_bfloat16>(plan->head_dim, p, s.page_cap, fresh, st);
+}
+
+}  // namespace
+
+extern "C" {
+
+int grm_b200_paged_append(const grm_b200_paged_plan* plan, const grm_b200_paged_arena* arena,
+                          const void* k_device, const void* v_device, int dtype,
+                          int64_t k_row_stride, int64_t k_head_stride, int64_t v_row_stride,
+                          int64_t v_head_stride, void* stream) {
+  return append(plan, arena, nullptr, k_device, v_device, dtype, k_row_stride, k_head_stride,
+                v_row_stride, v_head_stride, stream);
+}
+
+int grm_b200_paged_append_rotary(const grm_b200_paged_plan* plan, const grm_b200_paged_arena* arena,
+                                 const grm_b200_rotary* rotary, const void* k_device,
+                                 const void* v_device, int dtype, int64_t k_row_stride,
+                                 int64_t k_head_stride, int64_t v_row_stride,
+                                 int64_t v_head_stride, void* stream) {
+  const int rc = check_rotary("paged append", rotary);
+  if (rc) return rc;
+  if (plan && (rotary->layout == GRM_B200_ROTARY_PAIR_SWAP || rotary->dim % 16 ||
+               rotary->offset % 16 || (int64_t)rotary->offset + rotary->dim > plan->head_dim)) {
+    set_thread_error("paged append: rotates dims at multiples of 16 within head_dim %d, layout half "
+                     "or interleaved; got offset %d, dim %d, layout %d", plan->head_dim,
+                     rotary->offset, rotary->dim, rotary->layout);
+    return GRM_B200_EINVAL;
+  }
+  return append(plan, arena, rotary, k_device, v_device, dtype, k_row_stride, k_head_stride,
+                v_row_stride, v_head_stride, stream);
 }
 
 int grm_b200_paged_read(const grm_b200_paged_arena* arena, const int64_t* slots_device,

@@ -56,6 +56,7 @@ PAGE_TOKENS = (16, 32, 64, 128)
 HEAD_DIMS = (64, 128, 256)
 
 PLAN_BAD_LENGTH, PLAN_ROWS, PLAN_TABLE, PLAN_PAGES, PLAN_WAIT, PLAN_STALE = 1, 2, 4, 8, 16, 32
+PLAN_EXPAND = 64
 _REASONS = {
     PLAN_BAD_LENGTH: "a negative length, or one past 2^31 - 1024",
     PLAN_ROWS: "more new rows than the plan has room for (tokens, max_fresh)",
@@ -64,6 +65,7 @@ _REASONS = {
     PLAN_WAIT: "a wait inside attention gave up and left rows of NaN",
     PLAN_STALE: "its requests or free pages have changed since it was planned, and it was not "
                 "committed",
+    PLAN_EXPAND: "more tokens to expand than the plan has room for (expand_tokens)",
 }
 
 
@@ -205,6 +207,8 @@ class PagePlan(_Buffers):
     [requests + 1], ``positions`` and ``rows`` int32 [tokens], ``slots`` int64
     [tokens] (-1 past the last row), ``cursor`` int64 [2], ``status`` int32 [1]."""
 
+    latent = 0  # values of a latent row, in a plan for those
+
     def __init__(self, tables: "PageTables", tokens: int, kv_heads: int, query_heads: int,
                  head_dim: int, max_fresh: int | None):
         if head_dim not in HEAD_DIMS:
@@ -253,6 +257,7 @@ class PagePlan(_Buffers):
         self.planned, self.grow = False, True
         self._turn = None  # of the tables' joining steps, until it is committed
         self._ref = ctypes.byref(c)
+        self._step, self._step_ref = _lib.load().grm_b200_paged_plan_step, self._ref
 
     def _join(self, stream) -> None:  # and the tables, for every call that takes a plan
         super()._join(stream)
@@ -291,7 +296,6 @@ class PageTables(_Buffers):
         self.page_tokens = _check_page(page_tokens)
         self.device = _device(device)
         self._index, self._shape = self.device.index, torch.Size((self.requests,))
-        self._plan_step = _lib.load().grm_b200_paged_plan_step
         self._turn = 0  # joining steps planned so far, those under capture left out
         self.table = torch.full((requests, width), -1, dtype=torch.int32, device=self.device)
         self.lens = torch.zeros(requests, dtype=torch.int32, device=self.device)
@@ -321,7 +325,7 @@ class PageTables(_Buffers):
         if grow is not plan.grow:
             plan.grow = bool(grow)
             plan.c.grow = 1 if grow else 0
-        _call(self._plan_step, self._index, plan._ref, fresh.data_ptr(),
+        _call(plan._step, self._index, plan._step_ref, fresh.data_ptr(),
               _handle(stream, self._index, (plan,), fresh))
         plan.planned, plan._turn = True, None
         # a step that a graph plans again has no turn: the host does not see it
@@ -391,6 +395,7 @@ class PagedArena(_Buffers):
         lib = _lib.load()
         self._index = self.device.index
         self._append, self._attend = lib.grm_b200_paged_append, lib.grm_b200_paged_attend
+        self._append_rotary = lib.grm_b200_paged_append_rotary
         self._read = lib.grm_b200_paged_read
         self._scale = 1.0 / math.sqrt(head_dim)
 
@@ -416,6 +421,8 @@ class PagedArena(_Buffers):
         """The layer's buffers, for a plan that is good for a call."""
         if not plan.planned:
             raise ValueError("the plan has not been planned yet (PageTables.plan)")
+        if plan.latent:
+            raise ValueError("the plan was made for latent rows (LatentArena.make_plan)")
         if plan._index != self._index:
             raise ValueError(f"the plan is on {plan.device}, the arena on {self.device}")
         if plan._turn is not None:
@@ -433,9 +440,12 @@ class PagedArena(_Buffers):
                              f"{self.device}")
         return t
 
-    def append(self, plan: PagePlan, k, v, *, layer: int = 0, stream=None) -> None:
+    def append(self, plan: PagePlan, k, v, *, layer: int = 0, rotary=None, stream=None) -> None:
         """Quantise the step's rows ``k`` and ``v`` [tokens, kv_heads, head_dim]
-        into the pages of `layer`, before those of any later step."""
+        into the pages of `layer`, before those of any later step.  With a
+        ``rotary.Rotary`` (layout half or interleaved, dim and offset multiples of
+        16) the keys are rotated by ``plan.positions`` on the way, with no rounding
+        between rotation and codes."""
         ref = self._ready(plan, layer)
         kind, k_ptr, k_row, k_head = self._rows("k", k, plan.kv_shape)
         v_kind, v_ptr, v_row, v_head = self._rows("v", v, plan.kv_shape)
@@ -443,8 +453,19 @@ class PagedArena(_Buffers):
             raise ValueError(f"k and v differ in type: {k.dtype}, {v.dtype}")
         if not plan.grow:
             raise ValueError("the plan's rows do not join the arena (planned with grow=False)")
-        _call(self._append, self._index, plan._ref, ref, k_ptr, v_ptr, kind, k_row, k_head, v_row,
-              v_head, _handle(stream, self._index, (self, plan), k, v))
+        if rotary is None:
+            _call(self._append, self._index, plan._ref, ref, k_ptr, v_ptr, kind, k_row, k_head,
+                  v_row, v_head, _handle(stream, self._index, (self, plan), k, v))
+            return
+        rotary._on(self._index)
+        if (rotary.layout == "pair_swap" or rotary.dim % 16 or rotary.offset % 16 or
+                rotary.offset + rotary.dim > self.head_dim):
+            raise ValueError(f"append rotates dims at multiples of 16 within head_dim "
+                             f"{self.head_dim}, layout half or interleaved; the rotary has offset "
+                             f"{rotary.offset}, dim {rotary.dim}, layout {rotary.layout}")
+        _call(self._append_rotary, self._index, plan._ref, ref, rotary._ref, k_ptr, v_ptr, kind,
+              k_row, k_head, v_row, v_head, _handle(stream, self._index, (self, plan, rotary), k,
+                                                    v))
 
     def attend(self, plan: PagePlan, q, *, layer: int = 0, causal: bool = True,
                scale: float | None = None, out=None, lse=None, stream=None):

@@ -559,6 +559,132 @@ int grm_b200_paged_attend(const grm_b200_paged_plan* plan, const grm_b200_paged_
                           int64_t q_head_stride, float softmax_scale, int causal,
                           void* out_device, float* lse_device, void* stream);
 
+/* ---------------------------------------------------------- rotary positions */
+
+/* Rotary positions of `dim` values of a head, from `offset` on: pair i (of
+ * dim / 2) turns by position * turns[i] * 2^-64 of a full turn and is multiplied
+ * by `amplitude`.  turns (device, uint64 [dim / 2]) is 2^64 times a frequency
+ * over 2 pi, so that far positions lose nothing.  No reference counterpart as a
+ * call: the reference rotates inside its engine, by tables (core/graft_arena.py:339-367). */
+typedef struct grm_b200_rotary {
+  const uint64_t* turns;
+  int32_t dim;
+  int32_t offset;
+  int32_t layout;
+  float amplitude;
+} grm_b200_rotary;
+
+#define GRM_B200_ROTARY_HALF 0         /* pair i: values i and i + dim / 2 */
+#define GRM_B200_ROTARY_INTERLEAVED 1  /* pair i: values 2 i and 2 i + 1 */
+#define GRM_B200_ROTARY_PAIR_SWAP 2    /* taken from 2 i and 2 i + 1, put to i and i + dim / 2 */
+
+/* Rotate rows x [tokens, heads, head_dim] (GRM_B200_F32, _F16 or _BF16; strides in
+ * elements, a head's values contiguous) to out, by positions_device int32
+ * [tokens]; inverse != 0 takes the rotation off.  Out of place the other values of a
+ * head are copied, and rows with a negative position as they are; in place
+ * (out == x, the same strides, no pair swap) both are left alone.  fp32, one
+ * rounding.  out must not overlap x otherwise.  Any strides will do; multiples of
+ * 8 elements and 16-byte pointers are fast. */
+int grm_b200_rotate(const grm_b200_rotary* rotary, const void* x_device, int dtype, int64_t tokens,
+                    int64_t heads, int64_t head_dim, int64_t x_row_stride, int64_t x_head_stride,
+                    const int32_t* positions_device, int inverse, void* out_device,
+                    int64_t out_row_stride, int64_t out_head_stride, void* stream);
+
+/* grm_b200_paged_append with the keys rotated on the way, by plan->positions: the
+ * rotated keys are quantised as they are, in fp32, without a rounding of their own.
+ * Layouts HALF and INTERLEAVED, dim and offset multiples of 16. */
+int grm_b200_paged_append_rotary(const grm_b200_paged_plan* plan, const grm_b200_paged_arena* arena,
+                                 const grm_b200_rotary* rotary, const void* k_device,
+                                 const void* v_device, int dtype, int64_t k_row_stride,
+                                 int64_t k_head_stride, int64_t v_row_stride,
+                                 int64_t v_head_stride, void* stream);
+
+/* ------------------------------------------------- pages of latent rows
+ *
+ * Models with latent attention keep one row a token for all heads: `latent`
+ * values that every head's keys and values are made from, and `rope` values that
+ * hold the position (256 and 32 in the mount's workload).  The arena holds those
+ * rows as they are, in 16 bits, in pages of the same tables as the 8-bit arena's.
+ * No reference counterpart: the reference mounts such rows (core/graft_arena.py:303-311)
+ * and its engine attends to one request's. */
+typedef struct grm_b200_latent_arena {
+  void* rows; /* [pages, page_tokens, latent + rope] of type dtype, 16-byte aligned */
+  int64_t pages;
+  int32_t page_tokens;
+  int32_t latent; /* 128, 256 or 512 */
+  int32_t rope;   /* 32 or 64 */
+  int32_t dtype;  /* GRM_B200_F16 or GRM_B200_BF16 */
+} grm_b200_latent_arena;
+
+/* A step over latent rows: `step` as for the 8-bit arena, with kv_heads and
+ * query_heads 1 and head_dim 64, which are not used; `heads` query heads.
+ * nope and value: what the expanded form makes of a latent row for each head (both
+ * 64 or both 128; 0 where it is not used); expand_tokens: room for the tokens that
+ * it expands, the lengths of the requests with rows in the step, each rounded up to
+ * 64.  work: work_bytes (grm_b200_latent_work_bytes) of device memory, 256-byte
+ * aligned; calls that share it must not overlap on the GPU. */
+typedef struct grm_b200_latent_plan {
+  grm_b200_paged_plan step;
+  int32_t heads;
+  int32_t latent;
+  int32_t rope;
+  int32_t nope;
+  int32_t value;
+  int64_t expand_tokens;
+  void* work;
+  int64_t work_bytes;
+} grm_b200_latent_plan;
+
+#define GRM_B200_PLAN_EXPAND 64 /* more tokens to expand than expand_tokens */
+
+/* Bytes of work of a plan of these sizes (the pointers are not read). */
+int grm_b200_latent_work_bytes(const grm_b200_latent_plan* plan, int64_t* out_bytes);
+
+/* grm_b200_paged_plan_step and the lists of attention over latent rows.  A step
+ * with more tokens to expand than expand_tokens is planned and gets
+ * GRM_B200_PLAN_EXPAND; what attend_expanded answers for it is NaN. */
+int grm_b200_latent_plan_step(const grm_b200_latent_plan* plan, const int32_t* fresh_device,
+                              void* stream);
+
+/* Write a planned step's rows into their pages: latent [tokens, latent] and rope
+ * [tokens, rope], given by their row strides in elements (multiples of 8, 16-byte
+ * aligned pointers).  With a rotary (dim = rope, offset 0, any layout; NULL: none)
+ * the positional part is rotated by the step's positions on the way.  The plan
+ * must have been made with grow != 0. */
+int grm_b200_latent_append(const grm_b200_latent_plan* plan, const grm_b200_latent_arena* arena,
+                           const grm_b200_rotary* rotary, const void* latent_device,
+                           int64_t latent_row_stride, const void* rope_device,
+                           int64_t rope_row_stride, void* stream);
+
+/* Latent attention, absorbed form: queries in the latent space, q_latent [tokens,
+ * heads, latent] and q_rope [tokens, heads, rope] of the arena's type (strides and
+ * alignment as append's).  With (c_t, r_t) the row of token t,
+ *   out[i, h] = sum_t w_t c_t,  w = softmax_t(softmax_scale * (q_latent . c_t + q_rope . r_t))
+ * over the request's lens[r] tokens, or with causal != 0 over the positions up to
+ * the row's own.  out [tokens, heads, latent] has the arena's type; lse [tokens,
+ * heads] fp32 (may be NULL).  A row that sees nothing is 0 with lse -inf, as are the
+ * rows past the step's last one.  Tokens that a row does not see do not reach it,
+ * whatever they hold.  Results do not depend on the order in which blocks run. */
+int grm_b200_latent_attend(const grm_b200_latent_plan* plan, const grm_b200_latent_arena* arena,
+                           const void* q_latent_device, int64_t q_latent_row_stride,
+                           int64_t q_latent_head_stride, const void* q_rope_device,
+                           int64_t q_rope_row_stride, int64_t q_rope_head_stride,
+                           float softmax_scale, int causal, void* out_device, float* lse_device,
+                           void* stream);
+
+/* Latent attention, expanded form: weights [heads, nope + value, latent] (head and
+ * row strides, a row's values contiguous) make each head's keys and values,
+ *   k_t = (weights[h, :nope] c_t, r_t),  v_t = weights[h, nope:] c_t,
+ * rounded to the arena's type, and q [tokens, heads, nope + rope] attends to them;
+ * out [tokens, heads, value].  Otherwise as grm_b200_latent_attend.  Fewer
+ * operations than the absorbed form where a request has many rows (prompts). */
+int grm_b200_latent_attend_expanded(const grm_b200_latent_plan* plan,
+                                    const grm_b200_latent_arena* arena, const void* q_device,
+                                    int64_t q_row_stride, int64_t q_head_stride,
+                                    const void* weights_device, int64_t weights_head_stride,
+                                    int64_t weights_row_stride, float softmax_scale, int causal,
+                                    void* out_device, float* lse_device, void* stream);
+
 /* ----------------------------------------------------- multi-GPU top-k merge */
 
 /* Merge `lists` candidate lists of `per_list` (score, id) entries each (device
