@@ -14,45 +14,106 @@ using paged::check_plan;
 using paged::launch_status;
 
 constexpr int kScheduleThreads = 1024;
+constexpr int kForms = 2;  // absorbed, expanded
 
 struct ScheduleParams {
-  Work w;
+  Lists l[kForms];
+  Tiling tiling[kForms];
+  int forms;  // 1 where the plan has no expanded form
+  int32_t* room;
   const int32_t* lens;
   const int32_t* starts;
   int32_t* status;
   int64_t requests, expand_tokens;
+  int grow;
 };
 
-// One block: the requests in chunks, prefix sums of what they add.
-__global__ void __launch_bounds__(kScheduleThreads) schedule_kernel(const ScheduleParams p) {
-  __shared__ int64_t part[32];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  int64_t expand = 0;  // before the chunk
-  for (int64_t r0 = 0; r0 < p.requests; r0 += kScheduleThreads) {
-    const int64_t r = r0 + tid;
-    int64_t n = 0;
-    if (r < p.requests && p.starts[r + 1] > p.starts[r])
-      n = ((int64_t)p.lens[r] + kExpandAlign - 1) / kExpandAlign * kExpandAlign;
-    int64_t incl = n;
+// Inclusive prefix sum over the block; `part` is of the block's warps.
+__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* part, int64_t* all) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t up = __shfl_up_sync(kFull, v, o);
+    if (lane >= o) v += up;
+  }
+  __syncthreads();  // the sums of the call before have been read
+  if (lane == 31) part[warp] = v;
+  __syncthreads();
+  if (warp == 0) {
+    const int64_t own = part[lane];
+    int64_t w = own;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int64_t up = __shfl_up_sync(kFull, incl, o);
-      if (lane >= o) incl += up;
+      const int64_t up = __shfl_up_sync(kFull, w, o);
+      if (lane >= o) w += up;
     }
-    __syncthreads();
-    if (lane == 31) part[warp] = incl;
-    __syncthreads();
-    int64_t before = expand;
-    for (int w = 0; w < warp; ++w) before += part[w];
-    for (int w = 0; w < 32; ++w) expand += part[w];
-    if (r < p.requests)
-      p.w.base[r] = (int)min(before + incl - n, (int64_t)INT32_MAX);
+    part[lane] = w - own;
+    if (lane == 31) part[32] = w;
+  }
+  __syncthreads();
+  *all = part[32];
+  return part[warp] + v;
+}
+
+// One block for each form, and one for the room of what is expanded: prefix sums over
+// the requests, 1,024 at a time, then each worker's first request by a binary search.
+__global__ void __launch_bounds__(kScheduleThreads) schedule_kernel(const ScheduleParams p) {
+  __shared__ int64_t part[33];
+  __shared__ Header sh;
+  const int tid = threadIdx.x, form = blockIdx.x;
+  const bool sizes = form < p.forms;  // else: room
+  const Lists l = p.l[sizes ? form : 0];
+  const Tiling tiling = p.tiling[sizes ? form : 0];
+  int64_t before = 0, room = 0;
+  for (int64_t r0 = 0; r0 < p.requests; r0 += kScheduleThreads) {
+    const int64_t r = r0 + tid;
+    int64_t n = 0, tokens = 0;
+    if (r < p.requests) {
+      const Request q = request_of(p.starts[r], p.starts[r + 1], p.lens[r], tiling.per, p.grow);
+      if (q.n > 0) {
+        n = q.total * tiling.groups;
+        tokens = ((int64_t)q.len + kExpandAlign - 1) / kExpandAlign * kExpandAlign;
+      }
+    }
+    int64_t all = 0;
+    if (sizes) {
+      const int64_t incl = block_scan(n, part, &all);
+      if (r < p.requests) l.base[r] = before + incl - n;
+      before += all;
+    }
+    if (form > 0 || !sizes) {  // the second form's block wants to know if it has room
+      const int64_t incl = block_scan(tokens, part, &all);
+      if (!sizes && r < p.requests)
+        p.room[r] = (int)min(room + incl - tokens, (int64_t)INT32_MAX);
+      room += all;
+    }
+  }
+  const bool lost = p.expand_tokens > 0 && room > p.expand_tokens;
+  if (!sizes) {
+    if (tid == 0) {
+      p.room[p.requests] = lost ? 0 : (int)room;  // nothing is expanded then
+      if (lost) atomicOr(p.status, GRM_B200_PLAN_EXPAND);
+    }
+    return;
   }
   if (tid == 0) {
-    const bool over = p.expand_tokens > 0 && expand > p.expand_tokens;
-    p.w.base[p.requests] = (int)min(expand, (int64_t)INT32_MAX);
-    *p.w.header = Header{p.starts[p.requests], over};
-    if (over) atomicOr(p.status, GRM_B200_PLAN_EXPAND);
+    const int64_t most = before / kLeast;
+    const int workers = before == 0 ? 0 : (int)min((int64_t)tiling.workers, max(most, (int64_t)1));
+    sh = Header{before, workers ? before / workers : 0, workers ? (int)(before % workers) : 0,
+                workers, lost};
+    *l.header = sh;
+    l.base[p.requests] = before;
+  }
+  __syncthreads();  // and the block's own writes to base are there
+  for (int w = tid; w < sh.workers; w += kScheduleThreads) {
+    const int64_t u = worker_first(w, sh);
+    int64_t lo = 0, hi = p.requests;
+    while (hi - lo > 1) {
+      const int64_t mid = (lo + hi) >> 1;
+      if (l.base[mid] <= u) lo = mid;
+      else hi = mid;
+    }
+    l.start[w] = (int)lo;
   }
 }
 
@@ -132,6 +193,11 @@ int check_sizes(const grm_b200_latent_plan* p) {
   }
   if (p->heads < 1 || p->heads > 1024) {
     set_thread_error("latent plan: heads %d must be 1 to 1024", p->heads);
+    return GRM_B200_EINVAL;
+  }
+  if (p->step.tokens > INT32_MAX / p->heads) {
+    set_thread_error("latent plan: %lld rows of %d heads are more than 2^31 - 1",
+                     (long long)p->step.tokens, p->heads);
     return GRM_B200_EINVAL;
   }
   const bool none = p->nope == 0 && p->value == 0 && p->expand_tokens == 0;
@@ -219,7 +285,7 @@ int check_attend(const grm_b200_latent_plan* plan, const grm_b200_latent_arena* 
   return 0;
 }
 
-int fill(const grm_b200_latent_plan* plan, const grm_b200_latent_arena* arena,
+int fill(const grm_b200_latent_plan* plan, const grm_b200_latent_arena* arena, int form,
          float softmax_scale, int causal, void* out, float* lse, Params* p) {
   int sms = 0;
   int rc = paged::current_sms(&sms);
@@ -227,7 +293,13 @@ int fill(const grm_b200_latent_plan* plan, const grm_b200_latent_arena* arena,
   Shape s;
   make_shape(*plan, sms, &s);
   *p = Params{};
-  p->w = work_of(s, plan->work);
+  p->l = lists_of(s, form, plan->work);
+  p->tiling = s.tiling[form];
+  p->probes = std::min(scan_wait_limit(), paged::kProbes);
+  char* work = static_cast<char*>(plan->work);
+  p->room = reinterpret_cast<const int32_t*>(work + s.off_room);
+  p->keys = reinterpret_cast<uint16_t*>(work + s.off_keys);
+  p->values = reinterpret_cast<uint16_t*>(work + s.off_values);
   p->table = plan->step.table;
   p->lens = plan->step.lens;
   p->starts = plan->step.starts;
@@ -241,8 +313,9 @@ int fill(const grm_b200_latent_plan* plan, const grm_b200_latent_arena* arena,
   p->latent = plan->latent;
   p->rope = plan->rope;
   p->nope = plan->nope;
-  p->value = plan->value;
   p->causal = causal ? 1 : 0;
+  p->grow = plan->step.grow ? 1 : 0;
+  p->dtype = arena->dtype;
   p->cache = static_cast<const uint16_t*>(arena->rows);
   p->scale_log2 = softmax_scale * 1.44269504088896341f;
   p->out = static_cast<uint16_t*>(out);
@@ -254,16 +327,69 @@ int fill(const grm_b200_latent_plan* plan, const grm_b200_latent_arena* arena,
 }  // namespace
 
 int make_shape(const grm_b200_latent_plan& p, int sms, Shape* s) {
-  int64_t at = align256(sizeof(Header));
+  s->tiling[0] = absorbed_tiling(p.heads, p.latent, sms);
+  s->tiling[1] = expanded_tiling(p.heads, sms);
+  int64_t at = 0;
   auto take = [&](int64_t bytes) {
     const int64_t o = at;
     at += align256(bytes);
     return o;
   };
-  s->off_base = take((p.step.requests + 1) * 4);
-  s->off_keys = take(p.expand_tokens * p.heads * p.nope * 2);
+  for (int f = 0; f < kForms; ++f) {
+    s->off_header[f] = take(sizeof(Header));
+    s->off_base[f] = take((p.step.requests + 1) * 8);
+    s->off_start[f] = take((int64_t)s->tiling[f].workers * 4);
+  }
+  const int64_t absorbed = (int64_t)s->tiling[0].workers * s->tiling[0].splits *
+                           slot_floats(kRows, std::min(p.latent, 256));
+  const int64_t expanded =
+      p.nope ? (int64_t)s->tiling[1].workers * slot_floats(2 * kRows, p.value) : 0;
+  s->off_part = take(std::max(absorbed, expanded) * 2 * 4);
+  s->off_room = take((p.step.requests + 1) * 4);
+  s->off_keys = take(p.expand_tokens * p.heads * 2 * p.nope * 2);
   s->off_values = take(p.expand_tokens * p.heads * p.value * 2);
   s->bytes = at;
+  return 0;
+}
+
+// cuTensorMapEncodeTiled from the driver, looked up once (no libcuda link).
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
+                                 const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                 const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+static EncodeTiled encode_tiled() {
+  static const EncodeTiled fn = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault,
+                                         &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      f = nullptr;
+    return reinterpret_cast<EncodeTiled>(f);
+  }();
+  return fn;
+}
+
+int make_map(CUtensorMap* map, const void* base, int rank, const int64_t* dims,
+             const int64_t* strides, const int* box) {
+  const EncodeTiled encode = encode_tiled();
+  cuuint64_t d[3], s[2];
+  cuuint32_t b[3];
+  const cuuint32_t step[3] = {1, 1, 1};
+  for (int i = 0; i < rank; ++i) {
+    d[i] = (cuuint64_t)dims[i];
+    b[i] = (cuuint32_t)box[i];
+    if (i > 0) s[i - 1] = (cuuint64_t)strides[i - 1] * 2;
+  }
+  if (!encode ||
+      encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, rank, const_cast<void*>(base), d, s, b, step,
+             CU_TENSOR_MAP_INTERLEAVE_NONE,
+             box[0] == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS) {
+    set_thread_error("latent attend: no tensor map of rows of %lld values", (long long)dims[0]);
+    return GRM_B200_EINVAL;
+  }
   return 0;
 }
 
@@ -303,13 +429,20 @@ int grm_b200_latent_plan_step(const grm_b200_latent_plan* plan, const int32_t* f
   Shape s;
   make_shape(*plan, sms, &s);
   ScheduleParams p;
-  p.w = work_of(s, plan->work);
+  for (int f = 0; f < kForms; ++f) {
+    p.l[f] = lists_of(s, f, plan->work);
+    p.tiling[f] = s.tiling[f];
+  }
+  p.forms = plan->nope ? kForms : 1;
+  p.room = reinterpret_cast<int32_t*>(static_cast<char*>(plan->work) + s.off_room);
   p.lens = plan->step.lens;
   p.starts = plan->step.starts;
   p.status = plan->step.status;
   p.requests = plan->step.requests;
   p.expand_tokens = plan->expand_tokens;
-  schedule_kernel<<<1, kScheduleThreads, 0, static_cast<cudaStream_t>(stream)>>>(p);
+  p.grow = plan->step.grow ? 1 : 0;
+  schedule_kernel<<<plan->nope ? kForms + 1 : 1, kScheduleThreads, 0,
+                    static_cast<cudaStream_t>(stream)>>>(p);
   return launch_status("latent plan");
 }
 
@@ -368,7 +501,7 @@ int grm_b200_latent_attend(const grm_b200_latent_plan* plan, const grm_b200_late
       (rc = paged::check_rows("latent attend", q_rope_device, arena->dtype, q_rope_row_stride,
                               q_rope_head_stride)) ||
       (rc = check_latent_plan(plan)) ||
-      (rc = fill(plan, arena, softmax_scale, causal, out_device, lse_device, &p)))
+      (rc = fill(plan, arena, 0, softmax_scale, causal, out_device, lse_device, &p)))
     return rc;
   p.q = static_cast<const uint16_t*>(q_latent_device);
   p.q_row = q_latent_row_stride;
@@ -376,7 +509,7 @@ int grm_b200_latent_attend(const grm_b200_latent_plan* plan, const grm_b200_late
   p.qr = static_cast<const uint16_t*>(q_rope_device);
   p.qr_row = q_rope_row_stride;
   p.qr_head = q_rope_head_stride;
-  return launch_absorbed(arena->dtype, p, static_cast<cudaStream_t>(stream));
+  return launch_absorbed(p, static_cast<cudaStream_t>(stream));
 }
 
 int grm_b200_latent_attend_expanded(const grm_b200_latent_plan* plan,
@@ -398,7 +531,7 @@ int grm_b200_latent_attend_expanded(const grm_b200_latent_plan* plan,
     return GRM_B200_EINVAL;
   }
   if ((rc = check_latent_plan(plan)) ||
-      (rc = fill(plan, arena, softmax_scale, causal, out_device, lse_device, &p)))
+      (rc = fill(plan, arena, 1, softmax_scale, causal, out_device, lse_device, &p)))
     return rc;
   p.q = static_cast<const uint16_t*>(q_device);
   p.q_row = q_row_stride;
@@ -409,7 +542,9 @@ int grm_b200_latent_attend_expanded(const grm_b200_latent_plan* plan,
   p.weights = static_cast<const uint16_t*>(weights_device);
   p.w_head = weights_head_stride;
   p.w_row = weights_row_stride;
-  return launch_expanded(arena->dtype, p, static_cast<cudaStream_t>(stream));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if ((rc = launch_expand(p, st))) return rc;
+  return launch_expanded(p, st);
 }
 
 }  // extern "C"

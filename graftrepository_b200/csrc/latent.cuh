@@ -1,50 +1,97 @@
-// latent.cuh -- what the kernels over pages of latent rows share.
+// latent.cuh -- what the kernels over pages of latent rows share: how a step's
+// attention is cut into shares, and the layout of a plan's work area.
 #pragma once
+
+#include <cuda.h>
 
 #include "paged.cuh"
 
 namespace grm_b200 {
 namespace latent {
 
+constexpr int kStep = 64;   // tokens of a step of the softmax
+constexpr int kRows = 128;  // rows of a query tile
 // Tokens of a request are expanded from a multiple of this on.
 constexpr int kExpandAlign = 64;
 
-struct Header {      // written by the schedule kernel
-  int32_t rows;      // packed rows of the step
-  int32_t overflow;  // more tokens to expand than there is room for
+// Both forms of attention go over tiles of query rows, each of which sees some of
+// its request's tokens, and every worker (a block, one an SM) gets the same number of
+// units: a tile costs the tokens that it sees, and kStart more for its start and
+// end.  Tiles lie one after another, a request's by group (a head of the expanded
+// form; of the absorbed one 128 heads) and then by token; a worker's share may start
+// and end inside a tile, whose parts join_kernel puts together.
+constexpr int kStart = 128;
+// Fewest units of a worker.
+constexpr int kLeast = 384;
+
+struct Header {     // written by the schedule kernel, one for each form
+  int64_t units;    // of all tiles
+  int64_t share;    // units of a worker
+  int32_t more;     // workers that have one more
+  int32_t workers;  // that share them
+  int32_t lost;     // more tokens to expand than there is room for
 };
+
+struct Lists {
+  Header* header;
+  int64_t* base;   // [requests + 1] first unit of each request
+  int32_t* start;  // [workers] request of a worker's first unit
+  float* part;     // [workers * splits * 2] partial results, see slot_floats
+};
+
+// Tiles of one form: tokens and groups of a request, and how a row of a tile is one
+// of (token, head).
+struct Tiling {
+  int per;      // tokens of a tile
+  int groups;   // tiles of the same tokens
+  int splits;   // blocks that share a tile's values
+  int workers;  // most
+};
+__host__ __device__ inline Tiling absorbed_tiling(int heads, int latent, int sms) {
+  const int splits = latent > 256 ? latent / 256 : 1;
+  return {heads <= kRows ? kRows / heads : 1, heads <= kRows ? 1 : (heads + kRows - 1) / kRows,
+          splits, sms / splits};
+}
+__host__ __device__ inline Tiling expanded_tiling(int heads, int sms) {
+  return {2 * kRows, heads, 1, sms};
+}
+// fp32 of a partial result: [rows][values], then [rows][4] of reference exponent, sum,
+// sum of the rounded weights.
+__host__ __device__ constexpr int slot_floats(int rows, int values) { return rows * (values + 4); }
 
 // Byte offsets in the work area, which follow from the plan's sizes alone.
 struct Shape {
-  int64_t off_base, off_keys, off_values, bytes;
-};
-
-struct Work {
-  Header* header;
-  int32_t* base;     // [requests + 1] first expanded token of each request
-  uint16_t* keys;    // [heads][expand_tokens][nope]
-  uint16_t* values;  // [heads][expand_tokens][value]
+  Tiling tiling[2];  // absorbed, expanded
+  int64_t off_header[2], off_base[2], off_start[2];
+  int64_t off_part, off_room, off_keys, off_values, bytes;
 };
 
 int make_shape(const grm_b200_latent_plan& p, int sms, Shape* s);
-inline Work work_of(const Shape& s, void* work) {
+
+inline Lists lists_of(const Shape& s, int form, void* work) {
   char* b = static_cast<char*>(work);
-  return {reinterpret_cast<Header*>(b), reinterpret_cast<int32_t*>(b + s.off_base),
-          reinterpret_cast<uint16_t*>(b + s.off_keys),
-          reinterpret_cast<uint16_t*>(b + s.off_values)};
+  return {reinterpret_cast<Header*>(b + s.off_header[form]),
+          reinterpret_cast<int64_t*>(b + s.off_base[form]),
+          reinterpret_cast<int32_t*>(b + s.off_start[form]),
+          reinterpret_cast<float*>(b + s.off_part)};
 }
 
 struct Params {
-  Work w;
+  Lists l;
+  Tiling tiling;
+  unsigned probes;    // of a bounded wait: paged::kProbes, or less by GRM_B200_WAIT_LIMIT
+  const int32_t* room;  // [requests + 1] first expanded token of each request
+  uint16_t* keys;       // [heads][expand_tokens][2 * nope]: rounded, and what that left over
+  uint16_t* values;     // [heads][expand_tokens][value]
   const int32_t* table;
   const int32_t* lens;
   const int32_t* starts;
   int64_t requests, width, tokens, pages, expand_tokens;
-  int page_shift, heads, latent, rope, nope, value, causal;
+  int page_shift, heads, latent, rope, nope, causal, grow, dtype;
   const uint16_t* cache;
-  const uint16_t* q;      // absorbed: the latent part; expanded: nope + rope values
+  const uint16_t* q;  // absorbed: the latent part; expanded: nope + rope values
   int64_t q_row, q_head;
-  const uint16_t* qr;     // the positional part
+  const uint16_t* qr;  // the positional part
   int64_t qr_row, qr_head;
   const uint16_t* weights;
   int64_t w_head, w_row;
@@ -54,8 +101,144 @@ struct Params {
   int32_t* status;
 };
 
-int launch_absorbed(int dtype, const Params& p, cudaStream_t st);
-int launch_expanded(int dtype, const Params& p, cudaStream_t st);
+int launch_absorbed(const Params& p, cudaStream_t st);
+int launch_expanded(const Params& p, cudaStream_t st);
+int launch_expand(const Params& p, cudaStream_t st);
+
+// cuTensorMapEncodeTiled of 16-bit rows: `rank` dims (2 or 3), strides of all but the
+// first in elements.  The innermost box is 64 values (128-byte swizzle) or 32 (64).
+int make_map(CUtensorMap* map, const void* base, int rank, const int64_t* dims,
+             const int64_t* strides, const int* box);
+
+// ---- the shares
+
+__host__ __device__ inline int64_t worker_first(int64_t w, const Header& h) {
+  return w * h.share + (w < h.more ? w : h.more);
+}
+__host__ __device__ inline int worker_of(int64_t u, const Header& h) {
+  const int64_t big = h.more * (h.share + 1);
+  return (int)(u < big ? u / (h.share + 1) : h.more + (u - big) / h.share);
+}
+
+template <typename I>
+__host__ __device__ __forceinline__ I imin(I a, I b) {
+  return a < b ? a : b;
+}
+
+// Units of the first j tiles of a group: tile i sees cached + (i + 1) * per tokens of
+// a causal step, but no more than len.
+struct Request {
+  int start, n, len, cached, tiles;
+  int64_t total;  // units of a group
+};
+__host__ __device__ __forceinline__ int64_t units_before(const Request& q, int per, int grow, int j) {
+  if (!grow) return (int64_t)j * (q.len + kStart);
+  const int64_t u = (int64_t)j * (q.cached + kStart) + (int64_t)per * j * (j + 1) / 2;
+  return j < q.tiles ? u : u - ((int64_t)q.tiles * per - q.n);
+}
+__host__ __device__ __forceinline__ Request request_of(int start, int next, int len, int per, int grow) {
+  Request q{start, next - start, len, 0, 0, 0};
+  q.cached = grow ? len - q.n : len;
+  q.tiles = (q.n + per - 1) / per;
+  q.total = units_before(q, per, grow, q.tiles);
+  return q;
+}
+
+// The tile that holds a unit, and on from there.
+struct Walk {
+  int r, g, j;
+  Request q;
+  int64_t first, last;  // units of the tile
+
+  __host__ __device__ __forceinline__ void enter(const Params& p, int request) {
+    r = request;
+    q = request_of(p.starts[r], p.starts[r + 1], p.lens[r], p.tiling.per, p.grow);
+  }
+  __host__ __device__ __forceinline__ void bound(const Params& p) {
+    const int64_t at = p.l.base[r] + (int64_t)g * q.total;
+    first = at + units_before(q, p.tiling.per, p.grow, j);
+    last = at + units_before(q, p.tiling.per, p.grow, j + 1);
+  }
+  __host__ __device__ __forceinline__ void seek(const Params& p, int64_t u, int request) {
+    enter(p, request);
+    const int64_t x = u - p.l.base[r];
+    g = (int)(x / q.total);
+    const int64_t y = x - g * q.total;
+    int lo = 0, hi = q.tiles;  // the last tile that starts at y or before
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (units_before(q, p.tiling.per, p.grow, mid) <= y) lo = mid;
+      else hi = mid;
+    }
+    j = lo;
+    bound(p);
+  }
+  __host__ __device__ __forceinline__ void next(const Params& p) {  // there is one
+    if (++j == q.tiles) {
+      j = 0;
+      if (++g == p.tiling.groups) {
+        g = 0;
+        // the next request that has units
+        int lo = r + 1;
+        if (p.l.base[lo + 1] <= last) {
+          int hi = (int)p.requests;
+          while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (p.l.base[mid] <= last) lo = mid;
+            else hi = mid;
+          }
+        }
+        enter(p, lo);
+      }
+    }
+    bound(p);
+  }
+};
+
+// A worker's part of a tile.
+struct Part {
+  int r, g, tok0;       // request, group, first token of the tile within the step
+  int toks[2];          // tokens of the two query tiles (the second one's: expanded form)
+  int start, n, cached, len;
+  int step0, steps;     // of kStep tokens
+  int slot;             // where its result goes, -1: it is the whole tile's
+};
+
+// The parts of worker `w`, one after another.
+template <int QUERIES>
+struct Parts {
+  Walk walk;
+  int64_t u, end;
+  int w, count;
+
+  __host__ __device__ __forceinline__ Parts(const Params& p, const Header& h, int worker)
+      : u(worker_first(worker, h)), end(worker_first(worker + 1, h)), w(worker), count(0) {}
+  __host__ __device__ __forceinline__ bool next(const Params& p, Part* x) {
+    if (u >= end) return false;
+    if (count == 0) walk.seek(p, u, p.l.start[w]);
+    else walk.next(p);
+    x->r = walk.r;
+    x->g = walk.g;
+    x->start = walk.q.start;
+    x->n = walk.q.n;
+    x->cached = walk.q.cached;
+    x->len = walk.q.len;
+    x->tok0 = walk.j * p.tiling.per;
+    const int toks = imin(p.tiling.per, x->n - x->tok0);
+    x->toks[0] = QUERIES == 2 ? imin(toks, kRows) : toks;
+    x->toks[1] = QUERIES == 2 ? toks - x->toks[0] : 0;
+    const int sees = p.causal ? imin(x->len, x->cached + x->tok0 + toks) : x->len;
+    const int all = (sees + kStep - 1) / kStep;
+    const int64_t units = walk.last - walk.first;
+    const int64_t from = u - walk.first, to = imin(end, walk.last) - walk.first;
+    x->step0 = (int)(all * from / units);
+    x->steps = (int)(all * to / units) - x->step0;
+    x->slot = from == 0 && to == units ? -1 : 2 * w + (count > 0 ? 1 : 0);
+    u = imin(end, walk.last);
+    ++count;
+    return true;
+  }
+};
 
 }  // namespace latent
 }  // namespace grm_b200

@@ -1,185 +1,815 @@
-// latent_attend.cu -- attention over pages of latent rows, in its simplest form: a
-// block for each query row and head walks the tokens that the row sees, 128 at a
-// time, with the running maximum and sum of the softmax.
+// latent_attend.cu -- latent attention over pages of rows (c_t, r_t), both forms.
+//
+// With y_t = scale * log2(e) * (q . k_t) and the reference exponent m of a row,
+//   p_t = 2^(y_t - m),  out = sum_t p_t v_t / sum_t p_t,  lse = ln 2 (m + log2 sum_t p_t).
+// Absorbed: k_t = (c_t, r_t) and v_t = c_t, the same for all heads, so that a tile of
+// 128 rows is several heads of a few tokens and one copy of a token's row serves its
+// keys and its values.  Expanded: k_t and v_t are one head's (latent_expand.cu has made
+// them), and a block takes 2 x 128 tokens of it.  There k_t is held as two numbers of
+// the arena's type, the rounded key and what that left over, and multiplied twice:
+// with the first alone a score is off by 2^-9 of its products' size, which the log-sum
+// of a row of few tokens shows (1e-3 of it).  Values are rounded to the type, as
+// weights are, which the result's own rounding covers.
+//
+// A block's warps:
+//   4 a query tile  softmax, one row a thread: 64 scores from tensor memory, weights back
+//                   over them in the arena's type, and when a row's reference exponent
+//                   has to move (rarely: it trails by up to 8), its result rescaled
+//   1 a query tile  its products, issued by one elected lane: S = Q K^T, O += P V
+//   1               rows from their pages to shared memory by tensor-map copies, 64
+//                   tokens a stage, as many stages as there is room for
+// Scores are in two buffers of 64 tokens, so that products run under a softmax.
+// Queries are in tensor memory where there is room beside scores and results, so that
+// the products read keys and values alone from shared memory.  A result of 512 values
+// would take all of tensor memory: two blocks take 256 values each there and both
+// work out the scores.
+//
+// Work is shared by units (latent.cuh): a worker goes from tile to tile, its copies
+// running ahead over their borders, and leaves parts of the tiles at its ends for
+// join_kernel.
+//
+// Tokens that a row does not see have weight 0, and a product of 0 and what is no
+// number would be none: where a hidden token's score is not finite, the numbers of
+// its values that are not are set to 0 in shared memory before the weights go out
+// (scrub).
+#include <algorithm>
+#include <type_traits>
+
 #include "latent.cuh"
+#include "umma.cuh"
 
 namespace grm_b200 {
 namespace latent {
 
 namespace {
 
-constexpr int kThreads = 128;
+using paged::ex2;
+using paged::kLazy;
+using paged::kProbes;
+using paged::reference_of;
+
+constexpr int kAtom = kStep * 128;       // 64 tokens x 64 values
+constexpr int kQueryAtom = kRows * 128;  // 128 rows x 64 values
+constexpr uint32_t kTmemCols = 512;
+constexpr int kShared = 232448 - 1024;   // dynamic shared memory beside the barriers
+
+template <int MAIN, int ROPE, bool EXP>
+struct Layout {
+  static constexpr int kQueries = EXP ? 2 : 1;
+  static constexpr int kV = EXP || MAIN <= 256 ? MAIN : 256;  // values of a block's results
+  static constexpr int kSplits = MAIN / kV;
+  static constexpr int kAtoms = MAIN / 64;
+  static constexpr int kKeyAtoms = EXP ? 2 * kAtoms : kAtoms;
+  // a stage: keys, positional part, values where they are not the keys
+  static constexpr int kRopeAt = kKeyAtoms * kAtom;
+  static constexpr int kRopeBytes = kStep * ROPE * 2;
+  static constexpr int kValueAt = EXP ? kRopeAt + kRopeBytes : 0;
+  static constexpr int kStage = kRopeAt + kRopeBytes + (EXP ? kAtoms * kAtom : 0);
+  // tensor memory: scores, results, and queries in what is left
+  static constexpr int kFree = (int)kTmemCols - kQueries * (2 * kStep + kV);
+  static constexpr int kQTmem =
+      kFree / kQueries * 2 >= MAIN ? MAIN : kFree / kQueries * 2 / 64 * 64;
+  static constexpr uint32_t kScore = 0;
+  static constexpr uint32_t kResult = kQueries * 2 * kStep;
+  static constexpr uint32_t kQueryCol = kResult + kQueries * kV;
+  // the rest of the queries in shared memory, the positional part last
+  static constexpr int kQRopeAt = (MAIN - kQTmem) / 64 * kQueryAtom;
+  static constexpr int kQuery = kQRopeAt + kRows * ROPE * 2;
+  static constexpr int kFit = (kShared - 1024 - kQueries * kQuery) / kStage;
+  static constexpr int kStages = kFit > 8 ? 8 : kFit;
+  static constexpr int kUsed = 1024 + kQueries * kQuery + kStages * kStage;
+  // one block an SM: it owns all of tensor memory
+  static constexpr int kSmem = kUsed > 120 * 1024 ? kUsed : 120 * 1024;
+  static constexpr int kSoftWarps = 4 * kQueries;
+  static constexpr int kMmaWarp = kSoftWarps;
+  static constexpr int kLoadWarp = kMmaWarp + kQueries;
+  static constexpr int kThreads = (kLoadWarp + 1) * 32;
+  static constexpr int kSlot = slot_floats(kRows * kQueries, kV);
+  static_assert(kQueryCol + kQueries * kQTmem / 2 <= kTmemCols && kStages >= 2, "tiles");
+};
 
 template <typename T>
-__device__ __forceinline__ float value_of(uint16_t v);
+struct Kind;
 template <>
-__device__ __forceinline__ float value_of<__half>(uint16_t v) {
-  return __half2float(__ushort_as_half(v));
-}
+struct Kind<__half> {
+  static constexpr uint32_t kFormat = 0;
+  // Weights times 2^7, at most 2^15: lost at the small end is then what lies below
+  // 2^-32 of a row's largest, not 2^-25.
+  static constexpr float kLift = paged::kLift;
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    return paged::pack_half2(a, b);
+  }
+  static __device__ __forceinline__ float2 widen(uint32_t v) {
+    return __half22float2(*reinterpret_cast<const __half2*>(&v));
+  }
+  static constexpr uint32_t kNoNumber = 0x7C00u;  // exponent bits
+};
 template <>
-__device__ __forceinline__ float value_of<__nv_bfloat16>(uint16_t v) {
-  return __uint_as_float((unsigned)v << 16);
-}
+struct Kind<__nv_bfloat16> {
+  static constexpr uint32_t kFormat = (1u << 7) | (1u << 10);
+  static constexpr float kLift = 0.0f;
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    return paged::pack_out<__nv_bfloat16>(a, b);
+  }
+  static __device__ __forceinline__ float2 widen(uint32_t v) {
+    return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xFFFF0000u));
+  }
+  static constexpr uint32_t kNoNumber = 0x7F80u;
+};
+
+// fp32 accumulators, 16-bit operands, 128 rows, n columns; B K-major or (b_mn) not.
 template <typename T>
-__device__ __forceinline__ uint16_t bits_of(float v);
-template <>
-__device__ __forceinline__ uint16_t bits_of<__half>(float v) {
-  return __half_as_ushort(__float2half_rn(v));
-}
-template <>
-__device__ __forceinline__ uint16_t bits_of<__nv_bfloat16>(float v) {
-  return __bfloat16_as_ushort(__float2bfloat16_rn(v));
+__host__ __device__ constexpr uint32_t idesc(int n, bool b_mn) {
+  return (1u << 4) | Kind<T>::kFormat | (b_mn ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) |
+         ((uint32_t)(kRows >> 4) << 24);
 }
 
-__device__ __forceinline__ const uint16_t* row_of(const Params& p, int64_t r, int t) {
-  const int last = (1 << p.page_shift) - 1;
-  const int page = min(max(p.table[r * p.width + (t >> p.page_shift)], 0), (int)p.pages - 1);
-  return p.cache + (((int64_t)page << p.page_shift) + (t & last)) * (p.latent + p.rope);
+// Byte of 16-byte chunk c of row r: 128-byte rows of 8 chunks, 64-byte rows of 4.
+__device__ __forceinline__ uint32_t atom_byte(int r, int c) {
+  return r * 128 + ((c ^ (r & 7)) << 4);
+}
+__device__ __forceinline__ uint32_t half_atom_byte(int r, int c) {
+  return r * 64 + ((c ^ ((r >> 1) & 3)) << 4);
 }
 
-// Request of packed row x: the last whose first row is not past it.
-__device__ __forceinline__ int64_t request_of(const Params& p, int64_t x) {
-  int64_t lo = 0, hi = p.requests;
-  while (hi - lo > 1) {
-    const int64_t mid = (lo + hi) >> 1;
-    if (p.starts[mid] <= x) lo = mid;
-    else hi = mid;
+// Upper word of a shared-memory descriptor (umma.cuh's sw128_desc): 8-row groups of
+// 1024 bytes and a 128-byte swizzle, or of 512 and 64.
+constexpr uint32_t kHi128 = (uint32_t)(((uint64_t)64 << 32 | (uint64_t)1 << 46 |
+                                        (uint64_t)2 << 61) >> 32);
+constexpr uint32_t kHi64 = (uint32_t)(((uint64_t)32 << 32 | (uint64_t)1 << 46 |
+                                       (uint64_t)4 << 61) >> 32);
+
+__device__ __forceinline__ void tma_load(void* dst, const CUtensorMap* map, int x, int y,
+                                         uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3}], [%4];" ::"r"(smem_u32(dst)),
+      "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar))
+      : "memory");
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// Two numbers at a time.
+__device__ __forceinline__ float2 fma2(float a, float b, float k, float o) {
+  float2 r;
+  asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %4};\n"
+      " mov.b64 z, {%5, %5};\n fma.rn.f32x2 x, x, y, z;\n mov.b64 {%0, %1}, x;\n}\n"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a), "f"(b), "f"(k), "f"(o));
+  return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n .reg .b64 x, y;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n"
+      " add.rn.f32x2 x, x, y;\n mov.b64 {%0, %1}, x;\n}\n"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+
+// Every lane of a warp waits; false, for all of them, when a wait gave up.
+__device__ __noinline__ bool wait_long(uint64_t* bar, unsigned parity, volatile int* fail,
+                                       unsigned probes) {
+  bool ok = false;
+  for (unsigned i = 0; i < probes; ++i) {
+    if ((ok = mbar_try_wait(bar, parity))) break;
+    if (*fail) break;
   }
-  return lo;
+  ok = __all_sync(kFull, ok);
+  if (!ok) *fail = 1;
+  return ok;
+}
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, unsigned parity, volatile int* fail,
+                                          unsigned probes) {
+  if (__all_sync(kFull, mbar_try_wait(bar, parity))) return true;
+  return wait_long(bar, parity, fail, probes);
 }
 
-template <typename T, bool EXPANDED>
-__global__ void __launch_bounds__(kThreads) attend_kernel(const Params p) {
-  __shared__ float q[512 + 64], weight[kThreads], red[4];
-  const int64_t x = blockIdx.x / p.heads;
-  const int h = blockIdx.x % p.heads, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int wide = EXPANDED ? p.value : p.latent, main = EXPANDED ? p.nope : p.latent;
-  const int64_t orow = x * p.heads + h;
-  int n = 0;
-  int64_t r = 0;
-  if (x < p.starts[p.requests]) {
-    r = request_of(p, x);
-    n = p.lens[r];
-    if (p.causal) n = n - (p.starts[r + 1] - p.starts[r]) + (int)(x - p.starts[r]) + 1;
+// Row of query tile t: its token within the step, its head, and whether there is one.
+struct Row {
+  int token, head;
+  bool active;
+};
+template <bool EXP>
+__device__ __forceinline__ Row row_of(const Params& p, const Part& x, int t, int row) {
+  if (EXP) return {x.tok0 + t * kRows + row, x.g, row < x.toks[t]};
+  if (p.tiling.groups > 1) {
+    const int h = x.g * kRows + row;
+    return {x.tok0, min(h, p.heads - 1), h < p.heads};
   }
-  for (int i = tid; i < main; i += kThreads)
-    q[i] = value_of<T>(p.q[x * p.q_row + h * p.q_head + i]);
-  for (int i = tid; i < p.rope; i += kThreads)
-    q[main + i] = value_of<T>(p.qr[x * p.qr_row + h * p.qr_head + i]);
-  __syncthreads();
-  const bool lost = EXPANDED && p.w.header->overflow;
-  const int64_t base = EXPANDED && !lost ? p.w.base[r] : 0;
-  if (lost && n > 0) n = 1;
-  float m = -INFINITY, l = 0.0f, acc[4] = {};
-  for (int t0 = 0; t0 < n; t0 += kThreads) {
-    const int t = t0 + tid;
-    float s = -INFINITY;
-    if (t < n && !lost) {
-      const uint16_t* row = row_of(p, r, t);
-      const uint16_t* k = EXPANDED ? p.w.keys + ((int64_t)h * p.expand_tokens + base + t) * main
-                                   : row;
-      float y = 0.0f;
-      for (int i = 0; i < main; ++i) y = fmaf(q[i], value_of<T>(k[i]), y);
-      for (int i = 0; i < p.rope; ++i) y = fmaf(q[main + i], value_of<T>(row[p.latent + i]), y);
-      s = y * p.scale_log2;
-    }
-    if (lost) s = __int_as_float(0x7FC00000);
-    float top = s;
-    for (int o = 16; o; o >>= 1) {
-      const float u = __shfl_xor_sync(kFull, top, o);
-      top = u > top || u != u ? u : top;
-    }
-    if (lane == 0) red[warp] = top;
-    __syncthreads();
-    for (int w = 0; w < 4; ++w) top = red[w] > top || red[w] != red[w] ? red[w] : top;
-    const float next = top > m || top != top ? top : m;
-    const float ref = next == -INFINITY ? 0.0f : next;
-    const float a = paged::ex2(m - ref), e = paged::ex2(s - ref);
-    weight[tid] = e;
-    m = next;
-    float sum = e;
-    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
-    __syncthreads();
-    if (lane == 0) red[warp] = sum;
-    __syncthreads();
-    l = l * a + ((red[0] + red[1]) + (red[2] + red[3]));
+  const int token = row / p.heads;
+  return {x.tok0 + token, row - token * p.heads, token < x.toks[0]};
+}
+
+// Numbers that are none among the V values of token `t` of a stage set to 0.
+template <typename T, int V>
+__device__ __noinline__ void scrub(unsigned char* values, unsigned long long tokens) {
+  while (tokens) {
+    const int t = __ffsll((long long)tokens) - 1;
+    tokens &= tokens - 1;
+    for (int c = 0; c < V / 8; ++c) {
+      uint4* at = reinterpret_cast<uint4*>(values + (c / 8) * kAtom + atom_byte(t, c % 8));
+      const uint4 v = *at;
+      uint32_t x[4] = {v.x, v.y, v.z, v.w};
+      bool bad = false;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int d = tid + j * kThreads;
-      if (d < wide) {
-        float y = acc[j] * a;
-        for (int i = 0; i < min(kThreads, n - t0) && !lost; ++i) {
-          const uint16_t* v =
-              EXPANDED ? p.w.values + ((int64_t)h * p.expand_tokens + base + t0 + i) * wide
-                       : row_of(p, r, t0 + i);
-          y = fmaf(weight[i], value_of<T>(v[d]), y);
-        }
-        acc[j] = y;
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t e = Kind<T>::kNoNumber;
+        if ((x[i] & e) == e) { x[i] &= 0xFFFF0000u; bad = true; }
+        if ((x[i] >> 16 & e) == e) { x[i] &= 0x0000FFFFu; bad = true; }
+      }
+      if (bad) *at = make_uint4(x[0], x[1], x[2], x[3]);
+    }
+  }
+}
+
+// The rows of a worker in which a wait gave up: no numbers.
+template <int MAIN, int ROPE, bool EXP>
+__device__ __noinline__ void lose_rows(const Params& p, const Header& hd, int worker, int split) {
+  using LY = Layout<MAIN, ROPE, EXP>;
+  const float nan = __int_as_float(0x7FC00000);
+  const int t = threadIdx.x >> 7, row = threadIdx.x & 127;
+  Parts<LY::kQueries> parts(p, hd, worker);
+  Part x;
+  while (parts.next(p, &x)) {
+    const Row a = row_of<EXP>(p, x, t, row);
+    if (x.slot >= 0) {
+      float* slot = p.l.part + ((int64_t)x.slot * LY::kSplits + split) * LY::kSlot;
+      *reinterpret_cast<float4*>(slot + kRows * LY::kQueries * LY::kV + 4 * (t * kRows + row)) =
+          make_float4(-INFINITY, nan, nan, 0.0f);
+    } else if (a.active) {
+      const int64_t orow = (int64_t)(x.start + a.token) * p.heads + a.head;
+      for (int c = 0; c < LY::kV / 8; ++c)
+        reinterpret_cast<uint4*>(p.out + orow * MAIN + split * LY::kV)[c] =
+            make_uint4(0x7FFF7FFFu, 0x7FFF7FFFu, 0x7FFF7FFFu, 0x7FFF7FFFu);
+      if (p.lse && split == 0) p.lse[orow] = nan;
+    }
+  }
+}
+
+struct Maps {
+  CUtensorMap main;    // absorbed: 64 values of rows of the cache; expanded: of its keys
+  CUtensorMap rope;    // the positional part of rows of the cache
+  CUtensorMap values;  // expanded: 64 values of its values
+};
+
+template <typename T, int MAIN, int ROPE, bool EXP>
+__global__ void __launch_bounds__(Layout<MAIN, ROPE, EXP>::kThreads, 1)
+    attend_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) {
+  using LY = Layout<MAIN, ROPE, EXP>;
+  constexpr int kStages = LY::kStages, kQ = LY::kQueries;
+  extern __shared__ unsigned char raw[];
+  unsigned char* const sm = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
+  unsigned char* const sm_q = sm;                         // [kQ]
+  unsigned char* const sm_stage = sm + kQ * LY::kQuery;   // [kStages]
+  __shared__ __align__(8) uint64_t full[kStages], empty[kStages], q_full[kQ], drained[kQ],
+      s_full[kQ][2], p_full[kQ][2], o_full[kQ], o_done[kQ];
+  __shared__ uint32_t sh_tmem;
+  __shared__ int sh_fail;
+
+  const Header hd = *p.l.header;
+  const int worker = blockIdx.x / LY::kSplits, split = blockIdx.x % LY::kSplits;
+  asm volatile("griddepcontrol.launch_dependents;");
+  if (worker >= hd.workers) return;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (EXP && hd.lost) {
+    if (warp < LY::kSoftWarps) lose_rows<MAIN, ROPE, EXP>(p, hd, worker, split);
+    return;
+  }
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], kQ);
+    }
+    for (int t = 0; t < kQ; ++t) {
+      mbar_init(&q_full[t], 4);
+      mbar_init(&drained[t], 1);
+      mbar_init(&o_full[t], 1);
+      mbar_init(&o_done[t], 1);
+      for (int x = 0; x < 2; ++x) {
+        mbar_init(&s_full[t][x], 1);
+        mbar_init(&p_full[t][x], 4);
       }
     }
-    __syncthreads();
+    mbar_fence_init();
+    sh_fail = 0;
+  }
+  if (warp == LY::kMmaWarp) {
+    tmem_alloc(&sh_tmem, kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sh_tmem;
+  auto wait = [&](uint64_t* bar, unsigned parity) {
+    return warp_wait(bar, parity, &sh_fail, p.probes);
+  };
+  Parts<kQ> parts(p, hd, worker);
+  Part x;
+
+  if (warp < LY::kSoftWarps) {
+    // ------------------------------------------------------------- softmax
+    const int t = warp >> 2, row = (warp & 3) * 32 + lane;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t s_col = tmem + lanes + LY::kScore + t * 2 * kStep;
+    const uint32_t o_col = tmem + lanes + LY::kResult + t * LY::kV;
+    const uint32_t q_col = tmem + lanes + LY::kQueryCol + t * (LY::kQTmem / 2);
+    unsigned char* const my_q = sm_q + t * LY::kQuery;
+    bool ok = true;
+    int it = 0, tile = 0, stage0 = 0;  // steps and tiles of this query tile; stages so far
+#pragma unroll 1
+    while (ok && parts.next(p, &x)) {
+      const int steps = x.steps, stage_base = stage0;
+      stage0 += steps;
+      if (x.toks[t] == 0) continue;
+      const Row a = row_of<EXP>(p, x, t, row);
+      float m = -INFINITY, l = 0.0f, lr = 0.0f;
+      if (steps > 0) {
+        // the row's query, to tensor memory and shared memory
+        const uint16_t* qp = p.q + (int64_t)(x.start + a.token) * p.q_row + a.head * p.q_head;
+        const uint16_t* rp = p.qr + (int64_t)(x.start + a.token) * p.qr_row + a.head * p.qr_head;
+        auto chunk = [&](const uint16_t* from, int c) {
+          return a.active ? __ldg(reinterpret_cast<const uint4*>(from) + c)
+                          : make_uint4(0, 0, 0, 0);
+        };
+#pragma unroll 2
+        for (int c = 0; c < LY::kQTmem / 8; c += 4) {
+          uint32_t w[16];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint4 v = chunk(qp, c + i);
+            w[4 * i] = v.x;
+            w[4 * i + 1] = v.y;
+            w[4 * i + 2] = v.z;
+            w[4 * i + 3] = v.w;
+          }
+          tmem_st16(q_col + 4 * c, w);
+        }
+#pragma unroll 4
+        for (int c = LY::kQTmem / 8; c < MAIN / 8; ++c) {
+          const int y = c - LY::kQTmem / 8;
+          *reinterpret_cast<uint4*>(my_q + (y / 8) * kQueryAtom + atom_byte(row, y % 8)) =
+              chunk(qp, c);
+        }
+#pragma unroll
+        for (int c = 0; c < ROPE / 8; ++c)
+          *reinterpret_cast<uint4*>(my_q + LY::kQRopeAt +
+                                    (ROPE == 64 ? atom_byte(row, c) : half_atom_byte(row, c))) =
+              chunk(rp, c);
+        tmem_wait_st();
+        tc_fence_before();
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&q_full[t]);
+      }
+
+      // tokens that the row sees, from the part's first on
+      const int lim = (p.causal ? min(x.len, x.cached + a.token + 1) : x.len) - x.step0 * kStep;
+      const bool idle = !__any_sync(kFull, a.active);
+#pragma unroll 1
+      for (int i = 0; i < steps; ++i, ++it) {
+        const int buf = it & 1;
+        if (!(ok = wait(&s_full[t][buf], (it >> 1) & 1))) break;
+        tc_fence_after();
+        if (idle) {
+          if (lane == 0) mbar_arrive(&p_full[t][buf]);
+          continue;
+        }
+        uint32_t v[2][32];
+        tmem_ld32_nowait(s_col + buf * kStep, v[0]);
+        tmem_ld32_nowait(s_col + buf * kStep + 32, v[1]);
+        tmem_wait_ld32(v[0]);
+        tmem_wait_ld32(v[1]);
+        if (__any_sync(kFull, (i + 1) * kStep > lim)) {
+          unsigned bad[2] = {0, 0};
+#pragma unroll
+          for (int k = 0; k < kStep; ++k)
+            if (i * kStep + k >= lim) {
+              if ((v[k / 32][k % 32] & 0x7F800000u) == 0x7F800000u) bad[k / 32] |= 1u << (k % 32);
+              v[k / 32][k % 32] = 0xFF800000u;
+            }
+          if (__any_sync(kFull, (bad[0] | bad[1]) != 0)) {
+            const int st = stage_base + i;  // its copies landed before the scores were there
+            if (!(ok = wait(&full[st % kStages], (st / kStages) & 1))) break;
+            unsigned char* at = sm_stage + st % kStages * LY::kStage +
+                                LY::kValueAt + split * (LY::kV / 64) * kAtom;
+            scrub<T, LY::kV>(at, (unsigned long long)bad[1] << 32 | bad[0]);
+            fence_proxy_async_smem();
+          }
+        }
+        float top = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < kStep; k += 2)
+          top = max3(top, __uint_as_float(v[k / 32][k % 32]),
+                     __uint_as_float(v[k / 32][k % 32 + 1]));
+        top *= p.scale_log2;
+        if (__any_sync(kFull, top > m + kLazy)) {
+          const float next = top > m + kLazy ? reference_of(top) : m;
+          const float f = next == m ? 1.0f : ex2(m - next);
+          m = next;
+          l *= f;
+          lr *= f;
+          if (i > 0) {  // once the products of the step before have ended
+            if (!(ok = wait(&o_full[t], (it - 1) & 1))) break;
+            tc_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < LY::kV / 16; ++c) {
+              uint32_t o[16];
+              tmem_ld16(o_col + 16 * c, o);
+#pragma unroll
+              for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+              tmem_st16(o_col + 16 * c, o);
+            }
+          }
+        }
+        const float off = m == -INFINITY ? 0.0f : Kind<T>::kLift - m;
+        float2 sum = make_float2(0.0f, 0.0f), rounded = make_float2(0.0f, 0.0f);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t w[16];
+#pragma unroll
+          for (int k = 0; k < 32; k += 2) {
+            const float2 y = fma2(__uint_as_float(v[c][k]), __uint_as_float(v[c][k + 1]),
+                                  p.scale_log2, off);
+            const float2 e = make_float2(ex2(y.x), ex2(y.y));
+            sum = add2(sum, e);
+            w[k / 2] = Kind<T>::pack(e.x, e.y);
+            rounded = add2(rounded, Kind<T>::widen(w[k / 2]));
+          }
+          tmem_st16(s_col + buf * kStep + 16 * c, w);
+        }
+        l += sum.x + sum.y;
+        lr += rounded.x + rounded.y;
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[t][buf]);
+      }
+      if (!ok) break;
+      if (steps > 0) {
+        if (!(ok = wait(&o_done[t], tile & 1))) break;
+        tc_fence_after();
+        ++tile;
+      }
+      const int64_t orow = (int64_t)(x.start + a.token) * p.heads + a.head;
+      if (x.slot >= 0) {  // a part's result, for join_kernel
+        float* slot = p.l.part + ((int64_t)x.slot * LY::kSplits + split) * LY::kSlot;
+        float4* to = reinterpret_cast<float4*>(slot + (t * kRows + row) * LY::kV);
+        if (steps > 0 && !idle)
+#pragma unroll 1
+          for (int c = 0; c < LY::kV / 16; ++c) {
+            uint32_t o[16];
+            tmem_ld16(o_col + 16 * c, o);
+            if (a.active)
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                to[4 * c + k] =
+                    make_float4(__uint_as_float(o[4 * k]), __uint_as_float(o[4 * k + 1]),
+                                __uint_as_float(o[4 * k + 2]), __uint_as_float(o[4 * k + 3]));
+          }
+        if (a.active)
+          *reinterpret_cast<float4*>(slot + kRows * kQ * LY::kV + 4 * (t * kRows + row)) =
+              make_float4(m, l, lr, 0.0f);
+      } else if (!idle) {
+        const float inv = lr == 0.0f ? 0.0f : 1.0f / lr;
+        uint16_t* out = p.out + orow * MAIN + split * LY::kV;
+#pragma unroll 1
+        for (int c = 0; c < LY::kV / 16; ++c) {
+          uint32_t o[16];
+          if (steps > 0) tmem_ld16(o_col + 16 * c, o);
+          if (a.active)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              uint32_t w[4];
+#pragma unroll
+              for (int y = 0; y < 4; ++y)
+                w[y] = lr == 0.0f ? 0u
+                                  : Kind<T>::pack(__uint_as_float(o[8 * k + 2 * y]) * inv,
+                                                  __uint_as_float(o[8 * k + 2 * y + 1]) * inv);
+              reinterpret_cast<uint4*>(out)[2 * c + k] = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+        }
+        if (a.active && p.lse && split == 0)
+          p.lse[orow] = l == 0.0f ? -INFINITY
+                                  : (m - Kind<T>::kLift + log2f(l)) * 0.693147180559945309f;
+      }
+      // what the next tile's products overwrite has been read
+      tc_fence_before();
+    }
+  } else if (warp < LY::kLoadWarp) {
+    // ---------------------------------------------------------- products
+    // The whole warp runs this, an elected lane issues; what the instructions read is
+    // the same in every lane and known to be (broadcast), so that it stays in uniform
+    // registers.
+    const int t = __shfl_sync(kFull, warp, 0) - LY::kMmaWarp;
+    const uint32_t base = __shfl_sync(kFull, tmem, 0);
+    const uint32_t s_at = base + LY::kScore + t * 2 * kStep;
+    const uint32_t o_at = base + LY::kResult + t * LY::kV;
+    const uint32_t q_at = base + LY::kQueryCol + t * (LY::kQTmem / 2);
+    const uint32_t q_lo = (uint32_t)sw128_desc(sm_q + t * LY::kQuery);
+    const uint32_t k_lo = (uint32_t)sw128_desc(sm_stage);
+    const uint32_t v_lo = (uint32_t)sw128_mn_desc(
+        sm_stage + LY::kValueAt + split * (LY::kV / 64) * kAtom, kAtom);
+    auto desc = [&](uint32_t hi, uint32_t lo) { return (uint64_t)hi << 32 | lo; };
+    int it = 0, tile = 0, stage0 = 0;
+    bool ok = true;
+    auto scores = [&](int i) {  // of the it + i-th step, in the stage of the part's i-th
+      const uint32_t kd = k_lo + (uint32_t)((stage0 + i) % kStages) * (LY::kStage / 16);
+      const uint32_t to = s_at + ((it + i) & 1) * kStep;
+      if (elect_one()) {
+#pragma unroll
+        for (int part = 0; part < LY::kKeyAtoms / LY::kAtoms; ++part)
+#pragma unroll
+          for (int k = 0; k < MAIN / 16; ++k) {
+            const uint32_t k_step = ((part * LY::kAtoms + k / 4) * kAtom + (k % 4) * 32) / 16;
+            if (16 * k < LY::kQTmem) {
+              umma_f16_ts(to, q_at + 8 * k, desc(kHi128, kd + k_step), idesc<T>(kStep, false),
+                          part + k != 0);
+            } else {
+              const int y = k - LY::kQTmem / 16;
+              umma_f16(to, desc(kHi128, q_lo + ((y / 4) * kQueryAtom + (y % 4) * 32) / 16),
+                       desc(kHi128, kd + k_step), idesc<T>(kStep, false), part + k != 0);
+            }
+          }
+#pragma unroll
+        for (int k = 0; k < ROPE / 16; ++k) {
+          constexpr uint32_t kHi = ROPE == 64 ? kHi128 : kHi64;
+          umma_f16(to, desc(kHi, q_lo + (LY::kQRopeAt + k * 32) / 16),
+                   desc(kHi, kd + (LY::kRopeAt + k * 32) / 16), idesc<T>(kStep, false), 1);
+        }
+        umma_commit(&s_full[t][(it + i) & 1]);
+      }
+      __syncwarp();
+    };
+    auto next_scores = [&](int i) {
+      const int s = stage0 + i;
+      if (!wait(&full[s % kStages], (s / kStages) & 1)) return false;
+      tc_fence_after();
+      scores(i);
+      return true;
+    };
+#pragma unroll 1
+    while (ok && parts.next(p, &x)) {
+      const int steps = __shfl_sync(kFull, x.steps, 0);
+      if (x.toks[t] == 0) {  // nothing to do for this one: give the stages back
+#pragma unroll 1
+        for (int i = 0; i < steps && ok; ++i) {
+          const int s = stage0 + i;
+          ok = wait(&full[s % kStages], (s / kStages) & 1);
+          if (ok && lane == 0) mbar_arrive(&empty[s % kStages]);
+          __syncwarp();
+        }
+        stage0 += steps;
+        continue;
+      }
+      if (steps == 0) continue;
+      ok = wait(&q_full[t], tile & 1);
+      if (!ok) break;
+      tc_fence_after();
+      ok = next_scores(0) && (steps < 2 || next_scores(1));
+#pragma unroll 1
+      for (int i = 0; i < steps && ok; ++i) {
+        const int s = (stage0 + i) % kStages, buf = (it + i) & 1;
+        if (!(ok = wait(&p_full[t][buf], ((it + i) >> 1) & 1))) break;
+        tc_fence_after();
+        const uint32_t vd = v_lo + (uint32_t)s * (LY::kStage / 16);
+        if (elect_one()) {
+#pragma unroll
+          for (int k = 0; k < kStep / 16; ++k)
+            umma_f16_ts(o_at, s_at + buf * kStep + 8 * k, desc(kHi128, vd + k * (16 * 128 / 16)),
+                        idesc<T>(LY::kV, true), i != 0 || k != 0);
+          umma_commit(&o_full[t]);
+          umma_commit(&empty[s]);
+          if (i + 1 == steps) umma_commit(&o_done[t]);
+        }
+        __syncwarp();
+        if (i + 2 < steps) ok = next_scores(i + 2);  // in this step's place
+      }
+      stage0 += steps;
+      it += steps;
+      ++tile;
+    }
+    // whatever happened, nothing is in flight when tensor memory is given back
+    if (elect_one()) umma_commit(&drained[t]);
+    __syncwarp();
+    mbar_wait(&drained[t], 0, kProbes);
+  } else {
+    // ------------------------------------------------ rows from their pages
+    const int piece = min(1 << p.page_shift, kStep);  // tokens of one copy
+    const int pieces = kStep / piece;
+    const int my_tok = lane % pieces * piece;
+    int s = 0;  // stages so far
+    // With no probes at all the block gives up here: nothing comes, and everybody's
+    // waits run out.
+    bool ok = p.probes > 0;
+#pragma unroll 1
+    while (ok && parts.next(p, &x)) {
+      const int last = (x.len - 1) >> p.page_shift;
+      auto row_at = [&](int i) {  // of this lane's piece of step i
+        const int tok = (x.step0 + i) * kStep + my_tok;
+        const int at = min(tok >> p.page_shift, last);  // past the end: the last page again
+        const int page = min(max(__ldg(p.table + x.r * p.width + at), 0), (int)p.pages - 1);
+        return (page << p.page_shift) + (tok & ((1 << p.page_shift) - 1));
+      };
+      int at = x.steps > 0 ? row_at(0) : 0;
+      int64_t room = 0;
+      if (EXP) room = (int64_t)x.g * p.expand_tokens + p.room[x.r];
+#pragma unroll 1
+      for (int i = 0; i < x.steps; ++i, ++s) {
+        const int st = s % kStages, to_row = at;
+        if (i + 1 < x.steps) at = row_at(i + 1);
+        if (s >= kStages && !(ok = wait(&empty[st], (s / kStages - 1) & 1))) break;
+        unsigned char* to = sm_stage + st * LY::kStage;
+        if (lane == 0) mbar_arrive_expect_tx(&full[st], LY::kStage);
+        __syncwarp();
+        if (EXP) {
+          const int row = (int)(room + (int64_t)(x.step0 + i) * kStep);
+          if (lane < LY::kKeyAtoms) tma_load(to + lane * kAtom, &maps.main, lane * 64, row, &full[st]);
+          if (lane < LY::kAtoms)
+            tma_load(to + LY::kValueAt + lane * kAtom, &maps.values, lane * 64, row, &full[st]);
+        } else {
+#pragma unroll
+          for (int y = lane; y < LY::kAtoms * 4; y += 32) {
+            const int atom = y / pieces;
+            if (atom < LY::kAtoms)
+              tma_load(to + atom * kAtom + my_tok * 128, &maps.main, atom * 64, to_row, &full[st]);
+          }
+        }
+        if (lane < pieces)
+          tma_load(to + LY::kRopeAt + my_tok * ROPE * 2, &maps.rope, p.latent, to_row, &full[st]);
+      }
+    }
+    // no copy is in flight when the block ends, whatever happened
+    for (int i = max(s - kStages, 0); i < s; ++i)
+      mbar_wait(&full[i % kStages], (i / kStages) & 1, kProbes);
+  }
+
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == LY::kMmaWarp) tmem_dealloc(tmem, kTmemCols);
+  if (sh_fail) {
+    if (warp < LY::kSoftWarps) lose_rows<MAIN, ROPE, EXP>(p, hd, worker, split);
+    if (threadIdx.x == 0) atomicOr(p.status, GRM_B200_PLAN_WAIT);
+  }
+}
+
+// Parts of tiles that lie in the shares of several workers, and the rows past the
+// step's last one.  Boundary b is where worker b's share starts; the first one inside a
+// tile joins it, a warp a row.
+template <typename T, int MAIN, int ROPE, bool EXP>
+__global__ void __launch_bounds__(256) join_kernel(const Params p) {
+  using LY = Layout<MAIN, ROPE, EXP>;
+  constexpr int kLanes = LY::kV / 4;  // float4 of a row
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const Header hd = *p.l.header;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t used = p.starts[p.requests];
+  const int64_t id = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 256 + threadIdx.x;
+  for (int64_t i = used * p.heads * (MAIN / 8) + id; i < p.tokens * p.heads * (MAIN / 8);
+       i += (int64_t)gridDim.x * gridDim.y * 256) {
+    reinterpret_cast<uint4*>(p.out)[i] = make_uint4(0, 0, 0, 0);
+    if (p.lse && i % (MAIN / 8) == 0) p.lse[i / (MAIN / 8)] = -INFINITY;
+  }
+  const int b = blockIdx.x / LY::kSplits + 1, split = blockIdx.x % LY::kSplits;
+  if (b >= hd.workers) return;
+  const int64_t u = worker_first(b, hd);
+  Walk walk;
+  walk.seek(p, u, p.l.start[b]);
+  const int64_t before = worker_first(b - 1, hd);
+  if (walk.first == u || walk.first < before) return;
+  Part x;
+  x.r = walk.r;
+  x.g = walk.g;
+  x.tok0 = walk.j * p.tiling.per;
+  const int toks = min(p.tiling.per, walk.q.n - x.tok0);
+  x.toks[0] = EXP ? min(toks, kRows) : toks;
+  x.toks[1] = EXP ? toks - x.toks[0] : 0;
+  const int line = blockIdx.y * 8 + warp;  // of the tile's rows
+  const Row a = row_of<EXP>(p, x, line / kRows, line % kRows);
+  if (!a.active) return;
+  const int slot0 = 2 * (b - 1) + (walk.first == before ? 0 : 1);
+  const int parts = worker_of(walk.last - 1, hd) - b + 2;
+  auto slot = [&](int k) {
+    const int at = k == 0 ? slot0 : 2 * (b - 1 + k);
+    return p.l.part + ((int64_t)at * LY::kSplits + split) * LY::kSlot;
+  };
+  auto state = [&](int k) {
+    return *reinterpret_cast<const float4*>(slot(k) + kRows * LY::kQueries * LY::kV + 4 * line);
+  };
+  // the largest reference exponent of the parts that see something, lanes side by side
+  float m = -INFINITY;
+  for (int k = lane; k < parts; k += 32) {
+    const float4 s = state(k);
+    if (s.y != 0.0f) m = fmaxf(m, s.x);
   }
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int d = tid + j * kThreads;
-    if (d < wide) p.out[orow * wide + d] = bits_of<T>(l == 0.0f ? 0.0f : acc[j] / l);
+  for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kFull, m, o));
+  float l = 0.0f, lr = 0.0f;
+  constexpr int kMine = (kLanes + 31) / 32;
+  float4 o[kMine] = {};
+  for (int k = 0; k < parts; ++k) {
+    const float4 s = state(k);
+    if (s.y == 0.0f) continue;
+    const float f = s.x == m ? 1.0f : ex2(s.x - m);
+    l = fmaf(s.y, f, l);
+    lr = fmaf(s.z, f, lr);
+    const float4* from = reinterpret_cast<const float4*>(slot(k) + line * LY::kV);
+#pragma unroll
+    for (int i = 0; i < kMine; ++i)
+      if (lane + 32 * i < kLanes) {
+        const float4 v = from[lane + 32 * i];
+        o[i].x = fmaf(v.x, f, o[i].x);
+        o[i].y = fmaf(v.y, f, o[i].y);
+        o[i].z = fmaf(v.z, f, o[i].z);
+        o[i].w = fmaf(v.w, f, o[i].w);
+      }
   }
-  if (tid == 0 && p.lse)
-    p.lse[orow] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.693147180559945309f;
+  const int64_t orow = (int64_t)(walk.q.start + a.token) * p.heads + a.head;
+  const float inv = 1.0f / lr;
+#pragma unroll
+  for (int i = 0; i < kMine; ++i)
+    if (lane + 32 * i < kLanes)
+      reinterpret_cast<uint2*>(p.out + orow * MAIN + split * LY::kV)[lane + 32 * i] =
+          lr == 0.0f ? make_uint2(0, 0)
+                     : make_uint2(Kind<T>::pack(o[i].x * inv, o[i].y * inv),
+                                  Kind<T>::pack(o[i].z * inv, o[i].w * inv));
+  if (lane == 0 && p.lse && split == 0)
+    p.lse[orow] =
+        l == 0.0f ? -INFINITY : (m - Kind<T>::kLift + log2f(l)) * 0.693147180559945309f;
 }
 
-// 64 tokens of a request and one head's keys or values: a thread an output.
-template <typename T>
-__global__ void __launch_bounds__(256) expand_kernel(const Params p) {
-  if (p.w.header->overflow) return;
-  const int64_t t0 = (int64_t)blockIdx.x * kExpandAlign;
-  if (t0 >= p.w.base[p.requests]) return;
-  int64_t lo = 0, hi = p.requests;
-  while (hi - lo > 1) {
-    const int64_t mid = (lo + hi) >> 1;
-    if (p.w.base[mid] <= t0) lo = mid;
-    else hi = mid;
+template <typename T, int MAIN, int ROPE, bool EXP>
+int launch(const Params& p, cudaStream_t st) {
+  using LY = Layout<MAIN, ROPE, EXP>;
+  Maps maps;
+  const int64_t width = p.latent + p.rope, slots = p.pages << p.page_shift;
+  const int64_t cache[2] = {width, slots};
+  const int tokens = std::min(1 << p.page_shift, kStep);
+  const int box[2] = {64, tokens}, rope[2] = {ROPE, tokens}, tile[2] = {64, kStep};
+  int rc = make_map(&maps.rope, p.cache, 2, cache, &width, rope);
+  if (EXP) {
+    const int64_t rows = (int64_t)p.heads * p.expand_tokens;
+    const int64_t keys[2] = {2 * MAIN, rows}, values[2] = {MAIN, rows};
+    if (rc || (rc = make_map(&maps.main, p.keys, 2, keys, keys, tile)) ||
+        (rc = make_map(&maps.values, p.values, 2, values, values, tile)))
+      return rc;
+  } else {
+    if (rc || (rc = make_map(&maps.main, p.cache, 2, cache, &width, box))) return rc;
+    maps.values = maps.main;
   }
-  const int h = blockIdx.y, n = p.nope + p.value;
-  for (int x = threadIdx.x; x < kExpandAlign * n; x += 256) {
-    const int j = x % n;
-    const int t = (int)(t0 - p.w.base[lo]) + x / n;
-    float y = 0.0f;
-    if (t < p.lens[lo]) {
-      const uint16_t* row = row_of(p, lo, t);
-      const uint16_t* w = p.weights + h * p.w_head + j * p.w_row;
-      for (int i = 0; i < p.latent; ++i) y = fmaf(value_of<T>(row[i]), value_of<T>(w[i]), y);
-    }
-    const int64_t at = (int64_t)h * p.expand_tokens + t0 + x / n;
-    if (j < p.nope) p.w.keys[at * p.nope + j] = bits_of<T>(y);
-    else p.w.values[at * p.value + j - p.nope] = bits_of<T>(y);
+  auto kernel = attend_kernel<T, MAIN, ROPE, EXP>;
+  static std::atomic<uint64_t> done{0};
+  if ((rc = paged::allow_shared(reinterpret_cast<const void*>(kernel), LY::kSmem, &done)))
+    return rc;
+  kernel<<<(unsigned)(p.tiling.workers * LY::kSplits), LY::kThreads, LY::kSmem, st>>>(maps, p);
+  if ((rc = paged::launch_status("latent attend"))) return rc;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(std::max(p.tiling.workers - 1, 1) * LY::kSplits),
+                     kRows * LY::kQueries / 8);
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, join_kernel<T, MAIN, ROPE, EXP>, p);
+  if (e != cudaSuccess) {
+    set_thread_error("latent join launch failed: %s", cudaGetErrorString(e));
+    return cuda_status(e);
   }
+  return 0;
 }
 
-template <typename T>
-int absorbed(const Params& p, cudaStream_t st) {
-  attend_kernel<T, false><<<(unsigned)(p.tokens * p.heads), kThreads, 0, st>>>(p);
-  return paged::launch_status("latent attend");
+template <int MAIN, int ROPE, bool EXP>
+int launch_kind(const Params& p, cudaStream_t st) {
+  return p.dtype == GRM_B200_F16 ? launch<__half, MAIN, ROPE, EXP>(p, st)
+                                 : launch<__nv_bfloat16, MAIN, ROPE, EXP>(p, st);
 }
 
-template <typename T>
-int expanded(const Params& p, cudaStream_t st) {
-  const dim3 grid((unsigned)ceil_div64(p.expand_tokens, kExpandAlign), p.heads);
-  expand_kernel<T><<<grid, 256, 0, st>>>(p);
-  const int rc = paged::launch_status("latent expand");
-  if (rc) return rc;
-  attend_kernel<T, true><<<(unsigned)(p.tokens * p.heads), kThreads, 0, st>>>(p);
-  return paged::launch_status("latent attend");
+template <int MAIN, bool EXP>
+int launch_rope(const Params& p, cudaStream_t st) {
+  return p.rope == 32 ? launch_kind<MAIN, 32, EXP>(p, st) : launch_kind<MAIN, 64, EXP>(p, st);
 }
 
 }  // namespace
 
-int launch_absorbed(int dtype, const Params& p, cudaStream_t st) {
-  return dtype == GRM_B200_F16 ? absorbed<__half>(p, st) : absorbed<__nv_bfloat16>(p, st);
+int launch_absorbed(const Params& p, cudaStream_t st) {
+  return p.latent == 128   ? launch_rope<128, false>(p, st)
+         : p.latent == 256 ? launch_rope<256, false>(p, st)
+                           : launch_rope<512, false>(p, st);
 }
 
-int launch_expanded(int dtype, const Params& p, cudaStream_t st) {
-  return dtype == GRM_B200_F16 ? expanded<__half>(p, st) : expanded<__nv_bfloat16>(p, st);
+int launch_expanded(const Params& p, cudaStream_t st) {
+  return p.nope == 64 ? launch_rope<64, true>(p, st) : launch_rope<128, true>(p, st);
 }
 
 }  // namespace latent

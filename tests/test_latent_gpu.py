@@ -12,9 +12,9 @@ arena's type (2^-8 bf16, 2^-11 fp16):
   rounded ones, so twice that at most.
 * the result is rounded once: u relative, and 2^-25 for fp16's smallest.
 * the log-sum-exp is off by e, n 2^-24 from the sum, and 2^-22 of itself.
-* expanded keys and values are rounded to the type after sums of up to 512 products
-  (2^-16 of their magnitudes): each is off by u |k| + 2^-16 sum|w c|, which goes into e
-  for the keys and into the result for the values.
+* expanded keys and values are sums of up to 512 products (2^-16 of their magnitudes).
+  Keys are held as two numbers of the type, off by u^2 |k| (and fp16's 2^-25), which
+  goes into e; values as one, off by u |v|, which goes into the result.
 """
 
 import math
@@ -120,7 +120,9 @@ class Turn:
                 if expanded:
                     w = self.weights[h].double()
                     kv = rows[:, :C] @ w.T
-                    dkv = u * kv.abs() + 2.0 ** -16 * (rows[:, :C].abs() @ w.abs().T) + tiny
+                    dkv = 2.0 ** -16 * (rows[:, :C].abs() @ w.abs().T) + tiny
+                    dkv[:, :self.nope] += u * u * kv[:, :self.nope].abs()
+                    dkv[:, self.nope:] += u * kv[:, self.nope:].abs()
                     k = torch.cat([kv[:, :self.nope], rows[:, C:]], 1)
                     dk = torch.cat([dkv[:, :self.nope], torch.zeros_like(rows[:, C:])], 1)
                     v, dv = kv[:, self.nope:], dkv[:, self.nope:]
