@@ -530,6 +530,12 @@ int grm_b200_latent_attend_expanded(const grm_b200_latent_plan* plan,
     set_thread_error("latent attend: the plan has no room for the expanded form (expand_tokens)");
     return GRM_B200_EINVAL;
   }
+  if (weights_row_stride < arena->latent ||
+      (weights_head_stride != 0 && weights_head_stride < arena->latent)) {
+    set_thread_error("latent attend: weights' rows overlap (head stride %lld, row stride %lld)",
+                     (long long)weights_head_stride, (long long)weights_row_stride);
+    return GRM_B200_EINVAL;
+  }
   if ((rc = check_latent_plan(plan)) ||
       (rc = fill(plan, arena, 1, softmax_scale, causal, out_device, lse_device, &p)))
     return rc;
