@@ -18,14 +18,11 @@ constexpr int kForms = 2;  // absorbed, expanded
 
 struct ScheduleParams {
   Lists l[kForms];
-  Tiling tiling[kForms];
+  View v[kForms];
   int forms;  // 1 where the plan has no expanded form
   int32_t* room;
-  const int32_t* lens;
-  const int32_t* starts;
   int32_t* status;
-  int64_t requests, expand_tokens;
-  int grow;
+  int64_t expand_tokens;
 };
 
 // Inclusive prefix sum over the block; `part` is of the block's warps.
@@ -56,34 +53,35 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* part, int64_t*
 }
 
 // One block for each form, and one for the room of what is expanded: prefix sums over
-// the requests, 1,024 at a time, then each worker's first request by a binary search.
+// the requests, 1,024 at a time, then each worker's first tile by binary searches.
 __global__ void __launch_bounds__(kScheduleThreads) schedule_kernel(const ScheduleParams p) {
   __shared__ int64_t part[33];
   __shared__ Header sh;
   const int tid = threadIdx.x, form = blockIdx.x;
   const bool sizes = form < p.forms;  // else: room
   const Lists l = p.l[sizes ? form : 0];
-  const Tiling tiling = p.tiling[sizes ? form : 0];
+  const View v = p.v[sizes ? form : 0];
+  const int64_t requests = v.requests;
   int64_t before = 0, room = 0;
-  for (int64_t r0 = 0; r0 < p.requests; r0 += kScheduleThreads) {
+  for (int64_t r0 = 0; r0 < requests; r0 += kScheduleThreads) {
     const int64_t r = r0 + tid;
     int64_t n = 0, tokens = 0;
-    if (r < p.requests) {
-      const Request q = request_of(p.starts[r], p.starts[r + 1], p.lens[r], tiling.per, p.grow);
+    if (r < requests) {
+      const Request q = request_of(v.starts[r], v.starts[r + 1], v.lens[r], v.tiling.per, v.grow);
       if (q.n > 0) {
-        n = q.total * tiling.groups;
+        n = q.total * v.tiling.groups;
         tokens = ((int64_t)q.len + kExpandAlign - 1) / kExpandAlign * kExpandAlign;
       }
     }
     int64_t all = 0;
     if (sizes) {
       const int64_t incl = block_scan(n, part, &all);
-      if (r < p.requests) l.base[r] = before + incl - n;
+      if (r < requests) l.base[r] = before + incl - n;
       before += all;
     }
     if (form > 0 || !sizes) {  // the second form's block wants to know if it has room
       const int64_t incl = block_scan(tokens, part, &all);
-      if (!sizes && r < p.requests)
+      if (!sizes && r < requests)
         p.room[r] = (int)min(room + incl - tokens, (int64_t)INT32_MAX);
       room += all;
     }
@@ -91,29 +89,31 @@ __global__ void __launch_bounds__(kScheduleThreads) schedule_kernel(const Schedu
   const bool lost = p.expand_tokens > 0 && room > p.expand_tokens;
   if (!sizes) {
     if (tid == 0) {
-      p.room[p.requests] = lost ? 0 : (int)room;  // nothing is expanded then
+      p.room[requests] = lost ? 0 : (int)room;  // nothing is expanded then
       if (lost) atomicOr(p.status, GRM_B200_PLAN_EXPAND);
     }
     return;
   }
   if (tid == 0) {
     const int64_t most = before / kLeast;
-    const int workers = before == 0 ? 0 : (int)min((int64_t)tiling.workers, max(most, (int64_t)1));
+    const int workers = before == 0 ? 0 : (int)min((int64_t)v.tiling.workers, max(most, (int64_t)1));
     sh = Header{before, workers ? before / workers : 0, workers ? (int)(before % workers) : 0,
                 workers, lost};
     *l.header = sh;
-    l.base[p.requests] = before;
+    l.base[requests] = before;
   }
   __syncthreads();  // and the block's own writes to base are there
   for (int w = tid; w < sh.workers; w += kScheduleThreads) {
     const int64_t u = worker_first(w, sh);
-    int64_t lo = 0, hi = p.requests;
+    int lo = 0, hi = (int)requests;
     while (hi - lo > 1) {
-      const int64_t mid = (lo + hi) >> 1;
+      const int mid = (lo + hi) >> 1;
       if (l.base[mid] <= u) lo = mid;
       else hi = mid;
     }
-    l.start[w] = (int)lo;
+    Walk walk;
+    walk.seek(v, u, lo);
+    l.start[w] = Start{walk.r, walk.g, walk.j, walk.q.start, walk.q.n, walk.q.len, walk.first};
   }
 }
 
@@ -285,6 +285,11 @@ int check_attend(const grm_b200_latent_plan* plan, const grm_b200_latent_arena* 
   return 0;
 }
 
+View view_of(const grm_b200_latent_plan& plan, const Shape& s, int form) {
+  return {lists_of(s, form, plan.work).base, plan.step.starts, plan.step.lens, plan.step.requests,
+          s.tiling[form], plan.step.grow ? 1 : 0};
+}
+
 int fill(const grm_b200_latent_plan* plan, const grm_b200_latent_arena* arena, int form,
          float softmax_scale, int causal, void* out, float* lse, Params* p) {
   int sms = 0;
@@ -294,16 +299,13 @@ int fill(const grm_b200_latent_plan* plan, const grm_b200_latent_arena* arena, i
   make_shape(*plan, sms, &s);
   *p = Params{};
   p->l = lists_of(s, form, plan->work);
-  p->tiling = s.tiling[form];
+  p->v = view_of(*plan, s, form);
   p->probes = std::min(scan_wait_limit(), paged::kProbes);
   char* work = static_cast<char*>(plan->work);
   p->room = reinterpret_cast<const int32_t*>(work + s.off_room);
   p->keys = reinterpret_cast<uint16_t*>(work + s.off_keys);
   p->values = reinterpret_cast<uint16_t*>(work + s.off_values);
   p->table = plan->step.table;
-  p->lens = plan->step.lens;
-  p->starts = plan->step.starts;
-  p->requests = plan->step.requests;
   p->width = plan->step.table_width;
   p->tokens = plan->step.tokens;
   p->pages = plan->step.pages;
@@ -314,7 +316,6 @@ int fill(const grm_b200_latent_plan* plan, const grm_b200_latent_arena* arena, i
   p->rope = plan->rope;
   p->nope = plan->nope;
   p->causal = causal ? 1 : 0;
-  p->grow = plan->step.grow ? 1 : 0;
   p->dtype = arena->dtype;
   p->cache = static_cast<const uint16_t*>(arena->rows);
   p->scale_log2 = softmax_scale * 1.44269504088896341f;
@@ -338,7 +339,7 @@ int make_shape(const grm_b200_latent_plan& p, int sms, Shape* s) {
   for (int f = 0; f < kForms; ++f) {
     s->off_header[f] = take(sizeof(Header));
     s->off_base[f] = take((p.step.requests + 1) * 8);
-    s->off_start[f] = take((int64_t)s->tiling[f].workers * 4);
+    s->off_start[f] = take((int64_t)s->tiling[f].workers * (int64_t)sizeof(Start));
   }
   const int64_t absorbed = (int64_t)s->tiling[0].workers * s->tiling[0].splits *
                            slot_floats(kRows, std::min(p.latent, 256));
@@ -431,16 +432,12 @@ int grm_b200_latent_plan_step(const grm_b200_latent_plan* plan, const int32_t* f
   ScheduleParams p;
   for (int f = 0; f < kForms; ++f) {
     p.l[f] = lists_of(s, f, plan->work);
-    p.tiling[f] = s.tiling[f];
+    p.v[f] = view_of(*plan, s, f);
   }
   p.forms = plan->nope ? kForms : 1;
   p.room = reinterpret_cast<int32_t*>(static_cast<char*>(plan->work) + s.off_room);
-  p.lens = plan->step.lens;
-  p.starts = plan->step.starts;
   p.status = plan->step.status;
-  p.requests = plan->step.requests;
   p.expand_tokens = plan->expand_tokens;
-  p.grow = plan->step.grow ? 1 : 0;
   schedule_kernel<<<plan->nope ? kForms + 1 : 1, kScheduleThreads, 0,
                     static_cast<cudaStream_t>(stream)>>>(p);
   return launch_status("latent plan");

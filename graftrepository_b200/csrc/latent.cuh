@@ -32,11 +32,18 @@ struct Header {     // written by the schedule kernel, one for each form
   int32_t lost;     // more tokens to expand than there is room for
 };
 
+// Where a worker starts: the tile of its first unit, and that tile's first unit.
+struct alignas(32) Start {
+  int32_t r, g, j;       // request, group, tile
+  int32_t from, n, len;  // the request's first packed row, rows, tokens
+  int64_t first;
+};
+
 struct Lists {
   Header* header;
-  int64_t* base;   // [requests + 1] first unit of each request
-  int32_t* start;  // [workers] request of a worker's first unit
-  float* part;     // [workers * splits * 2] partial results, see slot_floats
+  int64_t* base;  // [requests + 1] first unit of each request
+  Start* start;   // [workers]
+  float* part;    // [workers * splits * 2] partial results, see slot_floats
 };
 
 // Tiles of one form: tokens and groups of a request, and how a row of a tile is one
@@ -72,22 +79,30 @@ inline Lists lists_of(const Shape& s, int form, void* work) {
   char* b = static_cast<char*>(work);
   return {reinterpret_cast<Header*>(b + s.off_header[form]),
           reinterpret_cast<int64_t*>(b + s.off_base[form]),
-          reinterpret_cast<int32_t*>(b + s.off_start[form]),
+          reinterpret_cast<Start*>(b + s.off_start[form]),
           reinterpret_cast<float*>(b + s.off_part)};
 }
 
+// What the walk over a form's tiles goes by.
+struct View {
+  const int64_t* base;
+  const int32_t* starts;
+  const int32_t* lens;
+  int64_t requests;
+  Tiling tiling;
+  int grow;
+};
+
 struct Params {
   Lists l;
-  Tiling tiling;
+  View v;
   unsigned probes;    // of a bounded wait: paged::kProbes, or less by GRM_B200_WAIT_LIMIT
   const int32_t* room;  // [requests + 1] first expanded token of each request
   uint16_t* keys;       // [heads][expand_tokens][2 * nope]: rounded, and what that left over
   uint16_t* values;     // [heads][expand_tokens][value]
   const int32_t* table;
-  const int32_t* lens;
-  const int32_t* starts;
-  int64_t requests, width, tokens, pages, expand_tokens;
-  int page_shift, heads, latent, rope, nope, causal, grow, dtype;
+  int64_t width, tokens, pages, expand_tokens;
+  int page_shift, heads, latent, rope, nope, causal, dtype;
   const uint16_t* cache;
   const uint16_t* q;  // absorbed: the latent part; expanded: nope + rope values
   int64_t q_row, q_head;
@@ -150,48 +165,59 @@ struct Walk {
   Request q;
   int64_t first, last;  // units of the tile
 
-  __host__ __device__ __forceinline__ void enter(const Params& p, int request) {
+  __host__ __device__ __forceinline__ void enter(const View& v, int request) {
     r = request;
-    q = request_of(p.starts[r], p.starts[r + 1], p.lens[r], p.tiling.per, p.grow);
+    q = request_of(v.starts[r], v.starts[r + 1], v.lens[r], v.tiling.per, v.grow);
   }
-  __host__ __device__ __forceinline__ void bound(const Params& p) {
-    const int64_t at = p.l.base[r] + (int64_t)g * q.total;
-    first = at + units_before(q, p.tiling.per, p.grow, j);
-    last = at + units_before(q, p.tiling.per, p.grow, j + 1);
+  __host__ __device__ __forceinline__ int64_t cost(const View& v) const {  // of the tile
+    if (!v.grow) return q.len + kStart;
+    const int64_t sees = q.cached + (int64_t)(j + 1) * v.tiling.per;
+    return (j + 1 < q.tiles ? sees : q.len) + kStart;
   }
-  __host__ __device__ __forceinline__ void seek(const Params& p, int64_t u, int request) {
-    enter(p, request);
-    const int64_t x = u - p.l.base[r];
+  __host__ __device__ __forceinline__ void seek(const View& v, int64_t u, int request) {
+    enter(v, request);
+    const int64_t x = u - v.base[r];
     g = (int)(x / q.total);
     const int64_t y = x - g * q.total;
     int lo = 0, hi = q.tiles;  // the last tile that starts at y or before
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
-      if (units_before(q, p.tiling.per, p.grow, mid) <= y) lo = mid;
+      if (units_before(q, v.tiling.per, v.grow, mid) <= y) lo = mid;
       else hi = mid;
     }
     j = lo;
-    bound(p);
+    first = v.base[r] + g * q.total + units_before(q, v.tiling.per, v.grow, j);
+    last = first + cost(v);
   }
-  __host__ __device__ __forceinline__ void next(const Params& p) {  // there is one
+  __host__ __device__ __forceinline__ void start(const View& v, const Start& s) {
+    r = s.r;
+    g = s.g;
+    j = s.j;
+    q = Request{s.from, s.n, s.len, v.grow ? s.len - s.n : s.len,
+                (s.n + v.tiling.per - 1) / v.tiling.per, 0};
+    first = s.first;
+    last = first + cost(v);
+  }
+  __host__ __device__ __forceinline__ void next(const View& v) {  // there is one
+    first = last;
     if (++j == q.tiles) {
       j = 0;
-      if (++g == p.tiling.groups) {
+      if (++g == v.tiling.groups) {
         g = 0;
         // the next request that has units
         int lo = r + 1;
-        if (p.l.base[lo + 1] <= last) {
-          int hi = (int)p.requests;
+        if (v.base[lo + 1] <= first) {
+          int hi = (int)v.requests;
           while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;
-            if (p.l.base[mid] <= last) lo = mid;
+            if (v.base[mid] <= first) lo = mid;
             else hi = mid;
           }
         }
-        enter(p, lo);
+        enter(v, lo);
       }
     }
-    bound(p);
+    last = first + cost(v);
   }
 };
 
@@ -215,16 +241,16 @@ struct Parts {
       : u(worker_first(worker, h)), end(worker_first(worker + 1, h)), w(worker), count(0) {}
   __host__ __device__ __forceinline__ bool next(const Params& p, Part* x) {
     if (u >= end) return false;
-    if (count == 0) walk.seek(p, u, p.l.start[w]);
-    else walk.next(p);
+    if (count == 0) walk.start(p.v, p.l.start[w]);
+    else walk.next(p.v);
     x->r = walk.r;
     x->g = walk.g;
     x->start = walk.q.start;
     x->n = walk.q.n;
     x->cached = walk.q.cached;
     x->len = walk.q.len;
-    x->tok0 = walk.j * p.tiling.per;
-    const int toks = imin(p.tiling.per, x->n - x->tok0);
+    x->tok0 = walk.j * p.v.tiling.per;
+    const int toks = imin(p.v.tiling.per, x->n - x->tok0);
     x->toks[0] = QUERIES == 2 ? imin(toks, kRows) : toks;
     x->toks[1] = QUERIES == 2 ? toks - x->toks[0] : 0;
     const int sees = p.causal ? imin(x->len, x->cached + x->tok0 + toks) : x->len;

@@ -86,6 +86,7 @@ struct Layout {
   static constexpr int kThreads = (kLoadWarp + 1) * 32;
   static constexpr int kSlot = slot_floats(kRows * kQueries, kV);
   static_assert(kQueryCol + kQueries * kQTmem / 2 <= kTmemCols && kStages >= 2, "tiles");
+  static_assert(kQTmem % 128 == 0 || kQTmem == MAIN, "queries come 128 values at a time");
 };
 
 template <typename T>
@@ -197,12 +198,36 @@ struct Row {
 template <bool EXP>
 __device__ __forceinline__ Row row_of(const Params& p, const Part& x, int t, int row) {
   if (EXP) return {x.tok0 + t * kRows + row, x.g, row < x.toks[t]};
-  if (p.tiling.groups > 1) {
+  if (p.v.tiling.groups > 1) {
     const int h = x.g * kRows + row;
     return {x.tok0, min(h, p.heads - 1), h < p.heads};
   }
   const int token = row / p.heads;
   return {x.tok0 + token, row - token * p.heads, token < x.toks[0]};
+}
+
+// The scores of a step from the first hidden one on set to -inf, in tensor memory;
+// returns the hidden tokens whose score was no finite number.  A step of its own, few
+// instructions in a loop: unrolled into the softmax it took 5 us the first time a
+// block came by, on instructions that were not in its cache.
+__device__ __forceinline__ unsigned long long hide(uint32_t scores, int seen) {
+  unsigned long long bad = 0;
+#pragma unroll 1
+  for (int c = 0; c < kStep; c += 16) {
+    uint32_t v[16];
+    tmem_ld16(scores + c, v);
+    unsigned b = 0;
+#pragma unroll
+    for (int k = 0; k < 16; ++k)
+      if (c + k >= seen) {
+        if ((v[k] & 0x7F800000u) == 0x7F800000u) b |= 1u << k;
+        v[k] = 0xFF800000u;
+      }
+    tmem_st16(scores + c, v);
+    bad |= (unsigned long long)b << c;
+  }
+  tmem_wait_st();
+  return bad;
 }
 
 // Numbers that are none among the V values of token `t` of a stage set to 0.
@@ -338,30 +363,38 @@ __global__ void __launch_bounds__(Layout<MAIN, ROPE, EXP>::kThreads, 1)
           return a.active ? __ldg(reinterpret_cast<const uint4*>(from) + c)
                           : make_uint4(0, 0, 0, 0);
         };
-#pragma unroll 2
-        for (int c = 0; c < LY::kQTmem / 8; c += 4) {
-          uint32_t w[16];
+        // sixteen loads in flight
+#pragma unroll 1
+        for (int c = 0; c < MAIN / 8; c += 16) {
+          uint4 v[16];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint4 v = chunk(qp, c + i);
-            w[4 * i] = v.x;
-            w[4 * i + 1] = v.y;
-            w[4 * i + 2] = v.z;
-            w[4 * i + 3] = v.w;
+          for (int i = 0; i < 16; ++i) v[i] = MAIN >= 128 || i < MAIN / 8 ? chunk(qp, c + i) : uint4{};
+          if (c < LY::kQTmem / 8) {
+#pragma unroll
+            for (int i = 0; i < 16 && i < MAIN / 8; i += 4) {
+              const uint32_t w[16] = {v[i].x, v[i].y, v[i].z, v[i].w, v[i + 1].x, v[i + 1].y,
+                                      v[i + 1].z, v[i + 1].w, v[i + 2].x, v[i + 2].y, v[i + 2].z,
+                                      v[i + 2].w, v[i + 3].x, v[i + 3].y, v[i + 3].z, v[i + 3].w};
+              tmem_st16(q_col + 4 * (c + i), w);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16 && i < MAIN / 8; ++i) {
+              const int y = c + i - LY::kQTmem / 8;
+              *reinterpret_cast<uint4*>(my_q + (y / 8) * kQueryAtom + atom_byte(row, y % 8)) = v[i];
+            }
           }
-          tmem_st16(q_col + 4 * c, w);
         }
-#pragma unroll 4
-        for (int c = LY::kQTmem / 8; c < MAIN / 8; ++c) {
-          const int y = c - LY::kQTmem / 8;
-          *reinterpret_cast<uint4*>(my_q + (y / 8) * kQueryAtom + atom_byte(row, y % 8)) =
-              chunk(qp, c);
-        }
+        {
+          uint4 v[ROPE / 8];
 #pragma unroll
-        for (int c = 0; c < ROPE / 8; ++c)
-          *reinterpret_cast<uint4*>(my_q + LY::kQRopeAt +
-                                    (ROPE == 64 ? atom_byte(row, c) : half_atom_byte(row, c))) =
-              chunk(rp, c);
+          for (int c = 0; c < ROPE / 8; ++c) v[c] = chunk(rp, c);
+#pragma unroll
+          for (int c = 0; c < ROPE / 8; ++c)
+            *reinterpret_cast<uint4*>(
+                my_q + LY::kQRopeAt +
+                (ROPE == 64 ? atom_byte(row, c) : half_atom_byte(row, c))) = v[c];
+        }
         tmem_wait_st();
         tc_fence_before();
         fence_proxy_async_smem();
@@ -381,28 +414,22 @@ __global__ void __launch_bounds__(Layout<MAIN, ROPE, EXP>::kThreads, 1)
           if (lane == 0) mbar_arrive(&p_full[t][buf]);
           continue;
         }
+        if (__any_sync(kFull, (i + 1) * kStep > lim)) {
+          const unsigned long long bad = hide(s_col + buf * kStep, lim - i * kStep);
+          if (__any_sync(kFull, bad != 0)) {
+            const int st = stage_base + i;  // its copies landed before the scores were there
+            if (!(ok = wait(&full[st % kStages], (st / kStages) & 1))) break;
+            scrub<T, LY::kV>(sm_stage + st % kStages * LY::kStage + LY::kValueAt +
+                                 split * (LY::kV / 64) * kAtom,
+                             bad);
+            fence_proxy_async_smem();
+          }
+        }
         uint32_t v[2][32];
         tmem_ld32_nowait(s_col + buf * kStep, v[0]);
         tmem_ld32_nowait(s_col + buf * kStep + 32, v[1]);
         tmem_wait_ld32(v[0]);
         tmem_wait_ld32(v[1]);
-        if (__any_sync(kFull, (i + 1) * kStep > lim)) {
-          unsigned bad[2] = {0, 0};
-#pragma unroll
-          for (int k = 0; k < kStep; ++k)
-            if (i * kStep + k >= lim) {
-              if ((v[k / 32][k % 32] & 0x7F800000u) == 0x7F800000u) bad[k / 32] |= 1u << (k % 32);
-              v[k / 32][k % 32] = 0xFF800000u;
-            }
-          if (__any_sync(kFull, (bad[0] | bad[1]) != 0)) {
-            const int st = stage_base + i;  // its copies landed before the scores were there
-            if (!(ok = wait(&full[st % kStages], (st / kStages) & 1))) break;
-            unsigned char* at = sm_stage + st % kStages * LY::kStage +
-                                LY::kValueAt + split * (LY::kV / 64) * kAtom;
-            scrub<T, LY::kV>(at, (unsigned long long)bad[1] << 32 | bad[0]);
-            fence_proxy_async_smem();
-          }
-        }
         float top = -INFINITY;
 #pragma unroll
         for (int k = 0; k < kStep; k += 2)
@@ -463,13 +490,14 @@ __global__ void __launch_bounds__(Layout<MAIN, ROPE, EXP>::kThreads, 1)
         float4* to = reinterpret_cast<float4*>(slot + (t * kRows + row) * LY::kV);
         if (steps > 0 && !idle)
 #pragma unroll 1
-          for (int c = 0; c < LY::kV / 16; ++c) {
-            uint32_t o[16];
-            tmem_ld16(o_col + 16 * c, o);
+          for (int c = 0; c < LY::kV / 32; ++c) {
+            uint32_t o[32];
+            tmem_ld32_nowait(o_col + 32 * c, o);
+            tmem_wait_ld32(o);
             if (a.active)
 #pragma unroll
-              for (int k = 0; k < 4; ++k)
-                to[4 * c + k] =
+              for (int k = 0; k < 8; ++k)
+                to[8 * c + k] =
                     make_float4(__uint_as_float(o[4 * k]), __uint_as_float(o[4 * k + 1]),
                                 __uint_as_float(o[4 * k + 2]), __uint_as_float(o[4 * k + 3]));
           }
@@ -480,19 +508,22 @@ __global__ void __launch_bounds__(Layout<MAIN, ROPE, EXP>::kThreads, 1)
         const float inv = lr == 0.0f ? 0.0f : 1.0f / lr;
         uint16_t* out = p.out + orow * MAIN + split * LY::kV;
 #pragma unroll 1
-        for (int c = 0; c < LY::kV / 16; ++c) {
-          uint32_t o[16];
-          if (steps > 0) tmem_ld16(o_col + 16 * c, o);
+        for (int c = 0; c < LY::kV / 32; ++c) {
+          uint32_t o[32];
+          if (steps > 0) {
+            tmem_ld32_nowait(o_col + 32 * c, o);
+            tmem_wait_ld32(o);
+          }
           if (a.active)
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
+            for (int k = 0; k < 4; ++k) {
               uint32_t w[4];
 #pragma unroll
               for (int y = 0; y < 4; ++y)
                 w[y] = lr == 0.0f ? 0u
                                   : Kind<T>::pack(__uint_as_float(o[8 * k + 2 * y]) * inv,
                                                   __uint_as_float(o[8 * k + 2 * y + 1]) * inv);
-              reinterpret_cast<uint4*>(out)[2 * c + k] = make_uint4(w[0], w[1], w[2], w[3]);
+              reinterpret_cast<uint4*>(out)[4 * c + k] = make_uint4(w[0], w[1], w[2], w[3]);
             }
         }
         if (a.active && p.lse && split == 0)
@@ -661,89 +692,136 @@ __global__ void __launch_bounds__(Layout<MAIN, ROPE, EXP>::kThreads, 1)
   }
 }
 
+constexpr int kJoinBlocks = 16;  // for every border between two shares
+
 // Parts of tiles that lie in the shares of several workers, and the rows past the
-// step's last one.  Boundary b is where worker b's share starts; the first one inside a
-// tile joins it, a warp a row.
+// step's last one.  A tile in n parts has n - 1 borders inside, whose blocks share its
+// rows: 1 to 8 warps a row, each for some of the parts.
 template <typename T, int MAIN, int ROPE, bool EXP>
 __global__ void __launch_bounds__(256) join_kernel(const Params p) {
   using LY = Layout<MAIN, ROPE, EXP>;
   constexpr int kLanes = LY::kV / 4;  // float4 of a row
+  constexpr int kMine = (kLanes + 31) / 32;
+  __shared__ float4 sums[8][kLanes];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const Header hd = *p.l.header;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t used = p.starts[p.requests];
+  const int b = blockIdx.x / LY::kSplits + 1, split = blockIdx.x % LY::kSplits;
+  Start start;
+  if (b < hd.workers) start = p.l.start[b];
+  const int64_t used = p.v.starts[p.v.requests];
   const int64_t id = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 256 + threadIdx.x;
   for (int64_t i = used * p.heads * (MAIN / 8) + id; i < p.tokens * p.heads * (MAIN / 8);
        i += (int64_t)gridDim.x * gridDim.y * 256) {
     reinterpret_cast<uint4*>(p.out)[i] = make_uint4(0, 0, 0, 0);
     if (p.lse && i % (MAIN / 8) == 0) p.lse[i / (MAIN / 8)] = -INFINITY;
   }
-  const int b = blockIdx.x / LY::kSplits + 1, split = blockIdx.x % LY::kSplits;
   if (b >= hd.workers) return;
-  const int64_t u = worker_first(b, hd);
   Walk walk;
-  walk.seek(p, u, p.l.start[b]);
-  const int64_t before = worker_first(b - 1, hd);
-  if (walk.first == u || walk.first < before) return;
+  walk.start(p.v, start);
+  if (walk.first == worker_first(b, hd)) return;  // no border inside the tile
+  const int w0 = worker_of(walk.first, hd);       // worker of the tile's first part
+  const int parts = worker_of(walk.last - 1, hd) - w0 + 1;
   Part x;
   x.r = walk.r;
   x.g = walk.g;
-  x.tok0 = walk.j * p.tiling.per;
-  const int toks = min(p.tiling.per, walk.q.n - x.tok0);
+  x.tok0 = walk.j * p.v.tiling.per;
+  const int toks = min(p.v.tiling.per, walk.q.n - x.tok0);
   x.toks[0] = EXP ? min(toks, kRows) : toks;
   x.toks[1] = EXP ? toks - x.toks[0] : 0;
-  const int line = blockIdx.y * 8 + warp;  // of the tile's rows
-  const Row a = row_of<EXP>(p, x, line / kRows, line % kRows);
-  if (!a.active) return;
-  const int slot0 = 2 * (b - 1) + (walk.first == before ? 0 : 1);
-  const int parts = worker_of(walk.last - 1, hd) - b + 2;
+  const int rows = EXP ? toks
+                       : min(kRows, toks * (p.v.tiling.groups > 1 ? kRows : p.heads));
+  // rows of a block: 8, 4, 2 or 1, whichever is enough, and more where 8 are not
+  const int blocks = (parts - 1) * kJoinBlocks;
+  int each = 1;
+  while (each < 8 && each * blocks < rows) each *= 2;
+  const int warps = 8 / each, sub = warp % warps;  // of a row, and which of them
+  const int slot0 = 2 * w0 + (walk.first == worker_first(w0, hd) ? 0 : 1);
   auto slot = [&](int k) {
-    const int at = k == 0 ? slot0 : 2 * (b - 1 + k);
+    const int at = k == 0 ? slot0 : 2 * (w0 + k);
     return p.l.part + ((int64_t)at * LY::kSplits + split) * LY::kSlot;
   };
-  auto state = [&](int k) {
-    return *reinterpret_cast<const float4*>(slot(k) + kRows * LY::kQueries * LY::kV + 4 * line);
-  };
-  // the largest reference exponent of the parts that see something, lanes side by side
-  float m = -INFINITY;
-  for (int k = lane; k < parts; k += 32) {
-    const float4 s = state(k);
-    if (s.y != 0.0f) m = fmaxf(m, s.x);
-  }
+  const int block = (b - 1 - w0) * kJoinBlocks + blockIdx.y;
+  for (int row0 = block * each; row0 < rows; row0 += blocks * each) {
+    const int line = row0 + warp / warps;  // of the tile's rows
+    const Row a = row_of<EXP>(p, x, line / kRows, line % kRows);
+    const bool active = line < rows && a.active;
+    float m = -INFINITY, l = 0.0f, lr = 0.0f;
+    float4 o[kMine] = {};
+    if (active) {
+      auto state = [&](int k) {
+        return *reinterpret_cast<const float4*>(slot(k) + kRows * LY::kQueries * LY::kV +
+                                                4 * line);
+      };
+      // the largest reference exponent of the parts that see something, and the sums,
+      // lanes side by side
+      for (int k = lane; k < parts; k += 32) {
+        const float4 s = state(k);
+        if (s.y != 0.0f) m = fmaxf(m, s.x);
+      }
 #pragma unroll
-  for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kFull, m, o));
-  float l = 0.0f, lr = 0.0f;
-  constexpr int kMine = (kLanes + 31) / 32;
-  float4 o[kMine] = {};
-  for (int k = 0; k < parts; ++k) {
-    const float4 s = state(k);
-    if (s.y == 0.0f) continue;
-    const float f = s.x == m ? 1.0f : ex2(s.x - m);
-    l = fmaf(s.y, f, l);
-    lr = fmaf(s.z, f, lr);
-    const float4* from = reinterpret_cast<const float4*>(slot(k) + line * LY::kV);
+      for (int i = 16; i; i >>= 1) m = fmaxf(m, __shfl_xor_sync(kFull, m, i));
+      for (int k = lane; k < parts; k += 32) {
+        const float4 s = state(k);
+        const float f = s.x == m ? 1.0f : ex2(s.x - m);
+        if (s.y != 0.0f) {
+          l = fmaf(s.y, f, l);
+          lr = fmaf(s.z, f, lr);
+        }
+      }
+#pragma unroll
+      for (int i = 16; i; i >>= 1) {
+        l += __shfl_xor_sync(kFull, l, i);
+        lr += __shfl_xor_sync(kFull, lr, i);
+      }
+#pragma unroll 4
+      for (int k = sub; k < parts; k += warps) {
+        const float4 s = state(k);
+        const float f = s.x == m ? 1.0f : ex2(s.x - m);
+        const float4* from = reinterpret_cast<const float4*>(slot(k) + line * LY::kV);
+#pragma unroll
+        for (int i = 0; i < kMine; ++i)
+          if (lane + 32 * i < kLanes && s.y != 0.0f) {
+            const float4 v = from[lane + 32 * i];
+            o[i].x = fmaf(v.x, f, o[i].x);
+            o[i].y = fmaf(v.y, f, o[i].y);
+            o[i].z = fmaf(v.z, f, o[i].z);
+            o[i].w = fmaf(v.w, f, o[i].w);
+          }
+      }
+    }
+    if (warps > 1) {
+#pragma unroll
+      for (int i = 0; i < kMine; ++i)
+        if (lane + 32 * i < kLanes) sums[warp][lane + 32 * i] = o[i];
+      __syncthreads();
+      if (sub == 0)
+        for (int w = 1; w < warps; ++w)
+#pragma unroll
+          for (int i = 0; i < kMine; ++i)
+            if (lane + 32 * i < kLanes) {
+              const float4 v = sums[warp + w][lane + 32 * i];
+              o[i].x += v.x;
+              o[i].y += v.y;
+              o[i].z += v.z;
+              o[i].w += v.w;
+            }
+      __syncthreads();
+    }
+    if (!active || sub != 0) continue;
+    const int64_t orow = (int64_t)(walk.q.start + a.token) * p.heads + a.head;
+    const float inv = 1.0f / lr;
 #pragma unroll
     for (int i = 0; i < kMine; ++i)
-      if (lane + 32 * i < kLanes) {
-        const float4 v = from[lane + 32 * i];
-        o[i].x = fmaf(v.x, f, o[i].x);
-        o[i].y = fmaf(v.y, f, o[i].y);
-        o[i].z = fmaf(v.z, f, o[i].z);
-        o[i].w = fmaf(v.w, f, o[i].w);
-      }
+      if (lane + 32 * i < kLanes)
+        reinterpret_cast<uint2*>(p.out + orow * MAIN + split * LY::kV)[lane + 32 * i] =
+            lr == 0.0f ? make_uint2(0, 0)
+                       : make_uint2(Kind<T>::pack(o[i].x * inv, o[i].y * inv),
+                                    Kind<T>::pack(o[i].z * inv, o[i].w * inv));
+    if (lane == 0 && p.lse && split == 0)
+      p.lse[orow] =
+          l == 0.0f ? -INFINITY : (m - Kind<T>::kLift + log2f(l)) * 0.693147180559945309f;
   }
-  const int64_t orow = (int64_t)(walk.q.start + a.token) * p.heads + a.head;
-  const float inv = 1.0f / lr;
-#pragma unroll
-  for (int i = 0; i < kMine; ++i)
-    if (lane + 32 * i < kLanes)
-      reinterpret_cast<uint2*>(p.out + orow * MAIN + split * LY::kV)[lane + 32 * i] =
-          lr == 0.0f ? make_uint2(0, 0)
-                     : make_uint2(Kind<T>::pack(o[i].x * inv, o[i].y * inv),
-                                  Kind<T>::pack(o[i].z * inv, o[i].w * inv));
-  if (lane == 0 && p.lse && split == 0)
-    p.lse[orow] =
-        l == 0.0f ? -INFINITY : (m - Kind<T>::kLift + log2f(l)) * 0.693147180559945309f;
 }
 
 template <typename T, int MAIN, int ROPE, bool EXP>
@@ -769,11 +847,11 @@ int launch(const Params& p, cudaStream_t st) {
   static std::atomic<uint64_t> done{0};
   if ((rc = paged::allow_shared(reinterpret_cast<const void*>(kernel), LY::kSmem, &done)))
     return rc;
-  kernel<<<(unsigned)(p.tiling.workers * LY::kSplits), LY::kThreads, LY::kSmem, st>>>(maps, p);
+  kernel<<<(unsigned)(p.v.tiling.workers * LY::kSplits), LY::kThreads, LY::kSmem, st>>>(maps, p);
   if ((rc = paged::launch_status("latent attend"))) return rc;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(std::max(p.tiling.workers - 1, 1) * LY::kSplits),
-                     kRows * LY::kQueries / 8);
+  cfg.gridDim = dim3((unsigned)(std::max(p.v.tiling.workers - 1, 1) * LY::kSplits),
+                     kJoinBlocks);
   cfg.blockDim = dim3(256);
   cfg.stream = st;
   cudaLaunchAttribute attr;

@@ -122,7 +122,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ uint32_t sh_tmem;
   __shared__ int sh_fail;
 
-  const int total = p.room[p.requests];  // tokens, a multiple of 64
+  const int total = p.room[p.v.requests];  // tokens, a multiple of 64
   const int64_t pairs = ceil_div64(total, kTile) * p.heads;
   const int64_t first = pairs * blockIdx.x / gridDim.x;
   const int64_t end = pairs * (blockIdx.x + 1) / gridDim.x;
@@ -290,7 +290,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         for (int half = 0; half < halves; ++half) {
           const int t0 = (int)(tile * kTile) + half * 64;
-          int lo = 0, hi = (int)p.requests;
+          int lo = 0, hi = (int)p.v.requests;
           while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;
             if (p.room[mid] <= t0) lo = mid;
@@ -298,7 +298,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           // past the request's end the last page again: nothing sees those rows
           const int tok = t0 - p.room[lo] + lane % pieces * piece;
-          const int at = min(tok, p.lens[lo] - 1) >> p.page_shift;
+          const int at = min(tok, p.v.lens[lo] - 1) >> p.page_shift;
           const int page = min(max(p.table[lo * p.width + at], 0), (int)p.pages - 1);
           const int y = (page << p.page_shift) + (tok & ((1 << p.page_shift) - 1));
           for (int i = lane; i < LY::kAtoms * pieces; i += 32)
@@ -377,7 +377,7 @@ int launch_latent(const Params& p, int sms, cudaStream_t st) {
 }  // namespace
 
 int launch_expand(const Params& p, cudaStream_t st) {
-  const int sms = p.tiling.workers;
+  const int sms = p.v.tiling.workers;
   return p.dtype == GRM_B200_F16 ? launch_latent<__half>(p, sms, st)
                                  : launch_latent<__nv_bfloat16>(p, sms, st);
 }
