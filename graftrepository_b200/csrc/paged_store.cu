@@ -205,11 +205,13 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendParams p) {
 
 // ---- append with the keys rotated on the way
 //
-// As append_kernel, with the values held as fp32 and two in three registers: 32 of
-// them a thread.  A thread's 16 values of a row are eight pairs whole: 8 values of
-// the first half of the rotated part and the 8 that turn with them, or 16 in a row
-// where pairs are side by side.  Angles are worked out where they are used, by every
-// kv head anew: about 25 instructions a pair, against a table's 8 bytes from L2.
+// As append_kernel, with the values held as fp32, 32 of them a thread.  A thread's 16
+// values of a row are eight pairs whole: 8 values of the first half of the rotated
+// part and the 8 that turn with them, or 16 in a row where pairs are side by side.
+// A block is HEADS groups, for as many heads of one page, so that the angles of the
+// rows that they hold (about 25 instructions a pair) are worked out once and read from
+// shared memory; rows of a larger page beyond those work theirs out where they are
+// used.
 
 struct TurnedParams {
   AppendParams a;
@@ -244,42 +246,65 @@ __device__ __forceinline__ void quantise_turned(const float (&x)[16], float s, f
   }
 }
 
-template <typename T, int D, int GROUP, int CACHE>
-__global__ void __launch_bounds__(256) append_turned_kernel(const TurnedParams tp) {
+template <typename T, int D, int GROUP, int HEADS>
+__global__ void __launch_bounds__(GROUP * HEADS) append_turned_kernel(const TurnedParams tp) {
   const AppendParams& p = tp.a;
   constexpr int kLanes = D / 16;  // threads of a row
-  constexpr int kRowsPass = GROUP / kLanes;
-  __shared__ unsigned warp_max[8];
-  const int t = threadIdx.x % GROUP;
-  const int64_t job = (int64_t)blockIdx.x * (256 / GROUP) + threadIdx.x / GROUP;
-  const int heads2 = p.kv_heads * 2;
-  const int64_t unit = job / heads2;
+  constexpr int kRowsPass = GROUP / kLanes, kCache = 2, kHeld = kCache * kRowsPass;
+  __shared__ unsigned warp_max[GROUP * HEADS / 32];
+  __shared__ float2 angle[kHeld * (D / 2)];  // [rows][pairs], each row's eights apart
+  const int t = threadIdx.x % GROUP, group = threadIdx.x / GROUP;
+  const int sets2 = (p.kv_heads + HEADS - 1) / HEADS * 2;
+  const int64_t unit = blockIdx.x / sets2;
   if (unit >= p.header->pages) return;
-  const int side = (int)(job % heads2) & 1, h = (int)(job % heads2) >> 1;
+  const int side = (int)(blockIdx.x % sets2) & 1;
+  const int h = ((int)(blockIdx.x % sets2) >> 1) * HEADS + group;
+  const bool there = h < p.kv_heads;
   const int4 entry = p.pages[unit];
-  const int off = entry.z, rows = entry.w;
+  const int off = entry.z, rows = there ? entry.w : 0;
   const int64_t page = min(max((int64_t)entry.y, (int64_t)0), p.ring_size - 1);
   const int64_t row_stride = side ? p.row_stride[1] : p.row_stride[0];
-  const uint16_t* x = (side ? p.x[1] : p.x[0]) + (int64_t)entry.x * row_stride +
-                      (int64_t)h * (side ? p.head_stride[1] : p.head_stride[0]);
-  int8_t* codes = (side ? p.codes[1] : p.codes[0]) + (((page * p.kv_heads + h) << p.page_shift) * D);
-  float* scale = (side ? p.scales[1] : p.scales[0]) + page * p.kv_heads + h;
-  const int position0 = tp.positions[entry.x];
+  const uint16_t* const x = (side ? p.x[1] : p.x[0]) + (int64_t)entry.x * row_stride +
+                            h * (side ? p.head_stride[1] : p.head_stride[0]);
+  int8_t* const codes =
+      (side ? p.codes[1] : p.codes[0]) + (((page * p.kv_heads + h) << p.page_shift) * D);
+  float* const scale = (side ? p.scales[1] : p.scales[0]) + page * p.kv_heads + h;
 
-  // where the thread's two runs of 8 values lie, and its first pair (-1: none)
+  // where the thread's two runs of 8 values lie, and its first pair
   const int lane16 = (t % kLanes) * 16, within = lane16 - tp.r.offset;
   const bool halves = tp.r.layout == GRM_B200_ROTARY_HALF;
   const bool turns = side == 0 && within >= 0 && within < tp.r.dim;
-  const int pair0 = turns ? within / 2 : -1;
+  const int pair0 = within / 2;
   const int at0 = turns && halves ? tp.r.offset + pair0 : lane16;
   const int at1 = turns && halves ? at0 + tp.r.dim / 2 : lane16 + 8;
-  uint64_t freq[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) freq[i] = turns ? tp.r.turns[pair0 + i] : 0;
-
-  auto load = [&](int r, float (&v)[16]) {
+  const int r0 = t / kLanes;
+  auto load = [&](int r) {
     const uint16_t* row = x + r * row_stride;
-    const Chunk c{ld_nc16(row + at0), ld_nc16(row + at1)};
+    return Chunk{ld_nc16(row + at0), ld_nc16(row + at1)};
+  };
+  Chunk raw[kCache];
+#pragma unroll
+  for (int i = 0; i < kCache; ++i)
+    if (r0 + i * kRowsPass < rows) raw[i] = load(r0 + i * kRowsPass);
+  const float old = there && off > 0 ? *scale : 0.0f;
+
+  // Angle i of the pairs 8 n .. 8 n + 7 of row r is at (r * 8 + i) * eights + n: lanes
+  // of a row, whose eights follow one another, read different banks.
+  const int eights = tp.r.dim / 16;
+  int position0 = 0;
+  if (side == 0) {
+    position0 = tp.positions[entry.x];
+    const int pairs = tp.r.dim / 2, held = min(entry.w, kHeld) * pairs;
+    for (int y = threadIdx.x; y < held; y += GROUP * HEADS) {
+      const int r = y / pairs, i = y - r * pairs;
+      const Turn u = turn_of(position0 + r, tp.r.turns[i]);
+      angle[(r * 8 + i % 8) * eights + i / 8] =
+          make_float2(u.cos * tp.r.amplitude, u.sin * tp.r.amplitude);
+    }
+    __syncthreads();
+  }
+
+  auto take = [&](const Chunk& c, const float2 (&a)[8], float (&v)[16]) {
     const unsigned w[8] = {c.a.x, c.a.y, c.a.z, c.a.w, c.b.x, c.b.y, c.b.z, c.b.w};
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -290,10 +315,8 @@ __global__ void __launch_bounds__(256) append_turned_kernel(const TurnedParams t
     if (turns) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const Turn a = turn_of(position0 + r, freq[i]);
-        const float c1 = a.cos * tp.r.amplitude, s1 = a.sin * tp.r.amplitude;
         const float x1 = halves ? v[i] : v[2 * i], x2 = halves ? v[8 + i] : v[2 * i + 1];
-        const float y1 = x1 * c1 - x2 * s1, y2 = x2 * c1 + x1 * s1;
+        const float y1 = x1 * a[i].x - x2 * a[i].y, y2 = x2 * a[i].x + x1 * a[i].y;
         if (halves) {
           v[i] = y1;
           v[8 + i] = y2;
@@ -304,6 +327,17 @@ __global__ void __launch_bounds__(256) append_turned_kernel(const TurnedParams t
       }
     }
   };
+  auto again = [&](int r, float (&v)[16]) {  // a row that is not held
+    float2 a[8];
+    if (turns) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const Turn u = turn_of(position0 + r, tp.r.turns[pair0 + i]);
+        a[i] = make_float2(u.cos * tp.r.amplitude, u.sin * tp.r.amplitude);
+      }
+    }
+    take(load(r), a, v);
+  };
   // largest magnitude as bits, which order as numbers do, NaN above infinity
   auto widest = [](const float (&v)[16]) {
     unsigned m = 0;
@@ -312,31 +346,32 @@ __global__ void __launch_bounds__(256) append_turned_kernel(const TurnedParams t
     return m;
   };
 
-  const int r0 = t / kLanes;
-  float c[CACHE][16];
+  float c[kCache][16];
   unsigned m = 0;
 #pragma unroll
-  for (int i = 0; i < CACHE; ++i) {
+  for (int i = 0; i < kCache; ++i) {
     const int r = r0 + i * kRowsPass;
     if (r < rows) {
-      load(r, c[i]);
+      float2 a[8];
+      if (turns)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) a[k] = angle[(r * 8 + k) * eights + pair0 / 8];
+      take(raw[i], a, c[i]);
       m = max(m, widest(c[i]));
     }
   }
-  const float old = off > 0 ? *scale : 0.0f;
 #pragma unroll 1
-  for (int r = r0 + CACHE * kRowsPass; r < rows; r += kRowsPass) {
+  for (int r = r0 + kHeld; r < rows; r += kRowsPass) {
     float v[16];
-    load(r, v);
+    again(r, v);
     m = max(m, widest(v));
   }
   m = __reduce_max_sync(kFull, m);
   if (GROUP > 32) {  // the group's warps exchange their maxima
-    const int first = threadIdx.x / GROUP * (GROUP / 32);
     if (t % 32 == 0) warp_max[threadIdx.x / 32] = m;
-    asm volatile("bar.sync %0, %1;" ::"r"(1 + (int)threadIdx.x / GROUP), "n"(GROUP) : "memory");
+    asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(GROUP) : "memory");
 #pragma unroll
-    for (int w = 0; w < GROUP / 32; ++w) m = max(m, warp_max[first + w]);
+    for (int w = 0; w < GROUP / 32; ++w) m = max(m, warp_max[group * (GROUP / 32) + w]);
   }
   float s = __fdiv_rn(__uint_as_float(m), 127.0f);
   s = old > s || isnan(old) ? old : s;
@@ -352,16 +387,15 @@ __global__ void __launch_bounds__(256) append_turned_kernel(const TurnedParams t
     *reinterpret_cast<uint2*>(to + at1) = make_uint2(w[2], w[3]);
   };
 #pragma unroll
-  for (int i = 0; i < CACHE; ++i) {
-    const int r = r0 + i * kRowsPass;
-    if (r < rows) store(r, c[i]);
-  }
+  for (int i = 0; i < kCache; ++i)
+    if (r0 + i * kRowsPass < rows) store(r0 + i * kRowsPass, c[i]);
 #pragma unroll 1
-  for (int r = r0 + CACHE * kRowsPass; r < rows; r += kRowsPass) {
+  for (int r = r0 + kHeld; r < rows; r += kRowsPass) {
     float v[16];
-    load(r, v);
+    again(r, v);
     store(r, v);
   }
+  if (!there) return;
   if (off > 0 && !(s == old)) {
 #pragma unroll 1
     for (int r = r0; r < off; r += kRowsPass) {
@@ -379,19 +413,19 @@ __global__ void __launch_bounds__(256) append_turned_kernel(const TurnedParams t
   if (t == 0) *scale = s;
 }
 
-template <typename T, int D, int GROUP, int CACHE>
+template <typename T, int D, int GROUP, int HEADS>
 int launch_append_group(const TurnedParams& p, int64_t cap, cudaStream_t st) {
-  const int64_t blocks = ceil_div64(cap * p.a.kv_heads * 2, 256 / GROUP);
-  append_turned_kernel<T, D, GROUP, CACHE><<<(unsigned)blocks, 256, 0, st>>>(p);
+  const int64_t blocks = cap * ceil_div64(p.a.kv_heads, HEADS) * 2;
+  append_turned_kernel<T, D, GROUP, HEADS><<<(unsigned)blocks, GROUP * HEADS, 0, st>>>(p);
   return launch_status("paged append");
 }
 
 template <typename T, int D>
 int launch_append(const TurnedParams& p, int64_t cap, int64_t max_fresh, cudaStream_t st) {
   const int64_t values = std::min<int64_t>(max_fresh, (int64_t)1 << p.a.page_shift) * D;
-  if (values <= 32 * 32) return launch_append_group<T, D, 32, 2>(p, cap, st);
-  if (values <= 64 * 32) return launch_append_group<T, D, 64, 2>(p, cap, st);
-  if (values <= 128 * 32) return launch_append_group<T, D, 128, 2>(p, cap, st);
+  if (values <= 32 * 32) return launch_append_group<T, D, 32, 4>(p, cap, st);
+  if (values <= 64 * 32) return launch_append_group<T, D, 64, 4>(p, cap, st);
+  if (values <= 128 * 32) return launch_append_group<T, D, 128, 4>(p, cap, st);
   return launch_append_group<T, D, 256, 2>(p, cap, st);
 }
 

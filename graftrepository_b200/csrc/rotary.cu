@@ -4,10 +4,13 @@
 // and the inverse, which takes the same rotation off again (1 / a, -t).  fp32, one
 // rounding.
 //
-// Bound by HBM where rows are many: each value is read and written once.  A block
-// takes a few tokens: their angles go to shared memory once, whatever the number of
-// heads, then every thread takes eight pairs at a time (two loads and two stores of
-// 16 bytes), or one pair where strides, sizes or pointers are not multiples of that.
+// Bound by HBM where rows are many: each value is read and written once.  A warp takes
+// a token, or some heads of one where tokens are few.  Its first values are on their
+// way to registers, eight pairs a lane (two loads of 16 bytes), while it works out the
+// token's angles, once for all heads (about 25 instructions a pair; by each thread
+// anew they were half of the kernel's), into its own corner of shared memory, so that
+// no warp waits for another.  One pair at a time where strides, sizes or pointers are
+// not multiples of that.
 #include <algorithm>
 
 #include "rotary.cuh"
@@ -16,74 +19,105 @@ namespace grm_b200 {
 
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kAngles = 2048;  // pairs of a block's tokens: 16 KB of cos and sin
-constexpr int kMostDim = 2 * kAngles;
+// Heads that a lane holds at once: 128 bytes of values.
+template <typename T>
+constexpr int kHeldOf = sizeof(T) == 4 ? 2 : 4;
+constexpr int kMostDim = 4096;
+constexpr int kSharedAngles = 2048;  // of a block
 
 struct RotateParams {
   RotaryParams r;
   const void* x;
   void* out;
   const int32_t* positions;
-  int64_t tokens, x_row, x_head, out_row, out_head;
-  int heads, head_dim, inverse, copy;  // copy: values beside the rotated ones, too
-  int per_block;                       // tokens
-  int splits;                          // blocks that share a token's heads
+  int64_t x_row, x_head, out_row, out_head;
+  int tokens, heads, head_dim, inverse, copy;  // copy: values beside the rotated ones, too
+  int entries;  // places of V pairs, or of V values beside them, in a head
+  int lanes;    // heads that a warp takes side by side
+  int splits;   // warps that share a token's heads
+  int warps;    // of a block
 };
 
 template <typename T, int V, bool IN, bool OUT>
-__global__ void __launch_bounds__(kThreads) rotate_kernel(const RotateParams p) {
-  __shared__ float2 angle[kAngles];
-  const int pairs = p.r.dim >> 1;
-  const int64_t t0 = (int64_t)(blockIdx.x / p.splits) * p.per_block;
-  const int split = blockIdx.x % p.splits;
-  const int tokens = (int)(p.tokens - t0 < p.per_block ? p.tokens - t0 : p.per_block);
-  const float gain = p.inverse ? 1.0f / p.r.amplitude : p.r.amplitude;
-  for (int x = threadIdx.x; x < tokens * pairs; x += kThreads) {
-    const int position = p.positions[t0 + x / pairs];
-    // a row without a position stays as it is
-    Turn t{1.0f, 0.0f};
-    float g = 1.0f;
-    if (position >= 0) {
-      t = turn_of(position, p.r.turns[x % pairs]);
-      g = gain;
+__global__ void __launch_bounds__(256, 3) rotate_kernel(const RotateParams p) {
+  using W = Values<T, V>;
+  constexpr int kHeld = kHeldOf<T>;
+  __shared__ float2 angles[kSharedAngles];
+  const int pairs = p.r.dim >> 1, places = pairs / V, lane = threadIdx.x & 31;
+  // pair V n + i of the warp's token at i * places + n
+  float2* const angle = angles + (threadIdx.x >> 5) * pairs;
+  const unsigned warp = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  const int t = warp / p.splits, split = warp - t * p.splits;
+  if (t >= p.tokens) return;
+  const int h0 = p.heads * split / p.splits, h1 = p.heads * (split + 1) / p.splits;
+  const T* const x = static_cast<const T*>(p.x) + t * p.x_row;
+  T* const out = static_cast<T*>(p.out) + t * p.out_row;
+  const int first = lane / p.entries;  // of the heads side by side
+  const int position = p.positions[t];
+  bool turned = false;  // the angles are there
+#pragma unroll 1
+  for (int n = lane - first * p.entries; n - lane < p.entries; n += 32) {
+    const bool mine = first < p.lanes && n < p.entries, turns = n < places;
+    // where V pairs, or V values beside them, lie in a head
+    int i0 = p.r.offset + (IN ? 2 * n : n) * V, i1 = IN ? i0 + V : i0 + pairs;
+    int o0 = p.r.offset + (OUT ? 2 * n : n) * V, o1 = OUT ? o0 + V : o0 + pairs;
+    if (!turns) {
+      i0 = (n - places) * V;
+      if (i0 >= p.r.offset) i0 += p.r.dim;
+      i1 = o0 = o1 = i0;
     }
-    angle[x] = make_float2(t.cos * g, (p.inverse ? -t.sin : t.sin) * g);
-  }
-  __syncthreads();
-  const int h0 = (int)((int64_t)p.heads * split / p.splits);
-  const int h1 = (int)((int64_t)p.heads * (split + 1) / p.splits);
-  const T* const x = static_cast<const T*>(p.x);
-  T* const out = static_cast<T*>(p.out);
-  const int turned = pairs / V;  // entries of a head: its pairs, then what is copied
-  const int beside = p.copy ? (p.head_dim - p.r.dim) / V : 0;
-  const int entries = turned + beside, per_token = (h1 - h0) * entries;
-  for (int i = threadIdx.x; i < tokens * per_token; i += kThreads) {
-    const int t = i / per_token, y = i - t * per_token, h = h0 + y / entries, e = y % entries;
-    const T* from = x + (t0 + t) * p.x_row + h * p.x_head;
-    T* to = out + (t0 + t) * p.out_row + h * p.out_head;
-    if (e >= turned) {
-      int at = (e - turned) * V;
-      if (at >= p.r.offset) at += p.r.dim;
-      *reinterpret_cast<Values<T, V>*>(to + at) = *reinterpret_cast<const Values<T, V>*>(from + at);
-    } else if (p.positions[t0 + t] >= 0 || p.copy) {
-      if (p.positions[t0 + t] < 0) {  // out of place: as they came
-        for (int k = 0; k < 2 * V; ++k)
-          to[p.r.offset + 2 * e * V + k] = from[p.r.offset + 2 * e * V + k];
-        continue;
-      }
-      float2 a[V];
+    const T* from = x + (h0 + first) * p.x_head;
+    T* to = out + (h0 + first) * p.out_head;
+#pragma unroll 1
+    for (int h = h0 + first; h - first < h1; h += kHeld * p.lanes) {
+      W a[kHeld], b[kHeld];
 #pragma unroll
-      for (int k = 0; k < V; ++k) a[k] = angle[t * pairs + e * V + k];
-      turn_pairs<T, V, IN, OUT>(pairs, a, e * V, from + p.r.offset, to + p.r.offset);
+      for (int k = 0; k < kHeld; ++k)
+        if (mine && h + k * p.lanes < h1) {
+          a[k] = *reinterpret_cast<const W*>(from + k * p.lanes * p.x_head + i0);
+          if (turns) b[k] = *reinterpret_cast<const W*>(from + k * p.lanes * p.x_head + i1);
+        }
+      from += kHeld * p.lanes * p.x_head;
+      if (!turned) {
+        turned = true;
+        const float gain = p.inverse ? 1.0f / p.r.amplitude : p.r.amplitude;
+        for (int i = lane; i < pairs && position >= 0; i += 32) {
+          const Turn u = turn_of(position, p.r.turns[i]);
+          angle[i % V * places + i / V] =
+              make_float2(u.cos * gain, (p.inverse ? -u.sin : u.sin) * gain);
+        }
+        __syncwarp();
+      }
+      if (mine && turns && position >= 0) {
+        float2 c[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) c[i] = angle[i * places + n];
+#pragma unroll
+        for (int k = 0; k < kHeld; ++k)
+          if (h + k * p.lanes < h1) {
+            W y0, y1;
+            turn_values<T, V, IN, OUT>(c, a[k], b[k], &y0, &y1);
+            *reinterpret_cast<W*>(to + k * p.lanes * p.out_head + o0) = y0;
+            *reinterpret_cast<W*>(to + k * p.lanes * p.out_head + o1) = y1;
+          }
+      } else if (mine && p.copy) {
+        // beside the rotated ones, or a row without a position: as they came
+#pragma unroll
+        for (int k = 0; k < kHeld; ++k)
+          if (h + k * p.lanes < h1) {
+            *reinterpret_cast<W*>(to + k * p.lanes * p.out_head + i0) = a[k];
+            if (turns) *reinterpret_cast<W*>(to + k * p.lanes * p.out_head + i1) = b[k];
+          }
+      }
+      to += kHeld * p.lanes * p.out_head;
     }
   }
 }
 
 template <typename T, bool IN, bool OUT>
 void launch_layout(const RotateParams& p, bool wide, int64_t blocks, cudaStream_t st) {
-  if (wide) rotate_kernel<T, 8, IN, OUT><<<(unsigned)blocks, kThreads, 0, st>>>(p);
-  else rotate_kernel<T, 1, IN, OUT><<<(unsigned)blocks, kThreads, 0, st>>>(p);
+  if (wide) rotate_kernel<T, 8, IN, OUT><<<(unsigned)blocks, 32 * p.warps, 0, st>>>(p);
+  else rotate_kernel<T, 1, IN, OUT><<<(unsigned)blocks, 32 * p.warps, 0, st>>>(p);
 }
 
 template <typename T>
@@ -155,7 +189,7 @@ extern "C" int grm_b200_rotate(const grm_b200_rotary* rotary, const void* x_devi
   p.x = x_device;
   p.out = out_device;
   p.positions = positions_device;
-  p.tokens = tokens;
+  p.tokens = (int)tokens;
   p.x_row = x_row_stride;
   p.x_head = x_head_stride;
   p.out_row = out_row_stride;
@@ -170,17 +204,17 @@ extern "C" int grm_b200_rotate(const grm_b200_rotary* rotary, const void* x_devi
   const bool wide = words % 8 == 0 && p.r.dim % 16 == 0 &&
                     ((reinterpret_cast<uintptr_t>(x_device) |
                       reinterpret_cast<uintptr_t>(out_device)) & 15) == 0;
-  // about 4,096 values a block, fewer where that leaves SMs without one
-  const int64_t values = heads * head_dim;
-  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(4096 / std::max<int64_t>(values, 1),
-                                                              kAngles / (p.r.dim / 2)));
-  p.per_block = (int)std::max<int64_t>(1, std::min(most, tokens / (2 * info.sms)));
-  const int64_t groups = ceil_div64(tokens, p.per_block);
-  p.splits = groups >= 2 * info.sms
-                 ? 1
-                 : (int)std::min<int64_t>(heads, ceil_div64(2 * info.sms, groups));
+  const int v = wide ? 8 : 1;
+  p.entries = p.r.dim / 2 / v + (p.copy ? (p.head_dim - p.r.dim) / v : 0);
+  p.lanes = std::max(32 / p.entries, 1);
+  // a token's heads by several warps where that is what it takes to give every SM
+  // sixteen
+  p.splits = (int)std::max<int64_t>(
+      1, std::min<int64_t>(ceil_div64(heads, p.lanes), ceil_div64(16 * info.sms, tokens)));
+  const int64_t warps = tokens * p.splits;
+  p.warps = std::min(8, kSharedAngles / (p.r.dim / 2));
+  const int64_t blocks = ceil_div64(warps, p.warps);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const int64_t blocks = groups * p.splits;
   return dtype == GRM_B200_F32   ? launch<float>(p, wide, blocks, st)
          : dtype == GRM_B200_F16 ? launch<__half>(p, wide, blocks, st)
                                  : launch<__nv_bfloat16>(p, wide, blocks, st);

@@ -53,14 +53,14 @@ struct RotaryParams {
 };
 
 template <typename T>
-__device__ __forceinline__ float load1(const T* p);
+__device__ __forceinline__ float to_float(T v);
 template <>
-__device__ __forceinline__ float load1<float>(const float* p) { return *p; }
+__device__ __forceinline__ float to_float<float>(float v) { return v; }
 template <>
-__device__ __forceinline__ float load1<__half>(const __half* p) { return __half2float(*p); }
+__device__ __forceinline__ float to_float<__half>(__half v) { return __half2float(v); }
 template <>
-__device__ __forceinline__ float load1<__nv_bfloat16>(const __nv_bfloat16* p) {
-  return __bfloat162float(*p);
+__device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat16 v) {
+  return __bfloat162float(v);
 }
 template <typename T>
 __device__ __forceinline__ T round_to(float v);
@@ -72,15 +72,91 @@ template <>
 __device__ __forceinline__ __nv_bfloat16 round_to<__nv_bfloat16>(float v) {
   return __float2bfloat16_rn(v);
 }
+// Two 16-bit values in a word.
+template <typename T>
+__device__ __forceinline__ float2 unpack(uint32_t w);
+template <>
+__device__ __forceinline__ float2 unpack<__half>(uint32_t w) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+template <>
+__device__ __forceinline__ float2 unpack<__nv_bfloat16>(uint32_t w) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+}
+template <typename T>
+__device__ __forceinline__ uint32_t repack(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t repack<__half>(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t repack<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
 
-// V values of one load or store: 8, as 16 or 32 bytes, or 1.
+// V values of one load or store: 8 (16-bit ones two to a word, which half the
+// registers hold), or 1.
 template <typename T, int V>
-struct alignas(V * sizeof(T) < 16 ? sizeof(T) : 16) Values {
-  T v[V];
+struct Values;
+template <typename T>
+struct Values<T, 1> {
+  T v;
+  __device__ __forceinline__ void get(float (&x)[1]) const { x[0] = to_float(v); }
+  __device__ __forceinline__ void put(const float (&x)[1]) { v = round_to<T>(x[0]); }
+};
+template <typename T>
+struct alignas(16) Values<T, 8> {
+  uint32_t w[4];
+  __device__ __forceinline__ void get(float (&x)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 u = unpack<T>(w[i]);
+      x[2 * i] = u.x;
+      x[2 * i + 1] = u.y;
+    }
+  }
+  __device__ __forceinline__ void put(const float (&x)[8]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = repack<T>(x[2 * i], x[2 * i + 1]);
+  }
+};
+template <>
+struct alignas(16) Values<float, 8> {
+  float v[8];
+  __device__ __forceinline__ void get(float (&x)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = v[i];
+  }
+  __device__ __forceinline__ void put(const float (&x)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = x[i];
+  }
 };
 
-// V pairs of one head of 2 * half values, c the first of them, by their cos and
-// sin.  IN, OUT: a pair's members lie side by side.
+// V pairs by their cos and sin.  IN, OUT: a pair's members lie side by side (in a and
+// b one after another), else in a and b.
+template <typename T, int V, bool IN, bool OUT>
+__device__ __forceinline__ void turn_values(const float2 (&angle)[V], const Values<T, V>& a,
+                                            const Values<T, V>& b, Values<T, V>* c,
+                                            Values<T, V>* d) {
+  float x[V], y[V], u[V], v[V];
+  a.get(x);
+  b.get(y);
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const float x1 = IN ? (2 * i < V ? x[2 * i % V] : y[2 * i % V]) : x[i];
+    const float x2 = IN ? (2 * i + 1 < V ? x[(2 * i + 1) % V] : y[(2 * i + 1) % V]) : y[i];
+    const float y1 = x1 * angle[i].x - x2 * angle[i].y, y2 = x2 * angle[i].x + x1 * angle[i].y;
+    (OUT && 2 * i >= V ? v[2 * i % V] : u[OUT ? 2 * i % V : i]) = y1;
+    (OUT && 2 * i + 1 < V ? u[(2 * i + 1) % V] : v[OUT ? (2 * i + 1) % V : i]) = y2;
+  }
+  c->put(u);
+  d->put(v);
+}
+
+// The same of one head of 2 * half values, c the first pair.
 template <typename T, int V, bool IN, bool OUT>
 __device__ __forceinline__ void turn_pairs(int half, const float2 (&angle)[V], int c, const T* x,
                                            T* out) {
@@ -88,16 +164,7 @@ __device__ __forceinline__ void turn_pairs(int half, const float2 (&angle)[V], i
   const W a = *reinterpret_cast<const W*>(x + (IN ? 2 * c : c));
   const W b = *reinterpret_cast<const W*>(x + (IN ? 2 * c + V : half + c));
   W y0, y1;
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-    // pair i of V: members 2 i and 2 i + 1 of a and b side by side, or i of each
-    const float x1 = load1(IN && 2 * i >= V ? &b.v[2 * i - V] : &a.v[IN ? 2 * i : i]);
-    const float x2 = load1(IN && 2 * i + 1 < V ? &a.v[2 * i + 1] : &b.v[IN ? 2 * i + 1 - V : i]);
-    const float2 t = angle[i];
-    const T u = round_to<T>(x1 * t.x - x2 * t.y), v = round_to<T>(x2 * t.x + x1 * t.y);
-    (OUT && 2 * i >= V ? y1.v[OUT ? 2 * i - V : 0] : y0.v[OUT ? 2 * i : i]) = u;
-    (OUT && 2 * i + 1 < V ? y0.v[OUT ? 2 * i + 1 : 0] : y1.v[OUT ? 2 * i + 1 - V : i]) = v;
-  }
+  turn_values<T, V, IN, OUT>(angle, a, b, &y0, &y1);
   *reinterpret_cast<W*>(out + (OUT ? 2 * c : c)) = y0;
   *reinterpret_cast<W*>(out + (OUT ? 2 * c + V : half + c)) = y1;
 }
