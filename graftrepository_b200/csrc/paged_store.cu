@@ -123,17 +123,10 @@ __device__ __forceinline__ unsigned rescale4(unsigned v, float from, float to) {
 // read again (from L1 or L2).  Everything a group has to look up is one entry of
 // the step's list, so that two loads, not four, stand before the rows.
 template <typename T, int D, int GROUP, int CACHE>
-__global__ void __launch_bounds__(256) append_kernel(const AppendParams p) {
+__device__ __forceinline__ void append_one(const AppendParams& p, const int4 entry, int side, int h,
+                                           int t, int group, unsigned* warp_max) {
   constexpr int kLanes = D / 16;            // threads of a row
   constexpr int kRowsPass = GROUP / kLanes;
-  __shared__ unsigned warp_max[8];
-  const int t = threadIdx.x % GROUP;
-  const int64_t job = (int64_t)blockIdx.x * (256 / GROUP) + threadIdx.x / GROUP;
-  const int heads2 = p.kv_heads * 2;
-  const int64_t unit = job / heads2;
-  if (unit >= p.header->pages) return;
-  const int side = (int)(job % heads2) & 1, h = (int)(job % heads2) >> 1;
-  const int4 entry = p.pages[unit];
   const int off = entry.z;   // older tokens of the page
   const int rows = entry.w;  // the step's
   const int64_t page = min(max((int64_t)entry.y, (int64_t)0), p.ring_size - 1);
@@ -161,11 +154,10 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendParams p) {
     m = __vmaxu2(m, magnitude(load_chunk(x + r * row_stride)));
   m = __reduce_max_sync(kFull, max(m & 0xFFFFu, m >> 16));
   if (GROUP > 32) {  // the group's warps exchange their maxima
-    const int first = threadIdx.x / GROUP * (GROUP / 32);
     if (t % 32 == 0) warp_max[threadIdx.x / 32] = m;
-    asm volatile("bar.sync %0, %1;" ::"r"(1 + (int)threadIdx.x / GROUP), "n"(GROUP) : "memory");
+    asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(GROUP) : "memory");
 #pragma unroll
-    for (int w = 0; w < GROUP / 32; ++w) m = max(m, warp_max[first + w]);
+    for (int w = 0; w < GROUP / 32; ++w) m = max(m, warp_max[group * (GROUP / 32) + w]);
   }
   float s = __fdiv_rn(widen<T>(m).x, 127.0f);
   s = old > s || isnan(old) ? old : s;
@@ -203,6 +195,18 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendParams p) {
   if (t == 0) *scale = s;
 }
 
+template <typename T, int D, int GROUP, int CACHE>
+__global__ void __launch_bounds__(256) append_kernel(const AppendParams p) {
+  __shared__ unsigned warp_max[8];
+  const int64_t job = (int64_t)blockIdx.x * (256 / GROUP) + threadIdx.x / GROUP;
+  const int heads2 = p.kv_heads * 2;
+  const int64_t unit = job / heads2;
+  if (unit >= p.header->pages) return;
+  const int side = (int)(job % heads2) & 1, h = (int)(job % heads2) >> 1;
+  append_one<T, D, GROUP, CACHE>(p, p.pages[unit], side, h, threadIdx.x % GROUP,
+                                 threadIdx.x / GROUP, warp_max);
+}
+
 // ---- append with the keys rotated on the way
 //
 // As append_kernel, with the values held as fp32, 32 of them a thread.  A thread's 16
@@ -218,6 +222,13 @@ struct TurnedParams {
   RotaryParams r;
   const int32_t* positions;
 };
+
+// The largest of three, NaN if one of them is.
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 
 // Codes of 16 values in fp32, as quantise.
 __device__ __forceinline__ void quantise_turned(const float (&x)[16], float s, float inv,
@@ -247,10 +258,11 @@ __device__ __forceinline__ void quantise_turned(const float (&x)[16], float s, f
 }
 
 template <typename T, int D, int GROUP, int HEADS>
-__global__ void __launch_bounds__(GROUP * HEADS) append_turned_kernel(const TurnedParams tp) {
+__global__ void __launch_bounds__(GROUP * HEADS, 3) append_turned_kernel(const TurnedParams tp) {
   const AppendParams& p = tp.a;
   constexpr int kLanes = D / 16;  // threads of a row
   constexpr int kRowsPass = GROUP / kLanes, kCache = 2, kHeld = kCache * kRowsPass;
+  static_assert(GROUP * HEADS >= D / 2, "a thread a pair");
   __shared__ unsigned warp_max[GROUP * HEADS / 32];
   __shared__ float2 angle[kHeld * (D / 2)];  // [rows][pairs], each row's eights apart
   const int t = threadIdx.x % GROUP, group = threadIdx.x / GROUP;
@@ -261,19 +273,22 @@ __global__ void __launch_bounds__(GROUP * HEADS) append_turned_kernel(const Turn
   const int h = ((int)(blockIdx.x % sets2) >> 1) * HEADS + group;
   const bool there = h < p.kv_heads;
   const int4 entry = p.pages[unit];
+  if (side) {
+    if (there)
+      append_one<T, D, GROUP, GROUP == 32 ? 2 : 4>(p, entry, side, h, t, group, warp_max);
+    return;
+  }
   const int off = entry.z, rows = there ? entry.w : 0;
   const int64_t page = min(max((int64_t)entry.y, (int64_t)0), p.ring_size - 1);
-  const int64_t row_stride = side ? p.row_stride[1] : p.row_stride[0];
-  const uint16_t* const x = (side ? p.x[1] : p.x[0]) + (int64_t)entry.x * row_stride +
-                            h * (side ? p.head_stride[1] : p.head_stride[0]);
-  int8_t* const codes =
-      (side ? p.codes[1] : p.codes[0]) + (((page * p.kv_heads + h) << p.page_shift) * D);
-  float* const scale = (side ? p.scales[1] : p.scales[0]) + page * p.kv_heads + h;
+  const int64_t row_stride = p.row_stride[0];
+  const uint16_t* const x = p.x[0] + (int64_t)entry.x * row_stride + h * p.head_stride[0];
+  int8_t* const codes = p.codes[0] + (((page * p.kv_heads + h) << p.page_shift) * D);
+  float* const scale = p.scales[0] + page * p.kv_heads + h;
 
   // where the thread's two runs of 8 values lie, and its first pair
   const int lane16 = (t % kLanes) * 16, within = lane16 - tp.r.offset;
   const bool halves = tp.r.layout == GRM_B200_ROTARY_HALF;
-  const bool turns = side == 0 && within >= 0 && within < tp.r.dim;
+  const bool turns = within >= 0 && within < tp.r.dim;
   const int pair0 = within / 2;
   const int at0 = turns && halves ? tp.r.offset + pair0 : lane16;
   const int at1 = turns && halves ? at0 + tp.r.dim / 2 : lane16 + 8;
@@ -291,18 +306,18 @@ __global__ void __launch_bounds__(GROUP * HEADS) append_turned_kernel(const Turn
   // Angle i of the pairs 8 n .. 8 n + 7 of row r is at (r * 8 + i) * eights + n: lanes
   // of a row, whose eights follow one another, read different banks.
   const int eights = tp.r.dim / 16;
-  int position0 = 0;
-  if (side == 0) {
-    position0 = tp.positions[entry.x];
-    const int pairs = tp.r.dim / 2, held = min(entry.w, kHeld) * pairs;
-    for (int y = threadIdx.x; y < held; y += GROUP * HEADS) {
-      const int r = y / pairs, i = y - r * pairs;
-      const Turn u = turn_of(position0 + r, tp.r.turns[i]);
+  const int position0 = tp.positions[entry.x];
+  const int pairs = tp.r.dim / 2, held = min(entry.w, kHeld);
+  const int i = threadIdx.x % pairs, first = threadIdx.x / pairs;
+  const int step = max(GROUP * HEADS / pairs, 1);  // rows of a pass
+  const uint64_t turns_i = tp.r.turns[i];
+  if (first < step)
+    for (int r = first; r < held; r += step) {
+      const Turn u = turn_of(position0 + r, turns_i);
       angle[(r * 8 + i % 8) * eights + i / 8] =
           make_float2(u.cos * tp.r.amplitude, u.sin * tp.r.amplitude);
     }
-    __syncthreads();
-  }
+  __syncthreads();
 
   auto take = [&](const Chunk& c, const float2 (&a)[8], float (&v)[16]) {
     const unsigned w[8] = {c.a.x, c.a.y, c.a.z, c.a.w, c.b.x, c.b.y, c.b.z, c.b.w};
@@ -340,10 +355,10 @@ __global__ void __launch_bounds__(GROUP * HEADS) append_turned_kernel(const Turn
   };
   // largest magnitude as bits, which order as numbers do, NaN above infinity
   auto widest = [](const float (&v)[16]) {
-    unsigned m = 0;
+    float m = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) m = max(m, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-    return m;
+    for (int i = 0; i < 16; i += 2) m = max3_nan(m, fabsf(v[i]), fabsf(v[i + 1]));
+    return __float_as_uint(m) & 0x7FFFFFFFu;
   };
 
   float c[kCache][16];
@@ -423,10 +438,10 @@ int launch_append_group(const TurnedParams& p, int64_t cap, cudaStream_t st) {
 template <typename T, int D>
 int launch_append(const TurnedParams& p, int64_t cap, int64_t max_fresh, cudaStream_t st) {
   const int64_t values = std::min<int64_t>(max_fresh, (int64_t)1 << p.a.page_shift) * D;
-  if (values <= 32 * 32) return launch_append_group<T, D, 32, 4>(p, cap, st);
+  if (values <= 32 * 32) return launch_append_group<T, D, 32, 8>(p, cap, st);
   if (values <= 64 * 32) return launch_append_group<T, D, 64, 4>(p, cap, st);
-  if (values <= 128 * 32) return launch_append_group<T, D, 128, 4>(p, cap, st);
-  return launch_append_group<T, D, 256, 2>(p, cap, st);
+  if (values <= 128 * 32) return launch_append_group<T, D, 128, 2>(p, cap, st);
+  return launch_append_group<T, D, 256, 1>(p, cap, st);
 }
 
 template <typename T, int D, int GROUP, int CACHE>
