@@ -328,7 +328,7 @@ int fill(const grm_b200_latent_plan* plan, const grm_b200_latent_arena* arena, i
 }  // namespace
 
 int make_shape(const grm_b200_latent_plan& p, int sms, Shape* s) {
-  s->tiling[0] = absorbed_tiling(p.heads, p.latent, sms);
+  s->tiling[0] = absorbed_tiling(p.heads, p.latent, std::min(p.step.max_fresh, p.step.tokens), sms);
   s->tiling[1] = expanded_tiling(p.heads, sms);
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
@@ -341,8 +341,10 @@ int make_shape(const grm_b200_latent_plan& p, int sms, Shape* s) {
     s->off_base[f] = take((p.step.requests + 1) * 8);
     s->off_start[f] = take((int64_t)s->tiling[f].workers * (int64_t)sizeof(Start));
   }
-  const int64_t absorbed = (int64_t)s->tiling[0].workers * s->tiling[0].splits *
-                           slot_floats(kRows, std::min(p.latent, 256));
+  const Tiling& t = s->tiling[0];
+  const int64_t absorbed = (int64_t)t.workers * t.splits *
+                           (t.few ? slot_floats(t.few, p.latent)
+                                  : slot_floats(kRows, std::min(p.latent, 256)));
   const int64_t expanded =
       p.nope ? (int64_t)s->tiling[1].workers * slot_floats(2 * kRows, p.value) : 0;
   s->off_part = take(std::max(absorbed, expanded) * 2 * 4);
@@ -506,7 +508,8 @@ int grm_b200_latent_attend(const grm_b200_latent_plan* plan, const grm_b200_late
   p.qr = static_cast<const uint16_t*>(q_rope_device);
   p.qr_row = q_rope_row_stride;
   p.qr_head = q_rope_head_stride;
-  return launch_absorbed(p, static_cast<cudaStream_t>(stream));
+  return p.v.tiling.few ? launch_few(p, static_cast<cudaStream_t>(stream))
+                        : launch_absorbed(p, static_cast<cudaStream_t>(stream));
 }
 
 int grm_b200_latent_attend_expanded(const grm_b200_latent_plan* plan,

@@ -53,14 +53,21 @@ struct Tiling {
   int groups;   // tiles of the same tokens
   int splits;   // blocks that share a tile's values
   int workers;  // most
+  int few;      // columns of latent_few.cu's kernel, which serves the step; 0: it does not
 };
-__host__ __device__ inline Tiling absorbed_tiling(int heads, int latent, int sms) {
+// The absorbed form's kernel for few rows (latent_few.cu) takes requests whose rows of a
+// step fit its columns: 48, or 32 of a latent of 512.
+__host__ __device__ inline Tiling absorbed_tiling(int heads, int latent, int64_t most_tokens,
+                                                  int sms) {
+  const int64_t most = most_tokens * heads;
+  const int columns = latent == 512 ? 32 : 48;
+  if (most <= columns) return {(int)most_tokens, 1, 1, sms, most <= 16 ? 16 : columns};
   const int splits = latent > 256 ? latent / 256 : 1;
   return {heads <= kRows ? kRows / heads : 1, heads <= kRows ? 1 : (heads + kRows - 1) / kRows,
-          splits, sms / splits};
+          splits, sms / splits, 0};
 }
 __host__ __device__ inline Tiling expanded_tiling(int heads, int sms) {
-  return {2 * kRows, heads, 1, sms};
+  return {2 * kRows, heads, 1, sms, 0};
 }
 // fp32 of a partial result: [rows][values], then [rows][4] of reference exponent, sum,
 // sum of the rounded weights.
@@ -117,6 +124,7 @@ struct Params {
 };
 
 int launch_absorbed(const Params& p, cudaStream_t st);
+int launch_few(const Params& p, cudaStream_t st);
 int launch_expanded(const Params& p, cudaStream_t st);
 int launch_expand(const Params& p, cudaStream_t st);
 
@@ -226,12 +234,12 @@ struct Part {
   int r, g, tok0;       // request, group, first token of the tile within the step
   int toks[2];          // tokens of the two query tiles (the second one's: expanded form)
   int start, n, cached, len;
-  int step0, steps;     // of kStep tokens
+  int step0, steps;     // of STEP tokens
   int slot;             // where its result goes, -1: it is the whole tile's
 };
 
 // The parts of worker `w`, one after another.
-template <int QUERIES>
+template <int QUERIES, int STEP = kStep>
 struct Parts {
   Walk walk;
   int64_t u, end;
@@ -254,7 +262,7 @@ struct Parts {
     x->toks[0] = QUERIES == 2 ? imin(toks, kRows) : toks;
     x->toks[1] = QUERIES == 2 ? toks - x->toks[0] : 0;
     const int sees = p.causal ? imin(x->len, x->cached + x->tok0 + toks) : x->len;
-    const int all = (sees + kStep - 1) / kStep;
+    const int all = (sees + STEP - 1) / STEP;
     const int64_t units = walk.last - walk.first;
     const int64_t from = u - walk.first, to = imin(end, walk.last) - walk.first;
     x->step0 = (int)(all * from / units);

@@ -35,8 +35,7 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "latent.cuh"
-#include "umma.cuh"
+#include "latent_device.cuh"
 
 namespace grm_b200 {
 namespace latent {
@@ -89,121 +88,11 @@ struct Layout {
   static_assert(kQTmem % 128 == 0 || kQTmem == MAIN, "queries come 128 values at a time");
 };
 
-template <typename T>
-struct Kind;
-template <>
-struct Kind<__half> {
-  static constexpr uint32_t kFormat = 0;
-  // Weights times 2^7, at most 2^15: lost at the small end is then what lies below
-  // 2^-32 of a row's largest, not 2^-25.
-  static constexpr float kLift = paged::kLift;
-  static __device__ __forceinline__ uint32_t pack(float a, float b) {
-    return paged::pack_half2(a, b);
-  }
-  static __device__ __forceinline__ float2 widen(uint32_t v) {
-    return __half22float2(*reinterpret_cast<const __half2*>(&v));
-  }
-  static constexpr uint32_t kNoNumber = 0x7C00u;  // exponent bits
-};
-template <>
-struct Kind<__nv_bfloat16> {
-  static constexpr uint32_t kFormat = (1u << 7) | (1u << 10);
-  static constexpr float kLift = 0.0f;
-  static __device__ __forceinline__ uint32_t pack(float a, float b) {
-    return paged::pack_out<__nv_bfloat16>(a, b);
-  }
-  static __device__ __forceinline__ float2 widen(uint32_t v) {
-    return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xFFFF0000u));
-  }
-  static constexpr uint32_t kNoNumber = 0x7F80u;
-};
-
 // fp32 accumulators, 16-bit operands, 128 rows, n columns; B K-major or (b_mn) not.
 template <typename T>
 __host__ __device__ constexpr uint32_t idesc(int n, bool b_mn) {
   return (1u << 4) | Kind<T>::kFormat | (b_mn ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) |
          ((uint32_t)(kRows >> 4) << 24);
-}
-
-// Byte of 16-byte chunk c of row r: 128-byte rows of 8 chunks, 64-byte rows of 4.
-__device__ __forceinline__ uint32_t atom_byte(int r, int c) {
-  return r * 128 + ((c ^ (r & 7)) << 4);
-}
-__device__ __forceinline__ uint32_t half_atom_byte(int r, int c) {
-  return r * 64 + ((c ^ ((r >> 1) & 3)) << 4);
-}
-
-// Upper word of a shared-memory descriptor (umma.cuh's sw128_desc): 8-row groups of
-// 1024 bytes and a 128-byte swizzle, or of 512 and 64.
-constexpr uint32_t kHi128 = (uint32_t)(((uint64_t)64 << 32 | (uint64_t)1 << 46 |
-                                        (uint64_t)2 << 61) >> 32);
-constexpr uint32_t kHi64 = (uint32_t)(((uint64_t)32 << 32 | (uint64_t)1 << 46 |
-                                       (uint64_t)4 << 61) >> 32);
-
-__device__ __forceinline__ void tma_load(void* dst, const CUtensorMap* map, int x, int y,
-                                         uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%2, %3}], [%4];" ::"r"(smem_u32(dst)),
-      "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar))
-      : "memory");
-}
-
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
-}
-// Two numbers at a time.
-__device__ __forceinline__ float2 fma2(float a, float b, float k, float o) {
-  float2 r;
-  asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %4};\n"
-      " mov.b64 z, {%5, %5};\n fma.rn.f32x2 x, x, y, z;\n mov.b64 {%0, %1}, x;\n}\n"
-      : "=f"(r.x), "=f"(r.y)
-      : "f"(a), "f"(b), "f"(k), "f"(o));
-  return r;
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-  float2 r;
-  asm("{\n .reg .b64 x, y;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n"
-      " add.rn.f32x2 x, x, y;\n mov.b64 {%0, %1}, x;\n}\n"
-      : "=f"(r.x), "=f"(r.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return r;
-}
-
-// Every lane of a warp waits; false, for all of them, when a wait gave up.
-__device__ __noinline__ bool wait_long(uint64_t* bar, unsigned parity, volatile int* fail,
-                                       unsigned probes) {
-  bool ok = false;
-  for (unsigned i = 0; i < probes; ++i) {
-    if ((ok = mbar_try_wait(bar, parity))) break;
-    if (*fail) break;
-  }
-  ok = __all_sync(kFull, ok);
-  if (!ok) *fail = 1;
-  return ok;
-}
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, unsigned parity, volatile int* fail,
-                                          unsigned probes) {
-  if (__all_sync(kFull, mbar_try_wait(bar, parity))) return true;
-  return wait_long(bar, parity, fail, probes);
-}
-
-// Row of query tile t: its token within the step, its head, and whether there is one.
-struct Row {
-  int token, head;
-  bool active;
-};
-template <bool EXP>
-__device__ __forceinline__ Row row_of(const Params& p, const Part& x, int t, int row) {
-  if (EXP) return {x.tok0 + t * kRows + row, x.g, row < x.toks[t]};
-  if (p.v.tiling.groups > 1) {
-    const int h = x.g * kRows + row;
-    return {x.tok0, min(h, p.heads - 1), h < p.heads};
-  }
-  const int token = row / p.heads;
-  return {x.tok0 + token, row - token * p.heads, token < x.toks[0]};
 }
 
 // The scores of a step from the first hidden one on set to -inf, in tensor memory;
@@ -692,138 +581,6 @@ __global__ void __launch_bounds__(Layout<MAIN, ROPE, EXP>::kThreads, 1)
   }
 }
 
-constexpr int kJoinBlocks = 16;  // for every border between two shares
-
-// Parts of tiles that lie in the shares of several workers, and the rows past the
-// step's last one.  A tile in n parts has n - 1 borders inside, whose blocks share its
-// rows: 1 to 8 warps a row, each for some of the parts.
-template <typename T, int MAIN, int ROPE, bool EXP>
-__global__ void __launch_bounds__(256) join_kernel(const Params p) {
-  using LY = Layout<MAIN, ROPE, EXP>;
-  constexpr int kLanes = LY::kV / 4;  // float4 of a row
-  constexpr int kMine = (kLanes + 31) / 32;
-  __shared__ float4 sums[8][kLanes];
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const Header hd = *p.l.header;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int b = blockIdx.x / LY::kSplits + 1, split = blockIdx.x % LY::kSplits;
-  Start start;
-  if (b < hd.workers) start = p.l.start[b];
-  const int64_t used = p.v.starts[p.v.requests];
-  const int64_t id = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 256 + threadIdx.x;
-  for (int64_t i = used * p.heads * (MAIN / 8) + id; i < p.tokens * p.heads * (MAIN / 8);
-       i += (int64_t)gridDim.x * gridDim.y * 256) {
-    reinterpret_cast<uint4*>(p.out)[i] = make_uint4(0, 0, 0, 0);
-    if (p.lse && i % (MAIN / 8) == 0) p.lse[i / (MAIN / 8)] = -INFINITY;
-  }
-  if (b >= hd.workers) return;
-  Walk walk;
-  walk.start(p.v, start);
-  if (walk.first == worker_first(b, hd)) return;  // no border inside the tile
-  const int w0 = worker_of(walk.first, hd);       // worker of the tile's first part
-  const int parts = worker_of(walk.last - 1, hd) - w0 + 1;
-  Part x;
-  x.r = walk.r;
-  x.g = walk.g;
-  x.tok0 = walk.j * p.v.tiling.per;
-  const int toks = min(p.v.tiling.per, walk.q.n - x.tok0);
-  x.toks[0] = EXP ? min(toks, kRows) : toks;
-  x.toks[1] = EXP ? toks - x.toks[0] : 0;
-  const int rows = EXP ? toks
-                       : min(kRows, toks * (p.v.tiling.groups > 1 ? kRows : p.heads));
-  // rows of a block: 8, 4, 2 or 1, whichever is enough, and more where 8 are not
-  const int blocks = (parts - 1) * kJoinBlocks;
-  int each = 1;
-  while (each < 8 && each * blocks < rows) each *= 2;
-  const int warps = 8 / each, sub = warp % warps;  // of a row, and which of them
-  const int slot0 = 2 * w0 + (walk.first == worker_first(w0, hd) ? 0 : 1);
-  auto slot = [&](int k) {
-    const int at = k == 0 ? slot0 : 2 * (w0 + k);
-    return p.l.part + ((int64_t)at * LY::kSplits + split) * LY::kSlot;
-  };
-  const int block = (b - 1 - w0) * kJoinBlocks + blockIdx.y;
-  for (int row0 = block * each; row0 < rows; row0 += blocks * each) {
-    const int line = row0 + warp / warps;  // of the tile's rows
-    const Row a = row_of<EXP>(p, x, line / kRows, line % kRows);
-    const bool active = line < rows && a.active;
-    float m = -INFINITY, l = 0.0f, lr = 0.0f;
-    float4 o[kMine] = {};
-    if (active) {
-      auto state = [&](int k) {
-        return *reinterpret_cast<const float4*>(slot(k) + kRows * LY::kQueries * LY::kV +
-                                                4 * line);
-      };
-      // the largest reference exponent of the parts that see something, and the sums,
-      // lanes side by side
-      for (int k = lane; k < parts; k += 32) {
-        const float4 s = state(k);
-        if (s.y != 0.0f) m = fmaxf(m, s.x);
-      }
-#pragma unroll
-      for (int i = 16; i; i >>= 1) m = fmaxf(m, __shfl_xor_sync(kFull, m, i));
-      for (int k = lane; k < parts; k += 32) {
-        const float4 s = state(k);
-        const float f = s.x == m ? 1.0f : ex2(s.x - m);
-        if (s.y != 0.0f) {
-          l = fmaf(s.y, f, l);
-          lr = fmaf(s.z, f, lr);
-        }
-      }
-#pragma unroll
-      for (int i = 16; i; i >>= 1) {
-        l += __shfl_xor_sync(kFull, l, i);
-        lr += __shfl_xor_sync(kFull, lr, i);
-      }
-#pragma unroll 4
-      for (int k = sub; k < parts; k += warps) {
-        const float4 s = state(k);
-        const float f = s.x == m ? 1.0f : ex2(s.x - m);
-        const float4* from = reinterpret_cast<const float4*>(slot(k) + line * LY::kV);
-#pragma unroll
-        for (int i = 0; i < kMine; ++i)
-          if (lane + 32 * i < kLanes && s.y != 0.0f) {
-            const float4 v = from[lane + 32 * i];
-            o[i].x = fmaf(v.x, f, o[i].x);
-            o[i].y = fmaf(v.y, f, o[i].y);
-            o[i].z = fmaf(v.z, f, o[i].z);
-            o[i].w = fmaf(v.w, f, o[i].w);
-          }
-      }
-    }
-    if (warps > 1) {
-#pragma unroll
-      for (int i = 0; i < kMine; ++i)
-        if (lane + 32 * i < kLanes) sums[warp][lane + 32 * i] = o[i];
-      __syncthreads();
-      if (sub == 0)
-        for (int w = 1; w < warps; ++w)
-#pragma unroll
-          for (int i = 0; i < kMine; ++i)
-            if (lane + 32 * i < kLanes) {
-              const float4 v = sums[warp + w][lane + 32 * i];
-              o[i].x += v.x;
-              o[i].y += v.y;
-              o[i].z += v.z;
-              o[i].w += v.w;
-            }
-      __syncthreads();
-    }
-    if (!active || sub != 0) continue;
-    const int64_t orow = (int64_t)(walk.q.start + a.token) * p.heads + a.head;
-    const float inv = 1.0f / lr;
-#pragma unroll
-    for (int i = 0; i < kMine; ++i)
-      if (lane + 32 * i < kLanes)
-        reinterpret_cast<uint2*>(p.out + orow * MAIN + split * LY::kV)[lane + 32 * i] =
-            lr == 0.0f ? make_uint2(0, 0)
-                       : make_uint2(Kind<T>::pack(o[i].x * inv, o[i].y * inv),
-                                    Kind<T>::pack(o[i].z * inv, o[i].w * inv));
-    if (lane == 0 && p.lse && split == 0)
-      p.lse[orow] =
-          l == 0.0f ? -INFINITY : (m - Kind<T>::kLift + log2f(l)) * 0.693147180559945309f;
-  }
-}
-
 template <typename T, int MAIN, int ROPE, bool EXP>
 int launch(const Params& p, cudaStream_t st) {
   using LY = Layout<MAIN, ROPE, EXP>;
@@ -849,22 +606,7 @@ int launch(const Params& p, cudaStream_t st) {
     return rc;
   kernel<<<(unsigned)(p.v.tiling.workers * LY::kSplits), LY::kThreads, LY::kSmem, st>>>(maps, p);
   if ((rc = paged::launch_status("latent attend"))) return rc;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(std::max(p.v.tiling.workers - 1, 1) * LY::kSplits),
-                     kJoinBlocks);
-  cfg.blockDim = dim3(256);
-  cfg.stream = st;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, join_kernel<T, MAIN, ROPE, EXP>, p);
-  if (e != cudaSuccess) {
-    set_thread_error("latent join launch failed: %s", cudaGetErrorString(e));
-    return cuda_status(e);
-  }
-  return 0;
+  return launch_join<T, LY::kV, LY::kSplits, kRows * LY::kQueries, EXP>(p, st);
 }
 
 template <int MAIN, int ROPE, bool EXP>
