@@ -55,13 +55,13 @@ struct Tiling {
   int workers;  // most
   int few;      // columns of latent_few.cu's kernel, which serves the step; 0: it does not
 };
-// The absorbed form's kernel for few rows (latent_few.cu) takes requests whose rows of a
-// step fit its columns: 48, or 32 of a latent of 512.
+// The absorbed form's kernel for few rows (latent_few.cu) takes requests of up to 32 rows
+// of a step over a latent of 512, where latent_attend.cu's needs two blocks for a
+// tile and both work out the scores.
 __host__ __device__ inline Tiling absorbed_tiling(int heads, int latent, int64_t most_tokens,
                                                   int sms) {
   const int64_t most = most_tokens * heads;
-  const int columns = latent == 512 ? 32 : 48;
-  if (most <= columns) return {(int)most_tokens, 1, 1, sms, most <= 16 ? 16 : columns};
+  if (latent == 512 && most <= 32) return {(int)most_tokens, 1, 1, sms, most <= 16 ? 16 : 32};
   const int splits = latent > 256 ? latent / 256 : 1;
   return {heads <= kRows ? kRows / heads : 1, heads <= kRows ? 1 : (heads + kRows - 1) / kRows,
           splits, sms / splits, 0};

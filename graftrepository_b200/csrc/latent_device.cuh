@@ -77,6 +77,14 @@ __device__ __forceinline__ float2 fma2(float a, float b, float k, float o) {
       : "f"(a), "f"(b), "f"(k), "f"(o));
   return r;
 }
+__device__ __forceinline__ float2 fma2(float a, float b, float k, float2 o) {
+  float2 r;
+  asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %4};\n"
+      " mov.b64 z, {%5, %6};\n fma.rn.f32x2 x, x, y, z;\n mov.b64 {%0, %1}, x;\n}\n"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a), "f"(b), "f"(k), "f"(o.x), "f"(o.y));
+  return r;
+}
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   float2 r;
   asm("{\n .reg .b64 x, y;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n"

@@ -13,15 +13,15 @@
 // their exponentials 600.
 //
 // A block's warps:
-//   0-3  softmax, a token a lane: scores of all rows from tensor memory, weights to
-//        shared memory.  Reference exponents are the rows', in shared memory; they
-//        move (rarely, as they trail by up to 8) when a lane of the four warps finds a
-//        score too far above its row's
-//   4-7  queries to shared memory, results out
-//   8    products, issued by one elected lane
-//   9    rows from their pages to shared memory, 128 values of 128 tokens a place.  The
-//        next tokens' scores start on what has come while the weights of these are
-//        worked out, and a place is free when the values in it have been added up
+//   0-7   softmax, a token and half of the rows a lane: scores from tensor memory,
+//         weights to shared memory.  Reference exponents are the rows', in shared
+//         memory; they move (rarely, as they trail by up to 8) when a lane of the eight
+//         warps finds a score too far above its row's
+//   8-11  queries to shared memory, results out
+//   12    products, issued by one elected lane
+//   13    rows from their pages to shared memory, 128 values of 128 tokens a place.  The
+//         next tokens' scores start on what has come while the weights of these are
+//         worked out, and a place is free when the values in it have been added up
 #include <algorithm>
 
 #include "latent_device.cuh"
@@ -41,8 +41,9 @@ constexpr int kAtom = kTokens * 128;      // 128 tokens x 64 values
 constexpr int kPlace = 2 * kAtom;
 constexpr int kRopes = 2;
 constexpr uint32_t kTmemCols = 512;
-constexpr int kSoftWarps = 4, kOutWarps = 4, kMmaWarp = 8;  // and one that loads
-constexpr int kThreads = 10 * 32;
+constexpr int kSoftWarps = 8, kOutWarps = 4, kMmaWarp = 12;  // and one that loads
+constexpr int kSoftThreads = kSoftWarps * 32;
+constexpr int kThreads = 14 * 32;
 
 template <int LATENT, int ROPE, int N>
 struct Layout {
@@ -77,13 +78,13 @@ __host__ __device__ constexpr uint32_t idesc(int n, bool a_mn) {
 __device__ __forceinline__ bool soft_any(bool yes) {
   unsigned r;
   asm volatile("{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n"
-               " barrier.cta.red.or.pred q, 1, 128, p;\n selp.u32 %0, 1, 0, q;\n}\n"
+               " barrier.cta.red.or.pred q, 1, 256, p;\n selp.u32 %0, 1, 0, q;\n}\n"
                : "=r"(r)
                : "r"((unsigned)yes)
                : "memory");
   return r != 0;
 }
-__device__ __forceinline__ void soft_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+__device__ __forceinline__ void soft_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 __device__ __forceinline__ bool out_all(bool yes) {
   unsigned r;
   asm volatile("{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n"
@@ -98,19 +99,22 @@ __device__ __forceinline__ void out_sync() { asm volatile("bar.sync 2, 128;" :::
 // Sums over a warp's lanes of v[0..N), kSums<N> of them in a lane: those from
 // first_sum<N>(lane) on.  Lanes halve what they hold from step to step, as long as
 // that is an even number.
+constexpr int halvings(int n) { return n % 2 == 0 && n > 1 ? 1 + halvings(n / 2) : 0; }
 template <int N>
-constexpr int kSums = N % 32 == 0 ? N / 32 : N / 16;
+constexpr int kHalvings = halvings(N) < 5 ? halvings(N) : 5;
+template <int N>
+constexpr int kSums = N >> kHalvings<N>;
 template <int N>
 __device__ __forceinline__ int first_sum(int lane) {
-  return N % 32 == 0 ? lane * kSums<N> : (lane >> 1) * kSums<N>;
+  return (lane >> (5 - kHalvings<N>)) * kSums<N>;
 }
 template <int N>
 __device__ __forceinline__ void sum_lanes(float (&v)[N], int lane) {
-  int n = N;
 #pragma unroll
-  for (int o = 16; o; o >>= 1) {
-    if (n % 2 == 0) {
-      n >>= 1;
+  for (int step = 0; step < 5; ++step) {
+    const int o = 16 >> step;
+    if (step < kHalvings<N>) {
+      const int n = N >> (step + 1);
       const bool upper = lane & o;
 #pragma unroll
       for (int i = 0; i < N / 2; ++i)
@@ -125,13 +129,26 @@ __device__ __forceinline__ void sum_lanes(float (&v)[N], int lane) {
   }
 }
 
-// A float as an unsigned number of the same order.
-__device__ __forceinline__ unsigned ordered(float v) {
-  const unsigned b = __float_as_uint(v);
-  return b & 0x80000000u ? ~b : b | 0x80000000u;
+// Eight columns of a warp's 32 lanes; valid after a wait.
+__device__ __forceinline__ void tmem_ld8_nowait(uint32_t taddr, uint32_t* v) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]),
+                 "=r"(v[6]), "=r"(v[7])
+               : "r"(taddr));
 }
-__device__ __forceinline__ float from_ordered(unsigned v) {
-  return __uint_as_float(v & 0x80000000u ? v & 0x7FFFFFFFu : ~v);
+// A wait for such loads that also orders every use of v after it.
+template <int N>
+__device__ __forceinline__ void tmem_wait_all(uint32_t (&v)[N]) {
+  tmem_wait_ld();
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+r"(v[i]));
+}
+
+// The largest of a warp's 32 numbers, those that are none left out.
+__device__ __forceinline__ float warp_max(float v) {
+  float m;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
+  return m;
 }
 
 // Values of row `t` of a step's places that are no numbers, set to 0.
@@ -162,7 +179,7 @@ __device__ __noinline__ void lose_rows(const Params& p, const Header& hd, int wo
   while (parts.next(p, &x)) {
     const int rows = x.toks[0] * p.heads;
     const int64_t row0 = (int64_t)(x.start + x.tok0) * p.heads;
-    for (int n = threadIdx.x; n < rows; n += 128) {
+    for (int n = threadIdx.x; n < rows; n += kSoftThreads) {
       if (x.slot >= 0) {
         float* slot = p.l.part + (int64_t)x.slot * slot_floats(N, LATENT);
         *reinterpret_cast<float4*>(slot + N * LATENT + 4 * n) =
@@ -186,7 +203,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     few_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) {
   using LY = Layout<LATENT, ROPE, N>;
   constexpr int kPairs = LY::kPairs, kRing = LY::kRing;
-  constexpr int kCols = N % 32 == 0 ? 32 : 16;  // columns handled together
+  constexpr int kMine = N / 2;  // rows of a softmax lane
   extern __shared__ unsigned char raw[];
   unsigned char* const sm = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
   unsigned char* const sm_w = sm + LY::kWeightsAt;
@@ -198,8 +215,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ __align__(16) float ref[2][N];     // reference exponents of two tiles' rows
   __shared__ __align__(16) float off[N];        // what is added to a score: lift - reference
   __shared__ __align__(16) float factor[N];
-  __shared__ unsigned top[kSoftWarps][N];
-  __shared__ float sums[2][kSoftWarps][2][N];   // of weights, and of the rounded ones
+  __shared__ float top[4][N];
+  __shared__ float sums[2][4][2][N];            // of weights, and of the rounded ones
   __shared__ float inverse[N];
   __shared__ uint32_t sh_tmem;
   __shared__ int sh_fail;
@@ -246,9 +263,10 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp < kSoftWarps) {
     // ------------------------------------------------------------- softmax
-    const int tid = threadIdx.x;
-    const uint32_t lanes = (uint32_t)(warp * 32) << 16;
-    bool ok = true;  // the same in the four warps, which meet at barriers
+    const int tid = threadIdx.x, quarter = warp & 3, half = warp >> 2;
+    const int row0 = half * kMine, lane_tok = quarter * 32 + lane;
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+    bool ok = true;  // the same in the eight warps, which meet at barriers
     int it = 0, seg = 0;
 #pragma unroll 1
     while (ok && parts.next(p, &x)) {
@@ -261,86 +279,90 @@ __global__ void __launch_bounds__(kThreads, 1)
         off[tid] = INFINITY;
       }
       soft_sync();
-      float l[N], lr[N];
+      float l[kMine], lr[kMine];
 #pragma unroll
-      for (int n = 0; n < N; ++n) l[n] = lr[n] = 0.0f;
+      for (int n = 0; n < kMine; ++n) l[n] = lr[n] = 0.0f;
 #pragma unroll 1
       for (int i = 0; i < x.steps; ++i, ++it) {
         const int buf = it & 1;
-        const uint32_t s_col = tmem + lanes + LY::kScore + buf * N;
+        const uint32_t s_col = tmem + lanes + LY::kScore + buf * N + row0;
         ok = wait(&s_full[buf], (it >> 1) & 1);
         // and the weights of the step before last have been used
         if (ok && it >= 2) ok = wait(&pv_done[buf], ((it >> 1) - 1) & 1);
         tc_fence_after();
-        // rows from this one on see the lane's token
-        const int token = (x.step0 + i) * kTokens + tid;
+        uint32_t v[kMine];
+#pragma unroll
+        for (int c = 0; c < kMine; c += 8) tmem_ld8_nowait(s_col + c, v + c);
+        // rows from this one on (of the lane's) see the lane's token
+        const int token = (x.step0 + i) * kTokens + lane_tok;
         const int ahead = p.causal ? token - (x.cached + x.tok0) : 0;
-        const int from = token >= x.len ? N : ahead > 0 ? min(ahead * p.heads, N) : 0;
+        const int from = (token >= x.len ? N : ahead > 0 ? min(ahead * p.heads, N) : 0) - row0;
         const bool hides = __any_sync(kFull, from > 0);
-        // does a score pass its row's reference exponent by more than it may?
-        float far = -INFINITY;
+        tmem_wait_all(v);
+        // exponents; does one pass its row's reference by more than it may?
+        float y[kMine], far = -INFINITY;
+        auto exponents = [&] {
 #pragma unroll
-        for (int c = 0; c < N; c += kCols) {
-          uint32_t v[kCols];
-          if constexpr (kCols == 32) {
-            tmem_ld32_nowait(s_col + c, v);
-            tmem_wait_ld32(v);
-          } else {
-            tmem_ld16(s_col + c, v);
+          for (int k = 0; k < kMine; k += 4) {
+            const float4 o = *reinterpret_cast<const float4*>(&off[row0 + k]);
+            const float2 a = fma2(__uint_as_float(v[k]), __uint_as_float(v[k + 1]), p.scale_log2,
+                                  make_float2(o.x, o.y));
+            const float2 b = fma2(__uint_as_float(v[k + 2]), __uint_as_float(v[k + 3]),
+                                  p.scale_log2, make_float2(o.z, o.w));
+            y[k] = a.x;
+            y[k + 1] = a.y;
+            y[k + 2] = b.x;
+            y[k + 3] = b.y;
           }
+        };
+        exponents();
+        bool odd = false;  // a hidden score that is no finite number
+        if (hides) {
 #pragma unroll
-          for (int k = 0; k < kCols; k += 4) {
-            const float4 o = *reinterpret_cast<const float4*>(&off[c + k]);
-            float y[4] = {fmaf(__uint_as_float(v[k]), p.scale_log2, o.x),
-                          fmaf(__uint_as_float(v[k + 1]), p.scale_log2, o.y),
-                          fmaf(__uint_as_float(v[k + 2]), p.scale_log2, o.z),
-                          fmaf(__uint_as_float(v[k + 3]), p.scale_log2, o.w)};
-            if (hides)
-#pragma unroll
-              for (int j = 0; j < 4; ++j)
-                if (c + k + j < from) y[j] = -INFINITY;
-            far = max3(far, y[0], y[1]);
-            far = max3(far, y[2], y[3]);
-          }
+          for (int k = 0; k < kMine; ++k)
+            if (k < from) {
+              odd |= (v[k] & 0x7F800000u) == 0x7F800000u;
+              y[k] = -INFINITY;
+            }
         }
+#pragma unroll
+        for (int k = 0; k < kMine; k += 2) far = max3(far, y[k], y[k + 1]);
         if (soft_any(!ok || far > kLazy + Kind<T>::kLift)) {
           // every row's largest score, its reference exponent, what was added up so far
           if (soft_any(!ok)) { ok = false; break; }
-#pragma unroll 1
-          for (int c = 0; c < N; c += 16) {
-            uint32_t v[16];
-            tmem_ld16(s_col + c, v);
 #pragma unroll
-            for (int k = 0; k < 16; ++k) {
-              const float y = c + k < from ? -INFINITY : __uint_as_float(v[k]) * p.scale_log2;
-              const unsigned m = __reduce_max_sync(kFull, y != y ? 0u : ordered(y));
-              if (lane == 0) top[warp][c + k] = m;
-            }
+          for (int k = 0; k < kMine; ++k) {
+            const float m = warp_max(k < from ? -INFINITY : __uint_as_float(v[k]) * p.scale_log2);
+            if (lane == 0) top[quarter][row0 + k] = m;
           }
           soft_sync();
           if (tid < N) {
-            unsigned m = top[0][tid];
-#pragma unroll
-            for (int w = 1; w < kSoftWarps; ++w) m = max(m, top[w][tid]);
-            const float y = m == 0u ? -INFINITY : from_ordered(m), old = ref[ob][tid];
-            const float next = y > old + kLazy ? reference_of(y) : old;
+            const float m = fmaxf(fmaxf(top[0][tid], top[1][tid]), fmaxf(top[2][tid], top[3][tid]));
+            const float old = ref[ob][tid];
+            const float next = m > old + kLazy ? reference_of(m) : old;
             factor[tid] = next == old ? 1.0f : ex2(old - next);
             ref[ob][tid] = next;
             off[tid] = next == -INFINITY ? INFINITY : Kind<T>::kLift - next;
           }
           soft_sync();
+          exponents();
+          if (hides) {
+#pragma unroll
+            for (int k = 0; k < kMine; ++k)
+              if (k < from) y[k] = -INFINITY;
+          }
           if (i > 0) {
 #pragma unroll
-            for (int n = 0; n < N; ++n) {
-              l[n] *= factor[n];
-              lr[n] *= factor[n];
+            for (int n = 0; n < kMine; ++n) {
+              l[n] *= factor[row0 + n];
+              lr[n] *= factor[row0 + n];
             }
             // once the products of the step before have ended
             ok = wait(&pv_done[(it - 1) & 1], ((it - 1) >> 1) & 1);
             tc_fence_after();
             if (ok)
 #pragma unroll 1
-              for (int c = 0; c < kPairs * N; c += 16) {
+              for (int c = half * 16; c < kPairs * N; c += 32) {
                 const uint32_t at = tmem + lanes + LY::kResult + ob * kPairs * N + c;
                 uint32_t o[16];
                 tmem_ld16(at, o);
@@ -350,50 +372,23 @@ __global__ void __launch_bounds__(kThreads, 1)
                 tmem_st16(at, o);
               }
             tmem_wait_st();
-            tc_fence_before();
           }
         }
-        unsigned char* const weights = sm_w + buf * LY::kWeights + tid / 64 * (N * 128);
-        const int chunk = tid % 64 / 8;
-        bool odd = false;  // a hidden score that is no finite number
+        unsigned char* const weights =
+            sm_w + buf * LY::kWeights + lane_tok / 64 * (N * 128) + row0 * 128 + lane % 8 * 2;
+        const int chunk = lane_tok % 64 / 8;
 #pragma unroll
-        for (int c = 0; c < N; c += kCols) {
-          uint32_t v[kCols];
-          if constexpr (kCols == 32) {
-            tmem_ld32_nowait(s_col + c, v);
-            tmem_wait_ld32(v);
-          } else {
-            tmem_ld16(s_col + c, v);
-          }
-#pragma unroll
-          for (int k = 0; k < kCols; k += 4) {
-            const float4 o = *reinterpret_cast<const float4*>(&off[c + k]);
-            float e[4] = {ex2(fmaf(__uint_as_float(v[k]), p.scale_log2, o.x)),
-                          ex2(fmaf(__uint_as_float(v[k + 1]), p.scale_log2, o.y)),
-                          ex2(fmaf(__uint_as_float(v[k + 2]), p.scale_log2, o.z)),
-                          ex2(fmaf(__uint_as_float(v[k + 3]), p.scale_log2, o.w))};
-            if (hides)
-#pragma unroll
-              for (int j = 0; j < 4; ++j)
-                if (c + k + j < from) {
-                  odd |= (v[k + j] & 0x7F800000u) == 0x7F800000u;
-                  e[j] = 0.0f;
-                }
-#pragma unroll
-            for (int j = 0; j < 4; j += 2) {
-              const int n = c + k + j;
-              const uint32_t w = Kind<T>::pack(e[j], e[j + 1]);
-              const float2 r = Kind<T>::widen(w);
-              l[n] += e[j];
-              l[n + 1] += e[j + 1];
-              lr[n] += r.x;
-              lr[n + 1] += r.y;
-              *reinterpret_cast<uint16_t*>(weights + atom_byte(n, chunk) + tid % 8 * 2) =
-                  (uint16_t)w;
-              *reinterpret_cast<uint16_t*>(weights + atom_byte(n + 1, chunk) + tid % 8 * 2) =
-                  (uint16_t)(w >> 16);
-            }
-          }
+        for (int k = 0; k < kMine; k += 2) {
+          const float a = ex2(y[k]), b = ex2(y[k + 1]);
+          const uint32_t w = Kind<T>::pack(a, b);
+          const float2 r = Kind<T>::widen(w);
+          l[k] += a;
+          l[k + 1] += b;
+          lr[k] += r.x;
+          lr[k + 1] += r.y;
+          // rows of a half start at a multiple of eight: their places in it are the swizzle's
+          *reinterpret_cast<uint16_t*>(weights + atom_byte(k, chunk)) = (uint16_t)w;
+          *reinterpret_cast<uint16_t*>(weights + atom_byte(k + 1, chunk)) = (uint16_t)(w >> 16);
         }
         if (hides && __any_sync(kFull, odd)) {
           // the copies landed before the scores were there; seen here before the look at them
@@ -402,7 +397,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const unsigned s = (unsigned)it * kPairs + j;
             there = wait(&full[s % kRing], (s / kRing) & 1);
           }
-          if (there && odd) scrub<T, kPairs, kRing>(sm_ring, (unsigned)it * kPairs, tid);
+          if (there && odd) scrub<T, kPairs, kRing>(sm_ring, (unsigned)it * kPairs, lane_tok);
         }
         fence_proxy_async_smem();
         tc_fence_before();
@@ -411,45 +406,61 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (!ok) break;
       // sums over the tokens, for the warps that bring the results out
-      sum_lanes<N>(l, lane);
-      sum_lanes<N>(lr, lane);
+      sum_lanes<kMine>(l, lane);
+      sum_lanes<kMine>(lr, lane);
 #pragma unroll
-      for (int k = 0; k < kSums<N>; ++k) {
-        sums[ob][warp][0][first_sum<N>(lane) + k] = l[k];
-        sums[ob][warp][1][first_sum<N>(lane) + k] = lr[k];
+      for (int k = 0; k < kSums<kMine>; ++k) {
+        sums[ob][quarter][0][row0 + first_sum<kMine>(lane) + k] = l[k];
+        sums[ob][quarter][1][row0 + first_sum<kMine>(lane) + k] = lr[k];
       }
       __syncwarp();
-      soft_sync();  // nobody reads the next tile's exponents as this one's
       if (lane == 0) mbar_arrive(&fin_full[ob]);
       ++seg;
     }
   } else if (warp < kMmaWarp) {
     // ------------------------------------------------- queries in, results out
-    const int tid = threadIdx.x - 128;
+    const int tid = threadIdx.x - kSoftThreads;
     const uint32_t lanes = (uint32_t)((warp - kSoftWarps) * 32) << 16;
     bool ok = true;  // the same in the four warps
     int loaded = 0, seg = 0;
     auto queries = [&](const Part& y) {
       if (loaded > 0 && !(ok = wait(&q_empty, (loaded - 1) & 1))) return;
       ++loaded;
+      // a row's chunks of 16 bytes side by side, as many rows at a time as there are
+      // threads for, up to sixteen loads in flight
       constexpr int kChunks = (LATENT + ROPE) / 8;
+      constexpr int kRowLanes = kChunks <= 32 ? 32 : kChunks <= 64 ? 64 : 128;
+      constexpr int kRowsPass = 128 / kRowLanes, kPasses = N / kRowsPass;
+      constexpr int kBatch = kPasses <= 16 ? kPasses : kPasses % 16 == 0 ? 16 : 12;
+      static_assert(kPasses % kBatch == 0, "rows");
       const int rows = y.toks[0] * p.heads;
-#pragma unroll 4
-      for (int e = tid; e < N * kChunks; e += 128) {
-        const int n = e / kChunks, c = e - n * kChunks;
+#pragma unroll 1
+      for (int c = tid % kRowLanes; c < kChunks; c += kRowLanes) {
         const bool wide = c < LATENT / 8;
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (n < rows) {
-          const int t = n / p.heads, h = n - t * p.heads;
-          const int64_t token = y.start + y.tok0 + t;
-          v = wide ? __ldg(reinterpret_cast<const uint4*>(p.q + token * p.q_row + h * p.q_head) + c)
-                   : __ldg(reinterpret_cast<const uint4*>(p.qr + token * p.qr_row + h * p.qr_head) +
-                           (c - LATENT / 8));
-        }
         const int r = c - LATENT / 8;
-        *reinterpret_cast<uint4*>(
-            sm + (wide ? c / 8 * (N * 128) + atom_byte(n, c % 8)
-                       : LY::kQRopeAt + (ROPE == 64 ? atom_byte(n, r) : half_atom_byte(n, r)))) = v;
+        const uint16_t* const from = (wide ? p.q + c * 8 : p.qr + r * 8) +
+                                     (y.start + y.tok0) * (wide ? p.q_row : p.qr_row);
+        const int64_t row = wide ? p.q_row : p.qr_row, head = wide ? p.q_head : p.qr_head;
+#pragma unroll 1
+        for (int i0 = 0; i0 < kPasses; i0 += kBatch) {
+          uint4 v[kBatch];
+#pragma unroll
+          for (int i = 0; i < kBatch; ++i) {
+            const int n = (i0 + i) * kRowsPass + tid / kRowLanes;
+            const int t = y.toks[0] == 1 ? 0 : n / p.heads;
+            v[i] = n < rows ? __ldg(reinterpret_cast<const uint4*>(from + t * row +
+                                                                   (n - t * p.heads) * head))
+                            : make_uint4(0, 0, 0, 0);
+          }
+#pragma unroll
+          for (int i = 0; i < kBatch; ++i) {
+            const int n = (i0 + i) * kRowsPass + tid / kRowLanes;
+            *reinterpret_cast<uint4*>(
+                sm + (wide ? c / 8 * (N * 128) + atom_byte(n, c % 8)
+                           : LY::kQRopeAt + (ROPE == 64 ? atom_byte(n, r) : half_atom_byte(n, r)))) =
+                v[i];
+          }
+        }
       }
       fence_proxy_async_smem();
       __syncwarp();
@@ -477,7 +488,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (x.steps > 0) {
           m = ref[ob][tid];
 #pragma unroll
-          for (int w = 0; w < kSoftWarps; ++w) {
+          for (int w = 0; w < 4; ++w) {
             l += sums[ob][w][0][tid];
             lr += sums[ob][w][1][tid];
           }
@@ -492,26 +503,35 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       out_sync();
-      // a lane has one of the values, of all rows
+      // a lane has one of the values, of all rows: sixteen at a time
 #pragma unroll 1
-      for (int j = 0; j < kPairs; ++j) {
-        const int value = j * 128 + tid;
-#pragma unroll 1
-        for (int c = 0; c < N && c < rows; c += 16) {
-          uint32_t o[16];
-          if (x.steps > 0) tmem_ld16(tmem + lanes + LY::kResult + (ob * kPairs + j) * N + c, o);
+      for (int c = 0; c < N && c < rows; c += 16) {
+        uint32_t o[kPairs][16];
+        if (x.steps > 0)
 #pragma unroll
-          for (int k = 0; k < 16; ++k)
-            if (c + k < rows) {
-              if (x.slot >= 0) {
-                if (x.steps > 0) slot[(c + k) * LATENT + value] = __uint_as_float(o[k]);
-              } else {
-                const float inv = inverse[c + k];
-                p.out[(row0 + c + k) * LATENT + value] =
+          for (int j = 0; j < kPairs; ++j)
+            tmem_ld16(tmem + lanes + LY::kResult + (ob * kPairs + j) * N + c, o[j]);
+        if (x.slot >= 0) {
+          float* const to = slot + c * LATENT + tid;
+          if (x.steps > 0)
+#pragma unroll
+            for (int k = 0; k < 16; ++k)
+              if (c + k < rows)
+#pragma unroll
+                for (int j = 0; j < kPairs; ++j)
+                  to[k * LATENT + j * 128] = __uint_as_float(o[j][k]);
+        } else {
+          uint16_t* const to = p.out + (row0 + c) * LATENT + tid;
+#pragma unroll
+          for (int k = 0; k < 16; ++k) {
+            const float inv = inverse[c + k];
+            if (c + k < rows)
+#pragma unroll
+              for (int j = 0; j < kPairs; ++j)
+                to[k * LATENT + j * 128] =
                     inv == 0.0f ? (uint16_t)0
-                                : (uint16_t)Kind<T>::pack(__uint_as_float(o[k]) * inv, 0.0f);
-              }
-            }
+                                : (uint16_t)Kind<T>::pack(__uint_as_float(o[j][k]) * inv, 0.0f);
+          }
         }
       }
       tc_fence_before();
@@ -527,38 +547,54 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto desc = [&](uint32_t hi, uint32_t lo) { return (uint64_t)hi << 32 | lo; };
     int it = 0, seg = 0;
     bool ok = true;
-    // scores of step s from its places j0 .. j1 - 1, and from the positional part
-    auto scores = [&](int s, int j0, int j1) {
+    int part = 0;  // places of the step's scores that are done; kPairs: positional part next
+    // Goes on with the scores of step s, up to `most` places of it (kPairs + 1: all).  With a
+    // barrier `other` it gives way as soon as that one is through and rows are not there.
+    auto scores = [&](int s, int most, uint64_t* other, unsigned parity) {
       const uint32_t to = base + LY::kScore + (s & 1) * N;
 #pragma unroll 1
-      for (int j = j0; j < j1; ++j) {
-        const unsigned place = (unsigned)s * kPairs + j;
-        if (!(ok = wait(&full[place % kRing], (place / kRing) & 1))) return;
+      while (part < most) {
+        const unsigned place = (unsigned)s * kPairs + part;
+        const bool last = part == kPairs;
+        uint64_t* const bar = last ? &rope_full[s % kRopes] : &full[place % kRing];
+        const unsigned phase = (last ? (unsigned)s / kRopes : place / kRing) & 1;
+        if (other) {
+          bool there = false;
+          for (unsigned i = 0; i < p.probes; ++i) {
+            if ((there = __all_sync(kFull, mbar_try_wait(bar, phase)))) break;
+            if (__all_sync(kFull, mbar_try_wait(other, parity))) return;
+            if (*(volatile int*)&sh_fail) break;
+          }
+          if (!there) {
+            ok = wait(bar, phase);  // the limit is up, or somebody's was
+            if (!ok) return;
+          }
+        } else if (!(ok = wait(bar, phase))) {
+          return;
+        }
         tc_fence_after();
-        const uint32_t kd = k_lo + place % kRing * (kPlace / 16);
-        const uint32_t qd = q_lo + j * (2 * N * 128 / 16);
-        if (elect_one()) {
+        if (!last) {
+          const uint32_t kd = k_lo + place % kRing * (kPlace / 16);
+          const uint32_t qd = q_lo + part * (2 * N * 128 / 16);
+          if (elect_one()) {
 #pragma unroll
-          for (int k = 0; k < 8; ++k)
-            umma_f16(to, desc(kHi128, kd + (k / 4 * kAtom + k % 4 * 32) / 16),
-                     desc(kHi128, qd + (k / 4 * (N * 128) + k % 4 * 32) / 16),
-                     idesc<T>(N, false), j != 0 || k != 0);
+            for (int k = 0; k < 8; ++k)
+              umma_f16(to, desc(kHi128, kd + (k / 4 * kAtom + k % 4 * 32) / 16),
+                       desc(kHi128, qd + (k / 4 * (N * 128) + k % 4 * 32) / 16),
+                       idesc<T>(N, false), part != 0 || k != 0);
+          }
+        } else if (elect_one()) {
+          constexpr uint32_t kHi = ROPE == 64 ? kHi128 : kHi64;
+#pragma unroll
+          for (int k = 0; k < ROPE / 16; ++k)
+            umma_f16(to, desc(kHi, r_lo + (s % kRopes * LY::kRopeBytes + k * 32) / 16),
+                     desc(kHi, q_lo + (LY::kQRopeAt + k * 32) / 16), idesc<T>(N, false), 1);
+          umma_commit(&rope_empty[s % kRopes]);
+          umma_commit(&s_full[s & 1]);
         }
         __syncwarp();
+        ++part;
       }
-      if (j1 < kPairs) return;
-      if (!(ok = wait(&rope_full[s % kRopes], (s / kRopes) & 1))) return;
-      tc_fence_after();
-      if (elect_one()) {
-        constexpr uint32_t kHi = ROPE == 64 ? kHi128 : kHi64;
-#pragma unroll
-        for (int k = 0; k < ROPE / 16; ++k)
-          umma_f16(to, desc(kHi, r_lo + (s % kRopes * LY::kRopeBytes + k * 32) / 16),
-                   desc(kHi, q_lo + (LY::kQRopeAt + k * 32) / 16), idesc<T>(N, false), 1);
-        umma_commit(&rope_empty[s % kRopes]);
-        umma_commit(&s_full[s & 1]);
-      }
-      __syncwarp();
     };
 #pragma unroll 1
     while (ok && parts.next(p, &x)) {
@@ -568,15 +604,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       ok = wait(&q_full, seg & 1) && (seg < 2 || wait(&fin_empty[ob], ((seg >> 1) - 1) & 1));
       if (!ok) break;
       tc_fence_after();
-      scores(it, 0, kPairs);
+      part = 0;
+      scores(it, kPairs + 1, nullptr, 0);
       if (ok && steps == 1 && elect_one()) umma_commit(&q_empty);
       __syncwarp();
 #pragma unroll 1
       for (int i = 0; i < steps && ok; ++i) {
         const int s = it + i;
-        if (i + 1 < steps && LY::kPre > 0) scores(s + 1, 0, LY::kPre);
-        if (LY::kPre == kPairs && ok && i + 2 == steps && elect_one()) umma_commit(&q_empty);
-        __syncwarp();
+        part = 0;
+        // the next scores on what has come, as long as the weights are not there
+        if (i + 1 < steps)
+          scores(s + 1, LY::kPre == kPairs ? kPairs + 1 : LY::kPre, &p_full[s & 1], (s >> 1) & 1);
         if (!ok || !(ok = wait(&p_full[s & 1], (s >> 1) & 1))) break;
         tc_fence_after();
         const uint32_t wd = w_lo + (s & 1) * (LY::kWeights / 16);
@@ -599,8 +637,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           __syncwarp();
         }
-        if (i + 1 < steps && LY::kPre < kPairs) {
-          scores(s + 1, LY::kPre, kPairs);
+        if (i + 1 < steps) {
+          scores(s + 1, kPairs + 1, nullptr, 0);
           if (ok && i + 2 == steps && elect_one()) umma_commit(&q_empty);
           __syncwarp();
         }
@@ -700,20 +738,13 @@ int launch_kind(const Params& p, cudaStream_t st) {
 template <int LATENT, int ROPE>
 int launch_columns(const Params& p, cudaStream_t st) {
   return p.v.tiling.few == 16 ? launch_kind<LATENT, ROPE, 16>(p, st)
-                              : launch_kind<LATENT, ROPE, LATENT == 512 ? 32 : 48>(p, st);
-}
-
-template <int LATENT>
-int launch_rope(const Params& p, cudaStream_t st) {
-  return p.rope == 32 ? launch_columns<LATENT, 32>(p, st) : launch_columns<LATENT, 64>(p, st);
+                              : launch_kind<LATENT, ROPE, 32>(p, st);
 }
 
 }  // namespace
 
 int launch_few(const Params& p, cudaStream_t st) {
-  return p.latent == 128   ? launch_rope<128>(p, st)
-         : p.latent == 256 ? launch_rope<256>(p, st)
-                           : launch_rope<512>(p, st);
+  return p.rope == 32 ? launch_columns<512, 32>(p, st) : launch_columns<512, 64>(p, st);
 }
 
 }  // namespace latent
