@@ -20,9 +20,9 @@ constexpr int kExpandAlign = 64;
 // end.  Tiles lie one after another, a request's by group (a head of the expanded
 // form; of the absorbed one 128 heads) and then by token; a worker's share may start
 // and end inside a tile, whose parts join_kernel puts together.
-constexpr int kStart = 128;
+constexpr int kStart = 384;
 // Fewest units of a worker.
-constexpr int kLeast = 384;
+constexpr int kLeast = 640;
 
 struct Header {     // written by the schedule kernel, one for each form
   int64_t units;    // of all tiles
@@ -245,12 +245,14 @@ struct Parts {
   int64_t u, end;
   int w, count;
 
-  __host__ __device__ __forceinline__ Parts(const Params& p, const Header& h, int worker)
-      : u(worker_first(worker, h)), end(worker_first(worker + 1, h)), w(worker), count(0) {}
+  __host__ __device__ __forceinline__ Parts(const Params& p, const Header& h, int worker,
+                                            const Start& start)
+      : u(worker_first(worker, h)), end(worker_first(worker + 1, h)), w(worker), count(0) {
+    walk.start(p.v, start);
+  }
   __host__ __device__ __forceinline__ bool next(const Params& p, Part* x) {
     if (u >= end) return false;
-    if (count == 0) walk.start(p.v, p.l.start[w]);
-    else walk.next(p.v);
+    if (count > 0) walk.next(p.v);
     x->r = walk.r;
     x->g = walk.g;
     x->start = walk.q.start;

@@ -147,7 +147,7 @@ __device__ __noinline__ void lose_rows(const Params& p, const Header& hd, int wo
   using LY = Layout<MAIN, ROPE, EXP>;
   const float nan = __int_as_float(0x7FC00000);
   const int t = threadIdx.x >> 7, row = threadIdx.x & 127;
-  Parts<LY::kQueries> parts(p, hd, worker);
+  Parts<LY::kQueries> parts(p, hd, worker, p.l.start[worker]);
   Part x;
   while (parts.next(p, &x)) {
     const Row a = row_of<EXP>(p, x, t, row);
@@ -185,8 +185,9 @@ __global__ void __launch_bounds__(Layout<MAIN, ROPE, EXP>::kThreads, 1)
   __shared__ uint32_t sh_tmem;
   __shared__ int sh_fail;
 
-  const Header hd = *p.l.header;
   const int worker = blockIdx.x / LY::kSplits, split = blockIdx.x % LY::kSplits;
+  const Start begin = p.l.start[worker];  // on its way beside the header
+  const Header hd = *p.l.header;
   asm volatile("griddepcontrol.launch_dependents;");
   if (worker >= hd.workers) return;
 
@@ -224,7 +225,7 @@ __global__ void __launch_bounds__(Layout<MAIN, ROPE, EXP>::kThreads, 1)
   auto wait = [&](uint64_t* bar, unsigned parity) {
     return warp_wait(bar, parity, &sh_fail, p.probes);
   };
-  Parts<kQ> parts(p, hd, worker);
+  Parts<kQ> parts(p, hd, worker, begin);
   Part x;
 
   if (warp < LY::kSoftWarps) {
@@ -237,59 +238,69 @@ __global__ void __launch_bounds__(Layout<MAIN, ROPE, EXP>::kThreads, 1)
     unsigned char* const my_q = sm_q + t * LY::kQuery;
     bool ok = true;
     int it = 0, tile = 0, stage0 = 0;  // steps and tiles of this query tile; stages so far
+    // the row's query of a part, to tensor memory and shared memory
+    auto queries = [&](const Part& y) {
+      const Row b = row_of<EXP>(p, y, t, row);
+      const uint16_t* qp = p.q + (int64_t)(y.start + b.token) * p.q_row + b.head * p.q_head;
+      const uint16_t* rp = p.qr + (int64_t)(y.start + b.token) * p.qr_row + b.head * p.qr_head;
+      auto chunk = [&](const uint16_t* from, int c) {
+        return b.active ? __ldg(reinterpret_cast<const uint4*>(from) + c)
+                        : make_uint4(0, 0, 0, 0);
+      };
+      // sixteen loads in flight
 #pragma unroll 1
-    while (ok && parts.next(p, &x)) {
-      const int steps = x.steps, stage_base = stage0;
-      stage0 += steps;
-      if (x.toks[t] == 0) continue;
-      const Row a = row_of<EXP>(p, x, t, row);
-      float m = -INFINITY, l = 0.0f, lr = 0.0f;
-      if (steps > 0) {
-        // the row's query, to tensor memory and shared memory
-        const uint16_t* qp = p.q + (int64_t)(x.start + a.token) * p.q_row + a.head * p.q_head;
-        const uint16_t* rp = p.qr + (int64_t)(x.start + a.token) * p.qr_row + a.head * p.qr_head;
-        auto chunk = [&](const uint16_t* from, int c) {
-          return a.active ? __ldg(reinterpret_cast<const uint4*>(from) + c)
-                          : make_uint4(0, 0, 0, 0);
-        };
-        // sixteen loads in flight
-#pragma unroll 1
-        for (int c = 0; c < MAIN / 8; c += 16) {
-          uint4 v[16];
+      for (int c = 0; c < MAIN / 8; c += 16) {
+        uint4 v[16];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) v[i] = MAIN >= 128 || i < MAIN / 8 ? chunk(qp, c + i) : uint4{};
-          if (c < LY::kQTmem / 8) {
+        for (int i = 0; i < 16; ++i) v[i] = MAIN >= 128 || i < MAIN / 8 ? chunk(qp, c + i) : uint4{};
+        if (c < LY::kQTmem / 8) {
 #pragma unroll
-            for (int i = 0; i < 16 && i < MAIN / 8; i += 4) {
-              const uint32_t w[16] = {v[i].x, v[i].y, v[i].z, v[i].w, v[i + 1].x, v[i + 1].y,
-                                      v[i + 1].z, v[i + 1].w, v[i + 2].x, v[i + 2].y, v[i + 2].z,
-                                      v[i + 2].w, v[i + 3].x, v[i + 3].y, v[i + 3].z, v[i + 3].w};
-              tmem_st16(q_col + 4 * (c + i), w);
-            }
-          } else {
+          for (int i = 0; i < 16 && i < MAIN / 8; i += 4) {
+            const uint32_t w[16] = {v[i].x, v[i].y, v[i].z, v[i].w, v[i + 1].x, v[i + 1].y,
+                                    v[i + 1].z, v[i + 1].w, v[i + 2].x, v[i + 2].y, v[i + 2].z,
+                                    v[i + 2].w, v[i + 3].x, v[i + 3].y, v[i + 3].z, v[i + 3].w};
+            tmem_st16(q_col + 4 * (c + i), w);
+          }
+        } else {
 #pragma unroll
-            for (int i = 0; i < 16 && i < MAIN / 8; ++i) {
-              const int y = c + i - LY::kQTmem / 8;
-              *reinterpret_cast<uint4*>(my_q + (y / 8) * kQueryAtom + atom_byte(row, y % 8)) = v[i];
-            }
+          for (int i = 0; i < 16 && i < MAIN / 8; ++i) {
+            const int z = c + i - LY::kQTmem / 8;
+            *reinterpret_cast<uint4*>(my_q + (z / 8) * kQueryAtom + atom_byte(row, z % 8)) = v[i];
           }
         }
-        {
-          uint4 v[ROPE / 8];
-#pragma unroll
-          for (int c = 0; c < ROPE / 8; ++c) v[c] = chunk(rp, c);
-#pragma unroll
-          for (int c = 0; c < ROPE / 8; ++c)
-            *reinterpret_cast<uint4*>(
-                my_q + LY::kQRopeAt +
-                (ROPE == 64 ? atom_byte(row, c) : half_atom_byte(row, c))) = v[c];
-        }
-        tmem_wait_st();
-        tc_fence_before();
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&q_full[t]);
       }
+      {
+        uint4 v[ROPE / 8];
+#pragma unroll
+        for (int c = 0; c < ROPE / 8; ++c) v[c] = chunk(rp, c);
+#pragma unroll
+        for (int c = 0; c < ROPE / 8; ++c)
+          *reinterpret_cast<uint4*>(
+              my_q + LY::kQRopeAt +
+              (ROPE == 64 ? atom_byte(row, c) : half_atom_byte(row, c))) = v[c];
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&q_full[t]);
+    };
+    Part next;
+    bool more = parts.next(p, &next);
+    if (more && next.steps > 0 && next.toks[t] > 0) queries(next);
+#pragma unroll 1
+    while (ok && more) {
+      x = next;
+      more = parts.next(p, &next);
+      const bool queue = more && next.steps > 0 && next.toks[t] > 0;
+      const int steps = x.steps, stage_base = stage0;
+      stage0 += steps;
+      if (x.toks[t] == 0) {
+        if (queue) queries(next);
+        continue;
+      }
+      const Row a = row_of<EXP>(p, x, t, row);
+      float m = -INFINITY, l = 0.0f, lr = 0.0f;
 
       // tokens that the row sees, from the part's first on
       const int lim = (p.causal ? min(x.len, x.cached + a.token + 1) : x.len) - x.step0 * kStep;
@@ -368,6 +379,9 @@ __global__ void __launch_bounds__(Layout<MAIN, ROPE, EXP>::kThreads, 1)
         if (lane == 0) mbar_arrive(&p_full[t][buf]);
       }
       if (!ok) break;
+      // The scores of this tile are there, so its queries' place is free: the next
+      // tile's first scores are worked out while this one's result goes out.
+      if (queue) queries(next);
       if (steps > 0) {
         if (!(ok = wait(&o_done[t], tile & 1))) break;
         tc_fence_after();

@@ -174,7 +174,7 @@ __device__ __noinline__ void scrub(unsigned char* ring, unsigned place0, int t) 
 template <int LATENT, int N>
 __device__ __noinline__ void lose_rows(const Params& p, const Header& hd, int worker) {
   const float nan = __int_as_float(0x7FC00000);
-  Parts<1, kTokens> parts(p, hd, worker);
+  Parts<1, kTokens> parts(p, hd, worker, p.l.start[worker]);
   Part x;
   while (parts.next(p, &x)) {
     const int rows = x.toks[0] * p.heads;
@@ -221,8 +221,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ uint32_t sh_tmem;
   __shared__ int sh_fail;
 
-  const Header hd = *p.l.header;
   const int worker = blockIdx.x;
+  const Start begin = p.l.start[worker];  // on its way beside the header
+  const Header hd = *p.l.header;
   asm volatile("griddepcontrol.launch_dependents;");
   if (worker >= hd.workers) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -258,7 +259,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto wait = [&](uint64_t* bar, unsigned parity) {
     return warp_wait(bar, parity, &sh_fail, p.probes);
   };
-  Parts<1, kTokens> parts(p, hd, worker);
+  Parts<1, kTokens> parts(p, hd, worker, begin);
   Part x;
 
   if (warp < kSoftWarps) {
@@ -427,11 +428,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (loaded > 0 && !(ok = wait(&q_empty, (loaded - 1) & 1))) return;
       ++loaded;
       // a row's chunks of 16 bytes side by side, as many rows at a time as there are
-      // threads for, up to sixteen loads in flight
+      // threads for, eight loads in flight
       constexpr int kChunks = (LATENT + ROPE) / 8;
       constexpr int kRowLanes = kChunks <= 32 ? 32 : kChunks <= 64 ? 64 : 128;
       constexpr int kRowsPass = 128 / kRowLanes, kPasses = N / kRowsPass;
-      constexpr int kBatch = kPasses <= 16 ? kPasses : kPasses % 16 == 0 ? 16 : 12;
+      constexpr int kBatch = 8;
       static_assert(kPasses % kBatch == 0, "rows");
       const int rows = y.toks[0] * p.heads;
 #pragma unroll 1
@@ -505,32 +506,26 @@ __global__ void __launch_bounds__(kThreads, 1)
       out_sync();
       // a lane has one of the values, of all rows: sixteen at a time
 #pragma unroll 1
-      for (int c = 0; c < N && c < rows; c += 16) {
-        uint32_t o[kPairs][16];
-        if (x.steps > 0)
-#pragma unroll
-          for (int j = 0; j < kPairs; ++j)
-            tmem_ld16(tmem + lanes + LY::kResult + (ob * kPairs + j) * N + c, o[j]);
+      for (int c = 0; c < kPairs * N; c += 16) {
+        const int j = c / N, n = c % N;  // 128 values, and the first row
+        if (n >= rows) continue;
+        uint32_t o[16];
+        if (x.steps > 0) tmem_ld16(tmem + lanes + LY::kResult + ob * kPairs * N + c, o);
         if (x.slot >= 0) {
-          float* const to = slot + c * LATENT + tid;
+          float* const to = slot + n * LATENT + j * 128 + tid;
           if (x.steps > 0)
 #pragma unroll
             for (int k = 0; k < 16; ++k)
-              if (c + k < rows)
-#pragma unroll
-                for (int j = 0; j < kPairs; ++j)
-                  to[k * LATENT + j * 128] = __uint_as_float(o[j][k]);
+              if (n + k < rows) to[k * LATENT] = __uint_as_float(o[k]);
         } else {
-          uint16_t* const to = p.out + (row0 + c) * LATENT + tid;
+          uint16_t* const to = p.out + (row0 + n) * LATENT + j * 128 + tid;
 #pragma unroll
           for (int k = 0; k < 16; ++k) {
-            const float inv = inverse[c + k];
-            if (c + k < rows)
-#pragma unroll
-              for (int j = 0; j < kPairs; ++j)
-                to[k * LATENT + j * 128] =
-                    inv == 0.0f ? (uint16_t)0
-                                : (uint16_t)Kind<T>::pack(__uint_as_float(o[j][k]) * inv, 0.0f);
+            const float inv = inverse[n + k];
+            if (n + k < rows)
+              to[k * LATENT] =
+                  inv == 0.0f ? (uint16_t)0
+                              : (uint16_t)Kind<T>::pack(__uint_as_float(o[k]) * inv, 0.0f);
           }
         }
       }
