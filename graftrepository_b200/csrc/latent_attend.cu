@@ -291,14 +291,20 @@ __global__ void __launch_bounds__(Layout<MAIN, ROPE, EXP>::kThreads, 1)
 #pragma unroll 1
     while (ok && more) {
       x = next;
-      more = parts.next(p, &next);
-      const bool queue = more && next.steps > 0 && next.toks[t] > 0;
       const int steps = x.steps, stage_base = stage0;
       stage0 += steps;
+      bool queue = false;
+      // the next part, a chain of loads that lies under the wait for the second scores
+      auto look = [&] {
+        more = parts.next(p, &next);
+        queue = more && next.steps > 0 && next.toks[t] > 0;
+      };
       if (x.toks[t] == 0) {
+        look();
         if (queue) queries(next);
         continue;
       }
+      if (steps == 0) look();
       const Row a = row_of<EXP>(p, x, t, row);
       float m = -INFINITY, l = 0.0f, lr = 0.0f;
 
@@ -312,6 +318,7 @@ __global__ void __launch_bounds__(Layout<MAIN, ROPE, EXP>::kThreads, 1)
         tc_fence_after();
         if (idle) {
           if (lane == 0) mbar_arrive(&p_full[t][buf]);
+          if (i == 0) look();
           continue;
         }
         if (__any_sync(kFull, (i + 1) * kStep > lim)) {
@@ -377,6 +384,7 @@ __global__ void __launch_bounds__(Layout<MAIN, ROPE, EXP>::kThreads, 1)
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[t][buf]);
+        if (i == 0) look();
       }
       if (!ok) break;
       // The scores of this tile are there, so its queries' place is free: the next
@@ -488,9 +496,13 @@ __global__ void __launch_bounds__(Layout<MAIN, ROPE, EXP>::kThreads, 1)
       scores(i);
       return true;
     };
+    Part next;
+    bool more = parts.next(p, &next);
 #pragma unroll 1
-    while (ok && parts.next(p, &x)) {
+    while (ok && more) {
+      x = next;
       const int steps = __shfl_sync(kFull, x.steps, 0);
+      if (x.toks[t] == 0 || steps == 0) more = parts.next(p, &next);
       if (x.toks[t] == 0) {  // nothing to do for this one: give the stages back
 #pragma unroll 1
         for (int i = 0; i < steps && ok; ++i) {
@@ -507,6 +519,7 @@ __global__ void __launch_bounds__(Layout<MAIN, ROPE, EXP>::kThreads, 1)
       if (!ok) break;
       tc_fence_after();
       ok = next_scores(0) && (steps < 2 || next_scores(1));
+      more = parts.next(p, &next);  // under the first softmax
 #pragma unroll 1
       for (int i = 0; i < steps && ok; ++i) {
         const int s = (stage0 + i) % kStages, buf = (it + i) & 1;

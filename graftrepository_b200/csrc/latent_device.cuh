@@ -130,37 +130,42 @@ __device__ __forceinline__ Row row_of(const Params& p, const Part& x, int t, int
 
 // ---- joining the parts of tiles
 
-constexpr int kJoinBlocks = 16;  // for every border between two shares
+constexpr int kJoinBlocks = 8;  // for every border between two shares
 
 // Parts of tiles that lie in the shares of several workers, and the rows past the
 // step's last one.  A tile in n parts has n - 1 borders inside, whose blocks share its
-// rows: 1 to 8 warps a row, each for some of the parts.
+// rows: 1 to 8 warps a row, each for some of its values; lanes beyond those take every
+// so many of the parts.  Takes no shared memory, so that blocks get their place, and
+// find theirs in the lists, while attention still runs.
 // ROWS of a tile, V values of a block's results, SPLITS blocks that share a tile's.
 template <typename T, int V, int SPLITS, int ROWS, bool EXP>
 __global__ void __launch_bounds__(256) join_kernel(const Params p) {
   constexpr int kWide = V * SPLITS, kSlot = slot_floats(ROWS, V);
   constexpr int kLanes = V / 4;  // float4 of a row
   constexpr int kMine = (kLanes + 31) / 32;
-  __shared__ float4 sums[8][kLanes];
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const Header hd = *p.l.header;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int b = blockIdx.x / SPLITS + 1, split = blockIdx.x % SPLITS;
-  Start start;
-  if (b < hd.workers) start = p.l.start[b];
+  // the lists are the plan's, which was there before attention began
+  const Start start = p.l.start[min(b, p.v.tiling.workers - 1)];
+  const Header hd = *p.l.header;
   const int64_t used = p.v.starts[p.v.requests];
+  bool joins = b < hd.workers;
+  Walk walk;
+  int w0 = 0, parts = 0;
+  if (joins) {
+    walk.start(p.v, start);
+    joins = walk.first != worker_first(b, hd);  // a border inside the tile
+    w0 = worker_of(walk.first, hd);             // worker of the tile's first part
+    parts = worker_of(walk.last - 1, hd) - w0 + 1;
+  }
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int64_t id = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 256 + threadIdx.x;
   for (int64_t i = used * p.heads * (kWide / 8) + id; i < p.tokens * p.heads * (kWide / 8);
        i += (int64_t)gridDim.x * gridDim.y * 256) {
     reinterpret_cast<uint4*>(p.out)[i] = make_uint4(0, 0, 0, 0);
     if (p.lse && i % (kWide / 8) == 0) p.lse[i / (kWide / 8)] = -INFINITY;
   }
-  if (b >= hd.workers) return;
-  Walk walk;
-  walk.start(p.v, start);
-  if (walk.first == worker_first(b, hd)) return;  // no border inside the tile
-  const int w0 = worker_of(walk.first, hd);       // worker of the tile's first part
-  const int parts = worker_of(walk.last - 1, hd) - w0 + 1;
+  if (!joins) return;
   Part x;
   x.r = walk.r;
   x.g = walk.g;
@@ -174,90 +179,80 @@ __global__ void __launch_bounds__(256) join_kernel(const Params p) {
   const int blocks = (parts - 1) * kJoinBlocks;
   int each = 1;
   while (each < 8 && each * blocks < rows) each *= 2;
-  const int warps = 8 / each, sub = warp % warps;  // of a row, and which of them
+  const int warps = 8 / each;                // of a row
+  const int width = kLanes / warps;          // float4 of a warp, wide * mine
+  const int wide = width < 32 ? width : 32, mine = width / wide;
+  const int column = warp % warps * width + lane % wide, group = lane / wide;
   const int slot0 = 2 * w0 + (walk.first == worker_first(w0, hd) ? 0 : 1);
   auto slot = [&](int k) {
     const int at = k == 0 ? slot0 : 2 * (w0 + k);
     return p.l.part + ((int64_t)at * SPLITS + split) * kSlot;
   };
   const int block = (b - 1 - w0) * kJoinBlocks + blockIdx.y;
+#pragma unroll 1
   for (int row0 = block * each; row0 < rows; row0 += blocks * each) {
     const int line = row0 + warp / warps;  // of the tile's rows
     const Row a = row_of<EXP>(p, x, line / kRows, line % kRows);
-    const bool active = line < rows && a.active;
+    if (line >= rows || !a.active) continue;
+    auto state = [&](int k) {
+      return *reinterpret_cast<const float4*>(slot(k) + ROWS * V + 4 * line);
+    };
+    // the largest reference exponent of the parts that see something, and the sums,
+    // lanes side by side
     float m = -INFINITY, l = 0.0f, lr = 0.0f;
-    float4 o[kMine] = {};
-    if (active) {
-      auto state = [&](int k) {
-        return *reinterpret_cast<const float4*>(slot(k) + ROWS * V +
-                                                4 * line);
-      };
-      // the largest reference exponent of the parts that see something, and the sums,
-      // lanes side by side
-      for (int k = lane; k < parts; k += 32) {
-        const float4 s = state(k);
-        if (s.y != 0.0f) m = fmaxf(m, s.x);
-      }
+    for (int k = lane; k < parts; k += 32) {
+      const float4 s = state(k);
+      if (s.y != 0.0f) m = fmaxf(m, s.x);
+    }
 #pragma unroll
-      for (int i = 16; i; i >>= 1) m = fmaxf(m, __shfl_xor_sync(kFull, m, i));
-      for (int k = lane; k < parts; k += 32) {
-        const float4 s = state(k);
-        const float f = s.x == m ? 1.0f : paged::ex2(s.x - m);
-        if (s.y != 0.0f) {
-          l = fmaf(s.y, f, l);
-          lr = fmaf(s.z, f, lr);
-        }
-      }
-#pragma unroll
-      for (int i = 16; i; i >>= 1) {
-        l += __shfl_xor_sync(kFull, l, i);
-        lr += __shfl_xor_sync(kFull, lr, i);
-      }
-#pragma unroll 4
-      for (int k = sub; k < parts; k += warps) {
-        const float4 s = state(k);
-        const float f = s.x == m ? 1.0f : paged::ex2(s.x - m);
-        const float4* from = reinterpret_cast<const float4*>(slot(k) + line * V);
-#pragma unroll
-        for (int i = 0; i < kMine; ++i)
-          if (lane + 32 * i < kLanes && s.y != 0.0f) {
-            const float4 v = from[lane + 32 * i];
-            o[i].x = fmaf(v.x, f, o[i].x);
-            o[i].y = fmaf(v.y, f, o[i].y);
-            o[i].z = fmaf(v.z, f, o[i].z);
-            o[i].w = fmaf(v.w, f, o[i].w);
-          }
+    for (int i = 16; i; i >>= 1) m = fmaxf(m, __shfl_xor_sync(kFull, m, i));
+    for (int k = lane; k < parts; k += 32) {
+      const float4 s = state(k);
+      const float f = s.x == m ? 1.0f : paged::ex2(s.x - m);
+      if (s.y != 0.0f) {
+        l = fmaf(s.y, f, l);
+        lr = fmaf(s.z, f, lr);
       }
     }
-    if (warps > 1) {
+#pragma unroll
+    for (int i = 16; i; i >>= 1) {
+      l += __shfl_xor_sync(kFull, l, i);
+      lr += __shfl_xor_sync(kFull, lr, i);
+    }
+    float4 o[kMine] = {};
+    const int groups = 32 / wide;
+#pragma unroll 4
+    for (int k = group; k < parts; k += groups) {
+      const float4 s = state(k);
+      const float f = s.x == m ? 1.0f : paged::ex2(s.x - m);
+      const float4* from = reinterpret_cast<const float4*>(slot(k) + line * V) + column;
 #pragma unroll
       for (int i = 0; i < kMine; ++i)
-        if (lane + 32 * i < kLanes) sums[warp][lane + 32 * i] = o[i];
-      __syncthreads();
-      if (sub == 0)
-        for (int w = 1; w < warps; ++w)
-#pragma unroll
-          for (int i = 0; i < kMine; ++i)
-            if (lane + 32 * i < kLanes) {
-              const float4 v = sums[warp + w][lane + 32 * i];
-              o[i].x += v.x;
-              o[i].y += v.y;
-              o[i].z += v.z;
-              o[i].w += v.w;
-            }
-      __syncthreads();
+        if (i < mine && s.y != 0.0f) {
+          const float4 v = from[32 * i];
+          o[i].x = fmaf(v.x, f, o[i].x);
+          o[i].y = fmaf(v.y, f, o[i].y);
+          o[i].z = fmaf(v.z, f, o[i].z);
+          o[i].w = fmaf(v.w, f, o[i].w);
+        }
     }
-    if (!active || sub != 0) continue;
+    for (int d = wide; d < 32; d <<= 1) {  // there is one float4 then
+      o[0].x += __shfl_xor_sync(kFull, o[0].x, d);
+      o[0].y += __shfl_xor_sync(kFull, o[0].y, d);
+      o[0].z += __shfl_xor_sync(kFull, o[0].z, d);
+      o[0].w += __shfl_xor_sync(kFull, o[0].w, d);
+    }
+    if (group > 0) continue;
     const int64_t orow = (int64_t)(walk.q.start + a.token) * p.heads + a.head;
     const float inv = 1.0f / lr;
 #pragma unroll
     for (int i = 0; i < kMine; ++i)
-      if (lane + 32 * i < kLanes)
-        reinterpret_cast<uint2*>(p.out + orow * kWide + split * V)[lane + 32 * i] =
+      if (i < mine)
+        reinterpret_cast<uint2*>(p.out + orow * kWide + split * V)[column + 32 * i] =
             lr == 0.0f ? make_uint2(0, 0)
                        : make_uint2(Kind<T>::pack(o[i].x * inv, o[i].y * inv),
                                     Kind<T>::pack(o[i].z * inv, o[i].w * inv));
-    if (lane == 0 && p.lse && split == 0)
+    if (lane == 0 && warp % warps == 0 && p.lse && split == 0)
       p.lse[orow] =
           l == 0.0f ? -INFINITY : (m - Kind<T>::kLift + log2f(l)) * 0.693147180559945309f;
   }

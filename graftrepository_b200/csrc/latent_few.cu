@@ -269,9 +269,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
     bool ok = true;  // the same in the eight warps, which meet at barriers
     int it = 0, seg = 0;
+    Part next;
+    bool more = parts.next(p, &next);
 #pragma unroll 1
-    while (ok && parts.next(p, &x)) {
-      if (x.steps == 0) continue;
+    while (ok && more) {
+      x = next;
+      if (x.steps == 0) {
+        more = parts.next(p, &next);
+        continue;
+      }
       const int ob = seg & 1;
       if (seg >= 2) ok = wait(&fin_empty[ob], ((seg >> 1) - 1) & 1);
       if (soft_any(!ok)) { ok = false; break; }
@@ -404,6 +410,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[buf]);
+        // a chain of loads that lies under the wait for the next scores
+        if (i == 0) more = parts.next(p, &next);
       }
       if (!ok) break;
       // sums over the tokens, for the warps that bring the results out
@@ -591,10 +599,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         ++part;
       }
     };
+    Part next;
+    bool more = parts.next(p, &next);
 #pragma unroll 1
-    while (ok && parts.next(p, &x)) {
+    while (ok && more) {
+      x = next;
       const int steps = __shfl_sync(kFull, x.steps, 0);
-      if (steps == 0) continue;
+      if (steps == 0) {
+        more = parts.next(p, &next);
+        continue;
+      }
       const int ob = seg & 1;
       ok = wait(&q_full, seg & 1) && (seg < 2 || wait(&fin_empty[ob], ((seg >> 1) - 1) & 1));
       if (!ok) break;
@@ -603,6 +617,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       scores(it, kPairs + 1, nullptr, 0);
       if (ok && steps == 1 && elect_one()) umma_commit(&q_empty);
       __syncwarp();
+      more = parts.next(p, &next);  // under the first softmax
 #pragma unroll 1
       for (int i = 0; i < steps && ok; ++i) {
         const int s = it + i;
