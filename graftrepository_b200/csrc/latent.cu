@@ -114,6 +114,20 @@ __global__ void __launch_bounds__(kScheduleThreads) schedule_kernel(const Schedu
     Walk walk;
     walk.seek(v, u, lo);
     l.start[w] = Start{walk.r, walk.g, walk.j, walk.q.start, walk.q.n, walk.q.len, walk.first};
+    Join j{0, 0, 0, 0, 0, 0};
+    if (walk.first != u) {
+      const int w0 = worker_of(walk.first, sh);
+      const int tok0 = walk.j * v.tiling.per, toks = imin(v.tiling.per, walk.q.n - tok0);
+      const bool expanded = form == 1, wide = !expanded && v.tiling.groups > 1;
+      j.row = (int64_t)(walk.q.start + tok0) * v.heads +
+              (expanded ? walk.g : wide ? walk.g * kRows : 0);
+      j.rows = expanded ? toks : wide ? imin(kRows, v.heads - walk.g * kRows) : toks * v.heads;
+      j.parts = worker_of(walk.last - 1, sh) - w0 + 1;
+      j.slot = 2 * w0 + (walk.first == worker_first(w0, sh) ? 0 : 1);
+      j.worker = w0;
+      j.border = w - 1 - w0;
+    }
+    l.join[w] = j;
   }
 }
 
@@ -287,7 +301,7 @@ int check_attend(const grm_b200_latent_plan* plan, const grm_b200_latent_arena* 
 
 View view_of(const grm_b200_latent_plan& plan, const Shape& s, int form) {
   return {lists_of(s, form, plan.work).base, plan.step.starts, plan.step.lens, plan.step.requests,
-          s.tiling[form], plan.step.grow ? 1 : 0};
+          s.tiling[form], plan.step.grow ? 1 : 0, plan.heads};
 }
 
 int fill(const grm_b200_latent_plan* plan, const grm_b200_latent_arena* arena, int form,
@@ -340,6 +354,7 @@ int make_shape(const grm_b200_latent_plan& p, int sms, Shape* s) {
     s->off_header[f] = take(sizeof(Header));
     s->off_base[f] = take((p.step.requests + 1) * 8);
     s->off_start[f] = take((int64_t)s->tiling[f].workers * (int64_t)sizeof(Start));
+    s->off_join[f] = take((int64_t)s->tiling[f].workers * (int64_t)sizeof(Join));
   }
   const Tiling& t = s->tiling[0];
   const int64_t absorbed = (int64_t)t.workers * t.splits *

@@ -39,10 +39,22 @@ struct alignas(32) Start {
   int64_t first;
 };
 
+// A tile that lies in the shares of several workers, as join_kernel goes by: one for
+// each border between two shares that is inside a tile.
+struct alignas(32) Join {
+  int64_t row;     // of the results, [tokens * heads], of the tile's first row
+  int32_t rows;    // 0: the border is not inside a tile
+  int32_t parts;
+  int32_t slot;    // of the first part; the others' are 2 (worker + k)
+  int32_t worker;  // of the first part
+  int32_t border;  // of the tile's borders, from 0 on
+};
+
 struct Lists {
   Header* header;
   int64_t* base;  // [requests + 1] first unit of each request
   Start* start;   // [workers]
+  Join* join;     // [workers], of the border where each begins
   float* part;    // [workers * splits * 2] partial results, see slot_floats
 };
 
@@ -76,7 +88,7 @@ __host__ __device__ constexpr int slot_floats(int rows, int values) { return row
 // Byte offsets in the work area, which follow from the plan's sizes alone.
 struct Shape {
   Tiling tiling[2];  // absorbed, expanded
-  int64_t off_header[2], off_base[2], off_start[2];
+  int64_t off_header[2], off_base[2], off_start[2], off_join[2];
   int64_t off_part, off_room, off_keys, off_values, bytes;
 };
 
@@ -87,6 +99,7 @@ inline Lists lists_of(const Shape& s, int form, void* work) {
   return {reinterpret_cast<Header*>(b + s.off_header[form]),
           reinterpret_cast<int64_t*>(b + s.off_base[form]),
           reinterpret_cast<Start*>(b + s.off_start[form]),
+          reinterpret_cast<Join*>(b + s.off_join[form]),
           reinterpret_cast<float*>(b + s.off_part)};
 }
 
@@ -97,7 +110,7 @@ struct View {
   const int32_t* lens;
   int64_t requests;
   Tiling tiling;
-  int grow;
+  int grow, heads;
 };
 
 struct Params {

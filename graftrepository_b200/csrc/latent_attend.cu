@@ -286,31 +286,85 @@ __global__ void __launch_bounds__(Layout<MAIN, ROPE, EXP>::kThreads, 1)
       if (lane == 0) mbar_arrive(&q_full[t]);
     };
     Part next;
-    bool more = parts.next(p, &next);
-    if (more && next.steps > 0 && next.toks[t] > 0) queries(next);
+    bool more = parts.next(p, &next), held = false;  // held: a tile whose result is to go out
+    Row a{0, 0, false};
+    bool idle = false;
+    int steps = 0;
+    float m = 0.0f, l = 0.0f, lr = 0.0f;
 #pragma unroll 1
-    while (ok && more) {
-      x = next;
-      const int steps = x.steps, stage_base = stage0;
-      stage0 += steps;
-      bool queue = false;
-      // the next part, a chain of loads that lies under the wait for the second scores
-      auto look = [&] {
-        more = parts.next(p, &next);
-        queue = more && next.steps > 0 && next.toks[t] > 0;
-      };
-      if (x.toks[t] == 0) {
-        look();
-        if (queue) queries(next);
-        continue;
+    while (true) {
+      // The scores of the tile before are there, so its queries' place is free: the next
+      // tile's first scores are worked out while this one's result goes out.
+      if (more && next.steps > 0 && next.toks[t] > 0) queries(next);
+      if (held) {
+        if (steps > 0) {
+          if (!(ok = wait(&o_done[t], tile & 1))) break;
+          tc_fence_after();
+          ++tile;
+        }
+        const int64_t orow = (int64_t)(x.start + a.token) * p.heads + a.head;
+        if (x.slot >= 0) {  // a part's result, for join_kernel
+          float* slot = p.l.part + ((int64_t)x.slot * LY::kSplits + split) * LY::kSlot;
+          float4* to = reinterpret_cast<float4*>(slot + (t * kRows + row) * LY::kV);
+          if (steps > 0 && !idle)
+#pragma unroll 1
+            for (int c = 0; c < LY::kV / 32; ++c) {
+              uint32_t o[32];
+              tmem_ld32_nowait(o_col + 32 * c, o);
+              tmem_wait_ld32(o);
+              if (a.active)
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                  to[8 * c + k] =
+                      make_float4(__uint_as_float(o[4 * k]), __uint_as_float(o[4 * k + 1]),
+                                  __uint_as_float(o[4 * k + 2]), __uint_as_float(o[4 * k + 3]));
+            }
+          if (a.active)
+            *reinterpret_cast<float4*>(slot + kRows * kQ * LY::kV + 4 * (t * kRows + row)) =
+                make_float4(m, l, lr, 0.0f);
+        } else if (!idle) {
+          const float inv = lr == 0.0f ? 0.0f : 1.0f / lr;
+          uint16_t* out = p.out + orow * MAIN + split * LY::kV;
+#pragma unroll 1
+          for (int c = 0; c < LY::kV / 32; ++c) {
+            uint32_t o[32];
+            if (steps > 0) {
+              tmem_ld32_nowait(o_col + 32 * c, o);
+              tmem_wait_ld32(o);
+            }
+            if (a.active)
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                uint32_t w[4];
+#pragma unroll
+                for (int y = 0; y < 4; ++y)
+                  w[y] = lr == 0.0f ? 0u
+                                    : Kind<T>::pack(__uint_as_float(o[8 * k + 2 * y]) * inv,
+                                                    __uint_as_float(o[8 * k + 2 * y + 1]) * inv);
+                reinterpret_cast<uint4*>(out)[4 * c + k] = make_uint4(w[0], w[1], w[2], w[3]);
+              }
+          }
+          if (a.active && p.lse && split == 0)
+            p.lse[orow] = l == 0.0f ? -INFINITY
+                                    : (m - Kind<T>::kLift + log2f(l)) * 0.693147180559945309f;
+        }
+        // what the next tile's products overwrite has been read
+        tc_fence_before();
       }
-      if (steps == 0) look();
-      const Row a = row_of<EXP>(p, x, t, row);
-      float m = -INFINITY, l = 0.0f, lr = 0.0f;
-
+      if (!more) break;
+      x = next;
+      steps = x.steps;
+      const int stage_base = stage0;
+      stage0 += steps;
+      held = x.toks[t] > 0;
+      if (!held || steps == 0) more = parts.next(p, &next);
+      if (!held) continue;
+      a = row_of<EXP>(p, x, t, row);
+      m = -INFINITY;
+      l = lr = 0.0f;
       // tokens that the row sees, from the part's first on
       const int lim = (p.causal ? min(x.len, x.cached + a.token + 1) : x.len) - x.step0 * kStep;
-      const bool idle = !__any_sync(kFull, a.active);
+      idle = !__any_sync(kFull, a.active);
 #pragma unroll 1
       for (int i = 0; i < steps; ++i, ++it) {
         const int buf = it & 1;
@@ -318,7 +372,7 @@ __global__ void __launch_bounds__(Layout<MAIN, ROPE, EXP>::kThreads, 1)
         tc_fence_after();
         if (idle) {
           if (lane == 0) mbar_arrive(&p_full[t][buf]);
-          if (i == 0) look();
+          if (i == 0) more = parts.next(p, &next);
           continue;
         }
         if (__any_sync(kFull, (i + 1) * kStep > lim)) {
@@ -384,65 +438,10 @@ __global__ void __launch_bounds__(Layout<MAIN, ROPE, EXP>::kThreads, 1)
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[t][buf]);
-        if (i == 0) look();
+        // a chain of loads that lies under the wait for the second scores
+        if (i == 0) more = parts.next(p, &next);
       }
       if (!ok) break;
-      // The scores of this tile are there, so its queries' place is free: the next
-      // tile's first scores are worked out while this one's result goes out.
-      if (queue) queries(next);
-      if (steps > 0) {
-        if (!(ok = wait(&o_done[t], tile & 1))) break;
-        tc_fence_after();
-        ++tile;
-      }
-      const int64_t orow = (int64_t)(x.start + a.token) * p.heads + a.head;
-      if (x.slot >= 0) {  // a part's result, for join_kernel
-        float* slot = p.l.part + ((int64_t)x.slot * LY::kSplits + split) * LY::kSlot;
-        float4* to = reinterpret_cast<float4*>(slot + (t * kRows + row) * LY::kV);
-        if (steps > 0 && !idle)
-#pragma unroll 1
-          for (int c = 0; c < LY::kV / 32; ++c) {
-            uint32_t o[32];
-            tmem_ld32_nowait(o_col + 32 * c, o);
-            tmem_wait_ld32(o);
-            if (a.active)
-#pragma unroll
-              for (int k = 0; k < 8; ++k)
-                to[8 * c + k] =
-                    make_float4(__uint_as_float(o[4 * k]), __uint_as_float(o[4 * k + 1]),
-                                __uint_as_float(o[4 * k + 2]), __uint_as_float(o[4 * k + 3]));
-          }
-        if (a.active)
-          *reinterpret_cast<float4*>(slot + kRows * kQ * LY::kV + 4 * (t * kRows + row)) =
-              make_float4(m, l, lr, 0.0f);
-      } else if (!idle) {
-        const float inv = lr == 0.0f ? 0.0f : 1.0f / lr;
-        uint16_t* out = p.out + orow * MAIN + split * LY::kV;
-#pragma unroll 1
-        for (int c = 0; c < LY::kV / 32; ++c) {
-          uint32_t o[32];
-          if (steps > 0) {
-            tmem_ld32_nowait(o_col + 32 * c, o);
-            tmem_wait_ld32(o);
-          }
-          if (a.active)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              uint32_t w[4];
-#pragma unroll
-              for (int y = 0; y < 4; ++y)
-                w[y] = lr == 0.0f ? 0u
-                                  : Kind<T>::pack(__uint_as_float(o[8 * k + 2 * y]) * inv,
-                                                  __uint_as_float(o[8 * k + 2 * y + 1]) * inv);
-              reinterpret_cast<uint4*>(out)[4 * c + k] = make_uint4(w[0], w[1], w[2], w[3]);
-            }
-        }
-        if (a.active && p.lse && split == 0)
-          p.lse[orow] = l == 0.0f ? -INFINITY
-                                  : (m - Kind<T>::kLift + log2f(l)) * 0.693147180559945309f;
-      }
-      // what the next tile's products overwrite has been read
-      tc_fence_before();
     }
   } else if (warp < LY::kLoadWarp) {
     // ---------------------------------------------------------- products
@@ -518,24 +517,26 @@ __global__ void __launch_bounds__(Layout<MAIN, ROPE, EXP>::kThreads, 1)
       ok = wait(&q_full[t], tile & 1);
       if (!ok) break;
       tc_fence_after();
-      ok = next_scores(0) && (steps < 2 || next_scores(1));
-      more = parts.next(p, &next);  // under the first softmax
+      // scores two steps ahead of results, each of them in one place of the code
 #pragma unroll 1
-      for (int i = 0; i < steps && ok; ++i) {
-        const int s = (stage0 + i) % kStages, buf = (it + i) & 1;
-        if (!(ok = wait(&p_full[t][buf], ((it + i) >> 1) & 1))) break;
-        tc_fence_after();
-        const uint32_t vd = v_lo + (uint32_t)s * (LY::kStage / 16);
-        if (elect_one()) {
+      for (int i = -2; i < steps && ok; ++i) {
+        if (i == 0) more = parts.next(p, &next);  // under the first softmax
+        if (i >= 0) {
+          const int s = (stage0 + i) % kStages, buf = (it + i) & 1;
+          if (!(ok = wait(&p_full[t][buf], ((it + i) >> 1) & 1))) break;
+          tc_fence_after();
+          const uint32_t vd = v_lo + (uint32_t)s * (LY::kStage / 16);
+          if (elect_one()) {
 #pragma unroll
-          for (int k = 0; k < kStep / 16; ++k)
-            umma_f16_ts(o_at, s_at + buf * kStep + 8 * k, desc(kHi128, vd + k * (16 * 128 / 16)),
-                        idesc<T>(LY::kV, true), i != 0 || k != 0);
-          umma_commit(&o_full[t]);
-          umma_commit(&empty[s]);
-          if (i + 1 == steps) umma_commit(&o_done[t]);
+            for (int k = 0; k < kStep / 16; ++k)
+              umma_f16_ts(o_at, s_at + buf * kStep + 8 * k, desc(kHi128, vd + k * (16 * 128 / 16)),
+                          idesc<T>(LY::kV, true), i != 0 || k != 0);
+            umma_commit(&o_full[t]);
+            umma_commit(&empty[s]);
+            if (i + 1 == steps) umma_commit(&o_done[t]);
+          }
+          __syncwarp();
         }
-        __syncwarp();
         if (i + 2 < steps) ok = next_scores(i + 2);  // in this step's place
       }
       stage0 += steps;

@@ -130,13 +130,13 @@ __device__ __forceinline__ Row row_of(const Params& p, const Part& x, int t, int
 
 // ---- joining the parts of tiles
 
-constexpr int kJoinBlocks = 8;  // for every border between two shares
-
 // Parts of tiles that lie in the shares of several workers, and the rows past the
-// step's last one.  A tile in n parts has n - 1 borders inside, whose blocks share its
-// rows: 1 to 8 warps a row, each for some of its values; lanes beyond those take every
-// so many of the parts.  Takes no shared memory, so that blocks get their place, and
-// find theirs in the lists, while attention still runs.
+// step's last one.  A tile in n parts has n - 1 borders inside, whose blocks (one for
+// every eight of its rows) share the rows: 1 to 8 warps a row, each for some of its
+// values; lanes beyond those take every so many of the parts.  What is here runs once
+// in a launch, on instructions that are in no cache, so there are few of them: with
+// the tiles looked up here rather than in the plan, and a batch of parts unrolled, it
+// took 22 us where this takes 5 (64 conversations).
 // ROWS of a tile, V values of a block's results, SPLITS blocks that share a tile's.
 template <typename T, int V, int SPLITS, int ROWS, bool EXP>
 __global__ void __launch_bounds__(256) join_kernel(const Params p) {
@@ -145,124 +145,92 @@ __global__ void __launch_bounds__(256) join_kernel(const Params p) {
   constexpr int kMine = (kLanes + 31) / 32;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int b = blockIdx.x / SPLITS + 1, split = blockIdx.x % SPLITS;
-  // the lists are the plan's, which was there before attention began
-  const Start start = p.l.start[min(b, p.v.tiling.workers - 1)];
-  const Header hd = *p.l.header;
-  const int64_t used = p.v.starts[p.v.requests];
-  bool joins = b < hd.workers;
-  Walk walk;
-  int w0 = 0, parts = 0;
-  if (joins) {
-    walk.start(p.v, start);
-    joins = walk.first != worker_first(b, hd);  // a border inside the tile
-    w0 = worker_of(walk.first, hd);             // worker of the tile's first part
-    parts = worker_of(walk.last - 1, hd) - w0 + 1;
-  }
+  // the lists are the plan's, which were there before attention began
+  Join j = p.l.join[b < p.v.tiling.workers ? b : 0];
+  const int workers = p.l.header->workers, used = p.v.starts[p.v.requests];
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int64_t id = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 256 + threadIdx.x;
-  for (int64_t i = used * p.heads * (kWide / 8) + id; i < p.tokens * p.heads * (kWide / 8);
-       i += (int64_t)gridDim.x * gridDim.y * 256) {
-    reinterpret_cast<uint4*>(p.out)[i] = make_uint4(0, 0, 0, 0);
-    if (p.lse && i % (kWide / 8) == 0) p.lse[i / (kWide / 8)] = -INFINITY;
+  if (used < p.tokens) {
+    const int64_t id = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 256 + threadIdx.x;
+    for (int64_t i = (int64_t)used * p.heads * (kWide / 8) + id;
+         i < p.tokens * p.heads * (kWide / 8); i += (int64_t)gridDim.x * gridDim.y * 256) {
+      reinterpret_cast<uint4*>(p.out)[i] = make_uint4(0, 0, 0, 0);
+      if (p.lse && i % (kWide / 8) == 0) p.lse[i / (kWide / 8)] = -INFINITY;
+    }
   }
-  if (!joins) return;
-  Part x;
-  x.r = walk.r;
-  x.g = walk.g;
-  x.tok0 = walk.j * p.v.tiling.per;
-  const int toks = min(p.v.tiling.per, walk.q.n - x.tok0);
-  x.toks[0] = EXP ? min(toks, kRows) : toks;
-  x.toks[1] = EXP ? toks - x.toks[0] : 0;
-  const int rows = EXP ? toks
-                       : min(kRows, toks * (p.v.tiling.groups > 1 ? kRows : p.heads));
-  // rows of a block: 8, 4, 2 or 1, whichever is enough, and more where 8 are not
-  const int blocks = (parts - 1) * kJoinBlocks;
-  int each = 1;
-  while (each < 8 && each * blocks < rows) each *= 2;
-  const int warps = 8 / each;                // of a row
-  const int width = kLanes / warps;          // float4 of a warp, wide * mine
-  const int wide = width < 32 ? width : 32, mine = width / wide;
-  const int column = warp % warps * width + lane % wide, group = lane / wide;
-  const int slot0 = 2 * w0 + (walk.first == worker_first(w0, hd) ? 0 : 1);
-  auto slot = [&](int k) {
-    const int at = k == 0 ? slot0 : 2 * (w0 + k);
-    return p.l.part + ((int64_t)at * SPLITS + split) * kSlot;
-  };
-  const int block = (b - 1 - w0) * kJoinBlocks + blockIdx.y;
-#pragma unroll 1
-  for (int row0 = block * each; row0 < rows; row0 += blocks * each) {
-    const int line = row0 + warp / warps;  // of the tile's rows
-    const Row a = row_of<EXP>(p, x, line / kRows, line % kRows);
-    if (line >= rows || !a.active) continue;
-    auto state = [&](int k) {
-      return *reinterpret_cast<const float4*>(slot(k) + ROWS * V + 4 * line);
-    };
-    // the largest reference exponent of the parts that see something, and the sums,
-    // lanes side by side
-    float m = -INFINITY, l = 0.0f, lr = 0.0f;
-    for (int k = lane; k < parts; k += 32) {
-      const float4 s = state(k);
-      if (s.y != 0.0f) m = fmaxf(m, s.x);
-    }
-#pragma unroll
-    for (int i = 16; i; i >>= 1) m = fmaxf(m, __shfl_xor_sync(kFull, m, i));
-    for (int k = lane; k < parts; k += 32) {
-      const float4 s = state(k);
-      const float f = s.x == m ? 1.0f : paged::ex2(s.x - m);
-      if (s.y != 0.0f) {
-        l = fmaf(s.y, f, l);
-        lr = fmaf(s.z, f, lr);
-      }
-    }
-#pragma unroll
-    for (int i = 16; i; i >>= 1) {
-      l += __shfl_xor_sync(kFull, l, i);
-      lr += __shfl_xor_sync(kFull, lr, i);
-    }
-    float4 o[kMine] = {};
-    const int groups = 32 / wide;
-#pragma unroll 4
-    for (int k = group; k < parts; k += groups) {
-      const float4 s = state(k);
-      const float f = s.x == m ? 1.0f : paged::ex2(s.x - m);
-      const float4* from = reinterpret_cast<const float4*>(slot(k) + line * V) + column;
-#pragma unroll
-      for (int i = 0; i < kMine; ++i)
-        if (i < mine && s.y != 0.0f) {
-          const float4 v = from[32 * i];
-          o[i].x = fmaf(v.x, f, o[i].x);
-          o[i].y = fmaf(v.y, f, o[i].y);
-          o[i].z = fmaf(v.z, f, o[i].z);
-          o[i].w = fmaf(v.w, f, o[i].w);
-        }
-    }
-    for (int d = wide; d < 32; d <<= 1) {  // there is one float4 then
-      o[0].x += __shfl_xor_sync(kFull, o[0].x, d);
-      o[0].y += __shfl_xor_sync(kFull, o[0].y, d);
-      o[0].z += __shfl_xor_sync(kFull, o[0].z, d);
-      o[0].w += __shfl_xor_sync(kFull, o[0].w, d);
-    }
-    if (group > 0) continue;
-    const int64_t orow = (int64_t)(walk.q.start + a.token) * p.heads + a.head;
-    const float inv = 1.0f / lr;
+  if (b >= workers || j.rows == 0) return;
+  // rows of a block: 1, 2, 4 or 8, as many as it takes
+  const int blocks = (j.parts - 1) * gridDim.y;
+  int shift = 0;
+  while ((blocks << shift) < j.rows) ++shift;  // at most 3
+  const int width = kLanes >> (3 - shift);     // float4 of a warp's
+  const int wide = width < 32 ? width : 32;
+  const int of_row = warp & ((8 >> shift) - 1);
+  const int column = of_row * width + (lane & (wide - 1));
+  const int line = ((j.border * gridDim.y + blockIdx.y) << shift) + (warp >> (3 - shift));
+  if (line >= j.rows) return;
+  const float* const part = p.l.part + split * kSlot;
+  float m = -INFINITY, l = 0.0f, lr = 0.0f;
+  float4 o[kMine] = {};
+#pragma unroll 2
+  for (int k = lane / wide; k < j.parts; k += 32 / wide) {
+    const float* slot =
+        part + (int64_t)(k == 0 ? j.slot : 2 * (j.worker + k)) * (SPLITS * kSlot);
+    const float4 s = *reinterpret_cast<const float4*>(slot + ROWS * V + 4 * line);
+    float4 v[kMine];
 #pragma unroll
     for (int i = 0; i < kMine; ++i)
-      if (i < mine)
-        reinterpret_cast<uint2*>(p.out + orow * kWide + split * V)[column + 32 * i] =
-            lr == 0.0f ? make_uint2(0, 0)
-                       : make_uint2(Kind<T>::pack(o[i].x * inv, o[i].y * inv),
-                                    Kind<T>::pack(o[i].z * inv, o[i].w * inv));
-    if (lane == 0 && warp % warps == 0 && p.lse && split == 0)
-      p.lse[orow] =
-          l == 0.0f ? -INFINITY : (m - Kind<T>::kLift + log2f(l)) * 0.693147180559945309f;
+      if (32 * i < width) v[i] = (reinterpret_cast<const float4*>(slot + line * V) + column)[32 * i];
+    if (s.y == 0.0f) continue;  // a part that sees nothing
+    const float next = fmaxf(m, s.x);
+    const float a = m == next ? 1.0f : paged::ex2(m - next);
+    const float f = s.x == next ? 1.0f : paged::ex2(s.x - next);
+    m = next;
+    l = fmaf(l, a, s.y * f);
+    lr = fmaf(lr, a, s.z * f);
+#pragma unroll
+    for (int i = 0; i < kMine; ++i)
+      if (32 * i < width) {
+        o[i].x = fmaf(o[i].x, a, v[i].x * f);
+        o[i].y = fmaf(o[i].y, a, v[i].y * f);
+        o[i].z = fmaf(o[i].z, a, v[i].z * f);
+        o[i].w = fmaf(o[i].w, a, v[i].w * f);
+      }
   }
+#pragma unroll 1
+  for (int d = wide; d < 32; d <<= 1) {  // lanes with other parts; there is one float4 then
+    const float other = __shfl_xor_sync(kFull, m, d), next = fmaxf(m, other);
+    const float f = m == next ? 1.0f : paged::ex2(m - next);
+    m = next;
+    l *= f;
+    lr *= f;
+    l += __shfl_xor_sync(kFull, l, d);
+    lr += __shfl_xor_sync(kFull, lr, d);
+    o[0] = make_float4(o[0].x * f, o[0].y * f, o[0].z * f, o[0].w * f);
+    o[0].x += __shfl_xor_sync(kFull, o[0].x, d);
+    o[0].y += __shfl_xor_sync(kFull, o[0].y, d);
+    o[0].z += __shfl_xor_sync(kFull, o[0].z, d);
+    o[0].w += __shfl_xor_sync(kFull, o[0].w, d);
+  }
+  if (lane >= wide) return;
+  const int64_t row = j.row + (int64_t)line * (EXP ? p.heads : 1);
+  const float inv = 1.0f / lr;
+#pragma unroll
+  for (int i = 0; i < kMine; ++i)
+    if (32 * i < width)
+      reinterpret_cast<uint2*>(p.out + row * kWide + split * V)[column + 32 * i] =
+          lr == 0.0f ? make_uint2(0, 0)
+                     : make_uint2(Kind<T>::pack(o[i].x * inv, o[i].y * inv),
+                                  Kind<T>::pack(o[i].z * inv, o[i].w * inv));
+  if (lane == 0 && of_row == 0 && split == 0 && p.lse)
+    p.lse[row] = l == 0.0f ? -INFINITY : (m - Kind<T>::kLift + log2f(l)) * 0.693147180559945309f;
 }
 
 template <typename T, int V, int SPLITS, int ROWS, bool EXP>
 int launch_join(const Params& p, cudaStream_t st) {
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(std::max(p.v.tiling.workers - 1, 1) * SPLITS),
-                     kJoinBlocks);
+  const Tiling& t = p.v.tiling;
+  const int rows = EXP ? t.per : (int)std::min((int64_t)kRows, (int64_t)t.per * p.heads);
+  cfg.gridDim = dim3((unsigned)(std::max(t.workers - 1, 1) * SPLITS), (unsigned)(rows + 7) / 8);
   cfg.blockDim = dim3(256);
   cfg.stream = st;
   cudaLaunchAttribute attr;
