@@ -181,7 +181,7 @@ __global__ void __launch_bounds__(Layout<MAIN, ROPE, EXP>::kThreads, 1)
   unsigned char* const sm_q = sm;                         // [kQ]
   unsigned char* const sm_stage = sm + kQ * LY::kQuery;   // [kStages]
   __shared__ __align__(8) uint64_t full[kStages], empty[kStages], q_full[kQ], drained[kQ],
-      s_full[kQ][2], p_full[kQ][2], o_full[kQ], o_done[kQ];
+      s_full[kQ][2], p_full[kQ][2], o_full[kQ], o_done[kQ], turn[kQ][4];
   __shared__ uint32_t sh_tmem;
   __shared__ int sh_fail;
 
@@ -210,6 +210,7 @@ __global__ void __launch_bounds__(Layout<MAIN, ROPE, EXP>::kThreads, 1)
         mbar_init(&s_full[t][x], 1);
         mbar_init(&p_full[t][x], 4);
       }
+      for (int x = 0; x < 4; ++x) mbar_init(&turn[t][x], 1);
     }
     mbar_fence_init();
     sh_fail = 0;
@@ -238,6 +239,7 @@ __global__ void __launch_bounds__(Layout<MAIN, ROPE, EXP>::kThreads, 1)
     unsigned char* const my_q = sm_q + t * LY::kQuery;
     bool ok = true;
     int it = 0, tile = 0, stage0 = 0;  // steps and tiles of this query tile; stages so far
+    int turns = 0;  // steps of both query tiles so far
     // the row's query of a part, to tensor memory and shared memory
     auto queries = [&](const Part& y) {
       const Row b = row_of<EXP>(p, y, t, row);
@@ -370,9 +372,24 @@ __global__ void __launch_bounds__(Layout<MAIN, ROPE, EXP>::kThreads, 1)
         const int buf = it & 1;
         if (!(ok = wait(&s_full[t][buf], (it >> 1) & 1))) break;
         tc_fence_after();
+        // The two softmax warps of a scheduler take turns at the exponentials, so that one's
+        // other work lies under them (left to themselves they do both in step).
+        const bool two = kQ == 2 && x.toks[kQ - 1] > 0;
+        auto my_turn = [&] {
+          const bool go = t == 1 || turns > 0 ? wait(&turn[t][warp & 3], (turns - 1 + t) & 1) : true;
+          ++turns;
+          return go;
+        };
+        auto your_turn = [&] {
+          if (lane == 0) mbar_arrive(&turn[kQ - 1 - t][warp & 3]);
+        };
         if (idle) {
           if (lane == 0) mbar_arrive(&p_full[t][buf]);
           if (i == 0) more = parts.next(p, &next);
+          if (two) {
+            if (!(ok = my_turn())) break;
+            your_turn();
+          }
           continue;
         }
         if (__any_sync(kFull, (i + 1) * kStep > lim)) {
@@ -391,12 +408,12 @@ __global__ void __launch_bounds__(Layout<MAIN, ROPE, EXP>::kThreads, 1)
         tmem_ld32_nowait(s_col + buf * kStep + 32, v[1]);
         tmem_wait_ld32(v[0]);
         tmem_wait_ld32(v[1]);
-        float top = -INFINITY;
+        float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // chains side by side
 #pragma unroll
         for (int k = 0; k < kStep; k += 2)
-          top = max3(top, __uint_as_float(v[k / 32][k % 32]),
-                     __uint_as_float(v[k / 32][k % 32 + 1]));
-        top *= p.scale_log2;
+          tops[k / 2 % 4] = max3(tops[k / 2 % 4], __uint_as_float(v[k / 32][k % 32]),
+                                 __uint_as_float(v[k / 32][k % 32 + 1]));
+        const float top = fmaxf(max3(tops[0], tops[1], tops[2]), tops[3]) * p.scale_log2;
         if (__any_sync(kFull, top > m + kLazy)) {
           const float next = top > m + kLazy ? reference_of(top) : m;
           const float f = next == m ? 1.0f : ex2(m - next);
@@ -417,6 +434,7 @@ __global__ void __launch_bounds__(Layout<MAIN, ROPE, EXP>::kThreads, 1)
           }
         }
         const float off = m == -INFINITY ? 0.0f : Kind<T>::kLift - m;
+        if (two && !(ok = my_turn())) break;
         float2 sum = make_float2(0.0f, 0.0f), rounded = make_float2(0.0f, 0.0f);
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
@@ -429,6 +447,8 @@ __global__ void __launch_bounds__(Layout<MAIN, ROPE, EXP>::kThreads, 1)
             sum = add2(sum, e);
             w[k / 2] = Kind<T>::pack(e.x, e.y);
             rounded = add2(rounded, Kind<T>::widen(w[k / 2]));
+            // three quarters done: the other's first ones fill the gaps of the last
+            if (c == 1 && k == 14 && two) your_turn();
           }
           tmem_st16(s_col + buf * kStep + 16 * c, w);
         }
