@@ -15,8 +15,7 @@
 // 31,000 tokens of 40 heads of 64 + 64) against 0.8 GFLOP a MB.
 #include <algorithm>
 
-#include "latent.cuh"
-#include "umma.cuh"
+#include "latent_device.cuh"
 
 namespace grm_b200 {
 namespace latent {
@@ -47,47 +46,6 @@ struct Maps {
   CUtensorMap rows, weights, keys, values;
 };
 
-template <typename T>
-struct Kind;
-template <>
-struct Kind<__half> {
-  static constexpr uint32_t kFormat = 0;
-  static constexpr uint32_t kNoNumber = 0x7C00u, kNan = 0x7FFFu;
-  static __device__ __forceinline__ uint32_t pack(float a, float b) {
-    return paged::pack_half2(a, b);
-  }
-  static __device__ __forceinline__ float2 widen(uint32_t v) {
-    return __half22float2(*reinterpret_cast<const __half2*>(&v));
-  }
-};
-template <>
-struct Kind<__nv_bfloat16> {
-  static constexpr uint32_t kFormat = (1u << 7) | (1u << 10);
-  static constexpr uint32_t kNoNumber = 0x7F80u, kNan = 0x7FFFu;
-  static __device__ __forceinline__ uint32_t pack(float a, float b) {
-    return paged::pack_out<__nv_bfloat16>(a, b);
-  }
-  static __device__ __forceinline__ float2 widen(uint32_t v) {
-    return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xFFFF0000u));
-  }
-};
-
-__device__ __forceinline__ void tma_load(void* dst, const CUtensorMap* map, int x, int y,
-                                         uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%2, %3}], [%4];" ::"r"(smem_u32(dst)),
-      "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar))
-      : "memory");
-}
-__device__ __forceinline__ void tma_load(void* dst, const CUtensorMap* map, int x, int y, int z,
-                                         uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_u32(dst)),
-      "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
-      : "memory");
-}
 __device__ __forceinline__ void tma_store(const CUtensorMap* map, int x, int y, int z,
                                           const void* src) {
   asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];"
@@ -204,7 +162,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             // Keys of a token whose values are none in this type make its score none,
             // so that attention knows.
-            if (bad && c == 0 && col == 0) lo[0] = Kind<T>::kNan | (lo[0] & 0xFFFF0000u);
+            if (bad && c == 0 && col == 0) lo[0] = 0x7FFFu | (lo[0] & 0xFFFF0000u);
             const uint32_t at = row * 64 + ((c ^ ((row >> 1) & 3)) << 4);
             *reinterpret_cast<uint4*>(to + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
             if (!value)
