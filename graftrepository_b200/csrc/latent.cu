@@ -62,14 +62,15 @@ __global__ void __launch_bounds__(kScheduleThreads) schedule_kernel(const Schedu
   const Lists l = p.l[sizes ? form : 0];
   const View v = p.v[sizes ? form : 0];
   const int64_t requests = v.requests;
-  int64_t before = 0, room = 0;
+  int64_t before = 0, room = 0, tiles = 0;
   for (int64_t r0 = 0; r0 < requests; r0 += kScheduleThreads) {
     const int64_t r = r0 + tid;
-    int64_t n = 0, tokens = 0;
+    int64_t n = 0, tokens = 0, own_tiles = 0;
     if (r < requests) {
       const Request q = request_of(v.starts[r], v.starts[r + 1], v.lens[r], v.tiling.per, v.grow);
       if (q.n > 0) {
         n = q.total * v.tiling.groups;
+        own_tiles = (int64_t)q.tiles * v.tiling.groups;
         tokens = ((int64_t)q.len + kExpandAlign - 1) / kExpandAlign * kExpandAlign;
       }
     }
@@ -78,6 +79,11 @@ __global__ void __launch_bounds__(kScheduleThreads) schedule_kernel(const Schedu
       const int64_t incl = block_scan(n, part, &all);
       if (r < requests) l.base[r] = before + incl - n;
       before += all;
+    }
+    if (sizes && form > 0) {
+      const int64_t incl = block_scan(own_tiles, part, &all);
+      if (r < requests) l.tile[r] = (int)(tiles + incl - own_tiles);
+      tiles += all;
     }
     if (form > 0 || !sizes) {  // the second form's block wants to know if it has room
       const int64_t incl = block_scan(tokens, part, &all);
@@ -95,12 +101,31 @@ __global__ void __launch_bounds__(kScheduleThreads) schedule_kernel(const Schedu
     return;
   }
   if (tid == 0) {
-    const int64_t most = before / kLeast;
-    const int workers = before == 0 ? 0 : (int)min((int64_t)v.tiling.workers, max(most, (int64_t)1));
-    sh = Header{before, workers ? before / workers : 0, workers ? (int)(before % workers) : 0,
-                workers, lost};
-    *l.header = sh;
     l.base[requests] = before;
+    if (form > 0) l.tile[requests] = (int)tiles;
+    // whole tiles of each worker, and the unit that follows them
+    const int waves = form > 0 ? (int)(tiles / v.tiling.workers) - 1 : 0;
+    sh = Header{0, 0, 0, 0, max(waves, 0), lost};
+  }
+  __syncthreads();  // and the block's own writes are there
+  if (tid == 0) {
+    if (sh.waves > 0) {
+      Walk walk;
+      walk.enter(v, 0);
+      walk.tile(v, sh.waves * v.tiling.workers);
+      sh.first = l.base[walk.r] + walk.g * walk.q.total +
+                 units_before(walk.q, v.tiling.per, v.grow, walk.j);
+    }
+    const int64_t units = before - sh.first;
+    const int workers =
+        units == 0 ? 0
+                   : (int)min((int64_t)v.tiling.workers,
+                              sh.waves > 0 ? (int64_t)v.tiling.workers
+                                           : max(units / kLeast, (int64_t)1));
+    sh.share = workers ? units / workers : 0;
+    sh.more = workers ? (int)(units % workers) : 0;
+    sh.workers = workers;
+    *l.header = sh;
   }
   __syncthreads();  // and the block's own writes to base are there
   for (int w = tid; w < sh.workers; w += kScheduleThreads) {
@@ -300,7 +325,8 @@ int check_attend(const grm_b200_latent_plan* plan, const grm_b200_latent_arena* 
 }
 
 View view_of(const grm_b200_latent_plan& plan, const Shape& s, int form) {
-  return {lists_of(s, form, plan.work).base, plan.step.starts, plan.step.lens, plan.step.requests,
+  const Lists l = lists_of(s, form, plan.work);
+  return {l.base, l.tile, plan.step.starts, plan.step.lens, plan.step.requests,
           s.tiling[form], plan.step.grow ? 1 : 0, plan.heads};
 }
 
@@ -353,6 +379,7 @@ int make_shape(const grm_b200_latent_plan& p, int sms, Shape* s) {
   for (int f = 0; f < kForms; ++f) {
     s->off_header[f] = take(sizeof(Header));
     s->off_base[f] = take((p.step.requests + 1) * 8);
+    s->off_tile[f] = take(f > 0 ? (p.step.requests + 1) * 4 : 0);
     s->off_start[f] = take((int64_t)s->tiling[f].workers * (int64_t)sizeof(Start));
     s->off_join[f] = take((int64_t)s->tiling[f].workers * (int64_t)sizeof(Join));
   }

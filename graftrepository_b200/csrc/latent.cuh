@@ -24,11 +24,18 @@ constexpr int kStart = 384;
 // Fewest units of a worker.
 constexpr int kLeast = 640;
 
+// The expanded form's tiles are many where requests are long, and each head has keys and
+// values of its own: in equal shares one after another the workers would be at as many
+// heads as there are, whose keys and values L2 does not hold (8,449 rows of 40 heads:
+// 6.5 GB from HBM, 1.8 ms).  So all but the last one or two tiles of a worker go out
+// whole, tile i to worker i mod workers, and the rest in equal shares.
+
 struct Header {     // written by the schedule kernel, one for each form
-  int64_t units;    // of all tiles
+  int64_t first;    // unit that the shares begin with
   int64_t share;    // units of a worker
   int32_t more;     // workers that have one more
   int32_t workers;  // that share them
+  int32_t waves;    // tiles of each worker that go out whole
   int32_t lost;     // more tokens to expand than there is room for
 };
 
@@ -53,6 +60,7 @@ struct alignas(32) Join {
 struct Lists {
   Header* header;
   int64_t* base;  // [requests + 1] first unit of each request
+  int32_t* tile;  // [requests + 1] first tile of each request (expanded form)
   Start* start;   // [workers]
   Join* join;     // [workers], of the border where each begins
   float* part;    // [workers * splits * 2] partial results, see slot_floats
@@ -88,7 +96,7 @@ __host__ __device__ constexpr int slot_floats(int rows, int values) { return row
 // Byte offsets in the work area, which follow from the plan's sizes alone.
 struct Shape {
   Tiling tiling[2];  // absorbed, expanded
-  int64_t off_header[2], off_base[2], off_start[2], off_join[2];
+  int64_t off_header[2], off_base[2], off_tile[2], off_start[2], off_join[2];
   int64_t off_part, off_room, off_keys, off_values, bytes;
 };
 
@@ -98,6 +106,7 @@ inline Lists lists_of(const Shape& s, int form, void* work) {
   char* b = static_cast<char*>(work);
   return {reinterpret_cast<Header*>(b + s.off_header[form]),
           reinterpret_cast<int64_t*>(b + s.off_base[form]),
+          reinterpret_cast<int32_t*>(b + s.off_tile[form]),
           reinterpret_cast<Start*>(b + s.off_start[form]),
           reinterpret_cast<Join*>(b + s.off_join[form]),
           reinterpret_cast<float*>(b + s.off_part)};
@@ -106,6 +115,7 @@ inline Lists lists_of(const Shape& s, int form, void* work) {
 // What the walk over a form's tiles goes by.
 struct View {
   const int64_t* base;
+  const int32_t* tile;
   const int32_t* starts;
   const int32_t* lens;
   int64_t requests;
@@ -150,9 +160,10 @@ int make_map(CUtensorMap* map, const void* base, int rank, const int64_t* dims,
 // ---- the shares
 
 __host__ __device__ inline int64_t worker_first(int64_t w, const Header& h) {
-  return w * h.share + (w < h.more ? w : h.more);
+  return h.first + w * h.share + (w < h.more ? w : h.more);
 }
 __host__ __device__ inline int worker_of(int64_t u, const Header& h) {
+  u -= h.first;
   const int64_t big = h.more * (h.share + 1);
   return (int)(u < big ? u / (h.share + 1) : h.more + (u - big) / h.share);
 }
@@ -220,6 +231,21 @@ struct Walk {
     first = s.first;
     last = first + cost(v);
   }
+  // The i-th of all tiles, from the request where this one is on.
+  __host__ __device__ __forceinline__ void tile(const View& v, int i) {
+    if (i >= v.tile[r + 1]) {
+      int lo = r + 1, hi = (int)v.requests;
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (v.tile[mid] <= i) lo = mid;
+        else hi = mid;
+      }
+      enter(v, lo);
+    }
+    const int x = i - v.tile[r];
+    g = x / q.tiles;
+    j = x - g * q.tiles;
+  }
   __host__ __device__ __forceinline__ void next(const View& v) {  // there is one
     first = last;
     if (++j == q.tiles) {
@@ -257,16 +283,25 @@ template <int QUERIES, int STEP = kStep>
 struct Parts {
   Walk walk;
   int64_t u, end;
-  int w, count;
+  int w, whole, waves, count;
 
   __host__ __device__ __forceinline__ Parts(const Params& p, const Header& h, int worker,
                                             const Start& start)
-      : u(worker_first(worker, h)), end(worker_first(worker + 1, h)), w(worker), count(0) {
-    walk.start(p.v, start);
+      : u(worker_first(worker, h)), end(worker_first(worker + 1, h)), w(worker), whole(0),
+        waves(h.waves), count(0) {
+    if (QUERIES == 2 && waves > 0) walk.enter(p.v, 0);
+    else walk.start(p.v, start);
   }
   __host__ __device__ __forceinline__ bool next(const Params& p, Part* x) {
-    if (u >= end) return false;
-    if (count > 0) walk.next(p.v);
+    const bool all_of_it = QUERIES == 2 && whole < waves;
+    if (all_of_it) {
+      walk.tile(p.v, whole * p.v.tiling.workers + w);
+      ++whole;
+    } else {
+      if (u >= end) return false;
+      if (QUERIES == 2 && waves > 0 && count == 0) walk.start(p.v, p.l.start[w]);
+      if (count > 0) walk.next(p.v);
+    }
     x->r = walk.r;
     x->g = walk.g;
     x->start = walk.q.start;
@@ -279,10 +314,19 @@ struct Parts {
     x->toks[1] = QUERIES == 2 ? toks - x->toks[0] : 0;
     const int sees = p.causal ? imin(x->len, x->cached + x->tok0 + toks) : x->len;
     const int all = (sees + STEP - 1) / STEP;
-    const int64_t units = walk.last - walk.first;
-    const int64_t from = u - walk.first, to = imin(end, walk.last) - walk.first;
-    x->step0 = (int)(all * from / units);
-    x->steps = (int)(all * to / units) - x->step0;
+    if (all_of_it) {
+      x->step0 = 0;
+      x->steps = all;
+      x->slot = -1;
+      return true;
+    }
+    // The step that a unit of the tile falls on.  Any rounding will do, as the workers on
+    // both sides of a border round alike; a division in 64 bits is 100 instructions.
+    const int units = (int)(walk.last - walk.first), from = (int)(u - walk.first);
+    const int to = (int)(imin(end, walk.last) - walk.first);
+    const float per_unit = (float)all / (float)units;
+    x->step0 = imin(all, (int)((float)from * per_unit));
+    x->steps = (to == units ? all : imin(all, (int)((float)to * per_unit))) - x->step0;
     x->slot = from == 0 && to == units ? -1 : 2 * w + (count > 0 ? 1 : 0);
     u = imin(end, walk.last);
     ++count;

@@ -351,6 +351,17 @@ def test_expanded_long(latent, rope, nope, heads):
         close(turn.expanded(), turn.want(True, True))
 
 
+@pytest.mark.parametrize("latent,rope,nope", [(128, 32, 64), (128, 64, 128)])
+def test_expanded_of_more_tiles_than_blocks(latent, rope, nope):
+    """Tiles that go out whole, in the order of heads, before the rest is shared."""
+    turn = Turn([0, 300, 5], [2600, 0, 1900], 40, latent, rope, 64, BF, nope=nope)
+    close(turn.expanded(), turn.want(True, True))
+    turn = Turn([700] * 9, [300, 1, 256, 257, 0, 40, 512, 300, 300], 40, latent, rope, 16, HF,
+                nope=nope)
+    close(turn.expanded(), turn.want(True, True))
+    close(turn.expanded(causal=False), turn.want(False, True))
+
+
 def test_expanded_memory_and_the_absorbed_form_agree():
     """Rows that do not join; and the two forms of the same attention: queries taken
     into the latent space by the keys' weights, latent results out of it by the
