@@ -5,10 +5,13 @@
 // tokens at a time they are what that kernel waits for: 14 products of 64 clocks for
 // 64 tokens of each of its two query tiles, 1,800 clocks, where the exponentials take
 // 1,024.  Here scores are of 128 tokens (10 products) and results of 128 tokens and 64
-// values (8), 1,152 clocks for 64 tokens.  That leaves tensor memory for one buffer of
-// scores a query tile, so weights have a place of their own, and the next scores are
-// worked out as soon as the last of these have been read; queries are in shared
-// memory.
+// values (8), 1,152 clocks for 64 tokens.
+//
+// Tensor memory holds two results of 64 columns and three buffers of 128 scores, which
+// the tiles' steps take in turn, weights over the scores they are made from: while one
+// tile's softmax runs, the other's next scores are there and its own are on their way.
+// One warp issues all products, in the order in which the softmax warps take turns.
+// Queries are in shared memory.
 //
 // 8,449 rows of 3 requests of up to 16,000 tokens, 40 heads of 64 + 32, 64: 1.7 ms in
 // latent_attend.cu's way, @@ here.
@@ -30,6 +33,7 @@ constexpr int kTokens = 128;          // of a step
 constexpr int kHead = 64;             // values of a head's keys beside the positional part
 constexpr int kAtom = kTokens * 128;  // 128 tokens or rows x 64 values
 constexpr int kQ = 2;                 // query tiles
+constexpr int kBuffers = 3;           // of scores
 constexpr uint32_t kTmemCols = 512;
 
 template <int ROPE>
@@ -42,12 +46,11 @@ struct Layout {
   static constexpr int kQuery = kAtom + kRows * ROPE * 2;  // the positional part last
   static constexpr int kStages = (232448 - 1024 - 1024 - kQ * kQuery) / kStage;
   static constexpr int kSmem = 1024 + kQ * kQuery + kStages * kStage;
-  static constexpr uint32_t kScore = 0, kResult = kQ * kTokens;
-  static constexpr uint32_t kWeights = kResult + kQ * kHead;
-  static constexpr int kSoftWarps = 4 * kQ, kMmaWarp = kSoftWarps, kLoadWarp = kMmaWarp + kQ;
-  static constexpr int kThreads = (kLoadWarp + 1) * 32;
+  static constexpr uint32_t kResult = kBuffers * kTokens;
+  static constexpr int kSoftWarps = 4 * kQ, kMmaWarp = kSoftWarps;  // and one that loads
+  static constexpr int kThreads = (kMmaWarp + 2) * 32;
   static constexpr int kSlot = slot_floats(kRows * kQ, kHead);
-  static_assert(kStages >= 2 && kWeights + kQ * kTokens / 2 <= kTmemCols, "tiles");
+  static_assert(kStages >= 2 && kResult + kQ * kHead <= kTmemCols, "tiles");
 };
 
 // fp32 accumulators, 16-bit operands, 128 rows, n columns; B K-major or (b_mn) not.
@@ -140,8 +143,8 @@ __global__ void __launch_bounds__(Layout<ROPE>::kThreads, 1)
   unsigned char* const sm = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
   unsigned char* const sm_q = sm;                         // [kQ]
   unsigned char* const sm_stage = sm + kQ * LY::kQuery;   // [kStages]
-  __shared__ __align__(8) uint64_t full[kStages], empty[kStages], q_full[kQ], drained[kQ],
-      s_full[kQ], s_empty[kQ], p_full[kQ][2], o_full[kQ], o_done[kQ], turn[kQ][4];
+  __shared__ __align__(8) uint64_t full[kStages], empty[kStages], q_full[kQ], drained,
+      s_full[kBuffers], p_full[kBuffers][2], o_full[kQ], o_done[kQ], turn[kQ][4];
   __shared__ uint32_t sh_tmem;
   __shared__ int sh_fail;
 
@@ -159,18 +162,19 @@ __global__ void __launch_bounds__(Layout<ROPE>::kThreads, 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&full[i], 1);
-      mbar_init(&empty[i], kQ);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < kBuffers; ++i) {
+      mbar_init(&s_full[i], 1);
+      for (int x = 0; x < 2; ++x) mbar_init(&p_full[i][x], 4);
     }
     for (int t = 0; t < kQ; ++t) {
       mbar_init(&q_full[t], 4);
-      mbar_init(&drained[t], 1);
-      mbar_init(&s_full[t], 1);
-      mbar_init(&s_empty[t], 4);
       mbar_init(&o_full[t], 1);
       mbar_init(&o_done[t], 1);
-      for (int x = 0; x < 2; ++x) mbar_init(&p_full[t][x], 4);
       for (int x = 0; x < 4; ++x) mbar_init(&turn[t][x], 1);
     }
+    mbar_init(&drained, 1);
     mbar_fence_init();
     sh_fail = 0;
   }
@@ -192,13 +196,12 @@ __global__ void __launch_bounds__(Layout<ROPE>::kThreads, 1)
     // ------------------------------------------------------------- softmax
     const int t = warp >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t s_col = tmem + lanes + LY::kScore + t * kTokens;
     const uint32_t o_col = tmem + lanes + LY::kResult + t * kHead;
-    const uint32_t p_col = tmem + lanes + LY::kWeights + t * (kTokens / 2);
     unsigned char* const my_q = sm_q + t * LY::kQuery;
     bool ok = true;
     int it = 0, tile = 0, stage0 = 0;  // steps and tiles of this query tile; stages so far
     int turns = 0;                     // steps of both query tiles so far
+    unsigned scored = 0;               // scores of the parts before, of either tile
     // the row's query of a part, to shared memory
     auto queries = [&](const Part& y) {
       const Row b = row_of<true>(p, y, t, row);
@@ -283,8 +286,11 @@ __global__ void __launch_bounds__(Layout<ROPE>::kThreads, 1)
       if (!more) break;
       x = next;
       steps = x.steps;
+      const bool two = x.toks[1] > 0;
       const int stage_base = stage0;
+      const unsigned scored0 = scored;
       stage0 += steps;
+      scored += steps << two;
       held = x.toks[t] > 0;
       if (!held || steps == 0) more = parts.next(p, &next);
       if (!held) continue;
@@ -294,10 +300,11 @@ __global__ void __launch_bounds__(Layout<ROPE>::kThreads, 1)
       // tokens that the row sees, from the part's first on
       const int lim = (p.causal ? min(x.len, x.cached + a.token + 1) : x.len) - x.step0 * kTokens;
       idle = !__any_sync(kFull, a.active);
-      const bool two = x.toks[1] > 0;
 #pragma unroll 1
       for (int i = 0; i < steps; ++i, ++it) {
-        if (!(ok = wait(&s_full[t], it & 1))) break;
+        const unsigned n = scored0 + (two ? 2 * i + t : i), buf = n % kBuffers;
+        const uint32_t s_col = tmem + lanes + buf * kTokens;
+        if (!(ok = wait(&s_full[buf], (n / kBuffers) & 1))) break;
         tc_fence_after();
         // The two softmax warps of a scheduler take turns at the exponentials, so that one's
         // other work lies under them.
@@ -309,9 +316,8 @@ __global__ void __launch_bounds__(Layout<ROPE>::kThreads, 1)
         if (idle) {
           if (two && !(ok = my_turn())) break;
           if (lane == 0) {
-            mbar_arrive(&s_empty[t]);
-            mbar_arrive(&p_full[t][0]);
-            mbar_arrive(&p_full[t][1]);
+            mbar_arrive(&p_full[buf][0]);
+            mbar_arrive(&p_full[buf][1]);
             if (two) mbar_arrive(&turn[1 - t][warp & 3]);
           }
           if (i == 0) more = parts.next(p, &next);
@@ -343,18 +349,15 @@ __global__ void __launch_bounds__(Layout<ROPE>::kThreads, 1)
                                    __uint_as_float(v[k / 32][k % 32 + 1]));
         }
         const float top = fmaxf(max3(tops[0], tops[1], tops[2]), tops[3]) * p.scale_log2;
-        // the weights' place, once the products of the step before have ended
-        if (i > 0) {
-          if (!(ok = wait(&o_full[t], (it - 1) & 1))) break;
-          tc_fence_after();
-        }
         if (__any_sync(kFull, top > m + kLazy)) {
           const float now = top > m + kLazy ? reference_of(top) : m;
           const float f = now == m ? 1.0f : ex2(m - now);
           m = now;
           l *= f;
           lr *= f;
-          if (i > 0)
+          if (i > 0) {  // once the products of the step before have ended
+            if (!(ok = wait(&o_full[t], (it - 1) & 1))) break;
+            tc_fence_after();
 #pragma unroll 1
             for (int c = 0; c < kHead / 16; ++c) {
               uint32_t o[16];
@@ -363,6 +366,7 @@ __global__ void __launch_bounds__(Layout<ROPE>::kThreads, 1)
               for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
               tmem_st16(o_col + 16 * c, o);
             }
+          }
         }
         const float off = m == -INFINITY ? 0.0f : Kind<T>::kLift - m;
         if (two && !(ok = my_turn())) break;
@@ -371,13 +375,7 @@ __global__ void __launch_bounds__(Layout<ROPE>::kThreads, 1)
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           tmem_wait_ld32(v[c & 1]);
-          if (c < 3) {
-            tmem_ld32_nowait(s_col + 32 * (c + 1), v[(c + 1) & 1]);
-          } else {  // all scores have been read
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&s_empty[t]);
-          }
+          if (c < 3) tmem_ld32_nowait(s_col + 32 * (c + 1), v[(c + 1) & 1]);
           uint32_t w[16];
 #pragma unroll
           for (int k = 0; k < 32; k += 2) {
@@ -390,12 +388,12 @@ __global__ void __launch_bounds__(Layout<ROPE>::kThreads, 1)
             // seven eighths done: the other's first ones fill the gaps of the last
             if (c == 3 && k == 14 && two && lane == 0) mbar_arrive(&turn[1 - t][warp & 3]);
           }
-          tmem_st16(p_col + 16 * c, w);
+          tmem_st16(s_col + 16 * c, w);  // over scores that have been read
           if (c & 1) {  // half of the weights
             tmem_wait_st();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&p_full[t][c >> 1]);
+            if (lane == 0) mbar_arrive(&p_full[buf][c >> 1]);
           }
         }
         l += sum.x + sum.y;
@@ -405,98 +403,92 @@ __global__ void __launch_bounds__(Layout<ROPE>::kThreads, 1)
       }
       if (!ok) break;
     }
-  } else if (warp < LY::kLoadWarp) {
+  } else if (warp == LY::kMmaWarp) {
     // ---------------------------------------------------------- products
-    const int t = __shfl_sync(kFull, warp, 0) - LY::kMmaWarp;
     const uint32_t base = __shfl_sync(kFull, tmem, 0);
-    const uint32_t s_at = base + LY::kScore + t * kTokens;
-    const uint32_t o_at = base + LY::kResult + t * kHead;
-    const uint32_t p_at = base + LY::kWeights + t * (kTokens / 2);
-    const uint32_t q_lo = (uint32_t)sw128_desc(sm_q + t * LY::kQuery);
+    const uint32_t q_lo = (uint32_t)sw128_desc(sm_q);
     const uint32_t k_lo = (uint32_t)sw128_desc(sm_stage);
     const uint32_t v_lo = (uint32_t)sw128_mn_desc(sm_stage + LY::kValueAt, kAtom);
     auto desc = [&](uint32_t hi, uint32_t lo) { return (uint64_t)hi << 32 | lo; };
-    int it = 0, tile = 0, stage0 = 0;
+    int stage0 = 0;
+    unsigned tiles = 0, scored = 0;  // tiles so far: 16 bits for each query tile
     bool ok = true;
     Part next;
     bool more = parts.next(p, &next);
 #pragma unroll 1
     while (ok && more) {
       x = next;
-      const int steps = __shfl_sync(kFull, x.steps, 0);
-      if (x.toks[t] == 0 || steps == 0) more = parts.next(p, &next);
-      if (x.toks[t] == 0) {  // nothing to do for this one: give the stages back
+      const int two = __shfl_sync(kFull, x.toks[1] > 0 ? 1 : 0, 0);
+      const int count = __shfl_sync(kFull, x.steps, 0) << two;  // of scores
+      if (count == 0) more = parts.next(p, &next);
+      // Scores three ahead of results (of one tile alone no more steps than there are
+      // stages), each of them in one place of the code.  The buffer that scores go to
+      // held the weights of the products issued just before.
+      const int ahead = two || kStages >= kBuffers ? kBuffers : kStages;
 #pragma unroll 1
-        for (int i = 0; i < steps && ok; ++i) {
-          const int s = stage0 + i;
-          ok = wait(&full[s % kStages], (s / kStages) & 1);
-          if (ok && lane == 0) mbar_arrive(&empty[s % kStages]);
-          __syncwarp();
+      for (int n = -ahead; n < count && ok; ++n) {
+        if (n == 0) more = parts.next(p, &next);  // under the first softmax
+        if (n >= 0) {
+          const int t = n & two, i = n >> two, s = (stage0 + i) % kStages;
+          const unsigned buf = (scored + n) % kBuffers, phase = (scored + n) / kBuffers & 1;
+          const uint32_t vd = v_lo + (uint32_t)s * (LY::kStage / 16);
+          const uint32_t o_at = base + LY::kResult + t * kHead;
+#pragma unroll 1
+          for (int half = 0; half < 2; ++half) {
+            if (!(ok = wait(&p_full[buf][half], phase))) break;
+            tc_fence_after();
+            if (elect_one()) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                umma_f16_ts(o_at, base + buf * kTokens + half * 32 + 8 * k,
+                            desc(kHi128, vd + (half * 4 + k) * (16 * 128 / 16)),
+                            idesc<T>(kHead, true), i != 0 || half + k != 0);
+              if (half) {
+                umma_commit(&o_full[t]);
+                if (t == two) umma_commit(&empty[s]);
+                if (n + 1 + two - t >= count) umma_commit(&o_done[t]);
+              }
+            }
+            __syncwarp();
+          }
+          if (!ok) break;
         }
-        stage0 += steps;
-        continue;
-      }
-      if (steps == 0) continue;
-      ok = wait(&q_full[t], tile & 1);
-      if (!ok) break;
-      tc_fence_after();
-      // scores a step ahead of results, each of them in one place of the code
-#pragma unroll 1
-      for (int i = -1; i < steps && ok; ++i) {
-        if (i == 0) more = parts.next(p, &next);  // under the first softmax
-        if (i + 1 < steps) {
-          const int s = stage0 + i + 1, n = it + i + 1;
-          // the scores before have been read
-          if (n > 0 && !(ok = wait(&s_empty[t], (n - 1) & 1))) break;
+        if (n + ahead < count) {
+          const int e = n + ahead, t = e & two, i = e >> two, s = stage0 + i;
+          const unsigned buf = (scored + e) % kBuffers;
+          if (i == 0) {
+            if (!(ok = wait(&q_full[t], tiles >> (16 * t) & 1))) break;
+            tiles = t ? tiles + 0x10000u : (tiles & 0xFFFF0000u) | ((tiles + 1) & 0xFFFFu);
+          }
           if (!(ok = wait(&full[s % kStages], (s / kStages) & 1))) break;
           tc_fence_after();
           const uint32_t kd = k_lo + (uint32_t)(s % kStages) * (LY::kStage / 16);
+          const uint32_t qd = q_lo + t * (LY::kQuery / 16), to = base + buf * kTokens;
           if (elect_one()) {
 #pragma unroll
             for (int half = 0; half < 2; ++half)
 #pragma unroll
               for (int k = 0; k < kHead / 16; ++k)
-                umma_f16(s_at, desc(kHi128, q_lo + k * 2), desc(kHi128, kd + (half * kAtom + k * 32) / 16),
-                         idesc<T>(kTokens, false), half + k != 0);
+                umma_f16(to, desc(kHi128, qd + k * 2),
+                         desc(kHi128, kd + (half * kAtom + k * 32) / 16), idesc<T>(kTokens, false),
+                         half + k != 0);
             constexpr uint32_t kHi = ROPE == 64 ? kHi128 : kHi64;
 #pragma unroll
             for (int k = 0; k < ROPE / 16; ++k)
-              umma_f16(s_at, desc(kHi, q_lo + (kAtom + k * 32) / 16),
+              umma_f16(to, desc(kHi, qd + (kAtom + k * 32) / 16),
                        desc(kHi, kd + (LY::kRopeAt + k * 32) / 16), idesc<T>(kTokens, false), 1);
-            umma_commit(&s_full[t]);
-          }
-          __syncwarp();
-        }
-        if (i < 0) continue;
-        const int s = (stage0 + i) % kStages;
-        const uint32_t vd = v_lo + (uint32_t)s * (LY::kStage / 16);
-#pragma unroll 1
-        for (int half = 0; half < 2; ++half) {
-          if (!(ok = wait(&p_full[t][half], (it + i) & 1))) break;
-          tc_fence_after();
-          if (elect_one()) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              umma_f16_ts(o_at, p_at + half * 32 + 8 * k,
-                          desc(kHi128, vd + (half * 4 + k) * (16 * 128 / 16)),
-                          idesc<T>(kHead, true), i != 0 || half + k != 0);
-            if (half) {
-              umma_commit(&o_full[t]);
-              umma_commit(&empty[s]);
-              if (i + 1 == steps) umma_commit(&o_done[t]);
-            }
+            umma_commit(&s_full[buf]);
           }
           __syncwarp();
         }
       }
-      stage0 += steps;
-      it += steps;
-      ++tile;
+      stage0 += count >> two;
+      scored += count;
     }
     // whatever happened, nothing is in flight when tensor memory is given back
-    if (elect_one()) umma_commit(&drained[t]);
+    if (elect_one()) umma_commit(&drained);
     __syncwarp();
-    mbar_wait(&drained[t], 0, kProbes);
+    mbar_wait(&drained, 0, kProbes);
   } else {
     // -------------------------------------- keys and values, positional parts from pages
     const int piece = min(1 << p.page_shift, kTokens), pieces = kTokens / piece;
