@@ -148,7 +148,6 @@ struct Params {
 
 int launch_absorbed(const Params& p, cudaStream_t st);
 int launch_few(const Params& p, cudaStream_t st);
-int launch_prompt(const Params& p, cudaStream_t st);
 int launch_expanded(const Params& p, cudaStream_t st);
 int launch_expand(const Params& p, cudaStream_t st);
 

@@ -677,7 +677,7 @@ int launch_absorbed(const Params& p, cudaStream_t st) {
 }
 
 int launch_expanded(const Params& p, cudaStream_t st) {
-  return p.nope == 64 ? launch_prompt(p, st) : launch_rope<128, true>(p, st);
+  return p.nope == 64 ? launch_rope<64, true>(p, st) : launch_rope<128, true>(p, st);
 }
 
 }  // namespace latent
