@@ -8,11 +8,15 @@
 // A block, one an SM, takes an equal share of (128 tokens, head) pairs, a tile of
 // tokens after another: their rows come to shared memory once a tile, from their pages
 // by tensor-map copies, and the heads' weights stream by, 128 rows of 64 columns at a
-// time.  Results go from tensor memory (two buffers, so that products run under the
-// conversion) through shared memory to global memory by tensor-map copies.
+// time.  Results go from tensor memory (four buffers, so that products run under the
+// conversion) through shared memory to global memory by tensor-map copies, one pair by
+// one group of four warps and the next by the other: what holds a group up is the
+// chain of conversion, barriers and copies.
 //
-// Bound by HBM's writes: 6 bytes out for a token, head and 2 * nope values (476 MB for
-// 31,000 tokens of 40 heads of 64 + 64) against 0.8 GFLOP a MB.
+// HBM's writes are the floor: 6 bytes for a token, head and value a head has of either
+// kind (476 MB, 73 us, for 31,000 tokens of 40 heads of 32 + 32).  What holds it up is the
+// conversion: 210 us there with one group of four warps and two buffers, 156 us with two
+// groups and four.
 #include <algorithm>
 
 #include "latent_device.cuh"
@@ -26,8 +30,10 @@ using paged::kProbes;
 
 constexpr int kTile = 128;               // tokens
 constexpr int kAtom = kTile * 128;       // 128 rows of 64 values
-constexpr int kEpilogueWarps = 4, kMmaWarp = 4;  // and one that loads
-constexpr int kThreads = 6 * 32;
+constexpr int kGroups = 2, kMmaWarp = 4 * kGroups;  // and one that loads
+constexpr int kThreads = (kMmaWarp + 2) * 32;
+constexpr int kBuffers = 4;              // of results in tensor memory
+constexpr uint32_t kTmemCols = kBuffers * 128;
 constexpr int kStages = 4;               // of weights
 constexpr int kCols = 32;                // results that go out together
 constexpr int kPlace = kTile * kCols * 2;
@@ -36,9 +42,9 @@ template <int LATENT>
 struct Layout {
   static constexpr int kAtoms = LATENT / 64;
   static constexpr int kWeights = kAtoms * kAtom;          // after the rows
-  // results on their way out: two places of numbers and what they left over
+  // results on their way out: a group's numbers and what they left over
   static constexpr int kOut = kWeights + kStages * kAtom;
-  static constexpr int kUsed = 1024 + kOut + 4 * kPlace;
+  static constexpr int kUsed = 1024 + kOut + 2 * kGroups * kPlace;
   static constexpr int kSmem = kUsed > 120 * 1024 ? kUsed : 120 * 1024;
 };
 
@@ -53,16 +59,16 @@ __device__ __forceinline__ void tma_store(const CUtensorMap* map, int x, int y, 
                : "memory");
 }
 
-__device__ __forceinline__ void epilogue_sync() {
-  asm volatile("bar.sync 1, 128;" ::: "memory");
+__device__ __forceinline__ void group_sync(int group) {
+  asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory");
 }
-// The same, and whether all of them are fine.
-__device__ __forceinline__ bool epilogue_all(bool ok) {
+// The same, and whether all of the group are fine.
+__device__ __forceinline__ bool group_all(int group, bool ok) {
   unsigned r;
   asm volatile("{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n"
-               " barrier.cta.red.and.pred q, 1, 128, p;\n selp.u32 %0, 1, 0, q;\n}\n"
+               " barrier.cta.red.and.pred q, %2, 128, p;\n selp.u32 %0, 1, 0, q;\n}\n"
                : "=r"(r)
-               : "r"((unsigned)ok)
+               : "r"((unsigned)ok), "r"(1 + group)
                : "memory");
   return r != 0;
 }
@@ -75,8 +81,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   unsigned char* const sm = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
   unsigned char* const sm_w = sm + LY::kWeights;
   unsigned char* const sm_out = sm + LY::kOut;
-  __shared__ __align__(8) uint64_t a_full, a_empty, b_full[kStages], b_empty[kStages], d_full[2],
-      d_empty[2], drained;
+  __shared__ __align__(8) uint64_t a_full, a_empty, b_full[kStages], b_empty[kStages],
+      d_full[kBuffers], d_empty[kBuffers], drained;
   __shared__ uint32_t sh_tmem;
   __shared__ int sh_fail;
 
@@ -94,16 +100,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&b_full[i], 1);
       mbar_init(&b_empty[i], 1);
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < kBuffers; ++i) {
       mbar_init(&d_full[i], 1);
-      mbar_init(&d_empty[i], kEpilogueWarps);
+      mbar_init(&d_empty[i], 4);
     }
     mbar_init(&drained, 1);
     mbar_fence_init();
     sh_fail = 0;
   }
   if (warp == kMmaWarp) {
-    tmem_alloc(&sh_tmem, 256);
+    tmem_alloc(&sh_tmem, kTmemCols);
     tmem_relinquish();
   }
   tc_fence_before();
@@ -121,32 +127,34 @@ __global__ void __launch_bounds__(kThreads, 1)
     return ok;
   };
 
-  if (warp < kEpilogueWarps) {
+  if (warp < kMmaWarp) {
     // ---------------------------------------- results to the arena's type and out
-    const int row = warp * 32 + lane;
-    const uint32_t lanes = (uint32_t)(warp * 32) << 16;
-    bool ok = true;  // the same in all four warps, which meet at barriers below
-    int it = 0, place = 0;
+    const int group = warp >> 2, row = (warp & 3) * 32 + lane;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const bool copies = (threadIdx.x & 127) == 0;  // one thread of the group
+    unsigned char* const to = sm_out + group * 2 * kPlace;
+    bool ok = true;  // the same in a group's four warps, which meet at barriers below
 #pragma unroll 1
-    for (int64_t x = first; x < end && ok; ++x) {
+    for (int64_t x = first + group; x < end && ok; x += kGroups) {
+      int it = (int)(x - first) * units;
       const int t0 = (int)(x / p.heads) * kTile, h = (int)(x % p.heads);
       bool bad = false;  // a value that is no number
 #pragma unroll 1
       for (int u = 0; u < units; ++u, ++it) {
-        if (!(ok = epilogue_all(wait(&d_full[it & 1], (it >> 1) & 1)))) break;
+        const int buf = it % kBuffers;
+        if (!(ok = group_all(group, wait(&d_full[buf], (it / kBuffers) & 1)))) break;
         tc_fence_after();
         // values first: the upper half of a unit of both, or a unit of their own
 #pragma unroll 1
-        for (int y = 128 / kCols - 1; y >= 0; --y, place ^= 1) {
+        for (int y = 128 / kCols - 1; y >= 0; --y) {
           const bool value = units == 1 ? y >= 64 / kCols : u == 0;
           const int col = (units == 1 ? y % (64 / kCols) : y) * kCols;  // of the head's
           uint32_t v[32];
-          tmem_ld32_nowait(tmem + lanes + (it & 1) * 128 + y * kCols, v);
+          tmem_ld32_nowait(tmem + lanes + buf * 128 + y * kCols, v);
           tmem_wait_ld32(v);
-          // the copies before the last have left this place
-          if (threadIdx.x == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
-          epilogue_sync();
-          unsigned char* const to = sm_out + place * 2 * kPlace;
+          // the copies before have left this place
+          if (copies) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+          group_sync(group);
 #pragma unroll
           for (int c = 0; c < kCols / 8; ++c) {
             uint32_t hi[4], lo[4];
@@ -169,8 +177,8 @@ __global__ void __launch_bounds__(kThreads, 1)
               *reinterpret_cast<uint4*>(to + kPlace + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
           }
           fence_proxy_async_smem();
-          epilogue_sync();
-          if (threadIdx.x == 0) {
+          group_sync(group);
+          if (copies) {
             for (int half = 0; half < 2; ++half) {
               const int t = t0 + half * 64, at = half * (kPlace / 2);
               if (t >= total) break;
@@ -186,10 +194,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&d_empty[it & 1]);
+        if (lane == 0) mbar_arrive(&d_empty[buf]);
       }
     }
-    if (threadIdx.x == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    if (copies) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   } else if (warp == kMmaWarp) {
     // ---------------------------------------------------------- products
     const uint32_t base = __shfl_sync(kFull, tmem, 0);
@@ -207,7 +215,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
 #pragma unroll 1
       for (int u = 0; u < units && ok; ++u, ++it) {
-        if (it >= 2 && !(ok = wait(&d_empty[it & 1], ((it >> 1) - 1) & 1))) break;
+        const int buf = it % kBuffers;
+        if (it >= kBuffers && !(ok = wait(&d_empty[buf], (it / kBuffers - 1) & 1))) break;
         tc_fence_after();
 #pragma unroll 1
         for (int c = 0; c < LY::kAtoms; ++c, ++s) {
@@ -216,14 +225,14 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (elect_one()) {
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              umma_f16(base + (it & 1) * 128, a_desc + (c * kAtom + k * 32) / 16,
+              umma_f16(base + buf * 128, a_desc + (c * kAtom + k * 32) / 16,
                        b_desc + (s % kStages * kAtom + k * 32) / 16, kIdesc, c + k != 0);
             umma_commit(&b_empty[s % kStages]);
           }
           __syncwarp();
         }
         if (ok && elect_one()) {
-          umma_commit(&d_full[it & 1]);
+          umma_commit(&d_full[buf]);
           if (u + 1 == units && (x + 1) / p.heads != tile) umma_commit(&a_empty);
         }
         __syncwarp();
@@ -290,7 +299,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == kMmaWarp) tmem_dealloc(tmem, 256);
+  if (warp == kMmaWarp) tmem_dealloc(tmem, kTmemCols);
   if (sh_fail && threadIdx.x == 0) {  // attention then leaves no numbers
     atomicOr(p.status, GRM_B200_PLAN_WAIT);
     atomicExch(&p.l.header->lost, 1);
