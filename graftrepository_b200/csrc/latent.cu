@@ -241,11 +241,12 @@ int check_sizes(const grm_b200_latent_plan* p) {
   }
   const bool none = p->nope == 0 && p->value == 0 && p->expand_tokens == 0;
   const bool some = (p->nope == 64 || p->nope == 128) && p->value == p->nope &&
-                    p->expand_tokens >= 1 && p->expand_tokens <= (1 << 28);
+                    p->expand_tokens >= 1 && p->expand_tokens <= (1 << 28) &&
+                    p->expand_tokens * p->heads <= INT32_MAX;  // rows of keys
   if (!none && !some) {
     set_thread_error("latent plan: nope %d and value %d must both be 64 or both 128, with "
-                     "expand_tokens %lld from 1 to 2^28 (or all 0)", p->nope, p->value,
-                     (long long)p->expand_tokens);
+                     "expand_tokens %lld from 1 to 2^28 and below 2^31 times the heads (or all 0)",
+                     p->nope, p->value, (long long)p->expand_tokens);
     return GRM_B200_EINVAL;
   }
   return 0;

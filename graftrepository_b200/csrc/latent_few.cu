@@ -1,5 +1,5 @@
-// latent_few.cu -- latent attention in the absorbed form for few query rows: decoding,
-// where a request brings a row of each head, up to 48 in all.
+// latent_few.cu -- latent attention in the absorbed form for few query rows: decoding over
+// a latent of 512, where a request brings a row of each head, up to 32 in all.
 //
 // The sums are latent_attend.cu's.  There rows are the 128 lanes of the tensor cores'
 // products; with few of them most lanes would do nothing, and a latent of 512 needs
@@ -8,9 +8,14 @@
 // the same copy of the tokens' rows being K (values of a token side by side) and V^T
 // (read the other way).  Results are 128 values of all rows in a lane each, few
 // columns, so that there are two of them and one goes out while the next tile is worked
-// on.  Bound by HBM: 128 tokens of 256 + 32 values are 73.7 KB, 3,200 clocks of an SM's
-// share, their products about 1,600 (shared memory: 4 KB of rows for each 16 x 128),
-// their exponentials 600.
+// on.  Bound by HBM: 128 tokens of 512 + 64 values are 147 KB, 6,400 clocks of an SM's
+// share, their products about 3,200 (shared memory: 4 KB of rows for each 16 x 128),
+// their exponentials 600.  As the next step's rows have to be on their way while this one's
+// are worked on, and there is room for 1.4 steps of them, a product waits for its rows: 250,007
+// tokens (288 MB, 44 us) of 16 heads take 100 us, 173 us with latent_attend.cu's kernel.
+// At latents of 128 and 256 that one is the faster (148 requests of 4,096 tokens, 40
+// heads of 256 + 32: 70 us, 102 us with this one), whose products cost as much
+// however few their columns are.
 //
 // A block's warps:
 //   0-7   softmax, a token and half of the rows a lane: scores from tensor memory,
@@ -366,18 +371,18 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             // once the products of the step before have ended
             ok = wait(&pv_done[(it - 1) & 1], ((it - 1) >> 1) & 1);
+            if (soft_any(!ok)) { ok = false; break; }  // all of them, or the others would wait
             tc_fence_after();
-            if (ok)
 #pragma unroll 1
-              for (int c = half * 16; c < kPairs * N; c += 32) {
-                const uint32_t at = tmem + lanes + LY::kResult + ob * kPairs * N + c;
-                uint32_t o[16];
-                tmem_ld16(at, o);
+            for (int c = half * 16; c < kPairs * N; c += 32) {
+              const uint32_t at = tmem + lanes + LY::kResult + ob * kPairs * N + c;
+              uint32_t o[16];
+              tmem_ld16(at, o);
 #pragma unroll
-                for (int k = 0; k < 16; ++k)
-                  o[k] = __float_as_uint(__uint_as_float(o[k]) * factor[c % N + k]);
-                tmem_st16(at, o);
-              }
+              for (int k = 0; k < 16; ++k)
+                o[k] = __float_as_uint(__uint_as_float(o[k]) * factor[c % N + k]);
+              tmem_st16(at, o);
+            }
             tmem_wait_st();
           }
         }
