@@ -21,7 +21,7 @@ ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = [
     "-std=c++17", "-O3", "-lineinfo", "--shared", "-Xcompiler", "-fPIC",
     "-Xcompiler", "-fvisibility=hidden", "--expt-relaxed-constexpr",
-    "-Xptxas", "-warn-spills",
+    "-Xptxas", "-warn-spills", "--threads=0",  # sources side by side
 ]
 
 

@@ -20,15 +20,22 @@ constexpr int kExpandAlign = 64;
 // end.  Tiles lie one after another, a request's by group (a head of the expanded
 // form; of the absorbed one 128 heads) and then by token; a worker's share may start
 // and end inside a tile, whose parts join_kernel puts together.
+//
+// kStart is what a tile's queries, result and first scores take, in tokens (64 take 0.87
+// us).  Measured, us of 64 requests of 32 to 16,384 tokens and one row, and of 16 requests
+// with 5 rows, 40 heads of 256 + 32: kStart 128 59.8 and 47, 256 57.6 and 45, 384 57.6 and
+// 43.  kLeast, the fewest units of a worker, weighs the parts that join_kernel has to read
+// against blocks that stand idle: 384, 512, 640 and 1,024 were within 2 % on those, and 640
+// the best for one request of 4,096 tokens.
 constexpr int kStart = 384;
-// Fewest units of a worker.
 constexpr int kLeast = 640;
 
 // The expanded form's tiles are many where requests are long, and each head has keys and
 // values of its own: in equal shares one after another the workers would be at as many
 // heads as there are, whose keys and values L2 does not hold (8,449 rows of 40 heads:
-// 6.5 GB from HBM, 1.8 ms).  So all but the last one or two tiles of a worker go out
-// whole, tile i to worker i mod workers, and the rest in equal shares.
+// 6.5 GB from HBM).  So all but the last one or two tiles of a worker go out whole, tile i
+// to worker i mod workers, and the rest in equal shares: 0.6 GB, in about the same time,
+// as the products are what it is bound by, but not at HBM's cost in power.
 
 struct Header {     // written by the schedule kernel, one for each form
   int64_t first;    // unit that the shares begin with
@@ -76,8 +83,10 @@ struct Tiling {
   int few;      // columns of latent_few.cu's kernel, which serves the step; 0: it does not
 };
 // The absorbed form's kernel for few rows (latent_few.cu) takes requests of up to 32 rows
-// of a step over a latent of 512, where latent_attend.cu's needs two blocks for a
-// tile and both work out the scores.
+// of a step over a latent of 512, where latent_attend.cu's needs two blocks for a tile and
+// both work out the scores (250,007 tokens of 16 heads: 173 us, 100 us with few.cu's).  Its
+// buffers have no room for more rows; over smaller latents it is the slower one (70 us
+// against 102 us for 148 requests of 4,096 tokens, 40 heads of 256 + 32).
 __host__ __device__ inline Tiling absorbed_tiling(int heads, int latent, int64_t most_tokens,
                                                   int sms) {
   const int64_t most = most_tokens * heads;

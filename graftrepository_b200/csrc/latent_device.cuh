@@ -144,7 +144,7 @@ __device__ __forceinline__ Row row_of(const Params& p, const Part& x, int t, int
 // values; lanes beyond those take every so many of the parts.  What is here runs once
 // in a launch, on instructions that are in no cache, so there are few of them: with
 // the tiles looked up here rather than in the plan, and a batch of parts unrolled, it
-// took 22 us where this takes 5 (64 conversations).
+// took 22 us where this takes 5 (64 requests of 32 to 16,384 tokens, one row each).
 // ROWS of a tile, V values of a block's results, SPLITS blocks that share a tile's.
 template <typename T, int V, int SPLITS, int ROWS, bool EXP>
 __global__ void __launch_bounds__(256) join_kernel(const Params p) {

@@ -11,6 +11,11 @@
 // anew they were half of the kernel's), into its own corner of shared memory, so that
 // no warp waits for another.  One pair at a time where strides, sizes or pointers are
 // not multiples of that.
+//
+// 8,449 bf16 rows of 32 heads of 128 (138 MB, 21.2 us at a copy's rate) take 25.0 us, 5.5
+// TB/s; 33 with a block's angles shared behind a barrier, 41 with a thread's own.  2,047 fp32
+// rows of 8 heads of 128, half of each rotated (17 MB, 2.6 us), take 8.4 and 61 bf16 rows of
+// 40 heads of 96 take 4.4: a launch, a token's angles and one trip to memory.
 #include <algorithm>
 
 #include "rotary.cuh"

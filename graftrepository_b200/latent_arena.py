@@ -74,9 +74,11 @@ class LatentPlan(PagePlan):
         if not 1 <= heads <= 1024:
             raise ValueError(f"heads must be 1 to 1024, got {heads}")
         if (nope, value, expand_tokens) != (0, 0, 0) and (
-                nope not in EXPANDED or value != nope or not 1 <= expand_tokens <= 1 << 28):
+                nope not in EXPANDED or value != nope or not 1 <= expand_tokens <= 1 << 28 or
+                expand_tokens * heads >= 1 << 31):
             raise ValueError(f"the expanded form takes nope = value of {EXPANDED} and "
-                             f"expand_tokens from 1 to 2^28, got {nope}, {value}, {expand_tokens}")
+                             f"expand_tokens from 1 to 2^28 and below 2^31 / heads, got {nope}, "
+                             f"{value}, {expand_tokens}")
         super().__init__(tables, tokens, 1, 1, 64, max_fresh)
         self.heads, self.latent, self.rope, self.dtype = int(heads), latent, rope, dtype
         self.nope, self.value, self.expand_tokens = int(nope), int(value), int(expand_tokens)
@@ -137,7 +139,7 @@ class LatentArena(_Buffers):
         becomes for each head (`nope` values of its keys, as many of its values, 64
         or 128) and room for `expand_tokens` tokens: the lengths of the requests
         with rows in a step, each rounded up to 64.  That room is expand_tokens *
-        heads * (nope + value) * 2 bytes.  A plan's steps may not overlap on the
+        heads * (2 * nope + value) * 2 bytes.  A plan's steps may not overlap on the
         GPU."""
         if tables.pages != self.pages or tables.page_tokens != self.page_tokens:
             raise ValueError(f"the tables have {tables.pages} pages of {tables.page_tokens} "
@@ -239,10 +241,12 @@ class LatentArena(_Buffers):
                         causal: bool = True, out=None, lse=None, stream=None):
         """Expanded form: queries ``q`` [tokens, heads, nope + rope]; ``weights`` [heads,
         nope + value, latent] make each head's keys (the first nope, beside the
-        row's positional part) and values from a row, rounded to the arena's type.
-        Returns (out [tokens, heads, value], lse); otherwise as ``attend``.  Where the
-        step has more tokens to expand than ``plan.expand_tokens`` (``plan.check``
-        says so) rows are NaN."""
+        row's positional part) and values from a row.  Values are rounded to the
+        arena's type, keys held as two numbers of it; a token of which one of these is
+        beyond the type's range makes the rows that see it NaN.  Returns (out
+        [tokens, heads, value], lse); otherwise as ``attend``.  Where the step has
+        more tokens to expand than ``plan.expand_tokens`` (``plan.check`` says so)
+        rows are NaN."""
         ref = self._ready(plan, layer)
         if not plan.nope:
             raise ValueError("the plan has no room for the expanded form (make_plan with nope, "

@@ -621,8 +621,10 @@ typedef struct grm_b200_latent_arena {
  * nope and value: what the expanded form makes of a latent row for each head (both
  * 64 or both 128; 0 where it is not used); expand_tokens: room for the tokens that
  * it expands, the lengths of the requests with rows in the step, each rounded up to
- * 64.  work: work_bytes (grm_b200_latent_work_bytes) of device memory, 256-byte
- * aligned; calls that share it must not overlap on the GPU. */
+ * 64 (expand_tokens * heads below 2^31).  work: work_bytes
+ * (grm_b200_latent_work_bytes; expand_tokens * heads * 2 * (2 * nope + value) of them
+ * are that room) of device memory, 256-byte aligned; calls that share it must not
+ * overlap on the GPU. */
 typedef struct grm_b200_latent_plan {
   grm_b200_paged_plan step;
   int32_t heads;
@@ -675,9 +677,13 @@ int grm_b200_latent_attend(const grm_b200_latent_plan* plan, const grm_b200_late
 /* Latent attention, expanded form: weights [heads, nope + value, latent] (head and
  * row strides, a row's values contiguous) make each head's keys and values,
  *   k_t = (weights[h, :nope] c_t, r_t),  v_t = weights[h, nope:] c_t,
- * rounded to the arena's type, and q [tokens, heads, nope + rope] attends to them;
- * out [tokens, heads, value].  Otherwise as grm_b200_latent_attend.  Fewer
- * operations than the absorbed form where a request has many rows (prompts). */
+ * and q [tokens, heads, nope + rope] attends to them; out [tokens, heads, value].
+ * Values are rounded to the arena's type, keys held as two numbers of it (what the
+ * first left over is the second).  A token of which a key or a value is beyond the type's
+ * range, or none, makes the rows that see it NaN.  Rows of weights must not overlap
+ * (head stride 0: the same weights for all heads).  Otherwise as
+ * grm_b200_latent_attend.  Fewer operations than the absorbed form where a request
+ * has many rows (prompts). */
 int grm_b200_latent_attend_expanded(const grm_b200_latent_plan* plan,
                                     const grm_b200_latent_arena* arena, const void* q_device,
                                     int64_t q_row_stride, int64_t q_head_stride,

@@ -139,3 +139,20 @@ def test_a_plan_for_latent_rows_is_not_the_8_bit_arena_s():
     arena.latent = 256
     with pytest.raises(ValueError, match="such rows"):
         arena._ready(plan, 0)
+
+
+@pytest.mark.parametrize("strides", [(1 << 15, 248), (1 << 15, 0), (248, 256), (8, 256)])
+def test_rows_of_weights_that_overlap(strides):
+    answer(expanded(latent_plan(), latent_arena(), w_strides=strides), "overlap")
+
+
+def test_room_for_more_rows_of_keys_than_there_are_numbers_for():
+    lib, need = _lib.load(), ctypes.c_int64(0)
+    for heads, tokens, refused in ((8, 1 << 28, True), (1024, 1 << 21, True),
+                                   (1024, (1 << 21) - 1, False)):
+        rc = lib.grm_b200_latent_work_bytes(
+            ctypes.byref(latent_plan(heads=heads, expand_tokens=tokens)), ctypes.byref(need))
+        if refused:
+            answer(rc, "2^31")
+        else:  # the next thing it looks at is the device
+            assert rc != -1
