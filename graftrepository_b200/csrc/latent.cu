@@ -166,18 +166,23 @@ struct AppendParams {
   int64_t latent_stride, rope_stride;
   uint16_t* cache;
   int latent, rope, rotary;
+  int copy_shift, rope_shift;  // threads of a row, as powers of two
 };
 
-// A thread for 8 values of a row, or for 8 pairs of its positional part.  Bound by
-// HBM where rows are many (1.5 us of 8,449 rows' 9.7 MB in and out), else a launch and three
-// dependent loads: 8.4 us for those rows with 32 of their 288 values rotated.
+// A thread for 8 values of a row, or for 8 pairs of its positional part, those of all
+// rows behind the others, so that a warp has one or the other to do: 8,358 rows of 256 +
+// 32 values (9.7 MB in and out, 1.5 us at a copy's rate) take 6.2 us with their positional
+// part rotated and 4.2 without, a launch and three dependent loads; 8.2 where every warp
+// had two lanes that rotate.
 template <typename T, bool IN, bool OUT>
 __global__ void __launch_bounds__(256) append_kernel(const AppendParams p) {
-  const int copies = p.latent / 8, entries = copies + (p.rotary ? p.rope / 16 : p.rope / 8);
+  const int copies = p.latent / 8;  // powers of two
   const int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t t = x / entries;
+  const int64_t y = x - p.tokens * copies;
+  const int shift = y < 0 ? p.copy_shift : p.rope_shift;
+  const int64_t t = (y < 0 ? x : y) >> shift;
   if (t >= p.tokens) return;
-  const int e = (int)(x - t * entries);
+  const int e = (int)((y < 0 ? x : y) & ((1 << shift) - 1)) + (y < 0 ? 0 : copies);
   const int64_t slot = p.slots[t];
   if (slot < 0 || slot >= p.limit) return;
   uint16_t* to = p.cache + slot * (p.latent + p.rope);
@@ -205,8 +210,8 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendParams p) {
 
 template <typename T>
 int launch_append(const AppendParams& p, cudaStream_t st) {
-  const int entries = p.latent / 8 + (p.rotary ? p.rope / 16 : p.rope / 8);
-  const unsigned blocks = (unsigned)ceil_div64(p.tokens * entries, 256);
+  const unsigned blocks = (unsigned)ceil_div64(
+      p.tokens * ((1 << p.copy_shift) + (1 << p.rope_shift)), 256);
   if (!p.rotary || p.r.layout == GRM_B200_ROTARY_HALF)
     append_kernel<T, false, false><<<blocks, 256, 0, st>>>(p);
   else if (p.r.layout == GRM_B200_ROTARY_INTERLEAVED)
@@ -525,6 +530,9 @@ int grm_b200_latent_append(const grm_b200_latent_plan* plan, const grm_b200_late
   p.latent = arena->latent;
   p.rope = arena->rope;
   p.rotary = rotary != nullptr;
+  auto log2_of = [](int n) { int s = 0; while (n > 1) { n >>= 1; ++s; } return s; };
+  p.copy_shift = log2_of(arena->latent / 8);
+  p.rope_shift = log2_of(arena->rope / (rotary ? 16 : 8));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return arena->dtype == GRM_B200_F16 ? launch_append<__half>(p, st)
                                       : launch_append<__nv_bfloat16>(p, st);

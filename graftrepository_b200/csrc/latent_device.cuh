@@ -140,8 +140,9 @@ __device__ __forceinline__ Row row_of(const Params& p, const Part& x, int t, int
 
 // Parts of tiles that lie in the shares of several workers, and the rows past the
 // step's last one.  A tile in n parts has n - 1 borders inside, whose blocks (one for
-// every eight of its rows) share the rows: 1 to 8 warps a row, each for some of its
-// values; lanes beyond those take every so many of the parts.  What is here runs once
+// every eight of its rows) share the rows: one warp a row or several, each for some of its
+// values; lanes beyond those take every so many of the parts.  A row in 148 parts is
+// many warps' (16 rows of 512 values: 35 us with eight of them at most, 13 with 64).  What is here runs once
 // in a launch, on instructions that are in no cache, so there are few of them: with
 // the tiles looked up here rather than in the plan, and a batch of parts unrolled, it
 // took 22 us where this takes 5 (64 requests of 32 to 16,384 tokens, one row each).
@@ -166,15 +167,19 @@ __global__ void __launch_bounds__(256) join_kernel(const Params p) {
     }
   }
   if (b >= workers || j.rows == 0) return;
-  // rows of a block: 1, 2, 4 or 8, as many as it takes
-  const int blocks = (j.parts - 1) * gridDim.y;
+  // warps of a row: 1, 2, 4 or 8, as many as there are, and beyond that as long as each lane
+  // has four parts or more to add up
+  const int warps = (j.parts - 1) * gridDim.y * 8;
   int shift = 0;
-  while ((blocks << shift) < j.rows) ++shift;  // at most 3
-  const int width = kLanes >> (3 - shift);     // float4 of a warp's
+  while ((j.rows << (shift + 1)) <= warps &&
+         (shift < 3 || (j.parts * (kLanes >> (shift + 1)) >= 128 && (kLanes >> (shift + 1)) >= 2)))
+    ++shift;
+  const int width = kLanes >> shift;  // float4 of a warp's
   const int wide = width < 32 ? width : 32;
-  const int of_row = warp & ((8 >> shift) - 1);
+  const int id = (j.border * gridDim.y + blockIdx.y) * 8 + warp;
+  const int of_row = id & ((1 << shift) - 1);
   const int column = of_row * width + (lane & (wide - 1));
-  const int line = ((j.border * gridDim.y + blockIdx.y) << shift) + (warp >> (3 - shift));
+  const int line = id >> shift;
   if (line >= j.rows) return;
   const float* const part = p.l.part + split * kSlot;
   float m = -INFINITY, l = 0.0f, lr = 0.0f;
