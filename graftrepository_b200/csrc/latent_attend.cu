@@ -32,11 +32,16 @@
 // Absorbed, a step of 64 tokens (40 heads of 256 + 32, one row) takes 0.87 us, 6.2 TB/s of
 // all SMs: its copies and its products are about level.  64 requests of 32 to 16,384
 // tokens (147 MB, 22.5 us at a copy's rate) take 52 us: 45 in this kernel, whose tiles' starts
-// and ends lie between steps, and 5 in join_kernel.  Expanded, it is bound by the issue of
-// products: 28 of them for 64 tokens of both query tiles, 64 + 32 wide, about 77 clocks
-// each; 8,449 rows on 31,000 tokens, 40 heads, take 1.75 ms, 0.68 PFLOP/s (keys count once).
-// Scores of 96 or 128 tokens were no faster: a product with both operands in shared memory
-// takes 100 clocks at 128 columns, 64 at least with queries in tensor memory.
+// and ends lie between steps, and 5 in join_kernel.  Expanded, it is bound by the two softmax
+// warps of a scheduler: 2,075 clocks for 64 tokens of both query tiles, of which a warp's
+// exponentials, their sums and roundings take 900, in turns; loads, maxima, waits and barriers
+// lie under the other's.  8,449 rows on 31,000 tokens, 40 heads of 64 + 32, take 1.75 ms, 0.6
+// PFLOP/s (keys count once).  Half of the exponentials left out make that 8 % less, the sum of
+// the rounded weights 6 %, half of the scores' products nothing: what a step takes apart from
+// its 64 tokens counts.  Scores of 96 or 128 tokens at a time were no faster all the same (a
+// product with both operands in shared memory takes 100 clocks at 128 columns, 64 at least with
+// queries in tensor memory), nor were keys and what they left over side by side in one
+// product of 128 columns, the sum left to the softmax (2.25 ms in all, where this takes 1.95).
 //
 // Tokens that a row does not see have weight 0, and a product of 0 and what is no
 // number would be none: where a hidden token's score is not finite, the numbers of
