@@ -41,7 +41,8 @@
 // its 64 tokens counts.  Scores of 96 or 128 tokens at a time were no faster all the same (a
 // product with both operands in shared memory takes 100 clocks at 128 columns, 64 at least with
 // queries in tensor memory), nor were keys and what they left over side by side in one
-// product of 128 columns, the sum left to the softmax (2.25 ms in all, where this takes 1.95).
+// product of 128 columns, the sum left to the softmax (2.25 ms in all, where this takes 1.95),
+// nor two threads a row (3.36 ms: 96 registers are too few).
 //
 // Tokens that a row does not see have weight 0, and a product of 0 and what is no
 // number would be none: where a hidden token's score is not finite, the numbers of
