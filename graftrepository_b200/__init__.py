@@ -7,6 +7,10 @@ for the device mount of routed grafts (core/graft_arena.py swap/unpack_node):
 * ``graft_mount``  -- fused dequantise + scatter into the bf16 arena
 * ``paged_arena``  -- keys and values of many requests at 8 bits in pages: step plans,
   append, attention, read-back
+* ``latent_arena`` -- pages of latent rows for many requests: append, latent attention in
+  the absorbed and the expanded form
+* ``rotary``       -- rotary positions put on and taken off, on their own or on the way
+  into either arena
 * ``sharded``      -- node-range sharded route over 1-8 GPUs (NCCL all-gather)
 * ``synth``        -- seeded synthetic banks with the benchmark configs' shapes
 

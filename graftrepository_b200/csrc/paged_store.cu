@@ -215,10 +215,10 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendParams p) {
 // A block is HEADS groups, for as many heads of one page, so that the angles of the
 // rows that they hold (about 25 instructions a pair) are worked out once and read from
 // shared memory; rows of a larger page beyond those work theirs out where they are
-// used.  22,500 fp16 rows of 8 heads of 128, 64 of them rotated (138 MB, 21.1 us at a copy's
-// rate), take 40.5 us, where a group of its own for each head took 58 and four heads
-// one after another 60; 61 bf16 rows of single tokens take 8.5, a launch and three
-// dependent loads.
+// used.  11,198 fp16 rows of 8 heads of 128, 64 values of each key's head rotated (69 MB
+// in and out, 10.5 us at a copy's rate), take 26.7 us and without the rotation 18.1; a group of
+// its own for each head took 44, four heads one after another 46.  61 bf16 rows of single
+// tokens take 4.2, with it or without: a launch and three dependent loads.
 
 struct TurnedParams {
   AppendParams a;
