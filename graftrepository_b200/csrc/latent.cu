@@ -57,6 +57,7 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* part, int64_t*
 __global__ void __launch_bounds__(kScheduleThreads) schedule_kernel(const ScheduleParams p) {
   __shared__ int64_t part[33];
   __shared__ Header sh;
+  __shared__ int64_t raw[kMostWorkers + 1], first;
   const int tid = threadIdx.x, form = blockIdx.x;
   const bool sizes = form < p.forms;  // else: room
   const Lists l = p.l[sizes ? form : 0];
@@ -67,7 +68,7 @@ __global__ void __launch_bounds__(kScheduleThreads) schedule_kernel(const Schedu
     const int64_t r = r0 + tid;
     int64_t n = 0, tokens = 0, own_tiles = 0;
     if (r < requests) {
-      const Request q = request_of(v.starts[r], v.starts[r + 1], v.lens[r], v.tiling.per, v.grow);
+      const Request q = request_of(v, (int)r);
       if (q.n > 0) {
         n = q.total * v.tiling.groups;
         own_tiles = (int64_t)q.tiles * v.tiling.groups;
@@ -105,7 +106,8 @@ __global__ void __launch_bounds__(kScheduleThreads) schedule_kernel(const Schedu
     if (form > 0) l.tile[requests] = (int)tiles;
     // whole tiles of each worker, and the unit that follows them
     const int waves = form > 0 ? (int)(tiles / v.tiling.workers) - 1 : 0;
-    sh = Header{0, 0, 0, 0, max(waves, 0), lost};
+    sh = Header{0, max(waves, 0), lost};
+    first = 0;
   }
   __syncthreads();  // and the block's own writes are there
   if (tid == 0) {
@@ -113,23 +115,56 @@ __global__ void __launch_bounds__(kScheduleThreads) schedule_kernel(const Schedu
       Walk walk;
       walk.enter(v, 0);
       walk.tile(v, sh.waves * v.tiling.workers);
-      sh.first = l.base[walk.r] + walk.g * walk.q.total +
-                 units_before(walk.q, v.tiling.per, v.grow, walk.j);
+      first = l.base[walk.r] + walk.g * walk.q.total + units_before(walk.q, v, walk.j);
     }
-    const int64_t units = before - sh.first;
-    const int workers =
-        units == 0 ? 0
-                   : (int)min((int64_t)v.tiling.workers,
-                              sh.waves > 0 ? (int64_t)v.tiling.workers
-                                           : max(units / kLeast, (int64_t)1));
-    sh.share = workers ? units / workers : 0;
-    sh.more = workers ? (int)(units % workers) : 0;
-    sh.workers = workers;
+    const int64_t units = before - first;
+    sh.workers = units == 0      ? 0
+                 : sh.waves > 0 ? v.tiling.workers
+                                : (int)min((int64_t)v.tiling.workers,
+                                           max(units / kLeast, (int64_t)1));
     *l.header = sh;
   }
-  __syncthreads();  // and the block's own writes to base are there
-  for (int w = tid; w < sh.workers; w += kScheduleThreads) {
-    const int64_t u = worker_first(w, sh);
+  __syncthreads();
+  // Shares that make up for what the whole tiles of a worker cost more or less than others'.
+  const int workers = sh.workers;
+  if (workers == 0) return;
+  const int64_t rest = before - first;
+  int64_t cost = 0, all = 0;
+  if (sh.waves > 0) {
+    if (tid < workers) {
+      Walk walk;
+      walk.enter(v, 0);
+      for (int i = 0; i < sh.waves; ++i) {
+        walk.tile(v, i * workers + tid);
+        cost += tile_units(walk.q, v, walk.j);
+      }
+    }
+    block_scan(cost, part, &all);
+  }
+  const int64_t mean = (all + rest) / workers;
+  const int64_t need = tid < workers ? max(mean - cost, (int64_t)v.tiling.start) : 0;
+  const int64_t incl = block_scan(need, part, &all);
+  if (tid < workers)
+    raw[tid] = first + (int64_t)((double)(incl - need) * ((double)rest / (double)all));
+  if (tid == 0) {
+    raw[workers] = before;
+    l.start[workers].u = before;
+  }
+  __syncthreads();
+  // The last worker whose share starts at u or before.
+  auto worker_of = [&](int64_t u) {
+    int lo = 0, hi = workers;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (raw[mid] <= u) lo = mid;
+      else hi = mid;
+    }
+    return lo;
+  };
+  const int snap = v.tiling.start + kStep;  // a share does not begin before that in a tile
+  if (tid < workers) {
+    const int w = tid;
+    const int64_t u = raw[w];
     int lo = 0, hi = (int)requests;
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
@@ -138,17 +173,19 @@ __global__ void __launch_bounds__(kScheduleThreads) schedule_kernel(const Schedu
     }
     Walk walk;
     walk.seek(v, u, lo);
-    l.start[w] = Start{walk.r, walk.g, walk.j, walk.q.start, walk.q.n, walk.q.len, walk.first};
+    const bool inside = u - walk.first >= snap;
+    l.start[w] = Start{walk.r, walk.g, walk.j, walk.q.start, walk.q.n, walk.q.len, walk.first,
+                       inside ? u : walk.first};
     Join j{0, 0, 0, 0, 0, 0};
-    if (walk.first != u) {
-      const int w0 = worker_of(walk.first, sh);
+    if (inside) {
+      const int w0 = worker_of(walk.first + snap - 1);  // whose share has the tile's first token
       const int tok0 = walk.j * v.tiling.per, toks = imin(v.tiling.per, walk.q.n - tok0);
       const bool expanded = form == 1, wide = !expanded && v.tiling.groups > 1;
       j.row = (int64_t)(walk.q.start + tok0) * v.heads +
               (expanded ? walk.g : wide ? walk.g * kRows : 0);
       j.rows = expanded ? toks : wide ? imin(kRows, v.heads - walk.g * kRows) : toks * v.heads;
-      j.parts = worker_of(walk.last - 1, sh) - w0 + 1;
-      j.slot = 2 * w0 + (walk.first == worker_first(w0, sh) ? 0 : 1);
+      j.parts = worker_of(walk.last - 1) - w0 + 1;
+      j.slot = 2 * w0 + (raw[w0] >= walk.first ? 0 : 1);
       j.worker = w0;
       j.border = w - 1 - w0;
     }
@@ -375,6 +412,7 @@ int fill(const grm_b200_latent_plan* plan, const grm_b200_latent_arena* arena, i
 }  // namespace
 
 int make_shape(const grm_b200_latent_plan& p, int sms, Shape* s) {
+  sms = std::min(sms, kMostWorkers);
   s->tiling[0] = absorbed_tiling(p.heads, p.latent, std::min(p.step.max_fresh, p.step.tokens), sms);
   s->tiling[1] = expanded_tiling(p.heads, sms);
   int64_t at = 0;
@@ -387,7 +425,7 @@ int make_shape(const grm_b200_latent_plan& p, int sms, Shape* s) {
     s->off_header[f] = take(sizeof(Header));
     s->off_base[f] = take((p.step.requests + 1) * 8);
     s->off_tile[f] = take(f > 0 ? (p.step.requests + 1) * 4 : 0);
-    s->off_start[f] = take((int64_t)s->tiling[f].workers * (int64_t)sizeof(Start));
+    s->off_start[f] = take((int64_t)(s->tiling[f].workers + 1) * (int64_t)sizeof(Start));
     s->off_join[f] = take((int64_t)s->tiling[f].workers * (int64_t)sizeof(Join));
   }
   const Tiling& t = s->tiling[0];

@@ -15,42 +15,47 @@ constexpr int kRows = 128;  // rows of a query tile
 constexpr int kExpandAlign = 64;
 
 // Both forms of attention go over tiles of query rows, each of which sees some of
-// its request's tokens, and every worker (a block, one an SM) gets the same number of
-// units: a tile costs the tokens that it sees, and kStart more for its start and
-// end.  Tiles lie one after another, a request's by group (a head of the expanded
-// form; of the absorbed one 128 heads) and then by token; a worker's share may start
-// and end inside a tile, whose parts join_kernel puts together.
+// its request's tokens, and every worker (a block, one an SM) gets work of the same
+// cost in units: a tile costs the tokens that it sees, and Tiling::start more for its
+// queries, first scores and result.  Tiles lie one after another, a request's by group (a
+// head of the expanded form; of the absorbed one 128 heads) and then by token; a worker's
+// share may start and end inside a tile, whose parts join_kernel puts together.  The units
+// of a tile's start come first, so that whoever takes some of its tokens from the
+// beginning pays them; who goes on inside a tile pays once, as nearly everybody does.  A
+// share does not begin among them, nor within a step after them: it takes the whole tile.
 //
-// kStart is what a tile's queries, result and first scores take, in tokens (64 take 0.87
-// us).  Measured, us of 64 requests of 32 to 16,384 tokens and one row, and of 16 requests
-// with 5 rows, 40 heads of 256 + 32: kStart 128 59.8 and 47, 256 57.6 and 45, 384 57.6 and
-// 43.  kLeast, the fewest units of a worker, weighs the parts that join_kernel has to read
-// against blocks that stand idle: 384, 512, 640 and 1,024 were within 2 % on those, and 640
-// the best for one request of 4,096 tokens.
-constexpr int kStart = 384;
+// A step of 64 tokens and a part of a tile take, by a fit over the blocks' times: 0.66 and
+// 5.9 us (64 requests of 32 to 16,384 tokens, one row, 40 heads of 256 + 32), 1.2 and 5.5
+// (16 of them with 5 rows), 0.97 and 6.0 expanded (8,449 rows on 31,000 tokens, 40 heads of 64
+// + 32), 2.2 and 3.6 (3,499 rows, 16 heads of 128 + 64).
+constexpr int kAbsorbedStart = 512, kExpandedStart = 320;
+// Fewest units of a worker: weighs the parts that join_kernel has to read against blocks
+// that stand idle.  384, 512, 640 and 1,024 were within 2 % on the first two of those, and
+// 640 the best for one request of 4,096 tokens.
 constexpr int kLeast = 640;
+constexpr int kMostWorkers = 1024;
+// A tile of the expanded form that has rows for one of its two query tiles takes about
+// so many eighths for a token.
+constexpr int kAlone = 5;
 
 // The expanded form's tiles are many where requests are long, and each head has keys and
 // values of its own: in equal shares one after another the workers would be at as many
 // heads as there are, whose keys and values L2 does not hold (8,449 rows of 40 heads:
 // 6.5 GB from HBM).  So all but the last one or two tiles of a worker go out whole, tile i
-// to worker i mod workers, and the rest in equal shares: 0.6 GB, in about the same time,
-// as the products are what it is bound by, but not at HBM's cost in power.
+// to worker i mod workers: 0.6 GB, in about the same time, as the softmax is what it is
+// bound by, but not at HBM's cost in power.  The rest is shared so that all have the same.
 
 struct Header {     // written by the schedule kernel, one for each form
-  int64_t first;    // unit that the shares begin with
-  int64_t share;    // units of a worker
-  int32_t more;     // workers that have one more
-  int32_t workers;  // that share them
+  int32_t workers;  // that have a share
   int32_t waves;    // tiles of each worker that go out whole
   int32_t lost;     // more tokens to expand than there is room for
 };
 
-// Where a worker starts: the tile of its first unit, and that tile's first unit.
-struct alignas(32) Start {
+// Where a worker's share starts: the tile, its first unit, and the share's.
+struct alignas(16) Start {
   int32_t r, g, j;       // request, group, tile
   int32_t from, n, len;  // the request's first packed row, rows, tokens
-  int64_t first;
+  int64_t first, u;
 };
 
 // A tile that lies in the shares of several workers, as join_kernel goes by: one for
@@ -68,7 +73,7 @@ struct Lists {
   Header* header;
   int64_t* base;  // [requests + 1] first unit of each request
   int32_t* tile;  // [requests + 1] first tile of each request (expanded form)
-  Start* start;   // [workers]
+  Start* start;   // [workers + 1]
   Join* join;     // [workers], of the border where each begins
   float* part;    // [workers * splits * 2] partial results, see slot_floats
 };
@@ -80,6 +85,7 @@ struct Tiling {
   int groups;   // tiles of the same tokens
   int splits;   // blocks that share a tile's values
   int workers;  // most
+  int start;    // units of a tile's start
   int few;      // columns of latent_few.cu's kernel, which serves the step; 0: it does not
 };
 // The absorbed form's kernel for few rows (latent_few.cu) takes requests of up to 32 rows
@@ -90,13 +96,14 @@ struct Tiling {
 __host__ __device__ inline Tiling absorbed_tiling(int heads, int latent, int64_t most_tokens,
                                                   int sms) {
   const int64_t most = most_tokens * heads;
-  if (latent == 512 && most <= 32) return {(int)most_tokens, 1, 1, sms, most <= 16 ? 16 : 32};
+  if (latent == 512 && most <= 32)
+    return {(int)most_tokens, 1, 1, sms, kAbsorbedStart, most <= 16 ? 16 : 32};
   const int splits = latent > 256 ? latent / 256 : 1;
   return {heads <= kRows ? kRows / heads : 1, heads <= kRows ? 1 : (heads + kRows - 1) / kRows,
-          splits, sms / splits, 0};
+          splits, sms / splits, kAbsorbedStart, 0};
 }
 __host__ __device__ inline Tiling expanded_tiling(int heads, int sms) {
-  return {2 * kRows, heads, 1, sms, 0};
+  return {2 * kRows, heads, 1, sms, kExpandedStart, 0};
 }
 // fp32 of a partial result: [rows][values], then [rows][4] of reference exponent, sum,
 // sum of the rounded weights.
@@ -167,36 +174,35 @@ int make_map(CUtensorMap* map, const void* base, int rank, const int64_t* dims,
 
 // ---- the shares
 
-__host__ __device__ inline int64_t worker_first(int64_t w, const Header& h) {
-  return h.first + w * h.share + (w < h.more ? w : h.more);
-}
-__host__ __device__ inline int worker_of(int64_t u, const Header& h) {
-  u -= h.first;
-  const int64_t big = h.more * (h.share + 1);
-  return (int)(u < big ? u / (h.share + 1) : h.more + (u - big) / h.share);
-}
-
 template <typename I>
 __host__ __device__ __forceinline__ I imin(I a, I b) {
   return a < b ? a : b;
 }
 
-// Units of the first j tiles of a group: tile i sees cached + (i + 1) * per tokens of
-// a causal step, but no more than len.
 struct Request {
   int start, n, len, cached, tiles;
   int64_t total;  // units of a group
 };
-__host__ __device__ __forceinline__ int64_t units_before(const Request& q, int per, int grow, int j) {
-  if (!grow) return (int64_t)j * (q.len + kStart);
-  const int64_t u = (int64_t)j * (q.cached + kStart) + (int64_t)per * j * (j + 1) / 2;
-  return j < q.tiles ? u : u - ((int64_t)q.tiles * per - q.n);
+// Units of tile j, which sees cached + (j + 1) * per tokens of a causal step, but no more
+// than len.
+__host__ __device__ __forceinline__ int64_t tile_units(const Request& q, const View& v, int j) {
+  const int per = v.tiling.per;
+  const bool last = j + 1 == q.tiles;
+  const int64_t sees = !v.grow || last ? (int64_t)q.len : q.cached + (int64_t)(j + 1) * per;
+  const bool alone = per == 2 * kRows && last && q.n - j * per <= kRows;
+  return (alone ? sees * kAlone / 8 : sees) + v.tiling.start;
 }
-__host__ __device__ __forceinline__ Request request_of(int start, int next, int len, int per, int grow) {
-  Request q{start, next - start, len, 0, 0, 0};
-  q.cached = grow ? len - q.n : len;
-  q.tiles = (q.n + per - 1) / per;
-  q.total = units_before(q, per, grow, q.tiles);
+// Of the first j tiles of a group.
+__host__ __device__ __forceinline__ int64_t units_before(const Request& q, const View& v, int j) {
+  const int full = imin(j, q.tiles - 1);
+  int64_t u = (int64_t)full * (q.cached + v.tiling.start);
+  if (v.grow) u += (int64_t)v.tiling.per * full * (full + 1) / 2;
+  return j < q.tiles ? u : u + tile_units(q, v, j - 1);
+}
+__host__ __device__ __forceinline__ Request request_of(const View& v, int r) {
+  const int start = v.starts[r], n = v.starts[r + 1] - start, len = v.lens[r];
+  Request q{start, n, len, v.grow ? len - n : len, (n + v.tiling.per - 1) / v.tiling.per, 0};
+  q.total = q.tiles > 0 ? units_before(q, v, q.tiles) : 0;
   return q;
 }
 
@@ -208,12 +214,7 @@ struct Walk {
 
   __host__ __device__ __forceinline__ void enter(const View& v, int request) {
     r = request;
-    q = request_of(v.starts[r], v.starts[r + 1], v.lens[r], v.tiling.per, v.grow);
-  }
-  __host__ __device__ __forceinline__ int64_t cost(const View& v) const {  // of the tile
-    if (!v.grow) return q.len + kStart;
-    const int64_t sees = q.cached + (int64_t)(j + 1) * v.tiling.per;
-    return (j + 1 < q.tiles ? sees : q.len) + kStart;
+    q = request_of(v, r);
   }
   __host__ __device__ __forceinline__ void seek(const View& v, int64_t u, int request) {
     enter(v, request);
@@ -223,12 +224,12 @@ struct Walk {
     int lo = 0, hi = q.tiles;  // the last tile that starts at y or before
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
-      if (units_before(q, v.tiling.per, v.grow, mid) <= y) lo = mid;
+      if (units_before(q, v, mid) <= y) lo = mid;
       else hi = mid;
     }
     j = lo;
-    first = v.base[r] + g * q.total + units_before(q, v.tiling.per, v.grow, j);
-    last = first + cost(v);
+    first = v.base[r] + g * q.total + units_before(q, v, j);
+    last = first + tile_units(q, v, j);
   }
   __host__ __device__ __forceinline__ void start(const View& v, const Start& s) {
     r = s.r;
@@ -237,7 +238,7 @@ struct Walk {
     q = Request{s.from, s.n, s.len, v.grow ? s.len - s.n : s.len,
                 (s.n + v.tiling.per - 1) / v.tiling.per, 0};
     first = s.first;
-    last = first + cost(v);
+    last = first + tile_units(q, v, j);
   }
   // The i-th of all tiles, from the request where this one is on.
   __host__ __device__ __forceinline__ void tile(const View& v, int i) {
@@ -273,7 +274,7 @@ struct Walk {
         enter(v, lo);
       }
     }
-    last = first + cost(v);
+    last = first + tile_units(q, v, j);
   }
 };
 
@@ -293,10 +294,10 @@ struct Parts {
   int64_t u, end;
   int w, whole, waves, count;
 
+  // `until`: where the next worker's share starts
   __host__ __device__ __forceinline__ Parts(const Params& p, const Header& h, int worker,
-                                            const Start& start)
-      : u(worker_first(worker, h)), end(worker_first(worker + 1, h)), w(worker), whole(0),
-        waves(h.waves), count(0) {
+                                            const Start& start, int64_t until)
+      : u(start.u), end(until), w(worker), whole(0), waves(h.waves), count(0) {
     if (QUERIES == 2 && waves > 0) walk.enter(p.v, 0);
     else walk.start(p.v, start);
   }
@@ -330,11 +331,12 @@ struct Parts {
     }
     // The step that a unit of the tile falls on.  Any rounding will do, as the workers on
     // both sides of a border round alike; a division in 64 bits is 100 instructions.
+    const int start = p.v.tiling.start;
     const int units = (int)(walk.last - walk.first), from = (int)(u - walk.first);
     const int to = (int)(imin(end, walk.last) - walk.first);
-    const float per_unit = (float)all / (float)units;
-    x->step0 = imin(all, (int)((float)from * per_unit));
-    x->steps = (to == units ? all : imin(all, (int)((float)to * per_unit))) - x->step0;
+    const float per_unit = (float)all / (float)(units - start);  // not used where that is 0
+    x->step0 = from == 0 ? 0 : imin(all, (int)((float)(from - start) * per_unit));
+    x->steps = (to == units ? all : imin(all, (int)((float)(to - start) * per_unit))) - x->step0;
     x->slot = from == 0 && to == units ? -1 : 2 * w + (count > 0 ? 1 : 0);
     u = imin(end, walk.last);
     ++count;

@@ -163,7 +163,7 @@ __device__ __noinline__ void lose_rows(const Params& p, const Header& hd, int wo
   using LY = Layout<MAIN, ROPE, EXP>;
   const float nan = __int_as_float(0x7FC00000);
   const int t = threadIdx.x >> 7, row = threadIdx.x & 127;
-  Parts<LY::kQueries> parts(p, hd, worker, p.l.start[worker]);
+  Parts<LY::kQueries> parts(p, hd, worker, p.l.start[worker], p.l.start[worker + 1].u);
   Part x;
   while (parts.next(p, &x)) {
     const Row a = row_of<EXP>(p, x, t, row);
@@ -202,7 +202,8 @@ __global__ void __launch_bounds__(Layout<MAIN, ROPE, EXP>::kThreads, 1)
   __shared__ int sh_fail;
 
   const int worker = blockIdx.x / LY::kSplits, split = blockIdx.x % LY::kSplits;
-  const Start begin = p.l.start[worker];  // on its way beside the header
+  const Start begin = p.l.start[worker];  // on their way beside the header
+  const int64_t until = p.l.start[worker + 1].u;
   const Header hd = *p.l.header;
   asm volatile("griddepcontrol.launch_dependents;");
   if (worker >= hd.workers) return;
@@ -242,7 +243,7 @@ __global__ void __launch_bounds__(Layout<MAIN, ROPE, EXP>::kThreads, 1)
   auto wait = [&](uint64_t* bar, unsigned parity) {
     return warp_wait(bar, parity, &sh_fail, p.probes);
   };
-  Parts<kQ> parts(p, hd, worker, begin);
+  Parts<kQ> parts(p, hd, worker, begin, until);
   Part x;
 
   if (warp < LY::kSoftWarps) {

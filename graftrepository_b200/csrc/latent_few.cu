@@ -179,7 +179,7 @@ __device__ __noinline__ void scrub(unsigned char* ring, unsigned place0, int t) 
 template <int LATENT, int N>
 __device__ __noinline__ void lose_rows(const Params& p, const Header& hd, int worker) {
   const float nan = __int_as_float(0x7FC00000);
-  Parts<1, kTokens> parts(p, hd, worker, p.l.start[worker]);
+  Parts<1, kTokens> parts(p, hd, worker, p.l.start[worker], p.l.start[worker + 1].u);
   Part x;
   while (parts.next(p, &x)) {
     const int rows = x.toks[0] * p.heads;
@@ -227,7 +227,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ int sh_fail;
 
   const int worker = blockIdx.x;
-  const Start begin = p.l.start[worker];  // on its way beside the header
+  const Start begin = p.l.start[worker];  // on their way beside the header
+  const int64_t until = p.l.start[worker + 1].u;
   const Header hd = *p.l.header;
   asm volatile("griddepcontrol.launch_dependents;");
   if (worker >= hd.workers) return;
@@ -264,7 +265,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto wait = [&](uint64_t* bar, unsigned parity) {
     return warp_wait(bar, parity, &sh_fail, p.probes);
   };
-  Parts<1, kTokens> parts(p, hd, worker, begin);
+  Parts<1, kTokens> parts(p, hd, worker, begin, until);
   Part x;
 
   if (warp < kSoftWarps) {
