@@ -179,63 +179,64 @@ __global__ void __launch_bounds__(256) join_kernel(const Params p) {
   const int id = (j.border * gridDim.y + blockIdx.y) * 8 + warp;
   const int of_row = id & ((1 << shift) - 1);
   const int column = of_row * width + (lane & (wide - 1));
-  const int line = id >> shift;
-  if (line >= j.rows) return;
   const float* const part = p.l.part + split * kSlot;
-  float m = -INFINITY, l = 0.0f, lr = 0.0f;
-  float4 o[kMine] = {};
-#pragma unroll 2
-  for (int k = lane / wide; k < j.parts; k += 32 / wide) {
-    const float* slot =
-        part + (int64_t)(k == 0 ? j.slot : 2 * (j.worker + k)) * (SPLITS * kSlot);
-    const float4 s = *reinterpret_cast<const float4*>(slot + ROWS * V + 4 * line);
-    float4 v[kMine];
-#pragma unroll
-    for (int i = 0; i < kMine; ++i)
-      if (32 * i < width) v[i] = (reinterpret_cast<const float4*>(slot + line * V) + column)[32 * i];
-    if (s.y == 0.0f) continue;  // a part that sees nothing
-    const float next = fmaxf(m, s.x);
-    const float a = m == next ? 1.0f : paged::ex2(m - next);
-    const float f = s.x == next ? 1.0f : paged::ex2(s.x - next);
-    m = next;
-    l = fmaf(l, a, s.y * f);
-    lr = fmaf(lr, a, s.z * f);
-#pragma unroll
-    for (int i = 0; i < kMine; ++i)
-      if (32 * i < width) {
-        o[i].x = fmaf(o[i].x, a, v[i].x * f);
-        o[i].y = fmaf(o[i].y, a, v[i].y * f);
-        o[i].z = fmaf(o[i].z, a, v[i].z * f);
-        o[i].w = fmaf(o[i].w, a, v[i].w * f);
-      }
-  }
 #pragma unroll 1
-  for (int d = wide; d < 32; d <<= 1) {  // lanes with other parts; there is one float4 then
-    const float other = __shfl_xor_sync(kFull, m, d), next = fmaxf(m, other);
-    const float f = m == next ? 1.0f : paged::ex2(m - next);
-    m = next;
-    l *= f;
-    lr *= f;
-    l += __shfl_xor_sync(kFull, l, d);
-    lr += __shfl_xor_sync(kFull, lr, d);
-    o[0] = make_float4(o[0].x * f, o[0].y * f, o[0].z * f, o[0].w * f);
-    o[0].x += __shfl_xor_sync(kFull, o[0].x, d);
-    o[0].y += __shfl_xor_sync(kFull, o[0].y, d);
-    o[0].z += __shfl_xor_sync(kFull, o[0].z, d);
-    o[0].w += __shfl_xor_sync(kFull, o[0].w, d);
-  }
-  if (lane >= wide) return;
-  const int64_t row = j.row + (int64_t)line * (EXP ? p.heads : 1);
-  const float inv = 1.0f / lr;
+  for (int line = id >> shift; line < j.rows; line += warps >> shift) {
+    float m = -INFINITY, l = 0.0f, lr = 0.0f;
+    float4 o[kMine] = {};
+#pragma unroll 2
+    for (int k = lane / wide; k < j.parts; k += 32 / wide) {
+      const float* slot =
+          part + (int64_t)(k == 0 ? j.slot : 2 * (j.worker + k)) * (SPLITS * kSlot);
+      const float4 s = *reinterpret_cast<const float4*>(slot + ROWS * V + 4 * line);
+      float4 v[kMine];
 #pragma unroll
-  for (int i = 0; i < kMine; ++i)
-    if (32 * i < width)
-      reinterpret_cast<uint2*>(p.out + row * kWide + split * V)[column + 32 * i] =
-          lr == 0.0f ? make_uint2(0, 0)
-                     : make_uint2(Kind<T>::pack(o[i].x * inv, o[i].y * inv),
-                                  Kind<T>::pack(o[i].z * inv, o[i].w * inv));
-  if (lane == 0 && of_row == 0 && split == 0 && p.lse)
-    p.lse[row] = l == 0.0f ? -INFINITY : (m - Kind<T>::kLift + log2f(l)) * 0.693147180559945309f;
+      for (int i = 0; i < kMine; ++i)
+        if (32 * i < width) v[i] = (reinterpret_cast<const float4*>(slot + line * V) + column)[32 * i];
+      if (s.y == 0.0f) continue;  // a part that sees nothing
+      const float next = fmaxf(m, s.x);
+      const float a = m == next ? 1.0f : paged::ex2(m - next);
+      const float f = s.x == next ? 1.0f : paged::ex2(s.x - next);
+      m = next;
+      l = fmaf(l, a, s.y * f);
+      lr = fmaf(lr, a, s.z * f);
+#pragma unroll
+      for (int i = 0; i < kMine; ++i)
+        if (32 * i < width) {
+          o[i].x = fmaf(o[i].x, a, v[i].x * f);
+          o[i].y = fmaf(o[i].y, a, v[i].y * f);
+          o[i].z = fmaf(o[i].z, a, v[i].z * f);
+          o[i].w = fmaf(o[i].w, a, v[i].w * f);
+        }
+    }
+#pragma unroll 1
+    for (int d = wide; d < 32; d <<= 1) {  // lanes with other parts; there is one float4 then
+      const float other = __shfl_xor_sync(kFull, m, d), next = fmaxf(m, other);
+      const float f = m == next ? 1.0f : paged::ex2(m - next);
+      m = next;
+      l *= f;
+      lr *= f;
+      l += __shfl_xor_sync(kFull, l, d);
+      lr += __shfl_xor_sync(kFull, lr, d);
+      o[0] = make_float4(o[0].x * f, o[0].y * f, o[0].z * f, o[0].w * f);
+      o[0].x += __shfl_xor_sync(kFull, o[0].x, d);
+      o[0].y += __shfl_xor_sync(kFull, o[0].y, d);
+      o[0].z += __shfl_xor_sync(kFull, o[0].z, d);
+      o[0].w += __shfl_xor_sync(kFull, o[0].w, d);
+    }
+    if (lane >= wide) continue;
+    const int64_t row = j.row + (int64_t)line * (EXP ? p.heads : 1);
+    const float inv = 1.0f / lr;
+#pragma unroll
+    for (int i = 0; i < kMine; ++i)
+      if (32 * i < width)
+        reinterpret_cast<uint2*>(p.out + row * kWide + split * V)[column + 32 * i] =
+            lr == 0.0f ? make_uint2(0, 0)
+                       : make_uint2(Kind<T>::pack(o[i].x * inv, o[i].y * inv),
+                                    Kind<T>::pack(o[i].z * inv, o[i].w * inv));
+    if (lane == 0 && of_row == 0 && split == 0 && p.lse)
+      p.lse[row] = l == 0.0f ? -INFINITY : (m - Kind<T>::kLift + log2f(l)) * 0.693147180559945309f;
+  }
 }
 
 template <typename T, int V, int SPLITS, int ROWS, bool EXP>
@@ -243,7 +244,7 @@ int launch_join(const Params& p, cudaStream_t st) {
   cudaLaunchConfig_t cfg{};
   const Tiling& t = p.v.tiling;
   const int rows = EXP ? t.per : (int)std::min((int64_t)kRows, (int64_t)t.per * p.heads);
-  cfg.gridDim = dim3((unsigned)(std::max(t.workers - 1, 1) * SPLITS), (unsigned)(rows + 7) / 8);
+  cfg.gridDim = dim3((unsigned)(std::max(t.workers - 1, 1) * SPLITS), (unsigned)(rows + 31) / 32);
   cfg.blockDim = dim3(256);
   cfg.stream = st;
   cudaLaunchAttribute attr;
