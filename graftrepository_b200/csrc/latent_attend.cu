@@ -101,7 +101,7 @@ struct Layout {
   static constexpr int kThreads = (kLoadWarp + 1) * 32;
   static constexpr int kSlot = slot_floats(kRows * kQueries, kV);
   static_assert(kQueryCol + kQueries * kQTmem / 2 <= kTmemCols && kStages >= 2, "tiles");
-  static_assert(kQTmem % 128 == 0 || kQTmem == MAIN, "queries come 128 values at a time");
+  static_assert(kQTmem % 256 == 0 || kQTmem == MAIN, "queries come 256 values at a time");
 };
 
 // fp32 accumulators, 16-bit operands, 128 rows, n columns; B K-major or (b_mn) not.
@@ -266,15 +266,20 @@ __global__ void __launch_bounds__(Layout<MAIN, ROPE, EXP>::kThreads, 1)
         return b.active ? __ldg(reinterpret_cast<const uint4*>(from) + c)
                         : make_uint4(0, 0, 0, 0);
       };
-      // sixteen loads in flight
-#pragma unroll 1
-      for (int c = 0; c < MAIN / 8; c += 16) {
-        uint4 v[16];
+      // All loads in flight (of a latent of 512 half of them): in batches of sixteen, the
+      // positional part after them, it was three trips to memory, 1.5 us more of a tile's start.
+      constexpr int kBatch = MAIN / 8 < 32 ? MAIN / 8 : 32;
+      uint4 positional[ROPE / 8];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = MAIN >= 128 || i < MAIN / 8 ? chunk(qp, c + i) : uint4{};
+      for (int c = 0; c < ROPE / 8; ++c) positional[c] = chunk(rp, c);
+#pragma unroll 1
+      for (int c = 0; c < MAIN / 8; c += kBatch) {
+        uint4 v[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) v[i] = chunk(qp, c + i);
         if (c < LY::kQTmem / 8) {
 #pragma unroll
-          for (int i = 0; i < 16 && i < MAIN / 8; i += 4) {
+          for (int i = 0; i < kBatch; i += 4) {
             const uint32_t w[16] = {v[i].x, v[i].y, v[i].z, v[i].w, v[i + 1].x, v[i + 1].y,
                                     v[i + 1].z, v[i + 1].w, v[i + 2].x, v[i + 2].y, v[i + 2].z,
                                     v[i + 2].w, v[i + 3].x, v[i + 3].y, v[i + 3].z, v[i + 3].w};
@@ -282,22 +287,17 @@ __global__ void __launch_bounds__(Layout<MAIN, ROPE, EXP>::kThreads, 1)
           }
         } else {
 #pragma unroll
-          for (int i = 0; i < 16 && i < MAIN / 8; ++i) {
+          for (int i = 0; i < kBatch; ++i) {
             const int z = c + i - LY::kQTmem / 8;
             *reinterpret_cast<uint4*>(my_q + (z / 8) * kQueryAtom + atom_byte(row, z % 8)) = v[i];
           }
         }
       }
-      {
-        uint4 v[ROPE / 8];
 #pragma unroll
-        for (int c = 0; c < ROPE / 8; ++c) v[c] = chunk(rp, c);
-#pragma unroll
-        for (int c = 0; c < ROPE / 8; ++c)
-          *reinterpret_cast<uint4*>(
-              my_q + LY::kQRopeAt +
-              (ROPE == 64 ? atom_byte(row, c) : half_atom_byte(row, c))) = v[c];
-      }
+      for (int c = 0; c < ROPE / 8; ++c)
+        *reinterpret_cast<uint4*>(my_q + LY::kQRopeAt + (ROPE == 64 ? atom_byte(row, c)
+                                                                    : half_atom_byte(row, c))) =
+            positional[c];
       tmem_wait_st();
       tc_fence_before();
       fence_proxy_async_smem();
