@@ -58,6 +58,7 @@ __global__ void __launch_bounds__(kScheduleThreads) schedule_kernel(const Schedu
   __shared__ int64_t part[33];
   __shared__ Header sh;
   __shared__ int64_t raw[kMostWorkers + 1], first;
+  __shared__ unsigned long long whole[kScheduleThreads];
   const int tid = threadIdx.x, form = blockIdx.x;
   const bool sizes = form < p.forms;  // else: room
   const Lists l = p.l[sizes ? form : 0];
@@ -130,15 +131,19 @@ __global__ void __launch_bounds__(kScheduleThreads) schedule_kernel(const Schedu
   if (workers == 0) return;
   const int64_t rest = before - first;
   int64_t cost = 0, all = 0;
-  if (sh.waves > 0) {
-    if (tid < workers) {
-      Walk walk;
-      walk.enter(v, 0);
-      for (int i = 0; i < sh.waves; ++i) {
-        walk.tile(v, i * workers + tid);
-        cost += tile_units(walk.q, v, walk.j);
-      }
+  if (sh.waves > 0) {  // a warp a request, a lane a tile; sums of integers in any order
+    whole[tid] = 0;
+    __syncthreads();
+    const int count = sh.waves * workers;
+    for (int64_t r = tid / 32; r < requests; r += kScheduleThreads / 32) {
+      const Request q = request_of(v, (int)r);
+      const int from = l.tile[r], tiles = min(q.tiles * v.tiling.groups, count - from);
+      for (int x = tid % 32; x < tiles; x += 32)
+        atomicAdd(&whole[(from + x) % workers],
+                  (unsigned long long)tile_units(q, v, x % q.tiles));
     }
+    __syncthreads();
+    cost = tid < workers ? (int64_t)whole[tid] : 0;
     block_scan(cost, part, &all);
   }
   const int64_t mean = (all + rest) / workers;

@@ -29,20 +29,19 @@
 // running ahead over their borders, and leaves parts of the tiles at its ends for
 // join_kernel.
 //
-// Absorbed, a step of 64 tokens (40 heads of 256 + 32, one row) takes 0.87 us, 6.2 TB/s of
-// all SMs: its copies and its products are about level.  64 requests of 32 to 16,384
-// tokens (147 MB, 22.5 us at a copy's rate) take 52 us: 45 in this kernel, whose tiles' starts
-// and ends lie between steps, and 5 in join_kernel.  Expanded, it is bound by the two softmax
-// warps of a scheduler: 2,075 clocks for 64 tokens of both query tiles, of which a warp's
-// exponentials, their sums and roundings take 900, in turns; loads, maxima, waits and barriers
-// lie under the other's.  8,449 rows on 31,000 tokens, 40 heads of 64 + 32, take 1.75 ms, 0.6
-// PFLOP/s (keys count once).  Half of the exponentials left out make that 8 % less, the sum of
-// the rounded weights 6 %, half of the scores' products nothing: what a step takes apart from
-// its 64 tokens counts.  Scores of 96 or 128 tokens at a time were no faster all the same (a
-// product with both operands in shared memory takes 100 clocks at 128 columns, 64 at least with
-// queries in tensor memory), nor were keys and what they left over side by side in one
-// product of 128 columns, the sum left to the softmax (2.25 ms in all, where this takes 1.95),
-// nor two threads a row (3.36 ms: 96 registers are too few).
+// Absorbed, a step of 64 tokens (40 heads of 256 + 32, one row) takes 0.66 to 0.87 us, up to
+// 8 TB/s of all SMs: its copies and its products are about level.  64 requests of 32 to 16,384
+// tokens (147 MB, 22.5 us at a copy's rate) take 42 us: 32 in this kernel's blocks, 5.5 of
+// them a tile's start and end, then 5 in join_kernel and two launches.
+// Expanded, heads of 64 + 32: 28 products for 64 tokens of both query tiles, 64 clocks each
+// at least, are 1,792 of a step's 1,845 clocks, with the softmax of one tile under the products
+// of the other; 8,449 rows on 31,000 tokens, 40 heads, take 1.5 ms, 0.7 PFLOP/s (keys count
+// once).  Before the softmax warps' places left their registers it was they, 2,075 clocks, of
+// which a warp's exponentials, their sums and roundings take 900, in turns.  Tried then, and no
+// faster: scores of 96 or 128 tokens at a time (a product with both operands in shared memory
+// takes 100 clocks at 128 columns), keys and what they left over side by side in one product of
+// 128 columns, the sum left to the softmax (2.25 ms in all against 1.95), two threads a row
+// (3.36 ms: 96 registers are too few).
 //
 // Tokens that a row does not see have weight 0, and a product of 0 and what is no
 // number would be none: where a hidden token's score is not finite, the numbers of

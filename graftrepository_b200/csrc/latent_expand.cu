@@ -13,10 +13,10 @@
 // one group of four warps and the next by the other: what holds a group up is the
 // chain of conversion, barriers and copies.
 //
-// HBM's writes are the floor: 6 bytes for a token, head and value a head has of either
-// kind (476 MB, 73 us, for 31,000 tokens of 40 heads of 32 + 32).  What holds it up is the
-// conversion: 210 us there with one group of four warps and two buffers, 156 us with two
-// groups and four.
+// Bound by HBM's writes: 6 bytes for a token, head and value a head has of either kind, 476
+// MB for 31,000 tokens of 40 heads of 64 + 64.  A fill of as many takes 124 us, this 156
+// (210 with one group of four warps and two buffers; results 128 bytes of a row at a time,
+// or two places of them a group, changed nothing).
 #include <algorithm>
 
 #include "latent_device.cuh"
