@@ -28,14 +28,15 @@ constexpr int kExpandAlign = 64;
 // 5.9 us (64 requests of 32 to 16,384 tokens, one row, 40 heads of 256 + 32), 1.2 and 5.5
 // (16 of them with 5 rows), 0.97 and 6.0 expanded (8,449 rows on 31,000 tokens, 40 heads of 64
 // + 32), 2.2 and 3.6 (3,499 rows, 16 heads of 128 + 64).
-constexpr int kAbsorbedStart = 512, kExpandedStart = 320;
+// Both sides, us of those four: absorbed 448 46.2 and 33.6, 512 45.3 and 33.7, 640 45.4 and
+// 35.0; expanded 192 1,698 and 123.5, 256 1,697 and 117.0, 320 1,699 and 119.1.
+constexpr int kAbsorbedStart = 512, kExpandedStart = 256;
 // Fewest units of a worker: weighs the parts that join_kernel has to read against blocks
-// that stand idle.  384, 512, 640 and 1,024 were within 2 % on the first two of those, and
-// 640 the best for one request of 4,096 tokens.
+// that stand idle (with 1,024 the 16 requests of 5 rows take 39.0 us, with 640 33.4).
 constexpr int kLeast = 640;
 constexpr int kMostWorkers = 1024;
 // A tile of the expanded form that has rows for one of its two query tiles takes about
-// so many eighths for a token.
+// so many eighths for a token (6: the same times within 0.5 %).
 constexpr int kAlone = 5;
 
 // The expanded form's tiles are many where requests are long, and each head has keys and
