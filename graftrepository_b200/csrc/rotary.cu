@@ -14,7 +14,7 @@
 //
 // 8,449 bf16 rows of 32 heads of 128 (138 MB, 21.2 us at a copy's rate) take 25.0 us, 5.5
 // TB/s; 33 with a block's angles shared behind a barrier, 41 with a thread's own.  2,047 fp32
-// rows of 8 heads of 128, half of each rotated (17 MB, 2.6 us), take 8.4 and 61 bf16 rows of
+// rows of 8 heads of 128, half of each rotated (17 MB, 2.6 us), take 6.3 and 61 bf16 rows of
 // 40 heads of 96 take 4.4: a launch, a token's angles and one trip to memory.
 #include <algorithm>
 
@@ -212,10 +212,11 @@ extern "C" int grm_b200_rotate(const grm_b200_rotary* rotary, const void* x_devi
   const int v = wide ? 8 : 1;
   p.entries = p.r.dim / 2 / v + (p.copy ? (p.head_dim - p.r.dim) / v : 0);
   p.lanes = std::max(32 / p.entries, 1);
-  // a token's heads by several warps where that is what it takes to give every SM
-  // sixteen
+  // A token's heads by several warps where that is what it takes to give every SM twelve
+  // (2,047 rows of 32 x 128, 40 x 96 and fp32 8 x 128: 5.8, 9.5 and 5.4 us; with sixteen, a
+  // wave and a half, 6.7, 10.6 and 6.5; with eight 400 to 1,600 rows take up to a fifth more).
   p.splits = (int)std::max<int64_t>(
-      1, std::min<int64_t>(ceil_div64(heads, p.lanes), ceil_div64(16 * info.sms, tokens)));
+      1, std::min<int64_t>(ceil_div64(heads, p.lanes), ceil_div64(12 * info.sms, tokens)));
   const int64_t warps = tokens * p.splits;
   p.warps = std::min(8, kSharedAngles / (p.r.dim / 2));
   const int64_t blocks = ceil_div64(warps, p.warps);
