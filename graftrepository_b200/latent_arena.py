@@ -43,6 +43,7 @@ import torch
 from . import _lib
 from .paged_arena import (_Buffers, _TYPES, PagePlan, PageTables, _PlanC, _call, _check_page,
                           _device, _handle, _result)
+from .rotary import _first, _last
 
 __all__ = ["LATENTS", "ROPES", "EXPANDED", "LatentPlan", "LatentArena"]
 
@@ -181,13 +182,16 @@ class LatentArena(_Buffers):
             raise ValueError(f"layer {layer} of {self.layers}")
         return self._refs[layer]
 
-    def _result(self, name, t, pattern, stream):
+    def _result(self, name, t, pattern, stream, *queries):
         if t is None:
             return _result(pattern, stream)
         if (t.shape != pattern.shape or t.dtype is not pattern.dtype or
                 t.get_device() != self._index or not t.is_contiguous()):
             raise ValueError(f"{name} must be contiguous {pattern.dtype} {list(pattern.shape)} on "
                              f"{self.device}")
+        # other blocks may still read the queries of rows whose result is there
+        if any(_first(t) < _last(q) and _first(q) < _last(t) for q in queries):
+            raise ValueError(f"{name} overlaps the queries")
         return t
 
     def append(self, plan: LatentPlan, latent, rope, *, layer: int = 0, rotary=None,
@@ -223,15 +227,16 @@ class LatentArena(_Buffers):
         [tokens, heads, rope] over everything the row's request holds, or with
         `causal` over the positions up to the row's own.  `scale` (positive)
         multiplies the scores: for heads of nope + rope values usually (nope + rope)
-        ** -0.5.  Returns (out [tokens, heads, latent], lse fp32 [tokens, heads]);
-        rows that see nothing are 0 with lse -inf."""
+        ** -0.5.  Returns (out [tokens, heads, latent], lse fp32 [tokens, heads]), new
+        ones or those given, which may not overlap the queries; rows that see nothing
+        are 0 with lse -inf."""
         ref = self._ready(plan, layer)
         wide, narrow = plan.query_shapes
         c_ptr, c_row, c_head = self._rows("q_latent", q_latent, wide)
         r_ptr, r_row, r_head = self._rows("q_rope", q_rope, narrow)
         causal = self._causal(plan, causal)
-        out = self._result("out", out, plan._out_like, stream)
-        lse = self._result("lse", lse, plan._lse_like, stream)
+        out = self._result("out", out, plan._out_like, stream, q_latent, q_rope)
+        lse = self._result("lse", lse, plan._lse_like, stream, q_latent, q_rope)
         _call(self._attend, self._index, plan._step_ref, ref, c_ptr, c_row, c_head, r_ptr, r_row,
               r_head, float(scale), causal, out.data_ptr(), lse.data_ptr(),
               _handle(stream, self._index, (self, plan), q_latent, q_rope, out, lse))
@@ -254,8 +259,8 @@ class LatentArena(_Buffers):
         q_ptr, q_row, q_head = self._rows("q", q, plan.query_shape)
         w_ptr, w_head, w_row = self._rows("weights", weights, plan.weight_shape)
         causal = self._causal(plan, causal)
-        out = self._result("out", out, plan._expanded_like, stream)
-        lse = self._result("lse", lse, plan._lse_like, stream)
+        out = self._result("out", out, plan._expanded_like, stream, q)
+        lse = self._result("lse", lse, plan._lse_like, stream, q)
         _call(self._attend_expanded, self._index, plan._step_ref, ref, q_ptr, q_row, q_head,
               w_ptr, w_head, w_row, float(scale), causal, out.data_ptr(), lse.data_ptr(),
               _handle(stream, self._index, (self, plan), q, weights, out, lse))

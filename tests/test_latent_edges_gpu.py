@@ -123,3 +123,17 @@ def test_two_graphs_of_one_plan_and_of_two():
         close(made[0][1], turn.want(True))
         close(made[1][1], turn.want(True, True))
         assert all(torch.equal(a, b) for a, b in zip(made[0][1], made[2][1]))
+
+
+def test_results_over_the_queries_are_refused():
+    turn = Turn([700], [2], 16, 256, 32, nope=64)
+    with pytest.raises(ValueError, match="overlaps"):
+        turn.attend(out=turn.q_latent)
+    both = torch.zeros((3, 16, 256), dtype=BF, device=DEV)
+    with pytest.raises(ValueError, match="overlaps"):
+        turn.arena.attend(turn.plan, both[:2], turn.q_rope, scale=0.1, out=both[1:])
+    turn.q = torch.zeros(2 * 16 * 96 + 64, dtype=BF, device=DEV)
+    over = turn.q[1024:1024 + 2 * 16 * 64].view(2, 16, 64)
+    turn.q = turn.q[:2 * 16 * 96].view(2, 16, 96)
+    with pytest.raises(ValueError, match="overlaps"):
+        turn.expanded(out=over)
