@@ -146,8 +146,17 @@ __global__ void __launch_bounds__(kScheduleThreads) schedule_kernel(const Schedu
     cost = tid < workers ? (int64_t)whole[tid] : 0;
     block_scan(cost, part, &all);
   }
-  const int64_t mean = (all + rest) / workers;
-  const int64_t need = tid < workers ? max(mean - cost, (int64_t)v.tiling.start) : 0;
+  const int start = v.tiling.start;
+  int64_t level = share_level(rest, all, workers, workers, start);
+  for (int active = workers;;) {  // once more at the most where whole tiles cost much the same
+    const bool mine = tid < workers && level - cost >= start;
+    const int left = __syncthreads_count(mine);
+    if (left == active) break;
+    active = left;
+    block_scan(mine ? cost : 0, part, &all);
+    level = share_level(rest, all, workers, active, start);
+  }
+  const int64_t need = tid < workers ? max(level - cost, (int64_t)start) : 0;
   const int64_t incl = block_scan(need, part, &all);
   if (tid < workers)
     raw[tid] = first + (int64_t)((double)(incl - need) * ((double)rest / (double)all));
@@ -156,46 +165,7 @@ __global__ void __launch_bounds__(kScheduleThreads) schedule_kernel(const Schedu
     l.start[workers].u = before;
   }
   __syncthreads();
-  // The last worker whose share starts at u or before.
-  auto worker_of = [&](int64_t u) {
-    int lo = 0, hi = workers;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (raw[mid] <= u) lo = mid;
-      else hi = mid;
-    }
-    return lo;
-  };
-  const int snap = v.tiling.start + kStep;  // a share does not begin before that in a tile
-  if (tid < workers) {
-    const int w = tid;
-    const int64_t u = raw[w];
-    int lo = 0, hi = (int)requests;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (l.base[mid] <= u) lo = mid;
-      else hi = mid;
-    }
-    Walk walk;
-    walk.seek(v, u, lo);
-    const bool inside = u - walk.first >= snap;
-    l.start[w] = Start{walk.r, walk.g, walk.j, walk.q.start, walk.q.n, walk.q.len, walk.first,
-                       inside ? u : walk.first};
-    Join j{0, 0, 0, 0, 0, 0};
-    if (inside) {
-      const int w0 = worker_of(walk.first + snap - 1);  // whose share has the tile's first token
-      const int tok0 = walk.j * v.tiling.per, toks = imin(v.tiling.per, walk.q.n - tok0);
-      const bool expanded = form == 1, wide = !expanded && v.tiling.groups > 1;
-      j.row = (int64_t)(walk.q.start + tok0) * v.heads +
-              (expanded ? walk.g : wide ? walk.g * kRows : 0);
-      j.rows = expanded ? toks : wide ? imin(kRows, v.heads - walk.g * kRows) : toks * v.heads;
-      j.parts = worker_of(walk.last - 1) - w0 + 1;
-      j.slot = 2 * w0 + (raw[w0] >= walk.first ? 0 : 1);
-      j.worker = w0;
-      j.border = w - 1 - w0;
-    }
-    l.join[w] = j;
-  }
+  if (tid < workers) place_share(v, raw, workers, tid, form == 1, &l.start[tid], &l.join[tid]);
 }
 
 struct AppendParams {

@@ -279,6 +279,66 @@ struct Walk {
   }
 };
 
+// What whole tiles and share of a worker come to together: the same for all, but that a
+// share is a tile's start at the least, which is what workers get whose whole tiles cost
+// more than that leaves room for.  `active` workers, whose whole tiles cost `cost`, are not
+// among those.  Found by taking out, from all on, those that the level leaves less, until
+// there are none: it falls from step to step, and somebody is left, as the rest of the
+// tiles is as many as there are workers, each a start or more.  No share is empty then,
+// which join_kernel counts on: a worker that has a border inside a tile leaves a part.
+// (Needs that were cut to fit instead left shares of no unit where whole tiles cost very
+// different amounts: 64 heads of requests of 300, 10^6, 300, 300 and 300 tokens.)
+__host__ __device__ __forceinline__ int64_t share_level(int64_t rest, int64_t cost, int workers,
+                                                        int active, int start) {
+  return (rest - (int64_t)(workers - active) * start + cost) / active;
+}
+
+// The worker whose share has unit u, the last one that starts there or before.
+__host__ __device__ __forceinline__ int worker_of(const int64_t* raw, int workers, int64_t u) {
+  int lo = 0, hi = workers;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (raw[mid] <= u) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+// Where the share of worker w starts, which gets the units from raw[w] on, and the tile
+// that it shares with the one before.
+__host__ __device__ __forceinline__ void place_share(const View& v, const int64_t* raw,
+                                                     int workers, int w, bool expanded,
+                                                     Start* start, Join* join) {
+  const int snap = v.tiling.start + kStep;  // a share does not begin before that in a tile
+  const int64_t u = raw[w];
+  int lo = 0, hi = (int)v.requests;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (v.base[mid] <= u) lo = mid;
+    else hi = mid;
+  }
+  Walk walk;
+  walk.seek(v, u, lo);
+  const bool inside = u - walk.first >= snap;
+  *start = Start{walk.r, walk.g, walk.j, walk.q.start, walk.q.n, walk.q.len, walk.first,
+                 inside ? u : walk.first};
+  Join j{0, 0, 0, 0, 0, 0};
+  if (inside) {
+    // whose share has the tile's first token
+    const int w0 = worker_of(raw, workers, walk.first + snap - 1);
+    const int tok0 = walk.j * v.tiling.per, toks = imin(v.tiling.per, walk.q.n - tok0);
+    const bool wide = !expanded && v.tiling.groups > 1;
+    j.row = (int64_t)(walk.q.start + tok0) * v.heads +
+            (expanded ? walk.g : wide ? walk.g * kRows : 0);
+    j.rows = expanded ? toks : wide ? imin(kRows, v.heads - walk.g * kRows) : toks * v.heads;
+    j.parts = worker_of(raw, workers, walk.last - 1) - w0 + 1;
+    j.slot = 2 * w0 + (raw[w0] >= walk.first ? 0 : 1);
+    j.worker = w0;
+    j.border = w - 1 - w0;
+  }
+  *join = j;
+}
+
 // A worker's part of a tile.
 struct Part {
   int r, g, tok0;       // request, group, first token of the tile within the step
