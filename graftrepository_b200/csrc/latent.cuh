@@ -107,7 +107,12 @@ __host__ __device__ inline Tiling expanded_tiling(int heads, int sms) {
   return {2 * kRows, heads, 1, sms, kExpandedStart, 0};
 }
 // fp32 of a partial result: [rows][values], then [rows][4] of reference exponent, sum,
-// sum of the rounded weights.
+// sum of the rounded weights, and what there is of the row:
+constexpr float kNoResult = 0.0f;    // the part has no steps, and left no values
+constexpr float kSeesNothing = 1.0f;  // the row sees none of the part's tokens
+constexpr float kSees = 2.0f;
+// A row that sees tokens has a sum, but where all of their scores are -inf: that one is
+// NaN, as 0 / 0 is, and its log-sum -inf.
 __host__ __device__ constexpr int slot_floats(int rows, int values) { return rows * (values + 4); }
 
 // Byte offsets in the work area, which follow from the plan's sizes alone.

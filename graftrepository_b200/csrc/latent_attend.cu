@@ -170,7 +170,7 @@ __device__ __noinline__ void lose_rows(const Params& p, const Header& hd, int wo
     if (x.slot >= 0) {
       float* slot = p.l.part + ((int64_t)x.slot * LY::kSplits + split) * LY::kSlot;
       *reinterpret_cast<float4*>(slot + kRows * LY::kQueries * LY::kV + 4 * (t * kRows + row)) =
-          make_float4(-INFINITY, nan, nan, 0.0f);
+          make_float4(-INFINITY, nan, nan, kSees);
     } else if (a.active) {
       const int64_t orow = (int64_t)(x.start + a.token) * p.heads + a.head;
       for (int c = 0; c < LY::kV / 8; ++c)
@@ -327,7 +327,7 @@ __global__ void __launch_bounds__(Layout<MAIN, ROPE, EXP>::kThreads, 1)
     };
     bool more = advance(), held = false;  // held: a tile whose result is to go out
     Row a{0, 0, false};
-    bool idle = false;
+    bool idle = false, sees = false;  // sees: any of the part's tokens
     int steps = 0;
     float m = 0.0f, l = 0.0f, lr = 0.0f;
 #pragma unroll 1
@@ -360,9 +360,9 @@ __global__ void __launch_bounds__(Layout<MAIN, ROPE, EXP>::kThreads, 1)
             }
           if (a.active)
             *reinterpret_cast<float4*>(slot + kRows * kQ * LY::kV + 4 * (t * kRows + row)) =
-                make_float4(m, l, lr, 0.0f);
+                make_float4(m, l, lr, steps == 0 ? kNoResult : sees ? kSees : kSeesNothing);
         } else if (!idle) {
-          const float inv = lr == 0.0f ? 0.0f : 1.0f / lr;
+          const float inv = lr == 0.0f ? __int_as_float(0x7FC00000) : 1.0f / lr;
           uint16_t* out = p.out + orow * MAIN + split * LY::kV;
 #pragma unroll 1
           for (int c = 0; c < LY::kV / 32; ++c) {
@@ -377,9 +377,9 @@ __global__ void __launch_bounds__(Layout<MAIN, ROPE, EXP>::kThreads, 1)
                 uint32_t w[4];
 #pragma unroll
                 for (int y = 0; y < 4; ++y)
-                  w[y] = lr == 0.0f ? 0u
-                                    : Kind<T>::pack(__uint_as_float(o[8 * k + 2 * y]) * inv,
-                                                    __uint_as_float(o[8 * k + 2 * y + 1]) * inv);
+                  w[y] = sees ? Kind<T>::pack(__uint_as_float(o[8 * k + 2 * y]) * inv,
+                                              __uint_as_float(o[8 * k + 2 * y + 1]) * inv)
+                              : 0u;
                 reinterpret_cast<uint4*>(out)[4 * c + k] = make_uint4(w[0], w[1], w[2], w[3]);
               }
           }
@@ -402,7 +402,8 @@ __global__ void __launch_bounds__(Layout<MAIN, ROPE, EXP>::kThreads, 1)
       m = -INFINITY;
       l = lr = 0.0f;
       // tokens that the row sees, from the part's first on
-      const int lim = (p.causal ? min(x.len, x.cached + a.token + 1) : x.len) - x.step0 * kStep;
+      const int lim = seen_by(p, x, a.token) - x.step0 * kStep;
+      sees = lim > 0;
       idle = !__any_sync(kFull, a.active);
 #pragma unroll 1
       for (int i = 0; i < steps; ++i, ++it) {

@@ -125,6 +125,10 @@ struct Row {
   int token, head;
   bool active;
 };
+// Tokens of its request that a row sees: the first so many.
+__device__ __forceinline__ int seen_by(const Params& p, const Part& x, int token) {
+  return p.causal ? min(x.len, x.cached + token + 1) : x.len;
+}
 template <bool EXP>
 __device__ __forceinline__ Row row_of(const Params& p, const Part& x, int t, int row) {
   if (EXP) return {x.tok0 + t * kRows + row, x.g, row < x.toks[t]};
@@ -183,6 +187,7 @@ __global__ void __launch_bounds__(256) join_kernel(const Params p) {
 #pragma unroll 1
   for (int line = id >> shift; line < j.rows; line += warps >> shift) {
     float m = -INFINITY, l = 0.0f, lr = 0.0f;
+    bool sees = false;
     float4 o[kMine] = {};
 #pragma unroll 2
     for (int k = lane / wide; k < j.parts; k += 32 / wide) {
@@ -193,7 +198,8 @@ __global__ void __launch_bounds__(256) join_kernel(const Params p) {
 #pragma unroll
       for (int i = 0; i < kMine; ++i)
         if (32 * i < width) v[i] = (reinterpret_cast<const float4*>(slot + line * V) + column)[32 * i];
-      if (s.y == 0.0f) continue;  // a part that sees nothing
+      if (s.w == kNoResult) continue;
+      sees |= s.w == kSees;
       const float next = fmaxf(m, s.x);
       const float a = m == next ? 1.0f : paged::ex2(m - next);
       const float f = s.x == next ? 1.0f : paged::ex2(s.x - next);
@@ -224,16 +230,17 @@ __global__ void __launch_bounds__(256) join_kernel(const Params p) {
       o[0].z += __shfl_xor_sync(kFull, o[0].z, d);
       o[0].w += __shfl_xor_sync(kFull, o[0].w, d);
     }
+    sees = __any_sync(kFull, sees);
     if (lane >= wide) continue;
     const int64_t row = j.row + (int64_t)line * (EXP ? p.heads : 1);
-    const float inv = 1.0f / lr;
+    const float inv = lr == 0.0f ? __int_as_float(0x7FC00000) : 1.0f / lr;
 #pragma unroll
     for (int i = 0; i < kMine; ++i)
       if (32 * i < width)
         reinterpret_cast<uint2*>(p.out + row * kWide + split * V)[column + 32 * i] =
-            lr == 0.0f ? make_uint2(0, 0)
-                       : make_uint2(Kind<T>::pack(o[i].x * inv, o[i].y * inv),
-                                    Kind<T>::pack(o[i].z * inv, o[i].w * inv));
+            sees ? make_uint2(Kind<T>::pack(o[i].x * inv, o[i].y * inv),
+                              Kind<T>::pack(o[i].z * inv, o[i].w * inv))
+                 : make_uint2(0, 0);
     if (lane == 0 && of_row == 0 && split == 0 && p.lse)
       p.lse[row] = l == 0.0f ? -INFINITY : (m - Kind<T>::kLift + log2f(l)) * 0.693147180559945309f;
   }

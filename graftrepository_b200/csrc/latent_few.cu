@@ -49,6 +49,9 @@ constexpr uint32_t kTmemCols = 512;
 constexpr int kSoftWarps = 8, kOutWarps = 4, kMmaWarp = 12;  // and one that loads
 constexpr int kSoftThreads = kSoftWarps * 32;
 constexpr int kThreads = 14 * 32;
+// What is added to the scores of a row that has no reference exponent yet: far above what
+// one may be passed by for every finite score, and -inf for a score of -inf.
+constexpr float kNoReference = 3.402823466e38f;
 
 template <int LATENT, int ROPE, int N>
 struct Layout {
@@ -188,7 +191,7 @@ __device__ __noinline__ void lose_rows(const Params& p, const Header& hd, int wo
       if (x.slot >= 0) {
         float* slot = p.l.part + (int64_t)x.slot * slot_floats(N, LATENT);
         *reinterpret_cast<float4*>(slot + N * LATENT + 4 * n) =
-            make_float4(-INFINITY, nan, nan, 0.0f);
+            make_float4(-INFINITY, nan, nan, kSees);
       } else {
         for (int c = 0; c < LATENT / 8; ++c)
           reinterpret_cast<uint4*>(p.out + (row0 + n) * LATENT)[c] =
@@ -289,7 +292,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (soft_any(!ok)) { ok = false; break; }
       if (tid < N) {
         ref[ob][tid] = -INFINITY;
-        off[tid] = INFINITY;
+        off[tid] = kNoReference;
       }
       soft_sync();
       float l[kMine], lr[kMine];
@@ -355,7 +358,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const float next = m > old + kLazy ? reference_of(m) : old;
             factor[tid] = next == old ? 1.0f : ex2(old - next);
             ref[ob][tid] = next;
-            off[tid] = next == -INFINITY ? INFINITY : Kind<T>::kLift - next;
+            off[tid] = next == -INFINITY ? kNoReference : Kind<T>::kLift - next;
           }
           soft_sync();
           exponents();
@@ -508,10 +511,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             lr += sums[ob][w][1][tid];
           }
         }
-        inverse[tid] = lr == 0.0f ? 0.0f : 1.0f / lr;
+        // any of the part's tokens
+        const bool sees = seen_by(p, x, x.tok0 + tid / p.heads) > x.step0 * kTokens;
+        inverse[tid] = !sees ? 0.0f : lr == 0.0f ? __int_as_float(0x7FC00000) : 1.0f / lr;
         if (tid < rows) {
           if (x.slot >= 0)
-            *reinterpret_cast<float4*>(slot + N * LATENT + 4 * tid) = make_float4(m, l, lr, 0.0f);
+            *reinterpret_cast<float4*>(slot + N * LATENT + 4 * tid) =
+                make_float4(m, l, lr, x.steps == 0 ? kNoResult : sees ? kSees : kSeesNothing);
           else if (p.lse)
             p.lse[row0 + tid] =
                 l == 0.0f ? -INFINITY : (m - Kind<T>::kLift + log2f(l)) * 0.693147180559945309f;

@@ -229,7 +229,8 @@ class LatentArena(_Buffers):
         multiplies the scores: for heads of nope + rope values usually (nope + rope)
         ** -0.5.  Returns (out [tokens, heads, latent], lse fp32 [tokens, heads]), new
         ones or those given, which may not overlap the queries; rows that see nothing
-        are 0 with lse -inf."""
+        are 0 with lse -inf.  A visible score of NaN or +inf makes its row NaN; one of
+        -inf weighs nothing, and a row that has no other is NaN with lse -inf."""
         ref = self._ready(plan, layer)
         wide, narrow = plan.query_shapes
         c_ptr, c_row, c_head = self._rows("q_latent", q_latent, wide)
