@@ -46,8 +46,10 @@
 // Tokens that a row does not see have weight 0, and a product of 0 and what is no
 // number would be none: where a hidden token's score is not finite, the numbers of
 // its values that are not are set to 0 in shared memory before the weights go out
-// (scrub).
+// (scrub).  Rows of the tile that do see the token are told: a score of -inf has weight
+// 0, and 0 times what was there is no number.
 #include <algorithm>
+#include <climits>
 #include <type_traits>
 
 #include "latent_device.cuh"
@@ -66,6 +68,7 @@ constexpr int kAtom = kStep * 128;       // 64 tokens x 64 values
 constexpr int kQueryAtom = kRows * 128;  // 128 rows x 64 values
 constexpr uint32_t kTmemCols = 512;
 constexpr int kShared = 232448 - 1024;   // dynamic shared memory beside the barriers
+constexpr float kBlind = -3.402823466e38f;
 
 template <int MAIN, int ROPE, bool EXP>
 struct Layout {
@@ -135,9 +138,11 @@ __device__ __forceinline__ unsigned long long hide(uint32_t scores, int seen) {
   return bad;
 }
 
-// Numbers that are none among the V values of token `t` of a stage set to 0.
+// Numbers that are none among the V values of some tokens of a stage set to 0; returns
+// the first token that had one (kStep: none).
 template <typename T, int V>
-__device__ __noinline__ void scrub(unsigned char* values, unsigned long long tokens) {
+__device__ __noinline__ int scrub(unsigned char* values, unsigned long long tokens) {
+  int first = kStep;
   while (tokens) {
     const int t = __ffsll((long long)tokens) - 1;
     tokens &= tokens - 1;
@@ -152,9 +157,13 @@ __device__ __noinline__ void scrub(unsigned char* values, unsigned long long tok
         if ((x[i] & e) == e) { x[i] &= 0xFFFF0000u; bad = true; }
         if ((x[i] >> 16 & e) == e) { x[i] &= 0x0000FFFFu; bad = true; }
       }
-      if (bad) *at = make_uint4(x[0], x[1], x[2], x[3]);
+      if (bad) {
+        *at = make_uint4(x[0], x[1], x[2], x[3]);
+        first = min(first, t);
+      }
     }
   }
+  return first;
 }
 
 // The rows of a worker in which a wait gave up: no numbers.
@@ -210,6 +219,9 @@ __global__ void __launch_bounds__(Layout<MAIN, ROPE, EXP>::kThreads, 1)
   constexpr int kPlace = EXP ? (sizeof(Place) + 15) / 16 * 16 : 16;
   static_assert(!EXP || kPlace * LY::kSoftWarps <= LY::kWalks, "places");
   __shared__ __align__(16) unsigned char sh_place[LY::kSoftWarps][kPlace];
+  // First token of which each softmax warp took numbers out, in this tile and the one before.
+  // (Expanded, a token whose values are none has no score either.)
+  __shared__ int sh_scrubbed[2][4];
 
   const int worker = blockIdx.x / LY::kSplits, split = blockIdx.x % LY::kSplits;
   const Start begin = p.l.start[worker];  // on their way beside the header
@@ -327,7 +339,7 @@ __global__ void __launch_bounds__(Layout<MAIN, ROPE, EXP>::kThreads, 1)
     };
     bool more = advance(), held = false;  // held: a tile whose result is to go out
     Row a{0, 0, false};
-    bool idle = false, sees = false;  // sees: any of the part's tokens
+    bool idle = false;
     int steps = 0;
     float m = 0.0f, l = 0.0f, lr = 0.0f;
 #pragma unroll 1
@@ -342,6 +354,12 @@ __global__ void __launch_bounds__(Layout<MAIN, ROPE, EXP>::kThreads, 1)
           ++tile;
         }
         const int64_t orow = (int64_t)(x.start + a.token) * p.heads + a.head;
+        if (!EXP && steps > 0) {  // (tile was counted above)
+          const int* first = sh_scrubbed[(tile - 1) & 1];
+          if (seen_by(p, x, a.token) > min(min(first[0], first[1]), min(first[2], first[3])))
+            lr = __int_as_float(0x7FC00000);  // the row sees what is no number
+        }
+        const bool sees = m != kBlind || lr != 0.0f;
         if (x.slot >= 0) {  // a part's result, for join_kernel
           float* slot = p.l.part + ((int64_t)x.slot * LY::kSplits + split) * LY::kSlot;
           float4* to = reinterpret_cast<float4*>(slot + (t * kRows + row) * LY::kV);
@@ -399,12 +417,17 @@ __global__ void __launch_bounds__(Layout<MAIN, ROPE, EXP>::kThreads, 1)
       if (!held || steps == 0) more = advance();
       if (!held) continue;
       a = row_of<EXP>(p, x, t, row);
-      m = -INFINITY;
-      l = lr = 0.0f;
       // tokens that the row sees, from the part's first on
       const int lim = seen_by(p, x, a.token) - x.step0 * kStep;
-      sees = lim > 0;
+      // A row that sees none of the part's tokens keeps a reference exponent that says so (a
+      // flag costs the expanded form's loop a register, 1 % of its time).
+      m = lim > 0 ? -INFINITY : kBlind;
+      l = lr = 0.0f;
       idle = !__any_sync(kFull, a.active);
+      if (!EXP && steps > 0) {
+        if (lane == 0) sh_scrubbed[tile & 1][warp] = INT_MAX;
+        __syncwarp();
+      }
 #pragma unroll 1
       for (int i = 0; i < steps; ++i, ++it) {
         const int buf = it & 1;
@@ -435,9 +458,11 @@ __global__ void __launch_bounds__(Layout<MAIN, ROPE, EXP>::kThreads, 1)
           if (__any_sync(kFull, bad != 0)) {
             const int st = stage_base + i;  // its copies landed before the scores were there
             if (!(ok = wait(&full[st % kStages], (st / kStages) & 1))) break;
-            scrub<T, LY::kV>(sm_stage + st % kStages * LY::kStage + LY::kValueAt +
-                                 split * (LY::kV / 64) * kAtom,
-                             bad);
+            const int first = scrub<T, LY::kV>(sm_stage + st % kStages * LY::kStage +
+                                                   LY::kValueAt + split * (LY::kV / 64) * kAtom,
+                                               bad);
+            if (!EXP && first < kStep)
+              atomicMin(&sh_scrubbed[tile & 1][warp], (x.step0 + i) * kStep + first);
             fence_proxy_async_smem();
           }
         }

@@ -28,6 +28,7 @@
 //         next tokens' scores start on what has come while the weights of these are
 //         worked out, and a place is free when the values in it have been added up
 #include <algorithm>
+#include <climits>
 
 #include "latent_device.cuh"
 
@@ -159,9 +160,11 @@ __device__ __forceinline__ float warp_max(float v) {
   return m;
 }
 
-// Values of row `t` of a step's places that are no numbers, set to 0.
+// Values of row `t` of a step's places that are no numbers, set to 0; whether there were
+// any.
 template <typename T, int PAIRS, int RING>
-__device__ __noinline__ void scrub(unsigned char* ring, unsigned place0, int t) {
+__device__ __noinline__ bool scrub(unsigned char* ring, unsigned place0, int t) {
+  bool any = false;
   for (int c = 0; c < PAIRS * 16; ++c) {
     unsigned char* place = ring + (place0 + c / 16) % RING * kPlace;
     uint4* at = reinterpret_cast<uint4*>(place + c / 8 % 2 * kAtom + atom_byte(t, c % 8));
@@ -175,7 +178,9 @@ __device__ __noinline__ void scrub(unsigned char* ring, unsigned place0, int t) 
       if ((x[i] >> 16 & e) == e) { x[i] &= 0x0000FFFFu; bad = true; }
     }
     if (bad) *at = make_uint4(x[0], x[1], x[2], x[3]);
+    any |= bad;
   }
+  return any;
 }
 
 // The rows of a worker in which a wait gave up: no numbers.
@@ -226,6 +231,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ float top[4][N];
   __shared__ float sums[2][4][2][N];            // of weights, and of the rounded ones
   __shared__ float inverse[N];
+  __shared__ int scrubbed[2];  // first token of two tiles of which numbers were taken out
   __shared__ uint32_t sh_tmem;
   __shared__ int sh_fail;
 
@@ -293,6 +299,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (tid < N) {
         ref[ob][tid] = -INFINITY;
         off[tid] = kNoReference;
+        if (tid == 0) scrubbed[ob] = INT_MAX;
       }
       soft_sync();
       float l[kMine], lr[kMine];
@@ -413,7 +420,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             const unsigned s = (unsigned)it * kPairs + j;
             there = wait(&full[s % kRing], (s / kRing) & 1);
           }
-          if (there && odd) scrub<T, kPairs, kRing>(sm_ring, (unsigned)it * kPairs, lane_tok);
+          if (there && odd && scrub<T, kPairs, kRing>(sm_ring, (unsigned)it * kPairs, lane_tok))
+            atomicMin(&scrubbed[ob], token);
         }
         fence_proxy_async_smem();
         tc_fence_before();
@@ -511,8 +519,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             lr += sums[ob][w][1][tid];
           }
         }
-        // any of the part's tokens
-        const bool sees = seen_by(p, x, x.tok0 + tid / p.heads) > x.step0 * kTokens;
+        const int seen = seen_by(p, x, x.tok0 + tid / p.heads);
+        const bool sees = seen > x.step0 * kTokens;  // any of the part's tokens
+        // one that held what is no number: 0 times it, if its score is -inf
+        if (x.steps > 0 && seen > scrubbed[ob]) lr = __int_as_float(0x7FC00000);
         inverse[tid] = !sees ? 0.0f : lr == 0.0f ? __int_as_float(0x7FC00000) : 1.0f / lr;
         if (tid < rows) {
           if (x.slot >= 0)

@@ -129,3 +129,22 @@ def test_scores_without_a_number(form, kind, sizes, which):
         got = turn.expanded(causal) if expanded else turn.attend(causal)
         same(got, formula(turn, causal, expanded))
     turn.plan.check()
+
+
+@pytest.mark.parametrize("form", ["absorbed", "expanded"])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("column", [5, -70])
+@pytest.mark.parametrize("sizes", TURNS)
+def test_values_without_a_number(form, bad, column, sizes):
+    """In tokens that some rows of a tile see and others do not, of request 0 alone: those that
+    do have no number even where the score is -inf, those that do not do not notice."""
+    if form == "expanded" and sizes.get("max_fresh"):
+        pytest.skip("the form does not go by the most rows")
+    turn = Turn(**sizes, nope=64 if sizes["latent"] < 512 else 128)
+    expanded = form == "expanded"
+    c, n = turn.cached[0], turn.fresh[0]
+    put(turn, 0, {c + n // 3, c + n // 2, c + n - 1}, column, bad)
+    for causal in (True, False):
+        got = turn.expanded(causal) if expanded else turn.attend(causal)
+        same(got, formula(turn, causal, expanded))
+    turn.plan.check()
