@@ -148,7 +148,7 @@ __global__ void __launch_bounds__(kScheduleThreads) schedule_kernel(const Schedu
   }
   const int start = v.tiling.start;
   int64_t level = share_level(rest, all, workers, workers, start);
-  for (int active = workers;;) {  // once more at the most where whole tiles cost much the same
+  for (int active = workers; sh.waves > 0;) {  // once where whole tiles cost much the same
     const bool mine = tid < workers && level - cost >= start;
     const int left = __syncthreads_count(mine);
     if (left == active) break;
