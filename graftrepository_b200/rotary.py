@@ -182,7 +182,7 @@ class Rotary(_Buffers):
                 out.get_device() != self._index or out.stride(2) != 1):
             raise ValueError(f"out must be {x.dtype} {list(x.shape)} on {self.device}, a head's "
                              f"values contiguous")
-        if any(n > 1 and s < x.shape[2] for n, s in zip(out.shape[:2], out.stride()[:2])):
+        if _rows_overlap(out):
             raise ValueError(f"rows of out overlap (strides {out.stride()})")
         if out.data_ptr() == x.data_ptr():
             if out.stride() != x.stride() or self.layout == "pair_swap":
@@ -201,6 +201,22 @@ def _first(t) -> int:
 def _last(t) -> int:
     return t.data_ptr() + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * \
         t.element_size()
+
+
+def _steps(t):
+    """(stride, entries) of the dimensions of rows [tokens, heads, head_dim] but the last,
+    the larger stride first; those of one entry say nothing."""
+    return sorted(((s, n) for s, n in zip(t.stride()[:2], t.shape[:2]) if n > 1), reverse=True)
+
+
+def _rows_overlap(t) -> bool:
+    """Whether one row may lie on another: each stride has to pass what lies within it."""
+    span = t.shape[2]
+    for s, n in reversed(_steps(t)):
+        if s < span:
+            return True
+        span += (n - 1) * s
+    return False
 
 
 def _apart(x, out) -> bool:

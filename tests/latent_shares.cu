@@ -69,7 +69,7 @@ int main() {
     };
     if (workers) {
       int64_t level = share_level(rest, sum_of(cost), workers, workers, tiling.start);
-      for (int active = workers;;) {
+      for (int active = workers; h.waves > 0;) {
         int left = 0;
         int64_t sum = 0;
         for (int64_t c : cost)
