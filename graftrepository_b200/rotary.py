@@ -188,9 +188,7 @@ class Rotary(_Buffers):
             if out.stride() != x.stride() or self.layout == "pair_swap":
                 raise ValueError("in place takes the same strides, and no pair swap")
             return
-        if x.numel() and _first(x) < _last(out) and _first(out) < _last(x) and \
-                x.untyped_storage().data_ptr() == out.untyped_storage().data_ptr() and \
-                not _apart(x, out):
+        if x.numel() and _first(x) < _last(out) and _first(out) < _last(x) and not _apart(x, out):
             raise ValueError("out overlaps x")
 
 
@@ -220,13 +218,18 @@ def _rows_overlap(t) -> bool:
 
 
 def _apart(x, out) -> bool:
-    """Whether two views of one buffer with the same strides lie side by side, as the
-    query and key parts of a projection's rows do."""
-    if x.stride() != out.stride():
+    """Whether two views of one buffer share no value, where both lie the same way and rows of
+    neither overlap, as the query and key parts of a projection's rows do.  (Views that lie
+    in different ways are not looked into.)"""
+    steps = _steps(x)
+    step, odd = divmod(out.data_ptr() - x.data_ptr(), x.element_size())
+    if steps != _steps(out) or odd or _rows_overlap(x):
         return False
-    (tokens, heads, dim), (row, head, _) = x.shape, x.stride()
-    step = abs(out.data_ptr() - x.data_ptr()) // x.element_size()
-    span = (heads - 1) * head + dim  # of a row's heads
-    if tokens > 1 and step + span > row:
-        return False
-    return step >= span or (heads > 1 and dim <= step % head <= head - dim)
+
+    def meet(step, i):  # whether a row of x and one of out do, so many values apart
+        if i == len(steps):
+            return abs(step) < x.shape[2]
+        s, n = steps[i]  # what lies within a stride is shorter, so one of two multiples
+        return any(abs(k) < n and meet(step - k * s, i + 1) for k in (step // s, step // s + 1))
+
+    return not meet(step, 0)

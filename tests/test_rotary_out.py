@@ -57,3 +57,47 @@ def test_two_strides_that_each_hold_a_head(shape, strides):
     for out in (x, view(shape, strides, 2048)):
         assert "rows of out overlap" in answer(x, out)
     assert answer(torch.zeros(shape), torch.zeros(shape)) is None
+
+
+def test_results_over_rows():
+    """Against the values that both name: what shares one is refused, and what shares none
+    taken, where both lie the same way."""
+    for shape, strides in itertools.product(SHAPES, itertools.product(STRIDES, STRIDES)):
+        x = view(shape, strides, 512)
+        if answer(torch.zeros(shape), x) is not None:
+            continue
+        names = set(x.reshape(-1).tolist())
+        for offset in range(1, 1024, 7):
+            out = view(shape, strides, offset)
+            got = answer(x, out)
+            if out.data_ptr() == x.data_ptr():
+                assert got is None
+            elif names.intersection(out.reshape(-1).tolist()):
+                assert got == "out overlaps x", (shape, strides, offset)
+            else:
+                assert got is None, (shape, strides, offset, got)
+
+
+def test_heads_before_tokens_side_by_side():
+    both = torch.zeros((6, 2, 10, 32))  # heads, kind, tokens, values
+    x, out = both[:, 0].transpose(0, 1), both[:, 1].transpose(0, 1)
+    assert answer(x, out) is None and answer(out, x) is None
+    assert answer(x, both[:, 0].transpose(0, 1)) is None  # in place
+
+
+def test_one_token_or_head_lies_any_way():
+    x = view((1, 4, 8), (96, 16))
+    assert answer(x, view((1, 4, 8), (640, 16), 8)) is None
+    assert answer(x, view((1, 4, 8), (640, 16), 4)) == "out overlaps x"
+
+
+def test_the_same_memory_by_another_tensor():
+    """A tensor that shares memory without sharing torch's storage."""
+    import ctypes
+
+    raw = (ctypes.c_float * 256)()
+    x = torch.frombuffer(raw, dtype=torch.float32).view(4, 2, 32)
+    other = torch.frombuffer(raw, dtype=torch.float32, count=192, offset=64).view(3, 2, 32)
+    assert x.untyped_storage().data_ptr() != other.untyped_storage().data_ptr()
+    assert answer(x[:3], other) == "out overlaps x"
+    assert answer(x[:1], other[1:2]) is None
