@@ -182,17 +182,24 @@ class LatentArena(_Buffers):
             raise ValueError(f"layer {layer} of {self.layers}")
         return self._refs[layer]
 
-    def _result(self, name, t, pattern, stream, *queries):
+    def _result(self, name, t, pattern, stream):
         if t is None:
             return _result(pattern, stream)
         if (t.shape != pattern.shape or t.dtype is not pattern.dtype or
                 t.get_device() != self._index or not t.is_contiguous()):
             raise ValueError(f"{name} must be contiguous {pattern.dtype} {list(pattern.shape)} on "
                              f"{self.device}")
-        # other blocks may still read the queries of rows whose result is there
-        if any(_first(t) < _last(q) and _first(q) < _last(t) for q in queries):
-            raise ValueError(f"{name} overlaps the queries")
         return t
+
+    def _apart(self, out, lse, **read):
+        """Refuses results over what the call reads (other blocks may still read the queries
+        of rows whose result is there), and over each other."""
+        for name, t in (("out", out), ("lse", lse)):
+            for what, x in read.items():
+                if _first(t) < _last(x) and _first(x) < _last(t):
+                    raise ValueError(f"{name} overlaps {what}")
+        if _first(out) < _last(lse) and _first(lse) < _last(out):
+            raise ValueError("out overlaps lse")
 
     def append(self, plan: LatentPlan, latent, rope, *, layer: int = 0, rotary=None,
                stream=None) -> None:
@@ -228,16 +235,20 @@ class LatentArena(_Buffers):
         `causal` over the positions up to the row's own.  `scale` (positive)
         multiplies the scores: for heads of nope + rope values usually (nope + rope)
         ** -0.5.  Returns (out [tokens, heads, latent], lse fp32 [tokens, heads]), new
-        ones or those given, which may not overlap the queries; rows that see nothing
-        are 0 with lse -inf.  A visible score of NaN or +inf makes its row NaN; one of
-        -inf weighs nothing, and a row that has no other is NaN with lse -inf."""
+        ones or those given, which may not overlap what the call reads (or lie among its
+        rows) nor each other; rows that see nothing are 0 with lse -inf.  A
+        visible score of NaN or +inf makes its row NaN; one of -inf weighs nothing, and a
+        row that has no other is NaN with lse -inf."""
         ref = self._ready(plan, layer)
         wide, narrow = plan.query_shapes
         c_ptr, c_row, c_head = self._rows("q_latent", q_latent, wide)
         r_ptr, r_row, r_head = self._rows("q_rope", q_rope, narrow)
         causal = self._causal(plan, causal)
-        out = self._result("out", out, plan._out_like, stream, q_latent, q_rope)
-        lse = self._result("lse", lse, plan._lse_like, stream, q_latent, q_rope)
+        given = out is not None or lse is not None
+        out = self._result("out", out, plan._out_like, stream)
+        lse = self._result("lse", lse, plan._lse_like, stream)
+        if given:
+            self._apart(out, lse, q_latent=q_latent, q_rope=q_rope, rows=self.rows)
         _call(self._attend, self._index, plan._step_ref, ref, c_ptr, c_row, c_head, r_ptr, r_row,
               r_head, float(scale), causal, out.data_ptr(), lse.data_ptr(),
               _handle(stream, self._index, (self, plan), q_latent, q_rope, out, lse))
@@ -260,8 +271,11 @@ class LatentArena(_Buffers):
         q_ptr, q_row, q_head = self._rows("q", q, plan.query_shape)
         w_ptr, w_head, w_row = self._rows("weights", weights, plan.weight_shape)
         causal = self._causal(plan, causal)
-        out = self._result("out", out, plan._expanded_like, stream, q)
-        lse = self._result("lse", lse, plan._lse_like, stream, q)
+        given = out is not None or lse is not None
+        out = self._result("out", out, plan._expanded_like, stream)
+        lse = self._result("lse", lse, plan._lse_like, stream)
+        if given:
+            self._apart(out, lse, q=q, weights=weights, rows=self.rows)
         _call(self._attend_expanded, self._index, plan._step_ref, ref, q_ptr, q_row, q_head,
               w_ptr, w_head, w_row, float(scale), causal, out.data_ptr(), lse.data_ptr(),
               _handle(stream, self._index, (self, plan), q, weights, out, lse))

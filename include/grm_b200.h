@@ -664,11 +664,12 @@ int grm_b200_latent_append(const grm_b200_latent_plan* plan, const grm_b200_late
  *   out[i, h] = sum_t w_t c_t,  w = softmax_t(softmax_scale * (q_latent . c_t + q_rope . r_t))
  * over the request's lens[r] tokens, or with causal != 0 over the positions up to
  * the row's own.  out [tokens, heads, latent] has the arena's type; lse [tokens,
- * heads] fp32 (may be NULL); neither may overlap the queries.  A row that sees nothing
- * is 0 with lse -inf, as are the rows past the step's last one.  Tokens that a row does
- * not see do not reach it, whatever they hold.  A visible score of NaN or +inf makes the
- * row and its lse NaN; one of -inf weighs nothing, and a row that has no other is NaN with
- * lse -inf.  Results do not depend on the order in which blocks run. */
+ * heads] fp32 (may be NULL); neither may overlap the queries, the rows of the cache or
+ * the other.  A row that sees nothing is 0 with lse -inf, as are the rows past the step's
+ * last one.  Tokens that a row does not see do not reach it, whatever they hold.  A visible
+ * score of NaN or +inf makes the row and its lse NaN; one of -inf weighs nothing, and a row
+ * that has no other is NaN with lse -inf.  Results do not depend on the order in which
+ * blocks run. */
 int grm_b200_latent_attend(const grm_b200_latent_plan* plan, const grm_b200_latent_arena* arena,
                            const void* q_latent_device, int64_t q_latent_row_stride,
                            int64_t q_latent_head_stride, const void* q_rope_device,
