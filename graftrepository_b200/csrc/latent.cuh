@@ -29,7 +29,9 @@ constexpr int kExpandAlign = 64;
 // (16 of them with 5 rows), 0.97 and 6.0 expanded (8,449 rows on 31,000 tokens, 40 heads of 64
 // + 32), 2.2 and 3.6 (3,499 rows, 16 heads of 128 + 64).
 // Both sides, us of those four: absorbed 448 46.2 and 33.6, 512 45.3 and 33.7, 640 45.4 and
-// 35.0; expanded 192 1,698 and 123.5, 256 1,697 and 117.0, 320 1,699 and 119.1.
+// 35.0; expanded 192 1,698 and 123.5, 256 1,697 and 117.0, 320 1,699 and 119.1.  Those four
+// are all that stands behind them: a fit for one case alone would be 570, 290, 395 or 105, and
+// latents of 128 and 512 and latent_few.cu's kernel go by the same without one.
 constexpr int kAbsorbedStart = 512, kExpandedStart = 256;
 // Fewest units of a worker: weighs the parts that join_kernel has to read against blocks
 // that stand idle (with 1,024 the 16 requests of 5 rows take 39.0 us, with 640 33.4).
@@ -91,9 +93,12 @@ struct Tiling {
 };
 // The absorbed form's kernel for few rows (latent_few.cu) takes requests of up to 32 rows
 // of a step over a latent of 512, where latent_attend.cu's needs two blocks for a tile and
-// both work out the scores (250,007 tokens of 16 heads: 170 us, 79 us with latent_few.cu's).  Its
-// buffers have no room for more rows; over smaller latents it is the slower one (70 us
-// against 102 us for 148 requests of 4,096 tokens, 40 heads of 256 + 32).
+// both work out the scores.  Both sides over 512 + 64, us: one request of 250,007 tokens, one
+// row of 16 heads, 158 and with latent_few.cu's 71, of 32 heads 157 and 85; 64 of 4,096 171
+// and 73, 173 and 87; 148 of 4,096, 16 heads, 344 and 124; 64 of 1,000 with 4 rows of 8 heads
+// 51 and 42; one of 333, 16 heads, 21 and 17.  Its buffers have no room for more rows; over
+// smaller latents it is the slower one (70 us against 102 us for 148 requests of 4,096
+// tokens, 40 heads of 256 + 32).
 __host__ __device__ inline Tiling absorbed_tiling(int heads, int latent, int64_t most_tokens,
                                                   int sms) {
   const int64_t most = most_tokens * heads;

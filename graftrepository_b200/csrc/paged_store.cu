@@ -217,7 +217,8 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendParams p) {
 // shared memory; rows of a larger page beyond those work theirs out where they are
 // used.  11,198 fp16 rows of 8 heads of 128, 64 values of each key's head rotated (69 MB
 // in and out, 10.5 us at a copy's rate), take 26.7 us and without the rotation 18.1; a group of
-// its own for each head took 44, four heads one after another 46.  61 bf16 rows of single
+// its own for each head took 44, four heads one after another 46.  At three blocks an SM, 80
+// registers, 80 to 88 bytes a thread are spilled, but for groups of 256.  61 bf16 rows of single
 // tokens take 4.2, with it or without: a launch and three dependent loads.
 
 struct TurnedParams {

@@ -13,7 +13,8 @@
 // not multiples of that.
 //
 // 8,449 bf16 rows of 32 heads of 128 (138 MB, 21.2 us at a copy's rate) take 25.0 us, 5.5
-// TB/s; 33 with a block's angles shared behind a barrier, 41 with a thread's own.  2,047 fp32
+// TB/s; 33 with a block's angles shared behind a barrier, 41 with a thread's own.  (At three
+// blocks an SM, 80 registers, the 16-bit kernels spill 12 to 48 bytes a thread.)  2,047 fp32
 // rows of 8 heads of 128, half of each rotated (17 MB, 2.6 us), take 6.3 and 61 bf16 rows of
 // 40 heads of 96 take 4.4: a launch, a token's angles and one trip to memory.
 #include <algorithm>

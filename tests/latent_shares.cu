@@ -54,7 +54,8 @@ int main() {
     const int64_t rest = base[n] - first;
     h.workers = rest == 0 ? 0
                 : h.waves ? tiling.workers
-                          : (int)std::min<int64_t>(tiling.workers, std::max<int64_t>(rest / kLeast, 1));
+                          : (int)std::min<int64_t>(tiling.workers,
+                                                   std::max<int64_t>(rest / kLeast, 1));
     const int workers = h.workers;
     std::vector<int64_t> cost(workers, 0), need(workers), raw(workers + 1);
     for (int r = 0; r < n && h.waves; ++r) {
